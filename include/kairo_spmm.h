@@ -400,6 +400,43 @@ KAIRO_API kairo_status kairo_sparse_scatter_grad(const void* grad_output, kairo_
 KAIRO_API kairo_status kairo_sparse_scatter_grad_workspace_size(int64_t nactive, int64_t nbatch, size_t* bytes);
 
 /* ------------------------------------------------------------------------
+ * Embedding lookup with scaling and the table's gradient by sorted tokens
+ * (no counterpart in the reference, whose embedding path is masked).
+ *   kairo_embedding_lookup  out[t, :] = scale * weight[ids[t], :], computed in
+ *                           fp32 and rounded once to out_dtype; an id outside
+ *                           [0, n_rows) gives a zero row.  weight is (n_rows,
+ *                           dim) with leading dimension ldw, out (nids, dim)
+ *                           contiguous; ids are int32 (id_bytes 4) or int64 (8).
+ *   kairo_token_sort        sorted[q] and perm[q], q < nids: the ids in
+ *                           ascending order, equal ids in token order, and the
+ *                           token of each.  Ids outside [0, n_rows) are written
+ *                           as n_rows, at the end.
+ *   kairo_embedding_grad    grad_weight (n_rows, dim; leading dimension ldo)
+ *                           row r = scale * the sum of grad_output's rows
+ *                           perm[q] with sorted[q] == r, zero where there is
+ *                           none.  With accumulate != 0 the sums are added to
+ *                           what grad_weight holds and other rows are not
+ *                           touched.  fp32 sums in an order fixed by the ids,
+ *                           no atomics; one rounding to out_dtype.
+ * dtype and out_dtype f32, f16 or bf16, in any combination; n_rows and nids
+ * below 2^31 - 4096.  All asynchronous on `stream`; the workspaces need no
+ * initial value.
+ * ---------------------------------------------------------------------- */
+KAIRO_API kairo_status kairo_embedding_lookup(const void* weight, int64_t n_rows, int64_t dim, int64_t ldw,
+                                              kairo_dtype dtype, const void* ids, int32_t id_bytes, int64_t nids,
+                                              float scale, void* out, kairo_dtype out_dtype, void* stream);
+KAIRO_API kairo_status kairo_token_sort(const void* ids, int32_t id_bytes, int64_t nids, int64_t n_rows,
+                                        int32_t* sorted, int32_t* perm, void* workspace, size_t workspace_bytes,
+                                        void* stream);
+KAIRO_API kairo_status kairo_token_sort_workspace_size(int64_t nids, int64_t n_rows, size_t* bytes);
+KAIRO_API kairo_status kairo_embedding_grad(const void* grad_output, int64_t ldg, kairo_dtype dtype,
+                                            const int32_t* sorted, const int32_t* perm, int64_t nids, int64_t n_rows,
+                                            int64_t dim, float scale, void* grad_weight, int64_t ldo,
+                                            kairo_dtype out_dtype, int32_t accumulate, void* workspace,
+                                            size_t workspace_bytes, void* stream);
+KAIRO_API kairo_status kairo_embedding_grad_workspace_size(int64_t nids, int64_t dim, size_t* bytes);
+
+/* ------------------------------------------------------------------------
  * Diagnostics (no counterpart in the reference): the rate at which the SMs
  * pull bulk copies of `load_bytes` (a multiple of 16 dividing 32768) from
  * pseudo-random offsets of `buffer` into shared memory, in GB/s summed over

@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
-from ctypes import POINTER, Structure, c_char_p, c_int32, c_int64, c_size_t, c_uint32, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_float, c_int32, c_int64, c_size_t, c_uint32, c_void_p
 
 import torch
 
@@ -204,6 +204,14 @@ _SIGNATURES = {
     "kairo_sparse_scatter_grad": (c_int32, [c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_int64, c_int64,
                                             c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
     "kairo_sparse_scatter_grad_workspace_size": (c_int32, [c_int64, c_int64, POINTER(c_size_t)]),
+    "kairo_embedding_lookup": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_int32, c_void_p, c_int32, c_int64,
+                                         c_float, c_void_p, c_int32, c_void_p]),
+    "kairo_token_sort": (c_int32, [c_void_p, c_int32, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_size_t,
+                                   c_void_p]),
+    "kairo_token_sort_workspace_size": (c_int32, [c_int64, c_int64, POINTER(c_size_t)]),
+    "kairo_embedding_grad": (c_int32, [c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_int64, c_int64, c_int64,
+                                       c_float, c_void_p, c_int64, c_int32, c_int32, c_void_p, c_size_t, c_void_p]),
+    "kairo_embedding_grad_workspace_size": (c_int32, [c_int64, c_int64, POINTER(c_size_t)]),
     "kairo_gather_probe": (c_int32, [c_void_p, c_size_t, c_uint32, c_int32, POINTER(ctypes.c_double), c_void_p]),
     "kairo_dense_to_tiles": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int32,
                                        c_int32, c_void_p, c_void_p]),

@@ -1,0 +1,76 @@
+// Conversions between the element types of the C ABI and fp32, and short
+// vectors of them: 16- or 8-byte loads and stores with every value held in
+// fp32 in between.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "../../include/kairo_spmm.h"
+
+namespace kairo {
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// One rounding (to nearest, ties to even) from fp32.
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// The words of N elements of T, aligned to their whole size.
+template <int BYTES>
+struct Words;
+template <>
+struct Words<2> { using type = uint16_t; };
+template <>
+struct Words<4> { using type = uint32_t; };
+template <>
+struct Words<8> { using type = uint2; };
+template <>
+struct Words<16> { using type = uint4; };
+
+template <typename T, int N>
+struct Pack {
+  union {
+    typename Words<N * static_cast<int>(sizeof(T))>::type raw;
+    T v[N];
+  };
+  __device__ __forceinline__ Pack() {}
+};
+
+template <typename T, int N>
+__device__ __forceinline__ void load_f32(const T* p, float (&f)[N]) {
+  Pack<T, N> k;
+  k.raw = *reinterpret_cast<const decltype(k.raw)*>(p);
+#pragma unroll
+  for (int i = 0; i < N; ++i) f[i] = to_f32<T>(k.v[i]);
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_f32(T* p, const float (&f)[N]) {
+  Pack<T, N> k;
+#pragma unroll
+  for (int i = 0; i < N; ++i) k.v[i] = from_f32<T>(f[i]);
+  *reinterpret_cast<decltype(k.raw)*>(p) = k.raw;
+}
+
+inline int element_bytes(kairo_dtype d) { return d == KAIRO_DTYPE_F32 ? 4 : 2; }
+inline bool known_dtype(kairo_dtype d) {
+  return d == KAIRO_DTYPE_F32 || d == KAIRO_DTYPE_F16 || d == KAIRO_DTYPE_BF16;
+}
+
+}  // namespace kairo

@@ -10,6 +10,13 @@ from __future__ import annotations
 
 from kairo_b200.ops._autotuner import TileAutotuner, TileConfig
 from kairo_b200.ops.embedding import MaskRows, sort_mask_rows, sparse_gather, sparse_scatter_grad
+from kairo_b200.ops.token_embedding import (
+    ScaledEmbedding,
+    TokenOrder,
+    embedding_grad,
+    embedding_lookup,
+    sort_tokens,
+)
 from kairo_b200.ops.backward import (
     BlockSparseLinear,
     TransposedBsr,
@@ -66,4 +73,9 @@ __all__ = [
     "sort_mask_rows",
     "sparse_gather",
     "sparse_scatter_grad",
+    "ScaledEmbedding",
+    "TokenOrder",
+    "embedding_grad",
+    "embedding_lookup",
+    "sort_tokens",
 ]

@@ -1,0 +1,208 @@
+"""Embedding lookup with scaling, and its gradient by sorted tokens (CUDA only).
+
+The dense-table counterpart of ``sparse_gather`` / ``sparse_scatter_grad``
+(the reference's embedding path, kairo/ops/sparse_embedding.py:59-161, is
+masked and wants a sorted unique id list):
+
+* ``embedding_lookup(weight, ids, scale=s)`` -- ``s * weight[ids]``, computed
+  in fp32 and rounded once.
+* ``sort_tokens(ids, N)`` -- the token positions in id order (stable), for
+  gradients of several tables or widths over one batch of ids.
+* ``embedding_grad(grad_output, ids, N, scale=s)`` -- the (N, D) gradient,
+  or the same added to an existing buffer (``out=..., accumulate=True``).
+* ``ScaledEmbedding`` -- both as an autograd-aware module.
+
+As in ``sparse_gather``, an id outside [0, N) gathers a zero row; it adds
+nothing to the gradient.  A negative id therefore serves as padding.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+
+import torch
+from torch import Tensor
+
+from kairo_b200 import _lib
+from kairo_b200.ops.spmm import _require_cuda
+
+
+def _same_device(*tensors: Tensor, op: str) -> torch.device:
+    dev = tensors[0].device
+    for t in tensors[1:]:
+        if t.device != dev:
+            raise ValueError(f"{op}: tensors are on {dev} and {t.device}; they must share a device")
+    return dev
+
+
+def _scratch(nbytes: int, device: torch.device) -> Tensor:
+    return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+
+
+def _flat_ids(ids: Tensor, op: str) -> Tensor:
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{op}: ids must be int32 or int64, got {ids.dtype}")
+    return ids.reshape(-1).contiguous()
+
+
+def _rows(t: Tensor) -> Tensor:
+    """``t`` (2-D) itself when its rows are contiguous and do not overlap."""
+    n, d = t.shape
+    return t if (d <= 1 or t.stride(1) == 1) and (n <= 1 or t.stride(0) >= d) else t.contiguous()
+
+
+def _ld(t: Tensor) -> int:
+    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+
+
+@dataclass(frozen=True)
+class TokenOrder:
+    """Token positions in id order (``sort_tokens``).
+
+    sorted_ids: (T,) int32, ids ascending, those outside [0, N) as N at the
+    end; perm: (T,) int32, the token of every sorted position, ascending
+    among equal ids; num_embeddings: N."""
+
+    sorted_ids: Tensor
+    perm: Tensor
+    num_embeddings: int
+
+
+def sort_tokens(ids: Tensor, num_embeddings: int) -> TokenOrder:
+    """Stable order of the tokens ``ids`` (any shape, int32 or int64) by id, on the device."""
+    _require_cuda(ids, op="sort_tokens")
+    n_rows = int(num_embeddings)
+    if n_rows < 0:
+        raise ValueError("num_embeddings must be non-negative")
+    flat = _flat_ids(ids, "sort_tokens")
+    dev = flat.device
+    n = flat.numel()
+    lib = _lib.lib()
+    out = torch.empty(n, dtype=torch.int32, device=dev)
+    perm = torch.empty(n, dtype=torch.int32, device=dev)
+    with torch.cuda.device(dev):
+        nbytes = ctypes.c_size_t(0)
+        _lib.check(lib.kairo_token_sort_workspace_size(n, n_rows, ctypes.byref(nbytes)), "sort_tokens")
+        if n:
+            ws = _scratch(nbytes.value, dev)
+            _lib.check(lib.kairo_token_sort(flat.data_ptr(), flat.element_size(), n, n_rows, out.data_ptr(),
+                                            perm.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev)),
+                       "sort_tokens")
+    return TokenOrder(sorted_ids=out, perm=perm, num_embeddings=n_rows)
+
+
+def embedding_lookup(weight: Tensor, ids: Tensor, *, scale: float = 1.0, out_dtype: torch.dtype | None = None,
+                     out: Tensor | None = None) -> Tensor:
+    """``scale * weight[ids]``: ids.shape + (D,), in ``out_dtype`` (default: weight's), rounded once from fp32.
+
+    weight: (N, D) float32, float16 or bfloat16; ids: int32 or int64, any
+    shape; an id outside [0, N) gives a zero row.  ``out``: a contiguous
+    tensor to write to."""
+    _require_cuda(weight, ids, op="embedding_lookup")
+    dev = _same_device(weight, ids, op="embedding_lookup")
+    if weight.dim() != 2 or weight.shape[1] < 1:
+        raise ValueError("weight must be 2-D (N, D) with D >= 1")
+    n, d = weight.shape
+    flat = _flat_ids(ids, "embedding_lookup")
+    in_dt = _lib.kairo_dtype(weight.dtype)
+    odt = out_dtype or (out.dtype if out is not None else weight.dtype)
+    out_dt = _lib.kairo_dtype(odt)
+    shape = tuple(ids.shape) + (d,)
+    if out is None:
+        out = torch.empty(shape, dtype=odt, device=dev)
+    elif tuple(out.shape) != shape or out.dtype != odt or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous {shape} {odt} tensor")
+    elif out.device != dev:
+        raise ValueError("out must be on the weight's device")
+    w = _rows(weight)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().kairo_embedding_lookup(w.data_ptr(), n, d, _ld(w), in_dt, flat.data_ptr(),
+                                                     flat.element_size(), flat.numel(), float(scale), out.data_ptr(),
+                                                     out_dt, _lib.stream_handle(dev)), "embedding_lookup")
+    return out
+
+
+def embedding_grad(grad_output: Tensor, ids: Tensor | TokenOrder, num_embeddings: int, *, scale: float = 1.0,
+                   out_dtype: torch.dtype | None = None, out: Tensor | None = None,
+                   accumulate: bool = False) -> Tensor:
+    """Gradient of ``embedding_lookup`` by its table: (N, D), row r = ``scale``
+    times the sum of ``grad_output[t]`` over the tokens t with id r.
+
+    grad_output: ids.shape + (D,); ids: the token ids or their
+    ``sort_tokens(ids, N)``.  Sums are fp32 in an order fixed by the ids
+    (deterministic, no atomics), rounded once to ``out_dtype`` (default:
+    grad_output's).  With ``accumulate=True`` the sums are added to ``out``,
+    whose other rows are neither read nor written; otherwise every row of
+    ``out`` (or of a new tensor) is written."""
+    n_rows = int(num_embeddings)
+    if isinstance(ids, TokenOrder):
+        if ids.num_embeddings != n_rows:
+            raise ValueError(f"the token order is of {ids.num_embeddings} rows, not {n_rows}")
+        tokens, where = ids.perm.numel(), ids.perm
+    else:
+        tokens, where = ids.numel(), ids
+    _require_cuda(grad_output, where, op="embedding_grad")
+    dev = _same_device(grad_output, where, op="embedding_grad")
+    if n_rows < 0:
+        raise ValueError("num_embeddings must be non-negative")
+    if grad_output.dim() < 1 or grad_output.shape[-1] < 1:
+        raise ValueError("grad_output must be (..., D) with D >= 1")
+    d = grad_output.shape[-1]
+    if not isinstance(ids, TokenOrder) and tuple(grad_output.shape[:-1]) != tuple(ids.shape):
+        raise ValueError(f"grad_output must be {tuple(ids.shape) + (d,)}, got {tuple(grad_output.shape)}")
+    g = _rows(grad_output.reshape(-1, d))
+    if g.shape[0] != tokens:
+        raise ValueError(f"grad_output has {g.shape[0]} rows for {tokens} tokens")
+    odt = out_dtype or (out.dtype if out is not None else g.dtype)
+    in_dt, out_dt = _lib.kairo_dtype(g.dtype), _lib.kairo_dtype(odt)
+    if accumulate and out is None:
+        raise ValueError("accumulate=True needs out")
+    if out is None:
+        out = torch.empty(n_rows, d, dtype=odt, device=dev)
+    elif tuple(out.shape) != (n_rows, d) or out.dtype != odt or out.device != dev or _rows(out) is not out:
+        raise ValueError(f"out must be a row-major ({n_rows}, {d}) {odt} tensor on {dev}")
+    order = ids if isinstance(ids, TokenOrder) else sort_tokens(ids, n_rows)
+    lib = _lib.lib()
+    with torch.cuda.device(dev):
+        nbytes = ctypes.c_size_t(0)
+        _lib.check(lib.kairo_embedding_grad_workspace_size(tokens, d, ctypes.byref(nbytes)), "embedding_grad")
+        ws = _scratch(nbytes.value, dev)
+        _lib.check(lib.kairo_embedding_grad(g.data_ptr(), _ld(g), in_dt, order.sorted_ids.data_ptr(),
+                                            order.perm.data_ptr(), tokens, n_rows, d, float(scale), out.data_ptr(),
+                                            _ld(out), out_dt, 1 if accumulate else 0, ws.data_ptr(), ws.numel(),
+                                            _lib.stream_handle(dev)), "embedding_grad")
+    return out
+
+
+class _LookupFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight: Tensor, ids: Tensor, scale: float, out_dtype: torch.dtype | None) -> Tensor:
+        ctx.save_for_backward(ids)
+        ctx.rows, ctx.dtype, ctx.scale = weight.shape[0], weight.dtype, scale
+        return embedding_lookup(weight, ids, scale=scale, out_dtype=out_dtype)
+
+    @staticmethod
+    def backward(ctx, grad: Tensor):
+        (ids,) = ctx.saved_tensors
+        return embedding_grad(grad, ids, ctx.rows, scale=ctx.scale, out_dtype=ctx.dtype), None, None, None
+
+
+class ScaledEmbedding(torch.nn.Module):
+    """``scale * weight[ids]`` with the table's gradient from ``embedding_grad``.
+
+    weight: (num_embeddings, embedding_dim), N(0, 1) initialised;
+    ``out_dtype`` lets an fp32 table feed a 16-bit model."""
+
+    def __init__(self, num_embeddings: int, embedding_dim: int, *, scale: float = 1.0,
+                 dtype: torch.dtype = torch.float32, out_dtype: torch.dtype | None = None,
+                 device: torch.device | str | None = None) -> None:
+        super().__init__()
+        if num_embeddings <= 0 or embedding_dim <= 0:
+            raise ValueError("num_embeddings and embedding_dim must be positive")
+        self.weight = torch.nn.Parameter(torch.randn(num_embeddings, embedding_dim, dtype=dtype, device=device))
+        self.scale = float(scale)
+        self.out_dtype = out_dtype
+
+    def forward(self, ids: Tensor) -> Tensor:
+        return _LookupFn.apply(self.weight, ids, self.scale, self.out_dtype)
