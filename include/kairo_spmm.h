@@ -330,6 +330,34 @@ KAIRO_API kairo_status kairo_bsr_sddmm(const kairo_bsr* a, const int32_t* row_pt
 KAIRO_API kairo_status kairo_bsr_sddmm_workspace_size(const kairo_bsr* a, size_t* bytes);
 
 /* ------------------------------------------------------------------------
+ * Activations kept in 8 bits for the backward pass (no counterpart in the
+ * reference).  Every 64 columns of a row share a step a * (1 / 127), a the
+ * largest magnitude of the group: codes (n x k int8, leading dimension ldq, a
+ * multiple of 16, 16-byte aligned) hold round_half_even(x * inv) with inv =
+ * 127 * (1 / a), steps (ceil(k / 64) x n fp32, leading dimension lds) the
+ * steps; inv and step are computed in fp32, every operation rounded.  The
+ * value read back is code * step, rounded to the activation's type.  Groups with a < 2^-100 read back as zeros, groups
+ * with an infinity or NaN as NaN.  A row's codes are written up to the next
+ * multiple of 8 columns.
+ *   kairo_quantize_q8     x (n x k, leading dimension ldx) -> codes, steps
+ *   kairo_dequantize_q8   codes, steps -> x in `dtype`
+ *   kairo_bsr_sddmm_q8    kairo_bsr_sddmm with X (a's dtype) given by its
+ *                         codes and steps
+ * All asynchronous on `stream`.
+ * ---------------------------------------------------------------------- */
+KAIRO_API kairo_status kairo_quantize_q8(const void* x, int64_t n, int64_t k, int64_t ldx, kairo_dtype dtype,
+                                         int8_t* codes, int64_t ldq, float* steps, int64_t lds, void* stream);
+KAIRO_API kairo_status kairo_dequantize_q8(const int8_t* codes, int64_t ldq, const float* steps, int64_t lds,
+                                           int64_t n, int64_t k, void* x, int64_t ldx, kairo_dtype dtype,
+                                           void* stream);
+KAIRO_API kairo_status kairo_bsr_sddmm_q8(const kairo_bsr* a, const int32_t* row_ptr_t, const int32_t* col_idx_t,
+                                          const int32_t* perm_t, const void* dy, int64_t lddy, const int8_t* codes,
+                                          int64_t ldq, const float* steps, int64_t lds, int64_t n, void* dblocks,
+                                          kairo_dtype out_dtype, void* workspace, size_t workspace_bytes,
+                                          void* stream);
+KAIRO_API kairo_status kairo_bsr_sddmm_q8_workspace_size(const kairo_bsr* a, int64_t n, size_t* bytes);
+
+/* ------------------------------------------------------------------------
  * Block-granular pruning (no counterpart in the reference, which prunes
  * element by element: kairo/training/sparse_rec/topology.py:50-118).
  *   kairo_block_norms      L2 norm of every bm x bk block of a dense matrix

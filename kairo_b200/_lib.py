@@ -188,6 +188,14 @@ _SIGNATURES = {
     "kairo_bsr_sddmm": (c_int32, [POINTER(KairoBsr), c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
                                   c_int64, c_int64, c_void_p, c_int32, c_void_p, c_size_t, c_void_p]),
     "kairo_bsr_sddmm_workspace_size": (c_int32, [POINTER(KairoBsr), POINTER(c_size_t)]),
+    "kairo_quantize_q8": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_int32, c_void_p, c_int64, c_void_p,
+                                    c_int64, c_void_p]),
+    "kairo_dequantize_q8": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64,
+                                      c_int32, c_void_p]),
+    "kairo_bsr_sddmm_q8": (c_int32, [POINTER(KairoBsr), c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
+                                     c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int32, c_void_p, c_size_t,
+                                     c_void_p]),
+    "kairo_bsr_sddmm_q8_workspace_size": (c_int32, [POINTER(KairoBsr), c_int64, POINTER(c_size_t)]),
     "kairo_block_norms": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_int32, c_int32, c_int32, c_void_p,
                                     c_void_p]),
     "kairo_bsr_block_norms": (c_int32, [POINTER(KairoBsr), c_void_p, c_void_p]),

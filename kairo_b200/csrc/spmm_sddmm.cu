@@ -471,6 +471,25 @@ bool sdd_tc_ok(const kairo_bsr* a, const void* dy, int64_t lddy, const void* x, 
 }
 
 }  // namespace
+
+kairo_status sddmm_check(const kairo_bsr* a, const int32_t* row_ptr_t, const int32_t* col_idx_t,
+                         const int32_t* perm_t, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t n,
+                         const void* dblocks, kairo_dtype out_dtype, const void* workspace) {
+  if (!a) return fail(KAIRO_STATUS_INVALID_VALUE, "null BSR descriptor");
+  if (a->rows < 0 || a->cols < 0 || a->nnzb < 0 || a->bm <= 0 || a->bk <= 0 || n < 0)
+    return fail(KAIRO_STATUS_INVALID_VALUE, "invalid size");
+  if (a->nnzb > 0x7fffffffLL) return fail(KAIRO_STATUS_NOT_SUPPORTED, "more than 2^31-1 blocks");
+  if (a->dtype != KAIRO_DTYPE_F32 && a->dtype != KAIRO_DTYPE_F16 && a->dtype != KAIRO_DTYPE_BF16)
+    return fail(KAIRO_STATUS_INVALID_VALUE, "unknown dtype");
+  if (out_dtype != KAIRO_DTYPE_F32 && out_dtype != a->dtype)
+    return fail(KAIRO_STATUS_INVALID_VALUE, "dW dtype must be fp32 or the input dtype");
+  if (lddy < a->rows || ldx < a->cols) return fail(KAIRO_STATUS_INVALID_VALUE, "leading dimension too small");
+  if (a->nnzb == 0) return KAIRO_STATUS_SUCCESS;
+  if (!row_ptr_t || !col_idx_t || !perm_t || !a->col_idx || !dblocks || !workspace || (n > 0 && (!dy || !x)))
+    return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+  return KAIRO_STATUS_SUCCESS;
+}
+
 }  // namespace kairo
 
 using namespace kairo;
@@ -486,20 +505,11 @@ extern "C" kairo_status kairo_bsr_sddmm(const kairo_bsr* a, const int32_t* row_p
                                         const int32_t* perm_t, const void* dy, int64_t lddy, const void* x,
                                         int64_t ldx, int64_t n, void* dblocks, kairo_dtype out_dtype,
                                         void* workspace, size_t workspace_bytes, void* stream) {
-  if (!a) return fail(KAIRO_STATUS_INVALID_VALUE, "null BSR descriptor");
-  if (a->rows < 0 || a->cols < 0 || a->nnzb < 0 || a->bm <= 0 || a->bk <= 0 || n < 0)
-    return fail(KAIRO_STATUS_INVALID_VALUE, "invalid size");
-  if (a->nnzb > 0x7fffffffLL) return fail(KAIRO_STATUS_NOT_SUPPORTED, "more than 2^31-1 blocks");
-  if (a->dtype != KAIRO_DTYPE_F32 && a->dtype != KAIRO_DTYPE_F16 && a->dtype != KAIRO_DTYPE_BF16)
-    return fail(KAIRO_STATUS_INVALID_VALUE, "unknown dtype");
-  if (out_dtype != KAIRO_DTYPE_F32 && out_dtype != a->dtype)
-    return fail(KAIRO_STATUS_INVALID_VALUE, "dW dtype must be fp32 or the input dtype");
-  if (lddy < a->rows || ldx < a->cols) return fail(KAIRO_STATUS_INVALID_VALUE, "leading dimension too small");
+  kairo_status st = sddmm_check(a, row_ptr_t, col_idx_t, perm_t, dy, lddy, x, ldx, n, dblocks, out_dtype, workspace);
+  if (st) return st;
   if (a->nnzb == 0) return KAIRO_STATUS_SUCCESS;
-  if (!row_ptr_t || !col_idx_t || !perm_t || !a->col_idx || !dblocks || !workspace || (n > 0 && (!dy || !x)))
-    return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
   size_t need = 0;
-  kairo_status st = kairo_bsr_sddmm_workspace_size(a, &need);
+  st = kairo_bsr_sddmm_workspace_size(a, &need);
   if (st) return st;
   if (workspace_bytes < need) return fail(KAIRO_STATUS_WORKSPACE_TOO_SMALL, "SDDMM workspace too small");
   cudaStream_t s = static_cast<cudaStream_t>(stream);

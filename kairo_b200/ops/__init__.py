@@ -25,6 +25,7 @@ from kairo_b200.ops.backward import (
     sparse_linear_weight_grad,
     transpose_values,
 )
+from kairo_b200.ops.checkpoint import QuantizedActivations, dequantize_activations, quantize_activations
 from kairo_b200.ops.spmm import (
     KernelConfig,
     RowGroups,
@@ -73,6 +74,9 @@ __all__ = [
     "sort_mask_rows",
     "sparse_gather",
     "sparse_scatter_grad",
+    "QuantizedActivations",
+    "dequantize_activations",
+    "quantize_activations",
     "ScaledEmbedding",
     "TokenOrder",
     "embedding_grad",

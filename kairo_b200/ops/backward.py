@@ -11,7 +11,8 @@ sparse-training caller of ``sparse_linear`` needs, with W's sparsity fixed:
   tcgen05 kernel for 64 x 64 f16/bf16 blocks, CUDA cores otherwise).
 
 ``BlockSparseLinear`` wraps both in an autograd-aware module whose parameter
-is the (nnzb, bm, bk) block tensor.
+is the (nnzb, bm, bk) block tensor.  X may be kept in 8 bits in between
+(``checkpoint="int8"``; kairo_b200/ops/checkpoint.py).
 """
 
 from __future__ import annotations
@@ -23,6 +24,7 @@ import torch
 from torch import Tensor
 
 from kairo_b200 import _lib
+from kairo_b200.ops.checkpoint import QuantizedActivations, quantize_activations
 from kairo_b200.ops.spmm import KernelConfig, _bsr_desc, _require_cuda, sparse_linear
 from kairo_b200.types import BlockSparseMatrix
 
@@ -96,13 +98,18 @@ def transpose_values(a: BlockSparseMatrix, t: TransposedBsr) -> TransposedBsr:
     return t
 
 
-def sparse_linear_weight_grad(dY: Tensor, X: Tensor, W: BlockSparseMatrix, wt: TransposedBsr | None = None, *,
-                              out_dtype: torch.dtype = torch.float32, check: bool = False) -> Tensor:
+def sparse_linear_weight_grad(dY: Tensor, X: Tensor | QuantizedActivations, W: BlockSparseMatrix,
+                              wt: TransposedBsr | None = None, *, out_dtype: torch.dtype = torch.float32,
+                              check: bool = False) -> Tensor:
     """dW on W's nonzero blocks for Y = X @ W^T: (nnzb, bm, bk) in W's BSR
-    order, ``dW[p] = dY[:, i*bm:(i+1)*bm]^T @ X[:, j*bk:(j+1)*bk]``."""
-    _require_cuda(dY, X, W.blocks, op="sparse_linear_weight_grad")
+    order, ``dW[p] = dY[:, i*bm:(i+1)*bm]^T @ X[:, j*bk:(j+1)*bk]``.
+
+    X may be given in 8 bits (``quantize_activations``): the result is that
+    of the activation it reads back as."""
+    kept = X if isinstance(X, QuantizedActivations) else None
+    _require_cuda(dY, X.codes if kept else X, W.blocks, op="sparse_linear_weight_grad")
     m, k = W.shape
-    if dY.dim() != 2 or X.dim() != 2 or dY.shape[0] != X.shape[0] or dY.shape[1] != m or X.shape[1] != k:
+    if dY.dim() != 2 or len(X.shape) != 2 or dY.shape[0] != X.shape[0] or dY.shape[1] != m or X.shape[1] != k:
         raise ValueError(f"dY must be (batch, {m}) and X (batch, {k}); got {tuple(dY.shape)} and {tuple(X.shape)}")
     if dY.dtype != W.dtype or X.dtype != W.dtype:
         raise TypeError("dY, X and W must share a dtype")
@@ -110,12 +117,14 @@ def sparse_linear_weight_grad(dY: Tensor, X: Tensor, W: BlockSparseMatrix, wt: T
         raise TypeError("dW dtype must be float32 or the weight dtype")
     if dY.stride(1) != 1:
         dY = dY.contiguous()
-    if X.stride(1) != 1:
+    if kept is None and X.stride(1) != 1:
         X = X.contiguous()
     if wt is None:
         wt = bsr_transpose(W)
     bm, bk = W.block_size
     dev = W.device
+    if kept and not (dY.device == X.device == dev):
+        raise ValueError("dY, X and W must share a device")
     dw = torch.empty(W.nnzb, bm, bk, dtype=out_dtype, device=dev)
     if W.nnzb == 0:
         return dw
@@ -123,22 +132,36 @@ def sparse_linear_weight_grad(dY: Tensor, X: Tensor, W: BlockSparseMatrix, wt: T
     desc = _bsr_desc(W)
     with torch.cuda.device(dev):
         nbytes = ctypes.c_size_t(0)
-        _lib.check(lib.kairo_bsr_sddmm_workspace_size(ctypes.byref(desc), ctypes.byref(nbytes)), "sddmm")
+        if kept:
+            _lib.check(lib.kairo_bsr_sddmm_q8_workspace_size(ctypes.byref(desc), X.shape[0], ctypes.byref(nbytes)),
+                       "sddmm")
+        else:
+            _lib.check(lib.kairo_bsr_sddmm_workspace_size(ctypes.byref(desc), ctypes.byref(nbytes)), "sddmm")
         ws = _scratch(nbytes.value, dev)
-        _lib.check(lib.kairo_bsr_sddmm(ctypes.byref(desc), wt.matrix.row_ptr.data_ptr(), wt.matrix.col_idx.data_ptr(),
-                                       wt.perm.data_ptr(), dY.data_ptr(), dY.stride(0), X.data_ptr(), X.stride(0),
-                                       X.shape[0], dw.data_ptr(), _lib.kairo_dtype(out_dtype), ws.data_ptr(),
-                                       ws.numel(), _lib.stream_handle(dev)), "sparse_linear_weight_grad")
+        if kept:
+            _lib.check(lib.kairo_bsr_sddmm_q8(ctypes.byref(desc), wt.matrix.row_ptr.data_ptr(),
+                                              wt.matrix.col_idx.data_ptr(), wt.perm.data_ptr(), dY.data_ptr(),
+                                              max(dY.stride(0), m), X.codes.data_ptr(), X._ldq, X.steps.data_ptr(),
+                                              X._lds, X.shape[0], dw.data_ptr(), _lib.kairo_dtype(out_dtype),
+                                              ws.data_ptr(), ws.numel(), _lib.stream_handle(dev)),
+                       "sparse_linear_weight_grad")
+        else:
+            _lib.check(lib.kairo_bsr_sddmm(ctypes.byref(desc), wt.matrix.row_ptr.data_ptr(),
+                                           wt.matrix.col_idx.data_ptr(), wt.perm.data_ptr(), dY.data_ptr(),
+                                           dY.stride(0), X.data_ptr(), X.stride(0), X.shape[0], dw.data_ptr(),
+                                           _lib.kairo_dtype(out_dtype), ws.data_ptr(), ws.numel(),
+                                           _lib.stream_handle(dev)), "sparse_linear_weight_grad")
         if check:
             _lib.raise_on_device_error(ws)
     return dw
 
 
-def sparse_linear_backward(dY: Tensor, X: Tensor, W: BlockSparseMatrix, wt: TransposedBsr | None = None, *,
+def sparse_linear_backward(dY: Tensor, X: Tensor | QuantizedActivations, W: BlockSparseMatrix, wt: TransposedBsr | None = None, *,
                            need_dx: bool = True, need_dw: bool = True, dw_dtype: torch.dtype = torch.float32,
                            config: KernelConfig | None = None, check: bool = False):
     """(dX, dW) of Y = X @ W^T.  dX: (batch, in_features) in X's dtype; dW:
-    (nnzb, bm, bk) in ``dw_dtype``, W's BSR order.  Either may be None."""
+    (nnzb, bm, bk) in ``dw_dtype``, W's BSR order.  Either may be None.  X may
+    be given in 8 bits (``quantize_activations``)."""
     if wt is None:
         wt = bsr_transpose(W)
     dX = sparse_linear(dY, wt.matrix, out_dtype=X.dtype, config=config, check=check) if need_dx else None
@@ -150,13 +173,23 @@ class _SparseLinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, X: Tensor, blocks: Tensor, module: "BlockSparseLinear") -> Tensor:
         W = module.weight_matrix(blocks)
-        ctx.save_for_backward(X, blocks)
+        ctx.kept_dtype = None
+        if module.checkpoint is not None and ctx.needs_input_grad[1]:
+            q = quantize_activations(X)
+            ctx.save_for_backward(q.codes, q.steps, blocks)
+            ctx.kept_dtype = q.dtype
+        else:
+            ctx.save_for_backward(X, blocks)
         ctx.module = module
         return sparse_linear(X, W)
 
     @staticmethod
     def backward(ctx, dY: Tensor):
-        X, blocks = ctx.saved_tensors
+        if ctx.kept_dtype is not None:
+            codes, steps, blocks = ctx.saved_tensors
+            X = QuantizedActivations(codes=codes, steps=steps, dtype=ctx.kept_dtype)
+        else:
+            X, blocks = ctx.saved_tensors
         module: BlockSparseLinear = ctx.module
         W = module.weight_matrix(blocks)
         wt = transpose_values(W, module.transposed())
@@ -172,10 +205,18 @@ class BlockSparseLinear(torch.nn.Module):
     The trainable parameter is ``blocks`` (nnzb, bm, bk) in BSR order;
     ``row_ptr`` / ``col_idx`` are buffers.  Forward and both gradients run on
     this package's kernels (``sparse_linear``, ``bsr_transpose``,
-    ``kairo_bsr_sddmm``)."""
+    ``kairo_bsr_sddmm``).
 
-    def __init__(self, W: BlockSparseMatrix) -> None:
+    ``checkpoint="int8"`` keeps the input for dW in 8 bits
+    (``quantize_activations``): about half the activation memory between
+    forward and backward; dX is not affected, and dW is that of the activation
+    as it reads back."""
+
+    def __init__(self, W: BlockSparseMatrix, *, checkpoint: str | None = None) -> None:
         super().__init__()
+        if checkpoint not in (None, "int8"):
+            raise ValueError(f"checkpoint must be None or 'int8', got {checkpoint!r}")
+        self.checkpoint = checkpoint
         blocks = W.blocks if W.blk_idx is None else W.blocks[W.blk_idx.long()]
         self.blocks = torch.nn.Parameter(blocks.detach().clone())
         self.register_buffer("row_ptr", W.row_ptr.detach().clone())

@@ -1,0 +1,127 @@
+"""Activations kept in 8 bits for the backward pass (CUDA only).
+
+A layer that trains keeps its input for the weight gradient; in 8 bits it
+takes 1.06 bytes a value instead of 2.  Every 64 columns of a row share a step
+(the group's largest magnitude / 127), so that one loud column does not cost
+the others their resolution:
+
+* ``quantize_activations(X)`` -- the 8-bit codes and fp32 steps of X;
+* ``dequantize_activations(q)`` -- what they stand for, in X's own type;
+* ``sparse_linear_weight_grad(dY, q, W)`` and
+  ``adapter_linear_backward(dY, q, ...)`` take them in X's place, and
+  ``BlockSparseLinear(W, checkpoint="int8")`` keeps its input that way.
+
+The reference has no counterpart.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+from torch import Tensor
+
+from kairo_b200 import _lib
+from kairo_b200.ops.spmm import _require_cuda
+
+GROUP = 64  # columns that share a step
+
+
+@dataclass(frozen=True)
+class QuantizedActivations:
+    """An (n, k) activation in 8 bits.
+
+    codes: (n, k) int8, rows padded to 16 bytes; steps: (ceil(k / 64), n)
+    float32, the step of columns 64 g .. 64 g + 63 of row r at [g, r]; dtype:
+    the activation's type, in which ``code * step`` is read back."""
+
+    codes: Tensor
+    steps: Tensor
+    dtype: torch.dtype
+
+    def __post_init__(self) -> None:
+        if self.codes.dim() != 2 or self.codes.dtype != torch.int8:
+            raise ValueError("codes must be a 2-D int8 tensor")
+        n, k = self.codes.shape
+        if tuple(self.steps.shape) != ((k + GROUP - 1) // GROUP, n) or self.steps.dtype != torch.float32:
+            raise ValueError(f"steps must be a ({(k + GROUP - 1) // GROUP}, {n}) float32 tensor")
+        if self.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            raise TypeError(f"unsupported dtype {self.dtype}; expected float32, float16 or bfloat16")
+        if self.steps.device != self.codes.device:
+            raise ValueError("codes and steps must share a device")
+        if n * k > 0:
+            if self.codes.stride(1) != 1 or self.codes.data_ptr() % 16 or (n > 1 and (self.codes.stride(0) % 16 or
+                                                                                    self.codes.stride(0) < k)):
+                raise ValueError("codes must have 16-byte aligned rows")
+            if (n > 1 and self.steps.stride(1) != 1) or (self.steps.shape[0] > 1 and self.steps.stride(0) < n):
+                raise ValueError("steps must be row-major")
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return tuple(self.codes.shape)
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @property
+    def is_cuda(self) -> bool:
+        return self.codes.is_cuda
+
+    @property
+    def nbytes(self) -> int:
+        """Bytes kept: codes with their row padding, and steps."""
+        return self.shape[0] * self._ldq + 4 * self.steps.numel()
+
+    @property
+    def _ldq(self) -> int:
+        n, k = self.codes.shape
+        return self.codes.stride(0) if n > 1 else -(-k // 16) * 16
+
+    @property
+    def _lds(self) -> int:
+        return self.steps.stride(0) if self.steps.shape[0] > 1 else self.steps.shape[1]
+
+
+def quantize_activations(X: Tensor) -> QuantizedActivations:
+    """X (n, k) float32, float16 or bfloat16 -> 8-bit codes and steps.
+
+    A value is off by at most half a step, max|group| / 254.  A group whose
+    largest magnitude is under 2^-100 reads back as zeros; one that holds an
+    infinity or a NaN reads back as NaN."""
+    _require_cuda(X, op="quantize_activations")
+    if X.dim() != 2:
+        raise ValueError("X must be 2-D (n, k)")
+    dt = _lib.kairo_dtype(X.dtype)
+    if X.stride(1) != 1 or (X.shape[0] > 1 and X.stride(0) < X.shape[1]):
+        X = X.contiguous()
+    n, k = X.shape
+    dev = X.device
+    ldq = -(-k // 16) * 16
+    codes = torch.empty(n, ldq, dtype=torch.int8, device=dev)[:, :k]
+    steps = torch.empty(-(-k // GROUP), n, dtype=torch.float32, device=dev)
+    if n and k:
+        with torch.cuda.device(dev):
+            _lib.check(_lib.lib().kairo_quantize_q8(X.data_ptr(), n, k, max(X.stride(0), k), dt, codes.data_ptr(),
+                                                    ldq, steps.data_ptr(), n, _lib.stream_handle(dev)),
+                       "quantize_activations")
+    return QuantizedActivations(codes=codes, steps=steps, dtype=X.dtype)
+
+
+def dequantize_activations(q: QuantizedActivations, *, out: Tensor | None = None) -> Tensor:
+    """``code * step`` in the activation's type, (n, k)."""
+    _require_cuda(q.codes, op="dequantize_activations")
+    n, k = q.shape
+    dev = q.device
+    if out is None:
+        out = torch.empty(n, k, dtype=q.dtype, device=dev)
+    elif tuple(out.shape) != (n, k) or out.dtype != q.dtype or out.device != dev or (k > 1 and out.stride(1) != 1) or (
+            n > 1 and out.stride(0) < k):
+        raise ValueError(f"out must be a row-major ({n}, {k}) {q.dtype} tensor on {dev}")
+    if n and k:
+        with torch.cuda.device(dev):
+            _lib.check(_lib.lib().kairo_dequantize_q8(q.codes.data_ptr(), q._ldq, q.steps.data_ptr(), q._lds, n, k,
+                                                      out.data_ptr(), max(out.stride(0), k),
+                                                      _lib.kairo_dtype(q.dtype), _lib.stream_handle(dev)),
+                       "dequantize_activations")
+    return out
