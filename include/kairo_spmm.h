@@ -358,6 +358,44 @@ KAIRO_API kairo_status kairo_bsr_sddmm_q8(const kairo_bsr* a, const int32_t* row
 KAIRO_API kairo_status kairo_bsr_sddmm_q8_workspace_size(const kairo_bsr* a, int64_t n, size_t* bytes);
 
 /* ------------------------------------------------------------------------
+ * Low-rank adapters of many requests in one batch, beside a shared projection
+ * (no counterpart in the reference).
+ *   kairo_adapter_plan_build  orders the tokens of a batch by adapter.  ids
+ *                         (ntokens, int32 or int64) name each token's adapter;
+ *                         an id outside [0, nadapters) means none.  The plan
+ *                         lives in caller memory of kairo_adapter_plan_size
+ *                         bytes, is opaque, and serves every layer.
+ *   kairo_low_rank_apply  low[t] = scale[a] * x[t] down_a^T (ntokens x rank,
+ *                         fp32, written), y[t] = base[t] + low[t] up_a, a the
+ *                         adapter of token t; low = 0 and y = base for a
+ *                         token without one.  down is (nadapters, rank, k),
+ *                         up (nadapters, rank, n), both contiguous; scale may
+ *                         be NULL (1), base may be NULL (0) or y itself; with
+ *                         y NULL low alone is computed.  The
+ *                         sum is formed in fp32 and rounded once to y_dtype.
+ *                         The backward pass is this call on dY with up and
+ *                         down swapped.
+ *   kairo_low_rank_wgrad  grad (nadapters, rank, k) = for every adapter the
+ *                         sum over its tokens of low[t]^T z[t], zeros for one
+ *                         without tokens; no atomics.
+ * x, z, down, up f16 or bf16 (one dtype); base, y and grad that dtype or fp32.
+ * rank at most 128, at most 65535 adapters, 2^24 tokens, 2^22 features.  All
+ * asynchronous on `stream`.
+ * ---------------------------------------------------------------------- */
+KAIRO_API kairo_status kairo_adapter_plan_build(const void* ids, int32_t id_bytes, int64_t ntokens,
+                                                int64_t nadapters, void* plan, size_t plan_size, void* workspace,
+                                                size_t workspace_bytes, void* stream);
+KAIRO_API kairo_status kairo_adapter_plan_size(int64_t ntokens, int64_t nadapters, size_t* plan, size_t* workspace);
+KAIRO_API kairo_status kairo_low_rank_apply(const void* x, int64_t ldx, int64_t k, const void* down, const void* up,
+                                            int64_t n, int64_t rank, kairo_dtype dtype, const float* scale,
+                                            const void* plan, int64_t ntokens, int64_t nadapters, const void* base,
+                                            int64_t ldb, kairo_dtype base_dtype, void* y, int64_t ldy,
+                                            kairo_dtype y_dtype, float* low, void* stream);
+KAIRO_API kairo_status kairo_low_rank_wgrad(const float* low, int64_t rank, const void* z, int64_t ldz, int64_t k,
+                                            kairo_dtype dtype, const void* plan, int64_t ntokens, int64_t nadapters,
+                                            void* grad, kairo_dtype grad_dtype, void* stream);
+
+/* ------------------------------------------------------------------------
  * Block-granular pruning (no counterpart in the reference, which prunes
  * element by element: kairo/training/sparse_rec/topology.py:50-118).
  *   kairo_block_norms      L2 norm of every bm x bk block of a dense matrix

@@ -196,6 +196,14 @@ _SIGNATURES = {
                                      c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int32, c_void_p, c_size_t,
                                      c_void_p]),
     "kairo_bsr_sddmm_q8_workspace_size": (c_int32, [POINTER(KairoBsr), c_int64, POINTER(c_size_t)]),
+    "kairo_adapter_plan_build": (c_int32, [c_void_p, c_int32, c_int64, c_int64, c_void_p, c_size_t, c_void_p, c_size_t,
+                                           c_void_p]),
+    "kairo_adapter_plan_size": (c_int32, [c_int64, c_int64, POINTER(c_size_t), POINTER(c_size_t)]),
+    "kairo_low_rank_apply": (c_int32, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int32,
+                                       c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int32, c_void_p,
+                                       c_int64, c_int32, c_void_p, c_void_p]),
+    "kairo_low_rank_wgrad": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int32, c_void_p, c_int64,
+                                       c_int64, c_void_p, c_int32, c_void_p]),
     "kairo_block_norms": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_int32, c_int32, c_int32, c_void_p,
                                     c_void_p]),
     "kairo_bsr_block_norms": (c_int32, [POINTER(KairoBsr), c_void_p, c_void_p]),

@@ -25,6 +25,15 @@ from kairo_b200.ops.backward import (
     sparse_linear_weight_grad,
     transpose_values,
 )
+from kairo_b200.ops.adapters import (
+    AdaptedSparseLinear,
+    AdapterPlan,
+    LowRankAdapters,
+    adapted_sparse_linear,
+    adapter_linear,
+    adapter_linear_backward,
+    adapter_plan,
+)
 from kairo_b200.ops.checkpoint import QuantizedActivations, dequantize_activations, quantize_activations
 from kairo_b200.ops.spmm import (
     KernelConfig,
@@ -74,6 +83,13 @@ __all__ = [
     "sort_mask_rows",
     "sparse_gather",
     "sparse_scatter_grad",
+    "AdaptedSparseLinear",
+    "AdapterPlan",
+    "LowRankAdapters",
+    "adapted_sparse_linear",
+    "adapter_linear",
+    "adapter_linear_backward",
+    "adapter_plan",
     "QuantizedActivations",
     "dequantize_activations",
     "quantize_activations",

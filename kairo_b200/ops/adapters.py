@@ -1,0 +1,337 @@
+"""Low-rank adapters of many requests in one batch, beside a shared
+projection (CUDA only).
+
+Every token of a batch may name one of G adapters (a rank-R correction of the
+projection's weight) or none:
+
+    low[t] = scale[a] * X[t] down[a]^T        Y[t] = base[t] + low[t] up[a]
+
+``base`` is the shared projection's output (``sparse_linear`` or any other).
+``up`` is stored rank row by rank row like ``down`` -- (G, R, out_features),
+the transpose of the usual (out_features, R) -- so that the backward pass is
+the same kernel with the two swapped.
+
+* ``adapter_plan(ids, G)`` -- the batch's tokens ordered by adapter, on the
+  device; made once per batch, used by every layer.
+* ``adapter_linear`` -- Y, for single tokens and prompts alike.
+* ``adapter_linear_backward`` -- dX and the gradients of down and up.
+* ``adapted_sparse_linear`` -- ``sparse_linear`` and the adapters, summed in
+  fp32 and rounded once.
+* ``AdaptedSparseLinear`` -- the same as a module with autograd.
+
+The reference has no counterpart.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+
+import torch
+from torch import Tensor
+
+from kairo_b200 import _lib
+from kairo_b200.ops.backward import (
+    BlockSparseLinear,
+    sparse_linear_weight_grad,
+    transpose_values,
+)
+from kairo_b200.ops.checkpoint import QuantizedActivations, dequantize_activations, quantize_activations
+from kairo_b200.ops.spmm import KernelConfig, _require_cuda, sparse_linear
+from kairo_b200.ops.token_embedding import _flat_ids, _ld, _rows, _same_device, _scratch
+from kairo_b200.types import BlockSparseMatrix
+
+MAX_RANK = 128
+
+
+@dataclass(frozen=True)
+class LowRankAdapters:
+    """G adapters of one projection.
+
+    down: (G, R, in_features); up: (G, R, out_features), float16 or bfloat16,
+    contiguous; scale: (G,) float32, or None for 1.  Adapters of a smaller
+    rank are padded with zero rows."""
+
+    down: Tensor
+    up: Tensor
+    scale: Tensor | None = None
+
+    def __post_init__(self) -> None:
+        if self.down.dim() != 3 or self.up.dim() != 3 or self.down.shape[:2] != self.up.shape[:2]:
+            raise ValueError(f"down must be (G, R, in) and up (G, R, out), got {tuple(self.down.shape)} and "
+                             f"{tuple(self.up.shape)}")
+        if self.down.dtype != self.up.dtype:
+            raise TypeError("down and up must share a dtype")
+        if self.down.dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError(f"adapters must be float16 or bfloat16, got {self.down.dtype}")
+        if not 1 <= self.down.shape[1] <= MAX_RANK or self.down.shape[2] < 1 or self.up.shape[2] < 1:
+            raise ValueError(f"the rank must be 1 to {MAX_RANK} and the features positive")
+        if not (self.down.is_contiguous() and self.up.is_contiguous()):
+            raise ValueError("down and up must be contiguous")
+        if self.scale is not None and (tuple(self.scale.shape) != (self.down.shape[0],)
+                                       or self.scale.dtype != torch.float32 or not self.scale.is_contiguous()):
+            raise ValueError(f"scale must be a contiguous ({self.down.shape[0]},) float32 tensor")
+        for t in (self.up, self.scale):
+            if t is not None and t.device != self.down.device:
+                raise ValueError("down, up and scale must share a device")
+
+    @property
+    def count(self) -> int:
+        return self.down.shape[0]
+
+    @property
+    def rank(self) -> int:
+        return self.down.shape[1]
+
+    @property
+    def in_features(self) -> int:
+        return self.down.shape[2]
+
+    @property
+    def out_features(self) -> int:
+        return self.up.shape[2]
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return self.down.dtype
+
+
+@dataclass(frozen=True)
+class AdapterPlan:
+    """The tokens of a batch ordered by adapter (``adapter_plan``); opaque."""
+
+    memory: Tensor
+    num_tokens: int
+    num_adapters: int
+
+
+def adapter_plan(ids: Tensor, num_adapters: int) -> AdapterPlan:
+    """Plan of a batch whose token t uses adapter ``ids[t]`` (int32 or int64,
+    any shape, taken flat); an id outside [0, num_adapters), such as -1,
+    means none.  Asynchronous, no read-back."""
+    _require_cuda(ids, op="adapter_plan")
+    g = int(num_adapters)
+    if g < 0:
+        raise ValueError("num_adapters must be non-negative")
+    flat = _flat_ids(ids, "adapter_plan")
+    dev = flat.device
+    n = flat.numel()
+    lib = _lib.lib()
+    with torch.cuda.device(dev):
+        size, ws_size = ctypes.c_size_t(0), ctypes.c_size_t(0)
+        _lib.check(lib.kairo_adapter_plan_size(n, g, ctypes.byref(size), ctypes.byref(ws_size)), "adapter_plan")
+        mem = _scratch(size.value, dev)
+        ws = _scratch(ws_size.value, dev)
+        _lib.check(lib.kairo_adapter_plan_build(flat.data_ptr(), flat.element_size(), n, g, mem.data_ptr(),
+                                                mem.numel(), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev)),
+                   "adapter_plan")
+    return AdapterPlan(memory=mem, num_tokens=n, num_adapters=g)
+
+
+def _check_batch(X, features: int, adapters: LowRankAdapters, plan: AdapterPlan, name: str, op: str) -> None:
+    if len(X.shape) != 2 or X.shape[1] != features:
+        raise ValueError(f"{op}: {name} must be (tokens, {features}), got {tuple(X.shape)}")
+    if X.dtype != adapters.dtype:
+        raise TypeError(f"{op}: {name} is {X.dtype}, the adapters are {adapters.dtype}")
+    if plan.num_tokens != X.shape[0]:
+        raise ValueError(f"{op}: the plan is of {plan.num_tokens} tokens, {name} has {X.shape[0]}")
+    if plan.num_adapters != adapters.count:
+        raise ValueError(f"{op}: the plan is of {plan.num_adapters} adapters, not {adapters.count}")
+
+
+def _apply(X: Tensor, down: Tensor, up: Tensor, scale: Tensor | None, plan: AdapterPlan, base: Tensor | None,
+           out: Tensor | None, low: Tensor, op: str) -> None:
+    dev = X.device
+    n = up.shape[2]
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().kairo_low_rank_apply(
+            X.data_ptr(), _ld(X), X.shape[1], down.data_ptr(), up.data_ptr(), n, down.shape[1],
+            _lib.kairo_dtype(X.dtype), _lib.ptr(scale), plan.memory.data_ptr(), plan.num_tokens, plan.num_adapters,
+            _lib.ptr(base), _ld(base) if base is not None else n,
+            _lib.kairo_dtype(base.dtype if base is not None else X.dtype), _lib.ptr(out),
+            _ld(out) if out is not None else n, _lib.kairo_dtype(out.dtype if out is not None else X.dtype), low.data_ptr(), _lib.stream_handle(dev)), op)
+
+
+def _result(shape: tuple[int, int], base: Tensor | None, out: Tensor | None, dtype: torch.dtype | None,
+            adapters: LowRankAdapters, op: str) -> tuple[Tensor | None, Tensor]:
+    """The checked base (rows contiguous) and the tensor to write."""
+    dev = adapters.down.device
+    odt = dtype or (out.dtype if out is not None else adapters.dtype)
+    if odt not in (torch.float32, adapters.dtype):
+        raise TypeError(f"{op}: the output must be float32 or {adapters.dtype}, got {odt}")
+    if base is not None:
+        if tuple(base.shape) != shape or base.device != dev:
+            raise ValueError(f"{op}: base must be {shape} on {dev}")
+        if base.dtype not in (torch.float32, adapters.dtype):
+            raise TypeError(f"{op}: base must be float32 or {adapters.dtype}, got {base.dtype}")
+        base = _rows(base)
+    if out is None:
+        out = torch.empty(shape, dtype=odt, device=dev)
+    elif tuple(out.shape) != shape or out.dtype != odt or out.device != dev or _rows(out) is not out:
+        raise ValueError(f"{op}: out must be a row-major {shape} {odt} tensor on {dev}")
+    return base, out
+
+
+def adapter_linear(X: Tensor, adapters: LowRankAdapters, plan: AdapterPlan, *, base: Tensor | None = None,
+                   out_dtype: torch.dtype | None = None, out: Tensor | None = None,
+                   return_low: bool = False) -> Tensor | tuple[Tensor, Tensor]:
+    """``Y[t] = base[t] + scale[a] * (X[t] down[a]^T) up[a]`` for the adapter a of each token.
+
+    X: (tokens, in_features) in the adapters' dtype; base: (tokens,
+    out_features) in that dtype or float32, None for zero.  The sum is formed
+    in fp32 and rounded once to ``out_dtype`` (default: the adapters').
+    ``out`` may be ``base`` itself.  ``return_low=True`` also returns the
+    (tokens, rank) float32 values ``scale[a] * X[t] down[a]^T`` that
+    ``adapter_linear_backward`` takes."""
+    op = "adapter_linear"
+    _require_cuda(X, adapters.down, op=op)
+    _same_device(X, adapters.down, plan.memory, op=op)
+    _check_batch(X, adapters.in_features, adapters, plan, "X", op)
+    base, out = _result((X.shape[0], adapters.out_features), base, out, out_dtype, adapters, op)
+    low = torch.empty(X.shape[0], adapters.rank, dtype=torch.float32, device=X.device)
+    _apply(_rows(X), adapters.down, adapters.up, adapters.scale, plan, base, out, low, op)
+    return (out, low) if return_low else out
+
+
+def _wgrad(low: Tensor, Z: Tensor, plan: AdapterPlan, dtype: torch.dtype, op: str) -> Tensor:
+    dev = Z.device
+    grad = torch.empty(plan.num_adapters, low.shape[1], Z.shape[1], dtype=dtype, device=dev)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().kairo_low_rank_wgrad(low.data_ptr(), low.shape[1], Z.data_ptr(), _ld(Z), Z.shape[1],
+                                                   _lib.kairo_dtype(Z.dtype), plan.memory.data_ptr(),
+                                                   plan.num_tokens, plan.num_adapters, grad.data_ptr(),
+                                                   _lib.kairo_dtype(dtype), _lib.stream_handle(dev)), op)
+    return grad
+
+
+def adapter_linear_backward(dY: Tensor, X: Tensor | QuantizedActivations, adapters: LowRankAdapters,
+                            plan: AdapterPlan, *, low: Tensor | None = None, base_dx: Tensor | None = None,
+                            need_dx: bool = True, need_dw: bool = True, dx_dtype: torch.dtype | None = None,
+                            grad_dtype: torch.dtype | None = None
+                            ) -> tuple[Tensor | None, Tensor | None, Tensor | None]:
+    """(dX, d_down, d_up) of ``adapter_linear``; the gradient by its base is dY.
+
+    X may be given in 8 bits.  ``low``: what ``return_low`` gave (computed
+    anew from X otherwise).  ``base_dx``: the shared projection's part of
+    dX, added in fp32 before the one rounding to ``dx_dtype`` (default: the
+    adapters').  d_down and d_up are in ``grad_dtype`` (default: the
+    adapters'), zero for an adapter without tokens."""
+    op = "adapter_linear_backward"
+    kept = X if isinstance(X, QuantizedActivations) else None
+    _require_cuda(dY, kept.codes if kept else X, adapters.down, op=op)
+    _same_device(dY, kept.codes if kept else X, adapters.down, plan.memory, op=op)
+    _check_batch(dY, adapters.out_features, adapters, plan, "dY", op)
+    gdt = grad_dtype or adapters.dtype
+    if gdt not in (torch.float32, adapters.dtype):
+        raise TypeError(f"{op}: the gradients must be float32 or {adapters.dtype}, got {gdt}")
+    if need_dw:
+        _check_batch(X, adapters.in_features, adapters, plan, "X", op)
+        if kept and low is None:
+            raise ValueError(f"{op}: an X in 8 bits needs the low of the forward pass")
+        if low is not None and (tuple(low.shape) != (dY.shape[0], adapters.rank) or low.dtype != torch.float32
+                                or low.device != dY.device):
+            raise ValueError(f"{op}: low must be a ({dY.shape[0]}, {adapters.rank}) float32 tensor")
+    dX = None
+    if need_dx:
+        base_dx, dX = _result((dY.shape[0], adapters.in_features), base_dx, None, dx_dtype, adapters, op)
+    dY = _rows(dY)
+    dlow = torch.empty(dY.shape[0], adapters.rank, dtype=torch.float32, device=dY.device)
+    _apply(dY, adapters.up, adapters.down, adapters.scale, plan, base_dx if need_dx else None, dX, dlow, op)
+    if not need_dw:
+        return dX, None, None
+    Z = dequantize_activations(kept) if kept else _rows(X)
+    if low is None:
+        low = torch.empty_like(dlow)
+        _apply(Z, adapters.down, adapters.up, adapters.scale, plan, None, None, low, op)
+    d_down = _wgrad(dlow, Z, plan, gdt, op)
+    d_up = _wgrad(low.contiguous(), dY, plan, gdt, op)
+    return dX, d_down, d_up
+
+
+def adapted_sparse_linear(X: Tensor, W: BlockSparseMatrix, adapters: LowRankAdapters, plan: AdapterPlan, *,
+                          out_dtype: torch.dtype | None = None, config: KernelConfig | None = None,
+                          return_low: bool = False) -> Tensor | tuple[Tensor, Tensor]:
+    """``sparse_linear(X, W)`` plus each token's adapter: the projection's fp32
+    result and the adapter's are added before the one rounding to
+    ``out_dtype`` (default: X's)."""
+    if tuple(W.shape) != (adapters.out_features, adapters.in_features):
+        raise ValueError(f"W is {tuple(W.shape)}, the adapters are for "
+                         f"({adapters.out_features}, {adapters.in_features})")
+    odt = out_dtype or X.dtype
+    base = sparse_linear(X, W, out_dtype=torch.float32, config=config)
+    return adapter_linear(X, adapters, plan, base=base, out_dtype=odt,
+                          out=base if odt == torch.float32 else None, return_low=return_low)
+
+
+class _AdaptedLinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, X: Tensor, blocks: Tensor, down: Tensor, up: Tensor, module: "AdaptedSparseLinear",
+                plan: AdapterPlan) -> Tensor:
+        layer = module.layer
+        W = layer.weight_matrix(blocks)
+        Y, low = adapted_sparse_linear(X, W, module.adapters(down, up), plan, return_low=True)
+        need_x = any(ctx.needs_input_grad[1:4])
+        kept: list[Tensor] = []
+        ctx.kept_dtype = None
+        if need_x and layer.checkpoint is not None:
+            q = quantize_activations(X)
+            kept, ctx.kept_dtype = [q.codes, q.steps], q.dtype
+        elif need_x:
+            kept = [X]
+        ctx.save_for_backward(blocks, down, up, low, *kept)
+        ctx.module, ctx.plan, ctx.need_x = module, plan, need_x
+        return Y
+
+    @staticmethod
+    def backward(ctx, dY: Tensor):
+        blocks, down, up, low, *kept = ctx.saved_tensors
+        module: AdaptedSparseLinear = ctx.module
+        layer = module.layer
+        X = None
+        if ctx.need_x:
+            X = kept[0] if ctx.kept_dtype is None else QuantizedActivations(codes=kept[0], steps=kept[1],
+                                                                             dtype=ctx.kept_dtype)
+        W = layer.weight_matrix(blocks)
+        dY = dY.contiguous()
+        need_dx, need_blocks = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        need_dw = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
+        wt = transpose_values(W, layer.transposed()) if need_dx or need_blocks else None
+        base_dx = sparse_linear(dY, wt.matrix, out_dtype=torch.float32) if need_dx else None
+        dX = d_down = d_up = None
+        if need_dx or need_dw:
+            dX, d_down, d_up = adapter_linear_backward(dY, X, module.adapters(down, up), ctx.plan, low=low,
+                                                       base_dx=base_dx, need_dx=need_dx, need_dw=need_dw)
+        d_blocks = sparse_linear_weight_grad(dY, X, W, wt, out_dtype=blocks.dtype) if need_blocks else None
+        return dX, d_blocks, d_down, d_up, None, None
+
+
+class AdaptedSparseLinear(torch.nn.Module):
+    """A ``BlockSparseLinear`` with low-rank adapters: ``forward(X, plan)``.
+
+    ``down`` (G, R, in_features) and ``up`` (G, R, out_features) are
+    parameters; ``up`` starts at zero, so that a new adapter changes nothing.
+    The layer's blocks train too unless frozen
+    (``layer.blocks.requires_grad_(False)``).  A layer built with
+    ``checkpoint="int8"`` keeps its input in 8 bits for all three
+    gradients."""
+
+    def __init__(self, layer: BlockSparseLinear, num_adapters: int, rank: int, *,
+                 scale: float | Tensor = 1.0) -> None:
+        super().__init__()
+        out_features, in_features = layer.shape
+        if num_adapters < 1 or not 1 <= rank <= MAX_RANK:
+            raise ValueError(f"num_adapters must be positive and the rank 1 to {MAX_RANK}")
+        dev, dt = layer.blocks.device, layer.blocks.dtype
+        self.layer = layer
+        self.down = torch.nn.Parameter((torch.randn(num_adapters, rank, in_features, device=dev)
+                                        * in_features**-0.5).to(dt))
+        self.up = torch.nn.Parameter(torch.zeros(num_adapters, rank, out_features, dtype=dt, device=dev))
+        s = torch.as_tensor(scale, dtype=torch.float32, device=dev)
+        self.register_buffer("scale", s.expand(num_adapters).clone())
+
+    def adapters(self, down: Tensor | None = None, up: Tensor | None = None) -> LowRankAdapters:
+        return LowRankAdapters(down=(self.down if down is None else down).detach(),
+                               up=(self.up if up is None else up).detach(), scale=self.scale)
+
+    def forward(self, X: Tensor, plan: AdapterPlan) -> Tensor:
+        return _AdaptedLinearFn.apply(X, self.layer.blocks, self.down, self.up, self, plan)

@@ -10,9 +10,15 @@ import torch
 
 from kairo_b200 import _lib
 from kairo_b200.ops import (
+    AdapterPlan,
+    AdaptedSparseLinear,
     BlockSparseLinear,
+    LowRankAdapters,
     QuantizedActivations,
     ScaledEmbedding,
+    adapter_linear,
+    adapter_linear_backward,
+    adapter_plan,
     dequantize_activations,
     embedding_grad,
     embedding_lookup,
@@ -128,3 +134,72 @@ def test_checkpoint_c_refusals():
                {"ws": None}, {"dy": None}):
         assert wgrad(**kw) == _lib.INVALID_VALUE, kw
     assert wgrad(wsb=n.value - 1) == _lib.WORKSPACE_TOO_SMALL
+
+
+def test_adapter_refusals():
+    down, up = torch.zeros(3, 8, 64, dtype=torch.bfloat16), torch.zeros(3, 8, 32, dtype=torch.bfloat16)
+    a = LowRankAdapters(down=down, up=up)
+    assert (a.count, a.rank, a.in_features, a.out_features) == (3, 8, 64, 32)
+    for bad in ({"down": down[0]}, {"up": up[:2]}, {"up": up[:, :4]}, {"down": down.transpose(1, 2)},
+                {"down": torch.zeros(3, 129, 64, dtype=torch.bfloat16), "up": torch.zeros(3, 129, 32,
+                                                                                           dtype=torch.bfloat16)},
+                {"down": down[:, :0], "up": up[:, :0]}, {"scale": torch.ones(2)},
+                {"scale": torch.ones(3, dtype=torch.float64)}, {"scale": torch.ones(6)[::2]}):
+        with pytest.raises(ValueError):
+            LowRankAdapters(**{"down": down, "up": up, **bad})
+    for bad in ({"down": down.half()}, {"down": down.float(), "up": up.float()}):
+        with pytest.raises(TypeError):
+            LowRankAdapters(**{"down": down, "up": up, **bad})
+    plan = AdapterPlan(memory=torch.zeros(256, dtype=torch.uint8), num_tokens=4, num_adapters=3)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        adapter_plan(torch.zeros(4, dtype=torch.int64), 3)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        adapter_linear(torch.zeros(4, 64, dtype=torch.bfloat16), a, plan)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        adapter_linear_backward(torch.zeros(4, 32, dtype=torch.bfloat16), torch.zeros(4, 64, dtype=torch.bfloat16), a,
+                                plan)
+    layer = BlockSparseLinear(_bsr())
+    with pytest.raises(ValueError):
+        AdaptedSparseLinear(layer, 0, 8)
+    with pytest.raises(ValueError):
+        AdaptedSparseLinear(layer, 2, 200)
+
+
+def test_adapter_c_refusals():
+    lib = _lib.lib()
+    some = ctypes.c_void_p(256)
+    a, b = ctypes.c_size_t(0), ctypes.c_size_t(0)
+    size = lib.kairo_adapter_plan_size
+    assert size(10, 3, None, ctypes.byref(b)) == _lib.INVALID_VALUE
+    assert size(-1, 3, ctypes.byref(a), ctypes.byref(b)) == _lib.INVALID_VALUE
+    assert size(10, 65536, ctypes.byref(a), ctypes.byref(b)) == _lib.NOT_SUPPORTED
+    assert size((1 << 24) + 1, 3, ctypes.byref(a), ctypes.byref(b)) == _lib.NOT_SUPPORTED
+    assert size(10, 3, ctypes.byref(a), ctypes.byref(b)) == _lib.SUCCESS
+
+    def build(ids=some, idb=8, plan=some, pb=a.value, ws=some, wb=b.value):
+        return lib.kairo_adapter_plan_build(ids, idb, 10, 3, plan, pb, ws, wb, None)
+
+    for kw in ({"ids": None}, {"idb": 1}, {"plan": None}, {"pb": a.value - 1}, {"ws": None}):
+        assert build(**kw) == _lib.INVALID_VALUE, kw
+    assert build(wb=b.value - 1) == _lib.WORKSPACE_TOO_SMALL
+
+    def apply(x=some, ldx=64, k=64, down=some, up=some, n=32, rank=8, dt=2, plan=some, t=10, g=3, base=some, ldb=32,
+              bdt=2, y=some, ldy=32, ydt=2, low=some):
+        return lib.kairo_low_rank_apply(x, ldx, k, down, up, n, rank, dt, None, plan, t, g, base, ldb, bdt, y, ldy,
+                                        ydt, low, None)
+
+    for kw in ({"x": None}, {"ldx": 63}, {"k": 0}, {"down": None}, {"up": None}, {"n": 0}, {"rank": 0}, {"dt": 0},
+               {"plan": None}, {"t": -1}, {"g": -1}, {"ldb": 31}, {"bdt": 1}, {"ldy": 31}, {"ydt": 1}, {"low": None}):
+        assert apply(**kw) == _lib.INVALID_VALUE, kw
+    for kw in ({"rank": 129}, {"g": 65536}, {"t": (1 << 24) + 1}, {"k": (1 << 22) + 1, "ldx": 1 << 23}):
+        assert apply(**kw) == _lib.NOT_SUPPORTED, kw
+    assert apply(t=0) == _lib.SUCCESS
+
+    def wgrad(low=some, rank=8, z=some, ldz=64, k=64, dt=2, plan=some, t=10, g=3, grad=some, gdt=0):
+        return lib.kairo_low_rank_wgrad(low, rank, z, ldz, k, dt, plan, t, g, grad, gdt, None)
+
+    for kw in ({"low": None}, {"rank": 0}, {"z": None}, {"ldz": 63}, {"k": 0}, {"dt": 0}, {"plan": None}, {"t": -1},
+               {"g": -1}, {"grad": None}, {"gdt": 1}):
+        assert wgrad(**kw) == _lib.INVALID_VALUE, kw
+    assert wgrad(rank=129) == _lib.NOT_SUPPORTED
+    assert wgrad(g=0) == _lib.SUCCESS
