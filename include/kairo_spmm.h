@@ -366,7 +366,7 @@ KAIRO_API kairo_status kairo_bsr_sddmm_q8_workspace_size(const kairo_bsr* a, int
  *                         lives in caller memory of kairo_adapter_plan_size
  *                         bytes, is opaque, and serves every layer.
  *   kairo_low_rank_apply  low[t] = scale[a] * x[t] down_a^T (ntokens x rank,
- *                         fp32, written), y[t] = base[t] + low[t] up_a, a the
+ *                         fp32; written unless NULL), y[t] = base[t] + low[t] up_a, a the
  *                         adapter of token t; low = 0 and y = base for a
  *                         token without one.  down is (nadapters, rank, k),
  *                         up (nadapters, rank, n), both contiguous; scale may
@@ -378,6 +378,9 @@ KAIRO_API kairo_status kairo_bsr_sddmm_q8_workspace_size(const kairo_bsr* a, int
  *   kairo_low_rank_wgrad  grad (nadapters, rank, k) = for every adapter the
  *                         sum over its tokens of low[t]^T z[t], zeros for one
  *                         without tokens; no atomics.
+ *   kairo_low_rank_wgrad_q8  the same with z given in 8 bits
+ *                         (kairo_quantize_q8); dtype is the type it reads
+ *                         back in.
  * x, z, down, up f16 or bf16 (one dtype); base, y and grad that dtype or fp32.
  * rank at most 128, at most 65535 adapters, 2^24 tokens, 2^22 features.  All
  * asynchronous on `stream`.
@@ -394,6 +397,10 @@ KAIRO_API kairo_status kairo_low_rank_apply(const void* x, int64_t ldx, int64_t 
 KAIRO_API kairo_status kairo_low_rank_wgrad(const float* low, int64_t rank, const void* z, int64_t ldz, int64_t k,
                                             kairo_dtype dtype, const void* plan, int64_t ntokens, int64_t nadapters,
                                             void* grad, kairo_dtype grad_dtype, void* stream);
+KAIRO_API kairo_status kairo_low_rank_wgrad_q8(const float* low, int64_t rank, const int8_t* codes, int64_t ldq,
+                                               const float* steps, int64_t lds, int64_t k, kairo_dtype dtype,
+                                               const void* plan, int64_t ntokens, int64_t nadapters, void* grad,
+                                               kairo_dtype grad_dtype, void* stream);
 
 /* ------------------------------------------------------------------------
  * Block-granular pruning (no counterpart in the reference, which prunes

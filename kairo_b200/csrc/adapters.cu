@@ -16,27 +16,48 @@
 
 #include <algorithm>
 
-#include "convert.cuh"
+#include "adapters_kernel.cuh"
 #include "internal.h"
 
 namespace kairo {
 namespace {
 
-// Plan memory, int32 words: the token order (T), then starts (G + 2): the
-// tokens of adapter a are order[starts[a] .. starts[a + 1]), those without one
-// order[starts[G] .. starts[G + 1]).
+// Plan memory, int32 words: the number of tiles of 16, 32 and 64 tokens, the
+// token order (T), starts (G + 2: the tokens of adapter a are order[starts[a]
+// .. starts[a + 1]), those without one order[starts[G] .. starts[G + 1])), for
+// each tile size the first tile of every adapter (G + 2), and the tiles.
+constexpr int kTileSizes = 3;
+__host__ __device__ constexpr int tile_tokens(int which) { return 16 << which; }
+
 struct Plan {
+  int32_t* ntiles;
   int32_t* order;
   int32_t* starts;
+  int32_t* first[kTileSizes];
+  LowRankTile* tiles[kTileSizes];
 };
 
-Plan carve_plan(void* mem, int64_t t) {
-  int32_t* p = static_cast<int32_t*>(mem);
-  return Plan{p, p + align_up(static_cast<size_t>(t), 64)};
-}
+// Tiles of `size` tokens that a batch can have: whole ones, and a rest per
+// group of tokens (G adapters, and those without).
+int64_t max_tiles(int64_t t, int64_t g, int size) { return t / size + std::min(t, g + 1); }
 
-size_t plan_bytes(int64_t t, int64_t g) {
-  return (align_up(static_cast<size_t>(t), 64) + align_up(static_cast<size_t>(g + 2), 64)) * sizeof(int32_t);
+size_t carve_plan(void* mem, int64_t t, int64_t g, Plan* pl) {
+  int32_t* p = static_cast<int32_t*>(mem);
+  size_t at = 64;
+  auto take = [&](int64_t words) {
+    int32_t* q = p ? p + at : nullptr;
+    at += align_up(static_cast<size_t>(words), 64);
+    return q;
+  };
+  Plan q{};
+  q.ntiles = p;
+  q.order = take(t);
+  q.starts = take(g + 2);
+  for (int i = 0; i < kTileSizes; ++i) q.first[i] = take(g + 2);
+  for (int i = 0; i < kTileSizes; ++i)
+    q.tiles[i] = reinterpret_cast<LowRankTile*>(take(max_tiles(t, g, tile_tokens(i)) * 4));
+  if (pl) *pl = q;
+  return at * sizeof(int32_t);
 }
 
 __global__ void k_plan_starts(const uint32_t* __restrict__ sorted, int64_t t, int64_t g, int32_t* __restrict__ starts) {
@@ -52,88 +73,73 @@ __global__ void k_plan_starts(const uint32_t* __restrict__ sorted, int64_t t, in
   }
 }
 
-// The adapter of a position of the order (g: none).
-__device__ __forceinline__ int64_t adapter_at(const int32_t* starts, int64_t g, int64_t p) {
-  int64_t lo = 0, hi = g;  // last a with starts[a] <= p and tokens behind it
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (starts[mid + 1] <= p) lo = mid + 1;
-    else hi = mid;
-  }
-  return lo;
-}
-
-// One warp per (position, rank row).
-template <typename T>
-__global__ void __launch_bounds__(256) k_low(const T* __restrict__ x, int64_t ldx, int64_t k,
-                                             const T* __restrict__ down, int64_t rank,
-                                             const float* __restrict__ scale, const int32_t* __restrict__ order,
-                                             const int32_t* __restrict__ starts, int64_t t, int64_t g,
-                                             float* __restrict__ low) {
-  const int lane = threadIdx.x & 31;
-  const int64_t w = (blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x) >> 5;
-  const int64_t p = w / rank, r = w - p * rank;
-  if (p >= t) return;
-  const int64_t tok = order[p];
-  const int64_t a = adapter_at(starts, g, p);
-  float acc = 0.f;
-  if (a < g) {
-    const T* xr = x + tok * ldx;
-    const T* dr = down + (a * rank + r) * k;
-    for (int64_t c = lane; c < k; c += 32) acc += to_f32<T>(xr[c]) * to_f32<T>(dr[c]);
-    for (int o = 16; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-    if (scale) acc *= scale[a];
-  }
-  if (lane == 0) low[tok * rank + r] = acc;
-}
-
-template <typename T, typename TB, typename TY>
-__global__ void __launch_bounds__(256) k_expand(const float* __restrict__ low, int64_t rank,
-                                                const T* __restrict__ up, int64_t n, const TB* base, int64_t ldb,
-                                                TY* y, int64_t ldy, const int32_t* __restrict__ order,
-                                                const int32_t* __restrict__ starts, int64_t t, int64_t g) {
-  const int64_t p = blockIdx.x;
-  const int64_t tok = order[p];
-  const int64_t a = adapter_at(starts, g, p);
-  for (int64_t c = static_cast<int64_t>(blockIdx.y) * blockDim.x + threadIdx.x; c < n;
-       c += static_cast<int64_t>(gridDim.y) * blockDim.x) {
-    float acc = base ? to_f32<TB>(base[tok * ldb + c]) : 0.f;
-    if (a < g) {
-      float d = 0.f;
-      for (int64_t r = 0; r < rank; ++r) d += low[tok * rank + r] * to_f32<T>(up[(a * rank + r) * n + c]);
-      acc += d;
-    }
-    y[tok * ldy + c] = from_f32<TY>(acc);
-  }
-}
-
-// grad[a, r, c] = sum over the adapter's tokens of s[t, r] * z[t, c].
-template <typename T, typename TG>
-__global__ void __launch_bounds__(128) k_low_wgrad(const float* __restrict__ s, int64_t rank,
-                                                   const T* __restrict__ z, int64_t ldz, int64_t k,
-                                                   const int32_t* __restrict__ order,
-                                                   const int32_t* __restrict__ starts, TG* __restrict__ grad) {
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int64_t a = blockIdx.y;
-  if (c >= k) return;
-  const int p0 = starts[a], p1 = starts[a + 1];
-  for (int64_t r0 = 0; r0 < rank; r0 += 8) {
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int p = p0; p < p1; ++p) {
-      const int64_t tok = order[p];
-      const float v = to_f32<T>(z[tok * ldz + c]);
+// First tile of every adapter, and the number of tiles, for one tile size per CTA.
+__global__ void __launch_bounds__(1024) k_plan_first(Plan pl, int64_t g) {
+  __shared__ int sums[32];
+  __shared__ int carry;
+  const int size = tile_tokens(blockIdx.x);
+  int32_t* first = blockIdx.x == 0 ? pl.first[0] : (blockIdx.x == 1 ? pl.first[1] : pl.first[2]);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) carry = 0;
+  __syncthreads();
+  for (int64_t base = 0; base <= g; base += 1024) {
+    const int64_t a = base + threadIdx.x;  // g: tokens without an adapter
+    const int v = a <= g ? (pl.starts[a + 1] - pl.starts[a] + size - 1) / size : 0;
+    int x = v;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (r0 + i < rank) acc[i] += s[tok * rank + r0 + i] * v;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
     }
+    if (lane == 31) sums[warp] = x;
+    __syncthreads();
+    if (warp == 0) {
+      int w = sums[lane];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (r0 + i < rank) grad[(a * rank + r0 + i) * k + c] = from_f32<TG>(acc[i]);
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += y;
+      }
+      sums[lane] = w;
+    }
+    __syncthreads();
+    const int incl = carry + x + (warp ? sums[warp - 1] : 0);
+    if (a <= g) first[a] = incl - v;
+    __syncthreads();
+    if (threadIdx.x == 1023) carry = incl;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    first[g + 1] = carry;
+    pl.ntiles[blockIdx.x] = carry;
+  }
+}
+
+__global__ void k_plan_tiles(Plan pl, int64_t g) {
+  const int size = tile_tokens(blockIdx.y);
+  const int32_t* first = blockIdx.y == 0 ? pl.first[0] : (blockIdx.y == 1 ? pl.first[1] : pl.first[2]);
+  LowRankTile* tiles = blockIdx.y == 0 ? pl.tiles[0] : (blockIdx.y == 1 ? pl.tiles[1] : pl.tiles[2]);
+  const int n = first[g + 1];
+  for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) {
+    int64_t lo = 0, hi = g;  // the adapter a with first[a] <= i < first[a + 1]
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (first[mid + 1] <= i) lo = mid + 1;
+      else hi = mid;
+    }
+    LowRankTile tile;
+    tile.adapter = lo < g ? static_cast<int32_t>(lo) : -1;
+    tile.begin = pl.starts[lo] + (i - first[lo]) * size;
+    tile.count = min(size, pl.starts[lo + 1] - tile.begin);
+    tile.pad = 0;
+    tiles[i] = tile;
   }
 }
 
 constexpr int64_t kMaxAdapters = 65535;
 constexpr int64_t kMaxRank = 128;
+constexpr int kCluster = 8;        // CTAs that share a tile
+constexpr int kChunkTokens = 64;   // tokens of one step of the weight gradient
 
 kairo_status check_low_rank(int64_t t, int64_t k, int64_t n, int64_t rank, int64_t g, kairo_dtype dtype) {
   if (t < 0 || k <= 0 || n <= 0 || rank <= 0 || g < 0) return fail(KAIRO_STATUS_INVALID_VALUE, "invalid size");
@@ -146,31 +152,14 @@ kairo_status check_low_rank(int64_t t, int64_t k, int64_t n, int64_t rank, int64
   return KAIRO_STATUS_SUCCESS;
 }
 
-template <typename T, typename TB, typename TY>
-void apply_launch(const void* x, int64_t ldx, int64_t k, const void* down, const void* up, int64_t n, int64_t rank,
-                  const float* scale, const Plan& pl, int64_t t, int64_t g, const void* base, int64_t ldb, void* y,
-                  int64_t ldy, float* low, cudaStream_t s) {
-  k_low<T><<<static_cast<unsigned>(ceil_div64(t * rank, 8)), 256, 0, s>>>(
-      static_cast<const T*>(x), ldx, k, static_cast<const T*>(down), rank, scale, pl.order, pl.starts, t, g, low);
-  if (!y) return;
-  const dim3 grid(static_cast<unsigned>(t), static_cast<unsigned>(std::min<int64_t>(ceil_div64(n, 256), 64)));
-  k_expand<T, TB, TY><<<grid, 256, 0, s>>>(low, rank, static_cast<const T*>(up), n, static_cast<const TB*>(base), ldb,
-                                          static_cast<TY*>(y), ldy, pl.order, pl.starts, t, g);
-}
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-template <typename T>
-void apply_types(kairo_dtype base_dtype, kairo_dtype y_dtype, const void* x, int64_t ldx, int64_t k, const void* down,
-                 const void* up, int64_t n, int64_t rank, const float* scale, const Plan& pl, int64_t t, int64_t g,
-                 const void* base, int64_t ldb, void* y, int64_t ldy, float* low, cudaStream_t s) {
-  const bool bf = base_dtype == KAIRO_DTYPE_F32, yf = y_dtype == KAIRO_DTYPE_F32;
-  if (bf && yf)
-    apply_launch<T, float, float>(x, ldx, k, down, up, n, rank, scale, pl, t, g, base, ldb, y, ldy, low, s);
-  else if (bf)
-    apply_launch<T, float, T>(x, ldx, k, down, up, n, rank, scale, pl, t, g, base, ldb, y, ldy, low, s);
-  else if (yf)
-    apply_launch<T, T, float>(x, ldx, k, down, up, n, rank, scale, pl, t, g, base, ldb, y, ldy, low, s);
-  else
-    apply_launch<T, T, T>(x, ldx, k, down, up, n, rank, scale, pl, t, g, base, ldb, y, ldy, low, s);
+// Tokens per tile.  Small batches want many short tiles (one CTA cluster each)
+// for latency; long ones want tiles as tall as the accumulators allow,
+// because every tile reads its adapter's weights from L2 once.
+int pick_tile(int64_t t, int64_t rank, bool vec) {
+  if (!vec || t <= 2048 || rank > 64) return 16;
+  return rank <= 32 ? 64 : 32;
 }
 
 }  // namespace
@@ -185,7 +174,7 @@ extern "C" kairo_status kairo_adapter_plan_size(int64_t ntokens, int64_t nadapte
   size_t sort = 0;
   const kairo_status ss = kairo_token_sort_workspace_size(ntokens, nadapters, &sort);
   if (ss) return ss;
-  *plan = plan_bytes(ntokens, nadapters);
+  *plan = carve_plan(nullptr, ntokens, nadapters, nullptr);
   *workspace = align_up(static_cast<size_t>(ntokens) * sizeof(int32_t), 256) + sort;
   return KAIRO_STATUS_SUCCESS;
 }
@@ -201,7 +190,8 @@ extern "C" kairo_status kairo_adapter_plan_build(const void* ids, int32_t id_byt
   if (plan_size < need) return fail(KAIRO_STATUS_INVALID_VALUE, "plan memory too small");
   if (workspace_bytes < ws_need) return fail(KAIRO_STATUS_WORKSPACE_TOO_SMALL, "adapter plan workspace too small");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const Plan pl = carve_plan(plan, ntokens);
+  Plan pl;
+  carve_plan(plan, ntokens, nadapters, &pl);
   int32_t* sorted = static_cast<int32_t*>(workspace);
   const size_t col = align_up(static_cast<size_t>(ntokens) * sizeof(int32_t), 256);
   st = kairo_token_sort(ids, id_bytes, ntokens, nadapters, sorted, pl.order, static_cast<uint8_t*>(workspace) + col,
@@ -209,6 +199,9 @@ extern "C" kairo_status kairo_adapter_plan_build(const void* ids, int32_t id_byt
   if (st) return st;
   k_plan_starts<<<static_cast<unsigned>(ceil_div64(nadapters + 2, 256)), 256, 0, s>>>(
       reinterpret_cast<const uint32_t*>(sorted), ntokens, nadapters, pl.starts);
+  k_plan_first<<<kTileSizes, 1024, 0, s>>>(pl, nadapters);
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(ceil_div64(max_tiles(ntokens, nadapters, tile_tokens(0)), 256), 1024));
+  k_plan_tiles<<<dim3(static_cast<unsigned>(most), kTileSizes), 256, 0, s>>>(pl, nadapters);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "launch of the adapter plan");
   return KAIRO_STATUS_SUCCESS;
@@ -226,44 +219,103 @@ extern "C" kairo_status kairo_low_rank_apply(const void* x, int64_t ldx, int64_t
     return fail(KAIRO_STATUS_INVALID_VALUE, "base and y must be fp32 or the adapters' dtype");
   if (ldx < k || (y && ldy < n) || (base && ldb < n)) return fail(KAIRO_STATUS_INVALID_VALUE, "leading dimension too small");
   if (ntokens == 0) return KAIRO_STATUS_SUCCESS;
-  if (!x || !plan || !low || (nadapters > 0 && (!down || (y && !up))))
+  if (!x || !plan || (!y && !low) || (nadapters > 0 && (!down || (y && !up))))
     return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
-  const Plan pl = carve_plan(const_cast<void*>(plan), ntokens);
+  Plan pl;
+  carve_plan(const_cast<void*>(plan), ntokens, nadapters, &pl);
+  const int64_t e = 2;
+  const int64_t eb = base_dtype == KAIRO_DTYPE_F32 ? 4 : 2, ey = y_dtype == KAIRO_DTYPE_F32 ? 4 : 2;
+  const bool vec = k % 8 == 0 && n % 8 == 0 && ldx * e % 16 == 0 && aligned16(x) && aligned16(down) && aligned16(up) &&
+                   (!base || (ldb * eb % 16 == 0 && aligned16(base))) && (!y || (ldy * ey % 16 == 0 && aligned16(y)));
+  const int tile = pick_tile(ntokens, rank, vec);
+  const int which = tile == 16 ? 0 : (tile == 32 ? 1 : 2);
+  LowRankApplyArgs a{};
+  a.x = x;
+  a.down = down;
+  a.up = up;
+  a.base = base;
+  a.y = y;
+  a.low = low;
+  a.scale = scale;
+  a.order = pl.order;
+  a.tiles = pl.tiles[which];
+  a.ntiles = pl.ntiles + which;
+  a.ldx = ldx;
+  a.ldb = ldb;
+  a.ldy = ldy;
+  a.k = static_cast<int32_t>(k);
+  a.n = static_cast<int32_t>(n);
+  a.rank = static_cast<int32_t>(rank);
+  a.base_f32 = base && base_dtype == KAIRO_DTYPE_F32;
+  const int64_t clusters = max_tiles(ntokens, nadapters, tile);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (!base) base_dtype = dtype;
-  if (dtype == KAIRO_DTYPE_F16)
-    apply_types<__half>(base_dtype, y_dtype, x, ldx, k, down, up, n, rank, scale, pl, ntokens, nadapters, base, ldb, y,
-                        ldy, low, s);
-  else
-    apply_types<__nv_bfloat16>(base_dtype, y_dtype, x, ldx, k, down, up, n, rank, scale, pl, ntokens, nadapters, base,
-                               ldb, y, ldy, low, s);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, "launch of the low-rank product");
+  const bool yf = y && y_dtype == KAIRO_DTYPE_F32;
+  const cudaError_t err = dtype == KAIRO_DTYPE_F16
+                              ? launch_low_rank_apply<__half>(a, yf, vec, tile, clusters, kCluster, s)
+                              : launch_low_rank_apply<__nv_bfloat16>(a, yf, vec, tile, clusters, kCluster, s);
+  if (err != cudaSuccess) return cuda_fail(err, "launch of the low-rank product");
   return KAIRO_STATUS_SUCCESS;
 }
 
-extern "C" kairo_status kairo_low_rank_wgrad(const float* low, int64_t rank, const void* z, int64_t ldz, int64_t k,
-                                             kairo_dtype dtype, const void* plan, int64_t ntokens, int64_t nadapters,
-                                             void* grad, kairo_dtype grad_dtype, void* stream) {
+namespace {
+
+// Both forms of the gradient: z in its own type, or codes and steps.
+kairo_status wgrad(const float* low, int64_t rank, const void* z, int64_t ldz, const int8_t* codes, int64_t ldq,
+                   const float* steps, int64_t lds, int64_t k, kairo_dtype dtype, const void* plan, int64_t ntokens,
+                   int64_t nadapters, void* grad, kairo_dtype grad_dtype, void* stream) {
   const kairo_status st = check_low_rank(ntokens, k, 1, rank, nadapters, dtype);
   if (st) return st;
   if (grad_dtype != KAIRO_DTYPE_F32 && grad_dtype != dtype)
     return fail(KAIRO_STATUS_INVALID_VALUE, "the gradient must be fp32 or the adapters' dtype");
-  if (ldz < k) return fail(KAIRO_STATUS_INVALID_VALUE, "leading dimension too small");
   if (nadapters == 0) return KAIRO_STATUS_SUCCESS;
-  if (!plan || !grad || (ntokens > 0 && (!low || !z))) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
-  const Plan pl = carve_plan(const_cast<void*>(plan), ntokens);
+  if (!plan || !grad || (ntokens > 0 && !low)) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+  Plan pl;
+  carve_plan(const_cast<void*>(plan), ntokens, nadapters, &pl);
+  LowRankWgradArgs a{};
+  a.s = low;
+  a.z = z;
+  a.codes = codes;
+  a.steps = steps;
+  a.grad = grad;
+  a.order = pl.order;
+  a.starts = pl.starts;
+  a.ldz = ldz;
+  a.ldq = ldq;
+  a.lds = lds;
+  a.k = static_cast<int32_t>(k);
+  a.rank = static_cast<int32_t>(rank);
+  const bool vec = codes || (k % 8 == 0 && ldz % 8 == 0 && aligned16(z));
+  // One CTA takes 64 tokens at a time: no more CTAs per adapter than an
+  // evenly filled one has such chunks.
+  int cluster = 1;
+  while (cluster < kCluster && cluster * kChunkTokens < ntokens) cluster *= 2;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(ceil_div64(k, 128)), static_cast<unsigned>(nadapters));
-  auto go = [&](auto zt, auto gt) {
-    using T = decltype(zt);
-    using TG = decltype(gt);
-    k_low_wgrad<T, TG><<<grid, 128, 0, s>>>(low, rank, static_cast<const T*>(z), ldz, k, pl.order, pl.starts,
-                                           static_cast<TG*>(grad));
-  };
-  if (dtype == KAIRO_DTYPE_F16) grad_dtype == KAIRO_DTYPE_F32 ? go(__half{}, float{}) : go(__half{}, __half{});
-  else grad_dtype == KAIRO_DTYPE_F32 ? go(__nv_bfloat16{}, float{}) : go(__nv_bfloat16{}, __nv_bfloat16{});
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, "launch of the adapter gradient");
+  const bool gf = grad_dtype == KAIRO_DTYPE_F32;
+  const cudaError_t err = dtype == KAIRO_DTYPE_F16
+                              ? launch_low_rank_wgrad<__half>(a, gf, vec, nadapters, cluster, s)
+                              : launch_low_rank_wgrad<__nv_bfloat16>(a, gf, vec, nadapters, cluster, s);
+  if (err != cudaSuccess) return cuda_fail(err, "launch of the adapter gradient");
   return KAIRO_STATUS_SUCCESS;
+}
+
+}  // namespace
+
+extern "C" kairo_status kairo_low_rank_wgrad(const float* low, int64_t rank, const void* z, int64_t ldz, int64_t k,
+                                             kairo_dtype dtype, const void* plan, int64_t ntokens, int64_t nadapters,
+                                             void* grad, kairo_dtype grad_dtype, void* stream) {
+  if (ldz < k) return fail(KAIRO_STATUS_INVALID_VALUE, "leading dimension too small");
+  if (ntokens > 0 && nadapters > 0 && !z) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+  return wgrad(low, rank, z, ldz, nullptr, 0, nullptr, 0, k, dtype, plan, ntokens, nadapters, grad, grad_dtype, stream);
+}
+
+extern "C" kairo_status kairo_low_rank_wgrad_q8(const float* low, int64_t rank, const int8_t* codes, int64_t ldq,
+                                                const float* steps, int64_t lds, int64_t k, kairo_dtype dtype,
+                                                const void* plan, int64_t ntokens, int64_t nadapters, void* grad,
+                                                kairo_dtype grad_dtype, void* stream) {
+  if (ldq < k || lds < ntokens) return fail(KAIRO_STATUS_INVALID_VALUE, "leading dimension too small");
+  if (ldq % 16 || !aligned16(codes)) return fail(KAIRO_STATUS_INVALID_VALUE, "codes must have 16-byte aligned rows");
+  if (ntokens > 0 && nadapters > 0 && (!codes || !steps))
+    return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+  return wgrad(low, rank, nullptr, 0, codes, ldq, steps, lds, k, dtype, plan, ntokens, nadapters, grad, grad_dtype,
+               stream);
 }

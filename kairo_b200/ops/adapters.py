@@ -36,7 +36,7 @@ from kairo_b200.ops.backward import (
     sparse_linear_weight_grad,
     transpose_values,
 )
-from kairo_b200.ops.checkpoint import QuantizedActivations, dequantize_activations, quantize_activations
+from kairo_b200.ops.checkpoint import QuantizedActivations, quantize_activations
 from kairo_b200.ops.spmm import KernelConfig, _require_cuda, sparse_linear
 from kairo_b200.ops.token_embedding import _flat_ids, _ld, _rows, _same_device, _scratch
 from kairo_b200.types import BlockSparseMatrix
@@ -140,7 +140,7 @@ def _check_batch(X, features: int, adapters: LowRankAdapters, plan: AdapterPlan,
 
 
 def _apply(X: Tensor, down: Tensor, up: Tensor, scale: Tensor | None, plan: AdapterPlan, base: Tensor | None,
-           out: Tensor | None, low: Tensor, op: str) -> None:
+           out: Tensor | None, low: Tensor | None, op: str) -> None:
     dev = X.device
     n = up.shape[2]
     with torch.cuda.device(dev):
@@ -149,7 +149,8 @@ def _apply(X: Tensor, down: Tensor, up: Tensor, scale: Tensor | None, plan: Adap
             _lib.kairo_dtype(X.dtype), _lib.ptr(scale), plan.memory.data_ptr(), plan.num_tokens, plan.num_adapters,
             _lib.ptr(base), _ld(base) if base is not None else n,
             _lib.kairo_dtype(base.dtype if base is not None else X.dtype), _lib.ptr(out),
-            _ld(out) if out is not None else n, _lib.kairo_dtype(out.dtype if out is not None else X.dtype), low.data_ptr(), _lib.stream_handle(dev)), op)
+            _ld(out) if out is not None else n, _lib.kairo_dtype(out.dtype if out is not None else X.dtype), _lib.ptr(low),
+            _lib.stream_handle(dev)), op)
 
 
 def _result(shape: tuple[int, int], base: Tensor | None, out: Tensor | None, dtype: torch.dtype | None,
@@ -188,19 +189,28 @@ def adapter_linear(X: Tensor, adapters: LowRankAdapters, plan: AdapterPlan, *, b
     _same_device(X, adapters.down, plan.memory, op=op)
     _check_batch(X, adapters.in_features, adapters, plan, "X", op)
     base, out = _result((X.shape[0], adapters.out_features), base, out, out_dtype, adapters, op)
-    low = torch.empty(X.shape[0], adapters.rank, dtype=torch.float32, device=X.device)
+    low = torch.empty(X.shape[0], adapters.rank, dtype=torch.float32, device=X.device) if return_low else None
     _apply(_rows(X), adapters.down, adapters.up, adapters.scale, plan, base, out, low, op)
     return (out, low) if return_low else out
 
 
-def _wgrad(low: Tensor, Z: Tensor, plan: AdapterPlan, dtype: torch.dtype, op: str) -> Tensor:
+def _wgrad(low: Tensor, Z: Tensor | QuantizedActivations, plan: AdapterPlan, dtype: torch.dtype, op: str) -> Tensor:
     dev = Z.device
-    grad = torch.empty(plan.num_adapters, low.shape[1], Z.shape[1], dtype=dtype, device=dev)
+    k = Z.shape[1]
+    grad = torch.empty(plan.num_adapters, low.shape[1], k, dtype=dtype, device=dev)
+    lib = _lib.lib()
     with torch.cuda.device(dev):
-        _lib.check(_lib.lib().kairo_low_rank_wgrad(low.data_ptr(), low.shape[1], Z.data_ptr(), _ld(Z), Z.shape[1],
-                                                   _lib.kairo_dtype(Z.dtype), plan.memory.data_ptr(),
-                                                   plan.num_tokens, plan.num_adapters, grad.data_ptr(),
-                                                   _lib.kairo_dtype(dtype), _lib.stream_handle(dev)), op)
+        if isinstance(Z, QuantizedActivations):
+            _lib.check(lib.kairo_low_rank_wgrad_q8(low.data_ptr(), low.shape[1], Z.codes.data_ptr(), Z._ldq,
+                                                   Z.steps.data_ptr(), Z._lds, k, _lib.kairo_dtype(Z.dtype),
+                                                   plan.memory.data_ptr(), plan.num_tokens, plan.num_adapters,
+                                                   grad.data_ptr(), _lib.kairo_dtype(dtype),
+                                                   _lib.stream_handle(dev)), op)
+        else:
+            _lib.check(lib.kairo_low_rank_wgrad(low.data_ptr(), low.shape[1], Z.data_ptr(), _ld(Z), k,
+                                                _lib.kairo_dtype(Z.dtype), plan.memory.data_ptr(), plan.num_tokens,
+                                                plan.num_adapters, grad.data_ptr(), _lib.kairo_dtype(dtype),
+                                                _lib.stream_handle(dev)), op)
     return grad
 
 
@@ -239,7 +249,7 @@ def adapter_linear_backward(dY: Tensor, X: Tensor | QuantizedActivations, adapte
     _apply(dY, adapters.up, adapters.down, adapters.scale, plan, base_dx if need_dx else None, dX, dlow, op)
     if not need_dw:
         return dX, None, None
-    Z = dequantize_activations(kept) if kept else _rows(X)
+    Z = kept or _rows(X)
     if low is None:
         low = torch.empty_like(dlow)
         _apply(Z, adapters.down, adapters.up, adapters.scale, plan, None, None, low, op)

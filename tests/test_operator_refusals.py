@@ -189,7 +189,7 @@ def test_adapter_c_refusals():
                                         ydt, low, None)
 
     for kw in ({"x": None}, {"ldx": 63}, {"k": 0}, {"down": None}, {"up": None}, {"n": 0}, {"rank": 0}, {"dt": 0},
-               {"plan": None}, {"t": -1}, {"g": -1}, {"ldb": 31}, {"bdt": 1}, {"ldy": 31}, {"ydt": 1}, {"low": None}):
+               {"plan": None}, {"t": -1}, {"g": -1}, {"ldb": 31}, {"bdt": 1}, {"ldy": 31}, {"ydt": 1}, {"y": None, "low": None}):
         assert apply(**kw) == _lib.INVALID_VALUE, kw
     for kw in ({"rank": 129}, {"g": 65536}, {"t": (1 << 24) + 1}, {"k": (1 << 22) + 1, "ldx": 1 << 23}):
         assert apply(**kw) == _lib.NOT_SUPPORTED, kw
@@ -201,5 +201,12 @@ def test_adapter_c_refusals():
     for kw in ({"low": None}, {"rank": 0}, {"z": None}, {"ldz": 63}, {"k": 0}, {"dt": 0}, {"plan": None}, {"t": -1},
                {"g": -1}, {"grad": None}, {"gdt": 1}):
         assert wgrad(**kw) == _lib.INVALID_VALUE, kw
-    assert wgrad(rank=129) == _lib.NOT_SUPPORTED
+    def wgrad8(low=some, rank=8, q=some, ldq=64, steps=some, lds=10, k=64, dt=2, plan=some, t=10, g=3, grad=some, gdt=0):
+        return lib.kairo_low_rank_wgrad_q8(low, rank, q, ldq, steps, lds, k, dt, plan, t, g, grad, gdt, None)
+
+    for kw in ({"low": None}, {"rank": 0}, {"q": None}, {"ldq": 48}, {"ldq": 72}, {"steps": None}, {"lds": 9}, {"k": 0},
+               {"dt": 0}, {"plan": None}, {"t": -1}, {"g": -1}, {"grad": None}, {"gdt": 1},
+               {"q": ctypes.c_void_p(264)}):
+        assert wgrad8(**kw) == _lib.INVALID_VALUE, kw
+    assert wgrad(rank=129) == _lib.NOT_SUPPORTED and wgrad8(rank=129) == _lib.NOT_SUPPORTED
     assert wgrad(g=0) == _lib.SUCCESS
