@@ -303,6 +303,32 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def device_index(op: str, *tensors: torch.Tensor) -> int:
+    """The one CUDA device that all of ``tensors`` are on."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        i = t.get_device()
+        if i < 0:
+            raise RuntimeError(f"kairo_b200.{op} runs on CUDA tensors only (got a {t.device} tensor); "
+                               "this package has no CPU implementation")
+        if i != index:
+            raise ValueError(f"{op}: tensors are on cuda:{index} and cuda:{i}; they must share a device")
+    return index
+
+
+def launch(op: str, fn, index: int, *args) -> None:
+    """``fn(*args, stream)`` on the current stream of device ``index``, its
+    status checked.  The device is switched only when it is not the current
+    one: for calls of a few microseconds the switch would cost as much again."""
+    if torch._C._cuda_getDevice() == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status != SUCCESS:
+        check(status, op)
+
+
 # ------------------------------------------------------------------ workspaces
 
 _ws_lock = threading.Lock()

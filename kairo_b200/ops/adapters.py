@@ -25,6 +25,7 @@ The reference has no counterpart.
 from __future__ import annotations
 
 import ctypes
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -37,8 +38,8 @@ from kairo_b200.ops.backward import (
     transpose_values,
 )
 from kairo_b200.ops.checkpoint import QuantizedActivations, quantize_activations
-from kairo_b200.ops.spmm import KernelConfig, _require_cuda, sparse_linear
-from kairo_b200.ops.token_embedding import _flat_ids, _ld, _rows, _same_device, _scratch
+from kairo_b200.ops.spmm import KernelConfig, sparse_linear
+from kairo_b200.ops.token_embedding import _flat_ids, _ld, _rows
 from kairo_b200.types import BlockSparseMatrix
 
 MAX_RANK = 128
@@ -105,26 +106,29 @@ class AdapterPlan:
     num_adapters: int
 
 
+@functools.lru_cache(maxsize=4096)
+def _plan_bytes(tokens: int, num_adapters: int) -> tuple[int, int]:
+    size, ws = ctypes.c_size_t(0), ctypes.c_size_t(0)
+    _lib.check(_lib.lib().kairo_adapter_plan_size(tokens, num_adapters, ctypes.byref(size), ctypes.byref(ws)),
+               "adapter_plan")
+    return size.value, max(ws.value, 256)
+
+
 def adapter_plan(ids: Tensor, num_adapters: int) -> AdapterPlan:
     """Plan of a batch whose token t uses adapter ``ids[t]`` (int32 or int64,
     any shape, taken flat); an id outside [0, num_adapters), such as -1,
     means none.  Asynchronous, no read-back."""
-    _require_cuda(ids, op="adapter_plan")
+    index = _lib.device_index("adapter_plan", ids)
     g = int(num_adapters)
     if g < 0:
         raise ValueError("num_adapters must be non-negative")
     flat = _flat_ids(ids, "adapter_plan")
-    dev = flat.device
     n = flat.numel()
-    lib = _lib.lib()
-    with torch.cuda.device(dev):
-        size, ws_size = ctypes.c_size_t(0), ctypes.c_size_t(0)
-        _lib.check(lib.kairo_adapter_plan_size(n, g, ctypes.byref(size), ctypes.byref(ws_size)), "adapter_plan")
-        mem = _scratch(size.value, dev)
-        ws = _scratch(ws_size.value, dev)
-        _lib.check(lib.kairo_adapter_plan_build(flat.data_ptr(), flat.element_size(), n, g, mem.data_ptr(),
-                                                mem.numel(), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev)),
-                   "adapter_plan")
+    size, ws_size = _plan_bytes(n, g)
+    mem = flat.new_empty(size, dtype=torch.uint8)
+    ws = flat.new_empty(ws_size, dtype=torch.uint8)
+    _lib.launch("adapter_plan", _lib.lib().kairo_adapter_plan_build, index, flat.data_ptr(), flat.element_size(), n, g,
+                mem.data_ptr(), size, ws.data_ptr(), ws_size)
     return AdapterPlan(memory=mem, num_tokens=n, num_adapters=g)
 
 
@@ -139,37 +143,33 @@ def _check_batch(X, features: int, adapters: LowRankAdapters, plan: AdapterPlan,
         raise ValueError(f"{op}: the plan is of {plan.num_adapters} adapters, not {adapters.count}")
 
 
-def _apply(X: Tensor, down: Tensor, up: Tensor, scale: Tensor | None, plan: AdapterPlan, base: Tensor | None,
-           out: Tensor | None, low: Tensor | None, op: str) -> None:
-    dev = X.device
-    n = up.shape[2]
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().kairo_low_rank_apply(
-            X.data_ptr(), _ld(X), X.shape[1], down.data_ptr(), up.data_ptr(), n, down.shape[1],
-            _lib.kairo_dtype(X.dtype), _lib.ptr(scale), plan.memory.data_ptr(), plan.num_tokens, plan.num_adapters,
-            _lib.ptr(base), _ld(base) if base is not None else n,
-            _lib.kairo_dtype(base.dtype if base is not None else X.dtype), _lib.ptr(out),
-            _ld(out) if out is not None else n, _lib.kairo_dtype(out.dtype if out is not None else X.dtype), _lib.ptr(low),
-            _lib.stream_handle(dev)), op)
+def _apply(op: str, index: int, X: Tensor, down: Tensor, up: Tensor, scale: Tensor | None, plan: AdapterPlan,
+           base: Tensor | None, out: Tensor | None, low: Tensor | None) -> None:
+    k, n, dt = down.shape[2], up.shape[2], _lib.kairo_dtype(X.dtype)
+    _lib.launch(op, _lib.lib().kairo_low_rank_apply, index, X.data_ptr(), _ld(X), k, down.data_ptr(), up.data_ptr(), n,
+                down.shape[1], dt, None if scale is None else scale.data_ptr(), plan.memory.data_ptr(),
+                plan.num_tokens, plan.num_adapters,
+                *((None, n, dt) if base is None else (base.data_ptr(), _ld(base), _lib.kairo_dtype(base.dtype))),
+                *((None, n, dt) if out is None else (out.data_ptr(), _ld(out), _lib.kairo_dtype(out.dtype))),
+                None if low is None else low.data_ptr())
 
 
 def _result(shape: tuple[int, int], base: Tensor | None, out: Tensor | None, dtype: torch.dtype | None,
             adapters: LowRankAdapters, op: str) -> tuple[Tensor | None, Tensor]:
     """The checked base (rows contiguous) and the tensor to write."""
-    dev = adapters.down.device
     odt = dtype or (out.dtype if out is not None else adapters.dtype)
     if odt not in (torch.float32, adapters.dtype):
         raise TypeError(f"{op}: the output must be float32 or {adapters.dtype}, got {odt}")
     if base is not None:
-        if tuple(base.shape) != shape or base.device != dev:
-            raise ValueError(f"{op}: base must be {shape} on {dev}")
+        if base.shape != shape or base.get_device() != adapters.down.get_device():
+            raise ValueError(f"{op}: base must be {shape} on {adapters.down.device}")
         if base.dtype not in (torch.float32, adapters.dtype):
             raise TypeError(f"{op}: base must be float32 or {adapters.dtype}, got {base.dtype}")
         base = _rows(base)
     if out is None:
-        out = torch.empty(shape, dtype=odt, device=dev)
-    elif tuple(out.shape) != shape or out.dtype != odt or out.device != dev or _rows(out) is not out:
-        raise ValueError(f"{op}: out must be a row-major {shape} {odt} tensor on {dev}")
+        out = adapters.down.new_empty(shape, dtype=odt)
+    elif out.shape != shape or out.dtype != odt or out.device != adapters.down.device or _rows(out) is not out:
+        raise ValueError(f"{op}: out must be a row-major {shape} {odt} tensor on {adapters.down.device}")
     return base, out
 
 
@@ -185,32 +185,25 @@ def adapter_linear(X: Tensor, adapters: LowRankAdapters, plan: AdapterPlan, *, b
     (tokens, rank) float32 values ``scale[a] * X[t] down[a]^T`` that
     ``adapter_linear_backward`` takes."""
     op = "adapter_linear"
-    _require_cuda(X, adapters.down, op=op)
-    _same_device(X, adapters.down, plan.memory, op=op)
+    index = _lib.device_index(op, X, adapters.down, plan.memory)
     _check_batch(X, adapters.in_features, adapters, plan, "X", op)
     base, out = _result((X.shape[0], adapters.out_features), base, out, out_dtype, adapters, op)
-    low = torch.empty(X.shape[0], adapters.rank, dtype=torch.float32, device=X.device) if return_low else None
-    _apply(_rows(X), adapters.down, adapters.up, adapters.scale, plan, base, out, low, op)
+    low = X.new_empty((X.shape[0], adapters.rank), dtype=torch.float32) if return_low else None
+    _apply(op, index, _rows(X), adapters.down, adapters.up, adapters.scale, plan, base, out, low)
     return (out, low) if return_low else out
 
 
-def _wgrad(low: Tensor, Z: Tensor | QuantizedActivations, plan: AdapterPlan, dtype: torch.dtype, op: str) -> Tensor:
-    dev = Z.device
-    k = Z.shape[1]
-    grad = torch.empty(plan.num_adapters, low.shape[1], k, dtype=dtype, device=dev)
-    lib = _lib.lib()
-    with torch.cuda.device(dev):
-        if isinstance(Z, QuantizedActivations):
-            _lib.check(lib.kairo_low_rank_wgrad_q8(low.data_ptr(), low.shape[1], Z.codes.data_ptr(), Z._ldq,
-                                                   Z.steps.data_ptr(), Z._lds, k, _lib.kairo_dtype(Z.dtype),
-                                                   plan.memory.data_ptr(), plan.num_tokens, plan.num_adapters,
-                                                   grad.data_ptr(), _lib.kairo_dtype(dtype),
-                                                   _lib.stream_handle(dev)), op)
-        else:
-            _lib.check(lib.kairo_low_rank_wgrad(low.data_ptr(), low.shape[1], Z.data_ptr(), _ld(Z), k,
-                                                _lib.kairo_dtype(Z.dtype), plan.memory.data_ptr(), plan.num_tokens,
-                                                plan.num_adapters, grad.data_ptr(), _lib.kairo_dtype(dtype),
-                                                _lib.stream_handle(dev)), op)
+def _wgrad(op: str, index: int, low: Tensor, Z: Tensor | QuantizedActivations, plan: AdapterPlan,
+           dtype: torch.dtype) -> Tensor:
+    rank, k = low.shape[1], Z.shape[1]
+    grad = low.new_empty((plan.num_adapters, rank, k), dtype=dtype)
+    tail = (k, _lib.kairo_dtype(Z.dtype), plan.memory.data_ptr(), plan.num_tokens, plan.num_adapters,
+            grad.data_ptr(), _lib.kairo_dtype(dtype))
+    if isinstance(Z, QuantizedActivations):
+        _lib.launch(op, _lib.lib().kairo_low_rank_wgrad_q8, index, low.data_ptr(), rank, Z.codes.data_ptr(), Z._ldq,
+                    Z.steps.data_ptr(), Z._lds, *tail)
+    else:
+        _lib.launch(op, _lib.lib().kairo_low_rank_wgrad, index, low.data_ptr(), rank, Z.data_ptr(), _ld(Z), *tail)
     return grad
 
 
@@ -228,8 +221,7 @@ def adapter_linear_backward(dY: Tensor, X: Tensor | QuantizedActivations, adapte
     adapters'), zero for an adapter without tokens."""
     op = "adapter_linear_backward"
     kept = X if isinstance(X, QuantizedActivations) else None
-    _require_cuda(dY, kept.codes if kept else X, adapters.down, op=op)
-    _same_device(dY, kept.codes if kept else X, adapters.down, plan.memory, op=op)
+    index = _lib.device_index(op, dY, kept.codes if kept else X, adapters.down, plan.memory)
     _check_batch(dY, adapters.out_features, adapters, plan, "dY", op)
     gdt = grad_dtype or adapters.dtype
     if gdt not in (torch.float32, adapters.dtype):
@@ -245,16 +237,17 @@ def adapter_linear_backward(dY: Tensor, X: Tensor | QuantizedActivations, adapte
     if need_dx:
         base_dx, dX = _result((dY.shape[0], adapters.in_features), base_dx, None, dx_dtype, adapters, op)
     dY = _rows(dY)
-    dlow = torch.empty(dY.shape[0], adapters.rank, dtype=torch.float32, device=dY.device)
-    _apply(dY, adapters.up, adapters.down, adapters.scale, plan, base_dx if need_dx else None, dX, dlow, op)
+    dlow = dY.new_empty((dY.shape[0], adapters.rank), dtype=torch.float32) if need_dw else None
+    if need_dx or need_dw:
+        _apply(op, index, dY, adapters.up, adapters.down, adapters.scale, plan, base_dx if need_dx else None, dX, dlow)
     if not need_dw:
         return dX, None, None
     Z = kept or _rows(X)
     if low is None:
         low = torch.empty_like(dlow)
-        _apply(Z, adapters.down, adapters.up, adapters.scale, plan, None, None, low, op)
-    d_down = _wgrad(dlow, Z, plan, gdt, op)
-    d_up = _wgrad(low.contiguous(), dY, plan, gdt, op)
+        _apply(op, index, Z, adapters.down, adapters.up, adapters.scale, plan, None, None, low)
+    d_down = _wgrad(op, index, dlow, Z, plan, gdt)
+    d_up = _wgrad(op, index, low.contiguous(), dY, plan, gdt)
     return dX, d_down, d_up
 
 

@@ -22,7 +22,6 @@ import torch
 from torch import Tensor
 
 from kairo_b200 import _lib
-from kairo_b200.ops.spmm import _require_cuda
 
 GROUP = 64  # columns that share a step
 
@@ -43,7 +42,7 @@ class QuantizedActivations:
         if self.codes.dim() != 2 or self.codes.dtype != torch.int8:
             raise ValueError("codes must be a 2-D int8 tensor")
         n, k = self.codes.shape
-        if tuple(self.steps.shape) != ((k + GROUP - 1) // GROUP, n) or self.steps.dtype != torch.float32:
+        if self.steps.shape != ((k + GROUP - 1) // GROUP, n) or self.steps.dtype != torch.float32:
             raise ValueError(f"steps must be a ({(k + GROUP - 1) // GROUP}, {n}) float32 tensor")
         if self.dtype not in (torch.float32, torch.float16, torch.bfloat16):
             raise TypeError(f"unsupported dtype {self.dtype}; expected float32, float16 or bfloat16")
@@ -76,7 +75,7 @@ class QuantizedActivations:
     @property
     def _ldq(self) -> int:
         n, k = self.codes.shape
-        return self.codes.stride(0) if n > 1 else -(-k // 16) * 16
+        return self.codes.stride(0) if n > 1 and k > 0 else -(-k // 16) * 16
 
     @property
     def _lds(self) -> int:
@@ -89,39 +88,32 @@ def quantize_activations(X: Tensor) -> QuantizedActivations:
     A value is off by at most half a step, max|group| / 254.  A group whose
     largest magnitude is under 2^-100 reads back as zeros; one that holds an
     infinity or a NaN reads back as NaN."""
-    _require_cuda(X, op="quantize_activations")
+    index = _lib.device_index("quantize_activations", X)
     if X.dim() != 2:
         raise ValueError("X must be 2-D (n, k)")
     dt = _lib.kairo_dtype(X.dtype)
     if X.stride(1) != 1 or (X.shape[0] > 1 and X.stride(0) < X.shape[1]):
         X = X.contiguous()
     n, k = X.shape
-    dev = X.device
     ldq = -(-k // 16) * 16
-    codes = torch.empty(n, ldq, dtype=torch.int8, device=dev)[:, :k]
-    steps = torch.empty(-(-k // GROUP), n, dtype=torch.float32, device=dev)
-    if n and k:
-        with torch.cuda.device(dev):
-            _lib.check(_lib.lib().kairo_quantize_q8(X.data_ptr(), n, k, max(X.stride(0), k), dt, codes.data_ptr(),
-                                                    ldq, steps.data_ptr(), n, _lib.stream_handle(dev)),
-                       "quantize_activations")
+    codes = X.new_empty((n, ldq), dtype=torch.int8)
+    if ldq != k:
+        codes = codes[:, :k]
+    steps = X.new_empty((-(-k // GROUP), n), dtype=torch.float32)
+    _lib.launch("quantize_activations", _lib.lib().kairo_quantize_q8, index, X.data_ptr(), n, k, max(X.stride(0), k),
+                dt, codes.data_ptr(), ldq, steps.data_ptr(), n)
     return QuantizedActivations(codes=codes, steps=steps, dtype=X.dtype)
 
 
 def dequantize_activations(q: QuantizedActivations, *, out: Tensor | None = None) -> Tensor:
     """``code * step`` in the activation's type, (n, k)."""
-    _require_cuda(q.codes, op="dequantize_activations")
+    index = _lib.device_index("dequantize_activations", q.codes)
     n, k = q.shape
-    dev = q.device
     if out is None:
-        out = torch.empty(n, k, dtype=q.dtype, device=dev)
-    elif tuple(out.shape) != (n, k) or out.dtype != q.dtype or out.device != dev or (k > 1 and out.stride(1) != 1) or (
-            n > 1 and out.stride(0) < k):
-        raise ValueError(f"out must be a row-major ({n}, {k}) {q.dtype} tensor on {dev}")
-    if n and k:
-        with torch.cuda.device(dev):
-            _lib.check(_lib.lib().kairo_dequantize_q8(q.codes.data_ptr(), q._ldq, q.steps.data_ptr(), q._lds, n, k,
-                                                      out.data_ptr(), max(out.stride(0), k),
-                                                      _lib.kairo_dtype(q.dtype), _lib.stream_handle(dev)),
-                       "dequantize_activations")
+        out = q.codes.new_empty((n, k), dtype=q.dtype)
+    elif tuple(out.shape) != (n, k) or out.dtype != q.dtype or out.device != q.device or (
+            k > 1 and out.stride(1) != 1) or (n > 1 and out.stride(0) < k):
+        raise ValueError(f"out must be a row-major ({n}, {k}) {q.dtype} tensor on {q.device}")
+    _lib.launch("dequantize_activations", _lib.lib().kairo_dequantize_q8, index, q.codes.data_ptr(), q._ldq,
+                q.steps.data_ptr(), q._lds, n, k, out.data_ptr(), max(out.stride(0), k), _lib.kairo_dtype(q.dtype))
     return out

@@ -19,35 +19,27 @@ nothing to the gradient.  A negative id therefore serves as padding.
 from __future__ import annotations
 
 import ctypes
+import functools
 from dataclasses import dataclass
 
 import torch
 from torch import Tensor
 
 from kairo_b200 import _lib
-from kairo_b200.ops.spmm import _require_cuda
-
-
-def _same_device(*tensors: Tensor, op: str) -> torch.device:
-    dev = tensors[0].device
-    for t in tensors[1:]:
-        if t.device != dev:
-            raise ValueError(f"{op}: tensors are on {dev} and {t.device}; they must share a device")
-    return dev
-
-
-def _scratch(nbytes: int, device: torch.device) -> Tensor:
-    return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
 
 
 def _flat_ids(ids: Tensor, op: str) -> Tensor:
     if ids.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{op}: ids must be int32 or int64, got {ids.dtype}")
+    if ids.dim() == 1 and ids.is_contiguous():
+        return ids
     return ids.reshape(-1).contiguous()
 
 
 def _rows(t: Tensor) -> Tensor:
     """``t`` (2-D) itself when its rows are contiguous and do not overlap."""
+    if t.is_contiguous():
+        return t
     n, d = t.shape
     return t if (d <= 1 or t.stride(1) == 1) and (n <= 1 or t.stride(0) >= d) else t.contiguous()
 
@@ -69,26 +61,33 @@ class TokenOrder:
     num_embeddings: int
 
 
+@functools.lru_cache(maxsize=4096)
+def _sort_bytes(tokens: int, n_rows: int) -> int:
+    nbytes = ctypes.c_size_t(0)
+    _lib.check(_lib.lib().kairo_token_sort_workspace_size(tokens, n_rows, ctypes.byref(nbytes)), "sort_tokens")
+    return max(nbytes.value, 256)
+
+
+@functools.lru_cache(maxsize=4096)
+def _grad_bytes(tokens: int, dim: int) -> int:
+    nbytes = ctypes.c_size_t(0)
+    _lib.check(_lib.lib().kairo_embedding_grad_workspace_size(tokens, dim, ctypes.byref(nbytes)), "embedding_grad")
+    return max(nbytes.value, 256)
+
+
 def sort_tokens(ids: Tensor, num_embeddings: int) -> TokenOrder:
     """Stable order of the tokens ``ids`` (any shape, int32 or int64) by id, on the device."""
-    _require_cuda(ids, op="sort_tokens")
+    index = _lib.device_index("sort_tokens", ids)
     n_rows = int(num_embeddings)
     if n_rows < 0:
         raise ValueError("num_embeddings must be non-negative")
     flat = _flat_ids(ids, "sort_tokens")
-    dev = flat.device
     n = flat.numel()
-    lib = _lib.lib()
-    out = torch.empty(n, dtype=torch.int32, device=dev)
-    perm = torch.empty(n, dtype=torch.int32, device=dev)
-    with torch.cuda.device(dev):
-        nbytes = ctypes.c_size_t(0)
-        _lib.check(lib.kairo_token_sort_workspace_size(n, n_rows, ctypes.byref(nbytes)), "sort_tokens")
-        if n:
-            ws = _scratch(nbytes.value, dev)
-            _lib.check(lib.kairo_token_sort(flat.data_ptr(), flat.element_size(), n, n_rows, out.data_ptr(),
-                                            perm.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev)),
-                       "sort_tokens")
+    out = flat.new_empty(n, dtype=torch.int32)
+    perm = flat.new_empty(n, dtype=torch.int32)
+    ws = flat.new_empty(_sort_bytes(n, n_rows), dtype=torch.uint8)
+    _lib.launch("sort_tokens", _lib.lib().kairo_token_sort, index, flat.data_ptr(), flat.element_size(), n, n_rows,
+                out.data_ptr(), perm.data_ptr(), ws.data_ptr(), ws.numel())
     return TokenOrder(sorted_ids=out, perm=perm, num_embeddings=n_rows)
 
 
@@ -99,8 +98,7 @@ def embedding_lookup(weight: Tensor, ids: Tensor, *, scale: float = 1.0, out_dty
     weight: (N, D) float32, float16 or bfloat16; ids: int32 or int64, any
     shape; an id outside [0, N) gives a zero row.  ``out``: a contiguous
     tensor to write to."""
-    _require_cuda(weight, ids, op="embedding_lookup")
-    dev = _same_device(weight, ids, op="embedding_lookup")
+    index = _lib.device_index("embedding_lookup", weight, ids)
     if weight.dim() != 2 or weight.shape[1] < 1:
         raise ValueError("weight must be 2-D (N, D) with D >= 1")
     n, d = weight.shape
@@ -108,18 +106,16 @@ def embedding_lookup(weight: Tensor, ids: Tensor, *, scale: float = 1.0, out_dty
     in_dt = _lib.kairo_dtype(weight.dtype)
     odt = out_dtype or (out.dtype if out is not None else weight.dtype)
     out_dt = _lib.kairo_dtype(odt)
-    shape = tuple(ids.shape) + (d,)
+    shape = (*ids.shape, d)
     if out is None:
-        out = torch.empty(shape, dtype=odt, device=dev)
+        out = weight.new_empty(shape, dtype=odt)
     elif tuple(out.shape) != shape or out.dtype != odt or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {shape} {odt} tensor")
-    elif out.device != dev:
+    elif out.device != weight.device:
         raise ValueError("out must be on the weight's device")
     w = _rows(weight)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().kairo_embedding_lookup(w.data_ptr(), n, d, _ld(w), in_dt, flat.data_ptr(),
-                                                     flat.element_size(), flat.numel(), float(scale), out.data_ptr(),
-                                                     out_dt, _lib.stream_handle(dev)), "embedding_lookup")
+    _lib.launch("embedding_lookup", _lib.lib().kairo_embedding_lookup, index, w.data_ptr(), n, d, _ld(w), in_dt,
+                flat.data_ptr(), flat.element_size(), flat.numel(), float(scale), out.data_ptr(), out_dt)
     return out
 
 
@@ -142,8 +138,8 @@ def embedding_grad(grad_output: Tensor, ids: Tensor | TokenOrder, num_embeddings
         tokens, where = ids.perm.numel(), ids.perm
     else:
         tokens, where = ids.numel(), ids
-    _require_cuda(grad_output, where, op="embedding_grad")
-    dev = _same_device(grad_output, where, op="embedding_grad")
+    index = _lib.device_index("embedding_grad", grad_output, where)
+    dev = grad_output.device
     if n_rows < 0:
         raise ValueError("num_embeddings must be non-negative")
     if grad_output.dim() < 1 or grad_output.shape[-1] < 1:
@@ -159,19 +155,14 @@ def embedding_grad(grad_output: Tensor, ids: Tensor | TokenOrder, num_embeddings
     if accumulate and out is None:
         raise ValueError("accumulate=True needs out")
     if out is None:
-        out = torch.empty(n_rows, d, dtype=odt, device=dev)
+        out = g.new_empty((n_rows, d), dtype=odt)
     elif tuple(out.shape) != (n_rows, d) or out.dtype != odt or out.device != dev or _rows(out) is not out:
         raise ValueError(f"out must be a row-major ({n_rows}, {d}) {odt} tensor on {dev}")
     order = ids if isinstance(ids, TokenOrder) else sort_tokens(ids, n_rows)
-    lib = _lib.lib()
-    with torch.cuda.device(dev):
-        nbytes = ctypes.c_size_t(0)
-        _lib.check(lib.kairo_embedding_grad_workspace_size(tokens, d, ctypes.byref(nbytes)), "embedding_grad")
-        ws = _scratch(nbytes.value, dev)
-        _lib.check(lib.kairo_embedding_grad(g.data_ptr(), _ld(g), in_dt, order.sorted_ids.data_ptr(),
-                                            order.perm.data_ptr(), tokens, n_rows, d, float(scale), out.data_ptr(),
-                                            _ld(out), out_dt, 1 if accumulate else 0, ws.data_ptr(), ws.numel(),
-                                            _lib.stream_handle(dev)), "embedding_grad")
+    ws = g.new_empty(_grad_bytes(tokens, d), dtype=torch.uint8)
+    _lib.launch("embedding_grad", _lib.lib().kairo_embedding_grad, index, g.data_ptr(), _ld(g), in_dt,
+                order.sorted_ids.data_ptr(), order.perm.data_ptr(), tokens, n_rows, d, float(scale), out.data_ptr(),
+                _ld(out), out_dt, 1 if accumulate else 0, ws.data_ptr(), ws.numel())
     return out
 
 
