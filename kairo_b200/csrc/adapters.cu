@@ -159,7 +159,36 @@ bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 // because every tile reads its adapter's weights from L2 once.
 int pick_tile(int64_t t, int64_t rank, bool vec) {
   if (!vec || t <= 2048 || rank > 64) return 16;
-  return rank <= 32 ? 64 : 32;
+  return rank <= 16 ? 64 : 32;
+}
+
+// CTAs per tile, a power of two up to 8.  As many as the GPU holds at once (two
+// CTAs per SM) gives the shortest calls: 96 tokens in 71 tiles of 8192
+// features took 20.2, 12.8, 12.3 and 15.7 us with clusters of 1, 2, 4 and 8;
+// 8192 tokens in 260 tiles 96, 103, 101 and 124 us. But no more than leave
+// every warp a turn of 64 features (777 tokens, 1000 features: 6.1 us with
+// two, 12.3 with eight), and where the contraction is so long that a warp has
+// 32 turns, more, shorter CTAs even out the SMs (8192 tokens, 32768 features:
+// 142 us with two, 139 with four).
+int pick_cluster(int64_t tiles, int64_t k, int64_t n) {
+  const int64_t room = 2 * device_sm_count(current_device());
+  int c = 1;
+  while (c < kCluster && (tiles * 2 * c <= room || k >= int64_t(32) * 8 * 64 * c) &&
+         int64_t(2) * c * 8 * 64 <= std::max(k, n) + 511)
+    c *= 2;
+  return c;
+}
+
+// CTAs that share out an adapter's tokens: again as many as fill the GPU once
+// (8192 tokens of 4 adapters, rank 16, 8192 features: 31.9, 29.2 and 36.9 us
+// with 2, 4 and 8), and no more than there are chunks of 64 tokens.
+int pick_wgrad_cluster(int64_t ntokens, int64_t nadapters, int64_t k, int64_t rank) {
+  const int64_t groups = rank <= 16 ? 1 : (rank <= 32 ? 2 : (rank <= 64 ? 4 : 8));  // of 16 rank rows
+  const int64_t ctas = ceil_div64(k, 512 / groups) * nadapters;
+  const int64_t room = 2 * device_sm_count(current_device());
+  int c = 1;
+  while (c < kCluster && ctas * 2 * c <= room && c * kChunkTokens < ntokens) c *= 2;
+  return c;
 }
 
 }  // namespace
@@ -248,11 +277,12 @@ extern "C" kairo_status kairo_low_rank_apply(const void* x, int64_t ldx, int64_t
   a.rank = static_cast<int32_t>(rank);
   a.base_f32 = base && base_dtype == KAIRO_DTYPE_F32;
   const int64_t clusters = max_tiles(ntokens, nadapters, tile);
+  const int cluster = pick_cluster(clusters, k, n);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool yf = y && y_dtype == KAIRO_DTYPE_F32;
   const cudaError_t err = dtype == KAIRO_DTYPE_F16
-                              ? launch_low_rank_apply<__half>(a, yf, vec, tile, clusters, kCluster, s)
-                              : launch_low_rank_apply<__nv_bfloat16>(a, yf, vec, tile, clusters, kCluster, s);
+                              ? launch_low_rank_apply<__half>(a, yf, vec, tile, clusters, cluster, s)
+                              : launch_low_rank_apply<__nv_bfloat16>(a, yf, vec, tile, clusters, cluster, s);
   if (err != cudaSuccess) return cuda_fail(err, "launch of the low-rank product");
   return KAIRO_STATUS_SUCCESS;
 }
@@ -285,10 +315,7 @@ kairo_status wgrad(const float* low, int64_t rank, const void* z, int64_t ldz, c
   a.k = static_cast<int32_t>(k);
   a.rank = static_cast<int32_t>(rank);
   const bool vec = codes || (k % 8 == 0 && ldz % 8 == 0 && aligned16(z));
-  // One CTA takes 64 tokens at a time: no more CTAs per adapter than an
-  // evenly filled one has such chunks.
-  int cluster = 1;
-  while (cluster < kCluster && cluster * kChunkTokens < ntokens) cluster *= 2;
+  const int cluster = pick_wgrad_cluster(ntokens, nadapters, k, rank);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool gf = grad_dtype == KAIRO_DTYPE_F32;
   const cudaError_t err = dtype == KAIRO_DTYPE_F16

@@ -14,10 +14,14 @@
 //    the contraction places 2t, 2t+1, 2t+8, 2t+9 of two products, for tokens
 //    and rank rows alike;
 //  - features as columns (low up, and the weight gradients): lane (g, t)
-//    takes features 8 g .. 8 g + 7 of the rank rows (tokens) 2t, 2t+1, 2t+8,
-//    2t+9 as column g of eight products, and so holds of the result 16
-//    contiguous features 16 t .. 16 t + 15 of its rows.
-// Every access is a whole 16-byte vector of a fully used sector.
+//    takes 8 contiguous features of the rank rows (tokens) 2t, 2t+1, 2t+8,
+//    2t+9 as column g of eight products, and so holds of the result the 8
+//    features of column 2t and those of column 2t+1, for its rows.
+// Every access is a 16-byte vector, and the features of the columns are dealt
+// out so that the four lanes t of one access stand side by side: 64 bytes of a
+// row, whole sectors. (With columns 2t and 2t+1 side by side instead, each access touched
+// half sectors, and the rank-16 expansion of 8192 x 8192 took 91 us where it
+// now takes 56.)
 //
 // low is an fp32 value.  For a product with 16-bit weights it is split into
 // terms of the weights' type, each the rounding of what the ones before leave:
@@ -30,6 +34,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "convert.cuh"
@@ -63,7 +68,7 @@ struct LowRankApplyArgs {
 
 struct LowRankWgradArgs {
   const float* s;      // (tokens, rank)
-  const void* z;       // (tokens, k), or null when given in 8 bits
+  const void* z;       // (tokens, k), or null when given in 8 bits:
   const int8_t* codes;
   const float* steps;
   void* grad;          // (adapters, rank, k)
@@ -109,10 +114,42 @@ __device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-__device__ __forceinline__ float peer_load(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
+constexpr int kMaxCluster = 8;
+
+// The sum over the cluster, in rank order, of the value (or four) at the same
+// shared address of every CTA.  The loads are issued together: one after the
+// other, a peer's latency (some 700 cycles) would be paid for each.
+__device__ __forceinline__ float peer_sum(uint32_t addr, uint32_t csize) {
+  float v[kMaxCluster];
+#pragma unroll
+  for (uint32_t c = 0; c < kMaxCluster; ++c) {
+    v[c] = 0.f;
+    if (c < csize) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[c]) : "r"(peer_addr(addr, c)));
+  }
+  float s = v[0];
+#pragma unroll
+  for (uint32_t c = 1; c < kMaxCluster; ++c) s += v[c];
+  return s;
+}
+__device__ __forceinline__ float4 peer_sum4(uint32_t addr, uint32_t csize) {
+  float4 v[kMaxCluster];
+#pragma unroll
+  for (uint32_t c = 0; c < kMaxCluster; ++c) {
+    v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (c < csize)
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(v[c].x), "=f"(v[c].y), "=f"(v[c].z), "=f"(v[c].w)
+                   : "r"(peer_addr(addr, c)));
+  }
+  float4 s = v[0];
+#pragma unroll
+  for (uint32_t c = 1; c < kMaxCluster; ++c) {
+    s.x += v[c].x;
+    s.y += v[c].y;
+    s.z += v[c].z;
+    s.w += v[c].w;
+  }
+  return s;
 }
 __device__ __forceinline__ void peer_store(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
@@ -194,26 +231,121 @@ __device__ __forceinline__ void power_scale(float m, float* down, float* up) {
 
 // ---------------------------------------------------------------- apply
 
-template <int MT, int NT>
-struct ApplySmem {
+// A lane's own shared memory as an extension of its registers: asynchronous
+// copies land where the same lane reads them, so that many loads are in flight
+// without registers to hold them and without any barrier.  Vector i of a slot
+// stands at [i][lane].
+template <typename T, bool VEC>
+__device__ __forceinline__ void fetch(uint32_t dst, const T* p, int left) {
+  if constexpr (VEC) {
+    // no byte is read where left <= 0; 16 zero bytes are written
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(p), "r"(left > 0 ? 16 : 0) : "memory");
+  } else {
+    constexpr int N = 16 / static_cast<int>(sizeof(T));
+    uint4 v;
+    if constexpr (N == 8) {
+      v = load8<T, false>(p, left);
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = i < left ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
+      v = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                 : "memory");
+  }
+}
+// Place in a 512-byte vector slot of the 16 bytes that are chunk `c` of the 128
+// bytes of row `t`: a row is written as one (in lane order, a copy of four rows
+// took 16 passes over the banks instead of 4, and the weight gradient 46 us
+// where it now takes 29), and whole sectors of the rows change places so that
+// lanes that read together meet different banks.
+__device__ __forceinline__ uint32_t by_rows(int c, int t) {
+  return static_cast<uint32_t>(t * 8 + (c ^ (2 * t))) * 16u;
+}
+// The same for the 8 codes that are chunk `c` of the 64 codes of row `t`.
+__device__ __forceinline__ uint32_t codes_by_rows(int c, int t) {
+  return static_cast<uint32_t>(t * 8 + (c ^ (4 * (t >> 1)))) * 8u;
+}
+__device__ __forceinline__ uint4 landed(uint32_t src) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(src)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 landed_codes(uint32_t src) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(src) : "memory");
+  return v;
+}
+
+// Eight codes times their step, rounded to T.  A code with its sign bit flipped
+// is the low byte of the float 2^23 + 128 + code: one byte permutation and
+// one exact subtraction each, where a conversion instruction runs at a
+// quarter of their rate.
+template <typename T>
+__device__ __forceinline__ uint4 read_back(uint2 q, float step) {
+  const uint32_t b[2] = {q.x ^ 0x80808080u, q.y ^ 0x80808080u};
+  uint32_t w[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float f[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t m = __byte_perm(b[e >> 1], 0x4b000000u, 0x7650u + (e & 1) * 2 + h);
+      f[h] = __fmul_rn(__uint_as_float(m) - 8388736.f, step);
+    }
+    w[e] = static_cast<uint32_t>(bits16<T>(f[0])) | (static_cast<uint32_t>(bits16<T>(f[1])) << 16);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_all_but() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Tile shape and memory of one instance.  MT x 16 tokens, NT x 8 rank rows;
+// STAGES steps of 32 features in flight in the contraction.
+template <int MT_, int NT_, int STAGES_>
+struct ApplyShape {
+  static constexpr int MT = MT_, NT = NT_, STAGES = STAGES_;
   static constexpr int ROWS = 16 * MT;
   static constexpr int RP = 8 * NT;          // rank, padded
   static constexpr int PITCH = RP + 8;       // 16-bit terms: rows 16 bytes apart in banks
   static constexpr int LOW = ROWS * RP;      // floats of one low tile
+  static constexpr int KT = NT / 2;          // rank steps of 16
+  static constexpr int STEP = 2 * MT + NT;   // vectors of one contraction step
+  // Vectors per lane: the contraction's steps, or one turn of the expansion
+  // (4 for each rank step of up; 4 for the base rows of 16 tokens, 8 in fp32).
+  static constexpr int ring(bool base_f32) {
+    const int e = 4 * KT + (base_f32 ? 8 : 4) * MT;
+    return STAGES * STEP > e ? STAGES * STEP : e;
+  }
+  static constexpr size_t ring_bytes(bool base_f32) { return static_cast<size_t>(kWarps) * ring(base_f32) * 512; }
+  static constexpr size_t bytes(int terms, bool base_f32) {
+    return ring_bytes(base_f32) + static_cast<size_t>(kWarps / 2 * LOW + LOW + ROWS) * 4 + static_cast<size_t>(terms) * ROWS * PITCH * 2;
+  }
 };
 
 // One cluster per tile.  Its CTAs and warps share out the features of the
 // contraction, 64 at a time; partial low tiles meet in shared memory, then over
 // the cluster's distributed shared memory; each CTA gets the whole low tile
 // and its warps share out the output features, 64 at a time.  One launch, low
-// never travels through global memory.
-template <typename T, typename TY, int MT, int NT, int TERMS, bool VEC>
-__global__ void __launch_bounds__(kThreadsPerCta, NT > 8 ? 1 : 2) k_apply(const LowRankApplyArgs a) {
-  using S = ApplySmem<MT, NT>;
+// never travels through global memory.  The loads of the expansion (up and
+// base) are started before the tile is summed, so that the barriers cost no
+// memory time; afterwards each load of the next turn starts as soon as its slot
+// has been read.
+template <typename T, typename TY, typename S, int TERMS, bool BASE_F32, bool VEC, int MINB>
+__global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApplyArgs a) {
+  constexpr int MT = S::MT, NT = S::NT, KT = S::KT;
+  constexpr int RING = S::ring(BASE_F32);
   extern __shared__ __align__(16) uint8_t smem[];
-  float* red = reinterpret_cast<float*>(smem);                   // [kWarps][LOW], reused below
-  float* part = red + kWarps * S::LOW;                           // [LOW]: this CTA's partial tile
-  float* low = part + S::LOW;                                    // [LOW]: the whole tile
+  float* red = reinterpret_cast<float*>(smem + S::ring_bytes(BASE_F32));  // [kWarps / 2][LOW]
+  float* part = red;                                             // [LOW]: this CTA's partial tile
+  float* low = red + kWarps / 2 * S::LOW;                        // [LOW]: the whole tile
   float* row_up = low + S::LOW;                                  // [ROWS]: power of two of every row (fp16)
   uint16_t* terms = reinterpret_cast<uint16_t*>(row_up + S::ROWS);  // [TERMS][ROWS][PITCH]
 
@@ -224,8 +356,13 @@ __global__ void __launch_bounds__(kThreadsPerCta, NT > 8 ? 1 : 2) k_apply(const 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int slot = static_cast<int>(crank) * kWarps + warp;      // this warp among the cluster's
-  const int slots = static_cast<int>(csize) * kWarps;
+  const int stride = static_cast<int>(csize) * kWarps * 64;      // features between a warp's turns
   const int count = min(tile.count, S::ROWS);
+  const uint32_t ring0 = smem_addr(smem) + static_cast<uint32_t>(warp * RING * 512);
+  const uint32_t ring = ring0 + static_cast<uint32_t>(lane * 16);  // rows by g: the lanes t side by side
+  const int up_chunk = 4 * (g & 1) + (g >> 1);  // the 8 features of a turn of 64 that are this lane's columns
+  const uint32_t up_ring = ring0 + by_rows(up_chunk, t);
+  const bool live = tile.adapter >= 0;
   int tok[MT][2];  // tokens of this lane's rows, -1: none
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -235,62 +372,159 @@ __global__ void __launch_bounds__(kThreadsPerCta, NT > 8 ? 1 : 2) k_apply(const 
       tok[m][h] = row < count ? a.order[tile.begin + row] : -1;
     }
 
-  if (tile.adapter >= 0) {
-    const T* down = static_cast<const T*>(a.down) + static_cast<int64_t>(tile.adapter) * a.rank * a.k;
-    float acc[MT][NT][4];
+  float acc[MT][NT][4];
+  if (live) {
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
+    // Steps of 32 features, two to a turn of 64.
+    const int turns = slot * 64 < a.k ? (a.k - slot * 64 + stride - 1) / stride : 0;
+    const int steps = 2 * turns;
+    int kk = slot * 64 + 8 * t;  // this lane's features of the next step to start
+    const T* wrow = static_cast<const T*>(a.down) + (static_cast<int64_t>(tile.adapter) * a.rank + g) * a.k;
+    const int64_t wstep = static_cast<int64_t>(8) * a.k;
     const T* xrow[MT][2];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         xrow[m][h] = static_cast<const T*>(a.x) + static_cast<int64_t>(max(tok[m][h], 0)) * a.ldx;
-    for (int k0 = slot * 64; k0 < a.k; k0 += slots * 64) {
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int kk = k0 + half * 32 + 8 * t;
+    auto issue = [&](int i, int at) {
+      if (i < steps) {
         const int left = a.k - kk;
-        uint4 xa[MT][2], wb[NT];
+        const int off = left > 0 ? kk : 0;
+        const uint32_t dst = ring + static_cast<uint32_t>(at * S::STEP * 512);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          const int r = j * 8 + g;
-          wb[j] = load8<T, VEC>(down + static_cast<int64_t>(r) * a.k + kk, r < a.rank ? left : 0);
+          const bool there = j * 8 + g < a.rank;
+          fetch<T, VEC>(dst + j * 512, wrow + (there ? j * wstep + off : off - g * static_cast<int64_t>(a.k)),
+                        there ? left : 0);
         }
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) xa[m][h] = load8<T, VEC>(xrow[m][h] + kk, tok[m][h] >= 0 ? left : 0);
+          for (int h = 0; h < 2; ++h)
+            fetch<T, VEC>(dst + (NT + 2 * m + h) * 512, xrow[m][h] + off, tok[m][h] >= 0 ? left : 0);
+        kk += (i & 1) ? stride - 32 : 32;
+      }
+      commit();
+    };
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          const uint32_t a0[4] = {xa[m][0].x, xa[m][1].x, xa[m][0].y, xa[m][1].y};
-          const uint32_t a1[4] = {xa[m][0].z, xa[m][1].z, xa[m][0].w, xa[m][1].w};
+    for (int i = 0; i < S::STAGES; ++i) issue(i, i);
+    int at = 0;
+    for (int i = 0; i < steps; ++i) {
+      wait_all_but<S::STAGES - 1>();
+      const uint32_t src = ring + static_cast<uint32_t>(at * S::STEP * 512);
+      uint4 wb[NT];
 #pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            mma<T>(acc[m][j], a0, wb[j].x, wb[j].y);
-            mma<T>(acc[m][j], a1, wb[j].z, wb[j].w);
-          }
+      for (int j = 0; j < NT; ++j) wb[j] = landed(src + j * 512);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const uint4 x0 = landed(src + (NT + 2 * m) * 512), x1 = landed(src + (NT + 2 * m + 1) * 512);
+        const uint32_t a0[4] = {x0.x, x1.x, x0.y, x1.y};
+        const uint32_t a1[4] = {x0.z, x1.z, x0.w, x1.w};
+#pragma unroll
+        for (int j = 0; j < NT; ++j) mma<T>(acc[m][j], a0, wb[j].x, wb[j].y);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) mma<T>(acc[m][j], a1, wb[j].z, wb[j].w);
+      }
+      issue(i + S::STAGES, at);  // every vector of the slot is in use above
+      at = at + 1 == S::STAGES ? 0 : at + 1;
+    }
+  }
+
+  // Loads of a turn of the expansion, in the order of their use: one unit of up
+  // for each rank step, one of base for each 16 tokens (two in fp32).  Unit u
+  // has the slot of its own; a turn that does not exist, a tile without an
+  // adapter and a missing base fill theirs with zeros and read nothing.
+  constexpr int BU = BASE_F32 ? 2 : 1;
+  constexpr int UNITS = KT + BU * MT;
+  const T* up = static_cast<const T*>(a.up) + static_cast<int64_t>(max(tile.adapter, 0)) * a.rank * a.n;
+  auto issue_up = [&](int n0, int kt) {
+    const int c = n0 + 8 * up_chunk, left = live && c < a.n ? a.n - c : 0;
+    const uint32_t dst = up_ring + static_cast<uint32_t>(kt * 4 * 512);
+    const T* col = live ? up + (left > 0 ? c : 0) : static_cast<const T*>(a.x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = kt * 16 + 2 * t + (i & 1) + (i >> 1) * 8;
+      const bool there = live && r < a.rank;
+      fetch<T, VEC>(dst + i * 512, col + (there ? r * static_cast<int64_t>(a.n) : 0), there ? left : 0);
+    }
+    commit();
+  };
+  auto issue_base = [&](int n0, int m, int b) {  // m and b are known when compiled
+    const uint32_t dst = ring + static_cast<uint32_t>((KT + BU * m + b) * 4 * 512);
+    if constexpr (BASE_F32) {
+      const int tk = a.base ? tok[m][b] : -1;
+      const float* row = tk >= 0 ? static_cast<const float*>(a.base) + static_cast<int64_t>(tk) * a.ldb
+                                 : reinterpret_cast<const float*>(a.x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = n0 + 32 * (i >> 1) + 8 * t + 4 * (i & 1);
+        const int left = tk >= 0 ? a.n - c : 0;
+        fetch<float, VEC>(dst + i * 512, row + (left > 0 ? c : 0), left);
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int tk = a.base ? tok[m][h] : -1;
+        const T* row = tk >= 0 ? static_cast<const T*>(a.base) + static_cast<int64_t>(tk) * a.ldb
+                               : static_cast<const T*>(a.x);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int c = n0 + 32 * q + 8 * t;
+          const int left = tk >= 0 ? a.n - c : 0;
+          fetch<T, VEC>(dst + (2 * h + q) * 512, row + (left > 0 ? c : 0), left);
         }
       }
     }
+    commit();
+  };
+  if (a.y) {
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) issue_up(slot * 64, kt);
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        float* at = red + warp * S::LOW + (m * 16 + g) * S::RP + j * 8 + 2 * t;
-        *reinterpret_cast<float2*>(at) = make_float2(acc[m][j][0], acc[m][j][1]);
-        *reinterpret_cast<float2*>(at + 8 * S::RP) = make_float2(acc[m][j][2], acc[m][j][3]);
-      }
-    __syncthreads();
-    for (int i = threadIdx.x; i < S::LOW; i += kThreadsPerCta) {
-      float v = 0.f;
+      for (int b = 0; b < BU; ++b) issue_base(slot * 64, m, b);
+  }
+
+  if (live) {
+    // Sum over the CTA's warps as a tree: the upper half hands over to the lower.
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) v += red[w * S::LOW + i];
-      part[i] = v;
+    for (int half = kWarps / 2; half >= 1; half /= 2) {
+      if (warp >= half && warp < 2 * half) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              red[(warp - half) * S::LOW + ((m * NT + j) * 4 + i) * 32 + lane] = acc[m][j][i];
+      }
+      __syncthreads();
+      if (warp < half) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[m][j][i] += red[warp * S::LOW + ((m * NT + j) * 4 + i) * 32 + lane];
+      }
+      __syncthreads();
+    }
+    if (warp == 0) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          float* to = part + (m * 16 + g) * S::RP + j * 8 + 2 * t;
+          *reinterpret_cast<float2*>(to) = make_float2(acc[m][j][0], acc[m][j][1]);
+          *reinterpret_cast<float2*>(to + 8 * S::RP) = make_float2(acc[m][j][2], acc[m][j][3]);
+        }
     }
     cluster_sync();
     // Each CTA sums its share of the tile over the cluster, in rank order, and
@@ -300,9 +534,7 @@ __global__ void __launch_bounds__(kThreadsPerCta, NT > 8 ? 1 : 2) k_apply(const 
     const int share = (S::LOW + static_cast<int>(csize) - 1) / static_cast<int>(csize);
     const int i0 = static_cast<int>(crank) * share, i1 = min(S::LOW, i0 + share);
     for (int i = i0 + threadIdx.x; i < i1; i += kThreadsPerCta) {
-      float v = 0.f;
-      for (uint32_t c = 0; c < csize; ++c) v += peer_load(peer_addr(part_addr + 4u * i, c));
-      v *= scale;
+      const float v = peer_sum(part_addr + 4u * i, csize) * scale;
       for (uint32_t c = 0; c < csize; ++c) peer_store(peer_addr(low_addr + 4u * i, c), v);
       const int row = i / S::RP, r = i - row * S::RP;
       if (a.low && row < count && r < a.rank)
@@ -317,17 +549,16 @@ __global__ void __launch_bounds__(kThreadsPerCta, NT > 8 ? 1 : 2) k_apply(const 
   }
   if (!a.y) return;
 
-  const bool live = tile.adapter >= 0;
   if (live) {
     if constexpr (std::is_same_v<T, __half>) {
       for (int row = warp; row < S::ROWS; row += kWarps) {
         uint32_t m = 0;
         for (int r = lane; r < S::RP; r += 32) m = max(m, __float_as_uint(low[row * S::RP + r]) & 0x7fffffffu);
         m = __reduce_max_sync(0xffffffffu, m);
-        float dn, up;
-        power_scale(__uint_as_float(m), &dn, &up);
+        float dn, sc;
+        power_scale(__uint_as_float(m), &dn, &sc);
         for (int r = lane; r < S::RP; r += 32) low[row * S::RP + r] *= dn;
-        if (lane == 0) row_up[row] = up;
+        if (lane == 0) row_up[row] = sc;
       }
       __syncthreads();
     }
@@ -344,83 +575,54 @@ __global__ void __launch_bounds__(kThreadsPerCta, NT > 8 ? 1 : 2) k_apply(const 
     __syncthreads();
   }
 
-  constexpr int KT = NT / 2;  // rank steps of 16
-  const T* up = static_cast<const T*>(a.up) + static_cast<int64_t>(max(tile.adapter, 0)) * a.rank * a.n;
   TY* y = static_cast<TY*>(a.y);
   // ldmatrix: lane l names row l % 16 and rank half l / 16 of a 16 x 16 tile.
   const uint32_t terms_addr = smem_addr(terms) + static_cast<uint32_t>((lane & 15) * S::PITCH + (lane >> 4) * 8) * 2u;
-  for (int n0 = slot * 64; n0 < a.n; n0 += slots * 64) {
+  for (int n0 = slot * 64; n0 < a.n; n0 += stride) {
+    const int later = n0 + stride;
     uint32_t b0[KT][8], b1[KT][8];
-    if (live) {
-      const int c = n0 + 8 * g;
-      const int left = a.n - c;
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        uint4 v[4];
+    for (int kt = 0; kt < KT; ++kt) {
+      wait_all_but<UNITS - 1>();
+      const uint32_t src = up_ring + static_cast<uint32_t>(kt * 4 * 512);
+      const uint4 v0 = landed(src), v1 = landed(src + 512), v2 = landed(src + 1024), v3 = landed(src + 1536);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = kt * 16 + 2 * t + (i & 1) + (i >> 1) * 8;
-          v[i] = load8<T, VEC>(up + static_cast<int64_t>(r) * a.n + c, r < a.rank ? left : 0);
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          b0[kt][j] = pair_of(v[0], v[1], j);
-          b1[kt][j] = pair_of(v[2], v[3], j);
-        }
+      for (int j = 0; j < 8; ++j) {
+        b0[kt][j] = pair_of(v0, v1, j);
+        b1[kt][j] = pair_of(v2, v3, j);
       }
+      issue_up(later, kt);
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      if (m * 16 >= count) break;
-      float out[2][16];  // rows g and g + 8: features n0 + 16 t ..
+      float out[2][16];  // rows g and g + 8: features n0 + 8 t .., n0 + 32 + 8 t ..
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int b = 0; b < BU; ++b) {
+        wait_all_but<UNITS - 1>();
+        const uint32_t src = ring + static_cast<uint32_t>((KT + BU * m + b) * 4 * 512);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) out[h][i] = 0.f;
-        if (tok[m][h] < 0 || !a.base) continue;
-        const int c = n0 + 16 * t;
-        const int64_t at = static_cast<int64_t>(tok[m][h]) * a.ldb + c;
-        if (a.base_f32) {
-          const float* b = static_cast<const float*>(a.base) + at;
-          if constexpr (VEC) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (c + 4 * q < a.n) {
-                const float4 v = *reinterpret_cast<const float4*>(b + 4 * q);
-                out[h][4 * q] = v.x;
-                out[h][4 * q + 1] = v.y;
-                out[h][4 * q + 2] = v.z;
-                out[h][4 * q + 3] = v.w;
-              }
+        for (int i = 0; i < 4; ++i) {
+          const uint4 v = landed(src + i * 512);
+          if constexpr (BASE_F32) {
+            out[b][4 * i] = __uint_as_float(v.x);
+            out[b][4 * i + 1] = __uint_as_float(v.y);
+            out[b][4 * i + 2] = __uint_as_float(v.z);
+            out[b][4 * i + 3] = __uint_as_float(v.w);
           } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (c + i < a.n) out[h][i] = b[i];
-          }
-        } else {
-          const T* b = static_cast<const T*>(a.base) + at;
-          if constexpr (VEC) {
-#pragma unroll
-            for (int q = 0; q < 2; ++q)
-              if (c + 8 * q < a.n) {
-                float f[8];
-                load_f32<T, 8>(b + 8 * q, f);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) out[h][8 * q + i] = f[i];
-              }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (c + i < a.n) out[h][i] = to_f32<T>(b[i]);
+            for (int q = 0; q < 8; ++q)
+              out[i >> 1][(i & 1) * 8 + q] = value16<T>(static_cast<uint16_t>(word(v, q >> 1) >> (16 * (q & 1))));
           }
         }
+        issue_base(later, m, b);
       }
+      if (m * 16 >= count) continue;  // the same for the whole cluster
       if (live) {
-        float acc[8][4];
+        float d[8][4];
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
+          for (int i = 0; i < 4; ++i) d[j][i] = 0.f;
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -428,7 +630,7 @@ __global__ void __launch_bounds__(kThreadsPerCta, NT > 8 ? 1 : 2) k_apply(const 
             uint32_t f[4];
             ldmatrix4(f, terms_addr + static_cast<uint32_t>((q * S::ROWS + m * 16) * S::PITCH + kt * 16) * 2u);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) mma<T>(acc[j], f, b0[kt][j], b1[kt][j]);
+            for (int j = 0; j < 8; ++j) mma<T>(d[j], f, b0[kt][j], b1[kt][j]);
           }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -436,44 +638,60 @@ __global__ void __launch_bounds__(kThreadsPerCta, NT > 8 ? 1 : 2) k_apply(const 
           if constexpr (std::is_same_v<T, __half>) p = row_up[m * 16 + h * 8 + g];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            out[h][j] += acc[j][2 * h] * p;
-            out[h][8 + j] += acc[j][2 * h + 1] * p;
+            out[h][j] += d[j][2 * h] * p;
+            out[h][8 + j] += d[j][2 * h + 1] * p;
           }
         }
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         if (tok[m][h] < 0) continue;
-        const int c = n0 + 16 * t;
-        TY* d = y + static_cast<int64_t>(tok[m][h]) * a.ldy + c;
+        TY* to = y + static_cast<int64_t>(tok[m][h]) * a.ldy;
         if constexpr (VEC) {
           constexpr int W = 16 / static_cast<int>(sizeof(TY));  // features per 16 bytes
 #pragma unroll
-          for (int q = 0; q < 16 / W; ++q)
-            if (c + W * q < a.n) {
+          for (int q = 0; q < 16 / W; ++q) {
+            const int c = n0 + 32 * (W * q / 8) + 8 * t + W * q % 8;
+            if (c < a.n) {
               float f[W];
 #pragma unroll
               for (int i = 0; i < W; ++i) f[i] = out[h][W * q + i];
-              store_f32<TY, W>(d + W * q, f);
+              store_f32<TY, W>(to + c, f);
             }
+          }
         } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (c + i < a.n) d[i] = from_f32<TY>(out[h][i]);
+          for (int i = 0; i < 16; ++i) {
+            const int c = n0 + 32 * (i >> 3) + 8 * t + (i & 7);
+            if (c < a.n) to[c] = from_f32<TY>(out[h][i]);
+          }
         }
       }
     }
   }
 }
 
-template <typename T, typename TY, int MT, int NT, bool VEC>
-cudaError_t launch_apply(const LowRankApplyArgs& a, int64_t clusters, int cluster, cudaStream_t s) {
-  using S = ApplySmem<MT, NT>;
+// cudaFuncSetAttribute once per device and instance.
+template <typename F>
+cudaError_t allow_smem(F* fn, size_t bytes, std::atomic<uint64_t>* done) {
+  if (bytes <= 48 * 1024) return cudaSuccess;
+  const int dev = current_device();
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (dev >= 0 && dev < 64 && (done->load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (e == cudaSuccess && dev >= 0 && dev < 64) done->fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
+template <typename T, typename TY, typename S, bool BASE_F32, bool VEC>
+cudaError_t launch_apply_as(const LowRankApplyArgs& a, int64_t clusters, int cluster, cudaStream_t s) {
   constexpr int TERMS = std::is_same_v<TY, float> ? 3 : 2;
-  constexpr size_t bytes = static_cast<size_t>((kWarps + 2) * S::LOW + S::ROWS) * 4 +
-                           static_cast<size_t>(TERMS) * S::ROWS * S::PITCH * 2;
-  auto* fn = &k_apply<T, TY, MT, NT, TERMS, VEC>;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  constexpr size_t bytes = S::bytes(TERMS, BASE_F32);
+  static_assert(bytes <= 227 * 1024, "shared memory of one CTA");
+  constexpr int MINB = bytes <= 113 * 1024 ? 2 : 1;
+  auto* fn = &k_apply<T, TY, S, TERMS, BASE_F32, VEC, MINB>;
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem(fn, bytes, &done);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(clusters * cluster));
@@ -490,212 +708,320 @@ cudaError_t launch_apply(const LowRankApplyArgs& a, int64_t clusters, int cluste
   return cudaLaunchKernelEx(&cfg, fn, a);
 }
 
+template <typename T, typename TY, typename S, bool VEC>
+cudaError_t launch_apply(const LowRankApplyArgs& a, int64_t clusters, int cluster, cudaStream_t s) {
+  return a.base_f32 ? launch_apply_as<T, TY, S, true, VEC>(a, clusters, cluster, s)
+                    : launch_apply_as<T, TY, S, false, VEC>(a, clusters, cluster, s);
+}
+
 template <typename T, typename TY>
 cudaError_t pick_apply(const LowRankApplyArgs& a, bool vec, int tile, int64_t clusters, int cluster, cudaStream_t s) {
+  using R16 = ApplyShape<1, 2, 4>;
+  using R32 = ApplyShape<1, 4, 2>;
+  using R64 = ApplyShape<1, 8, 2>;
+  using R128 = ApplyShape<1, 16, 2>;
   if (!vec) {
-    if (a.rank <= 16) return launch_apply<T, TY, 1, 2, false>(a, clusters, cluster, s);
-    if (a.rank <= 32) return launch_apply<T, TY, 1, 4, false>(a, clusters, cluster, s);
-    if (a.rank <= 64) return launch_apply<T, TY, 1, 8, false>(a, clusters, cluster, s);
-    return launch_apply<T, TY, 1, 16, false>(a, clusters, cluster, s);
+    if (a.rank <= 16) return launch_apply<T, TY, R16, false>(a, clusters, cluster, s);
+    if (a.rank <= 32) return launch_apply<T, TY, R32, false>(a, clusters, cluster, s);
+    if (a.rank <= 64) return launch_apply<T, TY, R64, false>(a, clusters, cluster, s);
+    return launch_apply<T, TY, R128, false>(a, clusters, cluster, s);
   }
   if (a.rank <= 16)
-    return tile == 64 ? launch_apply<T, TY, 4, 2, true>(a, clusters, cluster, s)
-                      : launch_apply<T, TY, 1, 2, true>(a, clusters, cluster, s);
+    return tile == 64 ? launch_apply<T, TY, ApplyShape<4, 2, 2>, true>(a, clusters, cluster, s)
+                      : launch_apply<T, TY, R16, true>(a, clusters, cluster, s);
   if (a.rank <= 32)
-    return tile == 64 ? launch_apply<T, TY, 4, 4, true>(a, clusters, cluster, s)
-                      : launch_apply<T, TY, 1, 4, true>(a, clusters, cluster, s);
+    return tile == 32 ? launch_apply<T, TY, ApplyShape<2, 4, 2>, true>(a, clusters, cluster, s)
+                      : launch_apply<T, TY, R32, true>(a, clusters, cluster, s);
   if (a.rank <= 64)
-    return tile == 32 ? launch_apply<T, TY, 2, 8, true>(a, clusters, cluster, s)
-                      : launch_apply<T, TY, 1, 8, true>(a, clusters, cluster, s);
-  return launch_apply<T, TY, 1, 16, true>(a, clusters, cluster, s);
+    return tile == 32 ? launch_apply<T, TY, ApplyShape<2, 8, 3>, true>(a, clusters, cluster, s)
+                      : launch_apply<T, TY, R64, true>(a, clusters, cluster, s);
+  return launch_apply<T, TY, R128, true>(a, clusters, cluster, s);
 }
 
 // ---------------------------------------------------------------- weight gradient
 
-// grad[a, r, c] = sum over the tokens of adapter a of s[t, r] z[t, c].
-//
-// A warp owns 16 rank rows and 64 features; RG warps side by side cover the
-// rank, kWarps / RG column groups the CTA's features.  The tokens of the
-// adapter are shared out over the cluster in chunks of 64, whose s values are
-// split into terms once in shared memory for all warps.  A chunk's sum is
-// formed by the matrix units (4 steps per term) and added to the running
-// sum in fp32 with rounding, so that a long batch loses nothing to the units'
-// truncation.  The cluster's partial sums are added in rank order.
-template <typename T, bool Q8, bool VEC>
-__device__ __forceinline__ uint4 load_z(const LowRankWgradArgs& a, int tok, int c, int left) {
-  if (tok < 0) return make_uint4(0u, 0u, 0u, 0u);
-  if constexpr (!Q8) {
-    return load8<T, VEC>(static_cast<const T*>(a.z) + static_cast<int64_t>(tok) * a.ldz + c, left);
-  } else {
-    // code rows are 16-byte aligned: 8 codes may be read together when 8 exist
-    uint32_t w[4] = {0u, 0u, 0u, 0u};
-    if (left > 0) {
-      const int8_t* q = a.codes + static_cast<int64_t>(tok) * a.ldq + c;
-      const float step = a.steps[static_cast<int64_t>(c >> 6) * a.lds + tok];
-      uint32_t b[2] = {0u, 0u};
-      if (left >= 8) {
-        const uint2 v = *reinterpret_cast<const uint2*>(q);
-        b[0] = v.x;
-        b[1] = v.y;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < left) b[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(q[i])) << (8 * (i & 3));
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float f = static_cast<float>(static_cast<int8_t>(b[i >> 2] >> (8 * (i & 3)))) * step;
-        w[i >> 1] |= static_cast<uint32_t>(i < left ? bits16<T>(f) : 0) << (16 * (i & 1));
-      }
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-  }
-}
-
-template <int RG>
-struct WgradSmem {
-  static constexpr int RP = 16 * RG;
+// Tile shape and memory of one instance.  A warp owns MR x 16 rank rows and 64
+// features; RG warps side by side cover the rank, kWarps / RG column groups
+// the CTA's features; UNITS steps of 16 tokens in flight.
+template <int RG_, int MR_, int UNITS_>
+struct WgradShape {
+  static constexpr int RG = RG_, MR = MR_, UNITS = UNITS_;
+  static constexpr int RP = 16 * RG * MR;
   static constexpr int PITCH = RP + 8;
   static constexpr int COLS = 64 * (kWarps / RG);
+  static constexpr int PER_THREAD = kChunk * RP / kThreadsPerCta;  // s values of a chunk
+  static constexpr size_t RING_BYTES = static_cast<size_t>(kWarps) * UNITS * 4 * 512;
+  static constexpr size_t PART_BYTES = static_cast<size_t>(RP) * COLS * 4;
+  static constexpr size_t SHARED_BYTES = RING_BYTES > PART_BYTES ? RING_BYTES : PART_BYTES;
+  static constexpr size_t bytes(int terms, bool half, bool q8) {
+    return SHARED_BYTES + (q8 ? static_cast<size_t>(2 * kChunk * (COLS / 64)) * 4 : 0) + static_cast<size_t>(2 * RP + 4 * kChunk) * 4 +
+           2 * static_cast<size_t>(terms) * kChunk * PITCH * 2 + (half ? static_cast<size_t>(kChunk) * RP * 4 : 0);
+  }
 };
 
-template <typename T, typename TG, int RG, int TERMS, bool Q8, bool VEC>
-__global__ void __launch_bounds__(kThreadsPerCta, 2) k_wgrad(const LowRankWgradArgs a) {
-  using S = WgradSmem<RG>;
+// grad[a, r, c] = sum over the tokens of adapter a of s[t, r] z[t, c].
+//
+// The adapter's tokens are shared out over the cluster in chunks of 64, whose
+// s values are split into terms once in shared memory for all warps; z goes
+// straight to the lanes that use it, UNITS steps ahead.  A chunk's sum is
+// formed by the matrix units (4 steps per term) and added to the running sum in
+// fp32 with rounding, so that a long batch loses nothing to the units'
+// truncation.  The cluster's partial sums are added in rank order.
+template <typename T, typename TG, typename S, int TERMS, bool Q8, bool VEC, int MINB>
+__global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgradArgs a) {
+  constexpr int MR = S::MR, RP = S::RP;
+  constexpr bool HALF = std::is_same_v<T, __half>;
   extern __shared__ __align__(16) uint8_t smem[];
-  float* part = reinterpret_cast<float*>(smem);                    // [RP][COLS]: this CTA's sum
-  float* raw = part;                                               // [kChunk][RP]: s of a chunk (before the sum)
-  float* up = part + S::RP * S::COLS;                              // [RP]: power of two of every rank row (fp16)
-  int* toks = reinterpret_cast<int*>(up + S::RP);                  // [kChunk]
-  uint16_t* terms = reinterpret_cast<uint16_t*>(toks + kChunk);    // [TERMS][kChunk][PITCH]
+  float* part = reinterpret_cast<float*>(smem);                    // [RP][COLS]: this CTA's sum, after the ring's use
+  float* scales = reinterpret_cast<float*>(smem + S::SHARED_BYTES);  // [2][RP]: power of two of every rank row (fp16)
+  int* toks = reinterpret_cast<int*>(scales + 2 * RP);             // [4][kChunk]: -1 behind the last
+  float* steps = reinterpret_cast<float*>(toks + 4 * kChunk);      // [2][COLS / 64][kChunk] (8 bits)
+  uint16_t* terms = reinterpret_cast<uint16_t*>(steps + (Q8 ? 2 * (S::COLS / 64) * kChunk : 0));  // [2][TERMS][kChunk][PITCH]
+  float* raw = reinterpret_cast<float*>(terms + 2 * TERMS * kChunk * S::PITCH);  // [kChunk][RP] (fp16)
 
   const uint32_t crank = cluster_rank(), csize = cluster_size();
   const int adapter = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int rg = warp % RG;
-  const int lc = (warp / RG) * 64;                                 // first feature of the warp in the CTA
-  const int c0 = (blockIdx.x / csize) * S::COLS;
+  const int rg = warp % S::RG;
+  const int lc = (warp / S::RG) * 64;                              // first feature of the warp in the CTA
+  const int c0 = static_cast<int>(blockIdx.x / csize) * S::COLS;
   const int p0 = a.starts[adapter], p1 = a.starts[adapter + 1];
-  float sum[8][4];
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sum[j][i] = 0.f;
+  // This CTA's chunks: crank, crank + csize, ...; only the last of all is short.
+  const int first = p0 + static_cast<int>(crank) * kChunk;
+  const int hop = static_cast<int>(csize) * kChunk;
+  const int chunks = first < p1 ? (p1 - first + hop - 1) / hop : 0;
+  const int last_have = chunks > 0 ? min(kChunk, p1 - (first + (chunks - 1) * hop)) : 0;
+  const int units = chunks > 0 ? 4 * (chunks - 1) + (last_have + 15) / 16 : 0;
   const int cz = c0 + lc + 8 * g;  // features this lane loads
   const int left = a.k - cz;
-  const uint32_t terms_addr =
-      smem_addr(terms) +
-      static_cast<uint32_t>(((lane & 7) + ((lane >> 4) & 1) * 8) * S::PITCH + rg * 16 + ((lane >> 3) & 1) * 8) * 2u;
-  for (int q0 = p0 + static_cast<int>(crank) * kChunk; q0 < p1; q0 += static_cast<int>(csize) * kChunk) {
-    const int have = min(kChunk, p1 - q0);
-    __syncthreads();  // the last chunk's terms are no longer read
-    if (threadIdx.x < kChunk) toks[threadIdx.x] = threadIdx.x < have ? a.order[q0 + threadIdx.x] : -1;
-    __syncthreads();
-    for (int i = threadIdx.x; i < kChunk * S::RP; i += kThreadsPerCta) {
-      const int row = i / S::RP, r = i - row * S::RP;
-      const int tok = toks[row];
-      float v = (tok >= 0 && r < a.rank) ? a.s[static_cast<int64_t>(tok) * a.rank + r] : 0.f;
-      if constexpr (std::is_same_v<T, __half>) {
-        raw[i] = v;
-      } else {
+  const uint32_t ring = smem_addr(smem) + static_cast<uint32_t>(warp * S::UNITS * 4 * 512) +
+                        (Q8 ? codes_by_rows(g, t) : by_rows(g, t));
+
+  // The tokens of a chunk are in shared memory three chunks ahead of its use.
+  static_assert(S::UNITS <= 8, "a unit's tokens are known when it starts");
+  auto chunk_token = [&](int n) {
+    const int p = first + n * hop + threadIdx.x;
+    return n < chunks && p < p1 ? __ldg(a.order + p) : -1;
+  };
+  if (threadIdx.x < kChunk) {
 #pragma unroll
-        for (int q = 0; q < TERMS; ++q) {
-          const uint16_t b = bits16<T>(v);
-          terms[(q * kChunk + row) * S::PITCH + r] = b;
-          v -= value16<T>(b);
+    for (int n = 0; n < 3; ++n) toks[n * kChunk + threadIdx.x] = chunk_token(n);
+  }
+  __syncthreads();
+  // Unit u: 16 tokens of chunk u / 4, of which this lane takes 2t, 2t+1, 2t+8, 2t+9.
+  const T* zcol = Q8 ? nullptr : static_cast<const T*>(a.z) + (left > 0 ? cz : 0);
+  const int8_t* qcol = Q8 ? a.codes + (left > 0 ? cz : 0) : nullptr;
+  auto issue = [&](int u, int at) {
+    if (u < units) {
+      const uint32_t dst = ring + static_cast<uint32_t>(at * 4 * 512);
+      const int* mine = toks + ((u >> 2) & 3) * kChunk + (u & 3) * 16 + 2 * t;
+      const int2 ta = *reinterpret_cast<const int2*>(mine), tb = *reinterpret_cast<const int2*>(mine + 8);
+      const int tk[4] = {ta.x, ta.y, tb.x, tb.y};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int n = tk[i] >= 0 ? left : 0;
+        const int tok = max(tk[i], 0);
+        if constexpr (!Q8) {
+          fetch<T, VEC>(dst + i * 512, zcol + static_cast<int64_t>(tok) * a.ldz, n);
+        } else {
+          // code rows are 16-byte aligned and padded to 8
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst + i * 512),
+                       "l"(qcol + static_cast<int64_t>(tok) * a.ldq), "r"(max(0, min(n, 8)))
+                       : "memory");
         }
       }
     }
-    __syncthreads();
-    if constexpr (std::is_same_v<T, __half>) {
-      for (int r = warp; r < S::RP; r += kWarps) {
-        const uint32_t v0 = __float_as_uint(raw[lane * S::RP + r]) & 0x7fffffffu;
-        const uint32_t v1 = __float_as_uint(raw[(lane + 32) * S::RP + r]) & 0x7fffffffu;
-        const uint32_t m = __reduce_max_sync(0xffffffffu, max(v0, v1));
-        float dn, u;
-        power_scale(__uint_as_float(m), &dn, &u);
-        if (lane == 0) up[r] = u;
+    commit();
+  };
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = lane + 32 * h;
-          float v = raw[row * S::RP + r] * dn;
+  for (int u = 0; u < S::UNITS; ++u) issue(u, u);
+
+  // s of a chunk: the thread's share in registers, then split into terms.
+  // (A group of 64 features is one warp's: one step per token and warp.)
+  constexpr int STEPS = Q8 ? kChunk * (S::COLS / 64) / kThreadsPerCta + (kChunk * (S::COLS / 64) < kThreadsPerCta) : 1;
+  float mine[S::PER_THREAD], my_step[STEPS];
+  auto load_s = [&](int n) {
+    if constexpr (Q8) {
 #pragma unroll
-          for (int q = 0; q < TERMS; ++q) {
-            const uint16_t b = bits16<T>(v);
-            terms[(q * kChunk + row) * S::PITCH + r] = b;
-            v -= value16<T>(b);
-          }
-        }
+      for (int i = 0; i < STEPS; ++i) {
+        const int e = i * kThreadsPerCta + threadIdx.x;
+        const int tok = toks[(n & 3) * kChunk + e % kChunk], c = c0 + 64 * (e / kChunk);
+        my_step[i] = (tok >= 0 && e / kChunk < S::COLS / 64 && c < a.k)
+                         ? __ldg(a.steps + static_cast<int64_t>(c >> 6) * a.lds + tok)
+                         : 0.f;
       }
+    }
+#pragma unroll
+    for (int i = 0; i < S::PER_THREAD; ++i) {
+      const int e = i * kThreadsPerCta + threadIdx.x;
+      const int tok = toks[(n & 3) * kChunk + e / RP], r = e % RP;
+      mine[i] = (tok >= 0 && r < a.rank) ? __ldg(a.s + static_cast<int64_t>(tok) * a.rank + r) : 0.f;
+    }
+  };
+  auto split = [&](float v, int n, int row, int r) {
+#pragma unroll
+    for (int q = 0; q < TERMS; ++q) {
+      const uint16_t b = bits16<T>(v);
+      terms[(((n & 1) * TERMS + q) * kChunk + row) * S::PITCH + r] = b;
+      v -= value16<T>(b);
+    }
+  };
+  auto store_s = [&](int n) {
+    if constexpr (Q8) {
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        const int e = i * kThreadsPerCta + threadIdx.x;
+        if (e / kChunk < S::COLS / 64) steps[(n & 1) * (S::COLS / 64) * kChunk + e] = my_step[i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < S::PER_THREAD; ++i) {
+      const int e = i * kThreadsPerCta + threadIdx.x;
+      if constexpr (HALF) raw[e] = mine[i];
+      else split(mine[i], n, e / RP, e % RP);
+    }
+    if constexpr (HALF) {
       __syncthreads();
+      for (int r = warp; r < RP; r += kWarps) {
+        const float v0 = raw[lane * RP + r], v1 = raw[(lane + 32) * RP + r];
+        const uint32_t m = __reduce_max_sync(
+            0xffffffffu, max(__float_as_uint(v0) & 0x7fffffffu, __float_as_uint(v1) & 0x7fffffffu));
+        float dn, up;
+        power_scale(__uint_as_float(m), &dn, &up);
+        if (lane == 0) scales[(n & 1) * RP + r] = up;
+        split(v0 * dn, n, lane, r);
+        split(v1 * dn, n, lane + 32, r);
+      }
     }
-    float acc[8][4];
+  };
+  if (chunks > 0) {
+    load_s(0);
+    store_s(0);
+  }
+  __syncthreads();
+
+  float sum[MR][8][4];
+#pragma unroll
+  for (int m = 0; m < MR; ++m)
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
+      for (int i = 0; i < 4; ++i) sum[m][j][i] = 0.f;
+  const uint32_t terms_addr =
+      smem_addr(terms) + static_cast<uint32_t>(((lane & 7) + ((lane >> 4) & 1) * 8) * S::PITCH + rg * MR * 16 +
+                                               ((lane >> 3) & 1) * 8) * 2u;
+  int at = 0;
+  for (int n = 0; n < chunks; ++n) {
+    const int later = threadIdx.x < kChunk ? chunk_token(n + 3) : -1;
+    if (n + 1 < chunks) load_s(n + 1);
+    float acc[MR][8][4];
 #pragma unroll
-    for (int ks = 0; ks < kChunk / 16; ++ks) {
-      if (ks * 16 >= have) break;
+    for (int m = 0; m < MR; ++m)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
+    const int here = min(4, units - 4 * n);
+#pragma unroll 1
+    for (int ks = 0; ks < here; ++ks) {
+      wait_all_but<S::UNITS - 1>();
+      const uint32_t src = ring + static_cast<uint32_t>(at * 4 * 512);
       uint4 v[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v[i] = load_z<T, Q8, VEC>(a, toks[ks * 16 + 2 * t + (i & 1) + (i >> 1) * 8], cz, left);
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (!Q8) {
+          v[i] = landed(src + i * 512);
+        } else {
+          const int row = ks * 16 + 2 * t + (i & 1) + (i >> 1) * 8;
+          v[i] = read_back<T>(landed_codes(src + i * 512),
+                              steps[((n & 1) * (S::COLS / 64) + (lc >> 6)) * kChunk + row]);
+        }
+      }
+      uint32_t b0[8], b1[8];
 #pragma unroll
-      for (int q = TERMS - 1; q >= 0; --q) {
-        uint32_t f[4];
-        ldmatrix4_trans(f, terms_addr + static_cast<uint32_t>((q * kChunk + ks * 16) * S::PITCH) * 2u);
+      for (int j = 0; j < 8; ++j) {
+        b0[j] = pair_of(v[0], v[1], j);
+        b1[j] = pair_of(v[2], v[3], j);
+      }
+      issue(4 * n + ks + S::UNITS, at);
+      at = at + 1 == S::UNITS ? 0 : at + 1;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) mma<T>(acc[j], f, pair_of(v[0], v[1], j), pair_of(v[2], v[3], j));
+      for (int m = 0; m < MR; ++m)
+#pragma unroll
+        for (int q = TERMS - 1; q >= 0; --q) {
+          uint32_t f[4];
+          ldmatrix4_trans(f, terms_addr + static_cast<uint32_t>((((n & 1) * TERMS + q) * kChunk + ks * 16) * S::PITCH +
+                                                                m * 16) * 2u);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) mma<T>(acc[m][j], f, b0[j], b1[j]);
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+      float pa = 1.f, pb = 1.f;
+      if constexpr (HALF) {
+        pa = scales[(n & 1) * RP + (rg * MR + m) * 16 + g];
+        pb = scales[(n & 1) * RP + (rg * MR + m) * 16 + g + 8];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        sum[m][j][0] += acc[m][j][0] * pa;
+        sum[m][j][1] += acc[m][j][1] * pa;
+        sum[m][j][2] += acc[m][j][2] * pb;
+        sum[m][j][3] += acc[m][j][3] * pb;
       }
     }
-    float pa = 1.f, pb = 1.f;
-    if constexpr (std::is_same_v<T, __half>) {
-      pa = up[rg * 16 + g];
-      pb = up[rg * 16 + g + 8];
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      sum[j][0] += acc[j][0] * pa;
-      sum[j][1] += acc[j][1] * pa;
-      sum[j][2] += acc[j][2] * pb;
-      sum[j][3] += acc[j][3] * pb;
-    }
+    if (n + 1 < chunks) store_s(n + 1);  // the other half of terms: read by no warp since the last barrier
+    if (threadIdx.x < kChunk) toks[((n + 3) & 3) * kChunk + threadIdx.x] = later;
+    __syncthreads();
   }
-  __syncthreads();  // raw and part share memory
+  wait_all_but<0>();
+  __syncthreads();  // the ring becomes the partial sums
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float* row = part + (rg * 16 + h * 8 + g) * S::COLS + lc + 16 * t;
+  for (int m = 0; m < MR; ++m)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      row[j] = sum[j][2 * h];
-      row[8 + j] = sum[j][2 * h + 1];
+    for (int h = 0; h < 2; ++h) {
+      float* row = part + ((rg * MR + m) * 16 + h * 8 + g) * S::COLS + lc + 16 * t;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        *reinterpret_cast<float4*>(row + 4 * q) =
+            make_float4(sum[m][4 * q][2 * h], sum[m][4 * q + 1][2 * h], sum[m][4 * q + 2][2 * h], sum[m][4 * q + 3][2 * h]);
+        *reinterpret_cast<float4*>(row + 8 + 4 * q) =
+            make_float4(sum[m][4 * q][2 * h + 1], sum[m][4 * q + 1][2 * h + 1], sum[m][4 * q + 2][2 * h + 1],
+                        sum[m][4 * q + 3][2 * h + 1]);
+      }
     }
-  }
   cluster_sync();
   const uint32_t part_addr = smem_addr(part);
   TG* grad = static_cast<TG*>(a.grad) + static_cast<int64_t>(adapter) * a.rank * a.k;
-  const int total = a.rank * S::COLS;
+  const int total = a.rank * S::COLS / 4;
   for (int i = static_cast<int>(crank) * kThreadsPerCta + threadIdx.x; i < total;
        i += static_cast<int>(csize) * kThreadsPerCta) {
-    const int r = i / S::COLS, c = i - r * S::COLS;
-    float v = 0.f;
-    for (uint32_t q = 0; q < csize; ++q) v += peer_load(peer_addr(part_addr + 4u * i, q));
-    if (c0 + c < a.k) grad[static_cast<int64_t>(r) * a.k + c0 + c] = from_f32<TG>(v);
+    const int r = i / (S::COLS / 4), c = c0 + 4 * (i - r * (S::COLS / 4));
+    const float4 v = peer_sum4(part_addr + 16u * i, csize);
+    const float f[4] = {v.x, v.y, v.z, v.w};
+    TG* to = grad + static_cast<int64_t>(r) * a.k + c;
+    if (VEC && !Q8 && c < a.k) {  // k is a multiple of 8
+      store_f32<TG, 4>(to, f);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (c + q < a.k) to[q] = from_f32<TG>(f[q]);
+    }
   }
   cluster_sync();  // the others may still read this CTA's sums
 }
 
-template <typename T, typename TG, int RG, bool Q8, bool VEC>
+template <typename T, typename TG, typename S, bool Q8, bool VEC>
 cudaError_t launch_wgrad(const LowRankWgradArgs& a, int64_t adapters, int cluster, cudaStream_t s) {
-  using S = WgradSmem<RG>;
   constexpr int TERMS = std::is_same_v<TG, float> ? 3 : 2;
-  constexpr size_t bytes = static_cast<size_t>(S::RP * S::COLS + S::RP + kChunk) * 4 +
-                           static_cast<size_t>(TERMS) * kChunk * S::PITCH * 2;
-  static_assert(S::COLS >= kChunk, "raw fits in part");
-  auto* fn = &k_wgrad<T, TG, RG, TERMS, Q8, VEC>;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  constexpr size_t bytes = S::bytes(TERMS, std::is_same_v<T, __half>, Q8);
+  static_assert(bytes <= 227 * 1024, "shared memory of one CTA");
+  constexpr int MINB = S::MR == 1 && bytes <= 113 * 1024 ? 2 : 1;  // MR 2 needs the registers of both
+  auto* fn = &k_wgrad<T, TG, S, TERMS, Q8, VEC, MINB>;
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem(fn, bytes, &done);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(ceil_div64(a.k, S::COLS) * cluster), static_cast<unsigned>(adapters));
@@ -714,10 +1040,10 @@ cudaError_t launch_wgrad(const LowRankWgradArgs& a, int64_t adapters, int cluste
 
 template <typename T, typename TG, bool Q8, bool VEC>
 cudaError_t pick_wgrad(const LowRankWgradArgs& a, int64_t adapters, int cluster, cudaStream_t s) {
-  if (a.rank <= 16) return launch_wgrad<T, TG, 1, Q8, VEC>(a, adapters, cluster, s);
-  if (a.rank <= 32) return launch_wgrad<T, TG, 2, Q8, VEC>(a, adapters, cluster, s);
-  if (a.rank <= 64) return launch_wgrad<T, TG, 4, Q8, VEC>(a, adapters, cluster, s);
-  return launch_wgrad<T, TG, 8, Q8, VEC>(a, adapters, cluster, s);
+  if (a.rank <= 16) return launch_wgrad<T, TG, WgradShape<1, 1, 5>, Q8, VEC>(a, adapters, cluster, s);
+  if (a.rank <= 32) return launch_wgrad<T, TG, WgradShape<2, 1, 5>, Q8, VEC>(a, adapters, cluster, s);
+  if (a.rank <= 64) return launch_wgrad<T, TG, WgradShape<4, 1, 5>, Q8, VEC>(a, adapters, cluster, s);
+  return launch_wgrad<T, TG, WgradShape<8, 1, 4>, Q8, VEC>(a, adapters, cluster, s);
 }
 
 }  // namespace lowrank
