@@ -19,36 +19,17 @@
 
 #include "convert.cuh"
 #include "internal.h"
+#include "q8.cuh"
 
 namespace kairo {
 namespace {
 
 constexpr int kQThreads = 256;
+constexpr int kQWarps = kQThreads / 32;
 constexpr int kQGroup = 64;   // columns per step
 constexpr int kQLanes = 8;    // lanes per group, 8 columns each
-constexpr int kQRows = kQThreads / kQLanes;  // rows per CTA
-constexpr int kQGroups = 4;   // groups of a row per thread
-
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int64_t left, bool vec, float (&f)[8]) {
-  if (vec && left >= 8) {
-    if constexpr (sizeof(T) == 4) {
-      float lo[4], hi[4];
-      load_f32<T, 4>(p, lo);
-      load_f32<T, 4>(p + 4, hi);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f[i] = lo[i];
-        f[4 + i] = hi[i];
-      }
-    } else {
-      load_f32<T, 8>(p, f);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = i < left ? to_f32<T>(p[i]) : 0.f;
-  }
-}
+constexpr int kQCols = 4 * kQGroup;  // columns of a warp: 512 contiguous bytes of a 16-bit row
+constexpr int kQRows = 8;     // rows of a warp, all in flight; their steps fill a sector
 
 template <typename T>
 __device__ __forceinline__ void store8(T* p, int64_t left, bool vec, const float (&f)[8]) {
@@ -67,44 +48,105 @@ __device__ __forceinline__ void store8(T* p, int64_t left, bool vec, const float
   }
 }
 
+// Eight values of a row as they are stored, and their largest magnitude as the
+// bits of a float (magnitudes order as integers, with infinities and NaN on
+// top; 16-bit ones two at a time).
+template <typename T>
+struct Row8 {
+  uint32_t w[2 * sizeof(T)];
+  __device__ __forceinline__ void load(const T* p, int64_t left, bool vec) {
+    if (vec && left >= 8) {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+        const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+        w[4 * i] = v.x;
+        w[4 * i + 1] = v.y;
+        w[4 * i + 2] = v.z;
+        w[4 * i + 3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2 * static_cast<int>(sizeof(T)); ++i) w[i] = 0u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i < left) {
+          if constexpr (sizeof(T) == 4) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+          else w[i >> 1] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[i]) << (16 * (i & 1));
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ float value(int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[i]);
+    } else {
+      const uint16_t b = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+      return to_f32<T>(*reinterpret_cast<const T*>(&b));
+    }
+  }
+  __device__ __forceinline__ uint32_t max_bits() const {
+    if constexpr (sizeof(T) == 4) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7fffffffu);
+#pragma unroll
+      for (int o = 1; o < kQLanes; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      return m;
+    } else {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+#pragma unroll
+      for (int o = 1; o < kQLanes; o <<= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const uint16_t b = static_cast<uint16_t>(max(m >> 16, m & 0xffffu));
+      return __float_as_uint(to_f32<T>(*reinterpret_cast<const T*>(&b)));
+    }
+  }
+};
+
+// A warp takes 256 columns of 8 rows: 32 groups, of which each lane computes
+// the two quotients of one.  Bound by memory when that is done (3.06 bytes a
+// value of a 16-bit activation); with the quotients computed by all lanes for
+// every row, and the largest magnitude one value at a time, the instructions
+// bound it: 8192 x 32768 took 276 us.
 template <typename T>
 __global__ void __launch_bounds__(kQThreads) k_quantize(const T* __restrict__ x, int64_t n, int64_t k, int64_t ldx,
                                                         bool vec, int8_t* __restrict__ codes, int64_t ldq,
                                                         float* __restrict__ steps, int64_t lds) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kQRows + threadIdx.x / kQLanes;
-  const int sub = threadIdx.x % kQLanes;
-  const int64_t g0 = static_cast<int64_t>(blockIdx.y) * kQGroups;
-  if (row >= n) return;  // whole groups of kQLanes lanes leave together
-  const unsigned lanes = 0xffu << (threadIdx.x & 24);
-  float f[kQGroups][8];
+  const int lane = threadIdx.x & 31;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kQRows;
+  const int64_t c0 = (static_cast<int64_t>(blockIdx.y) * kQWarps + (threadIdx.x >> 5)) * kQCols;
+  const int64_t c = c0 + lane * 8;
+  if (c0 >= k) return;
+  Row8<T> f[kQRows];
 #pragma unroll
-  for (int u = 0; u < kQGroups; ++u) {
-    const int64_t c = (g0 + u) * kQGroup + sub * 8;
-    load8<T>(x + row * ldx + c, k - c, vec, f[u]);
+  for (int u = 0; u < kQRows; ++u) f[u].load(x + (r0 + u) * ldx + c, r0 + u < n ? k - c : 0, vec);
+  uint32_t mine = 0;  // largest magnitude of row r0 + lane % 8, group of lane / 8
+#pragma unroll
+  for (int u = 0; u < kQRows; ++u) {
+    const uint32_t m = f[u].max_bits();
+    if ((lane & 7) == u) mine = m;
   }
+  const float a = __uint_as_float(mine);
+  const bool broken = mine >= 0x7f800000u;
+  const bool live = !broken && a >= 0x1p-100f;
+  const float inv = live ? __fmul_rn(127.f, __frcp_rn(a)) : 0.f;
+  const int64_t group = (c0 >> 6) + (lane >> 3), row = r0 + (lane & 7);
+  if (group * kQGroup < k && row < n)
+    steps[group * lds + row] = broken ? __uint_as_float(0x7fffffffu) : (live ? __fmul_rn(a, 1.f / 127.f) : 0.f);
 #pragma unroll
-  for (int u = 0; u < kQGroups; ++u) {
-    const int64_t c = (g0 + u) * kQGroup + sub * 8;
-    if ((g0 + u) * kQGroup >= k) break;
-    // magnitudes order as integers, with infinities and NaN on top
-    unsigned m = 0;
+  for (int u = 0; u < kQRows; ++u) {
+    const float s = __shfl_sync(0xffffffffu, inv, (lane & 24) + u);
+    unsigned w[2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[u][i]) & 0x7fffffffu);
+    for (int h = 0; h < 2; ++h) {
+      unsigned q[4];
 #pragma unroll
-    for (int o = 1; o < kQLanes; o <<= 1) m = max(m, __shfl_xor_sync(lanes, m, o));
-    const float a = __uint_as_float(m);
-    const bool broken = m >= 0x7f800000u;
-    const bool live = !broken && a >= 0x1p-100f;
-    const float inv = live ? __fmul_rn(127.f, __frcp_rn(a)) : 0.f;
-    const float step = broken ? __uint_as_float(0x7fffffffu) : (live ? __fmul_rn(a, 1.f / 127.f) : 0.f);
-    unsigned w[2] = {0u, 0u};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float s = __fmaf_rn(live ? f[u][i] : 0.f, inv, 12582912.f);
-      w[i >> 2] |= (__float_as_uint(s) & 0xffu) << (8 * (i & 3));
+      for (int i = 0; i < 4; ++i) q[i] = __float_as_uint(__fmaf_rn(f[u].value(4 * h + i), s, 12582912.f));
+      w[h] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+      if (s == 0.f) w[h] = 0u;  // no code of an infinity or NaN
     }
-    if (c < k) *reinterpret_cast<uint2*>(codes + row * ldq + c) = make_uint2(w[0], w[1]);
-    if (sub == 0) steps[(g0 + u) * lds + row] = step;
+    if (c < k && r0 + u < n) *reinterpret_cast<uint2*>(codes + (r0 + u) * ldq + c) = make_uint2(w[0], w[1]);
   }
 }
 
@@ -112,54 +154,43 @@ template <typename T>
 __global__ void __launch_bounds__(kQThreads) k_dequantize(const int8_t* __restrict__ codes, int64_t ldq,
                                                           const float* __restrict__ steps, int64_t lds, int64_t n,
                                                           int64_t k, T* __restrict__ x, int64_t ldx, bool vec) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kQRows + threadIdx.x / kQLanes;
-  const int sub = threadIdx.x % kQLanes;
-  const int64_t g0 = static_cast<int64_t>(blockIdx.y) * kQGroups;
-  if (row >= n) return;
-  uint2 q[kQGroups];
-  float step[kQGroups];
+  const int lane = threadIdx.x & 31;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kQRows;
+  const int64_t c0 = (static_cast<int64_t>(blockIdx.y) * kQWarps + (threadIdx.x >> 5)) * kQCols;
+  const int64_t c = c0 + lane * 8;
+  if (c0 >= k) return;
+  const int64_t group = (c0 >> 6) + (lane >> 3), row = r0 + (lane & 7);
+  const float mine = group * kQGroup < k && row < n ? steps[group * lds + row] : 0.f;
+  uint2 q[kQRows];
 #pragma unroll
-  for (int u = 0; u < kQGroups; ++u) {
-    const int64_t c = (g0 + u) * kQGroup + sub * 8;
+  for (int u = 0; u < kQRows; ++u) {
     q[u] = make_uint2(0u, 0u);
-    step[u] = 0.f;
-    if (c < k) {
-      q[u] = *reinterpret_cast<const uint2*>(codes + row * ldq + c);
-      step[u] = steps[(g0 + u) * lds + row];
-    }
+    if (c < k && r0 + u < n) q[u] = *reinterpret_cast<const uint2*>(codes + (r0 + u) * ldq + c);
   }
 #pragma unroll
-  for (int u = 0; u < kQGroups; ++u) {
-    const int64_t c = (g0 + u) * kQGroup + sub * 8;
-    if (c >= k) break;
+  for (int u = 0; u < kQRows; ++u) {
+    const float step = __shfl_sync(0xffffffffu, mine, (lane & 24) + u);
     float f[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const unsigned word = i < 4 ? q[u].x : q[u].y;
-      f[i] = static_cast<float>(static_cast<int8_t>(word >> (8 * (i & 3)))) * step[u];
-    }
-    store8<T>(x + row * ldx + c, k - c, vec, f);
+    for (int i = 0; i < 8; ++i) f[i] = code_value(i < 4 ? q[u].x : q[u].y, i & 3) * step;
+    store8<T>(x + (r0 + u) * ldx + c, r0 + u < n ? k - c : 0, vec, f);
   }
 }
 
 kairo_status check_q8(int64_t n, int64_t k, int64_t ldx, kairo_dtype dtype, const void* codes, int64_t ldq,
                       const void* steps, int64_t lds) {
-  if (n < 0 || k < 0) return fail(KAIRO_STATUS_INVALID_VALUE, "invalid size");
   if (!known_dtype(dtype)) return fail(KAIRO_STATUS_INVALID_VALUE, "unknown dtype");
-  if (ldx < k || ldq < k || lds < n) return fail(KAIRO_STATUS_INVALID_VALUE, "leading dimension too small");
-  if (ldq % 16 != 0) return fail(KAIRO_STATUS_INVALID_VALUE, "ldq must be a multiple of 16");
-  if (k > int64_t(65535) * kQGroups * kQGroup || n > int64_t(0x7fffffff) * kQRows)
+  if (ldx < k) return fail(KAIRO_STATUS_INVALID_VALUE, "leading dimension too small");
+  const kairo_status st = q8_check(n, k, codes, ldq, steps, lds);
+  if (st) return st;
+  if (k > int64_t(65535) * kQWarps * kQCols || n > int64_t(0x7fffffff) * kQRows)
     return fail(KAIRO_STATUS_NOT_SUPPORTED, "activation too large");
-  if (n > 0 && k > 0) {
-    if (!codes || !steps) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
-    if (reinterpret_cast<uintptr_t>(codes) % 16) return fail(KAIRO_STATUS_INVALID_VALUE, "codes must be 16-byte aligned");
-  }
   return KAIRO_STATUS_SUCCESS;
 }
 
 dim3 q8_grid(int64_t n, int64_t k) {
   return dim3(static_cast<unsigned>(ceil_div64(n, kQRows)),
-              static_cast<unsigned>(ceil_div64(k, static_cast<int64_t>(kQGroups) * kQGroup)));
+              static_cast<unsigned>(ceil_div64(k, static_cast<int64_t>(kQWarps) * kQCols)));
 }
 
 // 16-byte accesses to x: rows and base aligned.
@@ -168,6 +199,18 @@ bool q8_vec(const void* x, int64_t ldx, kairo_dtype dtype) {
 }
 
 }  // namespace
+
+kairo_status q8_check(int64_t n, int64_t k, const void* codes, int64_t ldq, const void* steps, int64_t lds) {
+  if (n < 0 || k < 0) return fail(KAIRO_STATUS_INVALID_VALUE, "invalid size");
+  if (ldq < k || lds < n) return fail(KAIRO_STATUS_INVALID_VALUE, "leading dimension too small");
+  if (ldq % 16 != 0) return fail(KAIRO_STATUS_INVALID_VALUE, "ldq must be a multiple of 16");
+  if (n > 0 && k > 0) {
+    if (!codes || !steps) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+    if (reinterpret_cast<uintptr_t>(codes) % 16) return fail(KAIRO_STATUS_INVALID_VALUE, "codes must be 16-byte aligned");
+  }
+  return KAIRO_STATUS_SUCCESS;
+}
+
 }  // namespace kairo
 
 using namespace kairo;
@@ -215,45 +258,7 @@ extern "C" kairo_status kairo_dequantize_q8(const int8_t* codes, int64_t ldq, co
   return KAIRO_STATUS_SUCCESS;
 }
 
-namespace {
-
-// The read-back activation of the weight gradient, rows padded to 16 bytes.
-int64_t back_ld(const kairo_bsr* a) { return ceil_div64(a->cols, 8) * 8; }
-size_t back_bytes(const kairo_bsr* a, int64_t n) {
-  return align_up(static_cast<size_t>(n) * back_ld(a) * element_bytes(a->dtype), 256);
-}
-
-}  // namespace
-
 extern "C" kairo_status kairo_bsr_sddmm_q8_workspace_size(const kairo_bsr* a, int64_t n, size_t* bytes) {
   if (!a || !bytes || n < 0) return fail(KAIRO_STATUS_INVALID_VALUE, "invalid argument");
-  size_t base = 0;
-  const kairo_status st = kairo_bsr_sddmm_workspace_size(a, &base);
-  if (st) return st;
-  *bytes = align_up(base, 256) + back_bytes(a, n);
-  return KAIRO_STATUS_SUCCESS;
-}
-
-extern "C" kairo_status kairo_bsr_sddmm_q8(const kairo_bsr* a, const int32_t* row_ptr_t, const int32_t* col_idx_t,
-                                           const int32_t* perm_t, const void* dy, int64_t lddy, const int8_t* codes,
-                                           int64_t ldq, const float* steps, int64_t lds, int64_t n, void* dblocks,
-                                           kairo_dtype out_dtype, void* workspace, size_t workspace_bytes,
-                                           void* stream) {
-  size_t need = 0, base = 0;
-  kairo_status st = kairo_bsr_sddmm_q8_workspace_size(a, n, &need);
-  if (st) return st;
-  st = check_q8(n, a->cols, a->cols, a->dtype, codes, ldq, steps, lds);
-  if (st) return st;
-  st = sddmm_check(a, row_ptr_t, col_idx_t, perm_t, dy, lddy, codes, a->cols, n, dblocks, out_dtype, workspace);
-  if (st) return st;
-  if (a->nnzb == 0) return KAIRO_STATUS_SUCCESS;
-  if (!workspace) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
-  if (workspace_bytes < need) return fail(KAIRO_STATUS_WORKSPACE_TOO_SMALL, "SDDMM workspace too small");
-  st = kairo_bsr_sddmm_workspace_size(a, &base);
-  if (st) return st;
-  uint8_t* back = static_cast<uint8_t*>(workspace) + align_up(base, 256);
-  st = kairo_dequantize_q8(codes, ldq, steps, lds, n, a->cols, back, back_ld(a), a->dtype, stream);
-  if (st) return st;
-  return kairo_bsr_sddmm(a, row_ptr_t, col_idx_t, perm_t, dy, lddy, back, back_ld(a), n, dblocks, out_dtype, workspace,
-                         base, stream);
+  return kairo_bsr_sddmm_workspace_size(a, bytes);
 }

@@ -39,6 +39,7 @@
 
 #include "convert.cuh"
 #include "internal.h"
+#include "q8.cuh"
 
 namespace kairo {
 
@@ -281,26 +282,6 @@ __device__ __forceinline__ uint2 landed_codes(uint32_t src) {
   return v;
 }
 
-// Eight codes times their step, rounded to T.  A code with its sign bit flipped
-// is the low byte of the float 2^23 + 128 + code: one byte permutation and
-// one exact subtraction each, where a conversion instruction runs at a
-// quarter of their rate.
-template <typename T>
-__device__ __forceinline__ uint4 read_back(uint2 q, float step) {
-  const uint32_t b[2] = {q.x ^ 0x80808080u, q.y ^ 0x80808080u};
-  uint32_t w[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    float f[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t m = __byte_perm(b[e >> 1], 0x4b000000u, 0x7650u + (e & 1) * 2 + h);
-      f[h] = __fmul_rn(__uint_as_float(m) - 8388736.f, step);
-    }
-    w[e] = static_cast<uint32_t>(bits16<T>(f[0])) | (static_cast<uint32_t>(bits16<T>(f[1])) << 16);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
 __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void wait_all_but() {

@@ -174,6 +174,9 @@ kairo_status sddmm_check(const kairo_bsr* a, const int32_t* row_ptr_t, const int
                          const int32_t* perm_t, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t n,
                          const void* dblocks, kairo_dtype out_dtype, const void* workspace);
 
+// Checks of an activation in 8 bits (activation_q8.cu).
+kairo_status q8_check(int64_t n, int64_t k, const void* codes, int64_t ldq, const void* steps, int64_t lds);
+
 // BSR construction (bsr_build.cu)
 size_t bsr_build_ws_bytes(int64_t num_tiles, int32_t nbr);
 

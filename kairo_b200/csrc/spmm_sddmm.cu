@@ -26,6 +26,14 @@
 // allocator + MMA issuer, warps 2..5 epilogue (TMEM -> dW).  Every mbarrier
 // wait is bounded as in spmm_tc.cu.
 //
+// X in 8 bits (kairo_bsr_sddmm_q8; codes and steps of activation_q8.cu).  The
+// X box of a stage is shared by up to 8 blocks, so reading it back costs little
+// here: four more warps load the 64 x 64 codes of the next slabs into registers
+// (16 bytes a lane, two slabs ahead), turn them into the box in its swizzled
+// layout, and count as four more arrivals on the stage's full barrier.
+// Against a separate pass that writes the whole activation back in 16 bits,
+// the 8192 x 32768 layer at batch 8192 saves 268 MB read and 537 MB written.
+//
 // A CUDA-core kernel covers the other block sizes and fp32.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -33,9 +41,11 @@
 
 #include <algorithm>
 #include <sstream>
+#include <type_traits>
 
 #include "internal.h"
 #include "ptx.cuh"
+#include "q8.cuh"
 #include "tc_common.cuh"
 
 namespace kairo {
@@ -131,7 +141,23 @@ struct SddArgs {
   int32_t nbr;
   int32_t nnzb;
   int32_t stages;
+  const int8_t* codes;       // X in 8 bits
+  const float* steps;
+  int64_t ldq, lds;
+  int32_t k;
 };
+
+constexpr int kSddConvert = 4;  // warps that read X back from 8 bits
+
+// Slabs whose sum the tensor cores form before an fp32 result takes it over
+// (X in 8 bits only; the other path keeps one sum).  They truncate at each
+// step, always towards zero: over 2048 rows that came to 2.5e-6 of the result
+// (2-norm), over 8192 to four times as much.  Sums of 12 slabs, added up with
+// rounding by the epilogue warps in the other half of TMEM, stay under 1e-6; a
+// 16-bit result keeps one sum, since its own rounding is hundreds of times as
+// large.  (Adding them up in dW itself nearly doubled the time: a thread's
+// row is 256 bytes, so its loads and stores touch 32 lines each.)
+constexpr int kSddSegment = 12;
 
 template <typename TOut>
 __device__ __forceinline__ void store_row16(TOut* dst, const float* v);
@@ -166,8 +192,8 @@ __device__ __forceinline__ void store_row16<__nv_bfloat16>(__nv_bfloat16* dst, c
 }
 
 // tcgen05 kernel for bm = bk = 64 (S = 2 blocks per stack, U stacks per item).
-template <int IN_FMT, typename TOut>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int IN_FMT, typename TOut, bool Q8>
+__global__ void __launch_bounds__(kThreads + (Q8 ? 32 * kSddConvert : 0), 1)
     bsr_sddmm_tc_kernel(const __grid_constant__ CUtensorMap tmap_dy, const __grid_constant__ CUtensorMap tmap_x,
                         const SddArgs args) {
   constexpr int BS = 64;
@@ -200,7 +226,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
-      ptx::mbar_init(&full[s], 1);
+      ptx::mbar_init(&full[s], Q8 ? 1 + kSddConvert : 1);
       ptx::mbar_init(&empty[s], 1);
       issued[s] = 0;
     }
@@ -214,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (warp == 0 && lane == 0) {
     ptx::prefetch_tmap(&tmap_dy);
-    ptx::prefetch_tmap(&tmap_x);
+    if (!Q8) ptx::prefetch_tmap(&tmap_x);
   }
   if (warp == 1) {
     ptx::tmem_alloc(tmem_slot, TMEM_COLS);
@@ -226,6 +252,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int nitems = *args.nitems;
   const int G = gridDim.x;
   const int nslabs = static_cast<int>((args.n + KB - 1) / KB);
+  constexpr bool SEGMENTS = Q8 && std::is_same<TOut, float>::value;
+  const int seg = SEGMENTS ? kSddSegment : nslabs;  // slabs per accumulator set
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -237,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int t = blockIdx.x; t < nitems && alive; t += G) {
       const SddItem it = args.items[t];
       const int nst = (it.cnt + S - 1) / S;  // stacks in this item
-      const uint32_t tx = static_cast<uint32_t>(nst * S + 1) * BOX_BYTES;
+      const uint32_t tx = static_cast<uint32_t>(nst * S + (Q8 ? 0 : 1)) * BOX_BYTES;
       // lane l < nst*S: block-row of item slot l (the last block repeated)
       int row = 0;
       if (lane < nst * S) {
@@ -261,7 +289,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         ptx::mbar_expect_tx_if(lane == 0 ? 1u : 0u, &full[sidx], tx);
         ptx::tma_load_2d_if(lane < nst * S ? 1u : 0u, st + lane * BOX_BYTES, &tmap_dy, row * BS, y, &full[sidx],
                             pol_dy);
-        ptx::tma_load_2d_if(lane == 31 ? 1u : 0u, st + SU * BOX_BYTES, &tmap_x, it.col * BS, y, &full[sidx], pol_x);
+        if constexpr (!Q8)
+          ptx::tma_load_2d_if(lane == 31 ? 1u : 0u, st + SU * BOX_BYTES, &tmap_x, it.col * BS, y, &full[sidx], pol_x);
         __syncwarp();
         ptx::mbar_arrive_if(lane == 0 ? 1u : 0u, &full[sidx]);
         if (++sidx == ST) {
@@ -287,37 +316,42 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool alive = true;
     for (int t = blockIdx.x; t < nitems && alive; t += G) {
       const int nst = (args.items[t].cnt + S - 1) / S;
-      int ok = ptx::wait_parity(&tempty[slot], aphase ^ 1u, abort_flag, args.err, kTagTmemEmpty, kWaitCycles);
-      ok = __shfl_sync(0xffffffffu, ok, 0);
-      if (!ok) break;
-      ptx::tc_fence_after();
-      const uint32_t d = tmem_base + static_cast<uint32_t>(slot) * SET_COLS;
-      for (int slab = 0; slab < nslabs; ++slab) {
-        ok = ptx::wait_parity(&full[sidx], sph, abort_flag, args.err, kTagFull, kWaitCycles);
+      for (int s0 = 0; s0 < nslabs; s0 += seg) {
+        int ok = ptx::wait_parity(&tempty[slot], aphase ^ 1u, abort_flag, args.err, kTagTmemEmpty, kWaitCycles);
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) {
           alive = false;
           break;
         }
-        const uint32_t s16 = static_cast<uint32_t>(sidx) * STAGE16;
-        for (int u = 0; u < nst; ++u) {
-          const uint32_t u16 = static_cast<uint32_t>(u * S * BOX_BYTES) >> 4;
+        ptx::tc_fence_after();
+        const uint32_t d = tmem_base + static_cast<uint32_t>(slot) * SET_COLS;
+        for (int slab = s0; slab < min(nslabs, s0 + seg); ++slab) {
+          ok = ptx::wait_parity(&full[sidx], sph, abort_flag, args.err, kTagFull, kWaitCycles);
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+          if (!ok) {
+            alive = false;
+            break;
+          }
+          const uint32_t s16 = static_cast<uint32_t>(sidx) * STAGE16;
+          for (int u = 0; u < nst; ++u) {
+            const uint32_t u16 = static_cast<uint32_t>(u * S * BOX_BYTES) >> 4;
 #pragma unroll
-          for (int kk = 0; kk < KB / 16; ++kk) {
-            ptx::mma_f16_ss_if(leader, d + static_cast<uint32_t>(u * BS), a_lo0 + s16 + u16 + kk * KSTEP16, a_hi,
-                               b_lo0 + s16 + kk * KSTEP16, b_hi, IDESC, (slab > 0 || kk > 0) ? 1u : 0u);
+            for (int kk = 0; kk < KB / 16; ++kk) {
+              ptx::mma_f16_ss_if(leader, d + static_cast<uint32_t>(u * BS), a_lo0 + s16 + u16 + kk * KSTEP16, a_hi,
+                                 b_lo0 + s16 + kk * KSTEP16, b_hi, IDESC, (slab > s0 || kk > 0) ? 1u : 0u);
+            }
+          }
+          ptx::mma_commit_if(leader, &empty[sidx]);
+          if (++sidx == ST) {
+            sidx = 0;
+            sph ^= 1u;
           }
         }
-        ptx::mma_commit_if(leader, &empty[sidx]);
-        if (++sidx == ST) {
-          sidx = 0;
-          sph ^= 1u;
-        }
+        if (!alive) break;
+        ptx::mma_commit_if(leader, &tfull[slot]);
+        slot ^= SEGMENTS ? 0 : 1;
+        if (slot == 0) aphase ^= 1u;
       }
-      if (!alive) break;
-      ptx::mma_commit_if(leader, &tfull[slot]);
-      slot ^= 1;
-      if (slot == 0) aphase ^= 1u;
     }
     ptx::mma_commit_if(leader, mma_done);
     int dummy = 0;
@@ -331,36 +365,124 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_addr = static_cast<uint32_t>(qtr * 32) << 16;
     int slot = 0;
     uint32_t aphase = 0;
-    for (int t = blockIdx.x; t < nitems; t += G) {
+    bool alive = true;
+    for (int t = blockIdx.x; t < nitems && alive; t += G) {
       const SddItem it = args.items[t];
-      int ok = ptx::wait_parity(&tfull[slot], aphase, abort_flag, args.err, kTagTmemFull, kWaitCycles, 200);
-      ok = __shfl_sync(0xffffffffu, ok, 0);
-      if (epi_any(!ok)) break;
-      ptx::tc_fence_after();
-      const int nst = (it.cnt + S - 1) / S;
-      for (int u = 0; u < nst; ++u) {
-        const int bi = u * S + sslot;  // block of the item in this lane's TMEM rows
-        int p = -1;
-        if (bi < it.cnt) {
-          const int q = it.q0 + bi;
-          p = (q >= 0 && q < args.nnzb) ? __ldg(args.perm_t + q) : -1;
-          if (p >= args.nnzb) p = -1;
+      for (int s0 = 0; s0 < nslabs; s0 += seg) {
+        int ok = ptx::wait_parity(&tfull[slot], aphase, abort_flag, args.err, kTagTmemFull, kWaitCycles, 200);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (epi_any(!ok)) {
+          alive = false;
+          break;
         }
-        TOut* dst = p >= 0 ? static_cast<TOut*>(args.dblocks) + (static_cast<int64_t>(p) * BS + r) * BS : nullptr;
-        const uint32_t cols = static_cast<uint32_t>(slot) * SET_COLS + static_cast<uint32_t>(u * BS);
+        ptx::tc_fence_after();
+        const int nst = (it.cnt + S - 1) / S;
+        for (int u = 0; u < nst; ++u) {
+          const int bi = u * S + sslot;  // block of the item in this lane's TMEM rows
+          int p = -1;
+          if (bi < it.cnt) {
+            const int q = it.q0 + bi;
+            p = (q >= 0 && q < args.nnzb) ? __ldg(args.perm_t + q) : -1;
+            if (p >= args.nnzb) p = -1;
+          }
+          TOut* dst = p >= 0 ? static_cast<TOut*>(args.dblocks) + (static_cast<int64_t>(p) * BS + r) * BS : nullptr;
+          const uint32_t cols = static_cast<uint32_t>(slot) * SET_COLS + static_cast<uint32_t>(u * BS);
+          const bool last = s0 + seg >= nslabs;
 #pragma unroll
-        for (int c0 = 0; c0 < BS; c0 += 16) {
-          float v[16];
-          ptx::tmem_ld16(tmem_base + lane_addr + cols + static_cast<uint32_t>(c0), v);
-          ptx::tmem_wait_ld();
-          if (dst) store_row16<TOut>(dst + c0, v);
+          for (int c0 = 0; c0 < BS; c0 += 16) {
+            float v[16];
+            ptx::tmem_ld16(tmem_base + lane_addr + cols + static_cast<uint32_t>(c0), v);
+            if constexpr (SEGMENTS) {
+              // the running sum stands in the other accumulator set
+              const uint32_t total = tmem_base + lane_addr + SET_COLS + static_cast<uint32_t>(u * BS + c0);
+              if (s0 > 0) {
+                float w[16];
+                ptx::tmem_ld16(total, w);
+                ptx::tmem_wait_ld();
+#pragma unroll
+                for (int q = 0; q < 16; ++q) v[q] += w[q];
+              } else {
+                ptx::tmem_wait_ld();
+              }
+              if (!last) ptx::tmem_st16(total, v);
+            } else {
+              ptx::tmem_wait_ld();
+            }
+            if (dst && last) store_row16<TOut>(dst + c0, v);
+          }
+        }
+        if constexpr (SEGMENTS) ptx::tmem_wait_st();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&tempty[slot]);
+        slot ^= SEGMENTS ? 0 : 1;
+        if (slot == 0) aphase ^= 1u;
+      }
+    }
+  } else if (Q8 && warp >= 6) {
+    // ------------------------------------------------------------ X from 8 bits
+    using T = typename std::conditional<IN_FMT == 0, __half, __nv_bfloat16>::type;
+    const int ct = threadIdx.x - kThreads;  // 0..127: row ct / 2 of the slab, half ct % 2 of its 64 columns
+    const int row = ct >> 1, half = ct & 1;
+    struct Codes {
+      uint4 q[2];
+      float step;
+      int left;  // columns of this half that exist
+    };
+    // Slabs of this CTA in order; `look` runs two ahead of the one written.
+    int lt = blockIdx.x, lslab = 0;
+    auto look = [&]() {
+      Codes c;
+      c.q[0] = c.q[1] = make_uint4(0u, 0u, 0u, 0u);
+      c.step = 0.f;
+      c.left = 32;
+      if (lt >= nitems) return c;
+      const int64_t col = static_cast<int64_t>(args.items[lt].col) * BS + half * 32;
+      const int64_t r = static_cast<int64_t>(lslab) * KB + row;
+      c.left = static_cast<int>(min(static_cast<int64_t>(32), max(static_cast<int64_t>(0), args.k - col)));
+      if (r < args.n && c.left > 0) {
+        const int8_t* p = args.codes + r * args.ldq + col;
+        c.q[0] = __ldg(reinterpret_cast<const uint4*>(p));
+        if (c.left > 16) c.q[1] = __ldg(reinterpret_cast<const uint4*>(p + 16));  // rows are padded to 16 codes
+        c.step = __ldg(args.steps + (col >> 6) * args.lds + r);
+      }
+      if (++lslab == nslabs) {
+        lslab = 0;
+        lt += G;
+      }
+      return c;
+    };
+    Codes ahead[2] = {look(), look()};
+    int sidx = 0;
+    uint32_t sph = 0;
+    bool alive = true;
+    for (int t = blockIdx.x; t < nitems && alive; t += G) {
+      for (int slab = 0; slab < nslabs; ++slab) {
+        const Codes c = ahead[0];
+        ahead[0] = ahead[1];
+        ahead[1] = look();
+        int ok = ptx::wait_parity(&empty[sidx], sph ^ 1u, abort_flag, args.err, kTagEmpty, kWaitCycles);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) {
+          alive = false;
+          break;
+        }
+        uint8_t* box = smem + sidx * STAGE_BYTES + SU * BOX_BYTES + row * 128;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // 8 columns each
+          uint4 w = read_back<T>(i & 1 ? make_uint2(c.q[i >> 1].z, c.q[i >> 1].w)
+                                       : make_uint2(c.q[i >> 1].x, c.q[i >> 1].y), c.step);
+          if (c.left < 8 * (i + 1)) w = keep_first(w, c.left - 8 * i);  // columns behind the last are zero
+          *reinterpret_cast<uint4*>(box + (((half * 4 + i) ^ (row & 7)) * 16)) = w;
+        }
+        ptx::fence_async_smem();
+        __syncwarp();
+        ptx::mbar_arrive_if(lane == 0 ? 1u : 0u, &full[sidx]);
+        if (++sidx == ST) {
+          sidx = 0;
+          sph ^= 1u;
         }
       }
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&tempty[slot]);
-      slot ^= 1;
-      if (slot == 0) aphase ^= 1u;
     }
   }
 
@@ -379,12 +501,32 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// X of the CUDA-core kernel: in its own type, or in 8 bits.
+template <typename TIn>
+struct DenseX {
+  const TIn* x;
+  int64_t ldx;
+  __device__ __forceinline__ float operator()(int64_t row, int64_t col) const {
+    return static_cast<float>(x[row * ldx + col]);
+  }
+};
+template <typename TIn>
+struct CodesX {
+  const int8_t* codes;
+  const float* steps;
+  int64_t ldq, lds;
+  __device__ __forceinline__ float operator()(int64_t row, int64_t col) const {
+    const float v = __fmul_rn(static_cast<float>(codes[row * ldq + col]), steps[(col >> 6) * lds + row]);
+    return to_f32<TIn>(from_f32<TIn>(v));
+  }
+};
+
 // CUDA-core kernel for every shape: one CTA per transposed position q
 // computes dW[perm_t[q]] (bm x bk) over the batch in slabs of 32 rows staged
 // in shared memory; each thread owns (bm * bk) / 256 outputs.
-template <typename TIn, typename TOut>
+template <typename TIn, typename TOut, typename X>
 __global__ void __launch_bounds__(256) bsr_sddmm_simt_kernel(
-    const TIn* __restrict__ dy, int64_t lddy, const TIn* __restrict__ x, int64_t ldx, int64_t n, int64_t m, int64_t k,
+    const TIn* __restrict__ dy, int64_t lddy, const X x, int64_t n, int64_t m, int64_t k,
     const int32_t* __restrict__ col_idx, const int32_t* __restrict__ col_idx_t, const int32_t* __restrict__ perm_t,
     int32_t nnzb, int32_t nbr, int32_t nbc, int32_t bm, int32_t bk, TOut* __restrict__ dblocks, unsigned* err) {
   __shared__ float sdy[32][65];
@@ -412,7 +554,7 @@ __global__ void __launch_bounds__(256) bsr_sddmm_simt_kernel(
       for (int e = threadIdx.x; e < 32 * bk; e += blockDim.x) {
         const int rr = e / bk, c = e - rr * bk;
         const int64_t row = n0 + rr, col = static_cast<int64_t>(j) * bk + c;
-        sx[rr][c] = (row < n && col < k) ? static_cast<float>(x[row * ldx + col]) : 0.f;
+        sx[rr][c] = (row < n && col < k) ? x(row, col) : 0.f;
       }
       __syncthreads();
 #pragma unroll
@@ -435,15 +577,28 @@ __global__ void __launch_bounds__(256) bsr_sddmm_simt_kernel(
   }
 }
 
+// The activation of one call: in W's type (x), or in 8 bits (codes, steps).
+struct SddX {
+  const void* x;
+  int64_t ldx;
+  const int8_t* codes;
+  int64_t ldq;
+  const float* steps;
+  int64_t lds;
+};
+
 template <typename TIn, typename TOut>
 kairo_status launch_simt(const kairo_bsr* a, const int32_t* col_idx_t, const int32_t* perm_t, const void* dy,
-                         int64_t lddy, const void* x, int64_t ldx, int64_t n, void* dblocks, unsigned* err,
-                         cudaStream_t s) {
+                         int64_t lddy, const SddX& x, int64_t n, void* dblocks, unsigned* err, cudaStream_t s) {
   const int nbc = static_cast<int>(ceil_div64(a->cols, a->bk));
   const int g = static_cast<int>(std::min<int64_t>(a->nnzb, static_cast<int64_t>(device_sm_count(current_device())) * 8));
-  bsr_sddmm_simt_kernel<TIn, TOut><<<g, 256, 0, s>>>(
-      static_cast<const TIn*>(dy), lddy, static_cast<const TIn*>(x), ldx, n, a->rows, a->cols, a->col_idx, col_idx_t,
-      perm_t, static_cast<int32_t>(a->nnzb), a->nbr, nbc, a->bm, a->bk, static_cast<TOut*>(dblocks), err);
+  auto go = [&](auto src) {
+    bsr_sddmm_simt_kernel<TIn, TOut><<<g, 256, 0, s>>>(
+        static_cast<const TIn*>(dy), lddy, src, n, a->rows, a->cols, a->col_idx, col_idx_t, perm_t,
+        static_cast<int32_t>(a->nnzb), a->nbr, nbc, a->bm, a->bk, static_cast<TOut*>(dblocks), err);
+  };
+  if (x.codes) go(CodesX<TIn>{x.codes, x.steps, x.ldq, x.lds});
+  else go(DenseX<TIn>{static_cast<const TIn*>(x.x), x.ldx});
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "launch of the CUDA-core SDDMM kernel");
   return KAIRO_STATUS_SUCCESS;
@@ -451,23 +606,24 @@ kairo_status launch_simt(const kairo_bsr* a, const int32_t* col_idx_t, const int
 
 using SddFn = void (*)(CUtensorMap, CUtensorMap, SddArgs);
 
+template <bool Q8>
 SddFn pick_sdd(kairo_dtype in, kairo_dtype out) {
   if (in == KAIRO_DTYPE_F16) {
-    if (out == KAIRO_DTYPE_F32) return reinterpret_cast<SddFn>(&bsr_sddmm_tc_kernel<0, float>);
-    if (out == KAIRO_DTYPE_F16) return reinterpret_cast<SddFn>(&bsr_sddmm_tc_kernel<0, __half>);
+    if (out == KAIRO_DTYPE_F32) return reinterpret_cast<SddFn>(&bsr_sddmm_tc_kernel<0, float, Q8>);
+    if (out == KAIRO_DTYPE_F16) return reinterpret_cast<SddFn>(&bsr_sddmm_tc_kernel<0, __half, Q8>);
   } else if (in == KAIRO_DTYPE_BF16) {
-    if (out == KAIRO_DTYPE_F32) return reinterpret_cast<SddFn>(&bsr_sddmm_tc_kernel<1, float>);
-    if (out == KAIRO_DTYPE_BF16) return reinterpret_cast<SddFn>(&bsr_sddmm_tc_kernel<1, __nv_bfloat16>);
+    if (out == KAIRO_DTYPE_F32) return reinterpret_cast<SddFn>(&bsr_sddmm_tc_kernel<1, float, Q8>);
+    if (out == KAIRO_DTYPE_BF16) return reinterpret_cast<SddFn>(&bsr_sddmm_tc_kernel<1, __nv_bfloat16, Q8>);
   }
   return nullptr;
 }
 
-bool sdd_tc_ok(const kairo_bsr* a, const void* dy, int64_t lddy, const void* x, int64_t ldx, kairo_dtype out) {
+bool sdd_tc_ok(const kairo_bsr* a, const void* dy, int64_t lddy, const SddX& x, kairo_dtype out) {
   if (a->bm != 64 || a->bk != 64) return false;
-  if (!pick_sdd(a->dtype, out)) return false;
-  if ((lddy % 8) || (ldx % 8)) return false;
-  if ((reinterpret_cast<uintptr_t>(dy) & 15u) || (reinterpret_cast<uintptr_t>(x) & 15u)) return false;
-  return true;
+  if (!pick_sdd<false>(a->dtype, out)) return false;
+  if ((lddy % 8) || (reinterpret_cast<uintptr_t>(dy) & 15u)) return false;
+  if (x.codes) return true;  // their rows are 16-byte aligned
+  return x.ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x.x) & 15u) == 0;
 }
 
 }  // namespace
@@ -501,11 +657,13 @@ extern "C" kairo_status kairo_bsr_sddmm_workspace_size(const kairo_bsr* a, size_
   return KAIRO_STATUS_SUCCESS;
 }
 
-extern "C" kairo_status kairo_bsr_sddmm(const kairo_bsr* a, const int32_t* row_ptr_t, const int32_t* col_idx_t,
-                                        const int32_t* perm_t, const void* dy, int64_t lddy, const void* x,
-                                        int64_t ldx, int64_t n, void* dblocks, kairo_dtype out_dtype,
-                                        void* workspace, size_t workspace_bytes, void* stream) {
-  kairo_status st = sddmm_check(a, row_ptr_t, col_idx_t, perm_t, dy, lddy, x, ldx, n, dblocks, out_dtype, workspace);
+namespace {
+
+kairo_status run_sddmm(const kairo_bsr* a, const int32_t* row_ptr_t, const int32_t* col_idx_t, const int32_t* perm_t,
+                       const void* dy, int64_t lddy, const SddX& x, int64_t n, void* dblocks, kairo_dtype out_dtype,
+                       void* workspace, size_t workspace_bytes, void* stream) {
+  kairo_status st = sddmm_check(a, row_ptr_t, col_idx_t, perm_t, dy, lddy, x.codes ? x.codes : x.x,
+                                x.codes ? a->cols : x.ldx, n, dblocks, out_dtype, workspace);
   if (st) return st;
   if (a->nnzb == 0) return KAIRO_STATUS_SUCCESS;
   size_t need = 0;
@@ -522,20 +680,20 @@ extern "C" kairo_status kairo_bsr_sddmm(const kairo_bsr* a, const int32_t* row_p
     if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync(dW)");
     return KAIRO_STATUS_SUCCESS;
   }
-  const bool tc = sdd_tc_ok(a, dy, lddy, x, ldx, out_dtype) && n <= 0x7fffffffLL && a->rows <= 0x7fffffffLL &&
+  const bool tc = sdd_tc_ok(a, dy, lddy, x, out_dtype) && n <= 0x7fffffffLL && a->rows <= 0x7fffffffLL &&
                   a->cols <= 0x7fffffffLL;
   if (!tc) {
     switch (a->dtype) {
       case KAIRO_DTYPE_F32:
-        return launch_simt<float, float>(a, col_idx_t, perm_t, dy, lddy, x, ldx, n, dblocks, w.err, s);
+        return launch_simt<float, float>(a, col_idx_t, perm_t, dy, lddy, x, n, dblocks, w.err, s);
       case KAIRO_DTYPE_F16:
         return out_dtype == KAIRO_DTYPE_F32
-                   ? launch_simt<__half, float>(a, col_idx_t, perm_t, dy, lddy, x, ldx, n, dblocks, w.err, s)
-                   : launch_simt<__half, __half>(a, col_idx_t, perm_t, dy, lddy, x, ldx, n, dblocks, w.err, s);
+                   ? launch_simt<__half, float>(a, col_idx_t, perm_t, dy, lddy, x, n, dblocks, w.err, s)
+                   : launch_simt<__half, __half>(a, col_idx_t, perm_t, dy, lddy, x, n, dblocks, w.err, s);
       default:
         return out_dtype == KAIRO_DTYPE_F32
-                   ? launch_simt<__nv_bfloat16, float>(a, col_idx_t, perm_t, dy, lddy, x, ldx, n, dblocks, w.err, s)
-                   : launch_simt<__nv_bfloat16, __nv_bfloat16>(a, col_idx_t, perm_t, dy, lddy, x, ldx, n, dblocks,
+                   ? launch_simt<__nv_bfloat16, float>(a, col_idx_t, perm_t, dy, lddy, x, n, dblocks, w.err, s)
+                   : launch_simt<__nv_bfloat16, __nv_bfloat16>(a, col_idx_t, perm_t, dy, lddy, x, n, dblocks,
                                                                w.err, s);
     }
   }
@@ -549,9 +707,13 @@ extern "C" kairo_status kairo_bsr_sddmm(const kairo_bsr* a, const int32_t* row_p
   st = make_map_2d(&map_dy, dy, dt, 2, static_cast<uint64_t>(a->rows), static_cast<uint64_t>(n),
                    static_cast<uint64_t>(lddy), 64, kSddKB, "dY");
   if (st) return st;
-  st = make_map_2d(&map_x, x, dt, 2, static_cast<uint64_t>(a->cols), static_cast<uint64_t>(n),
-                   static_cast<uint64_t>(ldx), 64, kSddKB, "X");
-  if (st) return st;
+  if (x.codes) {
+    map_x = map_dy;  // not used
+  } else {
+    st = make_map_2d(&map_x, x.x, dt, 2, static_cast<uint64_t>(a->cols), static_cast<uint64_t>(n),
+                     static_cast<uint64_t>(x.ldx), 64, kSddKB, "X");
+    if (st) return st;
+  }
   constexpr int stage_bytes = (2 * kSddU + 1) * 64 * kSddKB * 2;
   const int budget = kMaxSmem - 1024 - 1024;
   const int stages = std::min(8, budget / stage_bytes);
@@ -566,15 +728,43 @@ extern "C" kairo_status kairo_bsr_sddmm(const kairo_bsr* a, const int32_t* row_p
   args.nbr = a->nbr;
   args.nnzb = static_cast<int32_t>(a->nnzb);
   args.stages = stages;
-  SddFn fn = pick_sdd(a->dtype, out_dtype);
+  args.codes = x.codes;
+  args.steps = x.steps;
+  args.ldq = x.ldq;
+  args.lds = x.lds;
+  args.k = static_cast<int32_t>(a->cols);
+  SddFn fn = x.codes ? pick_sdd<true>(a->dtype, out_dtype) : pick_sdd<false>(a->dtype, out_dtype);
   const size_t smem = static_cast<size_t>(stages) * stage_bytes + 2048;
   e = cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(smem));
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic smem)");
   const int64_t max_items = a->nnzb / (2 * kSddU) + nbc;
   const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(device_sm_count(current_device()), max_items)));
-  fn<<<grid, kThreads, smem, s>>>(map_dy, map_x, args);
+  fn<<<grid, kThreads + (x.codes ? 32 * kSddConvert : 0), smem, s>>>(map_dy, map_x, args);
   e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "launch of the tcgen05 SDDMM kernel");
   return KAIRO_STATUS_SUCCESS;
+}
+
+}  // namespace
+
+extern "C" kairo_status kairo_bsr_sddmm(const kairo_bsr* a, const int32_t* row_ptr_t, const int32_t* col_idx_t,
+                                        const int32_t* perm_t, const void* dy, int64_t lddy, const void* x,
+                                        int64_t ldx, int64_t n, void* dblocks, kairo_dtype out_dtype,
+                                        void* workspace, size_t workspace_bytes, void* stream) {
+  return run_sddmm(a, row_ptr_t, col_idx_t, perm_t, dy, lddy, SddX{x, ldx, nullptr, 0, nullptr, 0}, n, dblocks,
+                   out_dtype, workspace, workspace_bytes, stream);
+}
+
+extern "C" kairo_status kairo_bsr_sddmm_q8(const kairo_bsr* a, const int32_t* row_ptr_t, const int32_t* col_idx_t,
+                                           const int32_t* perm_t, const void* dy, int64_t lddy, const int8_t* codes,
+                                           int64_t ldq, const float* steps, int64_t lds, int64_t n, void* dblocks,
+                                           kairo_dtype out_dtype, void* workspace, size_t workspace_bytes,
+                                           void* stream) {
+  if (!a) return fail(KAIRO_STATUS_INVALID_VALUE, "null BSR descriptor");
+  kairo_status st = q8_check(n, a->cols, codes, ldq, steps, lds);
+  if (st) return st;
+  if (!codes) ldq = 0;  // an empty batch
+  return run_sddmm(a, row_ptr_t, col_idx_t, perm_t, dy, lddy, SddX{nullptr, a->cols, codes, ldq, steps, lds}, n,
+                   dblocks, out_dtype, workspace, workspace_bytes, stream);
 }

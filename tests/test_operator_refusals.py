@@ -118,7 +118,7 @@ def test_checkpoint_c_refusals():
                    {"ldq": 72}, {"steps": None}, {"lds": 2}, {"codes": ctypes.c_void_p(264)}):
             assert fn(**kw) == _lib.INVALID_VALUE, kw
         assert fn(n=0) == _lib.SUCCESS and fn(k=0) == _lib.SUCCESS
-        assert fn(k=1 << 26, ldx=1 << 26, ldq=1 << 26) == _lib.NOT_SUPPORTED
+        assert fn(k=1 << 28, ldx=1 << 28, ldq=1 << 28) == _lib.NOT_SUPPORTED
     n = ctypes.c_size_t(0)
     d = _lib.KairoBsr(rows=64, cols=64, bm=64, bk=64, nbr=1, nnzb=1, nblocks_stored=1, dtype=_lib.DTYPE_BF16)
     d.col_idx = 256
