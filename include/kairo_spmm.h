@@ -485,12 +485,13 @@ KAIRO_API kairo_status kairo_sparse_scatter_grad_workspace_size(int64_t nactive,
  *                           token of each.  Ids outside [0, n_rows) are written
  *                           as n_rows, at the end.
  *   kairo_embedding_grad    grad_weight (n_rows, dim; leading dimension ldo)
- *                           row r = scale * the sum of grad_output's rows
- *                           perm[q] with sorted[q] == r, zero where there is
- *                           none.  With accumulate != 0 the sums are added to
+ *                           row r = scale * the sum of grad_output's rows t
+ *                           with ids[t] == r, zero where there is none.  With accumulate != 0 the sums are added to
  *                           what grad_weight holds and other rows are not
  *                           touched.  fp32 sums in an order fixed by the ids,
  *                           no atomics; one rounding to out_dtype.
+ *   kairo_embedding_grad_sorted  the same from the result of kairo_token_sort
+ *                           (and a workspace of the same size).
  * dtype and out_dtype f32, f16 or bf16, in any combination; n_rows and nids
  * below 2^31 - 4096.  All asynchronous on `stream`; the workspaces need no
  * initial value.
@@ -502,11 +503,15 @@ KAIRO_API kairo_status kairo_token_sort(const void* ids, int32_t id_bytes, int64
                                         int32_t* sorted, int32_t* perm, void* workspace, size_t workspace_bytes,
                                         void* stream);
 KAIRO_API kairo_status kairo_token_sort_workspace_size(int64_t nids, int64_t n_rows, size_t* bytes);
-KAIRO_API kairo_status kairo_embedding_grad(const void* grad_output, int64_t ldg, kairo_dtype dtype,
-                                            const int32_t* sorted, const int32_t* perm, int64_t nids, int64_t n_rows,
-                                            int64_t dim, float scale, void* grad_weight, int64_t ldo,
-                                            kairo_dtype out_dtype, int32_t accumulate, void* workspace,
-                                            size_t workspace_bytes, void* stream);
+KAIRO_API kairo_status kairo_embedding_grad(const void* grad_output, int64_t ldg, kairo_dtype dtype, const void* ids,
+                                            int32_t id_bytes, int64_t nids, int64_t n_rows, int64_t dim, float scale,
+                                            void* grad_weight, int64_t ldo, kairo_dtype out_dtype, int32_t accumulate,
+                                            void* workspace, size_t workspace_bytes, void* stream);
+KAIRO_API kairo_status kairo_embedding_grad_sorted(const void* grad_output, int64_t ldg, kairo_dtype dtype,
+                                                   const int32_t* sorted, const int32_t* perm, int64_t nids,
+                                                   int64_t n_rows, int64_t dim, float scale, void* grad_weight,
+                                                   int64_t ldo, kairo_dtype out_dtype, int32_t accumulate,
+                                                   void* workspace, size_t workspace_bytes, void* stream);
 KAIRO_API kairo_status kairo_embedding_grad_workspace_size(int64_t nids, int64_t dim, size_t* bytes);
 
 /* ------------------------------------------------------------------------

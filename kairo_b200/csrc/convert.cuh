@@ -52,20 +52,29 @@ struct Pack {
   __device__ __forceinline__ Pack() {}
 };
 
+// N elements at p, in pieces of up to 16 bytes; p is aligned to a piece.
 template <typename T, int N>
 __device__ __forceinline__ void load_f32(const T* p, float (&f)[N]) {
-  Pack<T, N> k;
-  k.raw = *reinterpret_cast<const decltype(k.raw)*>(p);
+  constexpr int P = N * static_cast<int>(sizeof(T)) > 16 ? 16 / static_cast<int>(sizeof(T)) : N;
 #pragma unroll
-  for (int i = 0; i < N; ++i) f[i] = to_f32<T>(k.v[i]);
+  for (int q = 0; q < N; q += P) {
+    Pack<T, P> k;
+    k.raw = *reinterpret_cast<const decltype(k.raw)*>(p + q);
+#pragma unroll
+    for (int i = 0; i < P; ++i) f[q + i] = to_f32<T>(k.v[i]);
+  }
 }
 
 template <typename T, int N>
 __device__ __forceinline__ void store_f32(T* p, const float (&f)[N]) {
-  Pack<T, N> k;
+  constexpr int P = N * static_cast<int>(sizeof(T)) > 16 ? 16 / static_cast<int>(sizeof(T)) : N;
 #pragma unroll
-  for (int i = 0; i < N; ++i) k.v[i] = from_f32<T>(f[i]);
-  *reinterpret_cast<decltype(k.raw)*>(p) = k.raw;
+  for (int q = 0; q < N; q += P) {
+    Pack<T, P> k;
+#pragma unroll
+    for (int i = 0; i < P; ++i) k.v[i] = from_f32<T>(f[q + i]);
+    *reinterpret_cast<decltype(k.raw)*>(p + q) = k.raw;
+  }
 }
 
 inline int element_bytes(kairo_dtype d) { return d == KAIRO_DTYPE_F32 ? 4 : 2; }

@@ -3,8 +3,10 @@
 // lookup  out[t, :] = scale * weight[id_t, :], one rounding; a zero row for
 //         an id outside [0, n_rows).
 // sort    the token positions ordered by id, equal ids in token order (an
-//         LSD radix sort of 8 bits a pass: counts per tile, one scan, a stable
-//         scatter).  Ids outside [0, n_rows) become n_rows and end up last.
+//         LSD radix sort).  Ids outside [0, n_rows) become n_rows and end up
+//         last.  Up to 65536 tokens are sorted by one cluster in one launch,
+//         keys and positions staying in its distributed shared memory between
+//         the passes; longer lists take three launches a pass.
 // grad    grad_weight[r, :] = scale * sum of grad_output[t, :] over id_t == r.
 //         The sorted positions are cut into chunks of equal length whatever
 //         the ids, so that a frequent token costs no more time than rare ones.
@@ -13,11 +15,13 @@
 //         the head and the tail of a run that crosses chunks go to fp32
 //         partial rows, which a second kernel adds up in chunk order.  All
 //         sums are fp32 in an order that depends on the ids alone, so that
-//         equal calls give equal bits.
+//         equal calls give equal bits.  Rows without tokens are zeroed by
+//         further CTAs of the first kernel, so that every row is written once.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "convert.cuh"
 #include "internal.h"
@@ -70,6 +74,19 @@ template <typename ID>
 __device__ __forceinline__ uint32_t token_key(const ID* ids, int64_t i, int64_t n_rows) {
   const int64_t id = static_cast<int64_t>(ids[i]);
   return static_cast<uint32_t>((id >= 0 && id < n_rows) ? id : n_rows);
+}
+
+// Lanes that hold the same `bits`-bit digit as this one, among those with ok.  A
+// vote per bit: the warp's match instruction takes some 500 cycles when the
+// digits differ (32768 tokens of 131072 rows: 26.4 us, with votes 22.6).
+__device__ __forceinline__ uint32_t same_digit(uint32_t d, bool ok, int bits) {
+  uint32_t same = __ballot_sync(0xffffffffu, ok);
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (d >> b) & 1u;
+    const uint32_t vote = __ballot_sync(0xffffffffu, one);
+    same &= one ? vote : ~vote;
+  }
+  return same;
 }
 
 // Keys of the first pass come from the ids, later ones from the last pass.
@@ -151,10 +168,9 @@ __global__ void __launch_bounds__(kSortThreads) k_sort_scatter(
     const int64_t i = base + j * 32;
     const bool ok = i < n;
     key[j] = ok ? sort_key(ids, keys, i, n_rows) : 0u;
-    // keys past the end share a digit of their own that is never counted
-    const uint32_t d = ok ? (key[j] >> shift) & (kBins - 1) : kBins;
-    const uint32_t same = __match_any_sync(0xffffffffu, d);
-    const int leader = __ffs(same) - 1;
+    const uint32_t d = (key[j] >> shift) & (kBins - 1);
+    const uint32_t same = same_digit(d, ok, 8);
+    const int leader = ok ? __ffs(same) - 1 : lane;
     uint32_t first = 0;
     if (lane == leader && ok) {
       first = where[warp][d];
@@ -186,22 +202,208 @@ __global__ void __launch_bounds__(kSortThreads) k_sort_scatter(
   }
 }
 
-int sort_passes(int64_t n_rows) {
+int key_bits(int64_t n_rows) {  // of the keys 0 .. n_rows
   int bits = 1;
   while (bits < 31 && (int64_t(1) << bits) <= n_rows) ++bits;
-  return (bits + 7) / 8;
+  return bits;
+}
+
+int sort_passes(int64_t n_rows) { return (key_bits(n_rows) + 7) / 8; }
+
+// The whole sort in one cluster.  CTA c holds positions c * per ..; in a pass
+// every warp ranks its share of them in order, the digit counts of all CTAs
+// are read over distributed shared memory, and each key and position is stored
+// straight into the shared memory of the CTA that holds its place (the last
+// pass: into the result).  32768 tokens of 131072 rows, two passes of 9 bits:
+// 15 us, where three passes of three launches took 74.
+constexpr int kClusterThreads = 1024;
+constexpr int kClusterWarps = kClusterThreads / 32;
+constexpr int kClusterItems = 8;   // positions per thread at most
+constexpr int kClusterMax = 8;     // CTAs
+constexpr int kMaxDigit = 9;       // bits of a pass
+constexpr int kMaxBins = 1 << kMaxDigit;
+constexpr int64_t kClusterTokens = int64_t(kClusterMax) * kClusterItems * kClusterThreads;
+
+size_t cluster_sort_smem(int per) {
+  return static_cast<size_t>(per) * 16 + static_cast<size_t>(kClusterWarps * kMaxBins + 2 * kMaxBins + 64) * 4;
+}
+
+__device__ __forceinline__ uint32_t cta_of(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void all_ctas() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
+template <typename ID>
+__global__ void __launch_bounds__(kClusterThreads) k_sort_cluster(const ID* __restrict__ ids, int n, int64_t n_rows,
+                                                                  int per, int passes, int digit,
+                                                                  uint32_t* __restrict__ sorted,
+                                                                  int32_t* __restrict__ perm) {
+  extern __shared__ __align__(16) uint32_t sm[];
+  uint32_t* keys = sm;                              // [2][per]
+  uint32_t* vals = keys + 2 * per;                  // [2][per]
+  uint32_t* where = vals + 2 * per;                 // [kClusterWarps][bins]
+  uint32_t* total = where + kClusterWarps * kMaxBins;  // [bins]: this CTA's count of every digit
+  uint32_t* base = total + kMaxBins;                // [bins]: first place of this CTA's keys of a digit
+  uint32_t* sums = base + kMaxBins;                 // [32]
+  uint32_t crank, csize;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(crank));
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(csize));
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int bins = 1 << digit;
+  const int first = static_cast<int>(crank) * per;
+  const int share = per / kClusterWarps;            // consecutive positions of a warp
+  for (int i = threadIdx.x; i < per; i += kClusterThreads) {
+    const bool ok = first + i < n;
+    keys[i] = ok ? token_key(ids, first + i, n_rows) : 0u;
+    vals[i] = static_cast<uint32_t>(first + i);
+  }
+  for (int p = 0; p < passes; ++p) {
+    const int shift = p * digit;
+    const uint32_t* from_k = keys + (p & 1) * per;
+    const uint32_t* from_v = vals + (p & 1) * per;
+    for (int i = threadIdx.x; i < kClusterWarps * bins; i += kClusterThreads) where[i] = 0;
+    __syncthreads();
+    uint32_t key[kClusterItems], rank[kClusterItems];
+    uint32_t* mine = where + warp * bins;
+#pragma unroll
+    for (int j = 0; j < kClusterItems; ++j) {
+      if (j * 32 < share) {
+        const int i = warp * share + j * 32 + lane;
+        const bool ok = first + i < n;
+        key[j] = from_k[i];
+        const uint32_t d = (key[j] >> shift) & (bins - 1);
+        const uint32_t same = same_digit(d, ok, digit);
+        const int leader = ok ? __ffs(same) - 1 : lane;
+        uint32_t at = 0;
+        if (lane == leader && ok) {
+          at = mine[d];
+          mine[d] = at + __popc(same);
+        }
+        at = __shfl_sync(0xffffffffu, at, leader);
+        rank[j] = at + __popc(same & ((1u << lane) - 1u));
+        __syncwarp();
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x < bins) {
+      uint32_t at = 0;
+#pragma unroll 8
+      for (int w = 0; w < kClusterWarps; ++w) {
+        const uint32_t c = where[w * bins + threadIdx.x];
+        where[w * bins + threadIdx.x] = at;
+        at += c;
+      }
+      total[threadIdx.x] = at;
+    }
+    all_ctas();
+    // Keys of smaller digits anywhere, and of this digit in CTAs before this one.
+    uint32_t all = 0, before = 0;
+    if (threadIdx.x < bins) {
+      const uint32_t addr = static_cast<uint32_t>(__cvta_generic_to_shared(total + threadIdx.x));
+      uint32_t c[kClusterMax];
+#pragma unroll
+      for (uint32_t r = 0; r < kClusterMax; ++r) {
+        c[r] = 0;
+        if (r < csize) asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(c[r]) : "r"(cta_of(addr, r)));
+      }
+#pragma unroll
+      for (uint32_t r = 0; r < kClusterMax; ++r) {
+        all += c[r];
+        if (r < crank) before += c[r];
+      }
+    }
+    uint32_t x = all;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) sums[warp] = x;
+    __syncthreads();
+    if (warp == 0) {
+      uint32_t s = sums[lane];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += y;
+      }
+      sums[lane] = s;
+    }
+    __syncthreads();
+    if (threadIdx.x < bins) base[threadIdx.x] = x - all + (warp ? sums[warp - 1] : 0u) + before;
+    __syncthreads();
+    const bool last = p + 1 == passes;
+    const uint32_t to_k = static_cast<uint32_t>(__cvta_generic_to_shared(keys + ((p + 1) & 1) * per));
+    const uint32_t to_v = static_cast<uint32_t>(__cvta_generic_to_shared(vals + ((p + 1) & 1) * per));
+#pragma unroll
+    for (int j = 0; j < kClusterItems; ++j) {
+      if (j * 32 < share) {
+        const int i = warp * share + j * 32 + lane;
+        if (first + i < n) {
+          const uint32_t d = (key[j] >> shift) & (bins - 1);
+          const uint32_t at = base[d] + mine[d] + rank[j];
+          if (last) {
+            sorted[at] = key[j];
+            perm[at] = static_cast<int32_t>(from_v[i]);
+          } else {
+            const uint32_t cta = at / static_cast<uint32_t>(per), off = 4u * (at - cta * per);
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cta_of(to_k + off, cta)), "r"(key[j]) : "memory");
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cta_of(to_v + off, cta)), "r"(from_v[i]) : "memory");
+          }
+        }
+      }
+    }
+    all_ctas();  // the next pass reads what the others stored here
+  }
+}
+
+template <typename ID>
+kairo_status sort_in_cluster(const ID* ids, int64_t n, int64_t n_rows, uint32_t* sorted, int32_t* perm,
+                             cudaStream_t s) {
+  int ctas = 1;
+  while (ctas < kClusterMax && ctas * kClusterThreads < n) ctas *= 2;
+  const int per = static_cast<int>(ceil_div64(ceil_div64(n, ctas), kClusterThreads)) * kClusterThreads;
+  const int bits = key_bits(n_rows);
+  const int passes = (bits + kMaxDigit - 1) / kMaxDigit;
+  auto* fn = &k_sort_cluster<ID>;
+  const size_t smem = cluster_sort_smem(per);
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(cluster_sort_smem(kClusterItems * kClusterThreads)));
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(token sort)");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(kClusterThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = static_cast<unsigned>(ctas);
+  at.val.clusterDim.y = 1;
+  at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, fn, ids, static_cast<int>(n), n_rows, per, passes, (bits + passes - 1) / passes, sorted,
+                         perm);
+  if (e != cudaSuccess) return cuda_fail(e, "launch of the token sort");
+  return KAIRO_STATUS_SUCCESS;
 }
 
 int64_t sort_tiles(int64_t n) { return std::max<int64_t>(1, ceil_div64(n, kSortTile)); }
 
 // Workspace: one spare copy of keys and positions, then the counts.
 size_t sort_ws_bytes(int64_t n) {
+  if (n <= kClusterTokens) return 256;  // nothing: the cluster's shared memory holds it all
   return 2 * align_up(static_cast<size_t>(n) * 4, 256) + align_up(static_cast<size_t>(sort_tiles(n)) * kBins * 4, 256);
 }
 
 template <typename ID>
 kairo_status sort_launch(const ID* ids, int64_t n, int64_t n_rows, uint32_t* sorted, int32_t* perm, void* ws,
                          cudaStream_t s) {
+  if (n <= kClusterTokens) return sort_in_cluster(ids, n, n_rows, sorted, perm, s);
   const size_t col = align_up(static_cast<size_t>(n) * 4, 256);
   uint32_t* keys_b = static_cast<uint32_t*>(ws);
   int32_t* vals_b = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(ws) + col);
@@ -230,7 +432,9 @@ kairo_status sort_launch(const ID* ids, int64_t n, int64_t n_rows, uint32_t* sor
 // ------------------------------------------------------------------ gradient
 
 constexpr int kGradThreads = 128;
-constexpr int kGradChunk = 32;  // sorted positions per chunk
+constexpr int kGradChunk = 32;   // sorted positions per chunk
+constexpr int kGradAhead = 8;    // rows under way per thread
+constexpr int kZeroRows = 32;    // rows of a zeroing CTA
 
 template <typename TO, int VE>
 __device__ __forceinline__ void emit_row(TO* dst, float (&acc)[VE], float scale, bool accumulate) {
@@ -241,71 +445,256 @@ __device__ __forceinline__ void emit_row(TO* dst, float (&acc)[VE], float scale,
   store_f32<TO, VE>(dst, f);
 }
 
-template <int VE>
-__device__ __forceinline__ void store_partial(float* dst, const float (&acc)[VE]) {
+// Rows r0 .. r0 + 31: zeros where no token has the row's id.
+template <typename TO, int VE>
+__device__ __forceinline__ void zero_rows(const uint32_t* __restrict__ sorted, int64_t n, int64_t n_rows, int64_t dim,
+                                          TO* __restrict__ out, int64_t ldo, int64_t r0) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = r0 + lane;
+  int64_t lo = 0, hi = n;  // first position whose id is >= row
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (sorted[mid] < row) lo = mid + 1;
+    else hi = mid;
+  }
+  const bool empty = row < n_rows && !(lo < n && sorted[lo] == row);
+  const uint32_t mask = __ballot_sync(0xffffffffu, empty);
+  float zero[VE];
 #pragma unroll
-  for (int i = 0; i < VE; ++i) dst[i] = acc[i];
+  for (int i = 0; i < VE; ++i) zero[i] = 0.f;
+  for (int r = warp; r < kZeroRows; r += kGradThreads / 32) {
+    if (!((mask >> r) & 1u)) continue;
+    TO* dst = out + (r0 + r) * ldo;
+    for (int64_t c = static_cast<int64_t>(lane) * VE; c < dim; c += 32 * VE) store_f32<TO, VE>(dst + c, zero);
+  }
 }
 
-// Partial rows: 2 * chunk is the part of a run that began before the chunk,
-// 2 * chunk + 1 the part of a run that begins in it and goes on behind it.
+// CTAs 0 .. chunks * slices - 1: one chunk and one slice of the columns each;
+// those behind them zero the rows without tokens.  Partial rows: 2 * chunk is
+// the part of a run that began before the chunk, 2 * chunk + 1 the part of a
+// run that begins in it and goes on behind it.
 template <typename TI, typename TO, int VE>
 __global__ void __launch_bounds__(kGradThreads) k_grad_chunks(
     const TI* __restrict__ grad, int64_t ldg, const uint32_t* __restrict__ sorted, const int32_t* __restrict__ perm,
     int64_t n, int64_t n_rows, int64_t dim, float scale, TO* __restrict__ out, int64_t ldo, bool accumulate,
-    float* __restrict__ partial) {
-  const int64_t col = (static_cast<int64_t>(blockIdx.y) * kGradThreads + threadIdx.x) * VE;
+    float* __restrict__ partial, int64_t chunks, int slices) {
+  if (static_cast<int64_t>(blockIdx.x) >= chunks * slices) {
+    zero_rows<TO, VE>(sorted, n, n_rows, dim, out, ldo, (blockIdx.x - chunks * slices) * kZeroRows);
+    return;
+  }
+  // The chunk's ids with their neighbours on both sides (n_rows + 1: none), and its tokens.
+  __shared__ uint32_t key[kGradChunk + 2];
+  __shared__ int tok[kGradChunk];
+  const int64_t chunk = blockIdx.x / slices;
+  const int64_t p0 = chunk * kGradChunk;
+  if (threadIdx.x < kGradChunk + 2) {
+    const int64_t p = p0 + threadIdx.x - 1;
+    key[threadIdx.x] = p >= 0 && p < n ? sorted[p] : static_cast<uint32_t>(n_rows + 1);
+  } else if (threadIdx.x >= 64 && threadIdx.x < 64 + kGradChunk) {
+    const int64_t p = p0 + threadIdx.x - 64;
+    const int t = p < n ? perm[p] : -1;
+    tok[threadIdx.x - 64] = t < n ? t : -1;
+  }
+  __syncthreads();
+  const int64_t col = (static_cast<int64_t>(blockIdx.x - chunk * slices) * kGradThreads + threadIdx.x) * VE;
   if (col >= dim) return;
-  const int64_t chunk = blockIdx.x;
-  const int64_t p0 = chunk * kGradChunk, p1 = min(n, p0 + kGradChunk);
-  bool open_left = p0 > 0 && sorted[p0 - 1] == sorted[p0];
+  const int have = static_cast<int>(min(static_cast<int64_t>(kGradChunk), n - p0));
+  bool open_left = key[0] == key[1];
   float acc[VE];
 #pragma unroll
   for (int i = 0; i < VE; ++i) acc[i] = 0.f;
-  for (int64_t p = p0; p < p1; ++p) {
-    const uint32_t key = sorted[p];
-    if (key >= n_rows) break;  // ids out of range come last
-    const int32_t t = perm[p];
-    if (t < 0 || t >= n) break;  // not a permutation: read nothing
-    float f[VE];
-    load_f32<TI, VE>(grad + static_cast<int64_t>(t) * ldg + col, f);
+#pragma unroll 1
+  for (int q0 = 0; q0 < have; q0 += kGradAhead) {
+    float f[kGradAhead][VE];
 #pragma unroll
-    for (int i = 0; i < VE; ++i) acc[i] += f[i];
-    const bool last = p + 1 == n || sorted[p + 1] != key;
-    if (last || p + 1 == p1) {
-      if (open_left) store_partial<VE>(partial + (2 * chunk) * dim + col, acc);
-      else if (!last) store_partial<VE>(partial + (2 * chunk + 1) * dim + col, acc);
-      else emit_row<TO, VE>(out + static_cast<int64_t>(key) * ldo + col, acc, scale, accumulate);
-      open_left = false;
+    for (int u = 0; u < kGradAhead; ++u) {
+      const int q = q0 + u;
+      if (q < have && key[q + 1] < n_rows && tok[q] >= 0) {
+        load_f32<TI, VE>(grad + static_cast<int64_t>(tok[q]) * ldg + col, f[u]);
+      } else {
 #pragma unroll
-      for (int i = 0; i < VE; ++i) acc[i] = 0.f;
+        for (int i = 0; i < VE; ++i) f[u][i] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kGradAhead; ++u) {
+      const int q = q0 + u;
+      if (q >= have || key[q + 1] >= n_rows) break;  // ids out of range come last
+#pragma unroll
+      for (int i = 0; i < VE; ++i) acc[i] += f[u][i];
+      const bool last = key[q + 1] != key[q + 2];
+      if (last || q + 1 == have) {
+        if (open_left) store_f32<float, VE>(partial + (2 * chunk) * dim + col, acc);
+        else if (!last) store_f32<float, VE>(partial + (2 * chunk + 1) * dim + col, acc);
+        else emit_row<TO, VE>(out + static_cast<int64_t>(key[q + 1]) * ldo + col, acc, scale, accumulate);
+        open_left = false;
+#pragma unroll
+        for (int i = 0; i < VE; ++i) acc[i] = 0.f;
+      }
     }
   }
 }
 
 // The chunk in which a run begins that goes on behind it adds up the run's
-// parts in order.
+// parts: kJoinGroups groups of threads take turns of kGradAhead parts each, in
+// order, and their sums are added in the order of the groups.
+constexpr int kJoinGroups = 4;
 template <typename TO, int VE>
-__global__ void __launch_bounds__(kGradThreads) k_grad_join(const uint32_t* __restrict__ sorted, int64_t n,
-                                                            int64_t n_rows, int64_t dim, float scale,
-                                                            TO* __restrict__ out, int64_t ldo, bool accumulate,
-                                                            const float* __restrict__ partial) {
-  const int64_t col = (static_cast<int64_t>(blockIdx.y) * kGradThreads + threadIdx.x) * VE;
-  if (col >= dim) return;
+__global__ void __launch_bounds__(kGradThreads * kJoinGroups) k_grad_join(const uint32_t* __restrict__ sorted,
+                                                                          int64_t n, int64_t n_rows, int64_t dim,
+                                                                          float scale, TO* __restrict__ out,
+                                                                          int64_t ldo, bool accumulate,
+                                                                          const float* __restrict__ partial) {
+  __shared__ float sums[kJoinGroups][kGradThreads * VE];
   const int64_t chunk = blockIdx.x;
   const int64_t p0 = chunk * kGradChunk, p1 = p0 + kGradChunk;
   if (p1 >= n) return;
   const uint32_t key = sorted[p1 - 1];
   if (key >= n_rows || sorted[p1] != key) return;
   if (p0 > 0 && sorted[p0] == key && sorted[p0 - 1] == key) return;  // began earlier
+  const int group = threadIdx.x / kGradThreads, thread = threadIdx.x % kGradThreads;
+  const int64_t col = (static_cast<int64_t>(blockIdx.y) * kGradThreads + thread) * VE;
+  const bool live = col < dim;
   float acc[VE];
 #pragma unroll
-  for (int i = 0; i < VE; ++i) acc[i] = partial[(2 * chunk + 1) * dim + col + i];
-  for (int64_t c = chunk + 1; c * kGradChunk < n && sorted[c * kGradChunk] == key; ++c) {
+  for (int i = 0; i < VE; ++i) acc[i] = 0.f;
+  if (group == 0 && live) load_f32<float, VE>(partial + (2 * chunk + 1) * dim + col, acc);
+  bool more = true;
+  for (int64_t c0 = chunk + 1 + group * kGradAhead; more; c0 += kJoinGroups * kGradAhead) {
+    float f[kGradAhead][VE];
+    bool in[kGradAhead];
 #pragma unroll
-    for (int i = 0; i < VE; ++i) acc[i] += partial[(2 * c) * dim + col + i];
+    for (int u = 0; u < kGradAhead; ++u) {
+      const int64_t p = (c0 + u) * kGradChunk;
+      in[u] = p < n && sorted[p] == key;
+      // read before it is known to be wanted: a chunk that does not begin with
+      // this id has another part there, or none
+      if (p < n && live) load_f32<float, VE>(partial + 2 * (c0 + u) * dim + col, f[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kGradAhead; ++u) {
+      more = in[u];
+      if (!more) break;
+#pragma unroll
+      for (int i = 0; i < VE; ++i) acc[i] += f[u][i];
+    }
   }
-  emit_row<TO, VE>(out + static_cast<int64_t>(key) * ldo + col, acc, scale, accumulate);
+#pragma unroll
+  for (int i = 0; i < VE; ++i) sums[group][thread * VE + i] = acc[i];
+  __syncthreads();
+  if (group == 0 && live) {
+#pragma unroll
+    for (int g = 1; g < kJoinGroups; ++g)
+#pragma unroll
+      for (int i = 0; i < VE; ++i) acc[i] += sums[g][thread * VE + i];
+    emit_row<TO, VE>(out + static_cast<int64_t>(key) * ldo + col, acc, scale, accumulate);
+  }
+}
+
+// A short list (kFewTokens at most) needs no sorted order: every CTA takes 32
+// rows, picks their tokens out of the whole list, and sums each row's in token
+// order.  One launch instead of three (10000 x 64 and 256 tokens: 4 us on the
+// GPU instead of 14).  A row's place in the sorted order is the number of
+// smaller ids, so the sum is cut where the chunks would cut it and its parts are
+// added as the join adds them: the result has the same bits.
+constexpr int kFewTokens = 512;
+static_assert(kFewTokens <= kGradChunk * 2 * kGradAhead, "a run has parts of the join's first two groups");
+template <typename TI, typename TO, typename ID, int VE>
+__global__ void __launch_bounds__(kGradThreads) k_grad_few(const TI* __restrict__ grad, int64_t ldg,
+                                                           const ID* __restrict__ ids, int n, int64_t n_rows,
+                                                           int64_t dim, float scale, TO* __restrict__ out, int64_t ldo,
+                                                           bool accumulate) {
+  __shared__ uint16_t tok[kFewTokens];   // tokens of these rows, in order
+  __shared__ uint8_t of[kFewTokens];     // the row of each, less the first
+  __shared__ int counts[2][kGradThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kZeroRows;
+  int have = 0, before = 0;  // tokens of these rows, and of smaller ids
+  for (int t0 = 0; t0 < n; t0 += kGradThreads) {
+    const int t = t0 + threadIdx.x;
+    const int64_t id = t < n ? static_cast<int64_t>(ids[t]) : -1;
+    const bool mine = id >= r0 && id < r0 + kZeroRows && id < n_rows;
+    const uint32_t vote = __ballot_sync(0xffffffffu, mine);
+    const uint32_t less = __ballot_sync(0xffffffffu, id >= 0 && id < r0);
+    if (lane == 0) {
+      counts[0][warp] = __popc(vote);
+      counts[1][warp] = __popc(less);
+    }
+    __syncthreads();
+    int at = have + __popc(vote & ((1u << lane) - 1u));
+#pragma unroll
+    for (int w = 0; w < kGradThreads / 32; ++w) {
+      if (w < warp) at += counts[0][w];
+      have += counts[0][w];
+      before += counts[1][w];
+    }
+    if (mine) {
+      tok[at] = static_cast<uint16_t>(t);
+      of[at] = static_cast<uint8_t>(id - r0);
+    }
+    __syncthreads();
+  }
+  // A warp per row; the lanes go through the list together.
+  for (int r = warp; r < kZeroRows && r0 + r < n_rows; r += kGradThreads / 32) {
+    int count = 0, smaller = 0;
+    for (int q = lane; q < have; q += 32) {
+      count += of[q] == r;
+      smaller += of[q] < r;
+    }
+    count = __reduce_add_sync(0xffffffffu, count);
+    if (!count && accumulate) continue;
+    const int first = before + __reduce_add_sync(0xffffffffu, smaller);  // place in the sorted order
+    TO* dst = out + (r0 + r) * ldo;
+    for (int64_t c0 = 0; c0 < dim; c0 += 32 * VE) {
+      const int64_t c = c0 + static_cast<int64_t>(lane) * VE;
+      // the part under way, and the join's first two groups
+      float acc[VE], group[2][VE];
+#pragma unroll
+      for (int i = 0; i < VE; ++i) acc[i] = group[0][i] = group[1][i] = 0.f;
+      int place = first, part = 0;
+      if (count) {
+        for (int q0 = 0; q0 < have; q0 += 32) {
+          uint32_t left = __ballot_sync(0xffffffffu, q0 + lane < have && of[q0 + lane] == r);
+          while (left) {
+            float f[4][VE];
+            uint32_t rest = left;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              if (rest && c < dim) load_f32<TI, VE>(grad + tok[q0 + __ffs(rest) - 1] * ldg + c, f[u]);
+              rest &= rest - 1;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              if (!left) break;
+              left &= left - 1;
+              if (place % kGradChunk == 0 && place != first) {  // a new chunk begins
+                const int to = part <= kGradAhead ? 0 : 1;
+#pragma unroll
+                for (int i = 0; i < VE; ++i) {
+                  if (to) group[1][i] += acc[i];
+                  else group[0][i] += acc[i];
+                  acc[i] = 0.f;
+                }
+                ++part;
+              }
+              ++place;
+#pragma unroll
+              for (int i = 0; i < VE; ++i) acc[i] += f[u][i];
+            }
+          }
+        }
+      }
+      if (part > 0) {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+          if (part <= kGradAhead) group[0][i] += acc[i];
+          else group[1][i] += acc[i];
+          acc[i] = group[0][i] + group[1][i];
+        }
+      }
+      if (c < dim) emit_row<TO, VE>(dst + c, acc, scale, accumulate);
+    }
+  }
 }
 
 size_t grad_ws_bytes(int64_t n, int64_t dim) {
@@ -315,24 +704,61 @@ size_t grad_ws_bytes(int64_t n, int64_t dim) {
 template <typename TI, typename TO, int VE>
 void grad_launch(const void* grad, int64_t ldg, const int32_t* sorted, const int32_t* perm, int64_t n, int64_t n_rows,
                  int64_t dim, float scale, void* out, int64_t ldo, bool accumulate, float* partial, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>(ceil_div64(n, kGradChunk)),
-                  static_cast<unsigned>(ceil_div64(dim, static_cast<int64_t>(kGradThreads) * VE)));
+  const int64_t chunks = ceil_div64(n, kGradChunk);
+  const int64_t slices = ceil_div64(dim, static_cast<int64_t>(kGradThreads) * VE);
+  const int64_t zeros = accumulate ? 0 : ceil_div64(n_rows, kZeroRows);
   const uint32_t* keys = reinterpret_cast<const uint32_t*>(sorted);
-  k_grad_chunks<TI, TO, VE><<<grid, kGradThreads, 0, s>>>(static_cast<const TI*>(grad), ldg, keys, perm, n, n_rows,
-                                                         dim, scale, static_cast<TO*>(out), ldo, accumulate, partial);
-  if (grid.x > 1)
-    k_grad_join<TO, VE><<<grid, kGradThreads, 0, s>>>(keys, n, n_rows, dim, scale, static_cast<TO*>(out), ldo,
-                                                      accumulate, partial);
+  TO* o = static_cast<TO*>(out);
+  k_grad_chunks<TI, TO, VE><<<static_cast<unsigned>(chunks * slices + zeros), kGradThreads, 0, s>>>(
+      static_cast<const TI*>(grad), ldg, keys, perm, n, n_rows, dim, scale, o, ldo, accumulate, partial, chunks,
+      static_cast<int>(slices));
+  if (chunks > 1)
+    k_grad_join<TO, VE><<<dim3(static_cast<unsigned>(chunks), static_cast<unsigned>(slices)),
+                          kGradThreads * kJoinGroups, 0, s>>>(
+        keys, n, n_rows, dim, scale, o, ldo, accumulate, partial);
+}
+
+// What a gradient call reads and writes.
+struct GradArgs {
+  const void* grad;
+  int64_t ldg;
+  const int32_t* sorted;
+  const int32_t* perm;
+  const void* ids;  // of a short list, instead of sorted and perm
+  bool ids64;
+  int64_t n, n_rows, dim;
+  float scale;
+  void* out;
+  int64_t ldo;
+  bool accumulate;
+  float* partial;
+};
+
+template <typename TI, typename TO, int VE>
+void grad_with(const GradArgs& a, cudaStream_t s) {
+  if (!a.ids) {
+    grad_launch<TI, TO, VE>(a.grad, a.ldg, a.sorted, a.perm, a.n, a.n_rows, a.dim, a.scale, a.out, a.ldo, a.accumulate,
+                            a.partial, s);
+    return;
+  }
+  const unsigned grid = static_cast<unsigned>(ceil_div64(a.n_rows, kZeroRows));
+  auto go = [&](auto* ids) {
+    using ID = typename std::remove_const<typename std::remove_pointer<decltype(ids)>::type>::type;
+    k_grad_few<TI, TO, ID, VE><<<grid, kGradThreads, 0, s>>>(static_cast<const TI*>(a.grad), a.ldg, ids,
+                                                            static_cast<int>(a.n), a.n_rows, a.dim, a.scale,
+                                                            static_cast<TO*>(a.out), a.ldo, a.accumulate);
+  };
+  if (a.ids64) go(static_cast<const int64_t*>(a.ids));
+  else go(static_cast<const int32_t*>(a.ids));
 }
 
 template <typename TI, typename TO>
-void grad_pick(int ve, const void* grad, int64_t ldg, const int32_t* sorted, const int32_t* perm, int64_t n,
-               int64_t n_rows, int64_t dim, float scale, void* out, int64_t ldo, bool accumulate, float* partial,
-               cudaStream_t s) {
-  if (ve == 4)
-    grad_launch<TI, TO, 4>(grad, ldg, sorted, perm, n, n_rows, dim, scale, out, ldo, accumulate, partial, s);
-  else
-    grad_launch<TI, TO, 1>(grad, ldg, sorted, perm, n, n_rows, dim, scale, out, ldo, accumulate, partial, s);
+void grad_pick(int ve, const GradArgs& a, cudaStream_t s) {
+  if constexpr (sizeof(TI) == 2 && sizeof(TO) == 2) {
+    if (ve == 8) return grad_with<TI, TO, 8>(a, s);
+  }
+  if (ve >= 4) grad_with<TI, TO, 4>(a, s);
+  else grad_with<TI, TO, 1>(a, s);
 }
 
 bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(bytes) == 0; }
@@ -414,7 +840,8 @@ extern "C" kairo_status kairo_token_sort(const void* ids, int32_t id_bytes, int6
   if (st) return st;
   if (id_bytes != 4 && id_bytes != 8) return fail(KAIRO_STATUS_INVALID_VALUE, "ids must be int32 or int64");
   if (nids == 0) return KAIRO_STATUS_SUCCESS;
-  if (!ids || !sorted || !perm || !workspace) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+  if (!ids || !sorted || !perm || !workspace)
+    return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
   if (workspace_bytes < need) return fail(KAIRO_STATUS_WORKSPACE_TOO_SMALL, "token sort workspace too small");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint32_t* keys = reinterpret_cast<uint32_t*>(sorted);
@@ -422,43 +849,101 @@ extern "C" kairo_status kairo_token_sort(const void* ids, int32_t id_bytes, int6
                        : sort_launch(static_cast<const int32_t*>(ids), nids, n_rows, keys, perm, workspace, s);
 }
 
-extern "C" kairo_status kairo_embedding_grad_workspace_size(int64_t nids, int64_t dim, size_t* bytes) {
-  if (!bytes || nids < 0 || dim <= 0) return fail(KAIRO_STATUS_INVALID_VALUE, "invalid argument");
-  *bytes = grad_ws_bytes(nids, dim);
-  return KAIRO_STATUS_SUCCESS;
-}
+namespace {
 
-extern "C" kairo_status kairo_embedding_grad(const void* grad_output, int64_t ldg, kairo_dtype dtype,
-                                             const int32_t* sorted, const int32_t* perm, int64_t nids, int64_t n_rows,
-                                             int64_t dim, float scale, void* grad_weight, int64_t ldo,
-                                             kairo_dtype out_dtype, int32_t accumulate, void* workspace,
-                                             size_t workspace_bytes, void* stream) {
+// Workspace: the partial rows, and for a call with ids the sorted order and the
+// sort's own.
+size_t order_bytes(int64_t n) { return 2 * align_up(static_cast<size_t>(n) * 4, 256); }
+
+kairo_status run_grad(const void* grad_output, int64_t ldg, kairo_dtype dtype, const int32_t* sorted,
+                      const int32_t* perm, const void* ids, int32_t id_bytes, int64_t nids, int64_t n_rows,
+                      int64_t dim, float scale, void* grad_weight, int64_t ldo, kairo_dtype out_dtype,
+                      int32_t accumulate, void* workspace, size_t workspace_bytes, void* stream) {
   if (n_rows < 0 || dim <= 0 || nids < 0) return fail(KAIRO_STATUS_INVALID_VALUE, "invalid size");
   if (nids > kMaxTokens || n_rows > kMaxRows) return fail(KAIRO_STATUS_NOT_SUPPORTED, "too many tokens or rows");
-  if (dim > static_cast<int64_t>(65535) * kGradThreads) return fail(KAIRO_STATUS_NOT_SUPPORTED, "dim too large");
+  if (dim > static_cast<int64_t>(65535) * kGradThreads ||
+      ceil_div64(nids, kGradChunk) * ceil_div64(dim, kGradThreads) + ceil_div64(n_rows, kZeroRows) > 0x7fffffffLL)
+    return fail(KAIRO_STATUS_NOT_SUPPORTED, "too many tokens for this width");
   if (ldg < dim || ldo < dim) return fail(KAIRO_STATUS_INVALID_VALUE, "leading dimension smaller than dim");
   if (!known_dtype(dtype) || !known_dtype(out_dtype)) return fail(KAIRO_STATUS_INVALID_VALUE, "unknown dtype");
+  if (id_bytes != 4 && id_bytes != 8) return fail(KAIRO_STATUS_INVALID_VALUE, "ids must be int32 or int64");
   if (n_rows == 0) return KAIRO_STATUS_SUCCESS;
   if (!grad_weight) return fail(KAIRO_STATUS_INVALID_VALUE, "null grad_weight");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t ob = element_bytes(out_dtype);
-  if (!accumulate) {
+  if (nids == 0) {
+    if (accumulate) return KAIRO_STATUS_SUCCESS;
     const cudaError_t e = cudaMemset2DAsync(grad_weight, static_cast<size_t>(ldo * ob), 0,
                                             static_cast<size_t>(dim * ob), static_cast<size_t>(n_rows), s);
     if (e != cudaSuccess) return cuda_fail(e, "cudaMemset2DAsync(grad_weight)");
+    return KAIRO_STATUS_SUCCESS;
   }
-  if (nids == 0) return KAIRO_STATUS_SUCCESS;
-  if (!grad_output || !sorted || !perm || !workspace) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
-  if (workspace_bytes < grad_ws_bytes(nids, dim))
-    return fail(KAIRO_STATUS_WORKSPACE_TOO_SMALL, "embedding gradient workspace too small");
+  if (!grad_output || (!ids && (!sorted || !perm)) || !workspace)
+    return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+  size_t need = grad_ws_bytes(nids, dim);
+  const size_t order_at = align_up(need, 256);
+  if (ids) need = order_at + order_bytes(nids) + sort_ws_bytes(nids);
+  if (workspace_bytes < need) return fail(KAIRO_STATUS_WORKSPACE_TOO_SMALL, "embedding gradient workspace too small");
+  GradArgs a{};
+  a.grad = grad_output;
+  a.ldg = ldg;
+  a.sorted = sorted;
+  a.perm = perm;
+  a.n = nids;
+  a.n_rows = n_rows;
+  a.dim = dim;
+  a.scale = scale;
+  a.out = grad_weight;
+  a.ldo = ldo;
+  a.accumulate = accumulate != 0;
+  a.partial = static_cast<float*>(workspace);
+  if (ids && nids <= kFewTokens) {
+    a.ids = ids;
+    a.ids64 = id_bytes == 8;
+  } else if (ids) {
+    uint8_t* p = static_cast<uint8_t*>(workspace) + order_at;
+    int32_t* order = reinterpret_cast<int32_t*>(p);
+    int32_t* tokens = reinterpret_cast<int32_t*>(p + order_bytes(nids) / 2);
+    const kairo_status st = kairo_token_sort(ids, id_bytes, nids, n_rows, order, tokens, p + order_bytes(nids),
+                                             workspace_bytes - order_at - order_bytes(nids), stream);
+    if (st) return st;
+    a.sorted = order;
+    a.perm = tokens;
+  }
   const int64_t ib = element_bytes(dtype);
-  const int ve = (dim % 4 == 0 && ldg % 4 == 0 && ldo % 4 == 0 && aligned(grad_output, 4 * ib) &&
-                  aligned(grad_weight, 4 * ob)) ? 4 : 1;
-  for_types(dtype, out_dtype, [&](auto ti, auto to) {
-    grad_pick<decltype(ti), decltype(to)>(ve, grad_output, ldg, sorted, perm, nids, n_rows, dim, scale, grad_weight,
-                                          ldo, accumulate != 0, static_cast<float*>(workspace), s);
-  });
+  auto fits = [&](int64_t ve) {
+    return dim % ve == 0 && ldg % ve == 0 && ldo % ve == 0 && aligned(grad_output, ve * ib) &&
+           aligned(grad_weight, ve * ob);
+  };
+  const int ve = ib == 2 && ob == 2 && fits(8) ? 8 : (fits(4) ? 4 : 1);
+  for_types(dtype, out_dtype, [&](auto ti, auto to) { grad_pick<decltype(ti), decltype(to)>(ve, a, s); });
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "launch of the embedding gradient");
   return KAIRO_STATUS_SUCCESS;
+}
+
+}  // namespace
+
+extern "C" kairo_status kairo_embedding_grad_workspace_size(int64_t nids, int64_t dim, size_t* bytes) {
+  if (!bytes || nids < 0 || dim <= 0) return fail(KAIRO_STATUS_INVALID_VALUE, "invalid argument");
+  *bytes = align_up(grad_ws_bytes(nids, dim), 256) + order_bytes(nids) + sort_ws_bytes(nids);
+  return KAIRO_STATUS_SUCCESS;
+}
+
+extern "C" kairo_status kairo_embedding_grad(const void* grad_output, int64_t ldg, kairo_dtype dtype, const void* ids,
+                                             int32_t id_bytes, int64_t nids, int64_t n_rows, int64_t dim, float scale,
+                                             void* grad_weight, int64_t ldo, kairo_dtype out_dtype, int32_t accumulate,
+                                             void* workspace, size_t workspace_bytes, void* stream) {
+  if (nids > 0 && n_rows > 0 && !ids) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+  return run_grad(grad_output, ldg, dtype, nullptr, nullptr, ids, id_bytes, nids, n_rows, dim, scale, grad_weight, ldo,
+                  out_dtype, accumulate, workspace, workspace_bytes, stream);
+}
+
+extern "C" kairo_status kairo_embedding_grad_sorted(const void* grad_output, int64_t ldg, kairo_dtype dtype,
+                                                    const int32_t* sorted, const int32_t* perm, int64_t nids,
+                                                    int64_t n_rows, int64_t dim, float scale, void* grad_weight,
+                                                    int64_t ldo, kairo_dtype out_dtype, int32_t accumulate,
+                                                    void* workspace, size_t workspace_bytes, void* stream) {
+  return run_grad(grad_output, ldg, dtype, sorted, perm, nullptr, 4, nids, n_rows, dim, scale, grad_weight, ldo,
+                  out_dtype, accumulate, workspace, workspace_bytes, stream);
 }

@@ -158,11 +158,16 @@ def embedding_grad(grad_output: Tensor, ids: Tensor | TokenOrder, num_embeddings
         out = g.new_empty((n_rows, d), dtype=odt)
     elif tuple(out.shape) != (n_rows, d) or out.dtype != odt or out.device != dev or _rows(out) is not out:
         raise ValueError(f"out must be a row-major ({n_rows}, {d}) {odt} tensor on {dev}")
-    order = ids if isinstance(ids, TokenOrder) else sort_tokens(ids, n_rows)
     ws = g.new_empty(_grad_bytes(tokens, d), dtype=torch.uint8)
-    _lib.launch("embedding_grad", _lib.lib().kairo_embedding_grad, index, g.data_ptr(), _ld(g), in_dt,
-                order.sorted_ids.data_ptr(), order.perm.data_ptr(), tokens, n_rows, d, float(scale), out.data_ptr(),
-                _ld(out), out_dt, 1 if accumulate else 0, ws.data_ptr(), ws.numel())
+    tail = (tokens, n_rows, d, float(scale), out.data_ptr(), _ld(out), out_dt, 1 if accumulate else 0, ws.data_ptr(),
+            ws.numel())
+    if isinstance(ids, TokenOrder):
+        _lib.launch("embedding_grad", _lib.lib().kairo_embedding_grad_sorted, index, g.data_ptr(), _ld(g), in_dt,
+                    ids.sorted_ids.data_ptr(), ids.perm.data_ptr(), *tail)
+    else:
+        flat = _flat_ids(ids, "embedding_grad")
+        _lib.launch("embedding_grad", _lib.lib().kairo_embedding_grad, index, g.data_ptr(), _ld(g), in_dt,
+                    flat.data_ptr(), flat.element_size(), *tail)
     return out
 
 

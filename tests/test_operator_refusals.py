@@ -66,15 +66,21 @@ def test_embedding_c_refusals():
     assert lib.kairo_token_sort(None, 8, 0, 70000, None, None, None, n.value, None) == _lib.SUCCESS
 
     def grad(ldg=8, dt=0, nids=3, rows=4, dim=8, ldo=8, odt=0, acc=1, ws=some, wsb=1 << 20, g=some, out=some):
-        return lib.kairo_embedding_grad(g, ldg, dt, some, some, nids, rows, dim, 1.0, out, ldo, odt, acc, ws, wsb,
-                                        None)
+        return lib.kairo_embedding_grad_sorted(g, ldg, dt, some, some, nids, rows, dim, 1.0, out, ldo, odt, acc, ws,
+                                               wsb, None)
 
-    for kw in ({"ldg": 7}, {"ldo": 7}, {"dt": 3}, {"odt": 3}, {"nids": -1}, {"rows": -1}, {"dim": 0}, {"g": None},
-               {"ws": None}, {"out": None}):
-        assert grad(**kw) == _lib.INVALID_VALUE, kw
-    assert grad(wsb=10) == _lib.WORKSPACE_TOO_SMALL
-    assert grad(nids=1 << 31) == _lib.NOT_SUPPORTED
-    assert grad(rows=0) == _lib.SUCCESS
+    def grad_ids(ldg=8, dt=0, nids=3, rows=4, dim=8, ldo=8, odt=0, acc=1, ws=some, wsb=1 << 20, g=some, out=some,
+                 ids=some, idb=8):
+        return lib.kairo_embedding_grad(g, ldg, dt, ids, idb, nids, rows, dim, 1.0, out, ldo, odt, acc, ws, wsb, None)
+
+    for fn in (grad, grad_ids):
+        for kw in ({"ldg": 7}, {"ldo": 7}, {"dt": 3}, {"odt": 3}, {"nids": -1}, {"rows": -1}, {"dim": 0}, {"g": None},
+                   {"ws": None}, {"out": None}):
+            assert fn(**kw) == _lib.INVALID_VALUE, kw
+        assert fn(wsb=10) == _lib.WORKSPACE_TOO_SMALL
+        assert fn(nids=1 << 31) == _lib.NOT_SUPPORTED
+        assert fn(rows=0) == _lib.SUCCESS
+    assert grad_ids(ids=None) == _lib.INVALID_VALUE and grad_ids(idb=2) == _lib.INVALID_VALUE
 
 
 def _bsr():
