@@ -381,6 +381,9 @@ KAIRO_API kairo_status kairo_bsr_sddmm_q8_workspace_size(const kairo_bsr* a, int
  *   kairo_low_rank_wgrad_q8  the same with z given in 8 bits
  *                         (kairo_quantize_q8); dtype is the type it reads
  *                         back in.
+ *   kairo_low_rank_wgrads  both gradients of one layer in one launch: d_down
+ *                         from dlow and x (k features), d_up from low and dy
+ *                         (n features).
  * x, z, down, up f16 or bf16 (one dtype); base, y and grad that dtype or fp32.
  * rank at most 128, at most 65535 adapters, 2^24 tokens, 2^22 features.  All
  * asynchronous on `stream`.
@@ -397,6 +400,10 @@ KAIRO_API kairo_status kairo_low_rank_apply(const void* x, int64_t ldx, int64_t 
 KAIRO_API kairo_status kairo_low_rank_wgrad(const float* low, int64_t rank, const void* z, int64_t ldz, int64_t k,
                                             kairo_dtype dtype, const void* plan, int64_t ntokens, int64_t nadapters,
                                             void* grad, kairo_dtype grad_dtype, void* stream);
+KAIRO_API kairo_status kairo_low_rank_wgrads(const float* dlow, const float* low, int64_t rank, const void* x,
+                                             int64_t ldx, int64_t k, const void* dy, int64_t lddy, int64_t n,
+                                             kairo_dtype dtype, const void* plan, int64_t ntokens, int64_t nadapters,
+                                             void* d_down, void* d_up, kairo_dtype grad_dtype, void* stream);
 KAIRO_API kairo_status kairo_low_rank_wgrad_q8(const float* low, int64_t rank, const int8_t* codes, int64_t ldq,
                                                const float* steps, int64_t lds, int64_t k, kairo_dtype dtype,
                                                const void* plan, int64_t ntokens, int64_t nadapters, void* grad,

@@ -204,6 +204,9 @@ _SIGNATURES = {
                                        c_int64, c_int32, c_void_p, c_void_p]),
     "kairo_low_rank_wgrad": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int32, c_void_p, c_int64,
                                        c_int64, c_void_p, c_int32, c_void_p]),
+    "kairo_low_rank_wgrads": (c_int32, [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64,
+                                        c_int64, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int32,
+                                        c_void_p]),
     "kairo_low_rank_wgrad_q8": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int32,
                                           c_void_p, c_int64, c_int64, c_void_p, c_int32, c_void_p]),
     "kairo_block_norms": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_int32, c_int32, c_int32, c_void_p,

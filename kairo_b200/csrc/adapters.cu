@@ -60,31 +60,38 @@ size_t carve_plan(void* mem, int64_t t, int64_t g, Plan* pl) {
   return at * sizeof(int32_t);
 }
 
-__global__ void k_plan_starts(const uint32_t* __restrict__ sorted, int64_t t, int64_t g, int32_t* __restrict__ starts) {
-  for (int64_t a = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; a < g + 2;
-       a += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    int64_t lo = 0, hi = t;  // first position whose key is >= a
+// The tiles of one size (blockIdx.x) from the sorted ids: where each adapter's
+// tokens start, how many tiles come before its own, and the tiles themselves.
+__global__ void __launch_bounds__(1024) k_plan_tiles(const uint32_t* __restrict__ sorted, int64_t t, int64_t g, Plan pl) {
+  __shared__ int sums[32];
+  __shared__ int carry;
+  const int which = blockIdx.x;
+  const int size = tile_tokens(which);
+  int32_t* first = which == 0 ? pl.first[0] : (which == 1 ? pl.first[1] : pl.first[2]);
+  LowRankTile* tiles = which == 0 ? pl.tiles[0] : (which == 1 ? pl.tiles[1] : pl.tiles[2]);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto start_of = [&](int64_t a) {  // first position whose id is >= a
+    int64_t lo = 0, hi = t;
     while (lo < hi) {
       const int64_t mid = (lo + hi) >> 1;
       if (sorted[mid] < static_cast<uint32_t>(a)) lo = mid + 1;
       else hi = mid;
     }
-    starts[a] = static_cast<int32_t>(lo);
-  }
-}
-
-// First tile of every adapter, and the number of tiles, for one tile size per CTA.
-__global__ void __launch_bounds__(1024) k_plan_first(Plan pl, int64_t g) {
-  __shared__ int sums[32];
-  __shared__ int carry;
-  const int size = tile_tokens(blockIdx.x);
-  int32_t* first = blockIdx.x == 0 ? pl.first[0] : (blockIdx.x == 1 ? pl.first[1] : pl.first[2]);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    return static_cast<int>(lo);
+  };
   if (threadIdx.x == 0) carry = 0;
   __syncthreads();
   for (int64_t base = 0; base <= g; base += 1024) {
     const int64_t a = base + threadIdx.x;  // g: tokens without an adapter
-    const int v = a <= g ? (pl.starts[a + 1] - pl.starts[a] + size - 1) / size : 0;
+    int v = 0;
+    if (a <= g) {
+      const int p0 = start_of(a), p1 = a < g ? start_of(a + 1) : static_cast<int>(t);
+      v = (p1 - p0 + size - 1) / size;
+      if (which == 0) {
+        pl.starts[a] = p0;
+        if (a == g) pl.starts[g + 1] = p1;
+      }
+    }
     int x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -109,28 +116,24 @@ __global__ void __launch_bounds__(1024) k_plan_first(Plan pl, int64_t g) {
     if (threadIdx.x == 1023) carry = incl;
     __syncthreads();
   }
+  const int n = carry;
   if (threadIdx.x == 0) {
-    first[g + 1] = carry;
-    pl.ntiles[blockIdx.x] = carry;
+    first[g + 1] = n;
+    pl.ntiles[which] = n;
   }
-}
-
-__global__ void k_plan_tiles(Plan pl, int64_t g) {
-  const int size = tile_tokens(blockIdx.y);
-  const int32_t* first = blockIdx.y == 0 ? pl.first[0] : (blockIdx.y == 1 ? pl.first[1] : pl.first[2]);
-  LowRankTile* tiles = blockIdx.y == 0 ? pl.tiles[0] : (blockIdx.y == 1 ? pl.tiles[1] : pl.tiles[2]);
-  const int n = first[g + 1];
-  for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) {
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += 1024) {
     int64_t lo = 0, hi = g;  // the adapter a with first[a] <= i < first[a + 1]
     while (lo < hi) {
       const int64_t mid = (lo + hi) >> 1;
       if (first[mid + 1] <= i) lo = mid + 1;
       else hi = mid;
     }
+    const int p0 = start_of(lo), p1 = lo < g ? start_of(lo + 1) : static_cast<int>(t);
     LowRankTile tile;
     tile.adapter = lo < g ? static_cast<int32_t>(lo) : -1;
-    tile.begin = pl.starts[lo] + (i - first[lo]) * size;
-    tile.count = min(size, pl.starts[lo + 1] - tile.begin);
+    tile.begin = p0 + (i - first[lo]) * size;
+    tile.count = min(size, p1 - tile.begin);
     tile.pad = 0;
     tiles[i] = tile;
   }
@@ -226,11 +229,7 @@ extern "C" kairo_status kairo_adapter_plan_build(const void* ids, int32_t id_byt
   st = kairo_token_sort(ids, id_bytes, ntokens, nadapters, sorted, pl.order, static_cast<uint8_t*>(workspace) + col,
                         workspace_bytes - col, stream);
   if (st) return st;
-  k_plan_starts<<<static_cast<unsigned>(ceil_div64(nadapters + 2, 256)), 256, 0, s>>>(
-      reinterpret_cast<const uint32_t*>(sorted), ntokens, nadapters, pl.starts);
-  k_plan_first<<<kTileSizes, 1024, 0, s>>>(pl, nadapters);
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(ceil_div64(max_tiles(ntokens, nadapters, tile_tokens(0)), 256), 1024));
-  k_plan_tiles<<<dim3(static_cast<unsigned>(most), kTileSizes), 256, 0, s>>>(pl, nadapters);
+  k_plan_tiles<<<kTileSizes, 1024, 0, s>>>(reinterpret_cast<const uint32_t*>(sorted), ntokens, nadapters, pl);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "launch of the adapter plan");
   return KAIRO_STATUS_SUCCESS;
@@ -289,33 +288,62 @@ extern "C" kairo_status kairo_low_rank_apply(const void* x, int64_t ldx, int64_t
 
 namespace {
 
-// Both forms of the gradient: z in its own type, or codes and steps.
-kairo_status wgrad(const float* low, int64_t rank, const void* z, int64_t ldz, const int8_t* codes, int64_t ldq,
-                   const float* steps, int64_t lds, int64_t k, kairo_dtype dtype, const void* plan, int64_t ntokens,
-                   int64_t nadapters, void* grad, kairo_dtype grad_dtype, void* stream) {
-  const kairo_status st = check_low_rank(ntokens, k, 1, rank, nadapters, dtype);
+// One contraction over tokens: z in its own type, or codes and steps.
+struct Grad {
+  const float* low;
+  const void* z;
+  int64_t ldz;
+  const int8_t* codes;
+  int64_t ldq;
+  const float* steps;
+  int64_t lds;
+  int64_t k;
+  void* grad;
+};
+
+kairo_status check_grad(const Grad& p, int64_t rank, kairo_dtype dtype, const void* plan, int64_t ntokens,
+                        int64_t nadapters, kairo_dtype grad_dtype) {
+  const kairo_status st = check_low_rank(ntokens, p.k, 1, rank, nadapters, dtype);
   if (st) return st;
   if (grad_dtype != KAIRO_DTYPE_F32 && grad_dtype != dtype)
     return fail(KAIRO_STATUS_INVALID_VALUE, "the gradient must be fp32 or the adapters' dtype");
   if (nadapters == 0) return KAIRO_STATUS_SUCCESS;
-  if (!plan || !grad || (ntokens > 0 && !low)) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+  if (!plan || !p.grad || (ntokens > 0 && !p.low)) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+  return KAIRO_STATUS_SUCCESS;
+}
+
+bool z_aligned(const Grad& p) { return p.codes || (p.k % 8 == 0 && p.ldz % 8 == 0 && aligned16(p.z)); }
+
+// One or two of them in one launch (two: neither in 8 bits).
+kairo_status run_grads(const Grad* p, int count, int64_t rank, kairo_dtype dtype, const void* plan, int64_t ntokens,
+                       int64_t nadapters, kairo_dtype grad_dtype, void* stream) {
+  if (nadapters == 0) return KAIRO_STATUS_SUCCESS;
   Plan pl;
   carve_plan(const_cast<void*>(plan), ntokens, nadapters, &pl);
   LowRankWgradArgs a{};
-  a.s = low;
-  a.z = z;
-  a.codes = codes;
-  a.steps = steps;
-  a.grad = grad;
+  bool vec = true;
+  int64_t widest = 0, total = 0;
+  for (int i = 0; i < count; ++i) {
+    LowRankWgradArgs::One& o = a.one[i];
+    o.s = p[i].low;
+    o.z = p[i].z;
+    o.codes = p[i].codes;
+    o.steps = p[i].steps;
+    o.grad = p[i].grad;
+    o.ldz = p[i].ldz;
+    o.ldq = p[i].ldq;
+    o.lds = p[i].lds;
+    o.k = static_cast<int32_t>(p[i].k);
+    vec = vec && z_aligned(p[i]);
+    widest = std::max(widest, p[i].k);
+    total += p[i].k;
+  }
   a.order = pl.order;
   a.starts = pl.starts;
-  a.ldz = ldz;
-  a.ldq = ldq;
-  a.lds = lds;
-  a.k = static_cast<int32_t>(k);
   a.rank = static_cast<int32_t>(rank);
-  const bool vec = codes || (k % 8 == 0 && ldz % 8 == 0 && aligned16(z));
-  const int cluster = pick_wgrad_cluster(ntokens, nadapters, k, rank);
+  a.count = count;
+  a.widest = static_cast<int32_t>(widest);
+  const int cluster = pick_wgrad_cluster(ntokens, nadapters, total, rank);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool gf = grad_dtype == KAIRO_DTYPE_F32;
   const cudaError_t err = dtype == KAIRO_DTYPE_F16
@@ -332,17 +360,32 @@ extern "C" kairo_status kairo_low_rank_wgrad(const float* low, int64_t rank, con
                                              void* grad, kairo_dtype grad_dtype, void* stream) {
   if (ldz < k) return fail(KAIRO_STATUS_INVALID_VALUE, "leading dimension too small");
   if (ntokens > 0 && nadapters > 0 && !z) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
-  return wgrad(low, rank, z, ldz, nullptr, 0, nullptr, 0, k, dtype, plan, ntokens, nadapters, grad, grad_dtype, stream);
+  const Grad p{low, z, ldz, nullptr, 0, nullptr, 0, k, grad};
+  const kairo_status st = check_grad(p, rank, dtype, plan, ntokens, nadapters, grad_dtype);
+  return st ? st : run_grads(&p, 1, rank, dtype, plan, ntokens, nadapters, grad_dtype, stream);
 }
 
 extern "C" kairo_status kairo_low_rank_wgrad_q8(const float* low, int64_t rank, const int8_t* codes, int64_t ldq,
                                                 const float* steps, int64_t lds, int64_t k, kairo_dtype dtype,
                                                 const void* plan, int64_t ntokens, int64_t nadapters, void* grad,
                                                 kairo_dtype grad_dtype, void* stream) {
-  if (ldq < k || lds < ntokens) return fail(KAIRO_STATUS_INVALID_VALUE, "leading dimension too small");
-  if (ldq % 16 || !aligned16(codes)) return fail(KAIRO_STATUS_INVALID_VALUE, "codes must have 16-byte aligned rows");
-  if (ntokens > 0 && nadapters > 0 && (!codes || !steps))
-    return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
-  return wgrad(low, rank, nullptr, 0, codes, ldq, steps, lds, k, dtype, plan, ntokens, nadapters, grad, grad_dtype,
-               stream);
+  kairo_status st = q8_check(ntokens, k, codes, ldq, steps, lds);
+  if (st) return st;
+  const Grad p{low, nullptr, 0, codes, ldq, steps, lds, k, grad};
+  st = check_grad(p, rank, dtype, plan, ntokens, nadapters, grad_dtype);
+  return st ? st : run_grads(&p, 1, rank, dtype, plan, ntokens, nadapters, grad_dtype, stream);
+}
+
+extern "C" kairo_status kairo_low_rank_wgrads(const float* dlow, const float* low, int64_t rank, const void* x,
+                                              int64_t ldx, int64_t k, const void* dy, int64_t lddy, int64_t n,
+                                              kairo_dtype dtype, const void* plan, int64_t ntokens, int64_t nadapters,
+                                              void* d_down, void* d_up, kairo_dtype grad_dtype, void* stream) {
+  if (ldx < k || lddy < n) return fail(KAIRO_STATUS_INVALID_VALUE, "leading dimension too small");
+  if (ntokens > 0 && nadapters > 0 && (!x || !dy)) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+  const Grad p[2] = {{dlow, x, ldx, nullptr, 0, nullptr, 0, k, d_down}, {low, dy, lddy, nullptr, 0, nullptr, 0, n, d_up}};
+  for (const Grad& q : p) {
+    const kairo_status st = check_grad(q, rank, dtype, plan, ntokens, nadapters, grad_dtype);
+    if (st) return st;
+  }
+  return run_grads(p, 2, rank, dtype, plan, ntokens, nadapters, grad_dtype, stream);
 }

@@ -67,16 +67,22 @@ struct LowRankApplyArgs {
   int32_t base_f32;
 };
 
+// One or two weight gradients of one launch.
 struct LowRankWgradArgs {
-  const float* s;      // (tokens, rank)
-  const void* z;       // (tokens, k), or null when given in 8 bits:
-  const int8_t* codes;
-  const float* steps;
-  void* grad;          // (adapters, rank, k)
+  struct One {
+    const float* s;      // (tokens, rank)
+    const void* z;       // (tokens, k), or null when given in 8 bits:
+    const int8_t* codes;
+    const float* steps;
+    void* grad;          // (adapters, rank, k)
+    int64_t ldz, ldq, lds;
+    int32_t k;
+  } one[2];
   const int32_t* order;
   const int32_t* starts;
-  int64_t ldz, ldq, lds;
-  int32_t k, rank;
+  int32_t rank;
+  int32_t count;
+  int32_t widest;        // largest k
 };
 
 // Launches (adapters_bf16.cu, adapters_f16.cu).  `tile` is 16, 32 or 64 tokens,
@@ -749,7 +755,9 @@ struct WgradShape {
 // fp32 with rounding, so that a long batch loses nothing to the units'
 // truncation.  The cluster's partial sums are added in rank order.
 template <typename T, typename TG, typename S, int TERMS, bool Q8, bool VEC, int MINB>
-__global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgradArgs a) {
+__global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgradArgs args) {
+  const LowRankWgradArgs::One& a = args.one[blockIdx.z];
+  const int rank = args.rank;
   constexpr int MR = S::MR, RP = S::RP;
   constexpr bool HALF = std::is_same_v<T, __half>;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -767,7 +775,8 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgr
   const int rg = warp % S::RG;
   const int lc = (warp / S::RG) * 64;                              // first feature of the warp in the CTA
   const int c0 = static_cast<int>(blockIdx.x / csize) * S::COLS;
-  const int p0 = a.starts[adapter], p1 = a.starts[adapter + 1];
+  if (c0 >= a.k) return;  // the whole cluster: the other gradient is wider
+  const int p0 = args.starts[adapter], p1 = args.starts[adapter + 1];
   // This CTA's chunks: crank, crank + csize, ...; only the last of all is short.
   const int first = p0 + static_cast<int>(crank) * kChunk;
   const int hop = static_cast<int>(csize) * kChunk;
@@ -783,7 +792,7 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgr
   static_assert(S::UNITS <= 8, "a unit's tokens are known when it starts");
   auto chunk_token = [&](int n) {
     const int p = first + n * hop + threadIdx.x;
-    return n < chunks && p < p1 ? __ldg(a.order + p) : -1;
+    return n < chunks && p < p1 ? __ldg(args.order + p) : -1;
   };
   if (threadIdx.x < kChunk) {
 #pragma unroll
@@ -837,7 +846,7 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgr
     for (int i = 0; i < S::PER_THREAD; ++i) {
       const int e = i * kThreadsPerCta + threadIdx.x;
       const int tok = toks[(n & 3) * kChunk + e / RP], r = e % RP;
-      mine[i] = (tok >= 0 && r < a.rank) ? __ldg(a.s + static_cast<int64_t>(tok) * a.rank + r) : 0.f;
+      mine[i] = (tok >= 0 && r < rank) ? __ldg(a.s + static_cast<int64_t>(tok) * rank + r) : 0.f;
     }
   };
   auto split = [&](float v, int n, int row, int r) {
@@ -975,8 +984,8 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgr
     }
   cluster_sync();
   const uint32_t part_addr = smem_addr(part);
-  TG* grad = static_cast<TG*>(a.grad) + static_cast<int64_t>(adapter) * a.rank * a.k;
-  const int total = a.rank * S::COLS / 4;
+  TG* grad = static_cast<TG*>(a.grad) + static_cast<int64_t>(adapter) * rank * a.k;
+  const int total = rank * S::COLS / 4;
   for (int i = static_cast<int>(crank) * kThreadsPerCta + threadIdx.x; i < total;
        i += static_cast<int>(csize) * kThreadsPerCta) {
     const int r = i / (S::COLS / 4), c = c0 + 4 * (i - r * (S::COLS / 4));
@@ -1005,7 +1014,8 @@ cudaError_t launch_wgrad(const LowRankWgradArgs& a, int64_t adapters, int cluste
   cudaError_t e = allow_smem(fn, bytes, &done);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(ceil_div64(a.k, S::COLS) * cluster), static_cast<unsigned>(adapters));
+  cfg.gridDim = dim3(static_cast<unsigned>(ceil_div64(a.widest, S::COLS) * cluster), static_cast<unsigned>(adapters),
+                     static_cast<unsigned>(a.count));
   cfg.blockDim = dim3(kThreadsPerCta);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = s;
@@ -1040,7 +1050,7 @@ cudaError_t pick_wgrad(const LowRankWgradArgs& a, int64_t adapters, int cluster,
   template <>                                                                                                        \
   cudaError_t launch_low_rank_wgrad<T>(const LowRankWgradArgs& a, bool grad_f32, bool vec, int64_t adapters,         \
                                        int cluster, cudaStream_t s) {                                               \
-    if (a.codes)                                                                                                     \
+    if (a.one[0].codes)                                                                                              \
       return grad_f32 ? lowrank::pick_wgrad<T, float, true, true>(a, adapters, cluster, s)                           \
                       : lowrank::pick_wgrad<T, T, true, true>(a, adapters, cluster, s);                              \
     if (vec)                                                                                                         \

@@ -246,8 +246,15 @@ def adapter_linear_backward(dY: Tensor, X: Tensor | QuantizedActivations, adapte
     if low is None:
         low = torch.empty_like(dlow)
         _apply(op, index, Z, adapters.down, adapters.up, adapters.scale, plan, None, None, low)
-    d_down = _wgrad(op, index, dlow, Z, plan, gdt)
-    d_up = _wgrad(op, index, low.contiguous(), dY, plan, gdt)
+    low = low.contiguous()
+    if kept:
+        return dX, _wgrad(op, index, dlow, Z, plan, gdt), _wgrad(op, index, low, dY, plan, gdt)
+    d_down = dlow.new_empty(adapters.down.shape, dtype=gdt)
+    d_up = dlow.new_empty(adapters.up.shape, dtype=gdt)
+    _lib.launch(op, _lib.lib().kairo_low_rank_wgrads, index, dlow.data_ptr(), low.data_ptr(), adapters.rank,
+                Z.data_ptr(), _ld(Z), adapters.in_features, dY.data_ptr(), _ld(dY), adapters.out_features,
+                _lib.kairo_dtype(dY.dtype), plan.memory.data_ptr(), plan.num_tokens, plan.num_adapters,
+                d_down.data_ptr(), d_up.data_ptr(), _lib.kairo_dtype(gdt))
     return dX, d_down, d_up
 
 

@@ -55,6 +55,13 @@ class QuantizedActivations:
             if (n > 1 and self.steps.stride(1) != 1) or (self.steps.shape[0] > 1 and self.steps.stride(0) < n):
                 raise ValueError("steps must be row-major")
 
+    @classmethod
+    def _made(cls, codes: Tensor, steps: Tensor, dtype: torch.dtype) -> "QuantizedActivations":
+        """One whose parts this package laid out itself: no checks."""
+        q = object.__new__(cls)
+        q.__dict__.update(codes=codes, steps=steps, dtype=dtype)
+        return q
+
     @property
     def shape(self) -> tuple[int, int]:
         return tuple(self.codes.shape)
@@ -102,7 +109,7 @@ def quantize_activations(X: Tensor) -> QuantizedActivations:
     steps = X.new_empty((-(-k // GROUP), n), dtype=torch.float32)
     _lib.launch("quantize_activations", _lib.lib().kairo_quantize_q8, index, X.data_ptr(), n, k, max(X.stride(0), k),
                 dt, codes.data_ptr(), ldq, steps.data_ptr(), n)
-    return QuantizedActivations(codes=codes, steps=steps, dtype=X.dtype)
+    return QuantizedActivations._made(codes, steps, X.dtype)
 
 
 def dequantize_activations(q: QuantizedActivations, *, out: Tensor | None = None) -> Tensor:

@@ -214,5 +214,14 @@ def test_adapter_c_refusals():
                {"dt": 0}, {"plan": None}, {"t": -1}, {"g": -1}, {"grad": None}, {"gdt": 1},
                {"q": ctypes.c_void_p(264)}):
         assert wgrad8(**kw) == _lib.INVALID_VALUE, kw
+    def wgrads(dlow=some, low=some, rank=8, x=some, ldx=64, k=64, dy=some, lddy=32, n=32, dt=2, plan=some, t=10, g=3,
+               dd=some, du=some, gdt=0):
+        return lib.kairo_low_rank_wgrads(dlow, low, rank, x, ldx, k, dy, lddy, n, dt, plan, t, g, dd, du, gdt, None)
+
+    for kw in ({"dlow": None}, {"low": None}, {"rank": 0}, {"x": None}, {"ldx": 63}, {"k": 0}, {"dy": None},
+               {"lddy": 31}, {"n": 0}, {"dt": 0}, {"plan": None}, {"t": -1}, {"g": -1}, {"dd": None}, {"du": None},
+               {"gdt": 1}):
+        assert wgrads(**kw) == _lib.INVALID_VALUE, kw
+    assert wgrads(rank=129) == _lib.NOT_SUPPORTED and wgrads(g=0) == _lib.SUCCESS
     assert wgrad(rank=129) == _lib.NOT_SUPPORTED and wgrad8(rank=129) == _lib.NOT_SUPPORTED
     assert wgrad(g=0) == _lib.SUCCESS
