@@ -75,6 +75,9 @@ class LowRankAdapters:
         for t in (self.up, self.scale):
             if t is not None and t.device != self.down.device:
                 raise ValueError("down, up and scale must share a device")
+        # What every call needs, read from the tensors once: (G, R, in, out) and the dtype's code.
+        object.__setattr__(self, "_sizes", (*self.down.shape, self.up.shape[2]))
+        object.__setattr__(self, "_code", _lib.kairo_dtype(self.down.dtype))
 
     @property
     def count(self) -> int:
@@ -132,44 +135,51 @@ def adapter_plan(ids: Tensor, num_adapters: int) -> AdapterPlan:
     return AdapterPlan(memory=mem, num_tokens=n, num_adapters=g)
 
 
-def _check_batch(X, features: int, adapters: LowRankAdapters, plan: AdapterPlan, name: str, op: str) -> None:
-    if len(X.shape) != 2 or X.shape[1] != features:
-        raise ValueError(f"{op}: {name} must be (tokens, {features}), got {tuple(X.shape)}")
-    if X.dtype != adapters.dtype:
-        raise TypeError(f"{op}: {name} is {X.dtype}, the adapters are {adapters.dtype}")
-    if plan.num_tokens != X.shape[0]:
+def _check_batch(op: str, name: str, X, features: int, adapters: LowRankAdapters, plan: AdapterPlan) -> None:
+    if X.shape != (plan.num_tokens, features):
+        if len(X.shape) != 2 or X.shape[1] != features:
+            raise ValueError(f"{op}: {name} must be (tokens, {features}), got {tuple(X.shape)}")
         raise ValueError(f"{op}: the plan is of {plan.num_tokens} tokens, {name} has {X.shape[0]}")
-    if plan.num_adapters != adapters.count:
-        raise ValueError(f"{op}: the plan is of {plan.num_adapters} adapters, not {adapters.count}")
+    if X.dtype != adapters.down.dtype:
+        raise TypeError(f"{op}: {name} is {X.dtype}, the adapters are {adapters.down.dtype}")
+    if plan.num_adapters != adapters._sizes[0]:
+        raise ValueError(f"{op}: the plan is of {plan.num_adapters} adapters, not {adapters._sizes[0]}")
 
 
-def _apply(op: str, index: int, X: Tensor, down: Tensor, up: Tensor, scale: Tensor | None, plan: AdapterPlan,
-           base: Tensor | None, out: Tensor | None, low: Tensor | None) -> None:
-    k, n, dt = down.shape[2], up.shape[2], _lib.kairo_dtype(X.dtype)
+def _apply(op: str, index: int, X: Tensor, down: Tensor, up: Tensor, k: int, n: int, rank: int, code: int,
+           scale: Tensor | None, plan: AdapterPlan, base: Tensor | None, out: Tensor | None,
+           low: Tensor | None) -> None:
+    if base is None:
+        base_ptr, base_ld, base_dt = None, n, code
+    else:
+        base_ptr, base_ld, base_dt = base.data_ptr(), _ld(base), _lib.kairo_dtype(base.dtype)
+    if out is None:
+        out_ptr, out_ld, out_dt = None, n, code
+    else:
+        out_ptr, out_ld, out_dt = out.data_ptr(), _ld(out), _lib.kairo_dtype(out.dtype)
     _lib.launch(op, _lib.lib().kairo_low_rank_apply, index, X.data_ptr(), _ld(X), k, down.data_ptr(), up.data_ptr(), n,
-                down.shape[1], dt, None if scale is None else scale.data_ptr(), plan.memory.data_ptr(),
-                plan.num_tokens, plan.num_adapters,
-                *((None, n, dt) if base is None else (base.data_ptr(), _ld(base), _lib.kairo_dtype(base.dtype))),
-                *((None, n, dt) if out is None else (out.data_ptr(), _ld(out), _lib.kairo_dtype(out.dtype))),
+                rank, code, None if scale is None else scale.data_ptr(), plan.memory.data_ptr(), plan.num_tokens,
+                plan.num_adapters, base_ptr, base_ld, base_dt, out_ptr, out_ld, out_dt,
                 None if low is None else low.data_ptr())
 
 
-def _result(shape: tuple[int, int], base: Tensor | None, out: Tensor | None, dtype: torch.dtype | None,
-            adapters: LowRankAdapters, op: str) -> tuple[Tensor | None, Tensor]:
-    """The checked base (rows contiguous) and the tensor to write."""
-    odt = dtype or (out.dtype if out is not None else adapters.dtype)
-    if odt not in (torch.float32, adapters.dtype):
-        raise TypeError(f"{op}: the output must be float32 or {adapters.dtype}, got {odt}")
+def _result(op: str, like: Tensor, shape: tuple[int, int], base: Tensor | None, out: Tensor | None,
+            dtype: torch.dtype | None) -> tuple[Tensor | None, Tensor]:
+    """The checked base (rows contiguous) and the tensor to write; ``like`` has the adapters' type and device."""
+    own = like.dtype
+    odt = dtype or (own if out is None else out.dtype)
+    if odt != own and odt != torch.float32:
+        raise TypeError(f"{op}: the output must be float32 or {own}, got {odt}")
     if base is not None:
-        if base.shape != shape or base.get_device() != adapters.down.get_device():
-            raise ValueError(f"{op}: base must be {shape} on {adapters.down.device}")
-        if base.dtype not in (torch.float32, adapters.dtype):
-            raise TypeError(f"{op}: base must be float32 or {adapters.dtype}, got {base.dtype}")
+        if base.shape != shape or base.get_device() != like.get_device():
+            raise ValueError(f"{op}: base must be {shape} on {like.device}")
+        if base.dtype != own and base.dtype != torch.float32:
+            raise TypeError(f"{op}: base must be float32 or {own}, got {base.dtype}")
         base = _rows(base)
     if out is None:
-        out = adapters.down.new_empty(shape, dtype=odt)
-    elif out.shape != shape or out.dtype != odt or out.device != adapters.down.device or _rows(out) is not out:
-        raise ValueError(f"{op}: out must be a row-major {shape} {odt} tensor on {adapters.down.device}")
+        out = like.new_empty(shape) if odt == own else like.new_empty(shape, dtype=odt)
+    elif out.shape != shape or out.dtype != odt or out.device != like.device or _rows(out) is not out:
+        raise ValueError(f"{op}: out must be a row-major {shape} {odt} tensor on {like.device}")
     return base, out
 
 
@@ -185,11 +195,13 @@ def adapter_linear(X: Tensor, adapters: LowRankAdapters, plan: AdapterPlan, *, b
     (tokens, rank) float32 values ``scale[a] * X[t] down[a]^T`` that
     ``adapter_linear_backward`` takes."""
     op = "adapter_linear"
+    _, rank, k, n = adapters._sizes
     index = _lib.device_index(op, X, adapters.down, plan.memory)
-    _check_batch(X, adapters.in_features, adapters, plan, "X", op)
-    base, out = _result((X.shape[0], adapters.out_features), base, out, out_dtype, adapters, op)
-    low = X.new_empty((X.shape[0], adapters.rank), dtype=torch.float32) if return_low else None
-    _apply(op, index, _rows(X), adapters.down, adapters.up, adapters.scale, plan, base, out, low)
+    _check_batch(op, "X", X, k, adapters, plan)
+    base, out = _result(op, adapters.down, (plan.num_tokens, n), base, out, out_dtype)
+    low = X.new_empty((plan.num_tokens, rank), dtype=torch.float32) if return_low else None
+    _apply(op, index, _rows(X), adapters.down, adapters.up, k, n, rank, adapters._code, adapters.scale, plan, base, out,
+           low)
     return (out, low) if return_low else out
 
 
@@ -220,40 +232,42 @@ def adapter_linear_backward(dY: Tensor, X: Tensor | QuantizedActivations, adapte
     adapters').  d_down and d_up are in ``grad_dtype`` (default: the
     adapters'), zero for an adapter without tokens."""
     op = "adapter_linear_backward"
+    _, rank, k, n = adapters._sizes
+    down, up, code = adapters.down, adapters.up, adapters._code
+    tokens = plan.num_tokens
     kept = X if isinstance(X, QuantizedActivations) else None
-    index = _lib.device_index(op, dY, kept.codes if kept else X, adapters.down, plan.memory)
-    _check_batch(dY, adapters.out_features, adapters, plan, "dY", op)
-    gdt = grad_dtype or adapters.dtype
-    if gdt not in (torch.float32, adapters.dtype):
-        raise TypeError(f"{op}: the gradients must be float32 or {adapters.dtype}, got {gdt}")
+    index = _lib.device_index(op, dY, kept.codes if kept else X, down, plan.memory)
+    _check_batch(op, "dY", dY, n, adapters, plan)
+    gdt = grad_dtype or down.dtype
+    if gdt != torch.float32 and gdt != down.dtype:
+        raise TypeError(f"{op}: the gradients must be float32 or {down.dtype}, got {gdt}")
     if need_dw:
-        _check_batch(X, adapters.in_features, adapters, plan, "X", op)
+        _check_batch(op, "X", X, k, adapters, plan)
         if kept and low is None:
             raise ValueError(f"{op}: an X in 8 bits needs the low of the forward pass")
-        if low is not None and (tuple(low.shape) != (dY.shape[0], adapters.rank) or low.dtype != torch.float32
-                                or low.device != dY.device):
-            raise ValueError(f"{op}: low must be a ({dY.shape[0]}, {adapters.rank}) float32 tensor")
+        if low is not None and (low.shape != (tokens, rank) or low.dtype != torch.float32
+                                or low.get_device() != index):
+            raise ValueError(f"{op}: low must be a ({tokens}, {rank}) float32 tensor")
     dX = None
     if need_dx:
-        base_dx, dX = _result((dY.shape[0], adapters.in_features), base_dx, None, dx_dtype, adapters, op)
+        base_dx, dX = _result(op, down, (tokens, k), base_dx, None, dx_dtype)
     dY = _rows(dY)
-    dlow = dY.new_empty((dY.shape[0], adapters.rank), dtype=torch.float32) if need_dw else None
+    dlow = dY.new_empty((tokens, rank), dtype=torch.float32) if need_dw else None
     if need_dx or need_dw:
-        _apply(op, index, dY, adapters.up, adapters.down, adapters.scale, plan, base_dx if need_dx else None, dX, dlow)
+        _apply(op, index, dY, up, down, n, k, rank, code, adapters.scale, plan, base_dx if need_dx else None, dX, dlow)
     if not need_dw:
         return dX, None, None
     Z = kept or _rows(X)
     if low is None:
         low = torch.empty_like(dlow)
-        _apply(op, index, Z, adapters.down, adapters.up, adapters.scale, plan, None, None, low)
+        _apply(op, index, Z, down, up, k, n, rank, code, adapters.scale, plan, None, None, low)
     low = low.contiguous()
     if kept:
         return dX, _wgrad(op, index, dlow, Z, plan, gdt), _wgrad(op, index, low, dY, plan, gdt)
-    d_down = dlow.new_empty(adapters.down.shape, dtype=gdt)
-    d_up = dlow.new_empty(adapters.up.shape, dtype=gdt)
-    _lib.launch(op, _lib.lib().kairo_low_rank_wgrads, index, dlow.data_ptr(), low.data_ptr(), adapters.rank,
-                Z.data_ptr(), _ld(Z), adapters.in_features, dY.data_ptr(), _ld(dY), adapters.out_features,
-                _lib.kairo_dtype(dY.dtype), plan.memory.data_ptr(), plan.num_tokens, plan.num_adapters,
+    d_down = torch.empty_like(down) if gdt == down.dtype else down.new_empty(down.shape, dtype=gdt)
+    d_up = torch.empty_like(up) if gdt == up.dtype else up.new_empty(up.shape, dtype=gdt)
+    _lib.launch(op, _lib.lib().kairo_low_rank_wgrads, index, dlow.data_ptr(), low.data_ptr(), rank, Z.data_ptr(),
+                _ld(Z), k, dY.data_ptr(), _ld(dY), n, code, plan.memory.data_ptr(), tokens, plan.num_adapters,
                 d_down.data_ptr(), d_up.data_ptr(), _lib.kairo_dtype(gdt))
     return dX, d_down, d_up
 

@@ -45,7 +45,8 @@ def _rows(t: Tensor) -> Tensor:
 
 
 def _ld(t: Tensor) -> int:
-    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+    n, d = t.shape
+    return max(t.stride(0), d) if n > 1 else d
 
 
 @dataclass(frozen=True)
@@ -108,7 +109,7 @@ def embedding_lookup(weight: Tensor, ids: Tensor, *, scale: float = 1.0, out_dty
     out_dt = _lib.kairo_dtype(odt)
     shape = (*ids.shape, d)
     if out is None:
-        out = weight.new_empty(shape, dtype=odt)
+        out = weight.new_empty(shape) if odt == weight.dtype else weight.new_empty(shape, dtype=odt)
     elif tuple(out.shape) != shape or out.dtype != odt or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {shape} {odt} tensor")
     elif out.device != weight.device:
@@ -155,7 +156,7 @@ def embedding_grad(grad_output: Tensor, ids: Tensor | TokenOrder, num_embeddings
     if accumulate and out is None:
         raise ValueError("accumulate=True needs out")
     if out is None:
-        out = g.new_empty((n_rows, d), dtype=odt)
+        out = g.new_empty((n_rows, d)) if odt == g.dtype else g.new_empty((n_rows, d), dtype=odt)
     elif tuple(out.shape) != (n_rows, d) or out.dtype != odt or out.device != dev or _rows(out) is not out:
         raise ValueError(f"out must be a row-major ({n_rows}, {d}) {odt} tensor on {dev}")
     ws = g.new_empty(_grad_bytes(tokens, d), dtype=torch.uint8)
