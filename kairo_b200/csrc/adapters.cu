@@ -182,15 +182,20 @@ int pick_cluster(int64_t tiles, int64_t k, int64_t n) {
   return c;
 }
 
-// CTAs that share out an adapter's tokens: again as many as fill the GPU once
-// (8192 tokens of 4 adapters, rank 16, 8192 features: 31.9, 29.2 and 36.9 us
-// with 2, 4 and 8), and no more than there are chunks of 64 tokens.
+// CTAs that share out an adapter's tokens.  Requests differ in length, so up to
+// twice what the GPU holds at once: the CTAs of short adapters make room early.
+// Both gradients of 8192 packed tokens of 4 adapters, 8192 features: rank 32
+// (one CTA per SM) 127, 95, 99 and 143 us with 1, 2, 4 and 8; rank 16 (two) 94,
+// 79, 63 and 67.  No more than leave the average adapter's CTAs a chunk of 64
+// tokens each, and two to spare (777 tokens of 5 adapters: 14.5, 10.0, 8.2 and
+// 9.1 us).
 int pick_wgrad_cluster(int64_t ntokens, int64_t nadapters, int64_t k, int64_t rank) {
-  const int64_t groups = rank <= 16 ? 1 : (rank <= 32 ? 2 : (rank <= 64 ? 4 : 8));  // of 16 rank rows
-  const int64_t ctas = ceil_div64(k, 512 / groups) * nadapters;
-  const int64_t room = 2 * device_sm_count(current_device());
+  const int64_t cols = rank <= 32 ? 512 : (rank <= 64 ? 256 : 128);  // features of a CTA
+  const int64_t room = (rank <= 16 ? 2 : 1) * device_sm_count(current_device());
+  const int64_t ctas = ceil_div64(k, cols) * nadapters;
   int c = 1;
-  while (c < kCluster && ctas * 2 * c <= room && c * kChunkTokens < ntokens) c *= 2;
+  while (c < kCluster && ctas * 2 * c <= 2 * room && 2 * c * kChunkTokens <= ntokens / nadapters + 2 * kChunkTokens)
+    c *= 2;
   return c;
 }
 

@@ -729,7 +729,10 @@ cudaError_t pick_apply(const LowRankApplyArgs& a, bool vec, int tile, int64_t cl
 
 // Tile shape and memory of one instance.  A warp owns MR x 16 rank rows and 64
 // features; RG warps side by side cover the rank, kWarps / RG column groups
-// the CTA's features; UNITS steps of 16 tokens in flight.
+// the CTA's features; UNITS steps of 16 tokens in flight.  From rank 17 on a
+// warp takes 32 rank rows and the registers of two CTAs: each z value read by
+// half as many warps is worth more than twice the warps (8192 tokens, 8192
+// features, 4 adapters: rank 32 54 -> 44 us, 64 130 -> 86, 128 293 -> 202).
 template <int RG_, int MR_, int UNITS_>
 struct WgradShape {
   static constexpr int RG = RG_, MR = MR_, UNITS = UNITS_;
@@ -1032,9 +1035,9 @@ cudaError_t launch_wgrad(const LowRankWgradArgs& a, int64_t adapters, int cluste
 template <typename T, typename TG, bool Q8, bool VEC>
 cudaError_t pick_wgrad(const LowRankWgradArgs& a, int64_t adapters, int cluster, cudaStream_t s) {
   if (a.rank <= 16) return launch_wgrad<T, TG, WgradShape<1, 1, 5>, Q8, VEC>(a, adapters, cluster, s);
-  if (a.rank <= 32) return launch_wgrad<T, TG, WgradShape<2, 1, 5>, Q8, VEC>(a, adapters, cluster, s);
-  if (a.rank <= 64) return launch_wgrad<T, TG, WgradShape<4, 1, 5>, Q8, VEC>(a, adapters, cluster, s);
-  return launch_wgrad<T, TG, WgradShape<8, 1, 4>, Q8, VEC>(a, adapters, cluster, s);
+  if (a.rank <= 32) return launch_wgrad<T, TG, WgradShape<1, 2, 8>, Q8, VEC>(a, adapters, cluster, s);
+  if (a.rank <= 64) return launch_wgrad<T, TG, WgradShape<2, 2, 8>, Q8, VEC>(a, adapters, cluster, s);
+  return launch_wgrad<T, TG, WgradShape<4, 2, 4>, Q8, VEC>(a, adapters, cluster, s);
 }
 
 }  // namespace lowrank
