@@ -322,6 +322,23 @@ def device_index(op: str, *tensors: torch.Tensor) -> int:
     return index
 
 
+def refuse_overlap(op: str, out: torch.Tensor, *inputs: torch.Tensor) -> None:
+    """Raises ValueError when ``out`` shares memory with an input: the kernels
+    write it while other threads still read."""
+    def span(t: torch.Tensor) -> tuple[int, int]:
+        start = t.data_ptr()
+        return start, start + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+    if out.numel() == 0:
+        return
+    lo, hi = span(out)
+    for t in inputs:
+        if t.numel():
+            a, b = span(t)
+            if a < hi and lo < b:
+                raise ValueError(f"{op}: out must not share memory with an input")
+
+
 def launch(op: str, fn, index: int, *args) -> None:
     """``fn(*args, stream)`` on the current stream of device ``index``, its
     status checked.  The device is switched only when it is not the current

@@ -166,15 +166,15 @@ int pick_tile(int64_t t, int64_t rank, bool vec) {
 }
 
 // CTAs per tile, a power of two up to 8.  As many as the GPU holds at once (two
-// CTAs per SM) gives the shortest calls: 96 tokens in 71 tiles of 8192
+// CTAs per SM; one where the low tile is large) gives the shortest calls: 96 tokens in 71 tiles of 8192
 // features took 20.2, 12.8, 12.3 and 15.7 us with clusters of 1, 2, 4 and 8;
 // 8192 tokens in 260 tiles 96, 103, 101 and 124 us. But no more than leave
 // every warp a turn of 64 features (777 tokens, 1000 features: 6.1 us with
 // two, 12.3 with eight), and where the contraction is so long that a warp has
 // 32 turns, more, shorter CTAs even out the SMs (8192 tokens, 32768 features:
 // 142 us with two, 139 with four).
-int pick_cluster(int64_t tiles, int64_t k, int64_t n) {
-  const int64_t room = 2 * device_sm_count(current_device());
+int pick_cluster(int64_t tiles, int tile, int64_t k, int64_t n, int64_t rank) {
+  const int64_t room = (tile * rank > 1024 ? 1 : 2) * device_sm_count(current_device());
   int c = 1;
   while (c < kCluster && (tiles * 2 * c <= room || k >= int64_t(32) * 8 * 64 * c) &&
          int64_t(2) * c * 8 * 64 <= std::max(k, n) + 511)
@@ -281,7 +281,7 @@ extern "C" kairo_status kairo_low_rank_apply(const void* x, int64_t ldx, int64_t
   a.rank = static_cast<int32_t>(rank);
   a.base_f32 = base && base_dtype == KAIRO_DTYPE_F32;
   const int64_t clusters = max_tiles(ntokens, nadapters, tile);
-  const int cluster = pick_cluster(clusters, k, n);
+  const int cluster = pick_cluster(clusters, tile, k, n, rank);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool yf = y && y_dtype == KAIRO_DTYPE_F32;
   const cudaError_t err = dtype == KAIRO_DTYPE_F16

@@ -30,6 +30,7 @@ from dataclasses import dataclass
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from kairo_b200 import _lib
 from kairo_b200.ops.backward import (
@@ -191,13 +192,16 @@ def adapter_linear(X: Tensor, adapters: LowRankAdapters, plan: AdapterPlan, *, b
     X: (tokens, in_features) in the adapters' dtype; base: (tokens,
     out_features) in that dtype or float32, None for zero.  The sum is formed
     in fp32 and rounded once to ``out_dtype`` (default: the adapters').
-    ``out`` may be ``base`` itself.  ``return_low=True`` also returns the
+    ``out`` may be ``base`` itself, and shares no memory with an input
+    otherwise.  ``return_low=True`` also returns the
     (tokens, rank) float32 values ``scale[a] * X[t] down[a]^T`` that
     ``adapter_linear_backward`` takes."""
     op = "adapter_linear"
     _, rank, k, n = adapters._sizes
     index = _lib.device_index(op, X, adapters.down, plan.memory)
     _check_batch(op, "X", X, k, adapters, plan)
+    if out is not None:
+        _lib.refuse_overlap(op, out, X, adapters.down, adapters.up, *(() if base is None or base is out else (base,)))
     base, out = _result(op, adapters.down, (plan.num_tokens, n), base, out, out_dtype)
     low = X.new_empty((plan.num_tokens, rank), dtype=torch.float32) if return_low else None
     _apply(op, index, _rows(X), adapters.down, adapters.up, k, n, rank, adapters._code, adapters.scale, plan, base, out,
@@ -307,6 +311,7 @@ class _AdaptedLinearFn(torch.autograd.Function):
         return Y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dY: Tensor):
         blocks, down, up, low, *kept = ctx.saved_tensors
         module: AdaptedSparseLinear = ctx.module
@@ -346,6 +351,8 @@ class AdaptedSparseLinear(torch.nn.Module):
         if num_adapters < 1 or not 1 <= rank <= MAX_RANK:
             raise ValueError(f"num_adapters must be positive and the rank 1 to {MAX_RANK}")
         dev, dt = layer.blocks.device, layer.blocks.dtype
+        if dt not in (torch.float16, torch.bfloat16):
+            raise TypeError(f"adapters must be float16 or bfloat16; the layer is {dt}")
         self.layer = layer
         self.down = torch.nn.Parameter((torch.randn(num_adapters, rank, in_features, device=dev)
                                         * in_features**-0.5).to(dt))

@@ -173,27 +173,32 @@ class _SparseLinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, X: Tensor, blocks: Tensor, module: "BlockSparseLinear") -> Tensor:
         W = module.weight_matrix(blocks)
+        # X is kept for dW alone: in 8 bits where the module says so, and not at
+        # all by a frozen layer that says so.
         ctx.kept_dtype = None
-        if module.checkpoint is not None and ctx.needs_input_grad[1]:
+        ctx.x_dtype = X.dtype
+        if module.checkpoint is None:
+            ctx.save_for_backward(X, blocks)
+        elif ctx.needs_input_grad[1]:
             q = quantize_activations(X)
             ctx.save_for_backward(q.codes, q.steps, blocks)
             ctx.kept_dtype = q.dtype
         else:
-            ctx.save_for_backward(X, blocks)
+            ctx.save_for_backward(None, blocks)
         ctx.module = module
         return sparse_linear(X, W)
 
     @staticmethod
     def backward(ctx, dY: Tensor):
-        if ctx.kept_dtype is not None:
-            codes, steps, blocks = ctx.saved_tensors
-            X = QuantizedActivations(codes=codes, steps=steps, dtype=ctx.kept_dtype)
-        else:
-            X, blocks = ctx.saved_tensors
+        *kept, blocks = ctx.saved_tensors
+        X = kept[0] if ctx.kept_dtype is None else QuantizedActivations(codes=kept[0], steps=kept[1],
+                                                                         dtype=ctx.kept_dtype)
         module: BlockSparseLinear = ctx.module
         W = module.weight_matrix(blocks)
         wt = transpose_values(W, module.transposed())
         dY = dY.contiguous()
+        if X is None:
+            return (sparse_linear(dY, wt.matrix, out_dtype=ctx.x_dtype) if ctx.needs_input_grad[0] else None), None, None
         dX, dW = sparse_linear_backward(dY, X, W, wt, need_dx=ctx.needs_input_grad[0],
                                         need_dw=ctx.needs_input_grad[1], dw_dtype=blocks.dtype)
         return dX, dW, None

@@ -121,6 +121,8 @@ def dequantize_activations(q: QuantizedActivations, *, out: Tensor | None = None
     elif tuple(out.shape) != (n, k) or out.dtype != q.dtype or out.device != q.device or (
             k > 1 and out.stride(1) != 1) or (n > 1 and out.stride(0) < k):
         raise ValueError(f"out must be a row-major ({n}, {k}) {q.dtype} tensor on {q.device}")
+    else:
+        _lib.refuse_overlap("dequantize_activations", out, q.codes, q.steps)
     _lib.launch("dequantize_activations", _lib.lib().kairo_dequantize_q8, index, q.codes.data_ptr(), q._ldq,
                 q.steps.data_ptr(), q._lds, n, k, out.data_ptr(), max(out.stride(0), k), _lib.kairo_dtype(q.dtype))
     return out

@@ -24,6 +24,7 @@ from dataclasses import dataclass
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from kairo_b200 import _lib
 
@@ -114,6 +115,8 @@ def embedding_lookup(weight: Tensor, ids: Tensor, *, scale: float = 1.0, out_dty
         raise ValueError(f"out must be a contiguous {shape} {odt} tensor")
     elif out.device != weight.device:
         raise ValueError("out must be on the weight's device")
+    else:
+        _lib.refuse_overlap("embedding_lookup", out, weight, flat)
     w = _rows(weight)
     _lib.launch("embedding_lookup", _lib.lib().kairo_embedding_lookup, index, w.data_ptr(), n, d, _ld(w), in_dt,
                 flat.data_ptr(), flat.element_size(), flat.numel(), float(scale), out.data_ptr(), out_dt)
@@ -159,6 +162,8 @@ def embedding_grad(grad_output: Tensor, ids: Tensor | TokenOrder, num_embeddings
         out = g.new_empty((n_rows, d)) if odt == g.dtype else g.new_empty((n_rows, d), dtype=odt)
     elif tuple(out.shape) != (n_rows, d) or out.dtype != odt or out.device != dev or _rows(out) is not out:
         raise ValueError(f"out must be a row-major ({n_rows}, {d}) {odt} tensor on {dev}")
+    else:
+        _lib.refuse_overlap("embedding_grad", out, g, where)
     ws = g.new_empty(_grad_bytes(tokens, d), dtype=torch.uint8)
     tail = (tokens, n_rows, d, float(scale), out.data_ptr(), _ld(out), out_dt, 1 if accumulate else 0, ws.data_ptr(),
             ws.numel())
@@ -180,6 +185,7 @@ class _LookupFn(torch.autograd.Function):
         return embedding_lookup(weight, ids, scale=scale, out_dtype=out_dtype)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad: Tensor):
         (ids,) = ctx.saved_tensors
         return embedding_grad(grad, ids, ctx.rows, scale=ctx.scale, out_dtype=ctx.dtype), None, None, None

@@ -241,6 +241,44 @@ def test_refusals_on_the_device():
         adapter_plan(torch.zeros(4, device=DEV), 3)
 
 
+def test_out_must_not_share_memory():
+    x, dy, a, ids = _problem(torch.bfloat16, 10, 64, 64, 8, 3, seed=5)
+    plan = adapter_plan(ids.to(DEV), 3)
+    with pytest.raises(ValueError, match="share memory"):
+        adapter_linear(x, a, plan, out=x)
+    wide = torch.zeros(11, 64, device=DEV, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="share memory"):
+        adapter_linear(x, a, plan, base=wide[1:], out=wide[:10])  # base, shifted by a row
+    adapter_linear(x, a, plan, base=wide[:10], out=wide[1:11].clone())
+    with pytest.raises(TypeError):
+        AdaptedSparseLinear(BlockSparseLinear(bsr_from_tiles(
+            torch.zeros(1, 64, 64, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV),
+            torch.zeros(1, dtype=torch.int32, device=DEV), (64, 64))), 2, 8)
+
+
+def test_two_calls_at_once():
+    """Two batches on two streams through the same adapters, started together."""
+    x, dy, a, _ = _problem(torch.bfloat16, 300, 512, 384, 16, 4, seed=13)
+    ids = [torch.randint(-1, 4, (300,), device=DEV) for _ in range(2)]
+    xs = [x, x.flip(0).contiguous()]
+
+    def step(k):
+        plan = adapter_plan(ids[k], 4)
+        y, low = adapter_linear(xs[k], a, plan, return_low=True)
+        return (y, *adapter_linear_backward(dy, xs[k], a, plan, low=low))
+
+    ref = [step(0), step(1)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    out = [[], []]
+    for _ in range(4):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                out[k].append(step(k))
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for k in range(2) for o in out[k] for p, q in zip(o, ref[k]))
+
+
 def test_backward_parts_and_checkpoint():
     x, dy, a, ids = _problem(torch.bfloat16, 150, 320, 128, 16, 3, seed=6)
     plan = adapter_plan(ids.to(DEV), 3)

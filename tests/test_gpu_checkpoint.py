@@ -224,7 +224,21 @@ def test_module_keeps_its_input_in_8_bits():
     saved.clear()
     with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
         kept(xs[1])
-    assert not any(t.dtype == torch.int8 for t in saved)
+    assert not any(t.dtype == torch.int8 or t.shape == x.shape for t in saved)
+    xg = x.clone().requires_grad_()
+    kept(xg).backward(dy)
+    assert torch.equal(xg.grad, xs[0].grad)
+
+
+def test_out_must_not_share_memory():
+    x = torch.randn(8, 64, device=DEV)
+    q = quantize_activations(x)
+    buf = torch.empty(8 * 64 * 4, dtype=torch.uint8, device=DEV)
+    codes = buf[:512].view(torch.int8).view(8, 64)
+    codes.copy_(q.codes)
+    with pytest.raises(ValueError, match="share memory"):
+        dequantize_activations(QuantizedActivations(codes=codes, steps=q.steps, dtype=torch.float32),
+                               out=buf.view(torch.float32).view(8, 64))
 
 
 def test_streams_and_graph():

@@ -255,3 +255,48 @@ def test_streams_and_graph():
         torch.cuda.synchronize()
         assert torch.equal(f, embedding_lookup(w, new, scale=2.0))
         assert torch.equal(g, embedding_grad(grad, new, n, scale=2.0))
+
+
+def test_out_must_not_share_memory():
+    w = torch.randn(20, 16, device=DEV)
+    ids = torch.arange(4, device=DEV)
+    with pytest.raises(ValueError, match="share memory"):
+        embedding_lookup(w, ids, out=w[2:6])
+    with pytest.raises(ValueError, match="share memory"):
+        embedding_grad(w[:4], ids, 20, out=w)
+    embedding_lookup(w, ids, out=torch.empty(4, 16, device=DEV))
+    with pytest.raises(TypeError):
+        embedding_lookup(w, ids.float())
+    with pytest.raises(ValueError):
+        embedding_grad(w[:3], ids, 20)
+    with pytest.raises(ValueError):
+        embedding_grad(w[:4], ids, 20, accumulate=True)
+    with pytest.raises(ValueError):
+        embedding_grad(w[:4], sort_tokens(ids, 19), 20)
+
+
+def test_second_derivative_is_refused():
+    m = ScaledEmbedding(10, 8, device=DEV)
+    out = m(torch.arange(4, device=DEV))
+    (g,) = torch.autograd.grad(out.square().sum(), m.weight, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+@pytest.mark.parametrize("tokens", [400, 3000, 70000])
+def test_two_calls_at_once(tokens):
+    """Gradients of two batches on two streams, started together, with no work between them to order them."""
+    n, d = 700, 64
+    grads = [torch.randn(tokens, d, device=DEV) for _ in range(2)]
+    ids = [_ids(n, tokens, seed=i, skew=3.0).to(DEV) for i in range(2)]
+    ref = [embedding_grad(g, i, n) for g, i in zip(grads, ids)]
+    _check_grad(grads[0], ids[0], n, 1.0, ref[0])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    out = [[], []]
+    for _ in range(5):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                out[k].append(embedding_grad(grads[k], ids[k], n))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, ref[k]) for k in range(2) for o in out[k])
