@@ -77,6 +77,19 @@ __device__ __forceinline__ void store_f32(T* p, const float (&f)[N]) {
   }
 }
 
+// The same N elements as they are stored, converted when they are used: half the
+// registers of fp32 values while 16-bit loads are under way.
+template <typename T, int N>
+struct Raw {
+  static constexpr int P = N * static_cast<int>(sizeof(T)) > 16 ? 16 / static_cast<int>(sizeof(T)) : N;
+  Pack<T, P> piece[N / P];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int q = 0; q < N / P; ++q) piece[q].raw = *reinterpret_cast<const decltype(piece[q].raw)*>(p + q * P);
+  }
+  __device__ __forceinline__ float operator[](int i) const { return to_f32<T>(piece[i / P].v[i % P]); }
+};
+
 inline int element_bytes(kairo_dtype d) { return d == KAIRO_DTYPE_F32 ? 4 : 2; }
 inline bool known_dtype(kairo_dtype d) {
   return d == KAIRO_DTYPE_F32 || d == KAIRO_DTYPE_F16 || d == KAIRO_DTYPE_BF16;

@@ -212,10 +212,12 @@ int sort_passes(int64_t n_rows) { return (key_bits(n_rows) + 7) / 8; }
 
 // The whole sort in one cluster.  CTA c holds positions c * per ..; in a pass
 // every warp ranks its share of them in order, the digit counts of all CTAs
-// are read over distributed shared memory, and each key and position is stored
-// straight into the shared memory of the CTA that holds its place (the last
-// pass: into the result).  32768 tokens of 131072 rows, two passes of 9 bits:
-// 15 us, where three passes of three launches took 74.
+// are read over distributed shared memory, the CTA brings its keys into digit
+// order, and each is stored straight into the shared memory of the CTA that
+// holds its place (the last pass: into the result), equal digits side by side.
+//
+// Clusters behind the first zero rows of the gradient meanwhile, which the
+// other SMs have time for.
 constexpr int kClusterThreads = 1024;
 constexpr int kClusterWarps = kClusterThreads / 32;
 constexpr int kClusterItems = 8;   // positions per thread at most
@@ -225,8 +227,14 @@ constexpr int kMaxBins = 1 << kMaxDigit;
 constexpr int64_t kClusterTokens = int64_t(kClusterMax) * kClusterItems * kClusterThreads;
 
 size_t cluster_sort_smem(int per) {
-  return static_cast<size_t>(per) * 16 + static_cast<size_t>(kClusterWarps * kMaxBins + 2 * kMaxBins + 64) * 4;
+  return static_cast<size_t>(per) * 16 + static_cast<size_t>(kClusterWarps * kMaxBins + 3 * kMaxBins + 64) * 4;
 }
+
+// Rows to zero: `vecs` 16-byte vectors each, `pitch` of them apart.
+struct ZeroRows {
+  uint4* first;
+  int64_t rows, vecs, pitch;
+};
 
 __device__ __forceinline__ uint32_t cta_of(uint32_t addr, uint32_t rank) {
   uint32_t r;
@@ -237,44 +245,78 @@ __device__ __forceinline__ void all_ctas() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
+// Exclusive scan of v over the CTA's threads.
+__device__ __forceinline__ uint32_t scan_cta(uint32_t v, uint32_t* sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) sums[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    uint32_t s = sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += y;
+    }
+    sums[lane] = s;
+  }
+  __syncthreads();
+  const uint32_t out = x - v + (warp ? sums[warp - 1] : 0u);
+  __syncthreads();
+  return out;
+}
+
 template <typename ID>
 __global__ void __launch_bounds__(kClusterThreads) k_sort_cluster(const ID* __restrict__ ids, int n, int64_t n_rows,
                                                                   int per, int passes, int digit,
                                                                   uint32_t* __restrict__ sorted,
-                                                                  int32_t* __restrict__ perm) {
+                                                                  int32_t* __restrict__ perm, const ZeroRows zero) {
   extern __shared__ __align__(16) uint32_t sm[];
   uint32_t* keys = sm;                              // [2][per]
   uint32_t* vals = keys + 2 * per;                  // [2][per]
   uint32_t* where = vals + 2 * per;                 // [kClusterWarps][bins]
   uint32_t* total = where + kClusterWarps * kMaxBins;  // [bins]: this CTA's count of every digit
-  uint32_t* base = total + kMaxBins;                // [bins]: first place of this CTA's keys of a digit
+  uint32_t* local = total + kMaxBins;               // [bins]: first of a digit in the CTA's own order
+  uint32_t* base = local + kMaxBins;                // [bins]: place of that one in the whole order
   uint32_t* sums = base + kMaxBins;                 // [32]
   uint32_t crank, csize;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(crank));
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(csize));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (blockIdx.x >= csize) {  // not the sorting cluster
+    const int64_t warps = static_cast<int64_t>(gridDim.x - csize) * kClusterWarps;
+    for (int64_t r = static_cast<int64_t>(blockIdx.x - csize) * kClusterWarps + warp; r < zero.rows; r += warps)
+      for (int64_t v = lane; v < zero.vecs; v += 32) zero.first[r * zero.pitch + v] = make_uint4(0u, 0u, 0u, 0u);
+    return;
+  }
   const int bins = 1 << digit;
   const int first = static_cast<int>(crank) * per;
+  const int have = max(0, min(per, n - first));     // positions of this CTA
   const int share = per / kClusterWarps;            // consecutive positions of a warp
-  for (int i = threadIdx.x; i < per; i += kClusterThreads) {
-    const bool ok = first + i < n;
-    keys[i] = ok ? token_key(ids, first + i, n_rows) : 0u;
+  for (int i = threadIdx.x; i < have; i += kClusterThreads) {
+    keys[i] = token_key(ids, first + i, n_rows);
     vals[i] = static_cast<uint32_t>(first + i);
   }
   for (int p = 0; p < passes; ++p) {
     const int shift = p * digit;
-    const uint32_t* from_k = keys + (p & 1) * per;
-    const uint32_t* from_v = vals + (p & 1) * per;
+    uint32_t* from_k = keys + (p & 1) * per;
+    uint32_t* from_v = vals + (p & 1) * per;
     for (int i = threadIdx.x; i < kClusterWarps * bins; i += kClusterThreads) where[i] = 0;
     __syncthreads();
-    uint32_t key[kClusterItems], rank[kClusterItems];
+    uint32_t key[kClusterItems], val[kClusterItems], rank[kClusterItems];
     uint32_t* mine = where + warp * bins;
 #pragma unroll
     for (int j = 0; j < kClusterItems; ++j) {
       if (j * 32 < share) {
         const int i = warp * share + j * 32 + lane;
-        const bool ok = first + i < n;
-        key[j] = from_k[i];
+        const bool ok = i < have;
+        key[j] = ok ? from_k[i] : 0u;
+        val[j] = ok ? from_v[i] : 0u;
         const uint32_t d = (key[j] >> shift) & (bins - 1);
         const uint32_t same = same_digit(d, ok, digit);
         const int leader = ok ? __ffs(same) - 1 : lane;
@@ -289,16 +331,18 @@ __global__ void __launch_bounds__(kClusterThreads) k_sort_cluster(const ID* __re
       }
     }
     __syncthreads();
+    uint32_t here = 0;
     if (threadIdx.x < bins) {
-      uint32_t at = 0;
 #pragma unroll 8
       for (int w = 0; w < kClusterWarps; ++w) {
         const uint32_t c = where[w * bins + threadIdx.x];
-        where[w * bins + threadIdx.x] = at;
-        at += c;
+        where[w * bins + threadIdx.x] = here;
+        here += c;
       }
-      total[threadIdx.x] = at;
+      total[threadIdx.x] = here;
     }
+    const uint32_t before_here = scan_cta(here, sums);
+    if (threadIdx.x < bins) local[threadIdx.x] = before_here;
     all_ctas();
     // Keys of smaller digits anywhere, and of this digit in CTAs before this one.
     uint32_t all = 0, before = 0;
@@ -316,45 +360,33 @@ __global__ void __launch_bounds__(kClusterThreads) k_sort_cluster(const ID* __re
         if (r < crank) before += c[r];
       }
     }
-    uint32_t x = all;
+    const uint32_t smaller = scan_cta(all, sums);
+    if (threadIdx.x < bins) base[threadIdx.x] = smaller + before;
+    // This CTA's keys in the order of their digits.
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    if (lane == 31) sums[warp] = x;
-    __syncthreads();
-    if (warp == 0) {
-      uint32_t s = sums[lane];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t y = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += y;
+    for (int j = 0; j < kClusterItems; ++j) {
+      if (j * 32 < share && warp * share + j * 32 + lane < have) {
+        const uint32_t d = (key[j] >> shift) & (bins - 1);
+        const uint32_t at = local[d] + mine[d] + rank[j];
+        from_k[at] = key[j];
+        from_v[at] = val[j];
       }
-      sums[lane] = s;
     }
-    __syncthreads();
-    if (threadIdx.x < bins) base[threadIdx.x] = x - all + (warp ? sums[warp - 1] : 0u) + before;
     __syncthreads();
     const bool last = p + 1 == passes;
     const uint32_t to_k = static_cast<uint32_t>(__cvta_generic_to_shared(keys + ((p + 1) & 1) * per));
     const uint32_t to_v = static_cast<uint32_t>(__cvta_generic_to_shared(vals + ((p + 1) & 1) * per));
-#pragma unroll
-    for (int j = 0; j < kClusterItems; ++j) {
-      if (j * 32 < share) {
-        const int i = warp * share + j * 32 + lane;
-        if (first + i < n) {
-          const uint32_t d = (key[j] >> shift) & (bins - 1);
-          const uint32_t at = base[d] + mine[d] + rank[j];
-          if (last) {
-            sorted[at] = key[j];
-            perm[at] = static_cast<int32_t>(from_v[i]);
-          } else {
-            const uint32_t cta = at / static_cast<uint32_t>(per), off = 4u * (at - cta * per);
-            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cta_of(to_k + off, cta)), "r"(key[j]) : "memory");
-            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cta_of(to_v + off, cta)), "r"(from_v[i]) : "memory");
-          }
-        }
+    for (int i = threadIdx.x; i < have; i += kClusterThreads) {
+      const uint32_t k = from_k[i], v = from_v[i];
+      const uint32_t d = (k >> shift) & (bins - 1);
+      const uint32_t at = base[d] + (static_cast<uint32_t>(i) - local[d]);
+      if (last) {
+        sorted[at] = k;
+        perm[at] = static_cast<int32_t>(v);
+      } else {
+        const uint32_t cta = at / static_cast<uint32_t>(per), off = 4u * (at - cta * per);
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cta_of(to_k + off, cta)), "r"(k) : "memory");
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cta_of(to_v + off, cta)), "r"(v) : "memory");
       }
     }
     all_ctas();  // the next pass reads what the others stored here
@@ -363,7 +395,7 @@ __global__ void __launch_bounds__(kClusterThreads) k_sort_cluster(const ID* __re
 
 template <typename ID>
 kairo_status sort_in_cluster(const ID* ids, int64_t n, int64_t n_rows, uint32_t* sorted, int32_t* perm,
-                             cudaStream_t s) {
+                             const ZeroRows& zero, cudaStream_t s) {
   int ctas = 1;
   while (ctas < kClusterMax && ctas * kClusterThreads < n) ctas *= 2;
   const int per = static_cast<int>(ceil_div64(ceil_div64(n, ctas), kClusterThreads)) * kClusterThreads;
@@ -374,8 +406,10 @@ kairo_status sort_in_cluster(const ID* ids, int64_t n, int64_t n_rows, uint32_t*
   cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        static_cast<int>(cluster_sort_smem(kClusterItems * kClusterThreads)));
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(token sort)");
+  // as many zeroing clusters as leave room for the sort
+  const int spare = zero.rows > 0 ? std::max(0, device_sm_count(current_device()) / ctas - 2) : 0;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas * (1 + spare)));
   cfg.blockDim = dim3(kClusterThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -387,7 +421,7 @@ kairo_status sort_in_cluster(const ID* ids, int64_t n, int64_t n_rows, uint32_t*
   cfg.attrs = &at;
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, fn, ids, static_cast<int>(n), n_rows, per, passes, (bits + passes - 1) / passes, sorted,
-                         perm);
+                         perm, zero);
   if (e != cudaSuccess) return cuda_fail(e, "launch of the token sort");
   return KAIRO_STATUS_SUCCESS;
 }
@@ -402,8 +436,8 @@ size_t sort_ws_bytes(int64_t n) {
 
 template <typename ID>
 kairo_status sort_launch(const ID* ids, int64_t n, int64_t n_rows, uint32_t* sorted, int32_t* perm, void* ws,
-                         cudaStream_t s) {
-  if (n <= kClusterTokens) return sort_in_cluster(ids, n, n_rows, sorted, perm, s);
+                         const ZeroRows& zero, cudaStream_t s) {
+  if (n <= kClusterTokens) return sort_in_cluster(ids, n, n_rows, sorted, perm, zero, s);
   const size_t col = align_up(static_cast<size_t>(n) * 4, 256);
   uint32_t* keys_b = static_cast<uint32_t*>(ws);
   int32_t* vals_b = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(ws) + col);
@@ -434,7 +468,7 @@ kairo_status sort_launch(const ID* ids, int64_t n, int64_t n_rows, uint32_t* sor
 constexpr int kGradThreads = 128;
 constexpr int kGradChunk = 32;   // sorted positions per chunk
 constexpr int kGradAhead = 8;    // rows under way per thread
-constexpr int kZeroRows = 32;    // rows of a zeroing CTA
+constexpr int kFewRows = 32;     // rows of a CTA that takes a short list
 
 template <typename TO, int VE>
 __device__ __forceinline__ void emit_row(TO* dst, float (&acc)[VE], float scale, bool accumulate) {
@@ -445,25 +479,32 @@ __device__ __forceinline__ void emit_row(TO* dst, float (&acc)[VE], float scale,
   store_f32<TO, VE>(dst, f);
 }
 
-// Rows r0 .. r0 + 31: zeros where no token has the row's id.
+// Rows r0 .. r0 + kZeroCtaRows - 1: zeros where no token has the row's id.  A
+// thread per row looks its id up in the sorted list; the more rows share that
+// wait (some 15 dependent reads), the less of the time it is.
+constexpr int kZeroCtaRows = 64;
 template <typename TO, int VE>
 __device__ __forceinline__ void zero_rows(const uint32_t* __restrict__ sorted, int64_t n, int64_t n_rows, int64_t dim,
                                           TO* __restrict__ out, int64_t ldo, int64_t r0) {
+  __shared__ uint32_t masks[kZeroCtaRows / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = r0 + lane;
-  int64_t lo = 0, hi = n;  // first position whose id is >= row
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (sorted[mid] < row) lo = mid + 1;
-    else hi = mid;
+  if (threadIdx.x < kZeroCtaRows) {
+    const int64_t row = r0 + threadIdx.x;
+    int64_t lo = 0, hi = n;  // first position whose id is >= row
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (sorted[mid] < row) lo = mid + 1;
+      else hi = mid;
+    }
+    const uint32_t mask = __ballot_sync(0xffffffffu, row < n_rows && !(lo < n && sorted[lo] == row));
+    if (lane == 0) masks[warp] = mask;
   }
-  const bool empty = row < n_rows && !(lo < n && sorted[lo] == row);
-  const uint32_t mask = __ballot_sync(0xffffffffu, empty);
+  __syncthreads();
   float zero[VE];
 #pragma unroll
   for (int i = 0; i < VE; ++i) zero[i] = 0.f;
-  for (int r = warp; r < kZeroRows; r += kGradThreads / 32) {
-    if (!((mask >> r) & 1u)) continue;
+  for (int r = warp; r < kZeroCtaRows; r += kGradThreads / 32) {
+    if (!((masks[r >> 5] >> (r & 31)) & 1u)) continue;
     TO* dst = out + (r0 + r) * ldo;
     for (int64_t c = static_cast<int64_t>(lane) * VE; c < dim; c += 32 * VE) store_f32<TO, VE>(dst + c, zero);
   }
@@ -473,13 +514,17 @@ __device__ __forceinline__ void zero_rows(const uint32_t* __restrict__ sorted, i
 // those behind them zero the rows without tokens.  Partial rows: 2 * chunk is
 // the part of a run that began before the chunk, 2 * chunk + 1 the part of a
 // run that begins in it and goes on behind it.
-template <typename TI, typename TO, int VE>
-__global__ void __launch_bounds__(kGradThreads) k_grad_chunks(
+//
+// Bound by memory: 32768 x 2048 bf16 tokens of some 20000 ids into 131072 rows are
+// 134 MB read and 537 MB written, of which zeros alone take 90 us (a memset of
+// the table takes 136).
+template <typename TI, typename TO, int VE, bool ADD>
+__global__ void __launch_bounds__(kGradThreads, 8) k_grad_chunks(
     const TI* __restrict__ grad, int64_t ldg, const uint32_t* __restrict__ sorted, const int32_t* __restrict__ perm,
-    int64_t n, int64_t n_rows, int64_t dim, float scale, TO* __restrict__ out, int64_t ldo, bool accumulate,
-    float* __restrict__ partial, int64_t chunks, int slices) {
+    int64_t n, int64_t n_rows, int64_t dim, float scale, TO* __restrict__ out, int64_t ldo,
+    float* __restrict__ partial, int64_t chunks, int slices, int64_t zero_rows_end) {
   if (static_cast<int64_t>(blockIdx.x) >= chunks * slices) {
-    zero_rows<TO, VE>(sorted, n, n_rows, dim, out, ldo, (blockIdx.x - chunks * slices) * kZeroRows);
+    zero_rows<TO, VE>(sorted, n, zero_rows_end, dim, out, ldo, (blockIdx.x - chunks * slices) * kZeroCtaRows);
     return;
   }
   // The chunk's ids with their neighbours on both sides (n_rows + 1: none), and its tokens.
@@ -500,33 +545,42 @@ __global__ void __launch_bounds__(kGradThreads) k_grad_chunks(
   if (col >= dim) return;
   const int have = static_cast<int>(min(static_cast<int64_t>(kGradChunk), n - p0));
   bool open_left = key[0] == key[1];
+  constexpr int AHEAD = ADD ? kGradAhead / 2 : kGradAhead;
   float acc[VE];
 #pragma unroll
   for (int i = 0; i < VE; ++i) acc[i] = 0.f;
 #pragma unroll 1
-  for (int q0 = 0; q0 < have; q0 += kGradAhead) {
-    float f[kGradAhead][VE];
+  for (int q0 = 0; q0 < have; q0 += AHEAD) {
+    Raw<TI, VE> f[AHEAD];
+    Raw<TO, VE> old[ADD ? AHEAD : 1];  // of the rows that end here
 #pragma unroll
-    for (int u = 0; u < kGradAhead; ++u) {
+    for (int u = 0; u < AHEAD; ++u) {
       const int q = q0 + u;
       if (q < have && key[q + 1] < n_rows && tok[q] >= 0) {
-        load_f32<TI, VE>(grad + static_cast<int64_t>(tok[q]) * ldg + col, f[u]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VE; ++i) f[u][i] = 0.f;
+        f[u].load(grad + static_cast<int64_t>(tok[q]) * ldg + col);
+        if (ADD && key[q + 1] != key[q + 2]) old[u].load(out + static_cast<int64_t>(key[q + 1]) * ldo + col);
       }
     }
 #pragma unroll
-    for (int u = 0; u < kGradAhead; ++u) {
+    for (int u = 0; u < AHEAD; ++u) {
       const int q = q0 + u;
       if (q >= have || key[q + 1] >= n_rows) break;  // ids out of range come last
+      if (tok[q] >= 0) {
 #pragma unroll
-      for (int i = 0; i < VE; ++i) acc[i] += f[u][i];
+        for (int i = 0; i < VE; ++i) acc[i] += f[u][i];
+      }
       const bool last = key[q + 1] != key[q + 2];
       if (last || q + 1 == have) {
-        if (open_left) store_f32<float, VE>(partial + (2 * chunk) * dim + col, acc);
-        else if (!last) store_f32<float, VE>(partial + (2 * chunk + 1) * dim + col, acc);
-        else emit_row<TO, VE>(out + static_cast<int64_t>(key[q + 1]) * ldo + col, acc, scale, accumulate);
+        if (open_left) {
+          store_f32<float, VE>(partial + (2 * chunk) * dim + col, acc);
+        } else if (!last) {
+          store_f32<float, VE>(partial + (2 * chunk + 1) * dim + col, acc);
+        } else if (!ADD || tok[q] >= 0) {
+          float v[VE];
+#pragma unroll
+          for (int i = 0; i < VE; ++i) v[i] = ADD ? old[ADD ? u : 0][i] + acc[i] * scale : acc[i] * scale;
+          store_f32<TO, VE>(out + static_cast<int64_t>(key[q + 1]) * ldo + col, v);
+        }
         open_left = false;
 #pragma unroll
         for (int i = 0; i < VE; ++i) acc[i] = 0.f;
@@ -538,7 +592,7 @@ __global__ void __launch_bounds__(kGradThreads) k_grad_chunks(
 // The chunk in which a run begins that goes on behind it adds up the run's
 // parts: kJoinGroups groups of threads take turns of kGradAhead parts each, in
 // order, and their sums are added in the order of the groups.
-constexpr int kJoinGroups = 4;
+constexpr int kJoinGroups = 2;
 template <typename TO, int VE>
 __global__ void __launch_bounds__(kGradThreads * kJoinGroups) k_grad_join(const uint32_t* __restrict__ sorted,
                                                                           int64_t n, int64_t n_rows, int64_t dim,
@@ -549,9 +603,9 @@ __global__ void __launch_bounds__(kGradThreads * kJoinGroups) k_grad_join(const 
   const int64_t chunk = blockIdx.x;
   const int64_t p0 = chunk * kGradChunk, p1 = p0 + kGradChunk;
   if (p1 >= n) return;
-  const uint32_t key = sorted[p1 - 1];
-  if (key >= n_rows || sorted[p1] != key) return;
-  if (p0 > 0 && sorted[p0] == key && sorted[p0 - 1] == key) return;  // began earlier
+  const uint32_t key = sorted[p1 - 1], after = sorted[p1], start = sorted[p0], before = sorted[p0 > 0 ? p0 - 1 : 0];
+  if (key >= n_rows || after != key) return;
+  if (p0 > 0 && start == key && before == key) return;  // began earlier
   const int group = threadIdx.x / kGradThreads, thread = threadIdx.x % kGradThreads;
   const int64_t col = (static_cast<int64_t>(blockIdx.y) * kGradThreads + thread) * VE;
   const bool live = col < dim;
@@ -608,12 +662,12 @@ __global__ void __launch_bounds__(kGradThreads) k_grad_few(const TI* __restrict_
   __shared__ uint8_t of[kFewTokens];     // the row of each, less the first
   __shared__ int counts[2][kGradThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kZeroRows;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kFewRows;
   int have = 0, before = 0;  // tokens of these rows, and of smaller ids
   for (int t0 = 0; t0 < n; t0 += kGradThreads) {
     const int t = t0 + threadIdx.x;
     const int64_t id = t < n ? static_cast<int64_t>(ids[t]) : -1;
-    const bool mine = id >= r0 && id < r0 + kZeroRows && id < n_rows;
+    const bool mine = id >= r0 && id < r0 + kFewRows && id < n_rows;
     const uint32_t vote = __ballot_sync(0xffffffffu, mine);
     const uint32_t less = __ballot_sync(0xffffffffu, id >= 0 && id < r0);
     if (lane == 0) {
@@ -635,7 +689,7 @@ __global__ void __launch_bounds__(kGradThreads) k_grad_few(const TI* __restrict_
     __syncthreads();
   }
   // A warp per row; the lanes go through the list together.
-  for (int r = warp; r < kZeroRows && r0 + r < n_rows; r += kGradThreads / 32) {
+  for (int r = warp; r < kFewRows && r0 + r < n_rows; r += kGradThreads / 32) {
     int count = 0, smaller = 0;
     for (int q = lane; q < have; q += 32) {
       count += of[q] == r;
@@ -703,15 +757,17 @@ size_t grad_ws_bytes(int64_t n, int64_t dim) {
 
 template <typename TI, typename TO, int VE>
 void grad_launch(const void* grad, int64_t ldg, const int32_t* sorted, const int32_t* perm, int64_t n, int64_t n_rows,
-                 int64_t dim, float scale, void* out, int64_t ldo, bool accumulate, float* partial, cudaStream_t s) {
+                 int64_t dim, float scale, void* out, int64_t ldo, bool accumulate, float* partial,
+                 int64_t zero_rows_end, cudaStream_t s) {
   const int64_t chunks = ceil_div64(n, kGradChunk);
   const int64_t slices = ceil_div64(dim, static_cast<int64_t>(kGradThreads) * VE);
-  const int64_t zeros = accumulate ? 0 : ceil_div64(n_rows, kZeroRows);
+  const int64_t zeros = ceil_div64(zero_rows_end, kZeroCtaRows);
   const uint32_t* keys = reinterpret_cast<const uint32_t*>(sorted);
   TO* o = static_cast<TO*>(out);
-  k_grad_chunks<TI, TO, VE><<<static_cast<unsigned>(chunks * slices + zeros), kGradThreads, 0, s>>>(
-      static_cast<const TI*>(grad), ldg, keys, perm, n, n_rows, dim, scale, o, ldo, accumulate, partial, chunks,
-      static_cast<int>(slices));
+  auto* fn = accumulate ? &k_grad_chunks<TI, TO, VE, true> : &k_grad_chunks<TI, TO, VE, false>;
+  fn<<<static_cast<unsigned>(chunks * slices + zeros), kGradThreads, 0, s>>>(
+      static_cast<const TI*>(grad), ldg, keys, perm, n, n_rows, dim, scale, o, ldo, partial, chunks,
+      static_cast<int>(slices), zero_rows_end);
   if (chunks > 1)
     k_grad_join<TO, VE><<<dim3(static_cast<unsigned>(chunks), static_cast<unsigned>(slices)),
                           kGradThreads * kJoinGroups, 0, s>>>(
@@ -732,16 +788,17 @@ struct GradArgs {
   int64_t ldo;
   bool accumulate;
   float* partial;
+  int64_t zero_rows_end;  // rows below it are zeroed where they have no token
 };
 
 template <typename TI, typename TO, int VE>
 void grad_with(const GradArgs& a, cudaStream_t s) {
   if (!a.ids) {
     grad_launch<TI, TO, VE>(a.grad, a.ldg, a.sorted, a.perm, a.n, a.n_rows, a.dim, a.scale, a.out, a.ldo, a.accumulate,
-                            a.partial, s);
+                            a.partial, a.zero_rows_end, s);
     return;
   }
-  const unsigned grid = static_cast<unsigned>(ceil_div64(a.n_rows, kZeroRows));
+  const unsigned grid = static_cast<unsigned>(ceil_div64(a.n_rows, kFewRows));
   auto go = [&](auto* ids) {
     using ID = typename std::remove_const<typename std::remove_pointer<decltype(ids)>::type>::type;
     k_grad_few<TI, TO, ID, VE><<<grid, kGradThreads, 0, s>>>(static_cast<const TI*>(a.grad), a.ldg, ids,
@@ -784,6 +841,12 @@ void lookup_ids(const void* weight, int64_t n_rows, int64_t dim, int64_t ldw, co
                 int64_t nids, float scale, void* out, cudaStream_t s) {
   if (ids64) lookup_pick<TI, TO, int64_t>(weight, n_rows, dim, ldw, ids, nids, scale, out, s);
   else lookup_pick<TI, TO, int32_t>(weight, n_rows, dim, ldw, ids, nids, scale, out, s);
+}
+
+kairo_status sort_tokens(const void* ids, int32_t id_bytes, int64_t n, int64_t n_rows, uint32_t* sorted, int32_t* perm,
+                         const ZeroRows& zero, void* ws, cudaStream_t s) {
+  return id_bytes == 8 ? sort_launch(static_cast<const int64_t*>(ids), n, n_rows, sorted, perm, ws, zero, s)
+                       : sort_launch(static_cast<const int32_t*>(ids), n, n_rows, sorted, perm, ws, zero, s);
 }
 
 constexpr int64_t kMaxTokens = 0x7fffffffLL - 4096;
@@ -845,8 +908,7 @@ extern "C" kairo_status kairo_token_sort(const void* ids, int32_t id_bytes, int6
   if (workspace_bytes < need) return fail(KAIRO_STATUS_WORKSPACE_TOO_SMALL, "token sort workspace too small");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint32_t* keys = reinterpret_cast<uint32_t*>(sorted);
-  return id_bytes == 8 ? sort_launch(static_cast<const int64_t*>(ids), nids, n_rows, keys, perm, workspace, s)
-                       : sort_launch(static_cast<const int32_t*>(ids), nids, n_rows, keys, perm, workspace, s);
+  return sort_tokens(ids, id_bytes, nids, n_rows, keys, perm, ZeroRows{}, workspace, s);
 }
 
 namespace {
@@ -862,7 +924,7 @@ kairo_status run_grad(const void* grad_output, int64_t ldg, kairo_dtype dtype, c
   if (n_rows < 0 || dim <= 0 || nids < 0) return fail(KAIRO_STATUS_INVALID_VALUE, "invalid size");
   if (nids > kMaxTokens || n_rows > kMaxRows) return fail(KAIRO_STATUS_NOT_SUPPORTED, "too many tokens or rows");
   if (dim > static_cast<int64_t>(65535) * kGradThreads ||
-      ceil_div64(nids, kGradChunk) * ceil_div64(dim, kGradThreads) + ceil_div64(n_rows, kZeroRows) > 0x7fffffffLL)
+      ceil_div64(nids, kGradChunk) * ceil_div64(dim, kGradThreads) + ceil_div64(n_rows, kFewRows) > 0x7fffffffLL)
     return fail(KAIRO_STATUS_NOT_SUPPORTED, "too many tokens for this width");
   if (ldg < dim || ldo < dim) return fail(KAIRO_STATUS_INVALID_VALUE, "leading dimension smaller than dim");
   if (!known_dtype(dtype) || !known_dtype(out_dtype)) return fail(KAIRO_STATUS_INVALID_VALUE, "unknown dtype");
@@ -897,6 +959,7 @@ kairo_status run_grad(const void* grad_output, int64_t ldg, kairo_dtype dtype, c
   a.ldo = ldo;
   a.accumulate = accumulate != 0;
   a.partial = static_cast<float*>(workspace);
+  a.zero_rows_end = accumulate ? 0 : n_rows;
   if (ids && nids <= kFewTokens) {
     a.ids = ids;
     a.ids64 = id_bytes == 8;
@@ -904,8 +967,21 @@ kairo_status run_grad(const void* grad_output, int64_t ldg, kairo_dtype dtype, c
     uint8_t* p = static_cast<uint8_t*>(workspace) + order_at;
     int32_t* order = reinterpret_cast<int32_t*>(p);
     int32_t* tokens = reinterpret_cast<int32_t*>(p + order_bytes(nids) / 2);
-    const kairo_status st = kairo_token_sort(ids, id_bytes, nids, n_rows, order, tokens, p + order_bytes(nids),
-                                             workspace_bytes - order_at - order_bytes(nids), stream);
+    // While one cluster sorts, the other SMs zero the last rows, tokens or not:
+    // about what they can write in that time (a sort of n tokens takes some 10 us
+    // and 0.4 us per 1024, 5 MB are written per us).  Frequent ids are small in
+    // most vocabularies, so few of these rows are written again.
+    ZeroRows zero{};
+    if (!accumulate && nids <= kClusterTokens && dim * ob % 16 == 0 && ldo * ob % 16 == 0 && aligned(grad_weight, 16)) {
+      const int64_t bytes = (int64_t(40) << 20) + nids * 2048;
+      zero.rows = std::min(n_rows, bytes / (dim * ob));
+      zero.vecs = dim * ob / 16;
+      zero.pitch = ldo * ob / 16;
+      a.zero_rows_end = n_rows - zero.rows;
+      zero.first = reinterpret_cast<uint4*>(static_cast<uint8_t*>(grad_weight) + a.zero_rows_end * ldo * ob);
+    }
+    const kairo_status st = sort_tokens(ids, id_bytes, nids, n_rows, reinterpret_cast<uint32_t*>(order), tokens, zero,
+                                        p + order_bytes(nids), s);
     if (st) return st;
     a.sorted = order;
     a.perm = tokens;
