@@ -106,7 +106,7 @@ struct Row8 {
 
 // A warp takes 256 columns of 8 rows: 32 groups, of which each lane computes
 // the two quotients of one.  Bound by memory when that is done (3.06 bytes a
-// value of a 16-bit activation); with the quotients computed by all lanes for
+// value of a 16-bit activation; 8192 x 32768 in 128 us, 6.4 TB/s); with the quotients computed by all lanes for
 // every row, and the largest magnitude one value at a time, the instructions
 // bound it: 8192 x 32768 took 276 us.
 template <typename T>

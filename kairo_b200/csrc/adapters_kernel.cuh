@@ -124,8 +124,8 @@ __device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
 constexpr int kMaxCluster = 8;
 
 // The sum over the cluster, in rank order, of the value (or four) at the same
-// shared address of every CTA.  The loads are issued together: one after the
-// other, a peer's latency (some 700 cycles) would be paid for each.
+// shared address of every CTA.  The loads are issued together, so that the
+// latency of a peer's memory is paid once and not for each of eight.
 __device__ __forceinline__ float peer_sum(uint32_t addr, uint32_t csize) {
   float v[kMaxCluster];
 #pragma unroll

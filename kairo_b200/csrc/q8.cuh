@@ -20,8 +20,8 @@ __device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float lo, float hi)
 }
 
 // Code `i` of four as a float.  With its sign bit flipped it is the low byte of
-// the float 2^23 + 128 + code: one byte permutation and one exact subtraction,
-// where a conversion instruction runs at a quarter of their rate.
+// the float 2^23 + 128 + code: one byte permutation and one exact subtraction, both
+// at the full rate that a conversion instruction does not have.
 __device__ __forceinline__ float code_value(uint32_t four, int i) {
   return __uint_as_float(__byte_perm(four ^ 0x80808080u, 0x4b000000u, 0x7650u + static_cast<unsigned>(i))) - 8388736.f;
 }

@@ -465,3 +465,24 @@ def test_captured_training_step_beside_an_eager_one():
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(ref, out))
     del alive
+
+
+def test_offsets_pass_32_bits():
+    """More than 2^31 values of X and of dX: the last tokens are read and written where they belong."""
+    t, k = 66_000, 32_768
+    x = torch.zeros(t, k, dtype=torch.bfloat16, device=DEV)
+    x[-1], x[-2, 5] = 1.0, 2.0
+    down = torch.full((2, 4, k), 2.0**-10, dtype=torch.bfloat16, device=DEV)
+    up = torch.ones(2, 4, 64, dtype=torch.bfloat16, device=DEV)
+    a = LowRankAdapters(down=down, up=up)
+    ids = torch.full((t,), -1, device=DEV)
+    ids[-1], ids[-2], ids[3] = 1, 0, 0
+    plan = adapter_plan(ids, 2)
+    y, low = adapter_linear(x, a, plan, return_low=True)  # low of the last: 32768 * 2^-10 = 32
+    assert low[-1].tolist() == [32.0] * 4 and low[-2].tolist() == [2.0**-9] * 4
+    assert y[-1].unique().tolist() == [128.0] and bool((y[:-2] == 0).all())
+    dy = torch.ones(t, 64, dtype=torch.bfloat16, device=DEV)
+    dx, dd, du = adapter_linear_backward(dy, x, a, plan, low=low)
+    # dlow = 64 for the three tokens with an adapter, dX = 4 * 64 * 2^-10
+    assert dx[-1].unique().tolist() == [0.25] and dx[3].unique().tolist() == [0.25] and int(dx[4].count_nonzero()) == 0
+    assert dd[1].unique().tolist() == [64.0] and dd[0, 0, 5].item() == 128.0 and du[1].unique().tolist() == [32.0]
