@@ -497,8 +497,9 @@ KAIRO_API kairo_status kairo_sparse_scatter_grad_workspace_size(int64_t nactive,
  *                           what grad_weight holds and other rows are not
  *                           touched.  fp32 sums in an order fixed by the ids,
  *                           no atomics; one rounding to out_dtype.
- *   kairo_embedding_grad_sorted  the same from the result of kairo_token_sort
- *                           (and a workspace of the same size).
+ *   kairo_embedding_grad_sorted  the same from the result of kairo_token_sort.
+ *   kairo_embedding_grad_workspace_size  bytes for either (sorted 0 or 1); 0
+ *                           means that none is needed.
  * dtype and out_dtype f32, f16 or bf16, in any combination; n_rows and nids
  * below 2^31 - 4096.  All asynchronous on `stream`; the workspaces need no
  * initial value.
@@ -519,7 +520,8 @@ KAIRO_API kairo_status kairo_embedding_grad_sorted(const void* grad_output, int6
                                                    int64_t n_rows, int64_t dim, float scale, void* grad_weight,
                                                    int64_t ldo, kairo_dtype out_dtype, int32_t accumulate,
                                                    void* workspace, size_t workspace_bytes, void* stream);
-KAIRO_API kairo_status kairo_embedding_grad_workspace_size(int64_t nids, int64_t dim, size_t* bytes);
+KAIRO_API kairo_status kairo_embedding_grad_workspace_size(int64_t nids, int64_t dim, int32_t sorted,
+                                                           size_t* bytes);
 
 /* ------------------------------------------------------------------------
  * Diagnostics (no counterpart in the reference): the rate at which the SMs

@@ -710,15 +710,15 @@ __global__ void __launch_bounds__(kGradThreads) k_grad_few(const TI* __restrict_
         for (int q0 = 0; q0 < have; q0 += 32) {
           uint32_t left = __ballot_sync(0xffffffffu, q0 + lane < have && of[q0 + lane] == r);
           while (left) {
-            float f[4][VE];
+            Raw<TI, VE> f[kGradAhead];
             uint32_t rest = left;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              if (rest && c < dim) load_f32<TI, VE>(grad + tok[q0 + __ffs(rest) - 1] * ldg + c, f[u]);
+            for (int u = 0; u < kGradAhead; ++u) {
+              if (rest && c < dim) f[u].load(grad + tok[q0 + __ffs(rest) - 1] * ldg + c);
               rest &= rest - 1;
             }
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+            for (int u = 0; u < kGradAhead; ++u) {
               if (!left) break;
               left &= left - 1;
               if (place % kGradChunk == 0 && place != first) {  // a new chunk begins
@@ -732,8 +732,10 @@ __global__ void __launch_bounds__(kGradThreads) k_grad_few(const TI* __restrict_
                 ++part;
               }
               ++place;
+              if (c < dim) {
 #pragma unroll
-              for (int i = 0; i < VE; ++i) acc[i] += f[u][i];
+                for (int i = 0; i < VE; ++i) acc[i] += f[u][i];
+              }
             }
           }
         }
@@ -940,11 +942,11 @@ kairo_status run_grad(const void* grad_output, int64_t ldg, kairo_dtype dtype, c
     if (e != cudaSuccess) return cuda_fail(e, "cudaMemset2DAsync(grad_weight)");
     return KAIRO_STATUS_SUCCESS;
   }
-  if (!grad_output || (!ids && (!sorted || !perm)) || !workspace)
-    return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+  if (!grad_output || (!ids && (!sorted || !perm))) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
   size_t need = grad_ws_bytes(nids, dim);
   const size_t order_at = align_up(need, 256);
-  if (ids) need = order_at + order_bytes(nids) + sort_ws_bytes(nids);
+  if (ids) need = nids <= kFewTokens ? 0 : order_at + order_bytes(nids) + sort_ws_bytes(nids);
+  if (need > 0 && !workspace) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
   if (workspace_bytes < need) return fail(KAIRO_STATUS_WORKSPACE_TOO_SMALL, "embedding gradient workspace too small");
   GradArgs a{};
   a.grad = grad_output;
@@ -1000,9 +1002,11 @@ kairo_status run_grad(const void* grad_output, int64_t ldg, kairo_dtype dtype, c
 
 }  // namespace
 
-extern "C" kairo_status kairo_embedding_grad_workspace_size(int64_t nids, int64_t dim, size_t* bytes) {
+extern "C" kairo_status kairo_embedding_grad_workspace_size(int64_t nids, int64_t dim, int32_t sorted, size_t* bytes) {
   if (!bytes || nids < 0 || dim <= 0) return fail(KAIRO_STATUS_INVALID_VALUE, "invalid argument");
-  *bytes = align_up(grad_ws_bytes(nids, dim), 256) + order_bytes(nids) + sort_ws_bytes(nids);
+  if (sorted) *bytes = grad_ws_bytes(nids, dim);
+  else if (nids <= kFewTokens) *bytes = 0;
+  else *bytes = align_up(grad_ws_bytes(nids, dim), 256) + order_bytes(nids) + sort_ws_bytes(nids);
   return KAIRO_STATUS_SUCCESS;
 }
 

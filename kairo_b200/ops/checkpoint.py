@@ -103,9 +103,10 @@ def quantize_activations(X: Tensor) -> QuantizedActivations:
         X = X.contiguous()
     n, k = X.shape
     ldq = -(-k // 16) * 16
-    codes = X.new_empty((n, ldq), dtype=torch.int8)
-    if ldq != k:
-        codes = codes[:, :k]
+    if ldq == k or n == 0:
+        codes = X.new_empty((n, k), dtype=torch.int8)
+    else:  # rows padded to 16 bytes; room for the padding of the last
+        codes = X.new_empty((n, ldq), dtype=torch.int8)[:, :k]
     steps = X.new_empty((-(-k // GROUP), n), dtype=torch.float32)
     _lib.launch("quantize_activations", _lib.lib().kairo_quantize_q8, index, X.data_ptr(), n, k, max(X.stride(0), k),
                 dt, codes.data_ptr(), ldq, steps.data_ptr(), n)

@@ -71,10 +71,11 @@ def _sort_bytes(tokens: int, n_rows: int) -> int:
 
 
 @functools.lru_cache(maxsize=4096)
-def _grad_bytes(tokens: int, dim: int) -> int:
+def _grad_bytes(tokens: int, dim: int, in_order: bool) -> int:
     nbytes = ctypes.c_size_t(0)
-    _lib.check(_lib.lib().kairo_embedding_grad_workspace_size(tokens, dim, ctypes.byref(nbytes)), "embedding_grad")
-    return max(nbytes.value, 256)
+    _lib.check(_lib.lib().kairo_embedding_grad_workspace_size(tokens, dim, 1 if in_order else 0, ctypes.byref(nbytes)),
+               "embedding_grad")
+    return nbytes.value
 
 
 def sort_tokens(ids: Tensor, num_embeddings: int) -> TokenOrder:
@@ -151,7 +152,7 @@ def embedding_grad(grad_output: Tensor, ids: Tensor | TokenOrder, num_embeddings
     d = grad_output.shape[-1]
     if not isinstance(ids, TokenOrder) and tuple(grad_output.shape[:-1]) != tuple(ids.shape):
         raise ValueError(f"grad_output must be {tuple(ids.shape) + (d,)}, got {tuple(grad_output.shape)}")
-    g = _rows(grad_output.reshape(-1, d))
+    g = _rows(grad_output if grad_output.dim() == 2 else grad_output.reshape(-1, d))
     if g.shape[0] != tokens:
         raise ValueError(f"grad_output has {g.shape[0]} rows for {tokens} tokens")
     odt = out_dtype or (out.dtype if out is not None else g.dtype)
@@ -164,10 +165,12 @@ def embedding_grad(grad_output: Tensor, ids: Tensor | TokenOrder, num_embeddings
         raise ValueError(f"out must be a row-major ({n_rows}, {d}) {odt} tensor on {dev}")
     else:
         _lib.refuse_overlap("embedding_grad", out, g, where)
-    ws = g.new_empty(_grad_bytes(tokens, d), dtype=torch.uint8)
-    tail = (tokens, n_rows, d, float(scale), out.data_ptr(), _ld(out), out_dt, 1 if accumulate else 0, ws.data_ptr(),
-            ws.numel())
-    if isinstance(ids, TokenOrder):
+    in_order = isinstance(ids, TokenOrder)
+    size = _grad_bytes(tokens, d, in_order)
+    ws = g.new_empty(size, dtype=torch.uint8) if size else None
+    tail = (tokens, n_rows, d, float(scale), out.data_ptr(), _ld(out), out_dt, 1 if accumulate else 0,
+            ws.data_ptr() if size else None, size)
+    if in_order:
         _lib.launch("embedding_grad", _lib.lib().kairo_embedding_grad_sorted, index, g.data_ptr(), _ld(g), in_dt,
                     ids.sorted_ids.data_ptr(), ids.perm.data_ptr(), *tail)
     else:

@@ -75,9 +75,14 @@ def test_embedding_c_refusals():
 
     for fn in (grad, grad_ids):
         for kw in ({"ldg": 7}, {"ldo": 7}, {"dt": 3}, {"odt": 3}, {"nids": -1}, {"rows": -1}, {"dim": 0}, {"g": None},
-                   {"ws": None}, {"out": None}):
+                   {"nids": 1000, "ws": None}, {"out": None}):
             assert fn(**kw) == _lib.INVALID_VALUE, kw
-        assert fn(wsb=10) == _lib.WORKSPACE_TOO_SMALL
+        assert fn(nids=1000, wsb=10) == _lib.WORKSPACE_TOO_SMALL
+    size = lib.kairo_embedding_grad_workspace_size
+    assert size(-1, 8, 0, ctypes.byref(n)) == _lib.INVALID_VALUE and size(3, 8, 0, None) == _lib.INVALID_VALUE
+    assert size(3, 8, 0, ctypes.byref(n)) == _lib.SUCCESS and n.value == 0  # a short list needs none
+    assert size(3, 8, 1, ctypes.byref(n)) == _lib.SUCCESS and n.value > 0
+    for fn in (grad, grad_ids):
         assert fn(nids=1 << 31) == _lib.NOT_SUPPORTED
         assert fn(rows=0) == _lib.SUCCESS
     assert grad_ids(ids=None) == _lib.INVALID_VALUE and grad_ids(idb=2) == _lib.INVALID_VALUE
