@@ -206,7 +206,8 @@ kairo_status q8_check(int64_t n, int64_t k, const void* codes, int64_t ldq, cons
   if (ldq % 16 != 0) return fail(KAIRO_STATUS_INVALID_VALUE, "ldq must be a multiple of 16");
   if (n > 0 && k > 0) {
     if (!codes || !steps) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
-    if (reinterpret_cast<uintptr_t>(codes) % 16) return fail(KAIRO_STATUS_INVALID_VALUE, "codes must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(codes) % 16)
+      return fail(KAIRO_STATUS_INVALID_VALUE, "codes must be 16-byte aligned");
   }
   return KAIRO_STATUS_SUCCESS;
 }

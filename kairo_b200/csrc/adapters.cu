@@ -62,7 +62,8 @@ size_t carve_plan(void* mem, int64_t t, int64_t g, Plan* pl) {
 
 // The tiles of one size (blockIdx.x) from the sorted ids: where each adapter's
 // tokens start, how many tiles come before its own, and the tiles themselves.
-__global__ void __launch_bounds__(1024) k_plan_tiles(const uint32_t* __restrict__ sorted, int64_t t, int64_t g, Plan pl) {
+__global__ void __launch_bounds__(1024) k_plan_tiles(const uint32_t* __restrict__ sorted, int64_t t, int64_t g,
+                                                     Plan pl) {
   __shared__ int sums[32];
   __shared__ int carry;
   const int which = blockIdx.x;
@@ -163,10 +164,14 @@ bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 // adapters, 4096 features: rank 16, 1024 tokens 9.1 us with tiles of 16 and
 // 13.0 with 64, 2048 tokens 12.8 and 14.0, 4096 tokens 22.8 and 22.4; rank 32,
 // 2048 tokens 17.3 and 17.6 (with 32), and 8192 tokens of 8192 features 117
-// and 96.
-int pick_tile(int64_t t, int64_t rank, bool vec) {
-  if (!vec || t <= 2048 || rank > 64) return 16;
-  return rank <= 16 ? 64 : 32;
+// and 96; rank 64, 1024 tokens 19.0 and 24.2, 4096 tokens 48.5 and 39.6; rank 128,
+// 4096 tokens 94.8 and 75.5 (with 32).
+int pick_tile(int64_t t, int64_t rank, bool vec, bool base_f32) {
+  if (!vec || t <= 2048) return 16;
+  if (rank <= 16) return 64;
+  if (rank <= 32) return 32;
+  if (rank <= 64) return base_f32 ? 32 : 64;
+  return base_f32 ? 16 : 32;
 }
 
 // CTAs per tile, a power of two up to 8.  As many as the GPU holds at once (two
@@ -254,7 +259,8 @@ extern "C" kairo_status kairo_low_rank_apply(const void* x, int64_t ldx, int64_t
   if ((base && base_dtype != KAIRO_DTYPE_F32 && base_dtype != dtype) ||
       (y && y_dtype != KAIRO_DTYPE_F32 && y_dtype != dtype))
     return fail(KAIRO_STATUS_INVALID_VALUE, "base and y must be fp32 or the adapters' dtype");
-  if (ldx < k || (y && ldy < n) || (base && ldb < n)) return fail(KAIRO_STATUS_INVALID_VALUE, "leading dimension too small");
+  if (ldx < k || (y && ldy < n) || (base && ldb < n))
+    return fail(KAIRO_STATUS_INVALID_VALUE, "leading dimension too small");
   if (ntokens == 0) return KAIRO_STATUS_SUCCESS;
   if (!x || !plan || (!y && !low) || (nadapters > 0 && (!down || (y && !up))))
     return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
@@ -264,7 +270,7 @@ extern "C" kairo_status kairo_low_rank_apply(const void* x, int64_t ldx, int64_t
   const int64_t eb = base_dtype == KAIRO_DTYPE_F32 ? 4 : 2, ey = y_dtype == KAIRO_DTYPE_F32 ? 4 : 2;
   const bool vec = k % 8 == 0 && n % 8 == 0 && ldx * e % 16 == 0 && aligned16(x) && aligned16(down) && aligned16(up) &&
                    (!base || (ldb * eb % 16 == 0 && aligned16(base))) && (!y || (ldy * ey % 16 == 0 && aligned16(y)));
-  const int tile = pick_tile(ntokens, rank, vec);
+  const int tile = pick_tile(ntokens, rank, vec, base && base_dtype == KAIRO_DTYPE_F32);
   const int which = tile == 16 ? 0 : (tile == 32 ? 1 : 2);
   LowRankApplyArgs a{};
   a.x = x;
@@ -391,7 +397,8 @@ extern "C" kairo_status kairo_low_rank_wgrads(const float* dlow, const float* lo
                                               void* d_down, void* d_up, kairo_dtype grad_dtype, void* stream) {
   if (ldx < k || lddy < n) return fail(KAIRO_STATUS_INVALID_VALUE, "leading dimension too small");
   if (ntokens > 0 && nadapters > 0 && (!x || !dy)) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
-  const Grad p[2] = {{dlow, x, ldx, nullptr, 0, nullptr, 0, k, d_down}, {low, dy, lddy, nullptr, 0, nullptr, 0, n, d_up}};
+  const Grad p[2] = {{dlow, x, ldx, nullptr, 0, nullptr, 0, k, d_down},
+                     {low, dy, lddy, nullptr, 0, nullptr, 0, n, d_up}};
   for (const Grad& q : p) {
     const kairo_status st = check_grad(q, rank, dtype, plan, ntokens, nadapters, grad_dtype);
     if (st) return st;

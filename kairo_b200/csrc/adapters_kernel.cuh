@@ -19,15 +19,16 @@
 //    features of column 2t and those of column 2t+1, for its rows.
 // Every access is a 16-byte vector, and the features of the columns are dealt
 // out so that the four lanes t of one access stand side by side: 64 bytes of a
-// row, whole sectors. (With columns 2t and 2t+1 side by side instead, each access touched
-// half sectors, and the rank-16 expansion of 8192 x 8192 took 91 us where it
-// now takes 56.)
+// row, whole sectors.  (With columns 2t and 2t+1 side by side instead, each
+// access touched half sectors, and the rank-16 expansion of 8192 x 8192 took 91
+// us where it now takes 56.)
 //
 // low is an fp32 value.  For a product with 16-bit weights it is split into
 // terms of the weights' type, each the rounding of what the ones before leave:
 // two for 16-bit results (rest at most 2^-17 of it), three for fp32 results
 // (2^-23).  In fp16, whose range is narrow, it is first scaled by a power of
-// two (exact) that brings the largest of the row to [1, 2).
+// two (exact) that brings the largest of the row to [1, 2), and the rest is
+// one of that largest.  A low value that is infinite makes its token's row NaN.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -295,10 +296,14 @@ __device__ __forceinline__ void wait_all_but() {
 }
 
 // Tile shape and memory of one instance.  MT x 16 tokens, NT x 8 rank rows;
-// STAGES steps of 32 features in flight in the contraction.
-template <int MT_, int NT_, int STAGES_>
+// STAGES steps of 32 features in flight in the contraction.  ALIAS: the warps'
+// partial tiles take the ring's place while they are summed, which makes room
+// for twice the tokens at ranks above 32; the expansion's loads then start behind
+// that sum.
+template <int MT_, int NT_, int STAGES_, bool ALIAS_ = false>
 struct ApplyShape {
   static constexpr int MT = MT_, NT = NT_, STAGES = STAGES_;
+  static constexpr bool ALIAS = ALIAS_;
   static constexpr int ROWS = 16 * MT;
   static constexpr int RP = 8 * NT;          // rank, padded
   static constexpr int PITCH = RP + 8;       // 16-bit terms: rows 16 bytes apart in banks
@@ -313,7 +318,8 @@ struct ApplyShape {
   }
   static constexpr size_t ring_bytes(bool base_f32) { return static_cast<size_t>(kWarps) * ring(base_f32) * 512; }
   static constexpr size_t bytes(int terms, bool base_f32) {
-    return ring_bytes(base_f32) + static_cast<size_t>(kWarps / 2 * LOW + LOW + ROWS) * 4 + static_cast<size_t>(terms) * ROWS * PITCH * 2;
+    const size_t tiles = (ALIAS ? 2 : kWarps / 2 + 1) * static_cast<size_t>(LOW);
+    return ring_bytes(base_f32) + (tiles + ROWS) * 4 + static_cast<size_t>(terms) * ROWS * PITCH * 2;
   }
 };
 
@@ -330,9 +336,10 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApp
   constexpr int MT = S::MT, NT = S::NT, KT = S::KT;
   constexpr int RING = S::ring(BASE_F32);
   extern __shared__ __align__(16) uint8_t smem[];
-  float* red = reinterpret_cast<float*>(smem + S::ring_bytes(BASE_F32));  // [kWarps / 2][LOW]
-  float* part = red;                                             // [LOW]: this CTA's partial tile
-  float* low = red + kWarps / 2 * S::LOW;                        // [LOW]: the whole tile
+  static_assert(!S::ALIAS || S::ring_bytes(BASE_F32) >= kWarps / 2 * S::LOW * 4, "partial tiles fit in the ring");
+  float* part = reinterpret_cast<float*>(smem + S::ring_bytes(BASE_F32));  // [LOW]: this CTA's partial tile
+  float* red = S::ALIAS ? reinterpret_cast<float*>(smem) : part;  // [kWarps / 2][LOW]
+  float* low = part + (S::ALIAS ? 1 : kWarps / 2) * S::LOW;      // [LOW]: the whole tile
   float* row_up = low + S::LOW;                                  // [ROWS]: power of two of every row (fp16)
   uint16_t* terms = reinterpret_cast<uint16_t*>(row_up + S::ROWS);  // [TERMS][ROWS][PITCH]
 
@@ -470,16 +477,22 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApp
     }
     commit();
   };
-  if (a.y) {
+  auto start_turn = [&]() {
+    if (!a.y) return;
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) issue_up(slot * 64, kt);
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int b = 0; b < BU; ++b) issue_base(slot * 64, m, b);
-  }
+  };
+  if (!S::ALIAS || !live) start_turn();
 
   if (live) {
+    if constexpr (S::ALIAS) {
+      wait_all_but<0>();  // of the empty groups: every copy has been used
+      __syncthreads();
+    }
     // Sum over the CTA's warps as a tree: the upper half hands over to the lower.
 #pragma unroll
     for (int half = kWarps / 2; half >= 1; half /= 2) {
@@ -503,6 +516,7 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApp
       }
       __syncthreads();
     }
+    if (S::ALIAS) start_turn();  // the ring is free again
     if (warp == 0) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
@@ -720,9 +734,12 @@ cudaError_t pick_apply(const LowRankApplyArgs& a, bool vec, int tile, int64_t cl
     return tile == 32 ? launch_apply<T, TY, ApplyShape<2, 4, 2>, true>(a, clusters, cluster, s)
                       : launch_apply<T, TY, R32, true>(a, clusters, cluster, s);
   if (a.rank <= 64)
-    return tile == 32 ? launch_apply<T, TY, ApplyShape<2, 8, 3>, true>(a, clusters, cluster, s)
-                      : launch_apply<T, TY, R64, true>(a, clusters, cluster, s);
-  return launch_apply<T, TY, R128, true>(a, clusters, cluster, s);
+    // an fp32 base takes twice the room of its loads
+    return tile == 64   ? launch_apply_as<T, TY, ApplyShape<4, 8, 2, true>, false, true>(a, clusters, cluster, s)
+           : tile == 32 ? launch_apply_as<T, TY, ApplyShape<2, 8, 3>, true, true>(a, clusters, cluster, s)
+                        : launch_apply<T, TY, R64, true>(a, clusters, cluster, s);
+  return tile == 32 ? launch_apply_as<T, TY, ApplyShape<2, 16, 2, true>, false, true>(a, clusters, cluster, s)
+                    : launch_apply<T, TY, R128, true>(a, clusters, cluster, s);
 }
 
 // ---------------------------------------------------------------- weight gradient
@@ -744,8 +761,9 @@ struct WgradShape {
   static constexpr size_t PART_BYTES = static_cast<size_t>(RP) * COLS * 4;
   static constexpr size_t SHARED_BYTES = RING_BYTES > PART_BYTES ? RING_BYTES : PART_BYTES;
   static constexpr size_t bytes(int terms, bool half, bool q8) {
-    return SHARED_BYTES + (q8 ? static_cast<size_t>(2 * kChunk * (COLS / 64)) * 4 : 0) + static_cast<size_t>(2 * RP + 4 * kChunk) * 4 +
-           2 * static_cast<size_t>(terms) * kChunk * PITCH * 2 + (half ? static_cast<size_t>(kChunk) * RP * 4 : 0);
+    return SHARED_BYTES + (q8 ? static_cast<size_t>(2 * kChunk * (COLS / 64)) * 4 : 0) +
+           static_cast<size_t>(2 * RP + 4 * kChunk) * 4 + 2 * static_cast<size_t>(terms) * kChunk * PITCH * 2 +
+           (half ? static_cast<size_t>(kChunk) * RP * 4 : 0);
   }
 };
 
@@ -768,7 +786,8 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgr
   float* scales = reinterpret_cast<float*>(smem + S::SHARED_BYTES);  // [2][RP]: power of two of every rank row (fp16)
   int* toks = reinterpret_cast<int*>(scales + 2 * RP);             // [4][kChunk]: -1 behind the last
   float* steps = reinterpret_cast<float*>(toks + 4 * kChunk);      // [2][COLS / 64][kChunk] (8 bits)
-  uint16_t* terms = reinterpret_cast<uint16_t*>(steps + (Q8 ? 2 * (S::COLS / 64) * kChunk : 0));  // [2][TERMS][kChunk][PITCH]
+  uint16_t* terms =  // [2][TERMS][kChunk][PITCH]
+      reinterpret_cast<uint16_t*>(steps + (Q8 ? 2 * (S::COLS / 64) * kChunk : 0));
   float* raw = reinterpret_cast<float*>(terms + 2 * TERMS * kChunk * S::PITCH);  // [kChunk][RP] (fp16)
 
   const uint32_t crank = cluster_rank(), csize = cluster_size();
@@ -978,11 +997,10 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgr
       float* row = part + ((rg * MR + m) * 16 + h * 8 + g) * S::COLS + lc + 16 * t;
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        *reinterpret_cast<float4*>(row + 4 * q) =
-            make_float4(sum[m][4 * q][2 * h], sum[m][4 * q + 1][2 * h], sum[m][4 * q + 2][2 * h], sum[m][4 * q + 3][2 * h]);
+        const float (*v)[4] = &sum[m][4 * q];
+        *reinterpret_cast<float4*>(row + 4 * q) = make_float4(v[0][2 * h], v[1][2 * h], v[2][2 * h], v[3][2 * h]);
         *reinterpret_cast<float4*>(row + 8 + 4 * q) =
-            make_float4(sum[m][4 * q][2 * h + 1], sum[m][4 * q + 1][2 * h + 1], sum[m][4 * q + 2][2 * h + 1],
-                        sum[m][4 * q + 3][2 * h + 1]);
+            make_float4(v[0][2 * h + 1], v[1][2 * h + 1], v[2][2 * h + 1], v[3][2 * h + 1]);
       }
     }
   cluster_sync();

@@ -820,7 +820,9 @@ void grad_pick(int ve, const GradArgs& a, cudaStream_t s) {
   else grad_with<TI, TO, 1>(a, s);
 }
 
-bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(bytes) == 0; }
+bool aligned(const void* p, int64_t bytes) {
+  return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(bytes) == 0;
+}
 
 template <typename TI, typename TO, typename ID>
 void lookup_pick(const void* weight, int64_t n_rows, int64_t dim, int64_t ldw, const void* ids, int64_t nids,

@@ -156,8 +156,8 @@ def sparse_linear_weight_grad(dY: Tensor, X: Tensor | QuantizedActivations, W: B
     return dw
 
 
-def sparse_linear_backward(dY: Tensor, X: Tensor | QuantizedActivations, W: BlockSparseMatrix, wt: TransposedBsr | None = None, *,
-                           need_dx: bool = True, need_dw: bool = True, dw_dtype: torch.dtype = torch.float32,
+def sparse_linear_backward(dY: Tensor, X: Tensor | QuantizedActivations, W: BlockSparseMatrix,
+                           wt: TransposedBsr | None = None, *, need_dx: bool = True, need_dw: bool = True, dw_dtype: torch.dtype = torch.float32,
                            config: KernelConfig | None = None, check: bool = False):
     """(dX, dW) of Y = X @ W^T.  dX: (batch, in_features) in X's dtype; dW:
     (nnzb, bm, bk) in ``dw_dtype``, W's BSR order.  Either may be None.  X may
@@ -198,7 +198,8 @@ class _SparseLinearFn(torch.autograd.Function):
         wt = transpose_values(W, module.transposed())
         dY = dY.contiguous()
         if X is None:
-            return (sparse_linear(dY, wt.matrix, out_dtype=ctx.x_dtype) if ctx.needs_input_grad[0] else None), None, None
+            dX = sparse_linear(dY, wt.matrix, out_dtype=ctx.x_dtype) if ctx.needs_input_grad[0] else None
+            return dX, None, None
         dX, dW = sparse_linear_backward(dY, X, W, wt, need_dx=ctx.needs_input_grad[0],
                                         need_dw=ctx.needs_input_grad[1], dw_dtype=blocks.dtype)
         return dX, dW, None

@@ -117,7 +117,10 @@ CASES = [
     (300, 640, 768, 64, 3),
     (129, 256, 256, 128, 2),
     (515, 320, 264, 33, 1),
-    (2100, 128, 192, 16, 3),
+    (2100, 128, 192, 16, 3),      # from here on the tall tiles of long batches
+    (2300, 136, 128, 30, 5),
+    (2300, 192, 136, 64, 3),
+    (2200, 128, 200, 100, 2),
 ]
 
 
