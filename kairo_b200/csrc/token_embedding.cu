@@ -393,6 +393,32 @@ __global__ void __launch_bounds__(kClusterThreads) k_sort_cluster(const ID* __re
   }
 }
 
+// A list of kRankTokens at most: the place of a token is the number of smaller
+// ids and of equal ones before it.  A warp counts for one token, 32 tokens to
+// a CTA; one pass, no exchange.  1024 tokens 3.1 us, 4096 6.7 and 8192 20; the
+// cluster's sort takes 10.8 us for 4097 tokens and 11.3 for 8192.
+constexpr int kRankTokens = 4096;
+template <typename ID>
+__global__ void __launch_bounds__(1024) k_sort_ranks(const ID* __restrict__ ids, int n, int64_t n_rows,
+                                                     uint32_t* __restrict__ sorted, int32_t* __restrict__ perm) {
+  __shared__ uint32_t keys[kRankTokens];
+  for (int i = threadIdx.x; i < n; i += 1024) keys[i] = token_key(ids, i, n_rows);
+  __syncthreads();
+  const int lane = threadIdx.x & 31, t = blockIdx.x * 32 + (threadIdx.x >> 5);
+  if (t >= n) return;
+  const uint32_t mine = keys[t];
+  int place = 0;
+  for (int i = lane; i < n; i += 32) {
+    const uint32_t k = keys[i];
+    place += k < mine || (k == mine && i < t);
+  }
+  place = __reduce_add_sync(0xffffffffu, place);
+  if (lane == 0) {
+    sorted[place] = mine;
+    perm[place] = t;
+  }
+}
+
 template <typename ID>
 kairo_status sort_in_cluster(const ID* ids, int64_t n, int64_t n_rows, uint32_t* sorted, int32_t* perm,
                              const ZeroRows& zero, cudaStream_t s) {
@@ -437,6 +463,12 @@ size_t sort_ws_bytes(int64_t n) {
 template <typename ID>
 kairo_status sort_launch(const ID* ids, int64_t n, int64_t n_rows, uint32_t* sorted, int32_t* perm, void* ws,
                          const ZeroRows& zero, cudaStream_t s) {
+  if (n <= kRankTokens) {
+    k_sort_ranks<ID><<<static_cast<unsigned>(ceil_div64(n, 32)), 1024, 0, s>>>(ids, static_cast<int>(n), n_rows, sorted,
+                                                                              perm);
+    const cudaError_t e = cudaGetLastError();
+    return e != cudaSuccess ? cuda_fail(e, "launch of the token sort") : KAIRO_STATUS_SUCCESS;
+  }
   if (n <= kClusterTokens) return sort_in_cluster(ids, n, n_rows, sorted, perm, zero, s);
   const size_t col = align_up(static_cast<size_t>(n) * 4, 256);
   uint32_t* keys_b = static_cast<uint32_t*>(ws);
@@ -646,110 +678,182 @@ __global__ void __launch_bounds__(kGradThreads * kJoinGroups) k_grad_join(const 
 }
 
 // A short list (kFewTokens at most) needs no sorted order: every CTA takes 32
-// rows, picks their tokens out of the whole list, and sums each row's in token
-// order.  One launch instead of three (256 tokens, 10000 x 64: a call takes 16 us
-// instead of 31, most of it the host's).  A row's place in the sorted order is the number of
-// smaller ids, so the sum is cut where the chunks would cut it and its parts are
-// added as the join adds them: the result has the same bits.
-constexpr int kFewTokens = 512;
-static_assert(kFewTokens <= kGradChunk * 2 * kGradAhead, "a run has parts of the join's first two groups");
+// rows and a slice of the columns, picks the rows' tokens out of the whole list,
+// groups them by row in token order, and sums them.  One launch instead of
+// three.  A row's place in the sorted order is the number of smaller ids, so the
+// sum is cut where the chunks would cut it: the parts are the warps' items,
+// and those of one row are added as the join adds them, to the same bits.
+// fp32, this kernel and the three: 256 tokens of 10000 x 64 8.4 and 11.4 us, 64
+// tokens 5.0 and 10; it does not spread a frequent row over the GPU, so 256
+// tokens of 8874 x 2888 take 43 and 35 us and 471 would take 49 and 36.
+constexpr int kFewTokens = 256;
+constexpr int kFewThreads = 256;
+constexpr int kFewWarps = kFewThreads / 32;
+constexpr int kFewChunks = kFewTokens / kGradChunk + 1;        // that the tokens of a CTA can have places in
+constexpr int kFewItems = kFewRows + kFewChunks;               // parts of the rows of a CTA at most
+static_assert(kFewRows == 32 && kJoinGroups == 2, "a lane per row; parts go to the groups in turns of kGradAhead");
 template <typename TI, typename TO, typename ID, int VE>
-__global__ void __launch_bounds__(kGradThreads) k_grad_few(const TI* __restrict__ grad, int64_t ldg,
-                                                           const ID* __restrict__ ids, int n, int64_t n_rows,
-                                                           int64_t dim, float scale, TO* __restrict__ out, int64_t ldo,
-                                                           bool accumulate) {
-  __shared__ uint16_t tok[kFewTokens];   // tokens of these rows, in order
-  __shared__ uint8_t of[kFewTokens];     // the row of each, less the first
-  __shared__ int counts[2][kGradThreads / 32];
+__global__ void __launch_bounds__(kFewThreads) k_grad_few(const TI* __restrict__ grad, int64_t ldg,
+                                                          const ID* __restrict__ ids, int n, int64_t n_rows,
+                                                          int64_t dim, float scale, TO* __restrict__ out, int64_t ldo,
+                                                          bool accumulate, int turns) {
+  __shared__ uint16_t tok[kFewTokens], grouped[kFewTokens];  // tokens of these rows, in order; then row by row
+  __shared__ uint8_t of[kFewTokens];                         // the row of each of tok, less the first
+  __shared__ int counts[2][kFewWarps];
+  __shared__ int row_count[kFewRows], row_start[kFewRows], item_row[kFewItems], nitems;
+  // Parts of rows of several: in a chunk, one that goes on from before it and one
+  // that goes on behind it.
+  __shared__ float parts[2 * kFewChunks][32 * VE];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kFewRows;
-  int have = 0, before = 0;  // tokens of these rows, and of smaller ids
-  for (int t0 = 0; t0 < n; t0 += kGradThreads) {
-    const int t = t0 + threadIdx.x;
-    const int64_t id = t < n ? static_cast<int64_t>(ids[t]) : -1;
-    const bool mine = id >= r0 && id < r0 + kFewRows && id < n_rows;
-    const uint32_t vote = __ballot_sync(0xffffffffu, mine);
-    const uint32_t less = __ballot_sync(0xffffffffu, id >= 0 && id < r0);
-    if (lane == 0) {
-      counts[0][warp] = __popc(vote);
-      counts[1][warp] = __popc(less);
-    }
-    __syncthreads();
-    int at = have + __popc(vote & ((1u << lane) - 1u));
+  // A warp looks through its share of the list.
+  constexpr int TURNS = kFewTokens / kFewThreads;
+  const int t0 = warp * (32 * TURNS);
+  int64_t id[TURNS];
+  int mine = 0, less = 0;
 #pragma unroll
-    for (int w = 0; w < kGradThreads / 32; ++w) {
-      if (w < warp) at += counts[0][w];
-      have += counts[0][w];
-      before += counts[1][w];
-    }
-    if (mine) {
-      tok[at] = static_cast<uint16_t>(t);
-      of[at] = static_cast<uint8_t>(id - r0);
-    }
-    __syncthreads();
+  for (int j = 0; j < TURNS; ++j) {
+    const int t = t0 + j * 32 + lane;
+    id[j] = t < n ? static_cast<int64_t>(ids[t]) : -1;
+    if (id[j] >= n_rows) id[j] = -1;
   }
-  // A warp per row; the lanes go through the list together.
-  for (int r = warp; r < kFewRows && r0 + r < n_rows; r += kGradThreads / 32) {
-    int count = 0, smaller = 0;
-    for (int q = lane; q < have; q += 32) {
-      count += of[q] == r;
-      smaller += of[q] < r;
+#pragma unroll
+  for (int j = 0; j < TURNS; ++j) {
+    mine += __popc(__ballot_sync(0xffffffffu, id[j] >= r0 && id[j] < r0 + kFewRows));
+    less += __popc(__ballot_sync(0xffffffffu, id[j] >= 0 && id[j] < r0));
+  }
+  if (lane == 0) {
+    counts[0][warp] = mine;
+    counts[1][warp] = less;
+  }
+  __syncthreads();
+  int have = 0, before = 0, at = 0;  // tokens of these rows, of smaller ids, of these rows in the warps before
+#pragma unroll
+  for (int w = 0; w < kFewWarps; ++w) {
+    if (w < warp) at += counts[0][w];
+    have += counts[0][w];
+    before += counts[1][w];
+  }
+#pragma unroll
+  for (int j = 0; j < TURNS; ++j) {
+    const bool in = id[j] >= r0 && id[j] < r0 + kFewRows;
+    const uint32_t vote = __ballot_sync(0xffffffffu, in);
+    if (in) {
+      const int to = at + __popc(vote & ((1u << lane) - 1u));
+      tok[to] = static_cast<uint16_t>(t0 + j * 32 + lane);
+      of[to] = static_cast<uint8_t>(id[j] - r0);
     }
-    count = __reduce_add_sync(0xffffffffu, count);
-    if (!count && accumulate) continue;
-    const int first = before + __reduce_add_sync(0xffffffffu, smaller);  // place in the sorted order
-    TO* dst = out + (r0 + r) * ldo;
-    for (int64_t c0 = 0; c0 < dim; c0 += 32 * VE) {
-      const int64_t c = c0 + static_cast<int64_t>(lane) * VE;
-      // the part under way, and the join's first two groups
-      float acc[VE], group[2][VE];
+    at += __popc(vote);
+  }
+  __syncthreads();
+  for (int r = warp; r < kFewRows; r += kFewWarps) {
+    int c = 0;
+    for (int q = lane; q < have; q += 32) c += of[q] == r;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (lane == 0) row_count[r] = c;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    const int c = row_count[lane];
+    int x = c;
 #pragma unroll
-      for (int i = 0; i < VE; ++i) acc[i] = group[0][i] = group[1][i] = 0.f;
-      int place = first, part = 0;
-      if (count) {
-        for (int q0 = 0; q0 < have; q0 += 32) {
-          uint32_t left = __ballot_sync(0xffffffffu, q0 + lane < have && of[q0 + lane] == r);
-          while (left) {
-            Raw<TI, VE> f[kGradAhead];
-            uint32_t rest = left;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    row_start[lane] = x - c;
+    // Parts of the row: the chunks that it has places in.
+    const int place = before + x - c;
+    const int np = c ? (place + c - 1) / kGradChunk - place / kGradChunk + 1 : 0;
+    int y = np;
 #pragma unroll
-            for (int u = 0; u < kGradAhead; ++u) {
-              if (rest && c < dim) f[u].load(grad + tok[q0 + __ffs(rest) - 1] * ldg + c);
-              rest &= rest - 1;
-            }
+    for (int o = 1; o < 32; o <<= 1) {
+      const int z = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) y += z;
+    }
+    for (int i = 0; i < np; ++i) item_row[y - np + i] = lane | (i << 8);
+    if (lane == 31) nitems = y;
+  }
+  __syncthreads();
+  for (int r = warp; r < kFewRows; r += kFewWarps) {
+    int to = row_start[r];
+    if (!row_count[r]) continue;
+    for (int q0 = 0; q0 < have; q0 += 32) {
+      const bool in = q0 + lane < have && of[q0 + lane] == r;
+      const uint32_t vote = __ballot_sync(0xffffffffu, in);
+      if (in) grouped[to + __popc(vote & ((1u << lane) - 1u))] = tok[q0 + lane];
+      to += __popc(vote);
+    }
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int turn = 0; turn < turns; ++turn) {
+    const int64_t c0 = (static_cast<int64_t>(blockIdx.y) * turns + turn) * (32 * VE);
+    if (c0 >= dim) break;
+    const int64_t c = c0 + static_cast<int64_t>(lane) * VE;
+    const bool live = c < dim;
+    float acc[VE];
+    for (int i = warp; i < nitems; i += kFewWarps) {
+      const int r = item_row[i] & 255, part = item_row[i] >> 8;
+      const int count = row_count[r], place = before + row_start[r];
+      // places of the part, counted from the row's first
+      const int p0 = part ? (place / kGradChunk + part) * kGradChunk - place : 0;
+      const int p1 = min(count, (place / kGradChunk + part + 1) * kGradChunk - place);
+      const uint16_t* list = grouped + row_start[r];
 #pragma unroll
-            for (int u = 0; u < kGradAhead; ++u) {
-              if (!left) break;
-              left &= left - 1;
-              if (place % kGradChunk == 0 && place != first) {  // a new chunk begins
-                const int to = part <= kGradAhead ? 0 : 1;
+      for (int e = 0; e < VE; ++e) acc[e] = 0.f;
+      for (int q = p0; q < p1; q += kGradAhead) {
+        Raw<TI, VE> f[kGradAhead];
 #pragma unroll
-                for (int i = 0; i < VE; ++i) {
-                  if (to) group[1][i] += acc[i];
-                  else group[0][i] += acc[i];
-                  acc[i] = 0.f;
-                }
-                ++part;
-              }
-              ++place;
-              if (c < dim) {
+        for (int u = 0; u < kGradAhead; ++u)
+          if (live && q + u < p1) f[u].load(grad + static_cast<int64_t>(list[q + u]) * ldg + c);
 #pragma unroll
-                for (int i = 0; i < VE; ++i) acc[i] += f[u][i];
-              }
-            }
-          }
+        for (int u = 0; u < kGradAhead; ++u) {
+          if (!live || q + u >= p1) break;
+#pragma unroll
+          for (int e = 0; e < VE; ++e) acc[e] += f[u][e];
         }
       }
-      if (part > 0) {
+      if (p0 == 0 && p1 == count) {
+        if (live) emit_row<TO, VE>(out + (r0 + r) * ldo + c, acc, scale, accumulate);
+      } else {
+        const int slot = 2 * (place / kGradChunk + part - before / kGradChunk) + (part == 0);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) {
-          if (part <= kGradAhead) group[0][i] += acc[i];
-          else group[1][i] += acc[i];
-          acc[i] = group[0][i] + group[1][i];
+        for (int e = 0; e < VE; ++e) parts[slot][lane * VE + e] = acc[e];
+      }
+    }
+    if (!accumulate) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) acc[e] = 0.f;
+      for (int r = warp; r < kFewRows && r0 + r < n_rows; r += kFewWarps)
+        if (!row_count[r] && live) store_f32<TO, VE>(out + (r0 + r) * ldo + c, acc);
+    }
+    __syncthreads();
+    // Rows of several parts: the first to group 0, then kGradAhead to each group in turn.
+    for (int i = warp; i < nitems; i += kFewWarps) {
+      const int r = item_row[i] & 255;
+      if (item_row[i] >> 8 || i + 1 >= nitems || (item_row[i + 1] & 255) != r) continue;
+      const int chunk = (before + row_start[r]) / kGradChunk - before / kGradChunk;
+      float group[kJoinGroups][VE];
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        group[0][e] = parts[2 * chunk + 1][lane * VE + e];
+        group[1][e] = 0.f;
+      }
+      for (int k = 1; i + k < nitems && (item_row[i + k] & 255) == r; ++k) {
+        const bool second = ((k - 1) / kGradAhead) & 1;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const float v = parts[2 * (chunk + k)][lane * VE + e];
+          if (second) group[1][e] += v;
+          else group[0][e] += v;
         }
       }
-      if (c < dim) emit_row<TO, VE>(dst + c, acc, scale, accumulate);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) acc[e] = group[0][e] + group[1][e];
+      if (live) emit_row<TO, VE>(out + (r0 + r) * ldo + c, acc, scale, accumulate);
     }
+    __syncthreads();
   }
 }
 
@@ -800,12 +904,18 @@ void grad_with(const GradArgs& a, cudaStream_t s) {
                             a.partial, a.zero_rows_end, s);
     return;
   }
-  const unsigned grid = static_cast<unsigned>(ceil_div64(a.n_rows, kFewRows));
+  // Slices of the columns, in turns of 32 * VE.  Each CTA looks through the whole
+  // list, but one that has a frequent id is not to have many columns of it: 471
+  // skewed tokens, 8874 x 2888 fp32, took 49 us with two turns and 63 with six.
+  const int64_t groups = ceil_div64(a.n_rows, kFewRows), all = ceil_div64(a.dim, static_cast<int64_t>(32) * VE);
+  const int64_t room = 32 * device_sm_count(current_device());
+  const int turns = static_cast<int>(ceil_div64(all, std::min(all, std::max<int64_t>(1, room / groups))));
+  const dim3 grid(static_cast<unsigned>(groups), static_cast<unsigned>(ceil_div64(all, turns)));
   auto go = [&](auto* ids) {
     using ID = typename std::remove_const<typename std::remove_pointer<decltype(ids)>::type>::type;
-    k_grad_few<TI, TO, ID, VE><<<grid, kGradThreads, 0, s>>>(static_cast<const TI*>(a.grad), a.ldg, ids,
-                                                            static_cast<int>(a.n), a.n_rows, a.dim, a.scale,
-                                                            static_cast<TO*>(a.out), a.ldo, a.accumulate);
+    k_grad_few<TI, TO, ID, VE><<<grid, kFewThreads, 0, s>>>(static_cast<const TI*>(a.grad), a.ldg, ids,
+                                                           static_cast<int>(a.n), a.n_rows, a.dim, a.scale,
+                                                           static_cast<TO*>(a.out), a.ldo, a.accumulate, turns);
   };
   if (a.ids64) go(static_cast<const int64_t*>(a.ids));
   else go(static_cast<const int32_t*>(a.ids));
@@ -817,6 +927,7 @@ void grad_pick(int ve, const GradArgs& a, cudaStream_t s) {
     if (ve == 8) return grad_with<TI, TO, 8>(a, s);
   }
   if (ve >= 4) grad_with<TI, TO, 4>(a, s);
+  else if (ve == 2) grad_with<TI, TO, 2>(a, s);
   else grad_with<TI, TO, 1>(a, s);
 }
 
@@ -976,7 +1087,8 @@ kairo_status run_grad(const void* grad_output, int64_t ldg, kairo_dtype dtype, c
     // and 0.4 us per 1024, 5 MB are written per us).  Frequent ids are small in
     // most vocabularies, so few of these rows are written again.
     ZeroRows zero{};
-    if (!accumulate && nids <= kClusterTokens && dim * ob % 16 == 0 && ldo * ob % 16 == 0 && aligned(grad_weight, 16)) {
+    if (!accumulate && nids > kRankTokens && nids <= kClusterTokens && dim * ob % 16 == 0 && ldo * ob % 16 == 0 &&
+        aligned(grad_weight, 16)) {
       const int64_t bytes = (int64_t(40) << 20) + nids * 2048;
       zero.rows = std::min(n_rows, bytes / (dim * ob));
       zero.vecs = dim * ob / 16;
@@ -995,7 +1107,7 @@ kairo_status run_grad(const void* grad_output, int64_t ldg, kairo_dtype dtype, c
     return dim % ve == 0 && ldg % ve == 0 && ldo % ve == 0 && aligned(grad_output, ve * ib) &&
            aligned(grad_weight, ve * ob);
   };
-  const int ve = ib == 2 && ob == 2 && fits(8) ? 8 : (fits(4) ? 4 : 1);
+  const int ve = ib == 2 && ob == 2 && fits(8) ? 8 : (fits(4) ? 4 : (fits(2) ? 2 : 1));
   for_types(dtype, out_dtype, [&](auto ti, auto to) { grad_pick<decltype(ti), decltype(to)>(ve, a, s); });
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "launch of the embedding gradient");

@@ -136,6 +136,23 @@ def test_grad(gt, ot, case):
                                            out_dtype=ot))
 
 
+@pytest.mark.parametrize("tokens", [255, 256, 257, 511, 512, 513, 4095, 4096, 4097, 65536, 65537])
+@pytest.mark.parametrize("dim", [6, 67, 264])
+def test_grad_at_the_list_lengths(tokens, dim):
+    """Lists on both sides of every length at which the order is found in another way."""
+    n = 90
+    g = torch.Generator().manual_seed(tokens)
+    grad = torch.randn(tokens, dim, generator=g).half()
+    ids = _ids(n, tokens, seed=dim, skew=3.0)
+    ids[2::13] = n
+    order = sort_tokens(ids.to(DEV), n)
+    key = torch.where(ids >= n, n, ids)
+    assert torch.equal(order.perm.cpu().long(), torch.argsort(key, stable=True))
+    out = embedding_grad(grad.to(DEV), ids.to(DEV), n, scale=0.5, out_dtype=torch.float32)
+    _check_grad(grad, ids, n, 0.5, out)
+    assert torch.equal(out, embedding_grad(grad.to(DEV), order, n, scale=0.5, out_dtype=torch.float32))
+
+
 @pytest.mark.parametrize("tokens", [1, 31, 32, 33, 64, 65, 1000, 20000])
 def test_grad_of_one_row(tokens):
     """All tokens share one id; the runs end before, at and behind chunk borders."""
