@@ -327,7 +327,10 @@ kairo_status check_grad(const Grad& p, int64_t rank, kairo_dtype dtype, const vo
   return KAIRO_STATUS_SUCCESS;
 }
 
-bool z_aligned(const Grad& p) { return p.codes || (p.k % 8 == 0 && p.ldz % 8 == 0 && aligned16(p.z)); }
+// 16-byte accesses to z and the gradient; an 8-bit z always has them, and its gradient is stored value by value.
+bool grad_aligned(const Grad& p) {
+  return p.codes || (p.k % 8 == 0 && p.ldz % 8 == 0 && aligned16(p.z) && aligned16(p.grad));
+}
 
 // One or two of them in one launch (two: neither in 8 bits).
 kairo_status run_grads(const Grad* p, int count, int64_t rank, kairo_dtype dtype, const void* plan, int64_t ntokens,
@@ -349,7 +352,7 @@ kairo_status run_grads(const Grad* p, int count, int64_t rank, kairo_dtype dtype
     o.ldq = p[i].ldq;
     o.lds = p[i].lds;
     o.k = static_cast<int32_t>(p[i].k);
-    vec = vec && z_aligned(p[i]);
+    vec = vec && grad_aligned(p[i]);
     widest = std::max(widest, p[i].k);
     total += p[i].k;
   }

@@ -12,6 +12,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from kairo_b200 import _lib
 from kairo_b200.ops import (
     AdaptedSparseLinear,
     BlockSparseLinear,
@@ -489,3 +490,29 @@ def test_offsets_pass_32_bits():
     # dlow = 64 for the three tokens with an adapter, dX = 4 * 64 * 2^-10
     assert dx[-1].unique().tolist() == [0.25] and dx[3].unique().tolist() == [0.25] and int(dx[4].count_nonzero()) == 0
     assert dd[1].unique().tolist() == [64.0] and dd[0, 0, 5].item() == 128.0 and du[1].unique().tolist() == [32.0]
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("gdt", [None, torch.float32])
+def test_gradients_at_any_address(dt, gdt):
+    """The library's entries write gradients that start beside a 16-byte boundary, and nothing around them."""
+    t, k, n, r, g = 70, 64, 72, 6, 3
+    gdt = gdt or dt
+    x, dy, a, ids = _problem(dt, t, k, n, r, g, seed=9)
+    plan = adapter_plan(ids.to(DEV), g)
+    _, low = adapter_linear(x, a, plan, return_low=True)
+    _, dd, du = adapter_linear_backward(dy, x, a, plan, low=low, grad_dtype=gdt)
+    _, dlow = adapter_linear(dy, LowRankAdapters(down=a.up, up=a.down, scale=a.scale), plan, return_low=True)
+    lib, code, gcode = _lib.lib(), _lib.kairo_dtype(dt), _lib.kairo_dtype(gdt)
+    s = torch.cuda.current_stream().cuda_stream
+    for off in (1, 3):
+        both = [torch.full((want.numel() + 8,), 7.0, dtype=gdt, device=DEV) for want in (dd, du)]
+        at = [b[off:].data_ptr() for b in both]
+        _lib.check(lib.kairo_low_rank_wgrads(dlow.data_ptr(), low.data_ptr(), r, x.data_ptr(), k, k, dy.data_ptr(), n, n,
+                                             code, plan.memory.data_ptr(), t, g, at[0], at[1], gcode, s), "wgrads")
+        one = torch.full((dd.numel() + 8,), 7.0, dtype=gdt, device=DEV)
+        _lib.check(lib.kairo_low_rank_wgrad(dlow.data_ptr(), r, x.data_ptr(), k, k, code, plan.memory.data_ptr(), t, g,
+                                            one[off:].data_ptr(), gcode, s), "wgrad")
+        for buf, want in ((both[0], dd), (both[1], du), (one, dd)):
+            assert torch.equal(buf[off : off + want.numel()].view_as(want), want)
+            assert bool((buf[:off] == 7).all()) and bool((buf[off + want.numel():] == 7).all())
