@@ -385,7 +385,9 @@ KAIRO_API kairo_status kairo_bsr_sddmm_q8_workspace_size(const kairo_bsr* a, int
  *                         from dlow and x (k features), d_up from low and dy
  *                         (n features).
  * x, z, down, up f16 or bf16 (one dtype); base, y and grad that dtype or fp32.
- * rank at most 128, at most 65535 adapters, 2^24 tokens, 2^22 features.  All
+ * rank at most 128, at most 65535 adapters, 2^24 tokens, 2^22 features.  plan
+ * and workspace start on a multiple of 16 bytes; the other operands may have any
+ * address of their type (slower where one is not a multiple of 16).  All
  * asynchronous on `stream`.
  * ---------------------------------------------------------------------- */
 KAIRO_API kairo_status kairo_adapter_plan_build(const void* ids, int32_t id_bytes, int64_t ntokens,
@@ -502,7 +504,7 @@ KAIRO_API kairo_status kairo_sparse_scatter_grad_workspace_size(int64_t nactive,
  *                           means that none is needed.
  * dtype and out_dtype f32, f16 or bf16, in any combination; n_rows and nids
  * below 2^31 - 4096.  All asynchronous on `stream`; the workspaces need no
- * initial value.
+ * initial value, and start on a multiple of 16 bytes.
  * ---------------------------------------------------------------------- */
 KAIRO_API kairo_status kairo_embedding_lookup(const void* weight, int64_t n_rows, int64_t dim, int64_t ldw,
                                               kairo_dtype dtype, const void* ids, int32_t id_bytes, int64_t nids,

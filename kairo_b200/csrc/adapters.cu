@@ -233,6 +233,8 @@ extern "C" kairo_status kairo_adapter_plan_build(const void* ids, int32_t id_byt
   if (st) return st;
   if (id_bytes != 4 && id_bytes != 8) return fail(KAIRO_STATUS_INVALID_VALUE, "ids must be int32 or int64");
   if (!plan || !workspace || (ntokens > 0 && !ids)) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+  if (!aligned16(plan) || !aligned16(workspace))
+    return fail(KAIRO_STATUS_INVALID_VALUE, "plan and workspace must be 16-byte aligned");
   if (plan_size < need) return fail(KAIRO_STATUS_INVALID_VALUE, "plan memory too small");
   if (workspace_bytes < ws_need) return fail(KAIRO_STATUS_WORKSPACE_TOO_SMALL, "adapter plan workspace too small");
   cudaStream_t s = static_cast<cudaStream_t>(stream);

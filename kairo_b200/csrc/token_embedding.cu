@@ -1020,6 +1020,7 @@ extern "C" kairo_status kairo_token_sort(const void* ids, int32_t id_bytes, int6
   if (nids == 0) return KAIRO_STATUS_SUCCESS;
   if (!ids || !sorted || !perm || !workspace)
     return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+  if (!aligned(workspace, 16)) return fail(KAIRO_STATUS_INVALID_VALUE, "workspace must be 16-byte aligned");
   if (workspace_bytes < need) return fail(KAIRO_STATUS_WORKSPACE_TOO_SMALL, "token sort workspace too small");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint32_t* keys = reinterpret_cast<uint32_t*>(sorted);
@@ -1060,6 +1061,8 @@ kairo_status run_grad(const void* grad_output, int64_t ldg, kairo_dtype dtype, c
   const size_t order_at = align_up(need, 256);
   if (ids) need = nids <= kFewTokens ? 0 : order_at + order_bytes(nids) + sort_ws_bytes(nids);
   if (need > 0 && !workspace) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+  if (need > 0 && !aligned(workspace, 16))
+    return fail(KAIRO_STATUS_INVALID_VALUE, "workspace must be 16-byte aligned");
   if (workspace_bytes < need) return fail(KAIRO_STATUS_WORKSPACE_TOO_SMALL, "embedding gradient workspace too small");
   GradArgs a{};
   a.grad = grad_output;

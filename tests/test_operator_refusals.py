@@ -88,6 +88,19 @@ def test_embedding_c_refusals():
     assert grad_ids(ids=None) == _lib.INVALID_VALUE and grad_ids(idb=2) == _lib.INVALID_VALUE
 
 
+def test_misaligned_memory_is_refused():
+    """Workspaces and plans are bytes to the caller and vectors to the kernels."""
+    lib = _lib.lib()
+    some, odd, big = ctypes.c_void_p(256), ctypes.c_void_p(260), 1 << 30
+    assert lib.kairo_token_sort(some, 8, 5000, 70000, some, some, odd, big, None) == _lib.INVALID_VALUE
+    assert lib.kairo_embedding_grad(some, 8, 0, some, 8, 5000, 4, 8, 1.0, some, 8, 0, 0, odd, big,
+                                    None) == _lib.INVALID_VALUE
+    assert lib.kairo_embedding_grad_sorted(some, 8, 0, some, some, 300, 4, 8, 1.0, some, 8, 0, 0, odd, big,
+                                           None) == _lib.INVALID_VALUE
+    assert lib.kairo_adapter_plan_build(some, 8, 10, 3, odd, big, some, big, None) == _lib.INVALID_VALUE
+    assert lib.kairo_adapter_plan_build(some, 8, 10, 3, some, big, odd, big, None) == _lib.INVALID_VALUE
+
+
 def _bsr():
     return BlockSparseMatrix(row_ptr=torch.tensor([0, 1], dtype=torch.int32), col_idx=torch.zeros(1, dtype=torch.int32),
                              blocks=torch.zeros(1, 64, 64), shape=(64, 64), block_size=(64, 64))
