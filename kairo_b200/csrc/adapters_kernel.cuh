@@ -200,23 +200,6 @@ __device__ __forceinline__ uint32_t pair_of(const uint4& lo, const uint4& hi, in
   return __byte_perm(word(lo, j >> 1), word(hi, j >> 1), (j & 1) ? 0x7632 : 0x5410);
 }
 
-// 8 elements at p, of which the first `left` exist (left may be <= 0).  VEC:
-// p is 16-byte aligned and left is a multiple of 8 or not positive.
-template <typename T, bool VEC>
-__device__ __forceinline__ uint4 load8(const T* p, int left) {
-  uint4 v = make_uint4(0u, 0u, 0u, 0u);
-  if constexpr (VEC) {
-    if (left > 0) v = __ldg(reinterpret_cast<const uint4*>(p));
-  } else {
-    uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < left) w[i >> 1] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[i]) << (16 * (i & 1));
-    v = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-  return v;
-}
-
 template <typename T>
 __device__ __forceinline__ uint16_t bits16(float v) {
   const T h = from_f32<T>(v);
@@ -243,25 +226,10 @@ __device__ __forceinline__ void power_scale(float m, float* down, float* up) {
 // copies land where the same lane reads them, so that many loads are in flight
 // without registers to hold them and without any barrier.  Vector i of a slot
 // stands at [i][lane].
-template <typename T, bool VEC>
+template <typename T>
 __device__ __forceinline__ void fetch(uint32_t dst, const T* p, int left) {
-  if constexpr (VEC) {
-    // no byte is read where left <= 0; 16 zero bytes are written
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(p), "r"(left > 0 ? 16 : 0) : "memory");
-  } else {
-    constexpr int N = 16 / static_cast<int>(sizeof(T));
-    uint4 v;
-    if constexpr (N == 8) {
-      v = load8<T, false>(p, left);
-    } else {
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = i < left ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
-      v = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-                 : "memory");
-  }
+  // no byte is read where left <= 0; 16 zero bytes are written
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(p), "r"(left > 0 ? 16 : 0) : "memory");
 }
 // Place in a 512-byte vector slot of the 16 bytes that are chunk `c` of the 128
 // bytes of row `t`: a row is written as one (in lane order, a copy of four rows
@@ -274,6 +242,25 @@ __device__ __forceinline__ uint32_t by_rows(int c, int t) {
 // The same for the 8 codes that are chunk `c` of the 64 codes of row `t`.
 __device__ __forceinline__ uint32_t codes_by_rows(int c, int t) {
   return static_cast<uint32_t>(t * 8 + (c ^ (4 * (t >> 1)))) * 8u;
+}
+// Operands at any address of their type (VEC false): the same slots, filled by
+// the whole warp value by value, a row at a time, so that an access meets one
+// line of one row (with every lane loading its own 8 values one by one it met
+// eight).  What a lane reads was then written by others: a warp barrier stands
+// between filling and reading, and between reading and the next filling.
+// CONST: nothing writes the operand during the launch (base may be y).
+template <typename T, bool CONST = true>
+__device__ __forceinline__ uint32_t value_at(const T* row, int c, int n) {
+  using Bits = std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t>;
+  if (c >= n) return 0u;
+  const Bits* p = reinterpret_cast<const Bits*>(row) + c;
+  return CONST ? __ldg(p) : *p;
+}
+__device__ __forceinline__ void put16(uint32_t dst, uint32_t v) {
+  asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst), "h"(static_cast<uint16_t>(v)) : "memory");
+}
+__device__ __forceinline__ void put32(uint32_t dst, uint32_t v) {
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst), "r"(v) : "memory");
 }
 __device__ __forceinline__ uint4 landed(uint32_t src) {
   uint4 v;
@@ -317,8 +304,15 @@ struct ApplyShape {
     return STAGES * STEP > e ? STAGES * STEP : e;
   }
   static constexpr size_t ring_bytes(bool base_f32) { return static_cast<size_t>(kWarps) * ring(base_f32) * 512; }
-  static constexpr size_t bytes(int terms, bool base_f32) {
-    const size_t tiles = (ALIAS ? 2 : kWarps / 2 + 1) * static_cast<size_t>(LOW);
+  // Floats of the warps' partial tiles; afterwards, with operands at any
+  // address, 8 rows of 64 results of every warp on their way out.
+  static constexpr int out_pitch(int y_bytes) { return 64 * y_bytes + 16; }
+  static constexpr int red(int y_bytes, bool vec) {
+    const int tiles = (ALIAS ? 1 : kWarps / 2) * LOW, out = kWarps * 8 * out_pitch(y_bytes) / 4;
+    return vec || tiles > out ? tiles : out;
+  }
+  static constexpr size_t bytes(int terms, bool base_f32, int y_bytes, bool vec) {
+    const size_t tiles = static_cast<size_t>(red(y_bytes, vec)) + LOW;
     return ring_bytes(base_f32) + (tiles + ROWS) * 4 + static_cast<size_t>(terms) * ROWS * PITCH * 2;
   }
 };
@@ -339,7 +333,7 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApp
   static_assert(!S::ALIAS || S::ring_bytes(BASE_F32) >= kWarps / 2 * S::LOW * 4, "partial tiles fit in the ring");
   float* part = reinterpret_cast<float*>(smem + S::ring_bytes(BASE_F32));  // [LOW]: this CTA's partial tile
   float* red = S::ALIAS ? reinterpret_cast<float*>(smem) : part;  // [kWarps / 2][LOW]
-  float* low = part + (S::ALIAS ? 1 : kWarps / 2) * S::LOW;      // [LOW]: the whole tile
+  float* low = part + S::red(sizeof(TY), VEC);                   // [LOW]: the whole tile
   float* row_up = low + S::LOW;                                  // [ROWS]: power of two of every row (fp16)
   uint16_t* terms = reinterpret_cast<uint16_t*>(row_up + S::ROWS);  // [TERMS][ROWS][PITCH]
 
@@ -388,20 +382,48 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApp
         xrow[m][h] = static_cast<const T*>(a.x) + static_cast<int64_t>(max(tok[m][h], 0)) * a.ldx;
     auto issue = [&](int i, int at) {
       if (i < steps) {
-        const int left = a.k - kk;
-        const int off = left > 0 ? kk : 0;
-        const uint32_t dst = ring + static_cast<uint32_t>(at * S::STEP * 512);
+        if constexpr (VEC) {
+          const int left = a.k - kk;
+          const int off = left > 0 ? kk : 0;
+          const uint32_t dst = ring + static_cast<uint32_t>(at * S::STEP * 512);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const bool there = j * 8 + g < a.rank;
-          fetch<T, VEC>(dst + j * 512, wrow + (there ? j * wstep + off : off - g * static_cast<int64_t>(a.k)),
-                        there ? left : 0);
+          for (int j = 0; j < NT; ++j) {
+            const bool there = j * 8 + g < a.rank;
+            fetch<T>(dst + j * 512, wrow + (there ? j * wstep + off : off - g * static_cast<int64_t>(a.k)),
+                     there ? left : 0);
+          }
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              fetch<T>(dst + (NT + 2 * m + h) * 512, xrow[m][h] + off, tok[m][h] >= 0 ? left : 0);
+        } else {
+          static_assert(MT == 1, "two vectors of tokens");
+          const int c = kk - 8 * t + lane;
+          const T* w0 = static_cast<const T*>(a.down) + static_cast<int64_t>(tile.adapter) * a.rank * a.k;
+          const uint32_t dst = ring0 + static_cast<uint32_t>(at * S::STEP * 512 + lane * 2);
+#pragma unroll
+          for (int v0 = 0; v0 < S::STEP; v0 += 2) {  // two vectors under way
+            uint32_t v[2][8];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int r = 0; r < 8; ++r) {
+                if (v0 < NT) {
+                  const int rr = (v0 + u) * 8 + r;
+                  v[u][r] = rr < a.rank ? value_at<T>(w0 + static_cast<int64_t>(rr) * a.k, c, a.k) : 0u;
+                } else {
+                  const int tk = __shfl_sync(0xffffffffu, tok[0][u], 4 * r);
+                  v[u][r] = tk >= 0 ? value_at<T>(static_cast<const T*>(a.x) + static_cast<int64_t>(tk) * a.ldx, c, a.k)
+                                    : 0u;
+                }
+              }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int r = 0; r < 8; ++r) put16(dst + (v0 + u) * 512 + r * 64, v[u][r]);
+          }
         }
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            fetch<T, VEC>(dst + (NT + 2 * m + h) * 512, xrow[m][h] + off, tok[m][h] >= 0 ? left : 0);
         kk += (i & 1) ? stride - 32 : 32;
       }
       commit();
@@ -411,6 +433,7 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApp
     int at = 0;
     for (int i = 0; i < steps; ++i) {
       wait_all_but<S::STAGES - 1>();
+      if constexpr (!VEC) __syncwarp();
       const uint32_t src = ring + static_cast<uint32_t>(at * S::STEP * 512);
       uint4 wb[NT];
 #pragma unroll
@@ -425,6 +448,7 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApp
 #pragma unroll
         for (int j = 0; j < NT; ++j) mma<T>(acc[m][j], a1, wb[j].z, wb[j].w);
       }
+      if constexpr (!VEC) __syncwarp();
       issue(i + S::STAGES, at);  // every vector of the slot is in use above
       at = at + 1 == S::STAGES ? 0 : at + 1;
     }
@@ -438,20 +462,77 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApp
   constexpr int UNITS = KT + BU * MT;
   const T* up = static_cast<const T*>(a.up) + static_cast<int64_t>(max(tile.adapter, 0)) * a.rank * a.n;
   auto issue_up = [&](int n0, int kt) {
-    const int c = n0 + 8 * up_chunk, left = live && c < a.n ? a.n - c : 0;
-    const uint32_t dst = up_ring + static_cast<uint32_t>(kt * 4 * 512);
-    const T* col = live ? up + (left > 0 ? c : 0) : static_cast<const T*>(a.x);
+    if constexpr (VEC) {
+      const int c = n0 + 8 * up_chunk, left = live && c < a.n ? a.n - c : 0;
+      const uint32_t dst = up_ring + static_cast<uint32_t>(kt * 4 * 512);
+      const T* col = live ? up + (left > 0 ? c : 0) : static_cast<const T*>(a.x);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = kt * 16 + 2 * t + (i & 1) + (i >> 1) * 8;
-      const bool there = live && r < a.rank;
-      fetch<T, VEC>(dst + i * 512, col + (there ? r * static_cast<int64_t>(a.n) : 0), there ? left : 0);
+      for (int i = 0; i < 4; ++i) {
+        const int r = kt * 16 + 2 * t + (i & 1) + (i >> 1) * 8;
+        const bool there = live && r < a.rank;
+        fetch<T>(dst + i * 512, col + (there ? r * static_cast<int64_t>(a.n) : 0), there ? left : 0);
+      }
+    } else if (live) {
+      // value `lane` and `lane` + 32 of row 2 q + .. of each vector
+      const uint32_t dst = ring0 + static_cast<uint32_t>(kt * 4 * 512 + 2 * (lane & 7));
+#pragma unroll
+      for (int i0 = 0; i0 < 4; i0 += 2) {
+        uint32_t v[2][4][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              const int r = kt * 16 + 2 * q + u + (i0 >> 1) * 8;
+              v[u][q][s] = r < a.rank ? value_at<T>(up + static_cast<int64_t>(r) * a.n, n0 + lane + 32 * s, a.n) : 0u;
+            }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+              put16(dst + (i0 + u) * 512 + by_rows((lane >> 3) + 4 * s, q), v[u][q][s]);
+      }
     }
     commit();
   };
   auto issue_base = [&](int n0, int m, int b) {  // m and b are known when compiled
-    const uint32_t dst = ring + static_cast<uint32_t>((KT + BU * m + b) * 4 * 512);
-    if constexpr (BASE_F32) {
+    const uint32_t dst = (VEC ? ring : ring0) + static_cast<uint32_t>((KT + BU * m + b) * 4 * 512);
+    if constexpr (!VEC) {
+      constexpr int ROWS_OF = BASE_F32 ? 1 : 2;  // halves of the tokens in this unit
+#pragma unroll
+      for (int h0 = 0; h0 < ROWS_OF; ++h0) {
+        const int mine = a.base ? tok[m][BASE_F32 ? b : h0] : -1;
+        uint32_t v[8][2];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const int tk = __shfl_sync(0xffffffffu, mine, 4 * r);
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const int c = n0 + 32 * s + lane;
+            if constexpr (BASE_F32)
+              v[r][s] = tk >= 0 ? value_at<float, false>(
+                                      static_cast<const float*>(a.base) + static_cast<int64_t>(tk) * a.ldb, c, a.n)
+                                : 0u;
+            else
+              v[r][s] = tk >= 0 ? value_at<T, false>(static_cast<const T*>(a.base) + static_cast<int64_t>(tk) * a.ldb, c,
+                                                     a.n)
+                                : 0u;
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            if constexpr (BASE_F32)
+              put32(dst + (2 * s + ((lane >> 2) & 1)) * 512 + (4 * r + (lane >> 3)) * 16 + (lane & 3) * 4, v[r][s]);
+            else
+              put16(dst + (2 * h0 + s) * 512 + r * 64 + lane * 2, v[r][s]);
+          }
+      }
+    } else if constexpr (BASE_F32) {
       const int tk = a.base ? tok[m][b] : -1;
       const float* row = tk >= 0 ? static_cast<const float*>(a.base) + static_cast<int64_t>(tk) * a.ldb
                                  : reinterpret_cast<const float*>(a.x);
@@ -459,7 +540,7 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApp
       for (int i = 0; i < 4; ++i) {
         const int c = n0 + 32 * (i >> 1) + 8 * t + 4 * (i & 1);
         const int left = tk >= 0 ? a.n - c : 0;
-        fetch<float, VEC>(dst + i * 512, row + (left > 0 ? c : 0), left);
+        fetch<float>(dst + i * 512, row + (left > 0 ? c : 0), left);
       }
     } else {
 #pragma unroll
@@ -471,7 +552,7 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApp
         for (int q = 0; q < 2; ++q) {
           const int c = n0 + 32 * q + 8 * t;
           const int left = tk >= 0 ? a.n - c : 0;
-          fetch<T, VEC>(dst + (2 * h + q) * 512, row + (left > 0 ? c : 0), left);
+          fetch<T>(dst + (2 * h + q) * 512, row + (left > 0 ? c : 0), left);
         }
       }
     }
@@ -585,6 +666,7 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApp
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
       wait_all_but<UNITS - 1>();
+      if constexpr (!VEC) __syncwarp();
       const uint32_t src = up_ring + static_cast<uint32_t>(kt * 4 * 512);
       const uint4 v0 = landed(src), v1 = landed(src + 512), v2 = landed(src + 1024), v3 = landed(src + 1536);
 #pragma unroll
@@ -592,6 +674,7 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApp
         b0[kt][j] = pair_of(v0, v1, j);
         b1[kt][j] = pair_of(v2, v3, j);
       }
+      if constexpr (!VEC) __syncwarp();
       issue_up(later, kt);
     }
 #pragma unroll
@@ -600,6 +683,7 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApp
 #pragma unroll
       for (int b = 0; b < BU; ++b) {
         wait_all_but<UNITS - 1>();
+        if constexpr (!VEC) __syncwarp();
         const uint32_t src = ring + static_cast<uint32_t>((KT + BU * m + b) * 4 * 512);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -615,6 +699,7 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApp
               out[i >> 1][(i & 1) * 8 + q] = value16<T>(static_cast<uint16_t>(word(v, q >> 1) >> (16 * (q & 1))));
           }
         }
+        if constexpr (!VEC) __syncwarp();
         issue_base(later, m, b);
       }
       if (m * 16 >= count) continue;  // the same for the whole cluster
@@ -646,9 +731,9 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApp
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (tok[m][h] < 0) continue;
-        TY* to = y + static_cast<int64_t>(tok[m][h]) * a.ldy;
         if constexpr (VEC) {
+          if (tok[m][h] < 0) continue;
+          TY* to = y + static_cast<int64_t>(tok[m][h]) * a.ldy;
           constexpr int W = 16 / static_cast<int>(sizeof(TY));  // features per 16 bytes
 #pragma unroll
           for (int q = 0; q < 16 / W; ++q) {
@@ -661,11 +746,29 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApp
             }
           }
         } else {
+          // 8 rows through the shared memory of the partial tiles, then row by row
+          constexpr int P = S::out_pitch(sizeof(TY));
+          uint8_t* rows = reinterpret_cast<uint8_t*>(part) + warp * 8 * P;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int c = n0 + 32 * (i >> 3) + 8 * t + (i & 7);
-            if (c < a.n) to[c] = from_f32<TY>(out[h][i]);
+          for (int q = 0; q < 2; ++q) {
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = out[h][8 * q + i];
+            store_f32<TY, 8>(reinterpret_cast<TY*>(rows + g * P) + 32 * q + 8 * t, f);
           }
+          __syncwarp();
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            const int tk = __shfl_sync(0xffffffffu, tok[m][h], 4 * r);
+            if (tk < 0) break;  // the rows behind the tile's last
+            const TY* from = reinterpret_cast<const TY*>(rows + r * P);
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              const int c = n0 + 32 * s + lane;
+              if (c < a.n) y[static_cast<int64_t>(tk) * a.ldy + c] = from[32 * s + lane];
+            }
+          }
+          __syncwarp();
         }
       }
     }
@@ -687,7 +790,7 @@ cudaError_t allow_smem(F* fn, size_t bytes, std::atomic<uint64_t>* done) {
 template <typename T, typename TY, typename S, bool BASE_F32, bool VEC>
 cudaError_t launch_apply_as(const LowRankApplyArgs& a, int64_t clusters, int cluster, cudaStream_t s) {
   constexpr int TERMS = std::is_same_v<TY, float> ? 3 : 2;
-  constexpr size_t bytes = S::bytes(TERMS, BASE_F32);
+  constexpr size_t bytes = S::bytes(TERMS, BASE_F32, sizeof(TY), VEC);
   static_assert(bytes <= 227 * 1024, "shared memory of one CTA");
   constexpr int MINB = bytes <= 113 * 1024 ? 2 : 1;
   auto* fn = &k_apply<T, TY, S, TERMS, BASE_F32, VEC, MINB>;
@@ -807,8 +910,8 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgr
   const int units = chunks > 0 ? 4 * (chunks - 1) + (last_have + 15) / 16 : 0;
   const int cz = c0 + lc + 8 * g;  // features this lane loads
   const int left = a.k - cz;
-  const uint32_t ring = smem_addr(smem) + static_cast<uint32_t>(warp * S::UNITS * 4 * 512) +
-                        (Q8 ? codes_by_rows(g, t) : by_rows(g, t));
+  const uint32_t ring0 = smem_addr(smem) + static_cast<uint32_t>(warp * S::UNITS * 4 * 512);
+  const uint32_t ring = ring0 + (Q8 ? codes_by_rows(g, t) : by_rows(g, t));
 
   // The tokens of a chunk are in shared memory three chunks ahead of its use.
   static_assert(S::UNITS <= 8, "a unit's tokens are known when it starts");
@@ -826,6 +929,35 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgr
   const int8_t* qcol = Q8 ? a.codes + (left > 0 ? cz : 0) : nullptr;
   auto issue = [&](int u, int at) {
     if (u < units) {
+      if constexpr (!VEC) {
+        const uint32_t dst = ring0 + static_cast<uint32_t>(at * 4 * 512 + 2 * (lane & 7));
+        const int* unit = toks + ((u >> 2) & 3) * kChunk + (u & 3) * 16;
+        const int c = c0 + lc + lane;
+#pragma unroll
+        for (int i0 = 0; i0 < 4; i0 += 2) {
+          uint32_t v[2][4][2];
+#pragma unroll
+          for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int tok = unit[2 * q + w + (i0 >> 1) * 8];
+#pragma unroll
+              for (int s = 0; s < 2; ++s)
+                v[w][q][s] =
+                    tok >= 0 ? value_at<T>(static_cast<const T*>(a.z) + static_cast<int64_t>(tok) * a.ldz, c + 32 * s, a.k)
+                             : 0u;
+            }
+#pragma unroll
+          for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int s = 0; s < 2; ++s)
+                put16(dst + (i0 + w) * 512 + by_rows((lane >> 3) + 4 * s, q), v[w][q][s]);
+        }
+        commit();
+        return;
+      }
       const uint32_t dst = ring + static_cast<uint32_t>(at * 4 * 512);
       const int* mine = toks + ((u >> 2) & 3) * kChunk + (u & 3) * 16 + 2 * t;
       const int2 ta = *reinterpret_cast<const int2*>(mine), tb = *reinterpret_cast<const int2*>(mine + 8);
@@ -835,7 +967,7 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgr
         const int n = tk[i] >= 0 ? left : 0;
         const int tok = max(tk[i], 0);
         if constexpr (!Q8) {
-          fetch<T, VEC>(dst + i * 512, zcol + static_cast<int64_t>(tok) * a.ldz, n);
+          fetch<T>(dst + i * 512, zcol + static_cast<int64_t>(tok) * a.ldz, n);
         } else {
           // code rows are 16-byte aligned and padded to 8
           asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst + i * 512),
@@ -938,6 +1070,7 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgr
 #pragma unroll 1
     for (int ks = 0; ks < here; ++ks) {
       wait_all_but<S::UNITS - 1>();
+      if constexpr (!VEC) __syncwarp();
       const uint32_t src = ring + static_cast<uint32_t>(at * 4 * 512);
       uint4 v[4];
 #pragma unroll
@@ -956,6 +1089,7 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgr
         b0[j] = pair_of(v[0], v[1], j);
         b1[j] = pair_of(v[2], v[3], j);
       }
+      if constexpr (!VEC) __syncwarp();
       issue(4 * n + ks + S::UNITS, at);
       at = at + 1 == S::UNITS ? 0 : at + 1;
 #pragma unroll
