@@ -182,7 +182,11 @@ int pick_tile(int64_t t, int64_t rank, bool vec, bool base_f32) {
 // two, 12.3 with eight), and where the contraction is so long that a warp has
 // 32 turns, more, shorter CTAs even out the SMs (8192 tokens, 32768 features:
 // 142 us with two, 139 with four).
-int pick_cluster(int64_t tiles, int tile, int64_t k, int64_t n, int64_t rank) {
+int pick_cluster(int64_t t, int64_t g, int tile, int64_t k, int64_t n, int64_t rank) {
+  // Half a tile is lost per adapter where one has several tokens for a tile; the
+  // bound on their number is too many then (4369 tokens of 11 adapters: 74
+  // against 80, and the difference between two CTAs per tile and one: 53 us and 87).
+  const int64_t tiles = t >= tile * (g + 1) ? t / tile + (g + 1) / 2 : max_tiles(t, g, tile);
   const int64_t room = (tile * rank > 1024 ? 1 : 2) * device_sm_count(current_device());
   int c = 1;
   while (c < kCluster && (tiles * 2 * c <= room || k >= int64_t(32) * 8 * 64 * c) &&
@@ -293,7 +297,7 @@ extern "C" kairo_status kairo_low_rank_apply(const void* x, int64_t ldx, int64_t
   a.rank = static_cast<int32_t>(rank);
   a.base_f32 = base && base_dtype == KAIRO_DTYPE_F32;
   const int64_t clusters = max_tiles(ntokens, nadapters, tile);
-  const int cluster = pick_cluster(clusters, tile, k, n, rank);
+  const int cluster = pick_cluster(ntokens, nadapters, tile, k, n, rank);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool yf = y && y_dtype == KAIRO_DTYPE_F32;
   const cudaError_t err = dtype == KAIRO_DTYPE_F16

@@ -866,7 +866,7 @@ struct WgradShape {
   static constexpr size_t bytes(int terms, bool half, bool q8) {
     return SHARED_BYTES + (q8 ? static_cast<size_t>(2 * kChunk * (COLS / 64)) * 4 : 0) +
            static_cast<size_t>(2 * RP + 4 * kChunk) * 4 + 2 * static_cast<size_t>(terms) * kChunk * PITCH * 2 +
-           (half ? static_cast<size_t>(kChunk) * RP * 4 : 0);
+           (half ? kThreadsPerCta * 4 : 0);
   }
 };
 
@@ -891,7 +891,7 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgr
   float* steps = reinterpret_cast<float*>(toks + 4 * kChunk);      // [2][COLS / 64][kChunk] (8 bits)
   uint16_t* terms =  // [2][TERMS][kChunk][PITCH]
       reinterpret_cast<uint16_t*>(steps + (Q8 ? 2 * (S::COLS / 64) * kChunk : 0));
-  float* raw = reinterpret_cast<float*>(terms + 2 * TERMS * kChunk * S::PITCH);  // [kChunk][RP] (fp16)
+  uint32_t* largest = reinterpret_cast<uint32_t*>(terms + 2 * TERMS * kChunk * S::PITCH);  // by thread (fp16)
 
   const uint32_t crank = cluster_rank(), csize = cluster_size();
   const int adapter = blockIdx.y;
@@ -1019,24 +1019,25 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgr
         if (e / kChunk < S::COLS / 64) steps[(n & 1) * (S::COLS / 64) * kChunk + e] = my_step[i];
       }
     }
+    float dn = 1.f;
+    if constexpr (HALF) {
+      // All values of a thread are of one rank row, which kThreadsPerCta / RP threads share.
+      static_assert(kThreadsPerCta % RP == 0, "a thread's values are of one rank row");
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < S::PER_THREAD; ++i) m = max(m, __float_as_uint(mine[i]) & 0x7fffffffu);
+      largest[threadIdx.x] = m;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kThreadsPerCta / RP; ++j) m = max(m, largest[j * RP + threadIdx.x % RP]);
+      float up;
+      power_scale(__uint_as_float(m), &dn, &up);
+      if (threadIdx.x < RP) scales[(n & 1) * RP + threadIdx.x] = up;
+    }
 #pragma unroll
     for (int i = 0; i < S::PER_THREAD; ++i) {
       const int e = i * kThreadsPerCta + threadIdx.x;
-      if constexpr (HALF) raw[e] = mine[i];
-      else split(mine[i], n, e / RP, e % RP);
-    }
-    if constexpr (HALF) {
-      __syncthreads();
-      for (int r = warp; r < RP; r += kWarps) {
-        const float v0 = raw[lane * RP + r], v1 = raw[(lane + 32) * RP + r];
-        const uint32_t m = __reduce_max_sync(
-            0xffffffffu, max(__float_as_uint(v0) & 0x7fffffffu, __float_as_uint(v1) & 0x7fffffffu));
-        float dn, up;
-        power_scale(__uint_as_float(m), &dn, &up);
-        if (lane == 0) scales[(n & 1) * RP + r] = up;
-        split(v0 * dn, n, lane, r);
-        split(v1 * dn, n, lane + 32, r);
-      }
+      split(HALF ? mine[i] * dn : mine[i], n, e / RP, e % RP);
     }
   };
   if (chunks > 0) {
