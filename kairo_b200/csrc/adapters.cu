@@ -364,6 +364,7 @@ kairo_status run_grads(const Grad* p, int count, int64_t rank, kairo_dtype dtype
   }
   a.order = pl.order;
   a.starts = pl.starts;
+  a.tokens = ntokens;
   a.rank = static_cast<int32_t>(rank);
   a.count = count;
   a.widest = static_cast<int32_t>(widest);

@@ -81,6 +81,7 @@ struct LowRankWgradArgs {
   } one[2];
   const int32_t* order;
   const int32_t* starts;
+  int64_t tokens;
   int32_t rank;
   int32_t count;
   int32_t widest;        // largest k
@@ -204,6 +205,16 @@ template <typename T>
 __device__ __forceinline__ uint16_t bits16(float v) {
   const T h = from_f32<T>(v);
   return *reinterpret_cast<const uint16_t*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t bits16x2(float v0, float v1) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 h = __floats2half2_rn(v0, v1);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v0, v1);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
 }
 template <typename T>
 __device__ __forceinline__ float value16(uint16_t b) {
@@ -866,7 +877,7 @@ struct WgradShape {
   static constexpr size_t bytes(int terms, bool half, bool q8) {
     return SHARED_BYTES + (q8 ? static_cast<size_t>(2 * kChunk * (COLS / 64)) * 4 : 0) +
            static_cast<size_t>(2 * RP + 4 * kChunk) * 4 + 2 * static_cast<size_t>(terms) * kChunk * PITCH * 2 +
-           (half ? kThreadsPerCta * 4 : 0);
+           (half ? kThreadsPerCta * 8 : 0);
   }
 };
 
@@ -878,12 +889,19 @@ struct WgradShape {
 // formed by the matrix units (4 steps per term) and added to the running sum in
 // fp32 with rounding, so that a long batch loses nothing to the units'
 // truncation.  The cluster's partial sums are added in rank order.
-template <typename T, typename TG, typename S, int TERMS, bool Q8, bool VEC, int MINB>
+//
+// DIRECT: bf16 results of batches up to kDirectTokens are added up by the units
+// themselves.  They lose 2^-23 of the sum at most per step and term, 2^-11 over
+// such a batch: a quarter of the result's own rounding at worst (8192 tokens,
+// 8192 features, rank 32 80 -> 73 us; 4096 tokens, rank 64 92 -> 83, 128 220 -> 188).
+constexpr int64_t kDirectTokens = 32768;
+template <typename T, typename TG, typename S, int TERMS, bool Q8, bool VEC, bool DIRECT, int MINB>
 __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgradArgs args) {
   const LowRankWgradArgs::One& a = args.one[blockIdx.z];
   const int rank = args.rank;
   constexpr int MR = S::MR, RP = S::RP;
   constexpr bool HALF = std::is_same_v<T, __half>;
+  static_assert(!DIRECT || (!HALF && sizeof(TG) == 2), "bf16 results only");
   extern __shared__ __align__(16) uint8_t smem[];
   float* part = reinterpret_cast<float*>(smem);                    // [RP][COLS]: this CTA's sum, after the ring's use
   float* scales = reinterpret_cast<float*>(smem + S::SHARED_BYTES);  // [2][RP]: power of two of every rank row (fp16)
@@ -891,7 +909,7 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgr
   float* steps = reinterpret_cast<float*>(toks + 4 * kChunk);      // [2][COLS / 64][kChunk] (8 bits)
   uint16_t* terms =  // [2][TERMS][kChunk][PITCH]
       reinterpret_cast<uint16_t*>(steps + (Q8 ? 2 * (S::COLS / 64) * kChunk : 0));
-  uint32_t* largest = reinterpret_cast<uint32_t*>(terms + 2 * TERMS * kChunk * S::PITCH);  // by thread (fp16)
+  uint2* largest = reinterpret_cast<uint2*>(terms + 2 * TERMS * kChunk * S::PITCH);  // by thread (fp16)
 
   const uint32_t crank = cluster_rank(), csize = cluster_size();
   const int adapter = blockIdx.y;
@@ -996,19 +1014,14 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgr
                          : 0.f;
       }
     }
+    // pairs of neighbours in a rank row's order, for words of two terms
+    const int r = 2 * static_cast<int>(threadIdx.x % (RP / 2));
 #pragma unroll
-    for (int i = 0; i < S::PER_THREAD; ++i) {
-      const int e = i * kThreadsPerCta + threadIdx.x;
-      const int tok = toks[(n & 3) * kChunk + e / RP], r = e % RP;
-      mine[i] = (tok >= 0 && r < rank) ? __ldg(a.s + static_cast<int64_t>(tok) * rank + r) : 0.f;
-    }
-  };
-  auto split = [&](float v, int n, int row, int r) {
-#pragma unroll
-    for (int q = 0; q < TERMS; ++q) {
-      const uint16_t b = bits16<T>(v);
-      terms[(((n & 1) * TERMS + q) * kChunk + row) * S::PITCH + r] = b;
-      v -= value16<T>(b);
+    for (int i = 0; i < S::PER_THREAD; i += 2) {
+      const int tok = toks[(n & 3) * kChunk + (i / 2 * kThreadsPerCta + threadIdx.x) / (RP / 2)];
+      const float* s = a.s + static_cast<int64_t>(max(tok, 0)) * rank + r;
+      mine[i] = (tok >= 0 && r < rank) ? __ldg(s) : 0.f;
+      mine[i + 1] = (tok >= 0 && r + 1 < rank) ? __ldg(s + 1) : 0.f;
     }
   };
   auto store_s = [&](int n) {
@@ -1019,25 +1032,43 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgr
         if (e / kChunk < S::COLS / 64) steps[(n & 1) * (S::COLS / 64) * kChunk + e] = my_step[i];
       }
     }
-    float dn = 1.f;
+    float dn0 = 1.f, dn1 = 1.f;
     if constexpr (HALF) {
-      // All values of a thread are of one rank row, which kThreadsPerCta / RP threads share.
-      static_assert(kThreadsPerCta % RP == 0, "a thread's values are of one rank row");
-      uint32_t m = 0;
+      // All pairs of a thread are of the same two rank rows, which it shares with
+      // kThreadsPerCta / (RP / 2) - 1 others.
+      static_assert(kThreadsPerCta % (RP / 2) == 0, "a thread's pairs are of two rank rows");
+      uint2 m = make_uint2(0u, 0u);
 #pragma unroll
-      for (int i = 0; i < S::PER_THREAD; ++i) m = max(m, __float_as_uint(mine[i]) & 0x7fffffffu);
+      for (int i = 0; i < S::PER_THREAD; i += 2) {
+        m.x = max(m.x, __float_as_uint(mine[i]) & 0x7fffffffu);
+        m.y = max(m.y, __float_as_uint(mine[i + 1]) & 0x7fffffffu);
+      }
       largest[threadIdx.x] = m;
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < kThreadsPerCta / RP; ++j) m = max(m, largest[j * RP + threadIdx.x % RP]);
-      float up;
-      power_scale(__uint_as_float(m), &dn, &up);
-      if (threadIdx.x < RP) scales[(n & 1) * RP + threadIdx.x] = up;
+      for (int j = 0; j < kThreadsPerCta / (RP / 2); ++j) {
+        const uint2 o = largest[j * (RP / 2) + threadIdx.x % (RP / 2)];
+        m.x = max(m.x, o.x);
+        m.y = max(m.y, o.y);
+      }
+      float up0, up1;
+      power_scale(__uint_as_float(m.x), &dn0, &up0);
+      power_scale(__uint_as_float(m.y), &dn1, &up1);
+      if (threadIdx.x < RP / 2)
+        *reinterpret_cast<float2*>(scales + (n & 1) * RP + 2 * threadIdx.x) = make_float2(up0, up1);
     }
 #pragma unroll
-    for (int i = 0; i < S::PER_THREAD; ++i) {
-      const int e = i * kThreadsPerCta + threadIdx.x;
-      split(HALF ? mine[i] * dn : mine[i], n, e / RP, e % RP);
+    for (int i = 0; i < S::PER_THREAD; i += 2) {
+      float v0 = mine[i] * dn0, v1 = mine[i + 1] * dn1;
+      uint16_t* to = terms + ((n & 1) * TERMS * kChunk + (i / 2 * kThreadsPerCta + threadIdx.x) / (RP / 2)) * S::PITCH +
+                     2 * (threadIdx.x % (RP / 2));
+#pragma unroll
+      for (int q = 0; q < TERMS; ++q) {
+        const uint32_t b = bits16x2<T>(v0, v1);
+        *reinterpret_cast<uint32_t*>(to + q * kChunk * S::PITCH) = b;
+        v0 -= value16<T>(static_cast<uint16_t>(b));
+        v1 -= value16<T>(static_cast<uint16_t>(b >> 16));
+      }
     }
   };
   if (chunks > 0) {
@@ -1060,63 +1091,70 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgr
   for (int n = 0; n < chunks; ++n) {
     const int later = threadIdx.x < kChunk ? chunk_token(n + 3) : -1;
     if (n + 1 < chunks) load_s(n + 1);
-    float acc[MR][8][4];
-#pragma unroll
-    for (int m = 0; m < MR; ++m)
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
-    const int here = min(4, units - 4 * n);
+    auto multiply = [&](float (&acc)[MR][8][4]) {
+      const int here = min(4, units - 4 * n);
 #pragma unroll 1
-    for (int ks = 0; ks < here; ++ks) {
-      wait_all_but<S::UNITS - 1>();
-      if constexpr (!VEC) __syncwarp();
-      const uint32_t src = ring + static_cast<uint32_t>(at * 4 * 512);
-      uint4 v[4];
+      for (int ks = 0; ks < here; ++ks) {
+        wait_all_but<S::UNITS - 1>();
+        if constexpr (!VEC) __syncwarp();
+        const uint32_t src = ring + static_cast<uint32_t>(at * 4 * 512);
+        uint4 v[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (!Q8) {
-          v[i] = landed(src + i * 512);
-        } else {
-          const int row = ks * 16 + 2 * t + (i & 1) + (i >> 1) * 8;
-          v[i] = read_back<T>(landed_codes(src + i * 512),
-                              steps[((n & 1) * (S::COLS / 64) + (lc >> 6)) * kChunk + row]);
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (!Q8) {
+            v[i] = landed(src + i * 512);
+          } else {
+            const int row = ks * 16 + 2 * t + (i & 1) + (i >> 1) * 8;
+            v[i] = read_back<T>(landed_codes(src + i * 512),
+                                steps[((n & 1) * (S::COLS / 64) + (lc >> 6)) * kChunk + row]);
+          }
         }
-      }
-      uint32_t b0[8], b1[8];
+        uint32_t b0[8], b1[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        b0[j] = pair_of(v[0], v[1], j);
-        b1[j] = pair_of(v[2], v[3], j);
+        for (int j = 0; j < 8; ++j) {
+          b0[j] = pair_of(v[0], v[1], j);
+          b1[j] = pair_of(v[2], v[3], j);
+        }
+        if constexpr (!VEC) __syncwarp();
+        issue(4 * n + ks + S::UNITS, at);
+        at = at + 1 == S::UNITS ? 0 : at + 1;
+#pragma unroll
+        for (int m = 0; m < MR; ++m)
+#pragma unroll
+          for (int q = TERMS - 1; q >= 0; --q) {
+            uint32_t f[4];
+            ldmatrix4_trans(f, terms_addr + static_cast<uint32_t>((((n & 1) * TERMS + q) * kChunk + ks * 16) * S::PITCH +
+                                                                  m * 16) * 2u);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) mma<T>(acc[m][j], f, b0[j], b1[j]);
+          }
       }
-      if constexpr (!VEC) __syncwarp();
-      issue(4 * n + ks + S::UNITS, at);
-      at = at + 1 == S::UNITS ? 0 : at + 1;
+    };
+    if constexpr (DIRECT) {
+      multiply(sum);
+    } else {
+      float acc[MR][8][4];
 #pragma unroll
       for (int m = 0; m < MR; ++m)
 #pragma unroll
-        for (int q = TERMS - 1; q >= 0; --q) {
-          uint32_t f[4];
-          ldmatrix4_trans(f, terms_addr + static_cast<uint32_t>((((n & 1) * TERMS + q) * kChunk + ks * 16) * S::PITCH +
-                                                                m * 16) * 2u);
+        for (int j = 0; j < 8; ++j)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) mma<T>(acc[m][j], f, b0[j], b1[j]);
+          for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
+      multiply(acc);
+#pragma unroll
+      for (int m = 0; m < MR; ++m) {
+        float pa = 1.f, pb = 1.f;
+        if constexpr (HALF) {
+          pa = scales[(n & 1) * RP + (rg * MR + m) * 16 + g];
+          pb = scales[(n & 1) * RP + (rg * MR + m) * 16 + g + 8];
         }
-    }
 #pragma unroll
-    for (int m = 0; m < MR; ++m) {
-      float pa = 1.f, pb = 1.f;
-      if constexpr (HALF) {
-        pa = scales[(n & 1) * RP + (rg * MR + m) * 16 + g];
-        pb = scales[(n & 1) * RP + (rg * MR + m) * 16 + g + 8];
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        sum[m][j][0] += acc[m][j][0] * pa;
-        sum[m][j][1] += acc[m][j][1] * pa;
-        sum[m][j][2] += acc[m][j][2] * pb;
-        sum[m][j][3] += acc[m][j][3] * pb;
+        for (int j = 0; j < 8; ++j) {
+          sum[m][j][0] += acc[m][j][0] * pa;
+          sum[m][j][1] += acc[m][j][1] * pa;
+          sum[m][j][2] += acc[m][j][2] * pb;
+          sum[m][j][3] += acc[m][j][3] * pb;
+        }
       }
     }
     if (n + 1 < chunks) store_s(n + 1);  // the other half of terms: read by no warp since the last barrier
@@ -1159,13 +1197,13 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgr
   cluster_sync();  // the others may still read this CTA's sums
 }
 
-template <typename T, typename TG, typename S, bool Q8, bool VEC>
+template <typename T, typename TG, typename S, bool Q8, bool VEC, bool DIRECT>
 cudaError_t launch_wgrad(const LowRankWgradArgs& a, int64_t adapters, int cluster, cudaStream_t s) {
   constexpr int TERMS = std::is_same_v<TG, float> ? 3 : 2;
   constexpr size_t bytes = S::bytes(TERMS, std::is_same_v<T, __half>, Q8);
   static_assert(bytes <= 227 * 1024, "shared memory of one CTA");
   constexpr int MINB = S::MR == 1 && bytes <= 113 * 1024 ? 2 : 1;  // MR 2 needs the registers of both
-  auto* fn = &k_wgrad<T, TG, S, TERMS, Q8, VEC, MINB>;
+  auto* fn = &k_wgrad<T, TG, S, TERMS, Q8, VEC, DIRECT, MINB>;
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(fn, bytes, &done);
   if (e != cudaSuccess) return e;
@@ -1185,12 +1223,20 @@ cudaError_t launch_wgrad(const LowRankWgradArgs& a, int64_t adapters, int cluste
   return cudaLaunchKernelEx(&cfg, fn, a);
 }
 
+template <typename T, typename TG, bool Q8, bool VEC, bool DIRECT>
+cudaError_t pick_shape(const LowRankWgradArgs& a, int64_t adapters, int cluster, cudaStream_t s) {
+  if (a.rank <= 16) return launch_wgrad<T, TG, WgradShape<1, 1, 5>, Q8, VEC, DIRECT>(a, adapters, cluster, s);
+  if (a.rank <= 32) return launch_wgrad<T, TG, WgradShape<1, 2, 8>, Q8, VEC, DIRECT>(a, adapters, cluster, s);
+  if (a.rank <= 64) return launch_wgrad<T, TG, WgradShape<2, 2, 8>, Q8, VEC, DIRECT>(a, adapters, cluster, s);
+  return launch_wgrad<T, TG, WgradShape<4, 2, 4>, Q8, VEC, DIRECT>(a, adapters, cluster, s);
+}
+
 template <typename T, typename TG, bool Q8, bool VEC>
 cudaError_t pick_wgrad(const LowRankWgradArgs& a, int64_t adapters, int cluster, cudaStream_t s) {
-  if (a.rank <= 16) return launch_wgrad<T, TG, WgradShape<1, 1, 5>, Q8, VEC>(a, adapters, cluster, s);
-  if (a.rank <= 32) return launch_wgrad<T, TG, WgradShape<1, 2, 8>, Q8, VEC>(a, adapters, cluster, s);
-  if (a.rank <= 64) return launch_wgrad<T, TG, WgradShape<2, 2, 8>, Q8, VEC>(a, adapters, cluster, s);
-  return launch_wgrad<T, TG, WgradShape<4, 2, 4>, Q8, VEC>(a, adapters, cluster, s);
+  if constexpr (std::is_same_v<T, __nv_bfloat16> && sizeof(TG) == 2) {
+    if (a.tokens <= kDirectTokens) return pick_shape<T, TG, Q8, VEC, true>(a, adapters, cluster, s);
+  }
+  return pick_shape<T, TG, Q8, VEC, false>(a, adapters, cluster, s);
 }
 
 }  // namespace lowrank

@@ -516,3 +516,24 @@ def test_gradients_at_any_address(dt, gdt):
         for buf, want in ((both[0], dd), (both[1], du), (one, dd)):
             assert torch.equal(buf[off : off + want.numel()].view_as(want), want)
             assert bool((buf[:off] == 7).all()) and bool((buf[off + want.numel():] == 7).all())
+
+
+@pytest.mark.parametrize("t", [32768, 32769])
+@pytest.mark.parametrize("r", [16, 40])
+def test_gradients_of_long_batches(t, r):
+    """Sums of one sign, where truncation adds up, on both sides of the length up to which the units add up all tokens."""
+    k, n = 72, 64
+    gen = torch.Generator().manual_seed(r)
+    x = (torch.rand(t, k, generator=gen) + 0.5).bfloat16().to(DEV)
+    dy = (torch.rand(t, n, generator=gen) + 0.5).bfloat16().to(DEV)
+    low = (torch.rand(t, r, generator=gen) + 0.5).to(DEV)
+    a = LowRankAdapters(down=torch.zeros(1, r, k, dtype=torch.bfloat16, device=DEV),
+                        up=torch.ones(1, r, n, dtype=torch.bfloat16, device=DEV))
+    plan = adapter_plan(torch.zeros(t, dtype=torch.int32, device=DEV), 1)
+    _, dd, du = adapter_linear_backward(dy, x, a, plan, low=low)
+    dlow = dy.double().sum(1, keepdim=True).expand(t, r)
+    # per 16 tokens and term at most one truncation inside the units and one of the sum
+    lost = 2 * (t / 16) * 2 * 2.0**-23 if t <= 32768 else (t / 64 + 32) * 2.0**-23
+    for got, ref, own in ((dd[0], dlow.t() @ x.double(), (n + 2) * 2.0**-23), (du[0], low.double().t() @ dy.double(), 0.0)):
+        slack = ref * (lost + own + 2.0**-17)
+        assert bool(((got.double() - ref).abs() <= _round_tol(ref, slack, torch.bfloat16)).all())
