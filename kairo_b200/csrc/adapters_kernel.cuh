@@ -257,8 +257,11 @@ __device__ __forceinline__ uint32_t codes_by_rows(int c, int t) {
 // Operands at any address of their type (VEC false): the same slots, filled by
 // the whole warp value by value, a row at a time, so that an access meets one
 // line of one row (with every lane loading its own 8 values one by one it met
-// eight).  What a lane reads was then written by others: a warp barrier stands
-// between filling and reading, and between reading and the next filling.
+// eight; 4431 tokens, 1776 -> 8734, rank 16: 249 -> 160 us.  Asynchronous copies of
+// aligned words, shifted when they are read, took 121 there, but 70 instead of 54
+// for 2349 tokens at rank 32 and 10.4 instead of 8.7 for one token).  What a lane
+// reads was then written by others: a warp barrier stands between filling and
+// reading, and between reading and the next filling.
 // CONST: nothing writes the operand during the launch (base may be y).
 template <typename T, bool CONST = true>
 __device__ __forceinline__ uint32_t value_at(const T* row, int c, int n) {
@@ -410,29 +413,33 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApp
               fetch<T>(dst + (NT + 2 * m + h) * 512, xrow[m][h] + off, tok[m][h] >= 0 ? left : 0);
         } else {
           static_assert(MT == 1, "two vectors of tokens");
+          constexpr int UW = 4;  // vectors under way: two took 9.1 us for one token, 661 -> 114, four 8.7
           const int c = kk - 8 * t + lane;
           const T* w0 = static_cast<const T*>(a.down) + static_cast<int64_t>(tile.adapter) * a.rank * a.k;
           const uint32_t dst = ring0 + static_cast<uint32_t>(at * S::STEP * 512 + lane * 2);
 #pragma unroll
-          for (int v0 = 0; v0 < S::STEP; v0 += 2) {  // two vectors under way
-            uint32_t v[2][8];
+          for (int v0 = 0; v0 < S::STEP; v0 += UW) {
+            uint32_t v[UW][8];
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < UW; ++u)
 #pragma unroll
               for (int r = 0; r < 8; ++r) {
-                if (v0 < NT) {
+                if (v0 + u >= S::STEP) {
+                  v[u][r] = 0u;
+                } else if (v0 + u < NT) {
                   const int rr = (v0 + u) * 8 + r;
                   v[u][r] = rr < a.rank ? value_at<T>(w0 + static_cast<int64_t>(rr) * a.k, c, a.k) : 0u;
                 } else {
-                  const int tk = __shfl_sync(0xffffffffu, tok[0][u], 4 * r);
+                  const int tk = __shfl_sync(0xffffffffu, tok[0][v0 + u - NT], 4 * r);
                   v[u][r] = tk >= 0 ? value_at<T>(static_cast<const T*>(a.x) + static_cast<int64_t>(tk) * a.ldx, c, a.k)
                                     : 0u;
                 }
               }
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < UW; ++u)
 #pragma unroll
-              for (int r = 0; r < 8; ++r) put16(dst + (v0 + u) * 512 + r * 64, v[u][r]);
+              for (int r = 0; r < 8; ++r)
+                if (v0 + u < S::STEP) put16(dst + (v0 + u) * 512 + r * 64, v[u][r]);
           }
         }
         kk += (i & 1) ? stride - 32 : 32;
@@ -486,26 +493,22 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApp
     } else if (live) {
       // value `lane` and `lane` + 32 of row 2 q + .. of each vector
       const uint32_t dst = ring0 + static_cast<uint32_t>(kt * 4 * 512 + 2 * (lane & 7));
+      uint32_t v[4][4][2];
 #pragma unroll
-      for (int i0 = 0; i0 < 4; i0 += 2) {
-        uint32_t v[2][4][2];
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int q = 0; q < 4; ++q)
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
+          for (int s = 0; s < 2; ++s) {
+            const int r = kt * 16 + 2 * q + (i & 1) + (i >> 1) * 8;
+            v[i][q][s] = r < a.rank ? value_at<T>(up + static_cast<int64_t>(r) * a.n, n0 + lane + 32 * s, a.n) : 0u;
+          }
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-              const int r = kt * 16 + 2 * q + u + (i0 >> 1) * 8;
-              v[u][q][s] = r < a.rank ? value_at<T>(up + static_cast<int64_t>(r) * a.n, n0 + lane + 32 * s, a.n) : 0u;
-            }
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int q = 0; q < 4; ++q)
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-              put16(dst + (i0 + u) * 512 + by_rows((lane >> 3) + 4 * s, q), v[u][q][s]);
-      }
+          for (int s = 0; s < 2; ++s) put16(dst + i * 512 + by_rows((lane >> 3) + 4 * s, q), v[i][q][s]);
     }
     commit();
   };

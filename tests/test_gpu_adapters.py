@@ -537,3 +537,25 @@ def test_gradients_of_long_batches(t, r):
     for got, ref, own in ((dd[0], dlow.t() @ x.double(), (n + 2) * 2.0**-23), (du[0], low.double().t() @ dy.double(), 0.0)):
         slack = ref * (lost + own + 2.0**-17)
         assert bool(((got.double() - ref).abs() <= _round_tol(ref, slack, torch.bfloat16)).all())
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("case", [
+    (3, 1, 1, 1, 1), (70, 2, 3, 2, 2), (64, 64, 65, 16, 1), (130, 1471, 334, 12, 4), (50, 333, 1025, 33, 2),
+    (20, 131, 99, 128, 2), (300, 97, 129, 64, 3),
+])
+def test_odd_features(dt, case):
+    """Rows that begin at any address; calls on NaN before each leave nothing behind that reaches a result."""
+    t, k, n, r, g = case
+    x, dy, a, ids = _problem(dt, t, k, n, r, g, seed=t + k)
+    nan = LowRankAdapters(down=torch.full_like(a.down, float("nan")), up=torch.full_like(a.up, float("nan")))
+    gen = torch.Generator().manual_seed(k)
+    for base_t, out_t in ((None, None), (dt, torch.float32), (torch.float32, None)):
+        base = base_dx = None
+        if base_t is not None:
+            wide = torch.randn(t, n + k + 3, generator=gen).to(base_t).to(DEV)
+            base, base_dx = wide[:, 1 : n + 1], wide[:, n + 2 : n + 2 + k]
+        plan = adapter_plan(torch.zeros(t, dtype=torch.int64, device=DEV), g)
+        y = adapter_linear(torch.full_like(x, float("nan")), nan, plan)
+        adapter_linear_backward(y, torch.full_like(x, float("nan")), nan, plan)
+        _check(x, dy, a, ids, base, base_dx, out_dtype=out_t, grad_dtype=out_t)
