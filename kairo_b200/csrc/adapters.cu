@@ -66,6 +66,7 @@ __global__ void __launch_bounds__(1024) k_plan_tiles(const uint32_t* __restrict_
                                                      Plan pl) {
   __shared__ int sums[32];
   __shared__ int carry;
+  __shared__ int begins[1024 + 1];  // of the adapters of one turn
   const int which = blockIdx.x;
   const int size = tile_tokens(which);
   int32_t* first = which == 0 ? pl.first[0] : (which == 1 ? pl.first[1] : pl.first[2]);
@@ -85,8 +86,11 @@ __global__ void __launch_bounds__(1024) k_plan_tiles(const uint32_t* __restrict_
   for (int64_t base = 0; base <= g; base += 1024) {
     const int64_t a = base + threadIdx.x;  // g: tokens without an adapter
     int v = 0;
+    begins[threadIdx.x] = a <= g ? start_of(a) : static_cast<int>(t);
+    if (threadIdx.x == 1023) begins[1024] = a < g ? start_of(a + 1) : static_cast<int>(t);
+    __syncthreads();
     if (a <= g) {
-      const int p0 = start_of(a), p1 = a < g ? start_of(a + 1) : static_cast<int>(t);
+      const int p0 = begins[threadIdx.x], p1 = begins[threadIdx.x + 1];
       v = (p1 - p0 + size - 1) / size;
       if (which == 0) {
         pl.starts[a] = p0;
@@ -130,7 +134,10 @@ __global__ void __launch_bounds__(1024) k_plan_tiles(const uint32_t* __restrict_
       if (first[mid + 1] <= i) lo = mid + 1;
       else hi = mid;
     }
-    const int p0 = start_of(lo), p1 = lo < g ? start_of(lo + 1) : static_cast<int>(t);
+    // the last turn's are still there
+    const int64_t turn = g / 1024 * 1024;
+    const int p0 = lo >= turn ? begins[lo - turn] : start_of(lo);
+    const int p1 = lo >= turn ? begins[lo - turn + 1] : start_of(lo + 1);
     LowRankTile tile;
     tile.adapter = lo < g ? static_cast<int32_t>(lo) : -1;
     tile.begin = p0 + (i - first[lo]) * size;

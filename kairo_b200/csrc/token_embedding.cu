@@ -470,7 +470,8 @@ size_t sort_ws_bytes(int64_t n) {
 template <typename ID>
 kairo_status sort_launch(const ID* ids, int64_t n, int64_t n_rows, uint32_t* sorted, int32_t* perm, void* ws,
                          const ZeroRows& zero, cudaStream_t s) {
-  if (n <= kRankTokens) {
+  // half as many where the cluster needs one pass only (ids below 512): 4096 tokens 5.9 us, counted 6.7
+  if (n <= (key_bits(n_rows) <= kMaxDigit ? kRankTokens / 2 : kRankTokens)) {
     k_sort_ranks<ID><<<static_cast<unsigned>(ceil_div64(n, 32)), 1024, 0, s>>>(ids, static_cast<int>(n), n_rows, sorted,
                                                                               perm);
     const cudaError_t e = cudaGetLastError();
