@@ -115,7 +115,7 @@ def sparse_linear_weight_grad(dY: Tensor, X: Tensor | QuantizedActivations, W: B
         raise TypeError("dY, X and W must share a dtype")
     if out_dtype not in (torch.float32, W.dtype):
         raise TypeError("dW dtype must be float32 or the weight dtype")
-    if dY.stride(1) != 1:
+    if dY.stride(1) != 1 or (dY.shape[0] > 1 and dY.stride(0) < m):  # a broadcast gradient has rows of pitch 0
         dY = dY.contiguous()
     if kept is None and X.stride(1) != 1:
         X = X.contiguous()

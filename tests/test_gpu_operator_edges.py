@@ -1,0 +1,58 @@
+"""Corners of the operators around the linear layer on the device.
+
+Plain implementations are in 64 bits.  Tolerances count half steps of the
+output's type (torch.finfo(t).eps / 2 of the value) and, for a sum of n products in
+fp32, n * 2^-23 of the sum of magnitudes.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from kairo_b200.ops import (
+    BlockSparseLinear,
+    bsr_from_tiles,
+    dequantize_activations,
+    quantize_activations,
+    sparse_linear_weight_grad,
+)
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _half(t):
+    return torch.finfo(t).eps / 2
+
+
+def _weight(dt, m, k, bs=64, seed=0):
+    """A weight with every second block of a checkerboard, its block-rows and block-columns."""
+    nbr, nbc = -(-m // bs), -(-k // bs)
+    pos = torch.tensor([p for p in range(nbr * nbc) if (p // nbc + p % nbc) % 2 == 0])
+    tiles = (torch.randn(pos.numel(), bs, bs, generator=torch.Generator().manual_seed(seed)) * 0.1).to(dt)
+    rows, cols = pos // nbc, pos % nbc
+    return bsr_from_tiles(tiles.to(DEV), rows.int().to(DEV), cols.int().to(DEV), (m, k)), rows.to(DEV), cols.to(DEV)
+
+
+def _blocks(dense, rows, cols, bs=64):
+    m, k = dense.shape
+    pad = torch.nn.functional.pad(dense, (0, -k % bs, 0, -m % bs))
+    return pad.view(-(-m // bs), bs, -(-k // bs), bs).permute(0, 2, 1, 3)[rows, cols]
+
+
+@pytest.mark.parametrize("bs", [64, 32])
+def test_weight_grad_of_a_broadcast_gradient(bs):
+    """dY whose rows share or overlap memory is read as the values that it stands for."""
+    w, rows, cols = _weight(torch.bfloat16, 128, 192, bs)
+    x = torch.randn(300, 192, device=DEV).bfloat16()
+    q = quantize_activations(x)
+    back = dequantize_activations(q).double()
+    one = torch.randn(128, device=DEV).bfloat16()
+    long = torch.randn(300 * 8 + 128, device=DEV).bfloat16()
+    for dy in (one.expand(300, 128), long.as_strided((300, 128), (8, 1))):
+        got = sparse_linear_weight_grad(dy, q, w)
+        ref = _blocks(dy.double().t() @ back, rows, cols, bs)
+        mag = _blocks(dy.double().abs().t() @ back.abs(), rows, cols, bs)
+        assert bool(((got.double() - ref).abs() <= mag * 300 * 2.0**-23 + ref.abs() * 2.0**-24).all())
+        assert torch.equal(got, sparse_linear_weight_grad(dy.contiguous(), q, w))

@@ -1,0 +1,76 @@
+"""Corners of the operators around the linear layer that need no device: what a
+call hands to the library, and what modules keep, with the library faked
+where a call would launch."""
+
+from __future__ import annotations
+
+import contextlib
+import ctypes
+
+import pytest
+import torch
+
+from kairo_b200 import _lib
+from kairo_b200.ops import QuantizedActivations, backward
+from kairo_b200.types import BlockSparseMatrix
+
+
+def _bsr(dtype=torch.float32, m=64, k=64):
+    nbr, nbc = -(-m // 64), -(-k // 64)
+    return BlockSparseMatrix(row_ptr=torch.arange(nbr + 1, dtype=torch.int32) * nbc,
+                             col_idx=torch.arange(nbc, dtype=torch.int32).repeat(nbr),
+                             blocks=torch.zeros(nbr * nbc, 64, 64, dtype=dtype), shape=(m, k), block_size=(64, 64))
+
+
+class _FakeLib:
+    """Records the arguments of every call; each succeeds and does nothing."""
+
+    def __init__(self):
+        self.calls = {}
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls[name] = args
+            return _lib.SUCCESS
+
+        return call
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    lib = _FakeLib()
+    monkeypatch.setattr(_lib, "lib", lambda: lib)
+    monkeypatch.setattr(_lib, "stream_handle", lambda dev: 0)
+    monkeypatch.setattr(torch.cuda, "device", lambda dev: contextlib.nullcontext())
+    monkeypatch.setattr(backward, "_require_cuda", lambda *t, op: None)
+    return lib
+
+
+@pytest.mark.parametrize("dy", [
+    torch.ones(64).expand(300, 64),            # a broadcast gradient: every row the same memory
+    torch.ones(300 * 8 + 64).as_strided((300, 64), (8, 1)),  # rows that overlap
+    torch.ones(300, 80)[:, :64],
+    torch.ones(64, 300).t(),
+    torch.ones(1, 64),
+])
+def test_weight_grad_reads_inside_dy(fake, dy):
+    """The rows that the library is told to read lie inside the gradient's memory."""
+    n = dy.shape[0]
+    seen = {}
+    contiguous = torch.Tensor.contiguous
+
+    def note(t):
+        out = contiguous(t)
+        seen[out.data_ptr()] = out
+        return out
+
+    with pytest.MonkeyPatch.context() as mp:
+        mp.setattr(torch.Tensor, "contiguous", note)
+        q = QuantizedActivations(codes=torch.zeros(n, 64, dtype=torch.int8), steps=torch.zeros(1, n),
+                                 dtype=torch.float32)
+        wt = backward.TransposedBsr(matrix=_bsr(), perm=torch.zeros(1, dtype=torch.int32))
+        backward.sparse_linear_weight_grad(dy, q, _bsr(), wt)
+    ptr, lddy = fake.calls["kairo_bsr_sddmm_q8"][4:6]
+    used = seen.get(ptr, dy)
+    room = used.untyped_storage().nbytes() // 4 - used.storage_offset()
+    assert ptr == used.data_ptr() and lddy >= 64 and (n - 1) * lddy + 64 <= room
