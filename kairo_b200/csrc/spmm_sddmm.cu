@@ -145,20 +145,25 @@ struct SddArgs {
   const float* steps;
   int64_t ldq, lds;
   int32_t k;
+  int32_t segment;           // slabs of one tensor-core sum (SEGMENTS)
 };
 
 constexpr int kSddConvert = 4;  // warps that read X back from 8 bits
 
-// Slabs whose sum the tensor cores form before an fp32 result takes it over
+// Slabs whose sum the tensor cores form before a running sum takes it over
 // (X in 8 bits only; the other path keeps one sum).  They truncate at each
-// step, always towards zero: over 2048 rows that came to 2.5e-6 of the result
-// (2-norm), and it grows with the batch.  Sums of 12 slabs, added up with
-// rounding by the epilogue warps in the other half of TMEM, stay at 0.9e-6; a
-// 16-bit result keeps one sum, since its own rounding is hundreds of times as
-// large.  (Adding them up in dW itself took 2.78 ms instead of 1.78 for the
-// 8192 x 32768 layer: a thread's row is 256 bytes, so its loads and stores touch
-// 32 lines each.)
-constexpr int kSddSegment = 12;
+// step of 16 rows, always towards zero: for values of one sign that came to
+// 1e-7 of the result a step at worst, 4.7e-5 after 8192 rows and 6.7e-3 after
+// 2^20.  Sums of one segment are added up with rounding by the epilogue warps
+// in the other half of TMEM.  fp32 results take over every 12 slabs (2048 rows
+// with signs 2.5e-6 -> 0.9e-6 of the result, 2-norm).  16-bit results keep one
+// sum, and both accumulator sets for it, up to 128 slabs, where it is off by a
+// tenth of fp16's half step; longer batches take over every 128.  (Adding
+// the segments up in dW itself took 2.78 ms instead of 1.78 for the 8192 x
+// 32768 layer: a thread's row is 256 bytes, so its loads and stores touch 32
+// lines each.)
+constexpr int kSddSegmentF32 = 12;
+constexpr int kSddSegment16 = 128;
 
 template <typename TOut>
 __device__ __forceinline__ void store_row16(TOut* dst, const float* v);
@@ -193,7 +198,7 @@ __device__ __forceinline__ void store_row16<__nv_bfloat16>(__nv_bfloat16* dst, c
 }
 
 // tcgen05 kernel for bm = bk = 64 (S = 2 blocks per stack, U stacks per item).
-template <int IN_FMT, typename TOut, bool Q8>
+template <int IN_FMT, typename TOut, bool Q8, bool SEGMENTS>
 __global__ void __launch_bounds__(kThreads + (Q8 ? 32 * kSddConvert : 0), 1)
     bsr_sddmm_tc_kernel(const __grid_constant__ CUtensorMap tmap_dy, const __grid_constant__ CUtensorMap tmap_x,
                         const SddArgs args) {
@@ -253,8 +258,8 @@ __global__ void __launch_bounds__(kThreads + (Q8 ? 32 * kSddConvert : 0), 1)
   const int nitems = *args.nitems;
   const int G = gridDim.x;
   const int nslabs = static_cast<int>((args.n + KB - 1) / KB);
-  constexpr bool SEGMENTS = Q8 && std::is_same<TOut, float>::value;
-  const int seg = SEGMENTS ? kSddSegment : nslabs;  // slabs per accumulator set
+  static_assert(Q8 || !SEGMENTS, "segments with X in 8 bits only");
+  const int seg = SEGMENTS ? args.segment : nslabs;  // slabs per accumulator set
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -607,21 +612,26 @@ kairo_status launch_simt(const kairo_bsr* a, const int32_t* col_idx_t, const int
 
 using SddFn = void (*)(CUtensorMap, CUtensorMap, SddArgs);
 
+// `segments`: a 16-bit result whose batch is longer than one sum (fp32 ones always have them).
 template <bool Q8>
-SddFn pick_sdd(kairo_dtype in, kairo_dtype out) {
+SddFn pick_sdd(kairo_dtype in, kairo_dtype out, bool segments) {
   if (in == KAIRO_DTYPE_F16) {
-    if (out == KAIRO_DTYPE_F32) return reinterpret_cast<SddFn>(&bsr_sddmm_tc_kernel<0, float, Q8>);
-    if (out == KAIRO_DTYPE_F16) return reinterpret_cast<SddFn>(&bsr_sddmm_tc_kernel<0, __half, Q8>);
+    if (out == KAIRO_DTYPE_F32) return reinterpret_cast<SddFn>(&bsr_sddmm_tc_kernel<0, float, Q8, Q8>);
+    if (out == KAIRO_DTYPE_F16)
+      return Q8 && segments ? reinterpret_cast<SddFn>(&bsr_sddmm_tc_kernel<0, __half, Q8, Q8>)
+                            : reinterpret_cast<SddFn>(&bsr_sddmm_tc_kernel<0, __half, Q8, false>);
   } else if (in == KAIRO_DTYPE_BF16) {
-    if (out == KAIRO_DTYPE_F32) return reinterpret_cast<SddFn>(&bsr_sddmm_tc_kernel<1, float, Q8>);
-    if (out == KAIRO_DTYPE_BF16) return reinterpret_cast<SddFn>(&bsr_sddmm_tc_kernel<1, __nv_bfloat16, Q8>);
+    if (out == KAIRO_DTYPE_F32) return reinterpret_cast<SddFn>(&bsr_sddmm_tc_kernel<1, float, Q8, Q8>);
+    if (out == KAIRO_DTYPE_BF16)
+      return Q8 && segments ? reinterpret_cast<SddFn>(&bsr_sddmm_tc_kernel<1, __nv_bfloat16, Q8, Q8>)
+                            : reinterpret_cast<SddFn>(&bsr_sddmm_tc_kernel<1, __nv_bfloat16, Q8, false>);
   }
   return nullptr;
 }
 
 bool sdd_tc_ok(const kairo_bsr* a, const void* dy, int64_t lddy, const SddX& x, kairo_dtype out) {
   if (a->bm != 64 || a->bk != 64) return false;
-  if (!pick_sdd<false>(a->dtype, out)) return false;
+  if (!pick_sdd<false>(a->dtype, out, false)) return false;
   if ((lddy % 8) || (reinterpret_cast<uintptr_t>(dy) & 15u)) return false;
   if (x.codes) return true;  // their rows are 16-byte aligned
   return x.ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x.x) & 15u) == 0;
@@ -734,7 +744,9 @@ kairo_status run_sddmm(const kairo_bsr* a, const int32_t* row_ptr_t, const int32
   args.ldq = x.ldq;
   args.lds = x.lds;
   args.k = static_cast<int32_t>(a->cols);
-  SddFn fn = x.codes ? pick_sdd<true>(a->dtype, out_dtype) : pick_sdd<false>(a->dtype, out_dtype);
+  args.segment = out_dtype == KAIRO_DTYPE_F32 ? kSddSegmentF32 : kSddSegment16;
+  const bool segments = n > static_cast<int64_t>(args.segment) * kSddKB;
+  SddFn fn = x.codes ? pick_sdd<true>(a->dtype, out_dtype, segments) : pick_sdd<false>(a->dtype, out_dtype, false);
   const size_t smem = static_cast<size_t>(stages) * stage_bytes + 2048;
   e = cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(smem));

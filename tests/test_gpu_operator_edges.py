@@ -56,3 +56,25 @@ def test_weight_grad_of_a_broadcast_gradient(bs):
         mag = _blocks(dy.double().abs().t() @ back.abs(), rows, cols, bs)
         assert bool(((got.double() - ref).abs() <= mag * 300 * 2.0**-23 + ref.abs() * 2.0**-24).all())
         assert torch.equal(got, sparse_linear_weight_grad(dy.contiguous(), q, w))
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n", [8192, 8193, (1 << 20) + 77])
+def test_weight_grad_of_a_long_batch(dt, n):
+    """Values of one sign, where the matrix units' truncation adds up: a 16-bit result stays at its own rounding."""
+    w = bsr_from_tiles(torch.zeros(1, 64, 64, dtype=dt, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV),
+                       torch.zeros(1, dtype=torch.int32, device=DEV), (64, 64))
+    torch.manual_seed(n)
+    x = (torch.rand(n, 64, device=DEV) * 0.01 + 0.005).to(dt)
+    dy = (torch.rand(n, 64, device=DEV) * 0.01 + 0.005).to(dt)
+    q = quantize_activations(x)
+    ref = dy.double().t() @ dequantize_activations(q).double()
+    # a sum of 8192 rows: 512 steps, each with a truncation inside the units and one of the sum; the sums of
+    # up to 129 such segments are added in fp32
+    lost = 512 * 2 * 2.0**-23 + 129 * 2.0**-24
+    got = sparse_linear_weight_grad(dy, q, w, out_dtype=dt)[0]
+    assert bool(((got.double() - ref).abs() <= ref * (lost + _half(dt) * (1 + lost))).all())
+    # fp32 results: 48 steps a segment, up to 1367 segments
+    lost = 48 * 2 * 2.0**-23 + 1367 * 2.0**-24
+    got = sparse_linear_weight_grad(dy, q, w, out_dtype=torch.float32)[0]
+    assert bool(((got.double() - ref).abs() <= ref * lost).all())
