@@ -172,9 +172,10 @@ bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 // 13.0 with 64, 2048 tokens 12.8 and 14.0, 4096 tokens 22.8 and 22.4; rank 32,
 // 2048 tokens 17.3 and 17.6 (with 32), and 8192 tokens of 8192 features 117
 // and 96; rank 64, 1024 tokens 19.0 and 24.2, 4096 tokens 48.5 and 39.6; rank 128,
-// 4096 tokens 94.8 and 75.5 (with 32).
-int pick_tile(int64_t t, int64_t rank, bool vec, bool base_f32) {
-  if (!vec || t <= 2048) return 16;
+// 4096 tokens 94.8 and 75.5 (with 32).  Contractions that are summed in parts
+// have tiles of 16 only.
+int pick_tile(int64_t t, int64_t k, int64_t rank, bool vec, bool base_f32) {
+  if (!vec || t <= 2048 || k > lowrank::kLongFeatures) return 16;
   if (rank <= 16) return 64;
   if (rank <= 32) return 32;
   if (rank <= 64) return base_f32 ? 32 : 64;
@@ -283,7 +284,7 @@ extern "C" kairo_status kairo_low_rank_apply(const void* x, int64_t ldx, int64_t
   const int64_t eb = base_dtype == KAIRO_DTYPE_F32 ? 4 : 2, ey = y_dtype == KAIRO_DTYPE_F32 ? 4 : 2;
   const bool vec = k % 8 == 0 && n % 8 == 0 && ldx * e % 16 == 0 && aligned16(x) && aligned16(down) && aligned16(up) &&
                    (!base || (ldb * eb % 16 == 0 && aligned16(base))) && (!y || (ldy * ey % 16 == 0 && aligned16(y)));
-  const int tile = pick_tile(ntokens, rank, vec, base && base_dtype == KAIRO_DTYPE_F32);
+  const int tile = pick_tile(ntokens, k, rank, vec, base && base_dtype == KAIRO_DTYPE_F32);
   const int which = tile == 16 ? 0 : (tile == 32 ? 1 : 2);
   LowRankApplyArgs a{};
   a.x = x;

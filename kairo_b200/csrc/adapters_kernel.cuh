@@ -101,6 +101,16 @@ namespace lowrank {
 constexpr int kWarps = 8;
 constexpr int kThreadsPerCta = kWarps * 32;
 constexpr int kChunk = 64;  // tokens per staged chunk of the weight gradient
+// Features up to which the matrix units add up a contraction by themselves, in
+// up to kContractSteps steps of 32 features a warp.  They truncate, always
+// towards zero: up to 1e-7 of the sum in each of the two products of a step, and
+// 1.1e-5 after 131072 features of one sign.  Longer contractions (LONG) are cut
+// into parts of that many steps, added with rounding; 2^22 features came to
+// 3.9e-4 in one sum.  (In one kernel for both, the registers that this takes
+// made the short ones spill.)
+constexpr int kContractSteps = 64;
+constexpr int kLongFeatures = kContractSteps * 32 * kWarps * 8;  // clusters of 8 from 131072 features on
+static_assert(kContractSteps % 2 == 0, "two steps to a turn of 64 features");
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -339,7 +349,7 @@ struct ApplyShape {
 // base) are started before the tile is summed, so that the barriers cost no
 // memory time; afterwards each load of the next turn starts as soon as its slot
 // has been read.
-template <typename T, typename TY, typename S, int TERMS, bool BASE_F32, bool VEC, int MINB>
+template <typename T, typename TY, typename S, int TERMS, bool BASE_F32, bool VEC, bool LONG, int MINB>
 __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApplyArgs a) {
   constexpr int MT = S::MT, NT = S::NT, KT = S::KT;
   constexpr int RING = S::ring(BASE_F32);
@@ -375,6 +385,33 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApp
     }
 
   float acc[MT][NT][4];
+  // Sum over the CTA's warps, into the first, as a tree: the upper half hands over to the lower.
+  auto sum_warps = [&]() {
+#pragma unroll
+    for (int half = kWarps / 2; half >= 1; half /= 2) {
+      if (warp >= half && warp < 2 * half) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              red[(warp - half) * S::LOW + ((m * NT + j) * 4 + i) * 32 + lane] = acc[m][j][i];
+      }
+      __syncthreads();
+      if (warp < half) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[m][j][i] += red[warp * S::LOW + ((m * NT + j) * 4 + i) * 32 + lane];
+      }
+      __syncthreads();
+    }
+  };
+  int parts = 1;  // of the contraction (LONG)
+  auto steps_from = [&](int first) { return first < a.k ? 2 * ((a.k - first + stride - 1) / stride) : 0; };
   if (live) {
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -382,9 +419,10 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApp
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
-    // Steps of 32 features, two to a turn of 64.
-    const int turns = slot * 64 < a.k ? (a.k - slot * 64 + stride - 1) / stride : 0;
-    const int steps = 2 * turns;
+    // Steps of 32 features, two to a turn of 64; `rest`: with those of later parts.
+    int rest = steps_from(slot * 64);
+    int steps = LONG ? min(rest, kContractSteps) : rest;
+    const int most = steps_from(static_cast<int>(crank) * kWarps * 64);  // of the CTA's first warp: the same for all
     int kk = slot * 64 + 8 * t;  // this lane's features of the next step to start
     const T* wrow = static_cast<const T*>(a.down) + (static_cast<int64_t>(tile.adapter) * a.rank + g) * a.k;
     const int64_t wstep = static_cast<int64_t>(8) * a.k;
@@ -446,29 +484,50 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApp
       }
       commit();
     };
+    for (;;) {
 #pragma unroll
-    for (int i = 0; i < S::STAGES; ++i) issue(i, i);
-    int at = 0;
-    for (int i = 0; i < steps; ++i) {
-      wait_all_but<S::STAGES - 1>();
-      if constexpr (!VEC) __syncwarp();
-      const uint32_t src = ring + static_cast<uint32_t>(at * S::STEP * 512);
-      uint4 wb[NT];
+      for (int i = 0; i < S::STAGES; ++i) issue(i, i);
+      int at = 0;
+      for (int i = 0; i < steps; ++i) {
+        wait_all_but<S::STAGES - 1>();
+        if constexpr (!VEC) __syncwarp();
+        const uint32_t src = ring + static_cast<uint32_t>(at * S::STEP * 512);
+        uint4 wb[NT];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) wb[j] = landed(src + j * 512);
+        for (int j = 0; j < NT; ++j) wb[j] = landed(src + j * 512);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const uint4 x0 = landed(src + (NT + 2 * m) * 512), x1 = landed(src + (NT + 2 * m + 1) * 512);
-        const uint32_t a0[4] = {x0.x, x1.x, x0.y, x1.y};
-        const uint32_t a1[4] = {x0.z, x1.z, x0.w, x1.w};
+        for (int m = 0; m < MT; ++m) {
+          const uint4 x0 = landed(src + (NT + 2 * m) * 512), x1 = landed(src + (NT + 2 * m + 1) * 512);
+          const uint32_t a0[4] = {x0.x, x1.x, x0.y, x1.y};
+          const uint32_t a1[4] = {x0.z, x1.z, x0.w, x1.w};
 #pragma unroll
-        for (int j = 0; j < NT; ++j) mma<T>(acc[m][j], a0, wb[j].x, wb[j].y);
+          for (int j = 0; j < NT; ++j) mma<T>(acc[m][j], a0, wb[j].x, wb[j].y);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) mma<T>(acc[m][j], a1, wb[j].z, wb[j].w);
+          for (int j = 0; j < NT; ++j) mma<T>(acc[m][j], a1, wb[j].z, wb[j].w);
+        }
+        if constexpr (!VEC) __syncwarp();
+        issue(i + S::STAGES, at);  // every vector of the slot is in use above
+        at = at + 1 == S::STAGES ? 0 : at + 1;
       }
-      if constexpr (!VEC) __syncwarp();
-      issue(i + S::STAGES, at);  // every vector of the slot is in use above
-      at = at + 1 == S::STAGES ? 0 : at + 1;
+      if (!LONG || parts * kContractSteps >= most) break;
+      // The whole CTA's sum so far is kept where the finished tile will stand:
+      // no peer writes there before the cluster's barrier.
+      wait_all_but<0>();
+      __syncthreads();
+      sum_warps();
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float* kept = low + ((m * NT + j) * 4 + i) * 32 + lane;
+            if (warp == 0) *kept = parts > 1 ? *kept + acc[m][j][i] : acc[m][j][i];
+            acc[m][j][i] = 0.f;
+          }
+      ++parts;
+      rest -= kContractSteps;
+      steps = min(rest, kContractSteps);
     }
   }
 
@@ -588,35 +647,17 @@ __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_apply(const LowRankApp
       wait_all_but<0>();  // of the empty groups: every copy has been used
       __syncthreads();
     }
-    // Sum over the CTA's warps as a tree: the upper half hands over to the lower.
-#pragma unroll
-    for (int half = kWarps / 2; half >= 1; half /= 2) {
-      if (warp >= half && warp < 2 * half) {
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              red[(warp - half) * S::LOW + ((m * NT + j) * 4 + i) * 32 + lane] = acc[m][j][i];
-      }
-      __syncthreads();
-      if (warp < half) {
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[m][j][i] += red[warp * S::LOW + ((m * NT + j) * 4 + i) * 32 + lane];
-      }
-      __syncthreads();
-    }
+    sum_warps();
     if (S::ALIAS) start_turn();  // the ring is free again
     if (warp == 0) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
+          if (LONG && parts > 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[m][j][i] += low[((m * NT + j) * 4 + i) * 32 + lane];
+          }
           float* to = part + (m * 16 + g) * S::RP + j * 8 + 2 * t;
           *reinterpret_cast<float2*>(to) = make_float2(acc[m][j][0], acc[m][j][1]);
           *reinterpret_cast<float2*>(to + 8 * S::RP) = make_float2(acc[m][j][2], acc[m][j][3]);
@@ -801,13 +842,13 @@ cudaError_t allow_smem(F* fn, size_t bytes, std::atomic<uint64_t>* done) {
   return e;
 }
 
-template <typename T, typename TY, typename S, bool BASE_F32, bool VEC>
+template <typename T, typename TY, typename S, bool BASE_F32, bool VEC, bool LONG = false>
 cudaError_t launch_apply_as(const LowRankApplyArgs& a, int64_t clusters, int cluster, cudaStream_t s) {
   constexpr int TERMS = std::is_same_v<TY, float> ? 3 : 2;
   constexpr size_t bytes = S::bytes(TERMS, BASE_F32, sizeof(TY), VEC);
   static_assert(bytes <= 227 * 1024, "shared memory of one CTA");
   constexpr int MINB = bytes <= 113 * 1024 ? 2 : 1;
-  auto* fn = &k_apply<T, TY, S, TERMS, BASE_F32, VEC, MINB>;
+  auto* fn = &k_apply<T, TY, S, TERMS, BASE_F32, VEC, LONG, MINB>;
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(fn, bytes, &done);
   if (e != cudaSuccess) return e;
@@ -828,6 +869,11 @@ cudaError_t launch_apply_as(const LowRankApplyArgs& a, int64_t clusters, int clu
 
 template <typename T, typename TY, typename S, bool VEC>
 cudaError_t launch_apply(const LowRankApplyArgs& a, int64_t clusters, int cluster, cudaStream_t s) {
+  if constexpr (S::MT == 1) {  // the shapes of 16 tokens
+    if (a.k > kLongFeatures)
+      return a.base_f32 ? launch_apply_as<T, TY, S, true, VEC, true>(a, clusters, cluster, s)
+                        : launch_apply_as<T, TY, S, false, VEC, true>(a, clusters, cluster, s);
+  }
   return a.base_f32 ? launch_apply_as<T, TY, S, true, VEC>(a, clusters, cluster, s)
                     : launch_apply_as<T, TY, S, false, VEC>(a, clusters, cluster, s);
 }

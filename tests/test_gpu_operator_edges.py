@@ -12,6 +12,9 @@ import torch
 
 from kairo_b200.ops import (
     BlockSparseLinear,
+    LowRankAdapters,
+    adapter_linear,
+    adapter_plan,
     bsr_from_tiles,
     dequantize_activations,
     quantize_activations,
@@ -78,3 +81,23 @@ def test_weight_grad_of_a_long_batch(dt, n):
     lost = 48 * 2 * 2.0**-23 + 1367 * 2.0**-24
     got = sparse_linear_weight_grad(dy, q, w, out_dtype=torch.float32)[0]
     assert bool(((got.double() - ref).abs() <= ref * lost).all())
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("k", [131072, 131073, (1 << 20) + 8, (1 << 20) + 3])
+@pytest.mark.parametrize("rank,t", [(4, 3), (20, 18), (40, 1), (100, 2)])
+def test_long_contractions(dt, k, rank, t):
+    """fp32 results of features of one sign, on both sides of the length up to which the units keep one sum."""
+    gen = torch.Generator(device=DEV).manual_seed(k + rank)
+    x = (torch.rand(t, k, generator=gen, device=DEV) + 0.5).to(dt)
+    down = ((torch.rand(2, rank, k, generator=gen, device=DEV) + 0.5) * 2**-8).to(dt)
+    up = torch.ones(2, rank, 72, dtype=dt, device=DEV)
+    ids = torch.arange(t, device=DEV) % 3 - 1  # the last of every three: adapter 1
+    plan = adapter_plan(ids, 2)
+    y, low = adapter_linear(x, LowRankAdapters(down=down, up=up), plan, out_dtype=torch.float32, return_low=True)
+    ref = torch.einsum("tk,trk->tr", x.double(), down.double()[ids.clamp(min=0)]) * (ids >= 0)[:, None]
+    # 128 products in a part, each with a truncation inside the units and one of the sum; up to 8 parts, 8 warps and 8 CTAs
+    lost = 128 * 2 * 2.0**-23 + 24 * 2.0**-24
+    assert bool(((low.double() - ref).abs() <= ref * lost).all())
+    want = ref.sum(1, keepdim=True).expand(t, 72)
+    assert bool(((y.double() - want).abs() <= want * (lost + (rank + 4) * 2.0**-23)).all())
