@@ -225,15 +225,15 @@ def _wgrad(op: str, index: int, low: Tensor, Z: Tensor | QuantizedActivations, p
     return grad
 
 
-def adapter_linear_backward(dY: Tensor, X: Tensor | QuantizedActivations, adapters: LowRankAdapters,
+def adapter_linear_backward(dY: Tensor, X: Tensor | QuantizedActivations | None, adapters: LowRankAdapters,
                             plan: AdapterPlan, *, low: Tensor | None = None, base_dx: Tensor | None = None,
                             need_dx: bool = True, need_dw: bool = True, dx_dtype: torch.dtype | None = None,
                             grad_dtype: torch.dtype | None = None
                             ) -> tuple[Tensor | None, Tensor | None, Tensor | None]:
     """(dX, d_down, d_up) of ``adapter_linear``; the gradient by its base is dY.
 
-    X may be given in 8 bits.  ``low``: what ``return_low`` gave (computed
-    anew from X otherwise).  ``base_dx``: the shared projection's part of
+    X may be given in 8 bits; with ``need_dw=False`` it is not read and may be
+    None.  ``low``: what ``return_low`` gave (computed anew from X otherwise).  ``base_dx``: the shared projection's part of
     dX, added in fp32 before the one rounding to ``dx_dtype`` (default: the
     adapters').  d_down and d_up are in ``grad_dtype`` (default: the
     adapters'), zero for an adapter without tokens."""
@@ -242,7 +242,10 @@ def adapter_linear_backward(dY: Tensor, X: Tensor | QuantizedActivations, adapte
     down, up, code = adapters.down, adapters.up, adapters._code
     tokens = plan.num_tokens
     kept = X if isinstance(X, QuantizedActivations) else None
-    index = _lib.device_index(op, dY, kept.codes if kept else X, down, plan.memory)
+    if need_dw and X is None:
+        raise ValueError(f"{op}: the gradients of down and up need X")
+    # X takes no part in dX
+    index = _lib.device_index(op, dY, down, plan.memory, *((kept.codes if kept else X,) if need_dw else ()))
     _check_batch(op, "dY", dY, n, adapters, plan)
     gdt = grad_dtype or down.dtype
     if gdt != torch.float32 and gdt != down.dtype:

@@ -11,9 +11,11 @@ import pytest
 import torch
 
 from kairo_b200.ops import (
+    AdaptedSparseLinear,
     BlockSparseLinear,
     LowRankAdapters,
     adapter_linear,
+    adapter_linear_backward,
     adapter_plan,
     bsr_from_tiles,
     dequantize_activations,
@@ -101,3 +103,42 @@ def test_long_contractions(dt, k, rank, t):
     assert bool(((low.double() - ref).abs() <= ref * lost).all())
     want = ref.sum(1, keepdim=True).expand(t, 72)
     assert bool(((y.double() - want).abs() <= want * (lost + (rank + 4) * 2.0**-23)).all())
+
+
+def _adapted(m=256, k=320, checkpoint=None, seed=1, dt=torch.bfloat16):
+    w, rows, cols = _weight(dt, m, k, seed=seed)
+    torch.manual_seed(seed)
+    layer = AdaptedSparseLinear(BlockSparseLinear(w, checkpoint=checkpoint), 3, 8, scale=torch.tensor([1.0, 0.5, 2.0]))
+    with torch.no_grad():
+        layer.up.normal_(std=0.3)
+    x = torch.randn(70, k, device=DEV).to(dt)
+    dy = (torch.randn(70, m, device=DEV) * 0.1).to(dt)
+    plan = adapter_plan(torch.arange(70, device=DEV) % 4 - 1, 3)
+    return layer, x, dy, plan
+
+
+def _gradients(layer, x, dy, plan):
+    """(dX, d_blocks, d_down, d_up) of one step; None where nothing asks for one."""
+    for p in layer.parameters():
+        p.grad = None
+    xi = x.clone().requires_grad_()
+    layer(xi, plan).backward(dy)
+    return xi.grad, layer.layer.blocks.grad, layer.down.grad, layer.up.grad
+
+
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_frozen_parameters_of_an_adapted_layer(checkpoint):
+    """Every subset of the parameters frozen, all of them too: what is left has the gradients of the whole."""
+    layer, x, dy, plan = _adapted(checkpoint=checkpoint)
+    params = [layer.layer.blocks, layer.down, layer.up]
+    whole = _gradients(layer, x, dy, plan)
+    for keep in range(8):
+        for i, p in enumerate(params):
+            p.requires_grad_(bool(keep >> i & 1))
+        got = _gradients(layer, x, dy, plan)
+        assert torch.equal(got[0], whole[0])
+        for i in range(3):
+            assert torch.equal(got[1 + i], whole[1 + i]) if keep >> i & 1 else got[1 + i] is None
+    a = layer.adapters()
+    dx, dd, du = adapter_linear_backward(dy, None, a, plan, need_dw=False)
+    assert torch.equal(dx, adapter_linear_backward(dy, x, a, plan)[0]) and dd is None and du is None

@@ -11,7 +11,7 @@ import pytest
 import torch
 
 from kairo_b200 import _lib
-from kairo_b200.ops import QuantizedActivations, backward
+from kairo_b200.ops import AdapterPlan, LowRankAdapters, QuantizedActivations, adapter_linear_backward, backward
 from kairo_b200.types import BlockSparseMatrix
 
 
@@ -74,3 +74,18 @@ def test_weight_grad_reads_inside_dy(fake, dy):
     used = seen.get(ptr, dy)
     room = used.untyped_storage().nbytes() // 4 - used.storage_offset()
     assert ptr == used.data_ptr() and lddy >= 64 and (n - 1) * lddy + 64 <= room
+
+
+def test_backward_without_x(monkeypatch):
+    """dX alone takes no X; the other gradients say that they need one."""
+    down, up = torch.zeros(2, 4, 64, dtype=torch.bfloat16), torch.zeros(2, 4, 32, dtype=torch.bfloat16)
+    a = LowRankAdapters(down=down, up=up)
+    plan = AdapterPlan(memory=torch.zeros(256, dtype=torch.uint8), num_tokens=3, num_adapters=2)
+    dy = torch.zeros(3, 32, dtype=torch.bfloat16)
+    seen = []
+    monkeypatch.setattr(_lib, "device_index", lambda op, *t: seen.append([x.get_device() for x in t]) or -1)
+    monkeypatch.setattr(_lib, "launch", lambda *args: None)
+    dx, dd, du = adapter_linear_backward(dy, None, a, plan, need_dw=False)
+    assert dx.shape == (3, 64) and dd is None and du is None and len(seen) == 1
+    with pytest.raises(ValueError, match="need X"):
+        adapter_linear_backward(dy, None, a, plan)
