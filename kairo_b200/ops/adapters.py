@@ -302,7 +302,8 @@ class _AdaptedLinearFn(torch.autograd.Function):
                 plan: AdapterPlan) -> Tensor:
         layer = module.layer
         W = layer.weight_matrix(blocks)
-        Y, low = adapted_sparse_linear(X, W, module.adapters(down, up), plan, return_low=True)
+        scale = module.scale
+        Y, low = adapted_sparse_linear(X, W, module.adapters(down, up, scale), plan, return_low=True)
         need_x = any(ctx.needs_input_grad[1:4])
         kept: list[Tensor] = []
         ctx.kept_dtype = None
@@ -311,14 +312,14 @@ class _AdaptedLinearFn(torch.autograd.Function):
             kept, ctx.kept_dtype = [q.codes, q.steps], q.dtype
         elif need_x:
             kept = [X]
-        ctx.save_for_backward(blocks, down, up, low, *kept)
+        ctx.save_for_backward(blocks, down, up, scale, low, *kept)
         ctx.module, ctx.plan, ctx.need_x = module, plan, need_x
         return Y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dY: Tensor):
-        blocks, down, up, low, *kept = ctx.saved_tensors
+        blocks, down, up, scale, low, *kept = ctx.saved_tensors
         module: AdaptedSparseLinear = ctx.module
         layer = module.layer
         X = None
@@ -333,7 +334,7 @@ class _AdaptedLinearFn(torch.autograd.Function):
         base_dx = sparse_linear(dY, wt.matrix, out_dtype=torch.float32) if need_dx else None
         dX = d_down = d_up = None
         if need_dx or need_dw:
-            dX, d_down, d_up = adapter_linear_backward(dY, X, module.adapters(down, up), ctx.plan, low=low,
+            dX, d_down, d_up = adapter_linear_backward(dY, X, module.adapters(down, up, scale), ctx.plan, low=low,
                                                        base_dx=base_dx, need_dx=need_dx, need_dw=need_dw)
         d_blocks = sparse_linear_weight_grad(dY, X, W, wt, out_dtype=blocks.dtype) if need_blocks else None
         return dX, d_blocks, d_down, d_up, None, None
@@ -347,7 +348,11 @@ class AdaptedSparseLinear(torch.nn.Module):
     The layer's blocks train too unless frozen
     (``layer.blocks.requires_grad_(False)``).  A layer built with
     ``checkpoint="int8"`` keeps its input in 8 bits for all three
-    gradients."""
+    gradients.
+
+    A step's backward pass uses the ``scale`` of its forward pass.  Like the
+    parameters it must not be written in between (autograd raises); to switch
+    the adapters off for a pass, assign another tensor to ``scale``."""
 
     def __init__(self, layer: BlockSparseLinear, num_adapters: int, rank: int, *,
                  scale: float | Tensor = 1.0) -> None:
@@ -365,9 +370,11 @@ class AdaptedSparseLinear(torch.nn.Module):
         s = torch.as_tensor(scale, dtype=torch.float32, device=dev)
         self.register_buffer("scale", s.expand(num_adapters).clone())
 
-    def adapters(self, down: Tensor | None = None, up: Tensor | None = None) -> LowRankAdapters:
+    def adapters(self, down: Tensor | None = None, up: Tensor | None = None,
+                 scale: Tensor | None = None) -> LowRankAdapters:
         return LowRankAdapters(down=(self.down if down is None else down).detach(),
-                               up=(self.up if up is None else up).detach(), scale=self.scale)
+                               up=(self.up if up is None else up).detach(),
+                               scale=self.scale if scale is None else scale)
 
     def forward(self, X: Tensor, plan: AdapterPlan) -> Tensor:
         return _AdaptedLinearFn.apply(X, self.layer.blocks, self.down, self.up, self, plan)

@@ -142,3 +142,24 @@ def test_frozen_parameters_of_an_adapted_layer(checkpoint):
     a = layer.adapters()
     dx, dd, du = adapter_linear_backward(dy, None, a, plan, need_dw=False)
     assert torch.equal(dx, adapter_linear_backward(dy, x, a, plan)[0]) and dd is None and du is None
+
+
+def test_scale_of_the_forward_pass():
+    """The gradients are those of the scale that the forward pass used, or autograd says that it was written."""
+    layer, x, dy, plan = _adapted()
+    ref = _gradients(layer, x, dy, plan)
+    for p in layer.parameters():
+        p.grad = None
+    xi = x.clone().requires_grad_()
+    y = layer(xi, plan)
+    used = layer.scale
+    layer.scale = torch.zeros_like(used)  # a reference pass without the adapters
+    assert torch.equal(layer(x, plan), layer.layer(x))
+    y.backward(dy)
+    layer.scale = used
+    got = xi.grad, layer.layer.blocks.grad, layer.down.grad, layer.up.grad
+    assert all(torch.equal(a, b) for a, b in zip(got, ref))
+    y = layer(xi, plan)
+    layer.scale.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(dy)

@@ -5,7 +5,6 @@ where a call would launch."""
 from __future__ import annotations
 
 import contextlib
-import ctypes
 
 import pytest
 import torch
