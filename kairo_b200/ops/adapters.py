@@ -370,6 +370,14 @@ class AdaptedSparseLinear(torch.nn.Module):
         s = torch.as_tensor(scale, dtype=torch.float32, device=dev)
         self.register_buffer("scale", s.expand(num_adapters).clone())
 
+    def _apply(self, fn, recurse: bool = True) -> "AdaptedSparseLinear":
+        # .to(dtype), .half() and the like cast every floating buffer; scale stays in fp32
+        kept = self.scale
+        super()._apply(fn, recurse)
+        if self.scale.dtype != torch.float32:
+            self.scale = kept.to(self.scale.device)
+        return self
+
     def adapters(self, down: Tensor | None = None, up: Tensor | None = None,
                  scale: Tensor | None = None) -> LowRankAdapters:
         return LowRankAdapters(down=(self.down if down is None else down).detach(),

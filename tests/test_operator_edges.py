@@ -10,7 +10,15 @@ import pytest
 import torch
 
 from kairo_b200 import _lib
-from kairo_b200.ops import AdapterPlan, LowRankAdapters, QuantizedActivations, adapter_linear_backward, backward
+from kairo_b200.ops import (
+    AdaptedSparseLinear,
+    AdapterPlan,
+    BlockSparseLinear,
+    LowRankAdapters,
+    QuantizedActivations,
+    adapter_linear_backward,
+    backward,
+)
 from kairo_b200.types import BlockSparseMatrix
 
 
@@ -88,3 +96,16 @@ def test_backward_without_x(monkeypatch):
     assert dx.shape == (3, 64) and dd is None and du is None and len(seen) == 1
     with pytest.raises(ValueError, match="need X"):
         adapter_linear_backward(dy, None, a, plan)
+
+
+def test_scale_stays_in_fp32():
+    """Casting a model leaves the adapters' scale in the type and with the values that the kernels take."""
+    scale = torch.tensor([1.0, 1 / 3, 1e-30])
+    for cast in (lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.bfloat16(),
+                 lambda m: torch.nn.Sequential(m).to(torch.float16)[0], lambda m: m.double().bfloat16(), lambda m: m.to("cpu")):
+        layer = AdaptedSparseLinear(BlockSparseLinear(_bsr(torch.bfloat16)), 3, 4, scale=scale)
+        layer = cast(layer)
+        assert layer.scale.dtype == torch.float32 and torch.equal(layer.scale, scale)
+        assert "scale" in dict(layer.named_buffers()) and layer.adapters().count == 3
+    layer = AdaptedSparseLinear(BlockSparseLinear(_bsr(torch.bfloat16)), 3, 4).to("meta")
+    assert layer.scale.device.type == "meta"
