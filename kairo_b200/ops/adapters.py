@@ -309,7 +309,7 @@ class _AdaptedLinearFn(torch.autograd.Function):
         ctx.kept_dtype = None
         if need_x and layer.checkpoint is not None:
             q = quantize_activations(X)
-            kept, ctx.kept_dtype = [q.codes, q.steps], q.dtype
+            kept, ctx.kept_dtype = list(q._parts()), q.dtype
         elif need_x:
             kept = [X]
         ctx.save_for_backward(blocks, down, up, scale, low, *kept)
@@ -324,8 +324,8 @@ class _AdaptedLinearFn(torch.autograd.Function):
         layer = module.layer
         X = None
         if ctx.need_x:
-            X = kept[0] if ctx.kept_dtype is None else QuantizedActivations(codes=kept[0], steps=kept[1],
-                                                                             dtype=ctx.kept_dtype)
+            X = kept[0] if ctx.kept_dtype is None else QuantizedActivations._from_parts(*kept, layer.shape[1],
+                                                                                         ctx.kept_dtype)
         W = layer.weight_matrix(blocks)
         dY = dY.contiguous()
         need_dx, need_blocks = ctx.needs_input_grad[0], ctx.needs_input_grad[1]

@@ -181,7 +181,7 @@ class _SparseLinearFn(torch.autograd.Function):
             ctx.save_for_backward(X, blocks)
         elif ctx.needs_input_grad[1]:
             q = quantize_activations(X)
-            ctx.save_for_backward(q.codes, q.steps, blocks)
+            ctx.save_for_backward(*q._parts(), blocks)
             ctx.kept_dtype = q.dtype
         else:
             ctx.save_for_backward(None, blocks)
@@ -191,9 +191,9 @@ class _SparseLinearFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dY: Tensor):
         *kept, blocks = ctx.saved_tensors
-        X = kept[0] if ctx.kept_dtype is None else QuantizedActivations(codes=kept[0], steps=kept[1],
-                                                                         dtype=ctx.kept_dtype)
         module: BlockSparseLinear = ctx.module
+        X = kept[0] if ctx.kept_dtype is None else QuantizedActivations._from_parts(*kept, module.shape[1],
+                                                                                     ctx.kept_dtype)
         W = module.weight_matrix(blocks)
         wt = transpose_values(W, module.transposed())
         dY = dY.contiguous()

@@ -62,6 +62,19 @@ class QuantizedActivations:
         q.__dict__.update(codes=codes, steps=steps, dtype=dtype)
         return q
 
+    def _parts(self) -> tuple[Tensor, Tensor]:
+        """Codes with the padding of their rows, and steps, for
+        ``save_for_backward``: a copy of them (offloading hooks make some) keeps
+        the padding, which a copy of ``codes`` does not."""
+        n, k = self.codes.shape
+        rows = self.codes if k % 16 == 0 else self.codes.as_strided((n, -(-k // 16) * 16), (self._ldq, 1))
+        return rows, self.steps
+
+    @classmethod
+    def _from_parts(cls, rows: Tensor, steps: Tensor, k: int, dtype: torch.dtype) -> "QuantizedActivations":
+        """The activation of k columns whose ``_parts()`` these are, or copies of them."""
+        return cls(codes=rows[:, :k], steps=steps, dtype=dtype)
+
     @property
     def shape(self) -> tuple[int, int]:
         return tuple(self.codes.shape)

@@ -163,3 +163,27 @@ def test_scale_of_the_forward_pass():
     layer.scale.zero_()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward(dy)
+
+
+@pytest.mark.parametrize("k", [320, 200, 72])
+@pytest.mark.parametrize("pin", [False, True])
+@pytest.mark.parametrize("tokens", [70, 1])
+def test_checkpoint_under_offloading_hooks(k, pin, tokens):
+    """What is kept survives a copy to the host and back, at widths that are no multiple of 16, too."""
+    layer, x, dy, _ = _adapted(k=k, checkpoint="int8")
+    x, dy = x[:tokens], dy[:tokens]
+    plan = adapter_plan(torch.arange(tokens, device=DEV) % 4, 3)
+    inner = layer.layer
+
+    def plain():
+        inner.blocks.grad = None
+        inner(x).backward(dy)
+        return inner.blocks.grad
+
+    ref, ref_plain = _gradients(layer, x, dy, plan), plain()
+    with torch.autograd.graph.save_on_cpu(pin_memory=pin):
+        got, got_plain = _gradients(layer, x, dy, plan), plain()
+    assert all(torch.equal(a, b) for a, b in zip(got, ref)) and torch.equal(got_plain, ref_plain)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), lambda t: t.clone()):
+        got, got_plain = _gradients(layer, x, dy, plan), plain()
+    assert all(torch.equal(a, b) for a, b in zip(got, ref)) and torch.equal(got_plain, ref_plain)

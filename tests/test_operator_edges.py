@@ -109,3 +109,16 @@ def test_scale_stays_in_fp32():
         assert "scale" in dict(layer.named_buffers()) and layer.adapters().count == 3
     layer = AdaptedSparseLinear(BlockSparseLinear(_bsr(torch.bfloat16)), 3, 4).to("meta")
     assert layer.scale.device.type == "meta"
+
+
+@pytest.mark.parametrize("n,k", [(5, 100), (1, 100), (3, 64), (1, 16), (4, 1), (0, 100)])
+@pytest.mark.parametrize("pitch", [0, 48])
+def test_checkpoint_parts_survive_copies(n, k, pitch):
+    """The parts that a backward pass keeps can be cloned or moved, and read back with rows of 16-byte pitch."""
+    ldq = -(-k // 16) * 16 + pitch
+    codes = torch.randint(-127, 128, (n, ldq), dtype=torch.int8)[:, :k]
+    q = QuantizedActivations(codes=codes, steps=torch.rand(-(-k // 64), n), dtype=torch.bfloat16)
+    for copy in (lambda t: t, lambda t: t.clone(), lambda t: torch.empty(t.size(), dtype=t.dtype).copy_(t)):
+        back = QuantizedActivations._from_parts(*(copy(t) for t in q._parts()), k, q.dtype)
+        assert torch.equal(back.codes, codes) and torch.equal(back.steps, q.steps) and back.dtype == q.dtype
+        assert back._ldq % 16 == 0
