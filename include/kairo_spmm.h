@@ -333,7 +333,7 @@ KAIRO_API kairo_status kairo_bsr_sddmm_workspace_size(const kairo_bsr* a, size_t
  * Activations kept in 8 bits for the backward pass (no counterpart in the
  * reference).  Every 64 columns of a row share a step a * (1 / 127), a the
  * largest magnitude of the group: codes (n x k int8, leading dimension ldq, a
- * multiple of 16, 16-byte aligned) hold round_half_even(x * inv) with inv =
+ * multiple of 16, 16-byte aligned, n * ldq bytes of memory) hold round_half_even(x * inv) with inv =
  * 127 * (1 / a), steps (ceil(k / 64) x n fp32, leading dimension lds) the
  * steps; inv and step are computed in fp32, every operation rounded.  The
  * value read back is code * step, rounded to the activation's type.  Groups with a < 2^-100 read back as zeros, groups

@@ -30,9 +30,10 @@ GROUP = 64  # columns that share a step
 class QuantizedActivations:
     """An (n, k) activation in 8 bits.
 
-    codes: (n, k) int8, rows padded to 16 bytes; steps: (ceil(k / 64), n)
-    float32, the step of columns 64 g .. 64 g + 63 of row r at [g, r]; dtype:
-    the activation's type, in which ``code * step`` is read back."""
+    codes: (n, k) int8, rows padded to 16 bytes (the last one too); steps:
+    (ceil(k / 64), n) float32, the step of columns 64 g .. 64 g + 63 of row r at
+    [g, r]; dtype: the activation's type, in which ``code * step`` is read
+    back."""
 
     codes: Tensor
     steps: Tensor
@@ -52,6 +53,10 @@ class QuantizedActivations:
             if self.codes.stride(1) != 1 or self.codes.data_ptr() % 16 or (n > 1 and (self.codes.stride(0) % 16 or
                                                                                     self.codes.stride(0) < k)):
                 raise ValueError("codes must have 16-byte aligned rows")
+            padded = -(-k // 16) * 16  # whole 16-byte vectors are read, of the last row too
+            end = self.codes.storage_offset() + (n - 1) * self.codes.stride(0) + padded
+            if end > self.codes.untyped_storage().nbytes():
+                raise ValueError(f"codes must have rows padded to 16 bytes: the last row's memory ends before column {padded}")
             if (n > 1 and self.steps.stride(1) != 1) or (self.steps.shape[0] > 1 and self.steps.stride(0) < n):
                 raise ValueError("steps must be row-major")
 

@@ -122,3 +122,18 @@ def test_checkpoint_parts_survive_copies(n, k, pitch):
         back = QuantizedActivations._from_parts(*(copy(t) for t in q._parts()), k, q.dtype)
         assert torch.equal(back.codes, codes) and torch.equal(back.steps, q.steps) and back.dtype == q.dtype
         assert back._ldq % 16 == 0
+
+
+@pytest.mark.parametrize("n,k", [(1, 100), (1, 1), (3, 100)])
+def test_codes_without_their_padding_are_refused(n, k):
+    """The kernels read whole 16-byte vectors: the last row's must lie inside the tensor's memory."""
+    ldq = -(-k // 16) * 16
+    steps = torch.ones(-(-k // 64), n)
+    full = torch.zeros(n * ldq, dtype=torch.int8)
+    QuantizedActivations(codes=full.view(n, ldq)[:, :k], steps=steps, dtype=torch.float32)
+    short = full[: (n - 1) * ldq + k].clone().as_strided((n, k), (ldq, 1))
+    with pytest.raises(ValueError, match="padded to 16"):
+        QuantizedActivations(codes=short, steps=steps, dtype=torch.float32)
+    if n == 1:  # the copy of a single row
+        with pytest.raises(ValueError, match="padded to 16"):
+            QuantizedActivations(codes=torch.zeros(1, k, dtype=torch.int8), steps=steps, dtype=torch.float32)
