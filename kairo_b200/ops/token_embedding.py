@@ -62,6 +62,13 @@ class TokenOrder:
     perm: Tensor
     num_embeddings: int
 
+    def __post_init__(self) -> None:
+        for name, t in (("sorted_ids", self.sorted_ids), ("perm", self.perm)):
+            if t.dim() != 1 or t.dtype != torch.int32 or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous 1-D int32 tensor")
+        if self.sorted_ids.shape != self.perm.shape or self.sorted_ids.device != self.perm.device:
+            raise ValueError("sorted_ids and perm must be of one length, on one device")
+
 
 @functools.lru_cache(maxsize=4096)
 def _sort_bytes(tokens: int, n_rows: int) -> int:
@@ -140,10 +147,10 @@ def embedding_grad(grad_output: Tensor, ids: Tensor | TokenOrder, num_embeddings
     if isinstance(ids, TokenOrder):
         if ids.num_embeddings != n_rows:
             raise ValueError(f"the token order is of {ids.num_embeddings} rows, not {n_rows}")
-        tokens, where = ids.perm.numel(), ids.perm
+        tokens, where = ids.perm.numel(), (ids.perm, ids.sorted_ids)
     else:
-        tokens, where = ids.numel(), ids
-    index = _lib.device_index("embedding_grad", grad_output, where)
+        tokens, where = ids.numel(), (ids,)
+    index = _lib.device_index("embedding_grad", grad_output, *where)
     dev = grad_output.device
     if n_rows < 0:
         raise ValueError("num_embeddings must be non-negative")
@@ -164,7 +171,7 @@ def embedding_grad(grad_output: Tensor, ids: Tensor | TokenOrder, num_embeddings
     elif tuple(out.shape) != (n_rows, d) or out.dtype != odt or out.device != dev or _rows(out) is not out:
         raise ValueError(f"out must be a row-major ({n_rows}, {d}) {odt} tensor on {dev}")
     else:
-        _lib.refuse_overlap("embedding_grad", out, g, where)
+        _lib.refuse_overlap("embedding_grad", out, g, *where)
     in_order = isinstance(ids, TokenOrder)
     size = _grad_bytes(tokens, d, in_order)
     ws = g.new_empty(size, dtype=torch.uint8) if size else None

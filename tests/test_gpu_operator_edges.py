@@ -14,12 +14,16 @@ from kairo_b200.ops import (
     AdaptedSparseLinear,
     BlockSparseLinear,
     LowRankAdapters,
+    TokenOrder,
     adapter_linear,
     adapter_linear_backward,
     adapter_plan,
     bsr_from_tiles,
     dequantize_activations,
+    embedding_grad,
+    embedding_lookup,
     quantize_activations,
+    sort_tokens,
     sparse_linear_weight_grad,
 )
 
@@ -187,3 +191,16 @@ def test_checkpoint_under_offloading_hooks(k, pin, tokens):
     with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), lambda t: t.clone()):
         got, got_plain = _gradients(layer, x, dy, plan), plain()
     assert all(torch.equal(a, b) for a, b in zip(got, ref)) and torch.equal(got_plain, ref_plain)
+
+
+def test_gradient_over_its_own_order_is_refused():
+    ids = torch.arange(16, device=DEV) % 5
+    order = sort_tokens(ids, 5)
+    out = torch.zeros(5, 32, device=DEV)
+    inside = out.view(-1)[:16].view(torch.int32)
+    g = torch.ones(16, 32, device=DEV)
+    for part in ("sorted_ids", "perm"):
+        parts = {"sorted_ids": order.sorted_ids, "perm": order.perm}
+        parts[part] = inside.copy_(parts[part])
+        with pytest.raises(ValueError, match="share memory"):
+            embedding_grad(g, TokenOrder(**parts, num_embeddings=5), 5, out=out)

@@ -16,6 +16,7 @@ from kairo_b200.ops import (
     BlockSparseLinear,
     LowRankAdapters,
     QuantizedActivations,
+    TokenOrder,
     adapter_linear_backward,
     backward,
 )
@@ -137,3 +138,14 @@ def test_codes_without_their_padding_are_refused(n, k):
     if n == 1:  # the copy of a single row
         with pytest.raises(ValueError, match="padded to 16"):
             QuantizedActivations(codes=torch.zeros(1, k, dtype=torch.int8), steps=steps, dtype=torch.float32)
+
+
+def test_token_order_refusals():
+    """A token order is passed on as two pointers and a length: its parts must fit them."""
+    ids, perm = torch.tensor([0, 2, 5], dtype=torch.int32), torch.tensor([1, 0, 2], dtype=torch.int32)
+    assert TokenOrder(sorted_ids=ids, perm=perm, num_embeddings=5).num_embeddings == 5
+    for bad in ({"perm": perm.long()}, {"sorted_ids": ids.long()}, {"sorted_ids": ids[:2]}, {"perm": perm[:2]},
+                {"perm": perm.view(1, 3)}, {"perm": torch.zeros(6, dtype=torch.int32)[::2]},
+                {"sorted_ids": torch.zeros(3, 2, dtype=torch.int32)[:, 0]}, {"sorted_ids": ids.to("meta")}):
+        with pytest.raises(ValueError):
+            TokenOrder(**{"sorted_ids": ids, "perm": perm, "num_embeddings": 5, **bad})
