@@ -439,8 +439,9 @@ kairo_status sort_in_cluster(const ID* ids, int64_t n, int64_t n_rows, uint32_t*
   cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        static_cast<int>(cluster_sort_smem(kClusterItems * kClusterThreads)));
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(token sort)");
-  // as many zeroing clusters as leave room for the sort
-  const int spare = zero.rows > 0 ? std::max(0, device_sm_count(current_device()) / ctas - 2) : 0;
+  // As many zeroing clusters as leave room for the sort, and one at least: the
+  // caller counts on these rows.
+  const int spare = zero.rows > 0 ? std::max(1, device_sm_count(current_device()) / ctas - 2) : 0;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas * (1 + spare)));
   cfg.blockDim = dim3(kClusterThreads);

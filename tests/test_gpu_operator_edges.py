@@ -204,3 +204,27 @@ def test_gradient_over_its_own_order_is_refused():
         parts[part] = inside.copy_(parts[part])
         with pytest.raises(ValueError, match="share memory"):
             embedding_grad(g, TokenOrder(**parts, num_embeddings=5), 5, out=out)
+
+
+@pytest.mark.parametrize("dt,d", [(torch.bfloat16, 2048), (torch.float32, 1024)])
+@pytest.mark.parametrize("tokens", [4097, 5000, 40000])
+def test_gradient_of_a_large_table(dt, d, tokens):
+    """Only the last rows are zeroed beside the sort (some 48 to 116 MB of them): rows with and without tokens on
+    both sides of the border, in a buffer that held NaN."""
+    n = 40000  # 160 MB
+    g = torch.Generator(device=DEV).manual_seed(tokens)
+    grad = torch.randn(tokens, d, generator=g, device=DEV).to(dt)
+    ids = torch.randint(-100, n + 100, (tokens,), generator=g, device=DEV)
+    ids[:40], ids[-40:] = n - 1, 0
+    out = torch.full((n, d), float("nan"), dtype=dt, device=DEV)
+    assert embedding_grad(grad, ids, n, scale=0.5, out=out) is out
+    ok = (ids >= 0) & (ids < n)
+    used, row = torch.unique(ids[ok], return_inverse=True)
+    ref = torch.zeros(used.numel(), d, dtype=torch.float64, device=DEV).index_add_(0, row, grad[ok].double() * 0.5)
+    mag = torch.zeros_like(ref).index_add_(0, row, grad[ok].double().abs() * 0.5)
+    # a sum of c fp32 values is off by at most (c - 1) * 2^-24 of the magnitudes; then the scale's product
+    tol = mag * (torch.bincount(row)[:, None] + 3) * 2.0**-24
+    assert bool(((out[used].double() - ref).abs() <= tol + (ref.abs() + tol) * _half(dt) * 1.01 + 1e-30).all())
+    rest = torch.ones(n, dtype=torch.bool, device=DEV)
+    rest[used] = False
+    assert int(rest.sum()) > 0 and bool((out[rest] == 0).all())
