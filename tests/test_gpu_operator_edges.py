@@ -228,3 +228,65 @@ def test_gradient_of_a_large_table(dt, d, tokens):
     rest = torch.ones(n, dtype=torch.bool, device=DEV)
     rest[used] = False
     assert int(rest.sum()) > 0 and bool((out[rest] == 0).all())
+
+
+@pytest.mark.parametrize("wt,ot", [(torch.float32, torch.bfloat16), (torch.bfloat16, torch.bfloat16),
+                                   (torch.float16, torch.float32)])
+@pytest.mark.parametrize("d", [64, 1000, 2048, 37])
+@pytest.mark.parametrize("tokens", [19999, 20480, 40001])
+def test_lookup_of_long_lists(wt, ot, d, tokens):
+    """Four rows of a thread under way: every width, ids outside the table, a last group that is not whole."""
+    n = 700
+    g = torch.Generator(device=DEV).manual_seed(d)
+    w = torch.randn(n, d, generator=g, device=DEV).to(wt)
+    ids = torch.randint(-3, n + 3, (tokens,), generator=g, device=DEV)
+    buf = torch.full((tokens + 1, d), 7.0, dtype=ot, device=DEV)
+    embedding_lookup(w, ids, scale=1.7, out=buf[:tokens])
+    ok = (ids >= 0) & (ids < n)
+    ref = w.double()[ids.clamp(0, n - 1)] * 1.7 * ok[:, None]
+    # half a step of the output, of the fp32 product and of 1.7 in fp32
+    tol = ref.abs() * (_half(ot) * 1.001 + 2 * 2.0**-24) + torch.finfo(ot).smallest_normal * _half(ot) * 2
+    assert bool(((buf[:tokens].double() - ref).abs() <= tol).all()) and bool((buf[tokens] == 7).all())
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("k,n", [(4096, 4096), (4104, 3592), (8192, 64), (72, 8192), (4097, 3601)])
+@pytest.mark.parametrize("tokens,rank", [(1, 16), (20, 16), (20, 40), (3, 128)])
+def test_wide_layers_of_few_tokens(dt, k, n, tokens, rank):
+    """Eight CTAs to a tile: features in 64 x 8 x 8 parts, whole and not, forward and backward against 64 bits."""
+    gen = torch.Generator(device=DEV).manual_seed(k + n + tokens)
+    rand = lambda *s: torch.randn(*s, generator=gen, device=DEV)  # noqa: E731
+    x, dy = rand(tokens, k).to(dt), (rand(tokens, n) * 0.1).to(dt)
+    down, up = (rand(3, rank, k) * k**-0.5).to(dt), (rand(3, rank, n) * rank**-0.5).to(dt)
+    scale = torch.tensor([1.0, 0.5, 2.0], device=DEV)
+    ids = torch.arange(tokens, device=DEV) % 4 - int(tokens > 1)  # -1: none
+    base, base_dx = rand(tokens, n).to(dt), rand(tokens, k).to(dt)
+    a, plan = LowRankAdapters(down=down, up=up, scale=scale), adapter_plan(ids, 3)
+    y, low = adapter_linear(x, a, plan, base=base, return_low=True)
+    dx, dd, du = adapter_linear_backward(dy, x, a, plan, low=low, base_dx=base_dx, grad_dtype=torch.float32)
+
+    mine = ((ids >= 0) & (ids < 3)).double() * scale.double()[ids.clamp(0, 2)]
+    at = ids.clamp(0, 2)
+
+    def forward(v, first, second, start, f=lambda t: t):
+        v, first, second = f(v.double()), f(first.double())[at], f(second.double())[at]
+        lo = torch.einsum("tk,trk->tr", v, first) * mine[:, None]
+        return lo, f(start.double()) + torch.einsum("tr,trn->tn", lo, second)
+
+    def inside(got, ref, mag, terms, rest, t):
+        slack = mag * (terms * 2.0**-23 + rest)
+        tiny = torch.finfo(t).smallest_normal * _half(t) * 2
+        assert bool(((got.double() - ref).abs() <= slack + (ref.abs() + slack) * _half(t) * 1.01 + tiny).all())
+
+    rl, ry = forward(x, down, up, base)
+    ml, my = forward(x, down, up, base, torch.abs)
+    rdl, rx = forward(dy, up, down, base_dx)
+    mdl, mx = forward(dy, up, down, base_dx, torch.abs)
+    inside(low, rl, ml, k + 2, 0.0, torch.float32)
+    inside(y, ry, my, k + rank + 4, 2.0**-17, dt)
+    inside(dx, rx, mx, n + rank + 4, 2.0**-17, dt)
+    one = torch.nn.functional.one_hot(at, 3).double() * ((ids >= 0) & (ids < 3))[:, None]
+    for got, s, sm, z, terms in ((dd, rdl, mdl, x, n), (du, rl, ml, dy, k)):
+        ref = torch.einsum("tg,tr,tk->grk", one, s, z.double())
+        mag = torch.einsum("tg,tr,tk->grk", one, sm, z.double().abs())
+        inside(got, ref, mag, terms + tokens + 4, 2.0**-23, torch.float32)
