@@ -149,3 +149,30 @@ def test_token_order_refusals():
                 {"sorted_ids": torch.zeros(3, 2, dtype=torch.int32)[:, 0]}, {"sorted_ids": ids.to("meta")}):
         with pytest.raises(ValueError):
             TokenOrder(**{"sorted_ids": ids, "perm": perm, "num_embeddings": 5, **bad})
+
+
+def test_overlap():
+    """Refused: memory that is shared.  Columns of one wider matrix, side by side, share none."""
+    buf = torch.zeros(8, 20)
+    out = buf[:, 4:10]
+
+    def refused(t, o=out):
+        try:
+            _lib.refuse_overlap("op", o, t)
+        except ValueError:
+            return True
+        return False
+
+    mine = {x.data_ptr() for x in (out[i, j] for i in range(8) for j in range(6))}
+    for c0 in range(20):
+        for c1 in range(c0 + 1, 21):
+            for r0, r1 in ((0, 8), (2, 7), (3, 5)):
+                t = buf[r0:r1, c0:c1]
+                theirs = {x.data_ptr() for x in (t[i, j] for i in range(r1 - r0) for j in range(c1 - c0))}
+                assert refused(t) == bool(mine & theirs), (c0, c1, r0, r1)
+    half = buf.view(torch.float16)  # rows of the same bytes in another type
+    assert not refused(half[:, :8]) and refused(half[:, :9]) and not refused(half[:, 20:]) and refused(half[:, 19:])
+    # where the pitches differ, any meeting of the spans counts
+    assert refused(buf.view(-1)[:40]) and refused(buf[::2, 12:]) and refused(buf.t()) and not refused(buf.clone())
+    assert not refused(buf[:, 4:4]) and refused(out) and refused(buf[0, 4].expand(3, 6))
+    assert not refused(buf.view(-1)[:4]) and not refused(buf.view(-1)[150:])
