@@ -203,7 +203,8 @@ def adapter_linear(X: Tensor, adapters: LowRankAdapters, plan: AdapterPlan, *, b
     if out is not None:
         in_place = base is not None and (base.data_ptr(), base.stride(), base.dtype) == (out.data_ptr(), out.stride(),
                                                                                          out.dtype)
-        _lib.refuse_overlap(op, out, X, adapters.down, adapters.up, *(() if base is None or in_place else (base,)))
+        _lib.refuse_overlap(op, out, X, adapters.down, adapters.up, plan.memory,
+                            *(t for t in (adapters.scale, None if in_place else base) if t is not None))
     base, out = _result(op, adapters.down, (plan.num_tokens, n), base, out, out_dtype)
     low = X.new_empty((plan.num_tokens, rank), dtype=torch.float32) if return_low else None
     _apply(op, index, _rows(X), adapters.down, adapters.up, k, n, rank, adapters._code, adapters.scale, plan, base, out,

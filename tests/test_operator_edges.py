@@ -17,6 +17,7 @@ from kairo_b200.ops import (
     LowRankAdapters,
     QuantizedActivations,
     TokenOrder,
+    adapter_linear,
     adapter_linear_backward,
     backward,
 )
@@ -176,3 +177,20 @@ def test_overlap():
     assert refused(buf.view(-1)[:40]) and refused(buf[::2, 12:]) and refused(buf.t()) and not refused(buf.clone())
     assert not refused(buf[:, 4:4]) and refused(out) and refused(buf[0, 4].expand(3, 6))
     assert not refused(buf.view(-1)[:4]) and not refused(buf.view(-1)[150:])
+
+
+def test_out_is_compared_with_every_input(monkeypatch):
+    """adapter_linear's result may not lie over its scale or its plan either."""
+    down, up = torch.zeros(2, 4, 64, dtype=torch.bfloat16), torch.zeros(2, 4, 32, dtype=torch.bfloat16)
+    monkeypatch.setattr(_lib, "device_index", lambda op, *t: -1)
+    monkeypatch.setattr(_lib, "launch", lambda *args: None)
+    x = torch.zeros(3, 64, dtype=torch.bfloat16)
+    out = torch.zeros(3, 32)
+    plain = LowRankAdapters(down=down, up=up)
+    plan = AdapterPlan(memory=torch.zeros(256, dtype=torch.uint8), num_tokens=3, num_adapters=2)
+    assert adapter_linear(x, plain, plan, out=out) is out
+    with pytest.raises(ValueError, match="share memory"):
+        adapter_linear(x, LowRankAdapters(down=down, up=up, scale=out.view(-1)[5:7]), plan, out=out)
+    over = AdapterPlan(memory=out.view(-1).view(torch.uint8)[:256], num_tokens=3, num_adapters=2)
+    with pytest.raises(ValueError, match="share memory"):
+        adapter_linear(x, plain, over, out=out)
