@@ -386,4 +386,6 @@ class AdaptedSparseLinear(torch.nn.Module):
                                scale=self.scale if scale is None else scale)
 
     def forward(self, X: Tensor, plan: AdapterPlan) -> Tensor:
+        if not torch.is_grad_enabled():  # no backward pass: nothing to keep
+            return adapted_sparse_linear(X, self.layer.weight_matrix(), self.adapters(), plan)
         return _AdaptedLinearFn.apply(X, self.layer.blocks, self.down, self.up, self, plan)

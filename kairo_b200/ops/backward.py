@@ -244,4 +244,6 @@ class BlockSparseLinear(torch.nn.Module):
         return self._wt
 
     def forward(self, X: Tensor) -> Tensor:
+        if self.checkpoint is not None and not torch.is_grad_enabled():
+            return sparse_linear(X, self.weight_matrix())  # no backward pass: nothing to keep in 8 bits
         return _SparseLinearFn.apply(X, self.blocks, self)

@@ -290,3 +290,12 @@ def test_wide_layers_of_few_tokens(dt, k, n, tokens, rank):
         ref = torch.einsum("tg,tr,tk->grk", one, s, z.double())
         mag = torch.einsum("tg,tr,tk->grk", one, sm, z.double().abs())
         inside(got, ref, mag, terms + tokens + 4, 2.0**-23, torch.float32)
+
+
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_layers_without_gradients(checkpoint):
+    """The same bits with and without a graph; without one nothing is allocated for a backward pass."""
+    layer, x, dy, plan = _adapted(checkpoint=checkpoint)
+    want, inner = layer(x, plan), layer.layer(x)
+    with torch.no_grad():
+        assert torch.equal(layer(x, plan), want) and torch.equal(layer.layer(x), inner)

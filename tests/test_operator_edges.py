@@ -19,6 +19,7 @@ from kairo_b200.ops import (
     TokenOrder,
     adapter_linear,
     adapter_linear_backward,
+    adapters,
     backward,
 )
 from kairo_b200.types import BlockSparseMatrix
@@ -194,3 +195,23 @@ def test_out_is_compared_with_every_input(monkeypatch):
     over = AdapterPlan(memory=out.view(-1).view(torch.uint8)[:256], num_tokens=3, num_adapters=2)
     with pytest.raises(ValueError, match="share memory"):
         adapter_linear(x, plain, over, out=out)
+
+
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+def test_nothing_is_kept_without_a_backward_pass(monkeypatch, mode):
+    """Without gradients a layer with 8-bit checkpoints quantises nothing."""
+    calls = []
+    x = torch.zeros(3, 64)
+    for module in (adapters, backward):
+        monkeypatch.setattr(module, "quantize_activations", lambda t: calls.append(t) or QuantizedActivations(
+            codes=torch.zeros(3, 64, dtype=torch.int8), steps=torch.zeros(1, 3), dtype=t.dtype))
+    monkeypatch.setattr(backward, "sparse_linear", lambda X, W, **kw: torch.ones(3, 64))
+    monkeypatch.setattr(adapters, "adapted_sparse_linear", lambda X, W, a, plan, return_low=False: (
+        (torch.ones(3, 64), torch.zeros(3, 4)) if return_low else torch.ones(3, 64)))
+    plain = BlockSparseLinear(_bsr(), checkpoint="int8")
+    adapted = AdaptedSparseLinear(BlockSparseLinear(_bsr(torch.bfloat16), checkpoint="int8"), 2, 4)
+    with mode():
+        for y in (plain(x), adapted(x, None)):
+            assert y.shape == (3, 64) and not y.requires_grad
+    assert not calls
+    assert plain(x).requires_grad and adapted(x, None).requires_grad and len(calls) == 2
