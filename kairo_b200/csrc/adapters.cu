@@ -172,14 +172,18 @@ bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 // 13.0 with 64, 2048 tokens 12.8 and 14.0, 4096 tokens 22.8 and 22.4; rank 32,
 // 2048 tokens 17.3 and 17.6 (with 32), and 8192 tokens of 8192 features 117
 // and 96; rank 64, 1024 tokens 19.0 and 24.2, 4096 tokens 48.5 and 39.6; rank 128,
-// 4096 tokens 94.8 and 75.5 (with 32).  Contractions that are summed in parts
+// 4096 tokens 94.8 and 75.5 (with 32).  An fp32 base takes twice the room of
+// its loads, one CTA per SM instead of two for the tall tiles of small ranks, and
+// more time than the weights: 8192 features, 4096 tokens of 4 adapters, rank 16
+// 82 us with tiles of 16 and 88 with 64, rank 32 88 and 94 (with 32), rank 64
+// 119 and 96 (with 32); 2100 tokens of 4096 features, rank 16 29 and 49.  Contractions that are summed in parts
 // have tiles of 16 only.
 int pick_tile(int64_t t, int64_t k, int64_t rank, bool vec, bool base_f32) {
   if (!vec || t <= 2048 || k > lowrank::kLongFeatures) return 16;
+  if (base_f32) return rank > 32 && rank <= 64 ? 32 : 16;
   if (rank <= 16) return 64;
   if (rank <= 32) return 32;
-  if (rank <= 64) return base_f32 ? 32 : 64;
-  return base_f32 ? 16 : 32;
+  return rank <= 64 ? 64 : 32;
 }
 
 // CTAs per tile, a power of two up to 8.  As many as the GPU holds at once (two

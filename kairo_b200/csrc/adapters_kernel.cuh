@@ -869,11 +869,10 @@ cudaError_t launch_apply_as(const LowRankApplyArgs& a, int64_t clusters, int clu
 
 template <typename T, typename TY, typename S, bool VEC>
 cudaError_t launch_apply(const LowRankApplyArgs& a, int64_t clusters, int cluster, cudaStream_t s) {
-  if constexpr (S::MT == 1) {  // the shapes of 16 tokens
-    if (a.k > kLongFeatures)
-      return a.base_f32 ? launch_apply_as<T, TY, S, true, VEC, true>(a, clusters, cluster, s)
-                        : launch_apply_as<T, TY, S, false, VEC, true>(a, clusters, cluster, s);
-  }
+  static_assert(S::MT == 1, "the shapes of 16 tokens");
+  if (a.k > kLongFeatures)
+    return a.base_f32 ? launch_apply_as<T, TY, S, true, VEC, true>(a, clusters, cluster, s)
+                      : launch_apply_as<T, TY, S, false, VEC, true>(a, clusters, cluster, s);
   return a.base_f32 ? launch_apply_as<T, TY, S, true, VEC>(a, clusters, cluster, s)
                     : launch_apply_as<T, TY, S, false, VEC>(a, clusters, cluster, s);
 }
@@ -890,14 +889,14 @@ cudaError_t pick_apply(const LowRankApplyArgs& a, bool vec, int tile, int64_t cl
     if (a.rank <= 64) return launch_apply<T, TY, R64, false>(a, clusters, cluster, s);
     return launch_apply<T, TY, R128, false>(a, clusters, cluster, s);
   }
+  // the tall tiles: 16-bit bases, but for 32 tokens at rank 64
   if (a.rank <= 16)
-    return tile == 64 ? launch_apply<T, TY, ApplyShape<4, 2, 2>, true>(a, clusters, cluster, s)
+    return tile == 64 ? launch_apply_as<T, TY, ApplyShape<4, 2, 2>, false, true>(a, clusters, cluster, s)
                       : launch_apply<T, TY, R16, true>(a, clusters, cluster, s);
   if (a.rank <= 32)
-    return tile == 32 ? launch_apply<T, TY, ApplyShape<2, 4, 2>, true>(a, clusters, cluster, s)
+    return tile == 32 ? launch_apply_as<T, TY, ApplyShape<2, 4, 2>, false, true>(a, clusters, cluster, s)
                       : launch_apply<T, TY, R32, true>(a, clusters, cluster, s);
   if (a.rank <= 64)
-    // an fp32 base takes twice the room of its loads
     return tile == 64   ? launch_apply_as<T, TY, ApplyShape<4, 8, 2, true>, false, true>(a, clusters, cluster, s)
            : tile == 32 ? launch_apply_as<T, TY, ApplyShape<2, 8, 3>, true, true>(a, clusters, cluster, s)
                         : launch_apply<T, TY, R64, true>(a, clusters, cluster, s);
