@@ -342,7 +342,8 @@ KAIRO_API kairo_status kairo_bsr_sddmm_workspace_size(const kairo_bsr* a, size_t
  *   kairo_quantize_q8     x (n x k, leading dimension ldx) -> codes, steps
  *   kairo_dequantize_q8   codes, steps -> x in `dtype`
  *   kairo_bsr_sddmm_q8    kairo_bsr_sddmm with X (a's dtype) given by its
- *                         codes and steps
+ *                         codes and steps; its workspace does not depend on
+ *                         the batch n
  * All asynchronous on `stream`.
  * ---------------------------------------------------------------------- */
 KAIRO_API kairo_status kairo_quantize_q8(const void* x, int64_t n, int64_t k, int64_t ldx, kairo_dtype dtype,
@@ -387,8 +388,9 @@ KAIRO_API kairo_status kairo_bsr_sddmm_q8_workspace_size(const kairo_bsr* a, int
  * x, z, down, up f16 or bf16 (one dtype); base, y and grad that dtype or fp32.
  * rank at most 128, at most 65535 adapters, 2^24 tokens, 2^22 features.  plan
  * and workspace start on a multiple of 16 bytes; the other operands may have any
- * address of their type (slower where one is not a multiple of 16).  All
- * asynchronous on `stream`.
+ * address of their type (slower where one is not a multiple of 16).  An infinity
+ * or NaN in an operand makes the results that it enters non-finite (NaN where
+ * the sum would be infinite, too) and no others.  All asynchronous on `stream`.
  * ---------------------------------------------------------------------- */
 KAIRO_API kairo_status kairo_adapter_plan_build(const void* ids, int32_t id_bytes, int64_t ntokens,
                                                 int64_t nadapters, void* plan, size_t plan_size, void* workspace,

@@ -28,7 +28,9 @@
 // two for 16-bit results (rest at most 2^-17 of it), three for fp32 results
 // (2^-23).  In fp16, whose range is narrow, it is first scaled by a power of
 // two (exact) that brings the largest of the row to [1, 2), and the rest is
-// one of that largest.  A low value that is infinite makes its token's row NaN.
+// one of that largest (2^-25 of it at least, a term's smallest step).  An infinity
+// in low, or in what it is multiplied by, spoils what it enters: of its terms some
+// are zero or of the other sign, so that the sum is NaN where it would be infinite.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -939,9 +941,12 @@ struct WgradShape {
 // truncation.  The cluster's partial sums are added in rank order.
 //
 // DIRECT: bf16 results of batches up to kDirectTokens are added up by the units
-// themselves.  They lose 2^-23 of the sum at most per step and term, 2^-11 over
-// such a batch: a quarter of the result's own rounding at worst (8192 tokens,
-// 8192 features, rank 32 80 -> 73 us; 4096 tokens, rank 64 92 -> 83, 128 220 -> 188).
+// themselves.  They truncate twice per step and term at most, 2^-10 of the sum over
+// such a batch, a quarter of half a step of the result, were all of it one CTA's;
+// 32768 tokens of one sign and one adapter came out 3.05e-4 too small on
+// average, and 3.0e-4 when added with rounding (the results' own rounding).
+// 8192 tokens, 8192 features, rank 32 80 -> 73 us; 4096 tokens, rank 64 92 -> 83, 128
+// 220 -> 188.
 constexpr int64_t kDirectTokens = 32768;
 template <typename T, typename TG, typename S, int TERMS, bool Q8, bool VEC, bool DIRECT, int MINB>
 __global__ void __launch_bounds__(kThreadsPerCta, MINB) k_wgrad(const LowRankWgradArgs args) {

@@ -168,12 +168,6 @@ bool simt_supported(const kairo_bsr* a, int32_t layout, kairo_dtype c_dtype, std
 kairo_status simt_launch(const kairo_bsr* a, const void* b, int64_t ldb, int64_t n, void* c,
                          int64_t ldc, void* workspace, cudaStream_t stream);
 
-// Argument checks of the weight gradient (spmm_sddmm.cu), before any launch;
-// x may be any pointer to the activation in whatever form it is given.
-kairo_status sddmm_check(const kairo_bsr* a, const int32_t* row_ptr_t, const int32_t* col_idx_t,
-                         const int32_t* perm_t, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t n,
-                         const void* dblocks, kairo_dtype out_dtype, const void* workspace);
-
 // Checks of an activation in 8 bits (activation_q8.cu).
 kairo_status q8_check(int64_t n, int64_t k, const void* codes, int64_t ldq, const void* steps, int64_t lds);
 

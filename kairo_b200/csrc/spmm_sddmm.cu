@@ -637,8 +637,8 @@ bool sdd_tc_ok(const kairo_bsr* a, const void* dy, int64_t lddy, const SddX& x, 
   return x.ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(x.x) & 15u) == 0;
 }
 
-}  // namespace
-
+// Argument checks, before any launch; x may be any pointer to the activation in
+// whatever form it is given.
 kairo_status sddmm_check(const kairo_bsr* a, const int32_t* row_ptr_t, const int32_t* col_idx_t,
                          const int32_t* perm_t, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t n,
                          const void* dblocks, kairo_dtype out_dtype, const void* workspace) {
@@ -657,6 +657,7 @@ kairo_status sddmm_check(const kairo_bsr* a, const int32_t* row_ptr_t, const int
   return KAIRO_STATUS_SUCCESS;
 }
 
+}  // namespace
 }  // namespace kairo
 
 using namespace kairo;

@@ -4,9 +4,11 @@
 //         an id outside [0, n_rows).
 // sort    the token positions ordered by id, equal ids in token order (an
 //         LSD radix sort).  Ids outside [0, n_rows) become n_rows and end up
-//         last.  Up to 65536 tokens are sorted by one cluster in one launch,
-//         keys and positions staying in its distributed shared memory between
-//         the passes; longer lists take three launches a pass.
+//         last.  Lists of up to 4096 tokens (2048 where ids are below 512) are
+//         ranked by counting; up to 65536 are sorted by one cluster, keys and
+//         positions staying in its distributed shared memory between the
+//         passes, both in one launch; longer lists take three launches a pass
+//         (65536 tokens of 131072 rows 35 us, 65537 64, 10^6 332).
 // grad    grad_weight[r, :] = scale * sum of grad_output[t, :] over id_t == r.
 //         The sorted positions are cut into chunks of equal length whatever
 //         the ids, so that a frequent token costs no more time than rare ones.
@@ -16,7 +18,9 @@
 //         partial rows, which a second kernel adds up in chunk order.  All
 //         sums are fp32 in an order that depends on the ids alone, so that
 //         equal calls give equal bits.  Rows without tokens are zeroed by
-//         further CTAs of the first kernel, so that every row is written once.
+//         further CTAs of the first kernel; the last rows of a large table are
+//         zeroed beside the cluster's sort, and those of them that have tokens
+//         written again.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -158,7 +162,7 @@ __global__ void __launch_bounds__(1024) k_sort_scan(uint32_t* __restrict__ count
 
 // Stable scatter of one digit.  A warp owns 32 * kSortItems consecutive keys
 // and takes them 32 at a time in order; lanes with equal digits rank
-// themselves by a match of the warp.
+// themselves by a vote per bit.
 template <typename ID>
 __global__ void __launch_bounds__(kSortThreads) k_sort_scatter(
     const ID* __restrict__ ids, const uint32_t* __restrict__ keys, const int32_t* __restrict__ vals, int64_t n,
@@ -692,9 +696,15 @@ __global__ void __launch_bounds__(kGradThreads * kJoinGroups) k_grad_join(const 
 // three.  A row's place in the sorted order is the number of smaller ids, so the
 // sum is cut where the chunks would cut it: the parts are the warps' items,
 // and those of one row are added as the join adds them, to the same bits.
-// fp32, this kernel and the three: 256 tokens of 10000 x 64 8.4 and 11.4 us, 64
-// tokens 5.0 and 10; it does not spread a frequent row over the GPU, so 256
-// tokens of 8874 x 2888 take 43 and 35 us and 471 would take 49 and 36.
+// This kernel and the three, 256 tokens (spread and skewed ids), cold: 10000 x 64
+// fp32 10 / 14 and 16 / 18 us, 8874 x 512 bf16 12 / 16 and 18 / 21, 8874 x 1024 fp32
+// 25 / 27 and 21 / 23, 131072 x 2048 180 / 178 and 176 / 176.  Each CTA groups its
+// rows' tokens before its first load and a frequent row is not spread over the
+// GPU, so wide rows of middling tables lose: 8874 x 2888 43 / 45 and 39 / 41
+// (bf16 33 / 33 and 25 / 27); the length alone decides, because a call that comes
+// from the host saves two launches.  An accumulating call looks through
+// the list for every 32 rows of the table all the same: 256 tokens into 10^6 x
+// 64 take 123 us, 257 through the sort 20.
 constexpr int kFewTokens = 256;
 constexpr int kFewThreads = 256;
 constexpr int kFewWarps = kFewThreads / 32;
@@ -914,8 +924,9 @@ void grad_with(const GradArgs& a, cudaStream_t s) {
     return;
   }
   // Slices of the columns, in turns of 32 * VE.  Each CTA looks through the whole
-  // list, but one that has a frequent id is not to have many columns of it: 471
-  // skewed tokens, 8874 x 2888 fp32, took 49 us with two turns and 63 with six.
+  // list, but one that has a frequent id is not to have many columns of it: 256
+  // skewed tokens, 8874 x 2888 fp32, take 45 us with two turns (the rule), 53 with
+  // one or six and 143 with all; 131072 x 2048 320, 219, 170 and 178 (the rule: all).
   const int64_t groups = ceil_div64(a.n_rows, kFewRows), all = ceil_div64(a.dim, static_cast<int64_t>(32) * VE);
   const int64_t room = 32 * device_sm_count(current_device());
   const int turns = static_cast<int>(ceil_div64(all, std::min(all, std::max<int64_t>(1, room / groups))));

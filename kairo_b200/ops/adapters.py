@@ -195,7 +195,11 @@ def adapter_linear(X: Tensor, adapters: LowRankAdapters, plan: AdapterPlan, *, b
     ``out`` may be ``base`` itself, and shares no memory with an input
     otherwise.  ``return_low=True`` also returns the
     (tokens, rank) float32 values ``scale[a] * X[t] down[a]^T`` that
-    ``adapter_linear_backward`` takes."""
+    ``adapter_linear_backward`` takes.
+
+    An infinity or a NaN in X, down, up or the scale makes the results that it
+    enters non-finite (NaN where the sum would be infinite, too) and reaches
+    no other token's."""
     op = "adapter_linear"
     _, rank, k, n = adapters._sizes
     index = _lib.device_index(op, X, adapters.down, plan.memory)
@@ -237,7 +241,8 @@ def adapter_linear_backward(dY: Tensor, X: Tensor | QuantizedActivations | None,
     None.  ``low``: what ``return_low`` gave (computed anew from X otherwise).  ``base_dx``: the shared projection's part of
     dX, added in fp32 before the one rounding to ``dx_dtype`` (default: the
     adapters').  d_down and d_up are in ``grad_dtype`` (default: the
-    adapters'), zero for an adapter without tokens."""
+    adapters'), zero for an adapter without tokens.  Infinities and NaN: as in
+    ``adapter_linear``."""
     op = "adapter_linear_backward"
     _, rank, k, n = adapters._sizes
     down, up, code = adapters.down, adapters.up, adapters._code

@@ -157,8 +157,9 @@ def sparse_linear_weight_grad(dY: Tensor, X: Tensor | QuantizedActivations, W: B
 
 
 def sparse_linear_backward(dY: Tensor, X: Tensor | QuantizedActivations, W: BlockSparseMatrix,
-                           wt: TransposedBsr | None = None, *, need_dx: bool = True, need_dw: bool = True, dw_dtype: torch.dtype = torch.float32,
-                           config: KernelConfig | None = None, check: bool = False):
+                           wt: TransposedBsr | None = None, *, need_dx: bool = True, need_dw: bool = True,
+                           dw_dtype: torch.dtype = torch.float32, config: KernelConfig | None = None,
+                           check: bool = False):
     """(dX, dW) of Y = X @ W^T.  dX: (batch, in_features) in X's dtype; dW:
     (nnzb, bm, bk) in ``dw_dtype``, W's BSR order.  Either may be None.  X may
     be given in 8 bits (``quantize_activations``)."""
