@@ -299,3 +299,97 @@ def test_layers_without_gradients(checkpoint):
     want, inner = layer(x, plan), layer.layer(x)
     with torch.no_grad():
         assert torch.equal(layer(x, plan), want) and torch.equal(layer.layer(x), inner)
+
+
+@pytest.mark.parametrize("ot", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tokens", [1, 31, 40, 256])
+@pytest.mark.parametrize("n,d", [(70, 40), (100_000, 36), (3000, 517)])
+def test_short_lists_accumulate(ot, tokens, n, d):
+    """A short list added to a caller's rows: base + sum with one rounding, other rows keep their bits, and the
+    same bits as through the sorted order."""
+    g = torch.Generator(device=DEV).manual_seed(tokens + n)
+    grad = torch.randn(tokens, d, generator=g, device=DEV)
+    ids = torch.randint(-2, n + 2, (tokens,), generator=g, device=DEV)
+    ids[: tokens // 3] = 5  # one id in several parts
+    ok = (ids >= 0) & (ids < n)
+    used = torch.zeros(n, dtype=torch.bool, device=DEV)
+    used[ids[ok]] = True
+    base = torch.randn(n, d, generator=g, device=DEV).to(ot)
+    base[~used] = float("nan")
+    wide = torch.full((n, d + 5), 3.0, dtype=ot, device=DEV)
+    out = wide[:, :d]
+    out.copy_(base)
+    assert embedding_grad(grad, ids, n, scale=0.25, out=out, accumulate=True) is out
+    other = base.clone()
+    embedding_grad(grad, sort_tokens(ids, n), n, scale=0.25, out=other, accumulate=True)
+    assert torch.equal(out[used], other[used]) and bool(other[~used].isnan().all())
+    assert bool(out[~used].isnan().all()) and bool((wide[:, d:] == 3).all())
+    ref = torch.zeros(n, d, dtype=torch.float64, device=DEV).index_add_(0, ids[ok], grad[ok].double() * 0.25)
+    mag = torch.zeros(n, d, dtype=torch.float64, device=DEV).index_add_(0, ids[ok], grad[ok].double().abs() * 0.25)
+    count = torch.zeros(n, dtype=torch.float64, device=DEV).index_add_(0, ids[ok], torch.ones(
+        int(ok.sum()), dtype=torch.float64, device=DEV))
+    ref, mag = ref[used] + base[used].double(), mag[used] + base[used].double().abs()
+    # a sum of count fp32 values, the scale's product and the sum with the base
+    s = mag * (count[used][:, None] + 3) * 2.0**-24
+    assert bool(((out[used].double() - ref).abs() <= s + (ref.abs() + s) * _half(ot) * 1.01 + 1e-38).all())
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("k,n", [(128, 64), (131, 67)])
+def test_infinities_in_the_factors(dt, k, n):
+    """An infinity makes what it enters non-finite and changes nothing else, forward and backward."""
+    gen = torch.Generator(device=DEV).manual_seed(k)
+    rand = lambda *s: torch.randn(*s, generator=gen, device=DEV).to(dt)  # noqa: E731
+    x, dy, down, up = rand(48, k), rand(48, n), rand(3, 8, k), rand(3, 8, n)
+    ids = torch.arange(48, device=DEV) % 4 - 1
+    plan = adapter_plan(ids, 3)
+
+    def step(x, dy, down, up):
+        a = LowRankAdapters(down=down, up=up)
+        y, low = adapter_linear(x, a, plan, return_low=True)
+        return (y, *adapter_linear_backward(dy, x, a, plan, low=low))
+
+    clean = step(x, dy, down, up)
+    inf = float("inf")
+    u = up.clone()
+    u[1, 2, 9] = inf  # enters column 9 of y, dlow and so dX and d_down of adapter 1's tokens
+    y, dx, dd, du = step(x, dy, down, u)
+    mine = ids == 1
+    col = torch.zeros(n, dtype=torch.bool, device=DEV)
+    col[9] = True
+    assert not bool(y[mine][:, col].isfinite().any()) and torch.equal(y[:, ~col], clean[0][:, ~col])
+    assert torch.equal(y[~mine], clean[0][~mine]) and torch.equal(dx[~mine], clean[1][~mine])
+    assert not bool(dx[mine].isfinite().any()) and torch.equal(du, clean[3])
+    assert not bool(dd[1, 2].isfinite().any()) and torch.equal(dd[[0, 2]], clean[2][[0, 2]])
+    z = x.clone()
+    z[6, 5] = -inf  # a token of adapter 1: its y and d_up, and one column of d_down
+    y, dx, dd, du = step(z, dy, down, up)
+    rest = torch.arange(48, device=DEV) != 6
+    assert not bool(y[6].isfinite().any()) and torch.equal(y[rest], clean[0][rest]) and torch.equal(dx, clean[1])
+    assert not bool(dd[1][:, 5].isfinite().any()) and not bool(du[1].isfinite().any())
+    assert torch.equal(dd[[0, 2]], clean[2][[0, 2]]) and torch.equal(du[[0, 2]], clean[3][[0, 2]])
+    keep = torch.arange(k, device=DEV) != 5
+    assert torch.equal(dd[1][:, keep], clean[2][1][:, keep])
+
+
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+@pytest.mark.parametrize("k", [320, 200])
+def test_an_empty_batch_through_the_layer(checkpoint, k):
+    layer, x, dy, _ = _adapted(k=k, checkpoint=checkpoint)
+    plan = adapter_plan(torch.zeros(0, dtype=torch.int64, device=DEV), 3)
+    dx, db, dd, du = _gradients(layer, x[:0], dy[:0], plan)
+    assert dx.shape == (0, k)
+    assert bool((db == 0).all()) and bool((dd == 0).all()) and bool((du == 0).all())
+
+
+def test_results_beside_their_inputs():
+    """Columns of one wider matrix: the input on the left, base and result in place on the right."""
+    layer, x, dy, plan = _adapted()
+    a = layer.adapters()
+    base = torch.randn(70, 256, device=DEV).bfloat16()
+    wide = torch.cat([x, base, torch.zeros_like(base)], dim=1)
+    xv, bv, ov = wide[:, :320], wide[:, 320:576], wide[:, 576:]
+    want = adapter_linear(x, a, plan, base=base)
+    assert torch.equal(adapter_linear(xv, a, plan, base=bv, out=ov), want)
+    assert torch.equal(wide[:, :320], x) and torch.equal(bv, base)
+    assert torch.equal(adapter_linear(xv, a, plan, base=bv, out=bv), want) and torch.equal(wide[:, :320], x)
