@@ -176,8 +176,9 @@ bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 // its loads, one CTA per SM instead of two for the tall tiles of small ranks, and
 // more time than the weights: 8192 features, 4096 tokens of 4 adapters, rank 16
 // 82 us with tiles of 16 and 88 with 64, rank 32 88 and 94 (with 32), rank 64
-// 119 and 96 (with 32); 2100 tokens of 4096 features, rank 16 29 and 49.  Contractions that are summed in parts
-// have tiles of 16 only.
+// 119 and 96 (with 32); 2100 tokens of 4096 features, rank 16 29 and 49.
+// Contractions that are summed in parts have tiles of 16 only: 4096 tokens, rank 16,
+// 131080 features 334 us (with 64, in one sum, 258), 262144 455 (801).
 int pick_tile(int64_t t, int64_t k, int64_t rank, bool vec, bool base_f32) {
   if (!vec || t <= 2048 || k > lowrank::kLongFeatures) return 16;
   if (base_f32) return rank > 32 && rank <= 64 ? 32 : 16;

@@ -238,9 +238,9 @@ def adapter_linear_backward(dY: Tensor, X: Tensor | QuantizedActivations | None,
     """(dX, d_down, d_up) of ``adapter_linear``; the gradient by its base is dY.
 
     X may be given in 8 bits; with ``need_dw=False`` it is not read and may be
-    None.  ``low``: what ``return_low`` gave (computed anew from X otherwise).  ``base_dx``: the shared projection's part of
-    dX, added in fp32 before the one rounding to ``dx_dtype`` (default: the
-    adapters').  d_down and d_up are in ``grad_dtype`` (default: the
+    None.  ``low``: what ``return_low`` gave (computed anew from X otherwise).
+    ``base_dx``: the shared projection's part of dX, added in fp32 before the
+    one rounding to ``dx_dtype`` (default: the adapters').  d_down and d_up are in ``grad_dtype`` (default: the
     adapters'), zero for an adapter without tokens.  Infinities and NaN: as in
     ``adapter_linear``."""
     op = "adapter_linear_backward"

@@ -56,7 +56,8 @@ class QuantizedActivations:
             padded = -(-k // 16) * 16  # whole 16-byte vectors are read, of the last row too
             end = self.codes.storage_offset() + (n - 1) * self.codes.stride(0) + padded
             if end > self.codes.untyped_storage().nbytes():
-                raise ValueError(f"codes must have rows padded to 16 bytes: the last row's memory ends before column {padded}")
+                raise ValueError("codes must have rows padded to 16 bytes: the last row's memory ends before "
+                                 f"column {padded}")
             if (n > 1 and self.steps.stride(1) != 1) or (self.steps.shape[0] > 1 and self.steps.stride(0) < n):
                 raise ValueError("steps must be row-major")
 

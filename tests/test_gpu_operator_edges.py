@@ -393,3 +393,26 @@ def test_results_beside_their_inputs():
     assert torch.equal(adapter_linear(xv, a, plan, base=bv, out=ov), want)
     assert torch.equal(wide[:, :320], x) and torch.equal(bv, base)
     assert torch.equal(adapter_linear(xv, a, plan, base=bv, out=bv), want) and torch.equal(wide[:, :320], x)
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("k", [131080, 131073, 1 << 19, (1 << 19) + 8, 1 << 20])
+@pytest.mark.parametrize("t,rank", [(2, 20), (2100, 8)])
+def test_long_contractions_to_16_bits(dt, k, t, rank):
+    """16-bit results without low stay at their own rounding, on both sides of the length of one sum."""
+    if t > 100 and k > 140_000:
+        t = 60
+    gen = torch.Generator(device=DEV).manual_seed(k + rank)
+    x = (torch.rand(t, k, generator=gen, device=DEV) + 0.5).to(dt)
+    down = ((torch.rand(2, rank, k, generator=gen, device=DEV) + 0.5) * 2**-14).to(dt)
+    up = torch.full((2, rank, 72), 2.0**-6, dtype=dt, device=DEV)
+    ids = torch.arange(t, device=DEV) % 2
+    y = adapter_linear(x, LowRankAdapters(down=down, up=up), adapter_plan(ids, 2))
+    low = torch.zeros(t, rank, dtype=torch.float64, device=DEV)
+    for g in range(2):
+        for c in range(0, k, 1 << 17):
+            low[ids == g] += x[ids == g, c : c + (1 << 17)].double() @ down[g, :, c : c + (1 << 17)].double().t()
+    want = low.sum(1, keepdim=True).expand(t, 72) * 2.0**-6
+    # 128 products in a part, two truncations each; low in two terms; sums over parts, warps, CTAs and ranks
+    slack = want * (128 * 2 * 2.0**-23 + 2.0**-17 + (rank + 24) * 2.0**-23)
+    assert bool(((y.double() - want).abs() <= slack + (want + slack) * _half(dt) * 1.01).all())
