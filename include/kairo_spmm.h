@@ -539,6 +539,47 @@ KAIRO_API kairo_status kairo_gather_probe(const void* buffer, size_t buffer_byte
                                           int32_t iterations, double* gb_per_s, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Softmax cross entropy of hidden states x (tokens x dim) against a
+ * vocabulary table w (vocab x dim), without keeping the logits (no counterpart
+ * in the reference).
+ *   z[t, v] = scale * x[t] . w[v],  lse[t] = log sum_v exp z[t, v],
+ *   loss[t] = lse[t] - z[t, targets[t]]
+ * x and w f16 or bf16 (one dtype), any alignment of their type (rows that are not
+ * 16-byte aligned are copied first); targets int32 or int64 (target_bytes);
+ * one outside [0, vocab) counts for nothing: loss 0, no gradient.
+ *   kairo_vocab_loss           loss (tokens for KAIRO_REDUCTION_NONE, else one
+ *                              number; MEAN divides by the targets that count)
+ *                              and lse (tokens), fp32
+ *   kairo_vocab_loss_backward  dx (tokens x dim) and dw (vocab x dim) in x's
+ *                              dtype, either may be NULL; grad: the gradient by
+ *                              the loss (tokens for NONE, else one number); lse
+ *                              from the forward call.  A token that does not
+ *                              count has a dx of zeros and does not enter dw.
+ * The workspace (256-byte aligned) depends on the sizes and on whether rows are
+ * aligned; its contents do not outlive a call.  error_word: a device word that
+ * receives a device error (a wait that ran out), as a workspace header's; it is
+ * not cleared.  All asynchronous on `stream`.
+ * ---------------------------------------------------------------------- */
+typedef enum kairo_reduction {
+  KAIRO_REDUCTION_NONE = 0,
+  KAIRO_REDUCTION_SUM = 1,
+  KAIRO_REDUCTION_MEAN = 2
+} kairo_reduction;
+KAIRO_API kairo_status kairo_vocab_loss_workspace_size(const void* x, int64_t ldx, const void* w, int64_t ldw,
+                                                       int64_t tokens, int64_t vocab, int64_t dim, int32_t backward,
+                                                       size_t* bytes);
+KAIRO_API kairo_status kairo_vocab_loss(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t tokens,
+                                        int64_t vocab, int64_t dim, kairo_dtype dtype, const void* targets,
+                                        int32_t target_bytes, float scale, int32_t reduction, float* loss, float* lse,
+                                        void* workspace, size_t workspace_bytes, unsigned* error_word, void* stream);
+KAIRO_API kairo_status kairo_vocab_loss_backward(const float* grad, const void* x, int64_t ldx, const void* w,
+                                                 int64_t ldw, int64_t tokens, int64_t vocab, int64_t dim,
+                                                 kairo_dtype dtype, const void* targets, int32_t target_bytes,
+                                                 float scale, int32_t reduction, const float* lse, void* dx,
+                                                 int64_t lddx, void* dw, int64_t lddw, void* workspace,
+                                                 size_t workspace_bytes, unsigned* error_word, void* stream);
+
+/* ------------------------------------------------------------------------
  * Dense A (M x K, leading dimension lda) -> tiles (num_tiles, tile, tile) in
  * COO order, zero-padding tiles that cross the right/bottom edge.  Replaces
  * the per-tile host loop of _dense_to_block_sparse (kairo/ops/spmm.py:16-55).

@@ -236,6 +236,14 @@ _SIGNATURES = {
                                               c_int64, c_float, c_void_p, c_int64, c_int32, c_int32, c_void_p,
                                               c_size_t, c_void_p]),
     "kairo_embedding_grad_workspace_size": (c_int32, [c_int64, c_int64, c_int32, POINTER(c_size_t)]),
+    "kairo_vocab_loss_workspace_size": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64,
+                                                  c_int32, POINTER(c_size_t)]),
+    "kairo_vocab_loss": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int32, c_void_p,
+                                   c_int32, c_float, c_int32, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p,
+                                   c_void_p]),
+    "kairo_vocab_loss_backward": (c_int32, [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64,
+                                            c_int32, c_void_p, c_int32, c_float, c_int32, c_void_p, c_void_p, c_int64,
+                                            c_void_p, c_int64, c_void_p, c_size_t, c_void_p, c_void_p]),
     "kairo_gather_probe": (c_int32, [c_void_p, c_size_t, c_uint32, c_int32, POINTER(ctypes.c_double), c_void_p]),
     "kairo_dense_to_tiles": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int32,
                                        c_int32, c_void_p, c_void_p]),
@@ -382,6 +390,24 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
         return buf
 
 
+_error_words: dict[tuple[int, int], torch.Tensor] = {}
+
+
+def error_word(index: int) -> torch.Tensor:
+    """The 256 zero-initialised bytes whose first word takes the device errors
+    of operators on the current stream of device ``index`` that bring their own
+    workspace to every call.  Kept for good: captured graphs may write it."""
+    key = (index, torch._C._cuda_getCurrentRawStream(index))
+    word = _error_words.get(key)
+    if word is None:
+        with _ws_lock:
+            word = _error_words.get(key)
+            if word is None:
+                word = torch.zeros(256, dtype=torch.uint8, device=torch.device("cuda", index))
+                _error_words[key] = word
+    return word
+
+
 def read_workspace_error(ws: torch.Tensor, clear: bool = True) -> int:
     code = c_uint32(0)
     check(lib().kairo_workspace_error(ws.data_ptr(), 1 if clear else 0, ctypes.byref(code),
@@ -426,4 +452,9 @@ def pending_device_error(device: torch.device | int | None = None, clear: bool =
         dev = torch.device("cuda", device)
     else:
         dev = torch.device(device)
-    return read_workspace_error(workspace(0, dev), clear=clear)
+    code = read_workspace_error(workspace(0, dev), clear=clear)
+    word = _error_words.get((dev.index if dev.index is not None else torch.cuda.current_device(),
+                             torch.cuda.current_stream(dev).cuda_stream))
+    if word is not None and (code == 0 or clear):
+        code = code or read_workspace_error(word, clear=clear)
+    return code

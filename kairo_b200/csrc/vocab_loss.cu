@@ -1,0 +1,682 @@
+// Softmax cross entropy of hidden states against a vocabulary table, without
+// keeping the logits, and its gradients.
+//
+//   z[t, v] = scale * X[t] . W[v]            X: tokens x dim, W: vocab x dim
+//   lse[t]  = log sum_v exp z[t, v]
+//   loss[t] = lse[t] - z[t, y_t]             0 where y_t is outside [0, vocab)
+//   G[t, v] = f[t] * (exp(z[t, v] - lse[t]) - [v = y_t])
+//   dX = scale * G W,   dW = scale * G^T X
+// with f[t] the gradient by token t's loss (0 where the token does not count).
+//
+// Forward: one pass of k_pair_gemm over W.  A thread of its epilogue owns one
+// token of the tile; it keeps the running maximum and sum of its columns (base
+// 2) and picks the target's logit as it goes by, so 8 bytes leave the SM per
+// token and 128 columns.  k_lse joins them.
+//
+// Backward: pieces of the vocabulary, as many columns as keep a 16-bit G of
+// all tokens within kPieceBytes.  Per piece the logits are formed again and
+// leave as G; dX += G W_piece and dW_piece = G^T X read it as it lies.  That is
+// 8 tokens * vocab * dim operations for the 6 that logits kept in memory would
+// need; it keeps 2 * tokens bytes a column of the piece instead of 4 * tokens * vocab.
+//
+// Rounding.  z, the maxima, sums and lse are fp32.  G is rounded once to the
+// operands' 16 bits, as an operand of both products must be: relative to each
+// entry 2^-9 (bf16) or 2^-12, as the results' own rounding.  The factor that all tokens
+// share (the gradient by a mean or a sum) stays out of G and is applied to the
+// fp32 sums: -1 + p of a target is then near -1, which rounds exactly, where f *
+// (-1 + p) would round every target's entry alike.  In fp16 G also carries 2^15,
+// so that probabilities down to 2^-39 are not lost.
+#include <algorithm>
+#include <cmath>
+
+#include "convert.cuh"
+#include "pair_gemm.cuh"
+
+namespace kairo {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int64_t kPieceBytes = 512LL << 20;
+constexpr float kHalfLift = 32768.f;  // 2^15, see above
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Token targets, int32 or int64.
+struct Targets {
+  const void* p;
+  int bytes;
+  __device__ __forceinline__ int64_t operator[](int64_t i) const {
+    return bytes == 8 ? static_cast<const int64_t*>(p)[i] : static_cast<int64_t>(static_cast<const int32_t*>(p)[i]);
+  }
+};
+
+// ------------------------------------------------------------ epilogues
+
+// Running maximum and sum of exp2 of one token's columns.
+struct StatsEpi {
+  struct Args {
+    float2* part;   // [slots][tokens]
+    float* target;  // [tokens], the target's logit
+    Targets ids;
+    int tokens, vocab;
+    float scale;
+    int by_cluster;  // one row of tiles: a CTA's tiles share a slot
+  };
+  const Args& a;
+  int row, part, mt = -1;
+  int64_t id = -1;
+  float m = -INFINITY, s = 0.f;
+
+  __device__ StatsEpi(const Args& args, int row_in_tile, int p) : a(args), row(row_in_tile), part(p) {}
+
+  __device__ __forceinline__ void flush(int token, int64_t slot) {
+    if (token < a.tokens) a.part[slot * a.tokens + token] = make_float2(m, s);
+    m = -INFINITY;
+    s = 0.f;
+  }
+
+  __device__ void tile(int tm, int tn, float (&v)[kPairEpiCols]) {
+    const int token = tm * kPairTileM + row;
+    if (__all_sync(0xffffffffu, token >= a.tokens)) return;
+    if (tm != mt) {
+      mt = tm;
+      id = token < a.tokens ? a.ids[token] : -1;
+    }
+    const int col0 = tn * kPairTileN + part * kPairEpiCols;
+    const int64_t at = id - col0;
+    const bool here = id >= 0 && id < a.vocab && at >= 0 && at < kPairEpiCols;
+    if (__any_sync(0xffffffffu, here)) {
+      float z = 0.f;
+#pragma unroll
+      for (int j = 0; j < kPairEpiCols; ++j)
+        if (at == j) z = v[j];
+      if (here && token < a.tokens) a.target[token] = z * a.scale;
+    }
+    const float k = a.scale * kLog2e;
+#pragma unroll
+    for (int j = 0; j < kPairEpiCols; ++j) v[j] *= k;
+    if (col0 + kPairEpiCols > a.vocab) {
+#pragma unroll
+      for (int j = 0; j < kPairEpiCols; ++j)
+        if (col0 + j >= a.vocab) v[j] = -INFINITY;
+    }
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < kPairEpiCols; ++j) top = fmaxf(top, v[j]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum[4] = {s * ex2(m - ref), 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < kPairEpiCols; ++j) sum[j & 3] += ex2(v[j] - ref);
+    m = top;
+    s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    if (!a.by_cluster) flush(token, static_cast<int64_t>(tn) * (kPairTileN / kPairEpiCols) + part);
+  }
+
+  __device__ void done() {
+    if (a.by_cluster) flush(row, static_cast<int64_t>(blockIdx.x >> 1) * (kPairTileN / kPairEpiCols) + part);
+  }
+};
+
+// 16 results of one row, rounded to T, at p: 16-byte stores where `vec`, the first `n` one by one otherwise.
+template <typename T>
+__device__ __forceinline__ void put16(T* p, const float* v, int n, bool vec) {
+  if (vec && n >= 16) {
+    float w[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) w[j] = v[j];
+    store_f32<T, 16>(p, w);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j < n) p[j] = from_f32<T>(v[j]);
+  }
+}
+
+// G of one piece of the vocabulary.
+template <typename T>
+struct GradEpi {
+  struct Args {
+    T* g;              // [tokens][ldg]
+    int64_t ldg;       // columns of the piece, a multiple of the tile
+    const float* lse;
+    const float* f;    // the token's factor, 0 where it does not count
+    Targets ids;
+    int tokens, vocab, v0;
+    float scale;
+  };
+  const Args& a;
+  int row, part, mt = -1;
+  int64_t id = -1;
+  float lse2 = 0.f, f = 0.f;
+
+  __device__ GradEpi(const Args& args, int row_in_tile, int p) : a(args), row(row_in_tile), part(p) {}
+
+  __device__ void tile(int tm, int tn, float (&v)[kPairEpiCols]) {
+    const int token = tm * kPairTileM + row;
+    if (tm != mt) {
+      mt = tm;
+      if (token < a.tokens) {
+        id = a.ids[token];
+        lse2 = a.lse[token] * kLog2e;
+        f = a.f[token];
+      }
+    }
+    const int col0 = tn * kPairTileN + part * kPairEpiCols;  // in the piece
+    const float k = a.scale * kLog2e;
+    const int64_t at = id - (a.v0 + col0);
+#pragma unroll
+    for (int j = 0; j < kPairEpiCols; ++j) v[j] = ex2(fmaf(v[j], k, -lse2)) * f;
+    if (__any_sync(0xffffffffu, at >= 0 && at < kPairEpiCols)) {
+#pragma unroll
+      for (int j = 0; j < kPairEpiCols; ++j)
+        if (at == j) v[j] -= f;
+    }
+    // a token that does not count has no gradient, whatever its logits are
+    const int n = f == 0.f ? 0 : a.vocab - (a.v0 + col0);
+    if (n < kPairEpiCols) {
+#pragma unroll
+      for (int j = 0; j < kPairEpiCols; ++j)
+        if (j >= n) v[j] = 0.f;
+    }
+    if (token >= a.tokens) return;
+    T* dst = a.g + static_cast<int64_t>(token) * a.ldg + col0;
+#pragma unroll
+    for (int c = 0; c < kPairEpiCols; c += 16) put16<T>(dst + c, v + c, 16, true);
+  }
+
+  __device__ void done() {}
+};
+
+// A sum over pieces (fp32, `acc`), the last one times *factor as T.
+template <typename T>
+struct SumEpi {
+  struct Args {
+    T* out;
+    int64_t ldo;
+    float* acc;        // [rows][ldacc], 16-byte aligned rows; read unless first, written unless last
+    int64_t ldacc;
+    const float* factor;
+    int rows, cols;
+    int first, last, vec;
+  };
+  const Args& a;
+  int row, part;
+  float factor;
+
+  __device__ SumEpi(const Args& args, int row_in_tile, int p) : a(args), row(row_in_tile), part(p), factor(*args.factor) {}
+
+  __device__ void tile(int tm, int tn, float (&v)[kPairEpiCols]) {
+    const int r = tm * kPairTileM + row;
+    const int col0 = tn * kPairTileN + part * kPairEpiCols;
+    const int n = a.cols - col0;
+    if (r >= a.rows || n <= 0) return;
+    float4* acc = reinterpret_cast<float4*>(a.acc + static_cast<int64_t>(r) * a.ldacc + col0);
+    if (!a.first) {
+#pragma unroll
+      for (int j = 0; j < kPairEpiCols / 4; ++j)
+        if (4 * j < n) {
+          const float4 w = acc[j];
+          v[4 * j] += w.x;
+          v[4 * j + 1] += w.y;
+          v[4 * j + 2] += w.z;
+          v[4 * j + 3] += w.w;
+        }
+    }
+    if (!a.last) {
+#pragma unroll
+      for (int j = 0; j < kPairEpiCols / 4; ++j)
+        if (4 * j < n) acc[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+      return;
+    }
+    T* dst = a.out + static_cast<int64_t>(r) * a.ldo + col0;
+#pragma unroll
+    for (int c = 0; c < kPairEpiCols; c += 16) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[c + j] *= factor;
+      put16<T>(dst + c, v + c, n - c, a.vec != 0);
+    }
+  }
+
+  __device__ void done() {}
+};
+
+// ------------------------------------------------------------ small kernels
+
+enum Reduction : int { kNone = KAIRO_REDUCTION_NONE, kSum = KAIRO_REDUCTION_SUM, kMean = KAIRO_REDUCTION_MEAN };
+
+// Sum of `v` over the CTA (any number of whole warps), in a fixed order; every thread gets it.
+__device__ float cta_sum(float v) {
+  __shared__ float w[32];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) w[threadIdx.x >> 5] = v;
+  __syncthreads();
+  const int nw = blockDim.x >> 5;
+  float t = (threadIdx.x & 31) < nw ? w[threadIdx.x & 31] : 0.f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  return t;
+}
+
+// lse and loss of 32 tokens a CTA from their partial maxima and sums; the CTA that finishes last
+// reduces the losses, always in the same order.
+__global__ void __launch_bounds__(1024) k_lse(const float2* __restrict__ part, int slots,
+                                              const float* __restrict__ target, Targets ids, int tokens, int vocab,
+                                              int reduction, float* __restrict__ each, float* __restrict__ lse,
+                                              float* __restrict__ loss, unsigned* ticket) {
+  __shared__ float2 sm[32][33];
+  __shared__ bool last;
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int t = blockIdx.x * 32 + x;
+  float m = -INFINITY, s = 0.f;
+  if (t < tokens) {
+    auto join = [&](float2 p) {
+      const float top = fmaxf(m, p.x);
+      const float ref = top == -INFINITY ? 0.f : top;
+      s = s * ex2(m - ref) + p.y * ex2(p.x - ref);
+      m = top;
+    };
+    int i = y;
+    for (; i + 96 < slots; i += 128) {
+      float2 p[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) p[u] = part[static_cast<int64_t>(i + 32 * u) * tokens + t];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) join(p[u]);
+    }
+    for (; i < slots; i += 32) join(part[static_cast<int64_t>(i) * tokens + t]);
+  }
+  sm[y][x] = make_float2(m, s);
+  __syncthreads();
+  if (y == 0 && t < tokens) {
+    float top = m;
+    for (int u = 1; u < 32; ++u) top = fmaxf(top, sm[u][x].x);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    for (int u = 0; u < 32; ++u) sum += sm[u][x].y * ex2(sm[u][x].x - ref);
+    const float l = (ref + log2f(sum)) * kLn2;
+    const int64_t id = ids[t];
+    const float v = id >= 0 && id < vocab ? l - target[t] : 0.f;
+    lse[t] = l;
+    each[t] = v;
+  }
+  if (reduction == kNone) return;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(ticket, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  float sum = 0.f, count = 0.f;
+  for (int i = threadIdx.x; i < tokens; i += blockDim.x) {
+    sum += __ldcg(each + i);
+    const int64_t id = ids[i];
+    count += id >= 0 && id < vocab ? 1.f : 0.f;
+  }
+  sum = cta_sum(sum);
+  count = cta_sum(count);
+  if (threadIdx.x == 0) *loss = reduction == kMean ? sum / fmaxf(count, 1.f) : sum;
+}
+
+// Rows of 16-bit values with 16-byte alignment: dst (rows x ldd, ldd a multiple of 8) = src, zeros
+// behind column `cols` and, where `ids` is given, in the rows of tokens that do not count.
+// CTA 0 writes the tokens' factors and the one they share (`factor`) first.
+struct PrepArgs {
+  const float* grad;  // by the loss: one number, or every token's (kNone)
+  Targets ids;
+  int tokens, vocab, reduction;
+  float scale, lift;
+  float* f;
+  float* factor;
+};
+
+__device__ void prep_factors(const PrepArgs& p) {
+  float count = 0.f, top = 0.f;
+  for (int i = threadIdx.x; i < p.tokens; i += blockDim.x) {
+    const int64_t id = p.ids[i];
+    if (id >= 0 && id < p.vocab) {
+      count += 1.f;
+      if (p.reduction == kNone) top = fmaxf(top, fabsf(p.grad[i]));
+    }
+  }
+  float shared_factor;
+  if (p.reduction == kNone) {
+    // the largest factor's power of two, so that factors of any size keep their digits in 16 bits
+    __shared__ float tops[32];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+    for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) top = fmaxf(top, tops[i]);
+    int e = 0;
+    if (top > 0.f && isfinite(top)) frexpf(top, &e);
+    shared_factor = ldexpf(1.f, max(-100, min(100, e)));
+  } else {
+    count = cta_sum(count);
+    shared_factor = *p.grad / (p.reduction == kMean ? fmaxf(count, 1.f) : 1.f);
+  }
+  for (int i = threadIdx.x; i < p.tokens; i += blockDim.x) {
+    const int64_t id = p.ids[i];
+    const float own = p.reduction == kNone ? p.grad[i] / shared_factor : 1.f;
+    p.f[i] = id >= 0 && id < p.vocab ? own * p.lift : 0.f;
+  }
+  if (threadIdx.x == 0) *p.factor = shared_factor * p.scale / p.lift;
+}
+
+__global__ void __launch_bounds__(256) k_rows(const uint16_t* __restrict__ src, int64_t lds, int64_t rows, int64_t cols,
+                                              uint16_t* __restrict__ dst, int64_t ldd, int vec, Targets ids, int vocab,
+                                              PrepArgs prep) {
+  int cta = blockIdx.x, ctas = gridDim.x;
+  if (prep.f) {
+    if (cta == 0) return prep_factors(prep);
+    --cta;
+    --ctas;
+  }
+  const int64_t pieces = ldd / 8, total = rows * pieces;
+  for (int64_t i = static_cast<int64_t>(cta) * blockDim.x + threadIdx.x; i < total;
+       i += static_cast<int64_t>(ctas) * blockDim.x) {
+    const int64_t r = i / pieces, c = (i - r * pieces) * 8;
+    uint4 w = make_uint4(0u, 0u, 0u, 0u);
+    bool live = true;
+    if (ids.p) {
+      const int64_t id = ids[r];
+      live = id >= 0 && id < vocab;
+    }
+    if (live) {
+      const uint16_t* p = src + r * lds + c;
+      if (vec && c + 8 <= cols) {
+        w = *reinterpret_cast<const uint4*>(p);
+      } else {
+        uint32_t h[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[j] = c + j < cols ? p[j] : 0u;
+        w = make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
+      }
+    }
+    *reinterpret_cast<uint4*>(dst + r * ldd + c) = w;
+  }
+}
+
+// ------------------------------------------------------------ host side
+
+struct Problem {
+  const void* x;
+  int64_t ldx;
+  const void* w;
+  int64_t ldw;
+  int64_t tokens, vocab, dim;
+  kairo_dtype dt;
+  Targets ids;
+  float scale;
+  int reduction;
+};
+
+bool rows_aligned(const void* p, int64_t ld, int64_t rows) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (ld % 8 == 0 || rows <= 1);
+}
+
+int64_t tiles(int64_t n) { return ceil_div64(n, kPairTileN); }
+
+// Columns of one piece of the backward pass: pieces of equal size, whole tiles.
+int64_t piece_cols(int64_t tokens, int64_t vocab) {
+  const int64_t most = std::max<int64_t>(1, kPieceBytes / (2 * std::max<int64_t>(1, tokens) * kPairTileN)) * kPairTileN;
+  const int64_t pieces = ceil_div64(vocab, most);
+  return tiles(ceil_div64(vocab, pieces)) * kPairTileN;
+}
+
+struct LossWs {
+  size_t ticket, target, each, part, x, w, total;
+};
+
+// Everything a call may need, whether or not its rows are aligned: the copies come last.
+LossWs loss_ws(const Problem& p) {
+  LossWs o{};
+  size_t at = kWorkspaceHeaderBytes;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at = align_up(at + bytes, 256);
+    return here;
+  };
+  o.ticket = 128;
+  o.target = take(4 * static_cast<size_t>(p.tokens));
+  o.each = take(4 * static_cast<size_t>(p.tokens));
+  const int64_t slots = 2 * tiles(p.vocab);
+  o.part = take(8 * static_cast<size_t>(p.tokens) * static_cast<size_t>(slots));
+  const size_t ld = align_up(static_cast<size_t>(p.dim), 8);
+  if (!rows_aligned(p.x, p.ldx, p.tokens)) o.x = take(2 * ld * static_cast<size_t>(p.tokens));
+  if (!rows_aligned(p.w, p.ldw, p.vocab)) o.w = take(2 * ld * static_cast<size_t>(p.vocab));
+  o.total = at;
+  return o;
+}
+
+struct GradWs {
+  size_t f, factor, acc, x, w, g, total;
+  int64_t cols;
+};
+
+GradWs grad_ws(const Problem& p) {
+  GradWs o{};
+  size_t at = kWorkspaceHeaderBytes;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at = align_up(at + bytes, 256);
+    return here;
+  };
+  const size_t ld = align_up(static_cast<size_t>(p.dim), 8);
+  o.cols = piece_cols(p.tokens, p.vocab);
+  o.factor = 128;
+  o.f = take(4 * static_cast<size_t>(p.tokens));
+  o.x = take(2 * ld * static_cast<size_t>(p.tokens));
+  if (o.cols < p.vocab) o.acc = take(4 * ld * static_cast<size_t>(p.tokens));
+  if (!rows_aligned(p.w, p.ldw, p.vocab)) o.w = take(2 * ld * static_cast<size_t>(p.vocab));
+  o.g = take(2 * static_cast<size_t>(p.tokens) * static_cast<size_t>(o.cols));
+  o.total = at;
+  return o;
+}
+
+kairo_status check_problem(const Problem& p) {
+  if (p.tokens < 0 || p.vocab < 1 || p.dim < 1) return fail(KAIRO_STATUS_INVALID_VALUE, "invalid size");
+  if (p.tokens > 0x7fffff00LL || p.vocab > 0x7fffff00LL || p.dim > 0x7fffff00LL ||
+      tiles(p.tokens) * tiles(p.vocab) > 0x7fffffffLL || tiles(p.dim) * tiles(std::max(p.tokens, p.vocab)) > 0x7fffffffLL)
+    return fail(KAIRO_STATUS_NOT_SUPPORTED, "sizes beyond 2^31 tiles");
+  if (p.dt != KAIRO_DTYPE_F16 && p.dt != KAIRO_DTYPE_BF16)
+    return fail(KAIRO_STATUS_INVALID_VALUE, "hidden states and table must be f16 or bf16");
+  if (p.ldx < p.dim || p.ldw < p.dim) return fail(KAIRO_STATUS_INVALID_VALUE, "leading dimension too small");
+  if (p.reduction < kNone || p.reduction > kMean) return fail(KAIRO_STATUS_INVALID_VALUE, "unknown reduction");
+  if (p.ids.bytes != 4 && p.ids.bytes != 8) return fail(KAIRO_STATUS_INVALID_VALUE, "targets must be int32 or int64");
+  return KAIRO_STATUS_SUCCESS;
+}
+
+// `src` with 16-byte aligned rows: itself, or a copy at `dst`.
+kairo_status aligned_rows(const void** src, int64_t* ld, int64_t rows, int64_t cols, uint8_t* dst, cudaStream_t s) {
+  if (rows_aligned(*src, *ld, rows)) return KAIRO_STATUS_SUCCESS;
+  const int64_t ldd = static_cast<int64_t>(align_up(static_cast<size_t>(cols), 8));
+  const int64_t work = ceil_div64(rows * (ldd / 8), 256);
+  const int grid = static_cast<int>(std::min<int64_t>(work, device_sm_count(current_device()) * 16));
+  k_rows<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(*src), *ld, rows, cols, reinterpret_cast<uint16_t*>(dst), ldd,
+                              0, Targets{nullptr, 8}, 0, PrepArgs{});
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "launch of the row copy");
+  *src = dst;
+  *ld = ldd;
+  return KAIRO_STATUS_SUCCESS;
+}
+
+// Rows of tiles visited together: their part of the row operand takes about a quarter of the L2.
+int group_rows(int64_t tiles_m, int64_t k) {
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(tiles_m, (32LL << 20) / (kPairTileM * 2 * std::max<int64_t>(k, 64)))));
+}
+
+// Stages of a segment.  Logits: 256 k, so that lse and losses are as exact as fp32 sums (7e-7 of a
+// logit at worst).  The gradients are rounded to 16 bits: 4096 k leave 1e-5.
+constexpr int kSegLogits = 4, kSegGrads = 64;
+
+PairShape shape_of(int64_t rows, int64_t cols, int64_t k, int seg) {
+  PairShape s;
+  s.seg = seg;
+  s.tiles_m = static_cast<int>(tiles(rows));
+  s.tiles_n = static_cast<int>(tiles(cols));
+  s.ksteps = static_cast<int>(ceil_div64(k, kPairK));
+  s.group_m = group_rows(s.tiles_m, k);
+  return s;
+}
+
+template <typename T, int FMT>
+kairo_status run_loss(Problem p, float* loss, float* lse, uint8_t* ws, unsigned* err, cudaStream_t s) {
+  const LossWs o = loss_ws(p);
+  kairo_status st = aligned_rows(&p.x, &p.ldx, p.tokens, p.dim, ws + o.x, s);
+  if (st == KAIRO_STATUS_SUCCESS) st = aligned_rows(&p.w, &p.ldw, p.vocab, p.dim, ws + o.w, s);
+  if (st) return st;
+  unsigned* ticket = reinterpret_cast<unsigned*>(ws + o.ticket);
+  if (p.reduction != kNone) {
+    const cudaError_t e = cudaMemsetAsync(ticket, 0, sizeof(unsigned), s);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync(ticket)");
+  }
+  CUtensorMap ma, mb;
+  st = pair_operand_map(&ma, p.x, p.dt, false, p.tokens, p.dim, p.ldx, "hidden states");
+  if (st == KAIRO_STATUS_SUCCESS) st = pair_operand_map(&mb, p.w, p.dt, false, p.vocab, p.dim, p.ldw, "vocabulary table");
+  if (st) return st;
+  const PairShape sh = shape_of(p.tokens, p.vocab, p.dim, kSegLogits);
+  const int clusters = std::min(sh.tiles_m * sh.tiles_n, std::max(1, device_sm_count(current_device()) / 2));
+  StatsEpi::Args a{reinterpret_cast<float2*>(ws + o.part), reinterpret_cast<float*>(ws + o.target), p.ids,
+                   static_cast<int>(p.tokens), static_cast<int>(p.vocab), p.scale, sh.tiles_m == 1};
+  st = launch_pair_gemm<FMT, false, false, StatsEpi>(ma, mb, sh, err, a, s);
+  if (st) return st;
+  const int slots = 2 * (a.by_cluster ? clusters : sh.tiles_n);
+  k_lse<<<static_cast<int>(ceil_div64(p.tokens, 32)), 1024, 0, s>>>(
+      a.part, slots, a.target, p.ids, a.tokens, a.vocab, p.reduction,
+      p.reduction == kNone ? loss : reinterpret_cast<float*>(ws + o.each), lse, loss, ticket);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "launch of k_lse");
+}
+
+template <typename T, int FMT>
+kairo_status run_grad(Problem p, const float* grad, const float* lse, T* dx, int64_t lddx, T* dw, int64_t lddw,
+                      uint8_t* ws, unsigned* err, cudaStream_t s) {
+  const GradWs o = grad_ws(p);
+  const int64_t ld = static_cast<int64_t>(align_up(static_cast<size_t>(p.dim), 8));
+  kairo_status st = aligned_rows(&p.w, &p.ldw, p.vocab, p.dim, ws + o.w, s);
+  if (st) return st;
+  float* f = reinterpret_cast<float*>(ws + o.f);
+  float* factor = reinterpret_cast<float*>(ws + o.factor);
+  void* x = ws + o.x;
+  {
+    PrepArgs pa{grad, p.ids, static_cast<int>(p.tokens), static_cast<int>(p.vocab), p.reduction, p.scale,
+                FMT == 0 ? kHalfLift : 1.f, f, factor};
+    const int64_t work = ceil_div64(p.tokens * (ld / 8), 256);
+    const int grid = 1 + static_cast<int>(std::min<int64_t>(work, device_sm_count(current_device()) * 8));
+    k_rows<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(p.x), p.ldx, p.tokens, p.dim, static_cast<uint16_t*>(x), ld,
+                                rows_aligned(p.x, p.ldx, p.tokens) ? 1 : 0, p.ids, static_cast<int>(p.vocab), pa);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(e, "launch of the tokens' factors");
+  }
+  T* g = reinterpret_cast<T*>(ws + o.g);
+  float* acc = reinterpret_cast<float*>(ws + o.acc);
+  CUtensorMap mx, mxt, mg, mgt;
+  st = pair_operand_map(&mx, x, p.dt, false, p.tokens, p.dim, ld, "hidden states");
+  if (st == KAIRO_STATUS_SUCCESS) st = pair_operand_map(&mxt, x, p.dt, true, p.dim, p.tokens, ld, "hidden states");
+  if (st == KAIRO_STATUS_SUCCESS) st = pair_operand_map(&mg, g, p.dt, false, p.tokens, o.cols, o.cols, "gradient of the logits");
+  if (st == KAIRO_STATUS_SUCCESS) st = pair_operand_map(&mgt, g, p.dt, true, o.cols, p.tokens, o.cols, "gradient of the logits");
+  if (st) return st;
+  for (int64_t v0 = 0; v0 < p.vocab; v0 += o.cols) {
+    const int64_t n = std::min(o.cols, p.vocab - v0);
+    const T* w = static_cast<const T*>(p.w) + v0 * p.ldw;
+    CUtensorMap mw, mwt;
+    st = pair_operand_map(&mw, w, p.dt, false, n, p.dim, p.ldw, "vocabulary table");
+    if (st == KAIRO_STATUS_SUCCESS) st = pair_operand_map(&mwt, w, p.dt, true, p.dim, n, p.ldw, "vocabulary table");
+    if (st) return st;
+    typename GradEpi<T>::Args ga{g, o.cols, lse, f, p.ids, static_cast<int>(p.tokens), static_cast<int>(p.vocab),
+                                 static_cast<int>(v0), p.scale};
+    st = launch_pair_gemm<FMT, false, false, GradEpi<T>>(mx, mw, shape_of(p.tokens, n, p.dim, kSegLogits), err, ga, s);
+    if (st) return st;
+    if (dx) {
+      typename SumEpi<T>::Args sa{dx, lddx, acc, ld, factor, static_cast<int>(p.tokens), static_cast<int>(p.dim),
+                                  v0 == 0, v0 + n == p.vocab, rows_aligned(dx, lddx, p.tokens)};
+      st = launch_pair_gemm<FMT, false, true, SumEpi<T>>(mg, mwt, shape_of(p.tokens, p.dim, n, kSegGrads), err, sa, s);
+      if (st) return st;
+    }
+    if (dw) {
+      T* out = dw + v0 * lddw;
+      typename SumEpi<T>::Args sa{out, lddw, acc, ld, factor, static_cast<int>(n), static_cast<int>(p.dim), 1, 1,
+                                  rows_aligned(out, lddw, n)};
+      st = launch_pair_gemm<FMT, true, true, SumEpi<T>>(mgt, mxt, shape_of(n, p.dim, p.tokens, kSegGrads), err, sa, s);
+      if (st) return st;
+    }
+  }
+  return KAIRO_STATUS_SUCCESS;
+}
+
+}  // namespace
+}  // namespace kairo
+
+using namespace kairo;
+
+extern "C" kairo_status kairo_vocab_loss_workspace_size(const void* x, int64_t ldx, const void* w, int64_t ldw,
+                                                        int64_t tokens, int64_t vocab, int64_t dim, int32_t backward,
+                                                        size_t* bytes) {
+  if (!bytes) return fail(KAIRO_STATUS_INVALID_VALUE, "null argument");
+  const Problem p{x, ldx, w, ldw, tokens, vocab, dim, KAIRO_DTYPE_BF16, Targets{nullptr, 8}, 1.f, kNone};
+  const kairo_status st = check_problem(p);
+  if (st) return st;
+  *bytes = backward ? grad_ws(p).total : loss_ws(p).total;
+  return KAIRO_STATUS_SUCCESS;
+}
+
+extern "C" kairo_status kairo_vocab_loss(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t tokens,
+                                         int64_t vocab, int64_t dim, kairo_dtype dtype, const void* targets,
+                                         int32_t target_bytes, float scale, int32_t reduction, float* loss, float* lse,
+                                         void* workspace, size_t workspace_bytes, unsigned* error_word, void* stream) {
+  const Problem p{x, ldx, w, ldw, tokens, vocab, dim, dtype, Targets{targets, target_bytes}, scale, reduction};
+  kairo_status st = check_problem(p);
+  if (st) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (tokens == 0) {
+    if (reduction == kNone) return KAIRO_STATUS_SUCCESS;
+    if (!loss) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+    const cudaError_t e = cudaMemsetAsync(loss, 0, sizeof(float), s);
+    return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "cudaMemsetAsync(loss)");
+  }
+  if (!x || !w || !targets || !loss || !lse || !workspace || !error_word)
+    return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+  if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(KAIRO_STATUS_INVALID_VALUE, "workspace must be 256-byte aligned");
+  if (workspace_bytes < loss_ws(p).total) return fail(KAIRO_STATUS_WORKSPACE_TOO_SMALL, "loss workspace too small");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  return dtype == KAIRO_DTYPE_F16 ? run_loss<__half, 0>(p, loss, lse, ws, error_word, s)
+                                  : run_loss<__nv_bfloat16, 1>(p, loss, lse, ws, error_word, s);
+}
+
+extern "C" kairo_status kairo_vocab_loss_backward(const float* grad, const void* x, int64_t ldx, const void* w,
+                                                  int64_t ldw, int64_t tokens, int64_t vocab, int64_t dim,
+                                                  kairo_dtype dtype, const void* targets, int32_t target_bytes,
+                                                  float scale, int32_t reduction, const float* lse, void* dx,
+                                                  int64_t lddx, void* dw, int64_t lddw, void* workspace,
+                                                  size_t workspace_bytes, unsigned* error_word, void* stream) {
+  const Problem p{x, ldx, w, ldw, tokens, vocab, dim, dtype, Targets{targets, target_bytes}, scale, reduction};
+  kairo_status st = check_problem(p);
+  if (st) return st;
+  if ((dx && lddx < dim) || (dw && lddw < dim)) return fail(KAIRO_STATUS_INVALID_VALUE, "leading dimension too small");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (!dx && !dw) return KAIRO_STATUS_SUCCESS;
+  if (tokens == 0) {
+    if (!dw) return KAIRO_STATUS_SUCCESS;
+    const cudaError_t e = cudaMemset2DAsync(dw, static_cast<size_t>(lddw) * 2, 0, static_cast<size_t>(dim) * 2,
+                                            static_cast<size_t>(vocab), s);
+    return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "cudaMemset2DAsync(dW)");
+  }
+  if (!grad || !x || !w || !targets || !lse || !workspace || !error_word)
+    return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+  if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(KAIRO_STATUS_INVALID_VALUE, "workspace must be 256-byte aligned");
+  if (workspace_bytes < grad_ws(p).total) return fail(KAIRO_STATUS_WORKSPACE_TOO_SMALL, "loss workspace too small");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  return dtype == KAIRO_DTYPE_F16
+             ? run_grad<__half, 0>(p, grad, lse, static_cast<__half*>(dx), lddx, static_cast<__half*>(dw), lddw, ws,
+                                   error_word, s)
+             : run_grad<__nv_bfloat16, 1>(p, grad, lse, static_cast<__nv_bfloat16*>(dx), lddx,
+                                          static_cast<__nv_bfloat16*>(dw), lddw, ws, error_word, s);
+}

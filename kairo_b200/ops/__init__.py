@@ -35,6 +35,7 @@ from kairo_b200.ops.adapters import (
     adapter_plan,
 )
 from kairo_b200.ops.checkpoint import QuantizedActivations, dequantize_activations, quantize_activations
+from kairo_b200.ops.vocab_loss import LinearCrossEntropy, linear_cross_entropy, linear_cross_entropy_backward
 from kairo_b200.ops.spmm import (
     KernelConfig,
     RowGroups,
@@ -93,6 +94,9 @@ __all__ = [
     "QuantizedActivations",
     "dequantize_activations",
     "quantize_activations",
+    "LinearCrossEntropy",
+    "linear_cross_entropy",
+    "linear_cross_entropy_backward",
     "ScaledEmbedding",
     "TokenOrder",
     "embedding_grad",
