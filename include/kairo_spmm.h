@@ -580,6 +580,48 @@ KAIRO_API kairo_status kairo_vocab_loss_backward(const float* grad, const void* 
                                                  size_t workspace_bytes, unsigned* error_word, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Gated projection of a feed-forward block, both weights block-sparse (no
+ * counterpart in the reference): G = X Wg^T, U = X Wu^T, H = act(G) * U.
+ * Wg and Wu are rows x cols with square blocks of 16, 32 or 64, f16 or bf16, in
+ * one block storage (nblocks x block x block, 16-byte aligned).  Block-row i's entries
+ * ent_ptr[i] .. ent_ptr[i + 1] - 1 are four int32 each (16-byte aligned):
+ * block-column, stored block of Wg or -1, stored block of Wu or -1, 0.
+ *   kairo_gated_linear       H (n x rows)
+ *   kairo_gated_linear_grad  dG = dH * U * act'(G) and dU = dH * act(G), G and U
+ *                            formed from X anew, as dP (n x 2 ceil(rows / block)
+ *                            block): block-rows 2i and 2i + 1 are block-row i of
+ *                            dG and of dU, zeros behind the last row
+ * X (n x cols, leading dimension ldx) needs 16-byte aligned rows for more than
+ * 32 tokens.  Sums are fp32, H, dG and dU rounded once.  A value of X that is
+ * not finite makes those results non-finite whose row keeps a block of Wg or Wu in
+ * its column.  error_word: see kairo_vocab_loss; an entry out of range is
+ * recorded there (KAIRO_DEVERR_BAD_INDEX) and counts as empty.  Asynchronous on `stream`.
+ * ---------------------------------------------------------------------- */
+typedef enum kairo_activation {
+  KAIRO_ACTIVATION_SILU = 0,
+  KAIRO_ACTIVATION_GELU = 1,
+  KAIRO_ACTIVATION_GELU_TANH = 2,
+  KAIRO_ACTIVATION_RELU = 3
+} kairo_activation;
+typedef struct kairo_gated {
+  int64_t rows;
+  int64_t cols;
+  int64_t nentries;
+  int64_t nblocks;
+  const int32_t* ent_ptr;
+  const int32_t* entries;
+  const void* blocks;
+  int32_t block;
+  kairo_dtype dtype;
+} kairo_gated;
+KAIRO_API kairo_status kairo_gated_linear(const kairo_gated* w, const void* x, int64_t ldx, int64_t n,
+                                          int32_t activation, void* h, int64_t ldh, unsigned* error_word,
+                                          void* stream);
+KAIRO_API kairo_status kairo_gated_linear_grad(const kairo_gated* w, const void* x, int64_t ldx, int64_t n,
+                                               int32_t activation, const void* dh, int64_t lddh, void* dp,
+                                               int64_t lddp, unsigned* error_word, void* stream);
+
+/* ------------------------------------------------------------------------
  * Dense A (M x K, leading dimension lda) -> tiles (num_tiles, tile, tile) in
  * COO order, zero-padding tiles that cross the right/bottom edge.  Replaces
  * the per-tile host loop of _dense_to_block_sparse (kairo/ops/spmm.py:16-55).

@@ -130,6 +130,22 @@ class KairoBsrStack(Structure):
     ]
 
 
+class KairoGated(Structure):
+    """kairo_gated: the two weights of a gated projection."""
+
+    _fields_ = [
+        ("rows", c_int64),
+        ("cols", c_int64),
+        ("nentries", c_int64),
+        ("nblocks", c_int64),
+        ("ent_ptr", c_void_p),
+        ("entries", c_void_p),
+        ("blocks", c_void_p),
+        ("block", c_int32),
+        ("dtype", c_int32),
+    ]
+
+
 class KairoLibraryError(RuntimeError):
     """The native library is missing, failed to build, or failed to load."""
 
@@ -244,6 +260,10 @@ _SIGNATURES = {
     "kairo_vocab_loss_backward": (c_int32, [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64,
                                             c_int32, c_void_p, c_int32, c_float, c_int32, c_void_p, c_void_p, c_int64,
                                             c_void_p, c_int64, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "kairo_gated_linear": (c_int32, [POINTER(KairoGated), c_void_p, c_int64, c_int64, c_int32, c_void_p, c_int64,
+                                     c_void_p, c_void_p]),
+    "kairo_gated_linear_grad": (c_int32, [POINTER(KairoGated), c_void_p, c_int64, c_int64, c_int32, c_void_p, c_int64,
+                                          c_void_p, c_int64, c_void_p, c_void_p]),
     "kairo_gather_probe": (c_int32, [c_void_p, c_size_t, c_uint32, c_int32, POINTER(ctypes.c_double), c_void_p]),
     "kairo_dense_to_tiles": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int32,
                                        c_int32, c_void_p, c_void_p]),

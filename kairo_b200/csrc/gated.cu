@@ -1,0 +1,716 @@
+// Gated projection of a feed-forward block with block-sparse weights:
+//
+//   G = X Wg^T,  U = X Wu^T,  H = act(G) * U         X: tokens x k, H: tokens x m
+//   dG = dH * U * act'(G),  dU = dH * act(G)         (kairo_gated_linear_grad)
+//
+// both products, the activation and the product of the two in one kernel: G and
+// U never leave the SM.  The backward call forms them again from X (as exact as
+// in the forward pass, where copies kept in 16 bits would cost another rounding
+// and 2 * tokens * m values) and writes dG and dU side by side as the stacked
+// dP of kairo_bsr_sddmm and of the SpMM with the stacked transposed weight:
+// block-rows 2i and 2i + 1 of the stacked matrix are block-row i of Wg and of Wu.
+//
+// Entries.  A block-row's entries are the block-columns where Wg or Wu keeps a
+// block, in column order, each with its two stored blocks (-1: none).  Both
+// products share the entry's panel of X, the larger operand; a missing block is
+// a copy from behind the block storage, which the copy engine fills with zeros.
+//
+// k_gated (tensor cores).  A cluster of two CTAs takes T * 256 tokens and one
+// block-row: an entry is one tcgen05.mma (cta_group::2) per 16 k and 256 tokens with
+// M = 256 tokens and N = 2 * BM outputs; the even CTA's shared memory holds
+// the gate block, the odd one's the up block, and each holds its own tokens'
+// panels of X.  With blocks of 64 an entry costs a CTA 32 KB of X and 8 KB of weights for
+// 512 tensor cycles, 80 bytes a cycle (two separate products: 160).
+//
+// k_gated_few (up to 32 tokens).  Bound by reading the blocks once.  A CTA takes 16
+// rows of a block-row, its warps share out the entries; mma.sync fragments come
+// straight from global memory, 16 bytes a lane (the order of k inside a block is
+// free as long as both operands agree), and the warps' sums meet in shared memory.
+#include <algorithm>
+
+#include "convert.cuh"
+#include "internal.h"
+#include "ptx.cuh"
+#include "tc_common.cuh"
+
+namespace kairo {
+namespace {
+
+enum Activation : int {
+  kSilu = KAIRO_ACTIVATION_SILU,
+  kGelu = KAIRO_ACTIVATION_GELU,
+  kGeluTanh = KAIRO_ACTIVATION_GELU_TANH,
+  kRelu = KAIRO_ACTIVATION_RELU
+};
+
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+
+// act(g), and act'(g) where GRAD.  Every act(0) is 0.
+template <bool GRAD>
+__device__ __forceinline__ float activate(int act, float g, float& slope) {
+  if (act == kSilu) {
+    const float s = sigmoid(g);
+    if (GRAD) slope = s * (1.f + g * (1.f - s));
+    return g * s;
+  }
+  if (act == kGelu) {
+    const float cdf = 0.5f * erfcf(g * -0.70710678118654752f);
+    if (GRAD) slope = cdf + g * 0.39894228040143268f * __expf(-0.5f * g * g);
+    return g * cdf;
+  }
+  if (act == kGeluTanh) {
+    // 0.5 * (1 + tanh(y)) = sigmoid(2 y), which keeps its digits for negative g
+    const float c2 = 1.5957691216057308f;  // 2 * sqrt(2 / pi)
+    const float s = sigmoid(c2 * (g + 0.044715f * g * g * g));
+    if (GRAD) slope = s + g * s * (1.f - s) * c2 * (1.f + 0.134145f * g * g);
+    return g * s;
+  }
+  if (GRAD) slope = g > 0.f ? 1.f : 0.f;
+  return fmaxf(g, 0.f);
+}
+
+struct GatedArgs {
+  const int32_t* ent_ptr;  // nbr + 1
+  const int4* entries;     // {block-column, gate block or -1, up block or -1, 0}
+  const void* blocks;      // stored blocks
+  const void* x;
+  int64_t ldx;
+  void* h;                 // forward
+  int64_t ldh;
+  const void* dh;          // backward
+  int64_t lddh;
+  void* dp;                // backward: tokens x (2 * nbr * BM)
+  int64_t lddp;
+  unsigned* err;
+  int32_t n, m, k;
+  int32_t nbr, nbc, nentries, nblocks;
+  int32_t act;
+  int32_t group;           // token tiles visited together
+  int32_t vec_h, vec_dh;   // rows may be accessed 16 bytes at a time
+};
+
+// N outputs of one token from their sums: H, or dG and dU.
+template <typename T, bool GRAD, int N>
+__device__ __forceinline__ void gated_out(const GatedArgs& a, int token, int row, int bm, int c0, const float* g,
+                                          const float* u) {
+  const int first = row * bm + c0;  // output
+  if constexpr (!GRAD) {
+    float v[N], none = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = activate<false>(a.act, g[j], none) * u[j];
+    T* p = static_cast<T*>(a.h) + static_cast<int64_t>(token) * a.ldh + first;
+    if (a.vec_h && first + N <= a.m) {
+      store_f32<T, N>(p, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (first + j < a.m) p[j] = from_f32<T>(v[j]);
+    }
+  } else {
+    float d[N];
+    const T* p = static_cast<const T*>(a.dh) + static_cast<int64_t>(token) * a.lddh + first;
+    if (a.vec_dh && first + N <= a.m) {
+      load_f32<T, N>(p, d);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) d[j] = first + j < a.m ? to_f32<T>(p[j]) : 0.f;
+    }
+    float dg[N], du[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      float slope = 0.f;
+      const float v = activate<true>(a.act, g[j], slope);
+      const bool out = first + j < a.m;  // behind the last output both are zero, whatever the blocks hold there
+      dg[j] = out ? d[j] * u[j] * slope : 0.f;
+      du[j] = out ? d[j] * v : 0.f;
+    }
+    T* q = static_cast<T*>(a.dp) + static_cast<int64_t>(token) * a.lddp + 2 * row * bm + c0;
+    store_f32<T, N>(q, dg);
+    store_f32<T, N>(q + bm, du);
+  }
+}
+
+// ------------------------------------------------------------ tensor cores
+
+constexpr int kGatedThreads = 320;
+constexpr int kGatedEpiWarps = 8;
+constexpr int kGatedStages = 5;
+
+// Entries of one stage, so that a stage holds 64 k.
+constexpr int gated_group(int bm) { return 64 / bm; }
+constexpr int gated_block_bytes(int bm) { return (bm * bm * 2 + 1023) / 1024 * 1024; }
+constexpr int gated_slot_bytes(int bm, int t) { return t * 128 * bm * 2 + gated_block_bytes(bm); }
+constexpr int gated_stage_bytes(int bm, int t) { return gated_group(bm) * gated_slot_bytes(bm, t); }
+constexpr size_t gated_smem(int bm, int t) { return static_cast<size_t>(kGatedStages) * gated_stage_bytes(bm, t) + 2048; }
+
+struct GatedItem {
+  int tile, row, e0, e1;  // token tile, block-row, entries
+};
+
+template <int BM, int T, int IN_FMT, typename TT, bool GRAD>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGatedThreads, 1)
+    k_gated(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
+            const GatedArgs args) {
+  constexpr int ST = kGatedStages;
+  constexpr int E = gated_group(BM);
+  constexpr int SLOT = gated_slot_bytes(BM, T);
+  constexpr int STAGE = gated_stage_bytes(BM, T);
+  constexpr int PANEL = T * 128 * BM * 2;
+  constexpr uint32_t TX = PANEL + BM * BM * 2;  // bytes of one entry in one CTA
+  constexpr uint32_t IDESC = ptx::make_idesc_f16(IN_FMT, 0u, 0u, 256u, 2 * BM);
+  constexpr uint32_t SW = ptx::swizzle_code_for_row_bytes(BM * 2);
+  constexpr uint32_t ACC = T * 2 * BM;  // columns of one accumulator
+  constexpr uint32_t TMEM_COLS = 2 * ACC < 32 ? 32 : 2 * ACC;
+  static_assert(TMEM_COLS <= 512 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "TMEM columns");
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + ST * STAGE);  // used in the leader
+  uint64_t* empty = full + ST;
+  uint64_t* tfull = empty + ST;
+  uint64_t* tempty = tfull + 2;  // used in the leader
+  uint64_t* mma_done = tempty + 2;
+  int* misc = reinterpret_cast<int*>(mma_done + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc);
+  volatile int* abort_flag = misc + 1;
+  int* issued = misc + 4;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = ptx::cluster_rank();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      ptx::mbar_init(&full[s], 1);
+      ptx::mbar_init(&empty[s], 1);
+      issued[s] = 0;
+    }
+    for (int k = 0; k < 2; ++k) {
+      ptx::mbar_init(&tfull[k], 1);
+      ptx::mbar_init(&tempty[k], 2 * kGatedEpiWarps);
+    }
+    ptx::mbar_init(mma_done, 1);
+    misc[1] = 0;
+    ptx::mbar_init_fence();
+  }
+  if (warp == 0 && lane == 0) {
+    ptx::prefetch_tmap(&tmap_x);
+    ptx::prefetch_tmap(&tmap_w);
+  }
+  __syncthreads();
+  ptx::cluster_sync();
+  if (warp == 1) {
+    ptx::tmem_alloc_pair(tmem_slot, TMEM_COLS);
+    ptx::tmem_relinquish_pair();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  constexpr int TOKENS = T * 256;  // of a cluster's tile
+  const int tiles = (args.n + TOKENS - 1) / TOKENS;
+  const int nitems = tiles * args.nbr;
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  // `group` token tiles at a time, their block-rows one after the other: the group's X stays in
+  // L2 while the weights go by, and a block-row's blocks serve the group's tiles at about the same time.
+  auto item = [&](int t) {
+    GatedItem it;
+    const int per = args.group * args.nbr;
+    const int g = t / per, r = t - g * per;
+    const int t0 = g * args.group;
+    const int gn = min(args.group, tiles - t0);
+    it.row = r / gn;
+    it.tile = t0 + (r - it.row * gn);
+    // offsets outside the entries are clamped by every role alike (and reported by the loads)
+    it.e0 = min(max(__ldg(args.ent_ptr + it.row), 0), args.nentries);
+    it.e1 = min(max(__ldg(args.ent_ptr + it.row + 1), it.e0), args.nentries);
+    return it;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ loads
+    const uint64_t pol_w = ptx::policy_evict_first();
+    const uint64_t pol_x = ptx::policy_evict_last();
+    int sidx = 0;
+    uint32_t sph = 0;
+    bool alive = true;
+    auto fetch = [&](const GatedItem& it, int at) {
+      const int e = it.e0 + at + lane;
+      return e < it.e1 ? __ldg(args.entries + e) : make_int4(0, -1, -1, 0);
+    };
+    // entries are read a window of 32 ahead of use, the next item's range and first window an item ahead
+    GatedItem cur{}, nxt{};
+    int4 w0 = make_int4(0, -1, -1, 0), n0 = w0;
+    if (first < nitems) {
+      cur = item(first);
+      w0 = fetch(cur, 0);
+    }
+    for (int t = first; t < nitems && alive; t += step) {
+      const bool more = t + step < nitems;
+      if (more) {
+        nxt = item(t + step);
+        n0 = fetch(nxt, 0);
+      }
+      const int cnt = cur.e1 - cur.e0;
+      const int y0 = cur.tile * TOKENS + static_cast<int>(rank) * (T * 128);
+      for (int at = 0; at < cnt && alive; at += 32) {
+        const int4 w = w0;
+        if (at + 32 < cnt) w0 = fetch(cur, at + 32);
+        int col = w.x, blk = rank == 0 ? w.y : w.z;
+        if (at + lane < cnt && (static_cast<unsigned>(col) >= static_cast<unsigned>(args.nbc) || blk < -1 ||
+                                blk >= args.nblocks)) {
+          atomicCAS(args.err, 0u, KAIRO_DEVERR_BAD_INDEX);
+          col = 0;
+          blk = -1;
+        }
+        if (blk < 0) blk = args.nblocks;  // behind the storage: zeros
+        for (int b0 = 0; b0 < 32 && at + b0 < cnt; b0 += E) {
+          const int take = min(E, cnt - at - b0);
+          int ok = ptx::wait_parity(&empty[sidx], sph ^ 1u, abort_flag, args.err, kTagEmpty, kWaitCycles);
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+          if (!ok) {
+            alive = false;
+            break;
+          }
+          const uint32_t bar = ptx::peer_smem_u32(&full[sidx], 0);
+          if (rank == 0) {
+            if (lane == 0) issued[sidx] = static_cast<int>(sph) + 1;
+            ptx::mbar_expect_tx_if(lane == 0 ? 1u : 0u, &full[sidx], 2u * TX * static_cast<uint32_t>(take));
+          }
+          const uint32_t mine = lane >= b0 && lane < b0 + take ? 1u : 0u;
+          uint8_t* st = smem + sidx * STAGE + (mine ? lane - b0 : 0) * SLOT;
+          ptx::tma_load_2d_pair_if(mine, st + PANEL, &tmap_w, 0, blk * BM, bar, pol_w);
+          ptx::tma_load_2d_pair_if(mine, st, &tmap_x, col * BM, y0, bar, pol_x);
+          __syncwarp();
+          if (rank == 0) ptx::mbar_arrive_if(lane == 0 ? 1u : 0u, &full[sidx]);
+          if (++sidx == ST) {
+            sidx = 0;
+            sph ^= 1u;
+          }
+        }
+      }
+      cur = nxt;
+      w0 = n0;
+    }
+  } else if (warp == 1 && rank == 0) {
+    // ------------------------------------------------------------ MMA issuer
+    const uint32_t leader = lane == 0 ? 1u : 0u;
+    const uint32_t sbase = ptx::smem_u32(smem);
+    const uint64_t adesc = ptx::make_smem_desc(sbase, 16, 8 * BM * 2, SW);
+    const uint64_t bdesc = ptx::make_smem_desc(sbase + PANEL, 16, 8 * BM * 2, SW);
+    const uint32_t a_lo = static_cast<uint32_t>(adesc), a_hi = static_cast<uint32_t>(adesc >> 32);
+    const uint32_t b_lo = static_cast<uint32_t>(bdesc), b_hi = static_cast<uint32_t>(bdesc >> 32);
+    int sidx = 0, slot = 0;
+    uint32_t sph = 0, aphase = 0;
+    bool alive = true;
+    for (int t = first; t < nitems && alive; t += step) {
+      const GatedItem it = item(t);
+      const int cnt = it.e1 - it.e0;
+      if (cnt == 0) continue;
+      int ok = ptx::wait_parity(&tempty[slot], aphase ^ 1u, abort_flag, args.err, kTagTmemEmpty, kWaitCycles);
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok) break;
+      ptx::tc_fence_after();
+      const uint32_t d = tmem_base + static_cast<uint32_t>(slot) * ACC;
+      for (int at = 0; at < cnt; at += E) {
+        ok = ptx::wait_parity(&full[sidx], sph, abort_flag, args.err, kTagFull, kWaitCycles);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) {
+          alive = false;
+          break;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          if (at + e >= cnt) break;
+          const uint32_t s16 = static_cast<uint32_t>(sidx * STAGE + e * SLOT) >> 4;
+#pragma unroll
+          for (int kk = 0; kk < BM / 16; ++kk) {
+#pragma unroll
+            for (int i = 0; i < T; ++i)
+              ptx::mma_f16_ss_pair_if(leader, d + static_cast<uint32_t>(i * 2 * BM),
+                                      a_lo + s16 + ((i * 128 * BM * 2 + kk * 32) >> 4), a_hi,
+                                      b_lo + s16 + ((kk * 32) >> 4), b_hi, IDESC, (at > 0 || e > 0 || kk > 0) ? 1u : 0u);
+          }
+        }
+        ptx::mma_commit_pair_if(leader, &empty[sidx]);
+        if (++sidx == ST) {
+          sidx = 0;
+          sph ^= 1u;
+        }
+      }
+      if (!alive) break;
+      ptx::mma_commit_pair_if(leader, &tfull[slot]);
+      slot ^= 1;
+      if (slot == 0) aphase ^= 1u;
+    }
+    ptx::mma_commit_pair_if(leader, mma_done);
+    int dummy = 0;
+    ptx::wait_parity(mma_done, 0, reinterpret_cast<volatile int*>(&dummy), args.err, kTagDrain, kWaitCycles);
+    __syncwarp();
+  } else if (warp == 1) {
+    // the leader's last commit arrives here after all its earlier ones
+    int dummy = 0;
+    ptx::wait_parity(mma_done, 0, reinterpret_cast<volatile int*>(&dummy), args.err, kTagDrain, 4 * kWaitCycles);
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ epilogue
+    constexpr int UN = BM < 32 ? BM : 32;  // outputs of one step
+    constexpr int STEPS = T * (BM / UN);
+    const int q = warp & 3;
+    const int part = (warp - 2) >> 2;
+    const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
+    int slot = 0;
+    uint32_t aphase = 0;
+    for (int t = first; t < nitems; t += step) {
+      const GatedItem it = item(t);
+      const bool some = it.e1 > it.e0;
+      if (some) {
+        int ok = ptx::wait_parity(&tfull[slot], aphase, abort_flag, args.err, kTagTmemFull, kWaitCycles, 100);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+        ptx::tc_fence_after();
+      }
+      const uint32_t at = tmem_base + lane_addr + static_cast<uint32_t>(slot) * ACC;
+      for (int s = part; s < STEPS; s += 2) {
+        const int i = s / (BM / UN), c0 = (s % (BM / UN)) * UN;
+        const int token = it.tile * TOKENS + static_cast<int>(rank) * (T * 128) + i * 128 + q * 32 + lane;
+        float g[UN], u[UN];
+        if (some) {
+          if constexpr (UN == 32) {
+            ptx::tmem_ld32(at + static_cast<uint32_t>(i * 2 * BM + c0), g);
+            ptx::tmem_ld32(at + static_cast<uint32_t>(i * 2 * BM + BM + c0), u);
+          } else {
+            ptx::tmem_ld16(at + static_cast<uint32_t>(i * 2 * BM + c0), g);
+            ptx::tmem_ld16(at + static_cast<uint32_t>(i * 2 * BM + BM + c0), u);
+          }
+          ptx::tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int j = 0; j < UN; ++j) g[j] = u[j] = 0.f;
+        }
+        if (token < args.n) gated_out<TT, GRAD, UN>(args, token, it.row, BM, c0, g, u);
+        __syncwarp();
+      }
+      if (some) {
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive_cluster(ptx::peer_smem_u32(&tempty[slot], 0));
+        slot ^= 1;
+        if (slot == 0) aphase ^= 1u;
+      }
+    }
+  }
+
+  __syncthreads();
+  if (rank == 0 && warp == 0 && lane == 0 && *abort_flag) {
+    int dummy = 0;
+    for (int s = 0; s < ST; ++s)
+      if (issued[s])
+        ptx::wait_parity(&full[s], static_cast<uint32_t>(issued[s] - 1), reinterpret_cast<volatile int*>(&dummy),
+                         args.err, kTagDrain, kWaitCycles);
+  }
+  __syncthreads();
+  ptx::cluster_sync();
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc_pair(tmem_base, TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------ few tokens
+
+template <typename T>
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma_16816<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                  uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 8 * C values of one row that lane t of a quad takes, in C pieces of 16 bytes (blocks of 64: C = 2; 32: 1),
+// or the 4 of a 16-wide block's row.  `w` holds them as pairs.
+template <int BM>
+struct RowPart {
+  static constexpr int WORDS = BM / 8;  // 32-bit words a lane takes of a row
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) w[i] = 0u;
+  }
+  // `row` points at the row's first value, 16-byte aligned
+  __device__ __forceinline__ void load(const uint16_t* row, int t) {
+    if constexpr (BM == 16) {
+      const uint2 v = __ldg(reinterpret_cast<const uint2*>(row) + t);
+      w[0] = v.x;
+      w[1] = v.y;
+    } else {
+#pragma unroll
+      for (int c = 0; c < BM / 32; ++c) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(row) + c * 4 + t);
+        w[4 * c] = v.x;
+        w[4 * c + 1] = v.y;
+        w[4 * c + 2] = v.z;
+        w[4 * c + 3] = v.w;
+      }
+    }
+  }
+  // the same of a row that ends after `left` values, value by value
+  __device__ __forceinline__ void load_edge(const uint16_t* row, int t, int left) {
+    constexpr int V = BM == 16 ? 4 : 8;
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+      const int at = (2 * i / V) * 4 * V + t * V + 2 * i % V;
+      const uint32_t lo = at < left ? row[at] : 0u, hi = at + 1 < left ? row[at + 1] : 0u;
+      w[i] = lo | (hi << 16);
+    }
+  }
+};
+
+constexpr int kFewWarps = 8;
+
+// NT * 8 tokens; grid: one CTA per 16 rows of a block-row.
+template <int BM, int NT, typename T, bool GRAD>
+__global__ void __launch_bounds__(32 * kFewWarps) k_gated_few(const GatedArgs a, int vec_x) {
+  constexpr int SLICES = BM / 16;
+  __shared__ float sums[kFewWarps][2][NT * 8][17];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int gid = lane >> 2, t = lane & 3;
+  const int row = blockIdx.x / SLICES, slice = blockIdx.x % SLICES;
+  const int e0 = min(max(__ldg(a.ent_ptr + row), 0), a.nentries);
+  const int e1 = min(max(__ldg(a.ent_ptr + row + 1), e0), a.nentries);
+  float g[NT][4], u[NT][4];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[i][j] = u[i][j] = 0.f;
+  const uint16_t* blocks = static_cast<const uint16_t*>(a.blocks) + (slice * 16 + gid) * BM;
+  const uint16_t* x = static_cast<const uint16_t*>(a.x);
+#pragma unroll 2
+  for (int e = e0 + warp; e < e1; e += kFewWarps) {
+    int4 w = __ldg(a.entries + e);
+    if (static_cast<unsigned>(w.x) >= static_cast<unsigned>(a.nbc) || w.y < -1 || w.y >= a.nblocks || w.z < -1 ||
+        w.z >= a.nblocks) {
+      atomicCAS(a.err, 0u, KAIRO_DEVERR_BAD_INDEX);
+      w = make_int4(0, -1, -1, 0);
+    }
+    RowPart<BM> g0, g1, u0, u1, xs[NT];
+    g0.zero();
+    g1.zero();
+    u0.zero();
+    u1.zero();
+    if (w.y >= 0) {
+      const uint16_t* p = blocks + static_cast<int64_t>(w.y) * BM * BM;
+      g0.load(p, t);
+      g1.load(p + 8 * BM, t);
+    }
+    if (w.z >= 0) {
+      const uint16_t* p = blocks + static_cast<int64_t>(w.z) * BM * BM;
+      u0.load(p, t);
+      u1.load(p + 8 * BM, t);
+    }
+    const int left = a.k - w.x * BM;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const int token = i * 8 + gid;
+      const uint16_t* p = x + static_cast<int64_t>(token) * a.ldx + w.x * BM;
+      xs[i].zero();
+      if (token < a.n) {
+        if (vec_x && left >= BM) xs[i].load(p, t);
+        else xs[i].load_edge(p, t, left);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < BM / 16; ++s)
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        mma_16816<T>(g[i], g0.w[2 * s], g1.w[2 * s], g0.w[2 * s + 1], g1.w[2 * s + 1], xs[i].w[2 * s], xs[i].w[2 * s + 1]);
+        mma_16816<T>(u[i], u0.w[2 * s], u1.w[2 * s], u0.w[2 * s + 1], u1.w[2 * s + 1], xs[i].w[2 * s], xs[i].w[2 * s + 1]);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int token = i * 8 + 2 * t + (j & 1), r = gid + (j >> 1) * 8;
+      sums[warp][0][token][r] = g[i][j];
+      sums[warp][1][token][r] = u[i][j];
+    }
+  __syncthreads();
+  for (int o = threadIdx.x; o < NT * 8 * 16; o += 32 * kFewWarps) {
+    const int token = o >> 4, r = o & 15;
+    if (token >= a.n) break;
+    float gs = 0.f, us = 0.f;
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) {
+      gs += sums[w][0][token][r];
+      us += sums[w][1][token][r];
+    }
+    gated_out<T, GRAD, 1>(a, token, row, BM, slice * 16 + r, &gs, &us);
+  }
+}
+
+// ------------------------------------------------------------ host side
+
+constexpr int kFewTokens = 32;
+
+template <int BM, int NT, typename T, bool GRAD>
+void launch_few(const GatedArgs& a, cudaStream_t s) {
+  const int vec_x = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && (a.ldx % 8 == 0 || a.n <= 1);
+  k_gated_few<BM, NT, T, GRAD><<<a.nbr * (BM / 16), 32 * kFewWarps, 0, s>>>(a, vec_x);
+}
+
+template <int BM, typename TT, int IN_FMT, bool GRAD>
+kairo_status run_gated(GatedArgs a, cudaStream_t s) {
+  if (a.n <= kFewTokens) {
+    if (a.n <= 8) launch_few<BM, 1, TT, GRAD>(a, s);
+    else if (a.n <= 16) launch_few<BM, 2, TT, GRAD>(a, s);
+    else launch_few<BM, 4, TT, GRAD>(a, s);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "launch of k_gated_few");
+  }
+  const CUtensorMapDataType dt = IN_FMT == 0 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  auto go = [&](auto tc) -> kairo_status {
+    constexpr int T = decltype(tc)::value;
+    CUtensorMap mx, mw;
+    kairo_status st = make_map_2d(&mx, a.x, dt, 2, static_cast<uint64_t>(a.k), static_cast<uint64_t>(a.n),
+                                  static_cast<uint64_t>(a.ldx), BM, T * 128, "X");
+    if (st == KAIRO_STATUS_SUCCESS)
+      st = make_map_2d(&mw, a.blocks, dt, 2, BM, static_cast<uint64_t>(std::max(1, a.nblocks)) * BM, BM, BM, BM,
+                       "block storage");
+    if (st) return st;
+    auto* fn = &k_gated<BM, T, IN_FMT, TT, GRAD>;
+    cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(gated_smem(BM, T)));
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic smem)");
+    const int tiles = static_cast<int>(ceil_div64(a.n, T * 256));
+    // a group's X takes about a quarter of the L2
+    a.group = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(tiles, (32LL << 20) / (static_cast<int64_t>(T) * 512 * a.k))));
+    const int64_t items = static_cast<int64_t>(tiles) * a.nbr;
+    const int clusters = static_cast<int>(std::min<int64_t>(items, std::max(1, device_sm_count(current_device()) / 2)));
+    fn<<<2 * clusters, kGatedThreads, gated_smem(BM, T), s>>>(mx, mw, a);
+    e = cudaGetLastError();
+    return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "launch of k_gated");
+  };
+  return a.n > 256 ? go(std::integral_constant<int, 2>{}) : go(std::integral_constant<int, 1>{});
+}
+
+template <bool GRAD>
+kairo_status dispatch_gated(const GatedArgs& a, int bm, kairo_dtype dt, cudaStream_t s) {
+  if (dt == KAIRO_DTYPE_F16) {
+    if (bm == 16) return run_gated<16, __half, 0, GRAD>(a, s);
+    if (bm == 32) return run_gated<32, __half, 0, GRAD>(a, s);
+    return run_gated<64, __half, 0, GRAD>(a, s);
+  }
+  if (bm == 16) return run_gated<16, __nv_bfloat16, 1, GRAD>(a, s);
+  if (bm == 32) return run_gated<32, __nv_bfloat16, 1, GRAD>(a, s);
+  return run_gated<64, __nv_bfloat16, 1, GRAD>(a, s);
+}
+
+bool row_vec(const void* p, int64_t ld, int64_t rows) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (ld % 8 == 0 || rows <= 1);
+}
+
+kairo_status gated_check(const kairo_gated* w, const void* x, int64_t ldx, int64_t n, int32_t act, const void* err) {
+  if (!w) return fail(KAIRO_STATUS_INVALID_VALUE, "null weight descriptor");
+  if (w->rows < 0 || w->cols < 0 || w->nentries < 0 || w->nblocks < 0 || n < 0)
+    return fail(KAIRO_STATUS_INVALID_VALUE, "invalid size");
+  if (w->block != 16 && w->block != 32 && w->block != 64)
+    return fail(KAIRO_STATUS_NOT_SUPPORTED, "the gated projection takes square blocks of 16, 32 or 64");
+  if (w->dtype != KAIRO_DTYPE_F16 && w->dtype != KAIRO_DTYPE_BF16)
+    return fail(KAIRO_STATUS_NOT_SUPPORTED, "the gated projection takes f16 or bf16");
+  if (w->rows > 0x3fffff00LL || w->cols > 0x7fffff00LL || n > 0x7fffff00LL || w->nentries > 0x7fffffffLL ||
+      (w->nblocks + 1) * w->block > 0x7fffffffLL ||
+      ceil_div64(n, 256) * ceil_div64(w->rows, w->block) > 0x7fffffffLL)
+    return fail(KAIRO_STATUS_NOT_SUPPORTED, "sizes beyond 32-bit coordinates");
+  if (act < kSilu || act > kRelu) return fail(KAIRO_STATUS_INVALID_VALUE, "unknown activation");
+  if (ldx < w->cols) return fail(KAIRO_STATUS_INVALID_VALUE, "leading dimension too small");
+  if (n == 0 || w->rows == 0) return KAIRO_STATUS_SUCCESS;
+  if (!w->ent_ptr || !err || (w->nentries > 0 && (!w->entries || !w->blocks || !x)))
+    return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+  if (reinterpret_cast<uintptr_t>(w->entries) % 16 || reinterpret_cast<uintptr_t>(w->blocks) % 16)
+    return fail(KAIRO_STATUS_INVALID_VALUE, "entries and blocks must be 16-byte aligned");
+  if (n > kFewTokens && w->nentries > 0 && !row_vec(x, ldx, n))
+    return fail(KAIRO_STATUS_INVALID_VALUE, "X must have 16-byte aligned rows");
+  return KAIRO_STATUS_SUCCESS;
+}
+
+GatedArgs gated_args(const kairo_gated* w, const void* x, int64_t ldx, int64_t n, int32_t act, unsigned* err) {
+  GatedArgs a{};
+  a.ent_ptr = w->ent_ptr;
+  a.entries = reinterpret_cast<const int4*>(w->entries);
+  a.blocks = w->blocks;
+  a.x = x;
+  a.ldx = ldx;
+  a.err = err;
+  a.n = static_cast<int32_t>(n);
+  a.m = static_cast<int32_t>(w->rows);
+  a.k = static_cast<int32_t>(w->cols);
+  a.nbr = static_cast<int32_t>(ceil_div64(w->rows, w->block));
+  a.nbc = static_cast<int32_t>(ceil_div64(w->cols, w->block));
+  a.nentries = static_cast<int32_t>(w->nentries);
+  a.nblocks = static_cast<int32_t>(w->nblocks);
+  a.act = act;
+  return a;
+}
+
+}  // namespace
+}  // namespace kairo
+
+using namespace kairo;
+
+extern "C" kairo_status kairo_gated_linear(const kairo_gated* w, const void* x, int64_t ldx, int64_t n,
+                                           int32_t activation, void* h, int64_t ldh, unsigned* error_word,
+                                           void* stream) {
+  kairo_status st = gated_check(w, x, ldx, n, activation, error_word);
+  if (st) return st;
+  if (ldh < w->rows) return fail(KAIRO_STATUS_INVALID_VALUE, "leading dimension too small");
+  if (n == 0 || w->rows == 0) return KAIRO_STATUS_SUCCESS;
+  if (!h) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (w->nentries == 0) {
+    const cudaError_t e = cudaMemset2DAsync(h, static_cast<size_t>(ldh) * 2, 0, static_cast<size_t>(w->rows) * 2,
+                                            static_cast<size_t>(n), s);
+    return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "cudaMemset2DAsync(H)");
+  }
+  GatedArgs a = gated_args(w, x, ldx, n, activation, error_word);
+  a.h = h;
+  a.ldh = ldh;
+  a.vec_h = row_vec(h, ldh, n);
+  return dispatch_gated<false>(a, w->block, w->dtype, s);
+}
+
+extern "C" kairo_status kairo_gated_linear_grad(const kairo_gated* w, const void* x, int64_t ldx, int64_t n,
+                                                int32_t activation, const void* dh, int64_t lddh, void* dp,
+                                                int64_t lddp, unsigned* error_word, void* stream) {
+  kairo_status st = gated_check(w, x, ldx, n, activation, error_word);
+  if (st) return st;
+  const int64_t stacked = 2 * ceil_div64(w->rows, w->block) * w->block;
+  if (lddh < w->rows || lddp < stacked || lddp % 8)
+    return fail(KAIRO_STATUS_INVALID_VALUE, "leading dimension too small, or that of dP no multiple of 8");
+  if (n == 0 || w->rows == 0) return KAIRO_STATUS_SUCCESS;
+  if (!dh || !dp) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+  if (reinterpret_cast<uintptr_t>(dp) % 16) return fail(KAIRO_STATUS_INVALID_VALUE, "dP must be 16-byte aligned");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (w->nentries == 0) {
+    const cudaError_t e = cudaMemset2DAsync(dp, static_cast<size_t>(lddp) * 2, 0, static_cast<size_t>(stacked) * 2,
+                                            static_cast<size_t>(n), s);
+    return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "cudaMemset2DAsync(dP)");
+  }
+  GatedArgs a = gated_args(w, x, ldx, n, activation, error_word);
+  a.dh = dh;
+  a.lddh = lddh;
+  a.vec_dh = row_vec(dh, lddh, n);
+  a.dp = dp;
+  a.lddp = lddp;
+  return dispatch_gated<true>(a, w->block, w->dtype, s);
+}

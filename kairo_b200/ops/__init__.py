@@ -35,6 +35,14 @@ from kairo_b200.ops.adapters import (
     adapter_plan,
 )
 from kairo_b200.ops.checkpoint import QuantizedActivations, dequantize_activations, quantize_activations
+from kairo_b200.ops.gated import (
+    GatedWeights,
+    SparseFeedForward,
+    SparseGatedLinear,
+    gated_weights,
+    sparse_gated_linear,
+    sparse_gated_linear_backward,
+)
 from kairo_b200.ops.vocab_loss import LinearCrossEntropy, linear_cross_entropy, linear_cross_entropy_backward
 from kairo_b200.ops.spmm import (
     KernelConfig,
@@ -94,6 +102,12 @@ __all__ = [
     "QuantizedActivations",
     "dequantize_activations",
     "quantize_activations",
+    "GatedWeights",
+    "SparseFeedForward",
+    "SparseGatedLinear",
+    "gated_weights",
+    "sparse_gated_linear",
+    "sparse_gated_linear_backward",
     "LinearCrossEntropy",
     "linear_cross_entropy",
     "linear_cross_entropy_backward",

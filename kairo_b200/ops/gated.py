@@ -1,0 +1,359 @@
+"""Gated projection of a feed-forward block with block-sparse weights (CUDA only).
+
+    G = X Wg^T      U = X Wu^T      H = act(G) * U
+
+Both products, the activation and the product of the two are one kernel: G and
+U are not in memory, neither in the forward pass nor for the backward pass,
+which forms them again from X.
+
+* ``gated_weights(gate, up)`` -- two block-sparse weights of one shape, laid out
+  side by side once.
+* ``sparse_gated_linear`` -- H, for single tokens and prompts alike.
+* ``sparse_gated_linear_backward`` -- the gradients by X and by both weights'
+  blocks.
+* ``SparseGatedLinear`` -- both as a module with autograd;
+  ``SparseFeedForward`` -- the whole block, ``down(act(gate(X)) * up(X))``.
+
+The reference has no counterpart.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass, field, replace
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from kairo_b200 import _lib
+from kairo_b200.ops.backward import (
+    BlockSparseLinear,
+    TransposedBsr,
+    bsr_transpose,
+    sparse_linear_weight_grad,
+    transpose_values,
+)
+from kairo_b200.ops.spmm import sparse_linear
+from kairo_b200.ops.token_embedding import _ld, _rows
+from kairo_b200.types import BlockSparseMatrix
+
+_ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
+_FEW_TOKENS = 32  # up to here X may have any alignment
+
+
+@dataclass(frozen=True)
+class GatedWeights:
+    """Gate and up weights of one gated projection (``gated_weights``).
+
+    blocks: (gate_blocks + up_blocks, b, b), the gate's in its BSR order, then
+    the up weight's; the gradients come in this order (``split``).  The other
+    tensors describe the patterns: ent_ptr / entries, the block-columns of every
+    block-row with the two weights' blocks, and ``stacked``, the pattern of the
+    (2 ceil(out / b) b, in) matrix whose block-rows 2i and 2i + 1 are block-row
+    i of gate and of up."""
+
+    blocks: Tensor
+    gate_blocks: int
+    shape: tuple[int, int]
+    block: int
+    ent_ptr: Tensor
+    entries: Tensor
+    row_ptr: Tensor   # of the stacked matrix
+    col_idx: Tensor   # its block-columns, in its order
+    blk_idx: Tensor   # stored block of each of its blocks
+    stored_col: Tensor  # block-column of every stored block
+    _structure: dict = field(default_factory=dict, repr=False, compare=False)
+
+    def __post_init__(self) -> None:
+        if self.blocks.dim() != 3 or self.blocks.shape[1:] != (self.block, self.block) or not self.blocks.is_contiguous():
+            raise ValueError(f"blocks must be a contiguous (n, {self.block}, {self.block}) tensor")
+        if self.blocks.shape[0] != self.stored_col.numel():
+            raise ValueError(f"the patterns have {self.stored_col.numel()} blocks, got {self.blocks.shape[0]}")
+        if self.blocks.dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError(f"gated weights must be float16 or bfloat16, got {self.blocks.dtype}")
+        if self.blocks.device != self.entries.device:
+            raise ValueError("blocks must be on the patterns' device")
+        if self.blocks.data_ptr() % 16:
+            raise ValueError("blocks must be 16-byte aligned")
+        d = _lib.KairoGated()
+        d.rows, d.cols = self.shape
+        d.nentries, d.nblocks = self.entries.shape[0], self.blocks.shape[0]
+        d.ent_ptr, d.entries, d.blocks = self.ent_ptr.data_ptr(), self.entries.data_ptr(), self.blocks.data_ptr()
+        d.block, d.dtype = self.block, _lib.kairo_dtype(self.blocks.dtype)
+        object.__setattr__(self, "_desc", d)
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return self.blocks.dtype
+
+    @property
+    def device(self) -> torch.device:
+        return self.blocks.device
+
+    def with_blocks(self, blocks: Tensor) -> "GatedWeights":
+        """The same patterns with other values."""
+        return replace(self, blocks=blocks)
+
+    def split(self, blocks: Tensor) -> tuple[Tensor, Tensor]:
+        """The gate's and the up weight's part of a tensor in ``blocks``' order."""
+        return blocks[:self.gate_blocks], blocks[self.gate_blocks:]
+
+    def matrices(self) -> tuple[BlockSparseMatrix, BlockSparseMatrix]:
+        """Gate and up as BlockSparseMatrix views of ``blocks``."""
+        out = []
+        rp = self.row_ptr.to(torch.int64)
+        for part, blocks in enumerate(self.split(self.blocks)):
+            counts = rp[part + 1::2] - rp[part::2][:rp[part + 1::2].numel()]
+            row_ptr = torch.zeros(counts.numel() + 1, dtype=torch.int32, device=self.device)
+            row_ptr[1:] = torch.cumsum(counts, 0)
+            cols = self.split(self.stored_col)[part].contiguous()
+            out.append(BlockSparseMatrix(row_ptr=row_ptr, col_idx=cols, blocks=blocks, shape=self.shape,
+                                         block_size=(self.block, self.block)))
+        return out[0], out[1]
+
+    def stacked(self) -> BlockSparseMatrix:
+        """The stacked matrix (see above) over ``blocks``."""
+        rows = (self.row_ptr.numel() - 1) * self.block
+        return BlockSparseMatrix(row_ptr=self.row_ptr, col_idx=self.col_idx, blocks=self.blocks,
+                                 shape=(rows, self.shape[1]), block_size=(self.block, self.block),
+                                 blk_idx=self.blk_idx)
+
+    def _transposed(self) -> TransposedBsr:
+        """The stacked matrix transposed, values of this call: its structure is made once per pattern."""
+        a = self.stacked()
+        if "t" not in self._structure:
+            t = bsr_transpose(a)
+            perm_stored = self.blk_idx[t.perm.long()] if a.nnzb else t.perm
+            self._structure["t"] = (t.matrix.row_ptr, t.matrix.col_idx, t.perm, perm_stored, t.matrix.max_row_blocks)
+        row_ptr, col_idx, perm, _, longest = self._structure["t"]
+        b = self.block
+        blocks_t = self.blocks.new_empty((a.nnzb, b, b))
+        t = TransposedBsr(matrix=BlockSparseMatrix(row_ptr=row_ptr, col_idx=col_idx, blocks=blocks_t,
+                                                   shape=(a.shape[1], a.shape[0]), block_size=(b, b),
+                                                   max_row_blocks=longest), perm=perm)
+        return transpose_values(a, t)
+
+
+def _in_order(a: BlockSparseMatrix) -> Tensor:
+    return a.blocks[:a.nnzb] if a.blk_idx is None else a.blocks[a.blk_idx.long()]
+
+
+def gated_weights(gate: BlockSparseMatrix, up: BlockSparseMatrix) -> GatedWeights:
+    """Lays out two block-sparse weights (out_features x in_features) of one
+    shape, block size (16, 32 or 64, square) and type (float16 or bfloat16) for
+    ``sparse_gated_linear``.  Their patterns may differ; neither may hold a
+    block twice.  The blocks are copied.  Synchronises."""
+    if not (gate.blocks.is_cuda and up.blocks.is_cuda):
+        raise RuntimeError("kairo_b200.gated_weights runs on CUDA tensors only; this package has no CPU implementation")
+    if gate.shape != up.shape or gate.block_size != up.block_size:
+        raise ValueError(f"gate is {gate.shape} in blocks of {gate.block_size}, up is {up.shape} in blocks of "
+                         f"{up.block_size}")
+    if gate.dtype != up.dtype or gate.device != up.device:
+        raise TypeError("gate and up must share a dtype and a device")
+    if gate.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"gated weights must be float16 or bfloat16, got {gate.dtype}")
+    b = gate.block_size[0]
+    if gate.block_size[1] != b or b not in (16, 32, 64):
+        raise ValueError(f"blocks must be 16 x 16, 32 x 32 or 64 x 64, got {gate.block_size}")
+    dev, nbr, nbc = gate.device, gate.nbr, gate.nbc
+    rows, keys = [], []
+    for a in (gate, up):
+        counts = (a.row_ptr[1:] - a.row_ptr[:-1]).long()
+        if a.nnzb and (int(counts.min()) < 0 or int(a.row_ptr[0]) != 0 or int(a.row_ptr[-1]) != a.nnzb
+                       or int(a.col_idx.min()) < 0 or int(a.col_idx.max()) >= nbc):
+            raise ValueError("a weight's row_ptr or col_idx is malformed")
+        r = torch.repeat_interleave(torch.arange(nbr, device=dev), counts, output_size=a.nnzb)
+        rows.append(r)
+        keys.append(r * nbc + a.col_idx.long())
+    n_gate, n_up = gate.nnzb, up.nnzb
+    merged, at = torch.unique(torch.cat(keys), return_inverse=True)
+    entries = torch.full((merged.numel(), 4), -1, dtype=torch.int32, device=dev)
+    entries[:, 0] = merged % max(nbc, 1)
+    entries[:, 3] = 0
+    for part, (lo, n) in enumerate(((0, n_gate), (n_gate, n_up))):
+        mine = at[lo:lo + n]
+        if torch.unique(mine).numel() != n:
+            raise ValueError("a weight holds the same block twice")
+        entries[mine, 1 + part] = torch.arange(lo, lo + n, dtype=torch.int32, device=dev)
+    ent_ptr = torch.searchsorted(merged, torch.arange(nbr + 1, device=dev) * nbc).to(torch.int32)
+    # the stacked matrix: row i of gate, row i of up, row i + 1 of gate, ...
+    gp, up_ptr = gate.row_ptr.long(), up.row_ptr.long()
+    row_ptr = torch.empty(2 * nbr + 1, dtype=torch.int64, device=dev)
+    row_ptr[0::2] = gp + up_ptr
+    row_ptr[1::2] = gp[1:] + up_ptr[:-1]
+    place = torch.cat([torch.arange(n_gate, device=dev) + up_ptr[rows[0]],
+                       torch.arange(n_up, device=dev) + gp[rows[1] + 1]])
+    stored_col = torch.cat([gate.col_idx, up.col_idx])
+    blk_idx = torch.empty(n_gate + n_up, dtype=torch.int32, device=dev)
+    blk_idx[place] = torch.arange(n_gate + n_up, dtype=torch.int32, device=dev)
+    col_idx = stored_col[blk_idx.long()]
+    return GatedWeights(blocks=torch.cat([_in_order(gate), _in_order(up)]), gate_blocks=n_gate, shape=tuple(gate.shape),
+                        block=b, ent_ptr=ent_ptr, entries=entries, row_ptr=row_ptr.to(torch.int32), col_idx=col_idx,
+                        blk_idx=blk_idx, stored_col=stored_col)
+
+
+def _input(op: str, X: Tensor, weights: GatedWeights, activation: str) -> tuple[Tensor, int]:
+    """X as rows that the kernels read (a copy where they must be 16-byte aligned and are not), activation code."""
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"{op}: activation must be one of {', '.join(_ACTIVATIONS)}, got {activation!r}")
+    k = weights.shape[1]
+    if X.dim() != 2 or X.shape[1] != k:
+        raise ValueError(f"{op}: Inner dimensions must match: X is {tuple(X.shape)}, the weights are {weights.shape}")
+    if X.dtype != weights.dtype:
+        raise TypeError(f"{op}: X is {X.dtype}, the weights are {weights.dtype}")
+    return _rows(X), _ACTIVATIONS[activation]
+
+
+def _aligned(X: Tensor) -> Tensor:
+    n, k = X.shape
+    if X.data_ptr() % 16 == 0 and (n <= 1 or X.stride(0) % 8 == 0):
+        return X
+    out = X.new_empty((n, -(-k // 8) * 8))[:, :k]
+    return out.copy_(X)
+
+
+def sparse_gated_linear(X: Tensor, weights: GatedWeights, *, activation: str = "silu", out: Tensor | None = None,
+                        check: bool = False) -> Tensor:
+    """``act(X Wg^T) * (X Wu^T)``: (tokens, out_features) in X's type, from fp32 sums, rounded once.
+
+    X: (tokens, in_features) in the weights' type.  activation: "silu", "gelu"
+    (by erf), "gelu_tanh" or "relu".  ``out``: a row-major tensor to write to,
+    sharing no memory with an input.
+
+    A value of X that is not finite makes those results non-finite whose row
+    keeps a block of gate or up in its column, and no others.  ``check=True``
+    synchronises and raises KairoDeviceError where a kernel met a malformed
+    entry or a wait ran out; without it ``pending_device_error`` tells."""
+    op = "sparse_gated_linear"
+    index = _lib.device_index(op, X, weights.blocks)
+    x, act = _input(op, X, weights, activation)
+    n, m = x.shape[0], weights.shape[0]
+    if n > _FEW_TOKENS:
+        x = _aligned(x)
+    if out is None:
+        out = x.new_empty((n, m))
+    elif out.shape != (n, m) or out.dtype != x.dtype or out.device != x.device or _rows(out) is not out:
+        raise ValueError(f"{op}: out must be a row-major ({n}, {m}) {x.dtype} tensor on {x.device}")
+    else:
+        _lib.refuse_overlap(op, out, X, weights.blocks)
+    err = _lib.error_word(index)
+    if check:
+        _lib.take_pending_error(err, op)
+    _lib.launch(op, _lib.lib().kairo_gated_linear, index, ctypes.byref(weights._desc), x.data_ptr(),
+                max(_ld(x), weights.shape[1]), n, act, out.data_ptr(), _ld(out), err.data_ptr())
+    if check:
+        _lib.raise_on_device_error(err)
+    return out
+
+
+def sparse_gated_linear_backward(dH: Tensor, X: Tensor, weights: GatedWeights, *, activation: str = "silu",
+                                 need_dx: bool = True, need_dw: bool = True, dw_dtype: torch.dtype | None = None,
+                                 check: bool = False) -> tuple[Tensor | None, Tensor | None]:
+    """(dX, d_blocks) of ``sparse_gated_linear``: dX in X's type; d_blocks in
+    ``dw_dtype`` (default: the weights'; or float32), in the order of
+    ``weights.blocks`` (``weights.split`` gives the two weights' parts).
+    Either may be left out (None).
+
+    dG and dU are rounded to the weights' type, as operands of both products."""
+    op = "sparse_gated_linear_backward"
+    index = _lib.device_index(op, dH, X, weights.blocks)
+    x, act = _input(op, X, weights, activation)
+    n, (m, k) = x.shape[0], weights.shape
+    if dH.shape != (n, m):
+        raise ValueError(f"{op}: dH must be ({n}, {m}), got {tuple(dH.shape)}")
+    if dH.dtype != x.dtype:
+        raise TypeError(f"{op}: dH is {dH.dtype}, X is {x.dtype}")
+    dwt = dw_dtype or weights.dtype
+    if dwt not in (torch.float32, weights.dtype):
+        raise TypeError(f"{op}: dw_dtype must be float32 or {weights.dtype}, got {dwt}")
+    if not (need_dx or need_dw):
+        return None, None
+    x, dh = _aligned(x), _rows(dH)
+    nbr = weights.ent_ptr.numel() - 1
+    dp = x.new_empty((n, 2 * nbr * weights.block))
+    err = _lib.error_word(index)
+    if check:
+        _lib.take_pending_error(err, op)
+    _lib.launch(op, _lib.lib().kairo_gated_linear_grad, index, ctypes.byref(weights._desc), x.data_ptr(),
+                max(_ld(x), k), n, act, dh.data_ptr(), max(_ld(dh), m), dp.data_ptr(), dp.shape[1], err.data_ptr())
+    if check:
+        _lib.raise_on_device_error(err)
+    wt = weights._transposed()
+    dX = sparse_linear(dp, wt.matrix, out_dtype=x.dtype, check=check) if need_dx else None
+    d_blocks = None
+    if need_dw:
+        # the weight gradient lands in the blocks' own order: positions of the transposed structure name stored blocks
+        perm_stored = weights._structure["t"][3]
+        stored = BlockSparseMatrix(row_ptr=weights.row_ptr, col_idx=weights.stored_col, blocks=weights.blocks,
+                                   shape=(2 * nbr * weights.block, k), block_size=(weights.block, weights.block))
+        d_blocks = sparse_linear_weight_grad(dp, x, stored, TransposedBsr(matrix=wt.matrix, perm=perm_stored),
+                                             out_dtype=dwt, check=check)
+    return dX, d_blocks
+
+
+class _GatedFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, X: Tensor, blocks: Tensor, module: "SparseGatedLinear") -> Tensor:
+        ctx.save_for_backward(X, blocks)
+        ctx.module = module
+        return sparse_gated_linear(X, module.weights(blocks), activation=module.activation)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dH: Tensor):
+        X, blocks = ctx.saved_tensors
+        dX, dW = sparse_gated_linear_backward(dH, X, ctx.module.weights(blocks), activation=ctx.module.activation,
+                                              need_dx=ctx.needs_input_grad[0], need_dw=ctx.needs_input_grad[1])
+        return dX, dW, None
+
+
+class SparseGatedLinear(torch.nn.Module):
+    """``act(X Wg^T) * (X Wu^T)`` with block-sparse weights of fixed patterns.
+
+    The parameter is ``blocks``: the gate's blocks in BSR order, then the up
+    weight's (``gate_blocks`` of them are the gate's)."""
+
+    def __init__(self, gate: BlockSparseMatrix, up: BlockSparseMatrix, *, activation: str = "silu") -> None:
+        super().__init__()
+        if activation not in _ACTIVATIONS:
+            raise ValueError(f"activation must be one of {', '.join(_ACTIVATIONS)}, got {activation!r}")
+        w = gated_weights(gate, up)
+        self.activation = activation
+        self.shape = w.shape
+        self.gate_blocks = w.gate_blocks
+        self.block = w.block
+        self.blocks = torch.nn.Parameter(w.blocks.detach())
+        for name in ("ent_ptr", "entries", "row_ptr", "col_idx", "blk_idx", "stored_col"):
+            self.register_buffer(name, getattr(w, name))
+        self._made: tuple | None = None
+
+    def weights(self, blocks: Tensor | None = None) -> GatedWeights:
+        b = (self.blocks if blocks is None else blocks).detach()
+        parts = (self.ent_ptr, self.entries, self.row_ptr, self.col_idx, self.blk_idx, self.stored_col)
+        # the patterns' transposed structure is kept as long as the buffers are the same tensors
+        if self._made is None or any(p is not q for p, q in zip(self._made[0], parts)):
+            self._made = (parts, {})
+        return GatedWeights(blocks=b, gate_blocks=self.gate_blocks, shape=self.shape, block=self.block,
+                            ent_ptr=parts[0], entries=parts[1], row_ptr=parts[2], col_idx=parts[3], blk_idx=parts[4],
+                            stored_col=parts[5], _structure=self._made[1])
+
+    def forward(self, X: Tensor) -> Tensor:
+        if not torch.is_grad_enabled():
+            return sparse_gated_linear(X, self.weights(), activation=self.activation)
+        return _GatedFn.apply(X, self.blocks, self)
+
+
+class SparseFeedForward(torch.nn.Module):
+    """The feed-forward block ``down(act(gate(X)) * up(X))`` of a ``SparseGatedLinear`` and a ``BlockSparseLinear``."""
+
+    def __init__(self, gate: BlockSparseMatrix, up: BlockSparseMatrix, down: BlockSparseMatrix, *,
+                 activation: str = "silu", checkpoint: str | None = None) -> None:
+        super().__init__()
+        if down.shape[1] != gate.shape[0]:
+            raise ValueError(f"down is {down.shape}, gate and up have {gate.shape[0]} outputs")
+        self.gated = SparseGatedLinear(gate, up, activation=activation)
+        self.down = BlockSparseLinear(down, checkpoint=checkpoint)
+
+    def forward(self, X: Tensor) -> Tensor:
+        return self.down(self.gated(X))
