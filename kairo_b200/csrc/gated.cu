@@ -231,6 +231,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGatedThreads, 1)
     // ------------------------------------------------------------ loads
     const uint64_t pol_w = ptx::policy_evict_first();
     const uint64_t pol_x = ptx::policy_evict_last();
+    constexpr int BOXES = T * 2 + 1;
+    static_assert(E * BOXES <= 32, "one lane per copy");
+    const void* map_x = &tmap_x;
+    const void* map_w = &tmap_w;
     int sidx = 0;
     uint32_t sph = 0;
     bool alive = true;
@@ -277,10 +281,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGatedThreads, 1)
             if (lane == 0) issued[sidx] = static_cast<int>(sph) + 1;
             ptx::mbar_expect_tx_if(lane == 0 ? 1u : 0u, &full[sidx], 2u * TX * static_cast<uint32_t>(take));
           }
-          const uint32_t mine = lane >= b0 && lane < b0 + take ? 1u : 0u;
-          uint8_t* st = smem + sidx * STAGE + (mine ? lane - b0 : 0) * SLOT;
-          ptx::tma_load_2d_pair_if(mine, st + PANEL, &tmap_w, 0, blk * BM, bar, pol_w);
-          ptx::tma_load_2d_pair_if(mine, st, &tmap_x, col * BM, y0, bar, pol_x);
+          // one lane per box of 64 tokens and per block, so that all copies of a stage are issued at once
+          const int e = lane / BOXES, part = lane - e * BOXES;  // entry of the stage; its panel's box, or its block
+          const uint32_t mine = e < take ? 1u : 0u;
+          const int ecol = __shfl_sync(0xffffffffu, col, (b0 + e) & 31);
+          const int eblk = __shfl_sync(0xffffffffu, blk, (b0 + e) & 31);
+          uint8_t* st = smem + sidx * STAGE + (mine ? e : 0) * SLOT;
+          const bool is_w = part == BOXES - 1;
+          ptx::tma_load_2d_pair_if(mine, is_w ? st + PANEL : st + part * (64 * BM * 2), is_w ? map_w : map_x,
+                                   is_w ? 0 : ecol * BM, is_w ? eblk * BM : y0 + part * 64, bar, is_w ? pol_w : pol_x);
           __syncwarp();
           if (rank == 0) ptx::mbar_arrive_if(lane == 0 ? 1u : 0u, &full[sidx]);
           if (++sidx == ST) {
@@ -365,7 +374,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGatedThreads, 1)
       const GatedItem it = item(t);
       const bool some = it.e1 > it.e0;
       if (some) {
-        int ok = ptx::wait_parity(&tfull[slot], aphase, abort_flag, args.err, kTagTmemFull, kWaitCycles, 100);
+        int ok = ptx::wait_parity(&tfull[slot], aphase, abort_flag, args.err, kTagTmemFull, kWaitCycles);
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
         ptx::tc_fence_after();
@@ -583,14 +592,14 @@ kairo_status run_gated(GatedArgs a, cudaStream_t s) {
     constexpr int T = decltype(tc)::value;
     CUtensorMap mx, mw;
     kairo_status st = make_map_2d(&mx, a.x, dt, 2, static_cast<uint64_t>(a.k), static_cast<uint64_t>(a.n),
-                                  static_cast<uint64_t>(a.ldx), BM, T * 128, "X");
+                                  static_cast<uint64_t>(a.ldx), BM, 64, "X");
     if (st == KAIRO_STATUS_SUCCESS)
       st = make_map_2d(&mw, a.blocks, dt, 2, BM, static_cast<uint64_t>(std::max(1, a.nblocks)) * BM, BM, BM, BM,
                        "block storage");
     if (st) return st;
     auto* fn = &k_gated<BM, T, IN_FMT, TT, GRAD>;
-    cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(gated_smem(BM, T)));
+    static std::atomic<uint64_t> ready{0};
+    cudaError_t e = allow_smem(reinterpret_cast<const void*>(fn), gated_smem(BM, T), &ready);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic smem)");
     const int tiles = static_cast<int>(ceil_div64(a.n, T * 256));
     // a group's X takes about a quarter of the L2

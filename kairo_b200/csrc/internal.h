@@ -1,6 +1,7 @@
 // Internal declarations shared by the translation units of libkairo_spmm.
 #pragma once
 
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 #include <string>
@@ -19,6 +20,18 @@ kairo_status cuda_fail(cudaError_t e, const char* what);
 
 int device_sm_count(int device);
 int current_device();
+
+// Raises a kernel's dynamic shared memory limit to `bytes` on the current device, once per device:
+// `ready` has a bit for each of the first 64 (the call costs about a microsecond otherwise).
+inline cudaError_t allow_smem(const void* fn, size_t bytes, std::atomic<uint64_t>* ready) {
+  const int dev = current_device();
+  const uint64_t bit = dev >= 0 && dev < 64 ? uint64_t{1} << dev : 0;
+  if (bit && (ready->load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  const cudaError_t e =
+      cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (e == cudaSuccess) ready->fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 inline int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }

@@ -45,32 +45,50 @@ constexpr int kPairTileN = 256;
 constexpr int kPairK = 64;           // k of one stage
 constexpr int kPairStages = 6;
 constexpr int kPairHalf = 128 * kPairK * 2;  // bytes of one operand's part of a stage in one CTA
+constexpr int kPairBoxes = 2;
+constexpr int kPairBoxRows = 128 / kPairBoxes;
 constexpr int kPairStageBytes = 2 * kPairHalf;
 constexpr int kPairEpiCols = kPairTileN / (kPairEpiWarps / 4);
-constexpr size_t kPairSmem = static_cast<size_t>(kPairStages) * kPairStageBytes + 2048;
+constexpr int kPairOutBytes = 4096;  // of each epilogue warp, to turn rows a lane into rows a warp
+constexpr size_t kPairSmem =
+    static_cast<size_t>(kPairStages) * kPairStageBytes + kPairEpiWarps * kPairOutBytes + 2048;
+constexpr int kPairClusters = 74;    // pairs of a B200's 148 SMs, for plans that must not depend on the current device
 static_assert(kPairSmem <= kMaxSmem, "shared memory");
 
 // Tiles of one product.  They are visited `group_m` rows of tiles at a time,
 // rows fastest: the group's A and the current columns' B stay in L2.
 struct PairShape {
   int tiles_m, tiles_n, ksteps, group_m;
-  int seg;  // stages of one segment
+  int seg;     // stages of one segment
+  int splits;  // parts of k, each a tile of its own
 };
 
-__device__ __forceinline__ void pair_tile(const PairShape& s, int t, int& mt, int& nt) {
+struct PairTile {
+  int mt, nt, split;
+  int k0, k1;  // stages
+};
+
+__device__ __forceinline__ PairTile pair_tile(const PairShape& s, int t) {
+  PairTile o;
+  const int all = s.tiles_m * s.tiles_n;
+  o.split = t / all;
+  t -= o.split * all;
   const int per = s.group_m * s.tiles_n;
   const int g = t / per, r = t - g * per;
   const int m0 = g * s.group_m;
   const int gm = min(s.group_m, s.tiles_m - m0);
-  nt = r / gm;
-  mt = m0 + (r - nt * gm);
+  o.nt = r / gm;
+  o.mt = m0 + (r - o.nt * gm);
+  o.k0 = static_cast<int>(static_cast<int64_t>(s.ksteps) * o.split / s.splits);
+  o.k1 = static_cast<int>(static_cast<int64_t>(s.ksteps) * (o.split + 1) / s.splits);
+  return o;
 }
 
 // Epi supplies `struct Args` and
-//   __device__ Epi(const Args&, int row_in_tile, int part)
-//   __device__ void tile(int mt, int nt, float (&v)[kPairEpiCols])   its columns of one tile
-//   __device__ void done()                                           after the CTA's last tile
-// and is made once per thread and launch.
+//   __device__ Epi(const Args&, int row_in_tile, int part, uint8_t* out)
+//   __device__ void tile(const PairTile&, float (&v)[kPairEpiCols])   its columns of one tile
+//   __device__ void done()                                            after the CTA's last tile
+// and is made once per thread and launch; `out` is the warp's kPairOutBytes.
 template <int IN_FMT, bool A_MN, bool B_MN, class Epi>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     k_pair_gemm(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
@@ -78,12 +96,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   constexpr int ST = kPairStages;
   constexpr uint32_t IDESC = ptx::make_idesc_f16(IN_FMT, A_MN ? 1u : 0u, B_MN ? 1u : 0u, kPairTileM, kPairTileN);
   constexpr uint32_t TMEM_COLS = 2 * kPairTileN;
-  // boxes of one CTA's half of an operand: 64 k x 128 rows, or twice 64 columns x 64 k
-  constexpr int NA = A_MN ? 2 : 1, NB = B_MN ? 2 : 1;
+  // A CTA's half of an operand comes in kPairBoxes boxes, one lane each: 64 k x 64 rows, or 64
+  // columns x 64 k.
+  constexpr int NA = kPairBoxes, NB = kPairBoxes;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + ST * kPairStageBytes);  // used in the leader
+  uint8_t* out = smem + ST * kPairStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(out + kPairEpiWarps * kPairOutBytes);  // used in the leader
   uint64_t* empty = full + ST;
   uint64_t* tfull = empty + ST;
   uint64_t* tempty = tfull + 2;  // used in the leader
@@ -124,7 +144,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const int ntiles = shape.tiles_m * shape.tiles_n;
+  const int ntiles = shape.tiles_m * shape.tiles_n * shape.splits;
   const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
 
   if (warp == 0) {
@@ -135,15 +155,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const void* map = is_a ? static_cast<const void*>(&tmap_a) : static_cast<const void*>(&tmap_b);
     const uint32_t mine = lane < NA + NB ? 1u : 0u;
     const bool mn = is_a ? A_MN : B_MN;
-    const uint32_t dst_off = (is_a ? 0u : kPairHalf) + static_cast<uint32_t>(mine ? box : 0) * (kPairHalf / 2);
+    const uint32_t dst_off = (is_a ? 0u : kPairHalf) + static_cast<uint32_t>(mine ? box : 0) * (kPairHalf / kPairBoxes);
     int sidx = 0;
     uint32_t sph = 0;
     bool alive = true;
     for (int t = first; t < ntiles && alive; t += step) {
-      int mt, nt;
-      pair_tile(shape, t, mt, nt);
-      const int r0 = (is_a ? mt : nt) * 256 + static_cast<int>(rank) * 128 + (mn ? box * 64 : 0);
-      for (int k = 0; k < shape.ksteps; ++k) {
+      const PairTile pt = pair_tile(shape, t);
+      const int r0 = (is_a ? pt.mt : pt.nt) * 256 + static_cast<int>(rank) * 128 + box * kPairBoxRows;
+      for (int k = pt.k0; k < pt.k1; ++k) {
         int ok = ptx::wait_parity(&empty[sidx], sph ^ 1u, abort_flag, err, kTagEmpty, kWaitCycles);
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) {
@@ -181,7 +200,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     uint32_t sph = 0, aphase = 0;
     bool alive = true;
     for (int t = first; t < ntiles && alive; t += step) {
-      for (int k0 = 0; k0 < shape.ksteps; k0 += shape.seg) {
+      const PairTile pt = pair_tile(shape, t);
+      for (int k0 = pt.k0; k0 < pt.k1; k0 += shape.seg) {
         int ok = ptx::wait_parity(&tempty[slot], aphase ^ 1u, abort_flag, err, kTagTmemEmpty, kWaitCycles);
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) {
@@ -190,7 +210,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         }
         ptx::tc_fence_after();
         const uint32_t d = tmem_base + static_cast<uint32_t>(slot * kPairTileN);
-        const int k1 = min(shape.ksteps, k0 + shape.seg);
+        const int k1 = min(pt.k1, k0 + shape.seg);
         for (int k = k0; k < k1; ++k) {
           ok = ptx::wait_parity(&full[sidx], sph, abort_flag, err, kTagFull, kWaitCycles);
           ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -228,15 +248,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     // ------------------------------------------------------------ epilogue
     const int q = warp & 3;
     const int part = (warp - 2) >> 2;  // which kPairEpiCols columns of the tile
-    Epi epi(eargs, static_cast<int>(rank) * 128 + q * 32 + lane, part);
+    Epi epi(eargs, static_cast<int>(rank) * 128 + q * 32 + lane, part, out + (warp - 2) * kPairOutBytes);
     const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
     int slot = 0;
     uint32_t aphase = 0;
     bool alive = true;
     for (int t = first; t < ntiles && alive; t += step) {
+      const PairTile pt = pair_tile(shape, t);
       float v[kPairEpiCols];
-      for (int k0 = 0; k0 < shape.ksteps; k0 += shape.seg) {
-        int ok = ptx::wait_parity(&tfull[slot], aphase, abort_flag, err, kTagTmemFull, kWaitCycles, 100);
+      for (int k0 = pt.k0; k0 < pt.k1; k0 += shape.seg) {
+        int ok = ptx::wait_parity(&tfull[slot], aphase, abort_flag, err, kTagTmemFull, kWaitCycles);
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) {
           alive = false;
@@ -244,7 +265,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         }
         ptx::tc_fence_after();
         const uint32_t at = tmem_base + lane_addr + static_cast<uint32_t>(slot * kPairTileN + part * kPairEpiCols);
-        if (k0 == 0) {
+        if (k0 == pt.k0) {
 #pragma unroll
           for (int c = 0; c < kPairEpiCols; c += 32) ptx::tmem_ld32(at + c, v + c);
           ptx::tmem_wait_ld();
@@ -265,9 +286,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         if (slot == 0) aphase ^= 1u;
       }
       if (!alive) break;
-      int mt, nt;
-      pair_tile(shape, t, mt, nt);
-      epi.tile(mt, nt, v);
+      epi.tile(pt, v);
     }
     if (alive) epi.done();
   }
@@ -297,18 +316,22 @@ inline kairo_status pair_operand_map(CUtensorMap* map, const void* base, kairo_d
   return mn ? make_map_2d(map, base, t, 2, static_cast<uint64_t>(rows), static_cast<uint64_t>(k),
                           static_cast<uint64_t>(ld), 64, kPairK, what)
             : make_map_2d(map, base, t, 2, static_cast<uint64_t>(k), static_cast<uint64_t>(rows),
-                          static_cast<uint64_t>(ld), kPairK, 128, what);
+                          static_cast<uint64_t>(ld), kPairK, kPairBoxRows, what);
+}
+
+// Clusters of a launch of `tiles` tiles.
+inline int pair_clusters(int64_t tiles) {
+  return static_cast<int>(std::min<int64_t>(tiles, std::max(1, device_sm_count(current_device()) / 2)));
 }
 
 template <int IN_FMT, bool A_MN, bool B_MN, class Epi>
 kairo_status launch_pair_gemm(const CUtensorMap& a, const CUtensorMap& b, const PairShape& shape, unsigned* err,
                               const typename Epi::Args& args, cudaStream_t s) {
   auto* fn = &k_pair_gemm<IN_FMT, A_MN, B_MN, Epi>;
-  cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(fn), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(kPairSmem));
+  static std::atomic<uint64_t> ready{0};
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(fn), kPairSmem, &ready);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic smem)");
-  const int64_t tiles = static_cast<int64_t>(shape.tiles_m) * shape.tiles_n;
-  const int clusters = static_cast<int>(std::min<int64_t>(tiles, std::max(1, device_sm_count(current_device()) / 2)));
+  const int clusters = pair_clusters(static_cast<int64_t>(shape.tiles_m) * shape.tiles_n * shape.splits);
   fn<<<2 * clusters, kPairThreads, kPairSmem, s>>>(a, b, shape, err, args);
   e = cudaGetLastError();
   return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "launch of the paired tensor-core product");

@@ -319,8 +319,11 @@ __device__ __forceinline__ uint32_t peer_smem_u32(const void* p, uint32_t rank) 
   return r;
 }
 
+// Arrival on a barrier of either CTA that orders nothing by itself: for giving back
+// TMEM columns whose loads have completed (tcgen05.wait::ld).  A releasing arrival would first
+// wait until the thread's earlier global stores have landed.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_dst, uint32_t ncols) {

@@ -66,13 +66,16 @@ struct StatsEpi {
     int tokens, vocab;
     float scale;
     int by_cluster;  // one row of tiles: a CTA's tiles share a slot
+    unsigned* ticket;  // of k_lse, zeroed here
   };
   const Args& a;
   int row, part, mt = -1;
   int64_t id = -1;
   float m = -INFINITY, s = 0.f;
 
-  __device__ StatsEpi(const Args& args, int row_in_tile, int p) : a(args), row(row_in_tile), part(p) {}
+  __device__ StatsEpi(const Args& args, int row_in_tile, int p, uint8_t*) : a(args), row(row_in_tile), part(p) {
+    if (blockIdx.x == 0 && row_in_tile == 0 && p == 0) *a.ticket = 0u;
+  }
 
   __device__ __forceinline__ void flush(int token, int64_t slot) {
     if (token < a.tokens) a.part[slot * a.tokens + token] = make_float2(m, s);
@@ -80,14 +83,14 @@ struct StatsEpi {
     s = 0.f;
   }
 
-  __device__ void tile(int tm, int tn, float (&v)[kPairEpiCols]) {
-    const int token = tm * kPairTileM + row;
+  __device__ void tile(const PairTile& pt, float (&v)[kPairEpiCols]) {
+    const int token = pt.mt * kPairTileM + row;
     if (__all_sync(0xffffffffu, token >= a.tokens)) return;
-    if (tm != mt) {
-      mt = tm;
+    if (pt.mt != mt) {
+      mt = pt.mt;
       id = token < a.tokens ? a.ids[token] : -1;
     }
-    const int col0 = tn * kPairTileN + part * kPairEpiCols;
+    const int col0 = pt.nt * kPairTileN + part * kPairEpiCols;
     const int64_t at = id - col0;
     const bool here = id >= 0 && id < a.vocab && at >= 0 && at < kPairEpiCols;
     if (__any_sync(0xffffffffu, here)) {
@@ -114,7 +117,7 @@ struct StatsEpi {
     for (int j = 0; j < kPairEpiCols; ++j) sum[j & 3] += ex2(v[j] - ref);
     m = top;
     s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    if (!a.by_cluster) flush(token, static_cast<int64_t>(tn) * (kPairTileN / kPairEpiCols) + part);
+    if (!a.by_cluster) flush(token, static_cast<int64_t>(pt.nt) * (kPairTileN / kPairEpiCols) + part);
   }
 
   __device__ void done() {
@@ -122,18 +125,89 @@ struct StatsEpi {
   }
 };
 
-// 16 results of one row, rounded to T, at p: 16-byte stores where `vec`, the first `n` one by one otherwise.
+// A warp's 32 rows x kPairEpiCols results, a row a lane, rounded to T at p (row pitch ld, `rows` and
+// `cols` of them exist).  They pass through shared memory, 64 columns at a time, so that a store
+// instruction writes 128 bytes of each of four rows (a row a lane: 16 bytes of 32 rows, and 2 where
+// rows are not aligned; there a warp writes one row at a time, 4 bytes a lane).
 template <typename T>
-__device__ __forceinline__ void put16(T* p, const float* v, int n, bool vec) {
-  if (vec && n >= 16) {
-    float w[16];
+__device__ __forceinline__ void put_rows(uint8_t* out, const float (&v)[kPairEpiCols], T* p, int64_t ld, int rows,
+                                         int cols, bool vec) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) w[j] = v[j];
-    store_f32<T, 16>(p, w);
-  } else {
+  for (int h = 0; h < kPairEpiCols; h += 64) {
+    if (h >= cols) return;
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (j < n) p[j] = from_f32<T>(v[j]);
+    for (int c = 0; c < 8; ++c) {
+      float w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = v[h + 8 * c + j];
+      store_f32<T, 8>(reinterpret_cast<T*>(out + lane * 128 + ((c ^ (lane & 7)) * 16)), w);
+    }
+    __syncwarp();
+    if (vec) {
+      const int c = lane & 7;
+      const int n = cols - (h + 8 * c);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 3);
+        if (r >= rows || n <= 0) continue;
+        const uint4 w = *reinterpret_cast<const uint4*>(out + r * 128 + ((c ^ (r & 7)) * 16));
+        T* dst = p + r * ld + h + 8 * c;
+        if (n >= 8) {
+          *reinterpret_cast<uint4*>(dst) = w;
+        } else {
+          const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j < n) dst[j] = e[j];
+        }
+      }
+    } else {
+      const int n = min(64, cols - h);
+      for (int r = 0; r < rows; ++r) {
+        T* dst = p + r * ld + h;
+        auto at = [&](int j) { return *reinterpret_cast<const uint16_t*>(out + r * 128 + (((j >> 3) ^ (r & 7)) * 16) + (j & 7) * 2); };
+        // pairs on 4-byte boundaries; an odd row begins and ends with half a pair
+        const int odd = static_cast<int>((reinterpret_cast<uintptr_t>(dst) >> 1) & 1u);
+        const int j = 2 * lane - odd;
+        uint16_t* d = reinterpret_cast<uint16_t*>(dst);
+        if (j >= 0 && j + 1 < n) *reinterpret_cast<uint32_t*>(d + j) = at(j) | (static_cast<uint32_t>(at(j + 1)) << 16);
+        else if (j >= 0 && j < n) d[j] = at(j);
+        else if (j == -1) d[0] = at(0);
+        if (odd && lane == 0 && n == 64) d[63] = at(63);
+      }
+    }
+    __syncwarp();
+  }
+}
+
+// The same in fp32 (rows of p 16-byte aligned, room for whole groups of 4 columns), added to what is there unless `first`.
+__device__ __forceinline__ void sum_rows(uint8_t* out, const float (&v)[kPairEpiCols], float* p, int64_t ld, int rows,
+                                         int cols, bool first) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int h = 0; h < kPairEpiCols; h += 32) {
+    if (h >= cols) return;
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      *reinterpret_cast<float4*>(out + lane * 128 + ((c ^ (lane & 7)) * 16)) =
+          make_float4(v[h + 4 * c], v[h + 4 * c + 1], v[h + 4 * c + 2], v[h + 4 * c + 3]);
+    __syncwarp();
+    const int c = lane & 7;
+    const bool in = h + 4 * c < cols;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + (lane >> 3);
+      if (r >= rows || !in) continue;
+      float4 w = *reinterpret_cast<const float4*>(out + r * 128 + ((c ^ (r & 7)) * 16));
+      float4* dst = reinterpret_cast<float4*>(p + r * ld + h + 4 * c);
+      if (!first) {
+        const float4 o = *dst;
+        w = make_float4(w.x + o.x, w.y + o.y, w.z + o.z, w.w + o.w);
+      }
+      *dst = w;
+    }
+    __syncwarp();
   }
 }
 
@@ -154,19 +228,23 @@ struct GradEpi {
   int64_t id = -1;
   float lse2 = 0.f, f = 0.f;
 
-  __device__ GradEpi(const Args& args, int row_in_tile, int p) : a(args), row(row_in_tile), part(p) {}
+  uint8_t* out;
 
-  __device__ void tile(int tm, int tn, float (&v)[kPairEpiCols]) {
-    const int token = tm * kPairTileM + row;
-    if (tm != mt) {
-      mt = tm;
+  __device__ GradEpi(const Args& args, int row_in_tile, int p, uint8_t* o) : a(args), row(row_in_tile), part(p), out(o) {}
+
+  __device__ void tile(const PairTile& pt, float (&v)[kPairEpiCols]) {
+    const int token = pt.mt * kPairTileM + row;
+    const int token0 = token - static_cast<int>(threadIdx.x & 31);  // of the warp
+    if (token0 >= a.tokens) return;
+    if (pt.mt != mt) {
+      mt = pt.mt;
       if (token < a.tokens) {
         id = a.ids[token];
         lse2 = a.lse[token] * kLog2e;
         f = a.f[token];
       }
     }
-    const int col0 = tn * kPairTileN + part * kPairEpiCols;  // in the piece
+    const int col0 = pt.nt * kPairTileN + part * kPairEpiCols;  // in the piece
     const float k = a.scale * kLog2e;
     const int64_t at = id - (a.v0 + col0);
 #pragma unroll
@@ -183,62 +261,45 @@ struct GradEpi {
       for (int j = 0; j < kPairEpiCols; ++j)
         if (j >= n) v[j] = 0.f;
     }
-    if (token >= a.tokens) return;
-    T* dst = a.g + static_cast<int64_t>(token) * a.ldg + col0;
-#pragma unroll
-    for (int c = 0; c < kPairEpiCols; c += 16) put16<T>(dst + c, v + c, 16, true);
+    put_rows<T>(out, v, a.g + static_cast<int64_t>(token0) * a.ldg + col0, a.ldg, a.tokens - token0, kPairEpiCols, true);
   }
 
   __device__ void done() {}
 };
 
-// A sum over pieces (fp32, `acc`), the last one times *factor as T.
+// Sums times *factor as T, or, where k is split or comes in pieces, fp32 sums of each split
+// (added to those of earlier pieces unless `first`), which k_join finishes.
 template <typename T>
 struct SumEpi {
   struct Args {
     T* out;
     int64_t ldo;
-    float* acc;        // [rows][ldacc], 16-byte aligned rows; read unless first, written unless last
+    float* acc;        // [splits][rows][ldacc], rows 16-byte aligned; NULL: to `out`
     int64_t ldacc;
     const float* factor;
     int rows, cols;
-    int first, last, vec;
+    int first, vec;
   };
   const Args& a;
   int row, part;
+  uint8_t* out;
   float factor;
 
-  __device__ SumEpi(const Args& args, int row_in_tile, int p) : a(args), row(row_in_tile), part(p), factor(*args.factor) {}
+  __device__ SumEpi(const Args& args, int row_in_tile, int p, uint8_t* o)
+      : a(args), row(row_in_tile), part(p), out(o), factor(*args.factor) {}
 
-  __device__ void tile(int tm, int tn, float (&v)[kPairEpiCols]) {
-    const int r = tm * kPairTileM + row;
-    const int col0 = tn * kPairTileN + part * kPairEpiCols;
-    const int n = a.cols - col0;
-    if (r >= a.rows || n <= 0) return;
-    float4* acc = reinterpret_cast<float4*>(a.acc + static_cast<int64_t>(r) * a.ldacc + col0);
-    if (!a.first) {
+  __device__ void tile(const PairTile& pt, float (&v)[kPairEpiCols]) {
+    const int r0 = pt.mt * kPairTileM + row - static_cast<int>(threadIdx.x & 31);  // the warp's first
+    const int col0 = pt.nt * kPairTileN + part * kPairEpiCols;
+    const int rows = a.rows - r0, cols = a.cols - col0;
+    if (rows <= 0 || cols <= 0) return;
+    if (a.acc) {
+      float* p = a.acc + (static_cast<int64_t>(pt.split) * a.rows + r0) * a.ldacc + col0;
+      sum_rows(out, v, p, a.ldacc, rows, cols, a.first != 0);
+    } else {
 #pragma unroll
-      for (int j = 0; j < kPairEpiCols / 4; ++j)
-        if (4 * j < n) {
-          const float4 w = acc[j];
-          v[4 * j] += w.x;
-          v[4 * j + 1] += w.y;
-          v[4 * j + 2] += w.z;
-          v[4 * j + 3] += w.w;
-        }
-    }
-    if (!a.last) {
-#pragma unroll
-      for (int j = 0; j < kPairEpiCols / 4; ++j)
-        if (4 * j < n) acc[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-      return;
-    }
-    T* dst = a.out + static_cast<int64_t>(r) * a.ldo + col0;
-#pragma unroll
-    for (int c = 0; c < kPairEpiCols; c += 16) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) v[c + j] *= factor;
-      put16<T>(dst + c, v + c, n - c, a.vec != 0);
+      for (int j = 0; j < kPairEpiCols; ++j) v[j] *= factor;
+      put_rows<T>(out, v, a.out + static_cast<int64_t>(r0) * a.ldo + col0, a.ldo, min(rows, 32), cols, a.vec != 0);
     }
   }
 
@@ -322,6 +383,34 @@ __global__ void __launch_bounds__(1024) k_lse(const float2* __restrict__ part, i
   sum = cta_sum(sum);
   count = cta_sum(count);
   if (threadIdx.x == 0) *loss = reduction == kMean ? sum / fmaxf(count, 1.f) : sum;
+}
+
+// out = *factor * the splits' sums, in their order.
+template <typename T>
+__global__ void __launch_bounds__(256) k_join(const float* __restrict__ acc, int64_t ldacc, int splits, int64_t rows,
+                                              int64_t cols, const float* __restrict__ factor, T* __restrict__ out,
+                                              int64_t ldo) {
+  const int64_t groups = (cols + 3) / 4, total = rows * groups;
+  const float f = *factor;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t r = i / groups, c = (i - r * groups) * 4;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) {
+      const float4 w = __ldcs(reinterpret_cast<const float4*>(acc + (k * rows + r) * ldacc + c));
+      s = make_float4(s.x + w.x, s.y + w.y, s.z + w.z, s.w + w.w);
+    }
+    const float v[4] = {s.x * f, s.y * f, s.z * f, s.w * f};
+    T* dst = out + r * ldo + c;
+    if (c + 4 <= cols && reinterpret_cast<uintptr_t>(dst) % 8 == 0) {
+      store_f32<T, 4>(dst, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + j < cols) dst[j] = from_f32<T>(v[j]);
+    }
+  }
 }
 
 // Rows of 16-bit values with 16-byte alignment: dst (rows x ldd, ldd a multiple of 8) = src, zeros
@@ -456,9 +545,29 @@ LossWs loss_ws(const Problem& p) {
 }
 
 struct GradWs {
-  size_t f, factor, acc, x, w, g, total;
+  size_t f, factor, acc_x, acc_w, x, w, g, total;
   int64_t cols;
+  int splits_x, splits_w;  // parts of the vocabulary piece for dX, of the tokens for dW
 };
+
+// Parts of k for a product of rows x cols: tiles that fill the clusters' rounds evenly, against the fp32
+// sums of each part, written and read once more.  In stages of one tile (about 0.27 us); a tile costs 8
+// beside its k (filling the pipeline, the epilogue's end).
+int splits_for(int64_t rows, int64_t cols, int64_t k) {
+  const int64_t t = tiles(rows) * tiles(cols), steps = ceil_div64(k, kPairK);
+  const double again = 8.0 * static_cast<double>(rows) * static_cast<double>(cols) / 6.5e12 / 0.27e-6;
+  int best = 1;
+  double least = 0.0;
+  for (int s = 1; s <= 64 && s <= steps; ++s) {
+    const double cost = static_cast<double>(ceil_div64(t * s, kPairClusters) * (ceil_div64(steps, s) + 8)) +
+                        (s > 1 ? again * s + 10.0 : 0.0);
+    if (s == 1 || cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
+}
 
 GradWs grad_ws(const Problem& p) {
   GradWs o{};
@@ -473,7 +582,10 @@ GradWs grad_ws(const Problem& p) {
   o.factor = 128;
   o.f = take(4 * static_cast<size_t>(p.tokens));
   o.x = take(2 * ld * static_cast<size_t>(p.tokens));
-  if (o.cols < p.vocab) o.acc = take(4 * ld * static_cast<size_t>(p.tokens));
+  o.splits_x = splits_for(p.tokens, p.dim, std::min(o.cols, p.vocab));
+  o.splits_w = splits_for(std::min(o.cols, p.vocab), p.dim, p.tokens);
+  if (o.cols < p.vocab || o.splits_x > 1) o.acc_x = take(4 * ld * static_cast<size_t>(p.tokens) * o.splits_x);
+  if (o.splits_w > 1) o.acc_w = take(4 * ld * static_cast<size_t>(std::min(o.cols, p.vocab)) * o.splits_w);
   if (!rows_aligned(p.w, p.ldw, p.vocab)) o.w = take(2 * ld * static_cast<size_t>(p.vocab));
   o.g = take(2 * static_cast<size_t>(p.tokens) * static_cast<size_t>(o.cols));
   o.total = at;
@@ -515,16 +627,27 @@ int group_rows(int64_t tiles_m, int64_t k) {
 
 // Stages of a segment.  Logits: 256 k, so that lse and losses are as exact as fp32 sums (7e-7 of a
 // logit at worst).  The gradients are rounded to 16 bits: 4096 k leave 1e-5.
-constexpr int kSegLogits = 4, kSegGrads = 64;
+constexpr int kSegLogits = 8, kSegGrads = 64;
 
-PairShape shape_of(int64_t rows, int64_t cols, int64_t k, int seg) {
+PairShape shape_of(int64_t rows, int64_t cols, int64_t k, int seg, int splits = 1) {
   PairShape s;
   s.seg = seg;
+  s.splits = splits;
   s.tiles_m = static_cast<int>(tiles(rows));
   s.tiles_n = static_cast<int>(tiles(cols));
   s.ksteps = static_cast<int>(ceil_div64(k, kPairK));
   s.group_m = group_rows(s.tiles_m, k);
   return s;
+}
+
+template <typename T>
+kairo_status join(const float* acc, int64_t ldacc, int splits, int64_t rows, int64_t cols, const float* factor, T* out,
+                  int64_t ldo, cudaStream_t s) {
+  const int64_t work = ceil_div64(rows * ceil_div64(cols, 4), 256);
+  const int grid = static_cast<int>(std::min<int64_t>(work, device_sm_count(current_device()) * 16));
+  k_join<T><<<grid, 256, 0, s>>>(acc, ldacc, splits, rows, cols, factor, out, ldo);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "launch of k_join");
 }
 
 template <typename T, int FMT>
@@ -534,21 +657,16 @@ kairo_status run_loss(Problem p, float* loss, float* lse, uint8_t* ws, unsigned*
   if (st == KAIRO_STATUS_SUCCESS) st = aligned_rows(&p.w, &p.ldw, p.vocab, p.dim, ws + o.w, s);
   if (st) return st;
   unsigned* ticket = reinterpret_cast<unsigned*>(ws + o.ticket);
-  if (p.reduction != kNone) {
-    const cudaError_t e = cudaMemsetAsync(ticket, 0, sizeof(unsigned), s);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync(ticket)");
-  }
   CUtensorMap ma, mb;
   st = pair_operand_map(&ma, p.x, p.dt, false, p.tokens, p.dim, p.ldx, "hidden states");
   if (st == KAIRO_STATUS_SUCCESS) st = pair_operand_map(&mb, p.w, p.dt, false, p.vocab, p.dim, p.ldw, "vocabulary table");
   if (st) return st;
   const PairShape sh = shape_of(p.tokens, p.vocab, p.dim, kSegLogits);
-  const int clusters = std::min(sh.tiles_m * sh.tiles_n, std::max(1, device_sm_count(current_device()) / 2));
   StatsEpi::Args a{reinterpret_cast<float2*>(ws + o.part), reinterpret_cast<float*>(ws + o.target), p.ids,
-                   static_cast<int>(p.tokens), static_cast<int>(p.vocab), p.scale, sh.tiles_m == 1};
+                   static_cast<int>(p.tokens), static_cast<int>(p.vocab), p.scale, sh.tiles_m == 1, ticket};
   st = launch_pair_gemm<FMT, false, false, StatsEpi>(ma, mb, sh, err, a, s);
   if (st) return st;
-  const int slots = 2 * (a.by_cluster ? clusters : sh.tiles_n);
+  const int slots = 2 * (a.by_cluster ? pair_clusters(sh.tiles_n) : sh.tiles_n);
   k_lse<<<static_cast<int>(ceil_div64(p.tokens, 32)), 1024, 0, s>>>(
       a.part, slots, a.target, p.ids, a.tokens, a.vocab, p.reduction,
       p.reduction == kNone ? loss : reinterpret_cast<float*>(ws + o.each), lse, loss, ticket);
@@ -577,7 +695,6 @@ kairo_status run_grad(Problem p, const float* grad, const float* lse, T* dx, int
     if (e != cudaSuccess) return cuda_fail(e, "launch of the tokens' factors");
   }
   T* g = reinterpret_cast<T*>(ws + o.g);
-  float* acc = reinterpret_cast<float*>(ws + o.acc);
   CUtensorMap mx, mxt, mg, mgt;
   st = pair_operand_map(&mx, x, p.dt, false, p.tokens, p.dim, ld, "hidden states");
   if (st == KAIRO_STATUS_SUCCESS) st = pair_operand_map(&mxt, x, p.dt, true, p.dim, p.tokens, ld, "hidden states");
@@ -596,16 +713,25 @@ kairo_status run_grad(Problem p, const float* grad, const float* lse, T* dx, int
     st = launch_pair_gemm<FMT, false, false, GradEpi<T>>(mx, mw, shape_of(p.tokens, n, p.dim, kSegLogits), err, ga, s);
     if (st) return st;
     if (dx) {
-      typename SumEpi<T>::Args sa{dx, lddx, acc, ld, factor, static_cast<int>(p.tokens), static_cast<int>(p.dim),
-                                  v0 == 0, v0 + n == p.vocab, rows_aligned(dx, lddx, p.tokens)};
-      st = launch_pair_gemm<FMT, false, true, SumEpi<T>>(mg, mwt, shape_of(p.tokens, p.dim, n, kSegGrads), err, sa, s);
+      const bool direct = o.splits_x == 1 && o.cols >= p.vocab;
+      // a last piece of few columns has fewer parts than the others: those it leaves out keep their sums
+      const int splits = static_cast<int>(std::min<int64_t>(o.splits_x, ceil_div64(n, kPairK)));
+      typename SumEpi<T>::Args sa{dx, lddx, direct ? nullptr : reinterpret_cast<float*>(ws + o.acc_x), ld, factor,
+                                  static_cast<int>(p.tokens), static_cast<int>(p.dim), v0 == 0,
+                                  rows_aligned(dx, lddx, p.tokens)};
+      st = launch_pair_gemm<FMT, false, true, SumEpi<T>>(mg, mwt, shape_of(p.tokens, p.dim, n, kSegGrads, splits), err,
+                                                         sa, s);
+      if (st == KAIRO_STATUS_SUCCESS && !direct && v0 + n == p.vocab)
+        st = join<T>(sa.acc, ld, o.splits_x, p.tokens, p.dim, factor, dx, lddx, s);
       if (st) return st;
     }
     if (dw) {
       T* out = dw + v0 * lddw;
-      typename SumEpi<T>::Args sa{out, lddw, acc, ld, factor, static_cast<int>(n), static_cast<int>(p.dim), 1, 1,
-                                  rows_aligned(out, lddw, n)};
-      st = launch_pair_gemm<FMT, true, true, SumEpi<T>>(mgt, mxt, shape_of(n, p.dim, p.tokens, kSegGrads), err, sa, s);
+      typename SumEpi<T>::Args sa{out, lddw, o.splits_w > 1 ? reinterpret_cast<float*>(ws + o.acc_w) : nullptr, ld,
+                                  factor, static_cast<int>(n), static_cast<int>(p.dim), 1, rows_aligned(out, lddw, n)};
+      st = launch_pair_gemm<FMT, true, true, SumEpi<T>>(mgt, mxt, shape_of(n, p.dim, p.tokens, kSegGrads, o.splits_w),
+                                                        err, sa, s);
+      if (st == KAIRO_STATUS_SUCCESS && sa.acc) st = join<T>(sa.acc, ld, o.splits_w, n, p.dim, factor, out, lddw, s);
       if (st) return st;
     }
   }
