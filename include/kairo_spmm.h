@@ -555,8 +555,8 @@ KAIRO_API kairo_status kairo_gather_probe(const void* buffer, size_t buffer_byte
  *                              the loss (tokens for NONE, else one number); lse
  *                              from the forward call.  A token that does not
  *                              count has a dx of zeros and does not enter dw.
- * The workspace (256-byte aligned) depends on the sizes and on whether rows are
- * aligned; its contents do not outlive a call.  error_word: a device word that
+ * The workspace (256-byte aligned) depends on the sizes and on whether rows of the
+ * operands and results are 16-byte aligned; its contents do not outlive a call.  error_word: a device word that
  * receives a device error (a wait that ran out), as a workspace header's; it is
  * not cleared.  All asynchronous on `stream`.
  * ---------------------------------------------------------------------- */
@@ -566,8 +566,10 @@ typedef enum kairo_reduction {
   KAIRO_REDUCTION_MEAN = 2
 } kairo_reduction;
 KAIRO_API kairo_status kairo_vocab_loss_workspace_size(const void* x, int64_t ldx, const void* w, int64_t ldw,
-                                                       int64_t tokens, int64_t vocab, int64_t dim, int32_t backward,
-                                                       size_t* bytes);
+                                                       int64_t tokens, int64_t vocab, int64_t dim, size_t* bytes);
+KAIRO_API kairo_status kairo_vocab_loss_backward_workspace_size(const void* w, int64_t ldw, int64_t tokens,
+                                                                int64_t vocab, int64_t dim, void* dx, int64_t lddx,
+                                                                void* dw, int64_t lddw, size_t* bytes);
 KAIRO_API kairo_status kairo_vocab_loss(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t tokens,
                                         int64_t vocab, int64_t dim, kairo_dtype dtype, const void* targets,
                                         int32_t target_bytes, float scale, int32_t reduction, float* loss, float* lse,
@@ -592,7 +594,7 @@ KAIRO_API kairo_status kairo_vocab_loss_backward(const float* grad, const void* 
  *                            block): block-rows 2i and 2i + 1 are block-row i of
  *                            dG and of dU, zeros behind the last row
  * X (n x cols, leading dimension ldx) needs 16-byte aligned rows for more than
- * 32 tokens.  Sums are fp32, H, dG and dU rounded once.  A value of X that is
+ * 8 tokens.  Sums are fp32, H, dG and dU rounded once.  A value of X that is
  * not finite makes those results non-finite whose row keeps a block of Wg or Wu in
  * its column.  error_word: see kairo_vocab_loss; an entry out of range is
  * recorded there (KAIRO_DEVERR_BAD_INDEX) and counts as empty.  Asynchronous on `stream`.

@@ -253,7 +253,9 @@ _SIGNATURES = {
                                               c_size_t, c_void_p]),
     "kairo_embedding_grad_workspace_size": (c_int32, [c_int64, c_int64, c_int32, POINTER(c_size_t)]),
     "kairo_vocab_loss_workspace_size": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64,
-                                                  c_int32, POINTER(c_size_t)]),
+                                                  POINTER(c_size_t)]),
+    "kairo_vocab_loss_backward_workspace_size": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p,
+                                                           c_int64, c_void_p, c_int64, POINTER(c_size_t)]),
     "kairo_vocab_loss": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int32, c_void_p,
                                    c_int32, c_float, c_int32, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p,
                                    c_void_p]),

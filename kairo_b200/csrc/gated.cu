@@ -22,6 +22,9 @@
 // panels of X.  With blocks of 64 an entry costs a CTA 32 KB of X and 8 KB of weights for
 // 512 tensor cycles, 80 bytes a cycle (two separate products: 160).
 //
+// k_gated_stream (9 to 64 tokens of many block-rows).  A warp brings blocks and panels of X into a ring in shared
+// memory with the copy engine, four more multiply them (mma.sync), each CTA whole block-rows.
+//
 // k_gated_few (up to 32 tokens).  Bound by reading the blocks once.  A CTA takes 16
 // rows of a block-row, its warps share out the entries; mma.sync fragments come
 // straight from global memory, 16 bytes a lane (the order of k inside a block is
@@ -145,6 +148,7 @@ constexpr size_t gated_smem(int bm, int t) { return static_cast<size_t>(kGatedSt
 
 struct GatedItem {
   int tile, row, e0, e1;  // token tile, block-row, entries
+  int subs;               // subtiles of the tile
 };
 
 template <int BM, int T, int IN_FMT, typename TT, bool GRAD>
@@ -156,7 +160,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGatedThreads, 1)
   constexpr int SLOT = gated_slot_bytes(BM, T);
   constexpr int STAGE = gated_stage_bytes(BM, T);
   constexpr int PANEL = T * 128 * BM * 2;
-  constexpr uint32_t TX = PANEL + BM * BM * 2;  // bytes of one entry in one CTA
   constexpr uint32_t IDESC = ptx::make_idesc_f16(IN_FMT, 0u, 0u, 256u, 2 * BM);
   constexpr uint32_t SW = ptx::swizzle_code_for_row_bytes(BM * 2);
   constexpr uint32_t ACC = T * 2 * BM;  // columns of one accumulator
@@ -207,7 +210,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGatedThreads, 1)
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  constexpr int TOKENS = T * 256;  // of a cluster's tile
+  // A tile is T subtiles of 256 tokens, 128 of them in each CTA.  What is left of the tokens after the
+  // whole tiles is a tile of fewer subtiles, whose items come last.
+  constexpr int TOKENS = T * 256;
+  const int whole = args.n / TOKENS;
   const int tiles = (args.n + TOKENS - 1) / TOKENS;
   const int nitems = tiles * args.nbr;
   const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
@@ -218,9 +224,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGatedThreads, 1)
     const int per = args.group * args.nbr;
     const int g = t / per, r = t - g * per;
     const int t0 = g * args.group;
-    const int gn = min(args.group, tiles - t0);
-    it.row = r / gn;
-    it.tile = t0 + (r - it.row * gn);
+    const int gn = min(args.group, whole - t0);
+    if (t >= whole * args.nbr) {
+      it.row = t - whole * args.nbr;
+      it.tile = whole;
+      it.subs = (args.n - whole * TOKENS + 255) / 256;
+    } else {
+      it.row = r / gn;
+      it.tile = t0 + (r - it.row * gn);
+      it.subs = T;
+    }
     // offsets outside the entries are clamped by every role alike (and reported by the loads)
     it.e0 = min(max(__ldg(args.ent_ptr + it.row), 0), args.nentries);
     it.e1 = min(max(__ldg(args.ent_ptr + it.row + 1), it.e0), args.nentries);
@@ -251,12 +264,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGatedThreads, 1)
     }
     for (int t = first; t < nitems && alive; t += step) {
       const bool more = t + step < nitems;
+      n0 = make_int4(0, -1, -1, 0);
       if (more) {
         nxt = item(t + step);
         n0 = fetch(nxt, 0);
       }
       const int cnt = cur.e1 - cur.e0;
-      const int y0 = cur.tile * TOKENS + static_cast<int>(rank) * (T * 128);
+      const int y0 = cur.tile * TOKENS + static_cast<int>(rank) * 128;
+      const uint32_t bytes = 2u * static_cast<uint32_t>(cur.subs * 128 * BM * 2 + BM * BM * 2);  // of an entry, both CTAs
       for (int at = 0; at < cnt && alive; at += 32) {
         const int4 w = w0;
         if (at + 32 < cnt) w0 = fetch(cur, at + 32);
@@ -279,17 +294,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGatedThreads, 1)
           const uint32_t bar = ptx::peer_smem_u32(&full[sidx], 0);
           if (rank == 0) {
             if (lane == 0) issued[sidx] = static_cast<int>(sph) + 1;
-            ptx::mbar_expect_tx_if(lane == 0 ? 1u : 0u, &full[sidx], 2u * TX * static_cast<uint32_t>(take));
+            ptx::mbar_expect_tx_if(lane == 0 ? 1u : 0u, &full[sidx], bytes * static_cast<uint32_t>(take));
           }
           // one lane per box of 64 tokens and per block, so that all copies of a stage are issued at once
           const int e = lane / BOXES, part = lane - e * BOXES;  // entry of the stage; its panel's box, or its block
-          const uint32_t mine = e < take ? 1u : 0u;
+          const bool is_w = part == BOXES - 1;
+          const uint32_t mine = e < take && (is_w || part < 2 * cur.subs) ? 1u : 0u;
           const int ecol = __shfl_sync(0xffffffffu, col, (b0 + e) & 31);
           const int eblk = __shfl_sync(0xffffffffu, blk, (b0 + e) & 31);
           uint8_t* st = smem + sidx * STAGE + (mine ? e : 0) * SLOT;
-          const bool is_w = part == BOXES - 1;
           ptx::tma_load_2d_pair_if(mine, is_w ? st + PANEL : st + part * (64 * BM * 2), is_w ? map_w : map_x,
-                                   is_w ? 0 : ecol * BM, is_w ? eblk * BM : y0 + part * 64, bar, is_w ? pol_w : pol_x);
+                                   is_w ? 0 : ecol * BM, is_w ? eblk * BM : y0 + (part >> 1) * 256 + (part & 1) * 64, bar, is_w ? pol_w : pol_x);
           __syncwarp();
           if (rank == 0) ptx::mbar_arrive_if(lane == 0 ? 1u : 0u, &full[sidx]);
           if (++sidx == ST) {
@@ -336,7 +351,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGatedThreads, 1)
           for (int kk = 0; kk < BM / 16; ++kk) {
 #pragma unroll
             for (int i = 0; i < T; ++i)
-              ptx::mma_f16_ss_pair_if(leader, d + static_cast<uint32_t>(i * 2 * BM),
+              ptx::mma_f16_ss_pair_if(i < it.subs ? leader : 0u, d + static_cast<uint32_t>(i * 2 * BM),
                                       a_lo + s16 + ((i * 128 * BM * 2 + kk * 32) >> 4), a_hi,
                                       b_lo + s16 + ((kk * 32) >> 4), b_hi, IDESC, (at > 0 || e > 0 || kk > 0) ? 1u : 0u);
           }
@@ -382,7 +397,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGatedThreads, 1)
       const uint32_t at = tmem_base + lane_addr + static_cast<uint32_t>(slot) * ACC;
       for (int s = part; s < STEPS; s += 2) {
         const int i = s / (BM / UN), c0 = (s % (BM / UN)) * UN;
-        const int token = it.tile * TOKENS + static_cast<int>(rank) * (T * 128) + i * 128 + q * 32 + lane;
+        if (i >= it.subs) break;
+        const int token = it.tile * TOKENS + i * 256 + static_cast<int>(rank) * 128 + q * 32 + lane;
         float g[UN], u[UN];
         if (some) {
           if constexpr (UN == 32) {
@@ -489,7 +505,7 @@ constexpr int kFewWarps = 8;
 
 // NT * 8 tokens; grid: one CTA per 16 rows of a block-row.
 template <int BM, int NT, typename T, bool GRAD>
-__global__ void __launch_bounds__(32 * kFewWarps) k_gated_few(const GatedArgs a, int vec_x) {
+__global__ void __launch_bounds__(32 * kFewWarps, NT == 1 ? 3 : 2) k_gated_few(const GatedArgs a, int vec_x) {
   constexpr int SLICES = BM / 16;
   __shared__ float sums[kFewWarps][2][NT * 8][17];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -504,47 +520,79 @@ __global__ void __launch_bounds__(32 * kFewWarps) k_gated_few(const GatedArgs a,
     for (int j = 0; j < 4; ++j) g[i][j] = u[i][j] = 0.f;
   const uint16_t* blocks = static_cast<const uint16_t*>(a.blocks) + (slice * 16 + gid) * BM;
   const uint16_t* x = static_cast<const uint16_t*>(a.x);
-#pragma unroll 2
-  for (int e = e0 + warp; e < e1; e += kFewWarps) {
-    int4 w = __ldg(a.entries + e);
+  struct Step {
+    RowPart<BM> g0, g1, u0, u1, xs[NT];
+  };
+  // A warp's entries are read once, one a lane.  The operands of an entry are under way while the one
+  // before it is multiplied, unless the registers of both would cost a resident CTA.
+  constexpr bool AHEAD = BM < 64 || NT == 2;
+  for (int base = e0; base < e1; base += 32 * kFewWarps) {
+    const int mine = base + warp + lane * kFewWarps;
+    int4 w = make_int4(0, -1, -1, 0);
+    if (mine < e1) w = __ldg(a.entries + mine);
     if (static_cast<unsigned>(w.x) >= static_cast<unsigned>(a.nbc) || w.y < -1 || w.y >= a.nblocks || w.z < -1 ||
         w.z >= a.nblocks) {
       atomicCAS(a.err, 0u, KAIRO_DEVERR_BAD_INDEX);
       w = make_int4(0, -1, -1, 0);
     }
-    RowPart<BM> g0, g1, u0, u1, xs[NT];
-    g0.zero();
-    g1.zero();
-    u0.zero();
-    u1.zero();
-    if (w.y >= 0) {
-      const uint16_t* p = blocks + static_cast<int64_t>(w.y) * BM * BM;
-      g0.load(p, t);
-      g1.load(p + 8 * BM, t);
-    }
-    if (w.z >= 0) {
-      const uint16_t* p = blocks + static_cast<int64_t>(w.z) * BM * BM;
-      u0.load(p, t);
-      u1.load(p + 8 * BM, t);
-    }
-    const int left = a.k - w.x * BM;
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const int token = i * 8 + gid;
-      const uint16_t* p = x + static_cast<int64_t>(token) * a.ldx + w.x * BM;
-      xs[i].zero();
-      if (token < a.n) {
-        if (vec_x && left >= BM) xs[i].load(p, t);
-        else xs[i].load_edge(p, t, left);
+    const int cnt = max(0, min(32, (e1 - base - warp + kFewWarps - 1) / kFewWarps));
+    auto load = [&](Step& s, int j) {
+      const int col = __shfl_sync(0xffffffffu, w.x, j), gb = __shfl_sync(0xffffffffu, w.y, j),
+                ub = __shfl_sync(0xffffffffu, w.z, j);
+      if (gb >= 0) {
+        const uint16_t* p = blocks + static_cast<int64_t>(gb) * BM * BM;
+        s.g0.load(p, t);
+        s.g1.load(p + 8 * BM, t);
+      } else {
+        s.g0.zero();
+        s.g1.zero();
       }
-    }
-#pragma unroll
-    for (int s = 0; s < BM / 16; ++s)
+      if (ub >= 0) {
+        const uint16_t* p = blocks + static_cast<int64_t>(ub) * BM * BM;
+        s.u0.load(p, t);
+        s.u1.load(p + 8 * BM, t);
+      } else {
+        s.u0.zero();
+        s.u1.zero();
+      }
+      const int left = a.k - col * BM;
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        mma_16816<T>(g[i], g0.w[2 * s], g1.w[2 * s], g0.w[2 * s + 1], g1.w[2 * s + 1], xs[i].w[2 * s], xs[i].w[2 * s + 1]);
-        mma_16816<T>(u[i], u0.w[2 * s], u1.w[2 * s], u0.w[2 * s + 1], u1.w[2 * s + 1], xs[i].w[2 * s], xs[i].w[2 * s + 1]);
+        const int token = i * 8 + gid;
+        const uint16_t* p = x + static_cast<int64_t>(token) * a.ldx + col * BM;
+        if (token >= a.n) s.xs[i].zero();
+        else if (vec_x && left >= BM) s.xs[i].load(p, t);
+        else s.xs[i].load_edge(p, t, left);
       }
+    };
+    auto multiply = [&](const Step& s) {
+#pragma unroll
+      for (int q = 0; q < BM / 16; ++q)
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          const uint32_t x0 = s.xs[i].w[2 * q], x1 = s.xs[i].w[2 * q + 1];
+          mma_16816<T>(g[i], s.g0.w[2 * q], s.g1.w[2 * q], s.g0.w[2 * q + 1], s.g1.w[2 * q + 1], x0, x1);
+          mma_16816<T>(u[i], s.u0.w[2 * q], s.u1.w[2 * q], s.u0.w[2 * q + 1], s.u1.w[2 * q + 1], x0, x1);
+        }
+    };
+    if constexpr (AHEAD) {
+      Step s0, s1;
+      if (cnt > 0) load(s0, 0);
+      for (int j = 0; j < cnt; j += 2) {
+        if (j + 1 < cnt) load(s1, j + 1);
+        multiply(s0);
+        if (j + 1 < cnt) {
+          if (j + 2 < cnt) load(s0, j + 2);
+          multiply(s1);
+        }
+      }
+    } else {
+      for (int j = 0; j < cnt; ++j) {
+        Step s0;
+        load(s0, j);
+        multiply(s0);
+      }
+    }
   }
 #pragma unroll
   for (int i = 0; i < NT; ++i)
@@ -568,9 +616,281 @@ __global__ void __launch_bounds__(32 * kFewWarps) k_gated_few(const GatedArgs a,
   }
 }
 
+// ------------------------------------------------------------ blocks streamed for a batch of tokens
+
+constexpr int kStreamThreads = 160;  // four warps that multiply, one that loads
+constexpr int kStreamSmem = 110 * 1024;  // two CTAs an SM
+
+// Both blocks and the panel of X: multiples of the swizzle's period (256, 512, 1024 bytes) all three.
+constexpr int stream_entry_bytes(int bm, int nt) { return 2 * bm * bm * 2 + nt * 8 * bm * 2; }
+// Entries of one stage (a power of two): up to 16 KB of blocks and about 20 KB in all, and four lanes
+// each, so that one instruction issues a stage's copies (one lane's copies go out one after the other,
+// some 450 cycles each).
+constexpr int stream_group(int bm, int nt) {
+  int e = 1;
+  while (e < 8 && 2 * e * bm * bm <= 4096 && 2 * e * stream_entry_bytes(bm, nt) <= 20 * 1024) e *= 2;
+  return e;
+}
+constexpr int stream_stage_bytes(int bm, int nt) { return stream_group(bm, nt) * stream_entry_bytes(bm, nt); }
+constexpr int stream_sums_bytes(int bm, int nt) { return bm == 64 ? 0 : 4 * 2 * 16 * (nt * 8 + 1) * 4; }
+constexpr int stream_stages(int bm, int nt) {
+  return (kStreamSmem - 2048 - stream_sums_bytes(bm, nt)) / stream_stage_bytes(bm, nt);
+}
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix2(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr));
+}
+
+// Byte offset of 16-byte chunk c of row r in a box of BM columns, as the copy engine's swizzle lays it out.
+template <int BM>
+__device__ __forceinline__ uint32_t box_at(int r, int c) {
+  const int x = BM == 64 ? (r & 7) : BM == 32 ? ((r >> 1) & 3) : ((r >> 2) & 1);
+  return static_cast<uint32_t>(r * BM * 2 + ((c ^ x) * 16));
+}
+
+// NT * 8 tokens; persistent, a CTA takes whole block-rows.
+template <int BM, int NT, typename TT, bool GRAD>
+__global__ void __launch_bounds__(kStreamThreads, 2)
+    k_gated_stream(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
+                   const GatedArgs args) {
+  constexpr int ST = stream_stages(BM, NT);
+  constexpr int E = stream_group(BM, NT);
+  constexpr int ENTRY = stream_entry_bytes(BM, NT), STAGE = stream_stage_bytes(BM, NT);
+  constexpr int BLOCK = BM * BM * 2, PANEL = NT * 8 * BM * 2;
+  constexpr int SLICES = BM / 16, GROUPS = 4 / SLICES;  // warps: slice of 16 rows x group of entries
+  static_assert(ST >= 2, "stages");
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* sums = reinterpret_cast<float*>(smem + ST * STAGE);  // [4 warps][gate, up][16][NT * 8 + 1]
+  __shared__ uint64_t full[ST], empty[ST];
+  __shared__ uint8_t has[ST][E];  // bit 0: gate, bit 1: up
+  __shared__ int abort_s, issued[ST];
+  volatile int* abort_flag = &abort_s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      ptx::mbar_init(&full[s], 1);
+      ptx::mbar_init(&empty[s], 4);
+      issued[s] = 0;
+    }
+    abort_s = 0;
+    ptx::mbar_init_fence();
+  }
+  __syncthreads();
+  auto range = [&](int row, int& e0, int& e1) {
+    e0 = min(max(__ldg(args.ent_ptr + row), 0), args.nentries);
+    e1 = min(max(__ldg(args.ent_ptr + row + 1), e0), args.nentries);
+  };
+  int sidx = 0;
+  uint32_t sph = 0;
+  auto advance = [&]() {
+    if (++sidx == ST) {
+      sidx = 0;
+      sph ^= 1u;
+    }
+  };
+
+  if (warp == 4) {
+    // ------------------------------------------------------------ loads
+    const uint64_t pol_w = ptx::policy_evict_first();
+    const uint64_t pol_x = ptx::policy_evict_last();
+    const void* map_x = &tmap_x;
+    const void* map_w = &tmap_w;
+    bool alive = true;
+    auto fetch = [&](int e, int e1) { return e < e1 ? __ldg(args.entries + e) : make_int4(0, -1, -1, 0); };
+    int e0 = 0, e1 = 0, n0 = 0, n1 = 0;
+    int4 w0 = make_int4(0, -1, -1, 0), nw = w0;
+    const int first = blockIdx.x, step = gridDim.x;
+    if (first < args.nbr) {
+      range(first, e0, e1);
+      w0 = fetch(e0 + lane, e1);
+    }
+    for (int row = first; row < args.nbr && alive; row += step) {
+      if (row + step < args.nbr) {
+        range(row + step, n0, n1);
+        nw = fetch(n0 + lane, n1);
+      }
+      for (int at = e0; at < e1 && alive; at += 32) {
+        int4 w = w0;
+        if (at + 32 < e1) w0 = fetch(at + 32 + lane, e1);
+        if (static_cast<unsigned>(w.x) >= static_cast<unsigned>(args.nbc) || w.y < -1 || w.y >= args.nblocks ||
+            w.z < -1 || w.z >= args.nblocks) {
+          atomicCAS(args.err, 0u, KAIRO_DEVERR_BAD_INDEX);
+          w = make_int4(0, -1, -1, 0);
+        }
+        for (int b0 = 0; b0 < 32 && at + b0 < e1; b0 += E) {
+          const int take = min(E, e1 - at - b0);
+          int ok = ptx::wait_parity(&empty[sidx], sph ^ 1u, abort_flag, args.err, kTagEmpty, kWaitCycles);
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+          if (!ok) {
+            alive = false;
+            break;
+          }
+          // lanes 4 l .. 4 l + 2: gate block, up block and panel of entry b0 + l of the window
+          const int slot = lane >> 2, part = lane & 3;
+          const int src = (b0 + slot) & 31;
+          const int col = __shfl_sync(0xffffffffu, w.x, src), gb = __shfl_sync(0xffffffffu, w.y, src),
+                    ub = __shfl_sync(0xffffffffu, w.z, src);
+          const bool mine = slot < take;
+          const bool wanted = part == 0 ? gb >= 0 : part == 1 ? ub >= 0 : part == 2 && (gb >= 0 || ub >= 0);
+          const uint32_t issue = mine && wanted ? 1u : 0u;
+          const unsigned sent = __ballot_sync(0xffffffffu, issue != 0u);
+          const uint32_t bytes = static_cast<uint32_t>(__popc(sent & 0x33333333u) * BLOCK + __popc(sent & 0x44444444u) * PANEL);
+          if (lane == 0) issued[sidx] = static_cast<int>(sph) + 1;
+          if (mine && part == 0) has[sidx][slot] = static_cast<uint8_t>((gb >= 0 ? 1 : 0) | (ub >= 0 ? 2 : 0));
+          ptx::mbar_expect_tx_if(lane == 0 ? 1u : 0u, &full[sidx], bytes);
+          __syncwarp();
+          uint8_t* st = smem + sidx * STAGE + (mine ? slot : 0) * ENTRY + (part < 2 ? part : 2) * BLOCK;
+          const bool is_w = part < 2;
+          ptx::tma_load_2d_if(issue, st, is_w ? map_w : map_x, is_w ? 0 : col * BM, is_w ? (part == 0 ? gb : ub) * BM : 0,
+                              &full[sidx], is_w ? pol_w : pol_x);
+          __syncwarp();
+          ptx::mbar_arrive_if(lane == 0 ? 1u : 0u, &full[sidx]);
+          advance();
+        }
+      }
+      e0 = n0;
+      e1 = n1;
+      w0 = nw;
+    }
+  } else {
+    // ------------------------------------------------------------ products
+    const int slice = warp % SLICES, group = warp / SLICES;
+    const int gid = lane >> 2, t = lane & 3;
+    bool alive = true;
+    for (int row = blockIdx.x; row < args.nbr && alive; row += gridDim.x) {
+      int e0, e1;
+      range(row, e0, e1);
+      float g[NT][4], u[NT][4];
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) g[i][j] = u[i][j] = 0.f;
+      // the same stages as the loads: windows of 32 entries, E at a time
+      for (int at = e0; at < e1; at += E) {
+        const int take = min(E, e1 - at);
+        int ok = ptx::wait_parity(&full[sidx], sph, abort_flag, args.err, kTagFull, kWaitCycles);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) {
+          alive = false;
+          break;
+        }
+        for (int e = group; e < take; e += GROUPS) {
+          const int have = has[sidx][e];
+          const uint32_t st = ptx::smem_u32(smem + sidx * STAGE + e * ENTRY);
+          const int ar = slice * 16 + (lane & 15), ac = lane >> 4;   // A: 16 rows, two chunks
+          const int br = lane & 7, bc = lane >> 3;                   // B: 8 tokens, four chunks
+          uint32_t ga[BM / 16][4], ua[BM / 16][4];
+          if (have & 1) {
+#pragma unroll
+            for (int q = 0; q < BM / 16; ++q) ldmatrix4(ga[q], st + box_at<BM>(ar, 2 * q + ac));
+          }
+          if (have & 2) {
+#pragma unroll
+            for (int q = 0; q < BM / 16; ++q) ldmatrix4(ua[q], st + BLOCK + box_at<BM>(ar, 2 * q + ac));
+          }
+          // 32 k and up to 8 groups of tokens at a time; successive products go to different sums
+          constexpr int TG = NT < 8 ? NT : 8;
+#pragma unroll
+          for (int i0 = 0; i0 < NT; i0 += TG) {
+#pragma unroll
+            for (int h = 0; h < (BM + 31) / 32; ++h) {
+              uint32_t xb[TG][4];
+#pragma unroll
+              for (int i = 0; i < TG; ++i) {
+                if constexpr (BM == 16) ldmatrix2(xb[i], st + 2 * BLOCK + box_at<BM>((i0 + i) * 8 + br, bc & 1));
+                else ldmatrix4(xb[i], st + 2 * BLOCK + box_at<BM>((i0 + i) * 8 + br, 4 * h + bc));
+              }
+#pragma unroll
+              for (int q = 2 * h; q < 2 * h + 2 && q < BM / 16; ++q) {
+                const int k = 2 * (q & 1);
+                if (have == 3) {
+#pragma unroll
+                  for (int i = 0; i < TG; ++i) {
+                    mma_16816<TT>(g[i0 + i], ga[q][0], ga[q][1], ga[q][2], ga[q][3], xb[i][k], xb[i][k + 1]);
+                    mma_16816<TT>(u[i0 + i], ua[q][0], ua[q][1], ua[q][2], ua[q][3], xb[i][k], xb[i][k + 1]);
+                  }
+                } else if (have == 1) {
+#pragma unroll
+                  for (int i = 0; i < TG; ++i)
+                    mma_16816<TT>(g[i0 + i], ga[q][0], ga[q][1], ga[q][2], ga[q][3], xb[i][k], xb[i][k + 1]);
+                } else if (have == 2) {
+#pragma unroll
+                  for (int i = 0; i < TG; ++i)
+                    mma_16816<TT>(u[i0 + i], ua[q][0], ua[q][1], ua[q][2], ua[q][3], xb[i][k], xb[i][k + 1]);
+                }
+              }
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&empty[sidx]);
+        advance();
+      }
+      if (!alive) break;
+      if constexpr (GROUPS > 1) {
+        // the groups' sums meet in shared memory; group 0 carries on with the total
+        constexpr int PITCH = NT * 8 + 1;
+        float* own = sums + warp * 2 * 16 * PITCH;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int at = (gid + (j >> 1) * 8) * PITCH + i * 8 + 2 * t + (j & 1);
+            own[at] = g[i][j];
+            own[16 * PITCH + at] = u[i][j];
+          }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (group == 0) {
+#pragma unroll
+          for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int at = (gid + (j >> 1) * 8) * PITCH + i * 8 + 2 * t + (j & 1);
+#pragma unroll
+              for (int q = 1; q < GROUPS; ++q) {
+                const float* other = sums + (warp + q * SLICES) * 2 * 16 * PITCH;
+                g[i][j] += other[at];
+                u[i][j] += other[16 * PITCH + at];
+              }
+            }
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+      }
+      if (group == 0) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int token = i * 8 + 2 * t + (j & 1);
+            if (token < args.n)
+              gated_out<TT, GRAD, 1>(args, token, row, BM, slice * 16 + gid + (j >> 1) * 8, &g[i][j], &u[i][j]);
+          }
+      }
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag) {
+    int dummy = 0;
+    for (int s = 0; s < ST; ++s)
+      if (issued[s])
+        ptx::wait_parity(&full[s], static_cast<uint32_t>(issued[s] - 1), reinterpret_cast<volatile int*>(&dummy),
+                         args.err, kTagDrain, kWaitCycles);
+  }
+}
+
 // ------------------------------------------------------------ host side
 
+constexpr int kAnyTokens = 8;   // up to here X may have any alignment
 constexpr int kFewTokens = 32;
+constexpr int kStreamTokens = 64;
+constexpr int kStreamRows = 256;  // block-rows
 
 template <int BM, int NT, typename T, bool GRAD>
 void launch_few(const GatedArgs& a, cudaStream_t s) {
@@ -578,11 +898,45 @@ void launch_few(const GatedArgs& a, cudaStream_t s) {
   k_gated_few<BM, NT, T, GRAD><<<a.nbr * (BM / 16), 32 * kFewWarps, 0, s>>>(a, vec_x);
 }
 
+template <int BM, int NT, typename TT, int IN_FMT, bool GRAD>
+kairo_status launch_stream(const GatedArgs& a, cudaStream_t s) {
+  const CUtensorMapDataType dt = IN_FMT == 0 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  CUtensorMap mx, mw;
+  kairo_status st = make_map_2d(&mx, a.x, dt, 2, static_cast<uint64_t>(a.k), static_cast<uint64_t>(a.n),
+                                static_cast<uint64_t>(a.ldx), BM, NT * 8, "X");
+  if (st == KAIRO_STATUS_SUCCESS)
+    st = make_map_2d(&mw, a.blocks, dt, 2, BM, static_cast<uint64_t>(std::max(1, a.nblocks)) * BM, BM, BM, BM,
+                     "block storage");
+  if (st) return st;
+  auto* fn = &k_gated_stream<BM, NT, TT, GRAD>;
+  static std::atomic<uint64_t> ready{0};
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(fn), kStreamSmem, &ready);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic smem)");
+  const int grid = std::min(a.nbr, 2 * device_sm_count(current_device()));
+  fn<<<grid, kStreamThreads, kStreamSmem, s>>>(mx, mw, a);
+  e = cudaGetLastError();
+  return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "launch of k_gated_stream");
+}
+
 template <int BM, typename TT, int IN_FMT, bool GRAD>
 kairo_status run_gated(GatedArgs a, cudaStream_t s) {
+  // Streamed blocks where a CTA per block-row fills the SMs.  Blocks of 64, 32768 x 8192 at 20 % twice (the
+  // blocks alone 33 us): 16 / 32 / 64 tokens 56 / 64 / 86 us, by fragments 64 / 82 / -, by k_gated 121;
+  // 4096 x 4096 (64 block-rows): 32 tokens 25 us, by fragments 15; 64 tokens 31, by k_gated 23.  Smaller blocks:
+  // fragments up to 32 tokens (12288 x 4096, blocks of 32, 24 tokens: 26 us against 40), then streamed (64
+  // tokens: 51 against 82 by k_gated).
+  const bool rows = a.nbr >= kStreamRows;
+  if (BM == 64 ? rows && a.n > 8 && a.n <= kStreamTokens : a.n > kFewTokens && a.n <= kStreamTokens) {
+    if constexpr (BM == 64) {
+      if (a.n <= 16) return launch_stream<BM, 2, TT, IN_FMT, GRAD>(a, s);
+      if (a.n <= 32) return launch_stream<BM, 4, TT, IN_FMT, GRAD>(a, s);
+    }
+    return launch_stream<BM, 8, TT, IN_FMT, GRAD>(a, s);
+  }
   if (a.n <= kFewTokens) {
     if (a.n <= 8) launch_few<BM, 1, TT, GRAD>(a, s);
     else if (a.n <= 16) launch_few<BM, 2, TT, GRAD>(a, s);
+    else if (a.n <= 24) launch_few<BM, 3, TT, GRAD>(a, s);
     else launch_few<BM, 4, TT, GRAD>(a, s);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "launch of k_gated_few");
@@ -603,7 +957,7 @@ kairo_status run_gated(GatedArgs a, cudaStream_t s) {
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic smem)");
     const int tiles = static_cast<int>(ceil_div64(a.n, T * 256));
     // a group's X takes about a quarter of the L2
-    a.group = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(tiles, (32LL << 20) / (static_cast<int64_t>(T) * 512 * a.k))));
+    a.group = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::max(1, a.n / (T * 256)), (32LL << 20) / (static_cast<int64_t>(T) * 512 * a.k))));
     const int64_t items = static_cast<int64_t>(tiles) * a.nbr;
     const int clusters = static_cast<int>(std::min<int64_t>(items, std::max(1, device_sm_count(current_device()) / 2)));
     fn<<<2 * clusters, kGatedThreads, gated_smem(BM, T), s>>>(mx, mw, a);
@@ -648,7 +1002,7 @@ kairo_status gated_check(const kairo_gated* w, const void* x, int64_t ldx, int64
     return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
   if (reinterpret_cast<uintptr_t>(w->entries) % 16 || reinterpret_cast<uintptr_t>(w->blocks) % 16)
     return fail(KAIRO_STATUS_INVALID_VALUE, "entries and blocks must be 16-byte aligned");
-  if (n > kFewTokens && w->nentries > 0 && !row_vec(x, ldx, n))
+  if (n > kAnyTokens && w->nentries > 0 && !row_vec(x, ldx, n))
     return fail(KAIRO_STATUS_INVALID_VALUE, "X must have 16-byte aligned rows");
   return KAIRO_STATUS_SUCCESS;
 }

@@ -125,13 +125,31 @@ struct StatsEpi {
   }
 };
 
-// A warp's 32 rows x kPairEpiCols results, a row a lane, rounded to T at p (row pitch ld, `rows` and
-// `cols` of them exist).  They pass through shared memory, 64 columns at a time, so that a store
-// instruction writes 128 bytes of each of four rows (a row a lane: 16 bytes of 32 rows, and 2 where
-// rows are not aligned; there a warp writes one row at a time, 4 bytes a lane).
+// The 8 16-bit values from value `e` (0..7) on of the 16 in a, b.
+__device__ __forceinline__ uint4 shift8(uint4 a, uint4 b, int e) {
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  if (e & 4) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  }
+  if (e & 2) {
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  }
+  if (e & 1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A warp's 32 rows x kPairEpiCols results, a row a lane, rounded to T at p (16-byte aligned rows of
+// pitch ld; `rows` and `cols` of them exist).  They pass through shared memory, 64 columns at a
+// time, so that a store instruction writes 128 bytes of each of four rows (a row a lane: 16 bytes of
+// each of 32 rows).
 template <typename T>
 __device__ __forceinline__ void put_rows(uint8_t* out, const float (&v)[kPairEpiCols], T* p, int64_t ld, int rows,
-                                         int cols, bool vec) {
+                                         int cols) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int h = 0; h < kPairEpiCols; h += 64) {
@@ -144,37 +162,21 @@ __device__ __forceinline__ void put_rows(uint8_t* out, const float (&v)[kPairEpi
       store_f32<T, 8>(reinterpret_cast<T*>(out + lane * 128 + ((c ^ (lane & 7)) * 16)), w);
     }
     __syncwarp();
-    if (vec) {
-      const int c = lane & 7;
-      const int n = cols - (h + 8 * c);
+    const int c = lane & 7;
+    const int n = cols - (h + 8 * c);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = 4 * i + (lane >> 3);
-        if (r >= rows || n <= 0) continue;
-        const uint4 w = *reinterpret_cast<const uint4*>(out + r * 128 + ((c ^ (r & 7)) * 16));
-        T* dst = p + r * ld + h + 8 * c;
-        if (n >= 8) {
-          *reinterpret_cast<uint4*>(dst) = w;
-        } else {
-          const T* e = reinterpret_cast<const T*>(&w);
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + (lane >> 3);
+      if (r >= rows || n <= 0) continue;
+      const uint4 w = *reinterpret_cast<const uint4*>(out + r * 128 + ((c ^ (r & 7)) * 16));
+      T* dst = p + r * ld + h + 8 * c;
+      if (n >= 8) {
+        *reinterpret_cast<uint4*>(dst) = w;
+      } else {
+        const T* e = reinterpret_cast<const T*>(&w);
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (j < n) dst[j] = e[j];
-        }
-      }
-    } else {
-      const int n = min(64, cols - h);
-      for (int r = 0; r < rows; ++r) {
-        T* dst = p + r * ld + h;
-        auto at = [&](int j) { return *reinterpret_cast<const uint16_t*>(out + r * 128 + (((j >> 3) ^ (r & 7)) * 16) + (j & 7) * 2); };
-        // pairs on 4-byte boundaries; an odd row begins and ends with half a pair
-        const int odd = static_cast<int>((reinterpret_cast<uintptr_t>(dst) >> 1) & 1u);
-        const int j = 2 * lane - odd;
-        uint16_t* d = reinterpret_cast<uint16_t*>(dst);
-        if (j >= 0 && j + 1 < n) *reinterpret_cast<uint32_t*>(d + j) = at(j) | (static_cast<uint32_t>(at(j + 1)) << 16);
-        else if (j >= 0 && j < n) d[j] = at(j);
-        else if (j == -1) d[0] = at(0);
-        if (odd && lane == 0 && n == 64) d[63] = at(63);
+        for (int j = 0; j < 8; ++j)
+          if (j < n) dst[j] = e[j];
       }
     }
     __syncwarp();
@@ -261,7 +263,7 @@ struct GradEpi {
       for (int j = 0; j < kPairEpiCols; ++j)
         if (j >= n) v[j] = 0.f;
     }
-    put_rows<T>(out, v, a.g + static_cast<int64_t>(token0) * a.ldg + col0, a.ldg, a.tokens - token0, kPairEpiCols, true);
+    put_rows<T>(out, v, a.g + static_cast<int64_t>(token0) * a.ldg + col0, a.ldg, a.tokens - token0, kPairEpiCols);
   }
 
   __device__ void done() {}
@@ -272,13 +274,13 @@ struct GradEpi {
 template <typename T>
 struct SumEpi {
   struct Args {
-    T* out;
+    T* out;            // rows 16-byte aligned
     int64_t ldo;
     float* acc;        // [splits][rows][ldacc], rows 16-byte aligned; NULL: to `out`
     int64_t ldacc;
     const float* factor;
     int rows, cols;
-    int first, vec;
+    int first;
   };
   const Args& a;
   int row, part;
@@ -299,7 +301,7 @@ struct SumEpi {
     } else {
 #pragma unroll
       for (int j = 0; j < kPairEpiCols; ++j) v[j] *= factor;
-      put_rows<T>(out, v, a.out + static_cast<int64_t>(r0) * a.ldo + col0, a.ldo, min(rows, 32), cols, a.vec != 0);
+      put_rows<T>(out, v, a.out + static_cast<int64_t>(r0) * a.ldo + col0, a.ldo, rows, cols);
     }
   }
 
@@ -385,22 +387,35 @@ __global__ void __launch_bounds__(1024) k_lse(const float2* __restrict__ part, i
   if (threadIdx.x == 0) *loss = reduction == kMean ? sum / fmaxf(count, 1.f) : sum;
 }
 
-// out = *factor * the splits' sums, in their order.
-template <typename T>
+// out = *factor * the splits' sums.  WAYS threads share the splits of 4 columns (their sums are added in
+// a fixed order): one thread would wait for 64 of them in turn.
+template <typename T, int WAYS>
 __global__ void __launch_bounds__(256) k_join(const float* __restrict__ acc, int64_t ldacc, int splits, int64_t rows,
                                               int64_t cols, const float* __restrict__ factor, T* __restrict__ out,
                                               int64_t ldo) {
   const int64_t groups = (cols + 3) / 4, total = rows * groups;
   const float f = *factor;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+  const int way = threadIdx.x % WAYS;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (256 / WAYS);
+  for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * (256 / WAYS); i0 < total; i0 += step) {
+    const int64_t i = i0 + threadIdx.x / WAYS;
     const int64_t r = i / groups, c = (i - r * groups) * 4;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int k = 0; k < splits; ++k) {
-      const float4 w = __ldcs(reinterpret_cast<const float4*>(acc + (k * rows + r) * ldacc + c));
-      s = make_float4(s.x + w.x, s.y + w.y, s.z + w.z, s.w + w.w);
+    if (i < total) {
+#pragma unroll 8
+      for (int k = way; k < splits; k += WAYS) {
+        const float4 w = __ldcs(reinterpret_cast<const float4*>(acc + (k * rows + r) * ldacc + c));
+        s = make_float4(s.x + w.x, s.y + w.y, s.z + w.z, s.w + w.w);
+      }
     }
+#pragma unroll
+    for (int o = 1; o < WAYS; o <<= 1) {
+      s.x += __shfl_xor_sync(0xffffffffu, s.x, o);
+      s.y += __shfl_xor_sync(0xffffffffu, s.y, o);
+      s.z += __shfl_xor_sync(0xffffffffu, s.z, o);
+      s.w += __shfl_xor_sync(0xffffffffu, s.w, o);
+    }
+    if (i >= total || way != 0) continue;
     const float v[4] = {s.x * f, s.y * f, s.z * f, s.w * f};
     T* dst = out + r * ldo + c;
     if (c + 4 <= cols && reinterpret_cast<uintptr_t>(dst) % 8 == 0) {
@@ -458,8 +473,15 @@ __device__ void prep_factors(const PrepArgs& p) {
   if (threadIdx.x == 0) *p.factor = shared_factor * p.scale / p.lift;
 }
 
+// A power of two of lanes, 32 at most, takes a row of `pieces` vectors: no division per vector.
+__device__ __forceinline__ int lanes_for(int64_t pieces) {
+  int l = 1;
+  while (l < 32 && l < pieces) l <<= 1;
+  return l;
+}
+
 __global__ void __launch_bounds__(256) k_rows(const uint16_t* __restrict__ src, int64_t lds, int64_t rows, int64_t cols,
-                                              uint16_t* __restrict__ dst, int64_t ldd, int vec, Targets ids, int vocab,
+                                              uint16_t* __restrict__ dst, int64_t ldd, Targets ids, int vocab,
                                               PrepArgs prep) {
   int cta = blockIdx.x, ctas = gridDim.x;
   if (prep.f) {
@@ -467,28 +489,80 @@ __global__ void __launch_bounds__(256) k_rows(const uint16_t* __restrict__ src, 
     --cta;
     --ctas;
   }
-  const int64_t pieces = ldd / 8, total = rows * pieces;
-  for (int64_t i = static_cast<int64_t>(cta) * blockDim.x + threadIdx.x; i < total;
-       i += static_cast<int64_t>(ctas) * blockDim.x) {
-    const int64_t r = i / pieces, c = (i - r * pieces) * 8;
-    uint4 w = make_uint4(0u, 0u, 0u, 0u);
+  const int64_t pieces = ldd / 8;
+  const int lanes = lanes_for(pieces), per = 256 / lanes;
+  const uint16_t* end = src + (rows - 1) * lds + cols;  // nothing is read outside [src, end)
+  for (int64_t r = static_cast<int64_t>(cta) * per + threadIdx.x / lanes; r < rows; r += static_cast<int64_t>(ctas) * per) {
     bool live = true;
     if (ids.p) {
       const int64_t id = ids[r];
       live = id >= 0 && id < vocab;
     }
-    if (live) {
-      const uint16_t* p = src + r * lds + c;
-      if (vec && c + 8 <= cols) {
-        w = *reinterpret_cast<const uint4*>(p);
-      } else {
-        uint32_t h[8];
+    // four vectors at a time, so that their loads are under way together
+    for (int64_t q0 = threadIdx.x % lanes; q0 < pieces; q0 += 4 * lanes) {
+      uint4 lo[4], hi[4];
+      bool whole[4];
+      const uint16_t* row = src + r * lds;
+      // past a 16-byte boundary (the same for all vectors of a row)
+      const int e = static_cast<int>((reinterpret_cast<uintptr_t>(row) >> 1) & 7u);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) h[j] = c + j < cols ? p[j] : 0u;
-        w = make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
+      for (int u = 0; u < 4; ++u) {
+        const int64_t c = (q0 + u * lanes) * 8;
+        const uint16_t* p = row + c - e;
+        whole[u] = live && c + 8 <= cols && p >= src && p + (e ? 16 : 8) <= end;
+        lo[u] = whole[u] ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0u, 0u, 0u, 0u);
+        hi[u] = whole[u] && e ? __ldg(reinterpret_cast<const uint4*>(p) + 1) : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t q = q0 + u * lanes, c = q * 8;
+        if (q >= pieces) break;
+        uint4 w = shift8(lo[u], hi[u], e);
+        if (live && !whole[u]) {
+          uint32_t h[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) h[j] = c + j < cols ? row[c + j] : 0u;
+          w = make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
+        }
+        *reinterpret_cast<uint4*>(dst + r * ldd + c) = w;
       }
     }
-    *reinterpret_cast<uint4*>(dst + r * ldd + c) = w;
+  }
+}
+
+// The way back: rows of a 16-byte aligned src (pitch lds) to rows at any address.
+__global__ void __launch_bounds__(256) k_rows_back(const uint16_t* __restrict__ src, int64_t lds, int64_t rows,
+                                                   int64_t cols, uint16_t* __restrict__ dst, int64_t ldd) {
+  const int64_t pieces = cols / 8 + 2;  // the values before the first 16-byte boundary, vectors, the rest
+  const int lanes = lanes_for(pieces), per = 256 / lanes;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / lanes; r < rows;
+       r += static_cast<int64_t>(gridDim.x) * per) {
+    const uint16_t* p = src + r * lds;
+    uint16_t* d = dst + r * ldd;
+    const int lead = static_cast<int>((8u - static_cast<unsigned>(reinterpret_cast<uintptr_t>(d) >> 1)) & 7u);
+    for (int64_t q0 = threadIdx.x % lanes; q0 < pieces; q0 += 4 * lanes) {
+      uint4 lo[4], hi[4];
+      const int e = lead & 7;  // of every vector's first value past a 16-byte boundary of src
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t q = q0 + u * lanes, e0 = lead + 8 * (q - 1);
+        const bool whole = q > 0 && e0 + 8 <= cols;
+        const uint4* at = reinterpret_cast<const uint4*>(p + (whole ? e0 - e : 0));
+        lo[u] = whole ? __ldg(at) : make_uint4(0u, 0u, 0u, 0u);
+        hi[u] = whole && e ? __ldg(at + 1) : make_uint4(0u, 0u, 0u, 0u);  // e0 + 8 <= cols <= lds: within the row
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t q = q0 + u * lanes, e0 = lead + 8 * (q - 1);
+        if (q >= pieces) break;
+        if (q > 0 && e0 + 8 <= cols) {
+          *reinterpret_cast<uint4*>(d + e0) = shift8(lo[u], hi[u], e);
+        } else {
+          const int64_t from = q == 0 ? 0 : e0, to = q == 0 ? min(static_cast<int64_t>(lead), cols) : cols;
+          for (int64_t i = from; i < to; ++i) d[i] = p[i];
+        }
+      }
+    }
   }
 }
 
@@ -544,10 +618,18 @@ LossWs loss_ws(const Problem& p) {
   return o;
 }
 
+struct Results {
+  void* dx;
+  int64_t lddx;
+  void* dw;
+  int64_t lddw;
+};
+
 struct GradWs {
-  size_t f, factor, acc_x, acc_w, x, w, g, total;
+  size_t f, factor, acc_x, acc_w, x, w, g, out, total;
   int64_t cols;
   int splits_x, splits_w;  // parts of the vocabulary piece for dX, of the tokens for dW
+  bool direct_x;           // dX leaves from its product
 };
 
 // Parts of k for a product of rows x cols: tiles that fill the clusters' rounds evenly, against the fp32
@@ -569,7 +651,8 @@ int splits_for(int64_t rows, int64_t cols, int64_t k) {
   return best;
 }
 
-GradWs grad_ws(const Problem& p) {
+// A dX whose rows are not 16-byte aligned leaves as fp32 sums and k_join, such a dW through a copy.
+GradWs grad_ws(const Problem& p, const Results& r) {
   GradWs o{};
   size_t at = kWorkspaceHeaderBytes;
   auto take = [&](size_t bytes) {
@@ -584,9 +667,12 @@ GradWs grad_ws(const Problem& p) {
   o.x = take(2 * ld * static_cast<size_t>(p.tokens));
   o.splits_x = splits_for(p.tokens, p.dim, std::min(o.cols, p.vocab));
   o.splits_w = splits_for(std::min(o.cols, p.vocab), p.dim, p.tokens);
-  if (o.cols < p.vocab || o.splits_x > 1) o.acc_x = take(4 * ld * static_cast<size_t>(p.tokens) * o.splits_x);
-  if (o.splits_w > 1) o.acc_w = take(4 * ld * static_cast<size_t>(std::min(o.cols, p.vocab)) * o.splits_w);
+  o.direct_x = o.cols >= p.vocab && o.splits_x == 1 && rows_aligned(r.dx, r.lddx, p.tokens);
+  if (r.dx && !o.direct_x) o.acc_x = take(4 * ld * static_cast<size_t>(p.tokens) * o.splits_x);
+  if (r.dw && o.splits_w > 1) o.acc_w = take(4 * ld * static_cast<size_t>(std::min(o.cols, p.vocab)) * o.splits_w);
   if (!rows_aligned(p.w, p.ldw, p.vocab)) o.w = take(2 * ld * static_cast<size_t>(p.vocab));
+  if (r.dw && o.splits_w == 1 && !rows_aligned(r.dw, r.lddw, p.vocab))
+    o.out = take(2 * ld * static_cast<size_t>(std::min(o.cols, p.vocab)));
   o.g = take(2 * static_cast<size_t>(p.tokens) * static_cast<size_t>(o.cols));
   o.total = at;
   return o;
@@ -612,7 +698,7 @@ kairo_status aligned_rows(const void** src, int64_t* ld, int64_t rows, int64_t c
   const int64_t work = ceil_div64(rows * (ldd / 8), 256);
   const int grid = static_cast<int>(std::min<int64_t>(work, device_sm_count(current_device()) * 16));
   k_rows<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(*src), *ld, rows, cols, reinterpret_cast<uint16_t*>(dst), ldd,
-                              0, Targets{nullptr, 8}, 0, PrepArgs{});
+                              Targets{nullptr, 8}, 0, PrepArgs{});
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "launch of the row copy");
   *src = dst;
@@ -643,9 +729,14 @@ PairShape shape_of(int64_t rows, int64_t cols, int64_t k, int seg, int splits = 
 template <typename T>
 kairo_status join(const float* acc, int64_t ldacc, int splits, int64_t rows, int64_t cols, const float* factor, T* out,
                   int64_t ldo, cudaStream_t s) {
-  const int64_t work = ceil_div64(rows * ceil_div64(cols, 4), 256);
-  const int grid = static_cast<int>(std::min<int64_t>(work, device_sm_count(current_device()) * 16));
-  k_join<T><<<grid, 256, 0, s>>>(acc, ldacc, splits, rows, cols, factor, out, ldo);
+  const int64_t groups = rows * ceil_div64(cols, 4);
+  const int64_t most = device_sm_count(current_device()) * 16;
+  if (splits >= 8)
+    k_join<T, 8><<<static_cast<int>(std::min<int64_t>(ceil_div64(groups, 32), most)), 256, 0, s>>>(
+        acc, ldacc, splits, rows, cols, factor, out, ldo);
+  else
+    k_join<T, 1><<<static_cast<int>(std::min<int64_t>(ceil_div64(groups, 256), most)), 256, 0, s>>>(
+        acc, ldacc, splits, rows, cols, factor, out, ldo);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "launch of k_join");
 }
@@ -675,9 +766,10 @@ kairo_status run_loss(Problem p, float* loss, float* lse, uint8_t* ws, unsigned*
 }
 
 template <typename T, int FMT>
-kairo_status run_grad(Problem p, const float* grad, const float* lse, T* dx, int64_t lddx, T* dw, int64_t lddw,
-                      uint8_t* ws, unsigned* err, cudaStream_t s) {
-  const GradWs o = grad_ws(p);
+kairo_status run_grad(Problem p, const float* grad, const float* lse, const Results& res, uint8_t* ws, unsigned* err,
+                      cudaStream_t s) {
+  const GradWs o = grad_ws(p, res);
+  T *dx = static_cast<T*>(res.dx), *dw = static_cast<T*>(res.dw);
   const int64_t ld = static_cast<int64_t>(align_up(static_cast<size_t>(p.dim), 8));
   kairo_status st = aligned_rows(&p.w, &p.ldw, p.vocab, p.dim, ws + o.w, s);
   if (st) return st;
@@ -690,7 +782,7 @@ kairo_status run_grad(Problem p, const float* grad, const float* lse, T* dx, int
     const int64_t work = ceil_div64(p.tokens * (ld / 8), 256);
     const int grid = 1 + static_cast<int>(std::min<int64_t>(work, device_sm_count(current_device()) * 8));
     k_rows<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(p.x), p.ldx, p.tokens, p.dim, static_cast<uint16_t*>(x), ld,
-                                rows_aligned(p.x, p.ldx, p.tokens) ? 1 : 0, p.ids, static_cast<int>(p.vocab), pa);
+                                p.ids, static_cast<int>(p.vocab), pa);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "launch of the tokens' factors");
   }
@@ -713,26 +805,33 @@ kairo_status run_grad(Problem p, const float* grad, const float* lse, T* dx, int
     st = launch_pair_gemm<FMT, false, false, GradEpi<T>>(mx, mw, shape_of(p.tokens, n, p.dim, kSegLogits), err, ga, s);
     if (st) return st;
     if (dx) {
-      const bool direct = o.splits_x == 1 && o.cols >= p.vocab;
       // a last piece of few columns has fewer parts than the others: those it leaves out keep their sums
       const int splits = static_cast<int>(std::min<int64_t>(o.splits_x, ceil_div64(n, kPairK)));
-      typename SumEpi<T>::Args sa{dx, lddx, direct ? nullptr : reinterpret_cast<float*>(ws + o.acc_x), ld, factor,
-                                  static_cast<int>(p.tokens), static_cast<int>(p.dim), v0 == 0,
-                                  rows_aligned(dx, lddx, p.tokens)};
+      typename SumEpi<T>::Args sa{dx, res.lddx, o.direct_x ? nullptr : reinterpret_cast<float*>(ws + o.acc_x), ld,
+                                  factor, static_cast<int>(p.tokens), static_cast<int>(p.dim), v0 == 0};
       st = launch_pair_gemm<FMT, false, true, SumEpi<T>>(mg, mwt, shape_of(p.tokens, p.dim, n, kSegGrads, splits), err,
                                                          sa, s);
-      if (st == KAIRO_STATUS_SUCCESS && !direct && v0 + n == p.vocab)
-        st = join<T>(sa.acc, ld, o.splits_x, p.tokens, p.dim, factor, dx, lddx, s);
+      if (st == KAIRO_STATUS_SUCCESS && !o.direct_x && v0 + n == p.vocab)
+        st = join<T>(sa.acc, ld, o.splits_x, p.tokens, p.dim, factor, dx, res.lddx, s);
       if (st) return st;
     }
     if (dw) {
-      T* out = dw + v0 * lddw;
-      typename SumEpi<T>::Args sa{out, lddw, o.splits_w > 1 ? reinterpret_cast<float*>(ws + o.acc_w) : nullptr, ld,
-                                  factor, static_cast<int>(n), static_cast<int>(p.dim), 1, rows_aligned(out, lddw, n)};
+      T* out = dw + v0 * res.lddw;
+      const bool copy = o.splits_w == 1 && !rows_aligned(dw, res.lddw, p.vocab);
+      typename SumEpi<T>::Args sa{copy ? reinterpret_cast<T*>(ws + o.out) : out, copy ? ld : res.lddw,
+                                  o.splits_w > 1 ? reinterpret_cast<float*>(ws + o.acc_w) : nullptr, ld,
+                                  factor, static_cast<int>(n), static_cast<int>(p.dim), 1};
       st = launch_pair_gemm<FMT, true, true, SumEpi<T>>(mgt, mxt, shape_of(n, p.dim, p.tokens, kSegGrads, o.splits_w),
                                                         err, sa, s);
-      if (st == KAIRO_STATUS_SUCCESS && sa.acc) st = join<T>(sa.acc, ld, o.splits_w, n, p.dim, factor, out, lddw, s);
+      if (st == KAIRO_STATUS_SUCCESS && sa.acc) st = join<T>(sa.acc, ld, o.splits_w, n, p.dim, factor, out, res.lddw, s);
       if (st) return st;
+      if (copy) {
+        const int grid = static_cast<int>(std::min<int64_t>(ceil_div64(n, 8), device_sm_count(current_device()) * 16));
+        k_rows_back<<<grid, 256, 0, s>>>(reinterpret_cast<const uint16_t*>(sa.out), ld, n, p.dim,
+                                         reinterpret_cast<uint16_t*>(out), res.lddw);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return cuda_fail(e, "launch of the row copy");
+      }
     }
   }
   return KAIRO_STATUS_SUCCESS;
@@ -744,13 +843,23 @@ kairo_status run_grad(Problem p, const float* grad, const float* lse, T* dx, int
 using namespace kairo;
 
 extern "C" kairo_status kairo_vocab_loss_workspace_size(const void* x, int64_t ldx, const void* w, int64_t ldw,
-                                                        int64_t tokens, int64_t vocab, int64_t dim, int32_t backward,
-                                                        size_t* bytes) {
+                                                        int64_t tokens, int64_t vocab, int64_t dim, size_t* bytes) {
   if (!bytes) return fail(KAIRO_STATUS_INVALID_VALUE, "null argument");
   const Problem p{x, ldx, w, ldw, tokens, vocab, dim, KAIRO_DTYPE_BF16, Targets{nullptr, 8}, 1.f, kNone};
   const kairo_status st = check_problem(p);
   if (st) return st;
-  *bytes = backward ? grad_ws(p).total : loss_ws(p).total;
+  *bytes = loss_ws(p).total;
+  return KAIRO_STATUS_SUCCESS;
+}
+
+extern "C" kairo_status kairo_vocab_loss_backward_workspace_size(const void* w, int64_t ldw, int64_t tokens,
+                                                                 int64_t vocab, int64_t dim, void* dx, int64_t lddx,
+                                                                 void* dw, int64_t lddw, size_t* bytes) {
+  if (!bytes) return fail(KAIRO_STATUS_INVALID_VALUE, "null argument");
+  const Problem p{nullptr, dim, w, ldw, tokens, vocab, dim, KAIRO_DTYPE_BF16, Targets{nullptr, 8}, 1.f, kNone};
+  const kairo_status st = check_problem(p);
+  if (st) return st;
+  *bytes = grad_ws(p, Results{dx, lddx, dw, lddw}).total;
   return KAIRO_STATUS_SUCCESS;
 }
 
@@ -798,11 +907,10 @@ extern "C" kairo_status kairo_vocab_loss_backward(const float* grad, const void*
   if (!grad || !x || !w || !targets || !lse || !workspace || !error_word)
     return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
   if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(KAIRO_STATUS_INVALID_VALUE, "workspace must be 256-byte aligned");
-  if (workspace_bytes < grad_ws(p).total) return fail(KAIRO_STATUS_WORKSPACE_TOO_SMALL, "loss workspace too small");
+  const Results res{dx, lddx, dw, lddw};
+  if (workspace_bytes < grad_ws(p, res).total) return fail(KAIRO_STATUS_WORKSPACE_TOO_SMALL, "loss workspace too small");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   return dtype == KAIRO_DTYPE_F16
-             ? run_grad<__half, 0>(p, grad, lse, static_cast<__half*>(dx), lddx, static_cast<__half*>(dw), lddw, ws,
-                                   error_word, s)
-             : run_grad<__nv_bfloat16, 1>(p, grad, lse, static_cast<__nv_bfloat16*>(dx), lddx,
-                                          static_cast<__nv_bfloat16*>(dw), lddw, ws, error_word, s);
+             ? run_grad<__half, 0>(p, grad, lse, res, ws, error_word, s)
+             : run_grad<__nv_bfloat16, 1>(p, grad, lse, res, ws, error_word, s);
 }

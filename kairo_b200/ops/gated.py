@@ -27,19 +27,13 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from kairo_b200 import _lib
-from kairo_b200.ops.backward import (
-    BlockSparseLinear,
-    TransposedBsr,
-    bsr_transpose,
-    sparse_linear_weight_grad,
-    transpose_values,
-)
-from kairo_b200.ops.spmm import sparse_linear
+from kairo_b200.ops.backward import BlockSparseLinear, bsr_transpose
+from kairo_b200.ops.spmm import KernelConfig, _bsr_desc
 from kairo_b200.ops.token_embedding import _ld, _rows
 from kairo_b200.types import BlockSparseMatrix
 
 _ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
-_FEW_TOKENS = 32  # up to here X may have any alignment
+_ANY_TOKENS = 8  # up to here X may have any alignment
 
 
 @dataclass(frozen=True)
@@ -119,20 +113,53 @@ class GatedWeights:
                                  shape=(rows, self.shape[1]), block_size=(self.block, self.block),
                                  blk_idx=self.blk_idx)
 
-    def _transposed(self) -> TransposedBsr:
-        """The stacked matrix transposed, values of this call: its structure is made once per pattern."""
-        a = self.stacked()
-        if "t" not in self._structure:
-            t = bsr_transpose(a)
-            perm_stored = self.blk_idx[t.perm.long()] if a.nnzb else t.perm
-            self._structure["t"] = (t.matrix.row_ptr, t.matrix.col_idx, t.perm, perm_stored, t.matrix.max_row_blocks)
-        row_ptr, col_idx, perm, _, longest = self._structure["t"]
-        b = self.block
-        blocks_t = self.blocks.new_empty((a.nnzb, b, b))
-        t = TransposedBsr(matrix=BlockSparseMatrix(row_ptr=row_ptr, col_idx=col_idx, blocks=blocks_t,
-                                                   shape=(a.shape[1], a.shape[0]), block_size=(b, b),
-                                                   max_row_blocks=longest), perm=perm)
-        return transpose_values(a, t)
+    def _backward_structure(self) -> "_Structure":
+        """What the backward products need beside the values; made once per pattern."""
+        made = self._structure.get("backward")
+        if made is None:
+            made = self._structure["backward"] = _Structure(self)
+        return made
+
+
+class _Structure:
+    """The stacked matrix transposed (structure only), descriptors and workspace sizes of the backward products."""
+
+    def __init__(self, w: GatedWeights) -> None:
+        a = w.stacked()
+        t = bsr_transpose(a)
+        self.kept = (t.matrix.row_ptr, t.matrix.col_idx, t.perm, w.row_ptr, w.col_idx, w.blk_idx, w.stored_col)
+        # positions of the transposed structure name stored blocks, so that the weight gradient lands in the blocks' own order
+        self.perm_stored = w.blk_idx[t.perm.long()] if a.nnzb else t.perm
+        self.desc = _bsr_desc(a)
+        self.desc_t = _bsr_desc(t.matrix)
+        self.desc_w = _bsr_desc(BlockSparseMatrix(row_ptr=w.row_ptr, col_idx=w.stored_col, blocks=w.blocks,
+                                                  shape=a.shape, block_size=a.block_size))
+        self.rows_t, self.longest_t = t.matrix.nbr, t.matrix.max_row_blocks
+        nbytes = ctypes.c_size_t(0)
+        _lib.check(_lib.lib().kairo_bsr_sddmm_workspace_size(ctypes.byref(self.desc_w), ctypes.byref(nbytes)), "sddmm")
+        self.sddmm_bytes = max(nbytes.value, 256)
+
+    def config(self, nnzb: int, tokens: int) -> _lib.KairoSpmmConfig:
+        """Schedule of dP times the stacked weight.  Whole block-rows per CTA (bands of one) beat the row-split
+        schedule, the library's own choice for few block-rows, from about 128 tokens on: it cuts nearly every
+        row into partial tiles (6000 tokens, 512 -> 512: 25 us against 1469; 1000 tokens, 8192 -> 8192 at 20 %:
+        107 against 126; 128 tokens, 16384 -> 4096: 62 against 32).  Tiles of 128 tokens where those of 256 do
+        not fill the 148 SMs (777 tokens, 520 -> 1000: 19.5 us against 23.6).  A few rows far longer than the
+        others would leave most SMs idle: split there."""
+        if tokens <= 128 or self.longest_t > 8 * nnzb / max(self.rows_t, 1) + 8:
+            return _AUTO
+        return _BANDS_128 if self.rows_t * -(-tokens // 256) < 148 else _BANDS_256
+
+
+_AUTO = KernelConfig().to_c()
+_BANDS_128 = KernelConfig(schedule="bands", band_rows=1, n_tile=128).to_c()
+_BANDS_256 = KernelConfig(schedule="bands", band_rows=1, n_tile=256).to_c()
+
+
+def _with_blocks(desc: _lib.KairoBsr, blocks: Tensor) -> _lib.KairoBsr:
+    d = _lib.KairoBsr.from_buffer_copy(desc)
+    d.blocks = blocks.data_ptr()
+    return d
 
 
 def _in_order(a: BlockSparseMatrix) -> Tensor:
@@ -229,7 +256,7 @@ def sparse_gated_linear(X: Tensor, weights: GatedWeights, *, activation: str = "
     index = _lib.device_index(op, X, weights.blocks)
     x, act = _input(op, X, weights, activation)
     n, m = x.shape[0], weights.shape[0]
-    if n > _FEW_TOKENS:
+    if n > _ANY_TOKENS:
         x = _aligned(x)
     if out is None:
         out = x.new_empty((n, m))
@@ -279,16 +306,42 @@ def sparse_gated_linear_backward(dH: Tensor, X: Tensor, weights: GatedWeights, *
                 max(_ld(x), k), n, act, dh.data_ptr(), max(_ld(dh), m), dp.data_ptr(), dp.shape[1], err.data_ptr())
     if check:
         _lib.raise_on_device_error(err)
-    wt = weights._transposed()
-    dX = sparse_linear(dp, wt.matrix, out_dtype=x.dtype, check=check) if need_dx else None
-    d_blocks = None
+    nnzb, b = weights.blocks.shape[0], weights.block
+    dX = d_blocks = None
+    if nnzb == 0 or n == 0:
+        dX = x.new_zeros((n, k)) if need_dx else None
+        return dX, weights.blocks.new_zeros(weights.blocks.shape, dtype=dwt) if need_dw else None
+    lib = _lib.lib()
+    st = weights._backward_structure()
+    nbytes = ctypes.c_size_t(0)
+    if need_dx:
+        # the transposed weight's values are of this call alone: the structure serves calls on several streams
+        blocks_t = weights.blocks.new_empty((nnzb, b, b))
+        scratch = x.new_empty(256, dtype=torch.uint8)
+        _lib.launch(op, lib.kairo_bsr_transpose_values, index, ctypes.byref(_with_blocks(st.desc, weights.blocks)),
+                    st.kept[2].data_ptr(), blocks_t.data_ptr(), scratch.data_ptr(), 256)
+        desc_t, cfg = _with_blocks(st.desc_t, blocks_t), st.config(nnzb, n)
+        dX = x.new_empty((n, k))
+        with torch.cuda.device(index):
+            _lib.check(lib.kairo_bsr_spmm_workspace_size(ctypes.byref(desc_t), _lib.LAYOUT_LINEAR, n, ctypes.byref(cfg),
+                                                         ctypes.byref(nbytes)), op)
+            ws = _lib.workspace(nbytes.value, x.device)
+        if check:
+            _lib.take_pending_error(ws, op)
+        _lib.launch(op, lib.kairo_bsr_spmm, index, ctypes.byref(desc_t), dp.data_ptr(), dp.shape[1],
+                    _lib.LAYOUT_LINEAR, n, dX.data_ptr(), k, _lib.kairo_dtype(x.dtype), ctypes.byref(cfg),
+                    ws.data_ptr(), ws.numel())
+        if check:
+            _lib.raise_on_device_error(ws)
     if need_dw:
-        # the weight gradient lands in the blocks' own order: positions of the transposed structure name stored blocks
-        perm_stored = weights._structure["t"][3]
-        stored = BlockSparseMatrix(row_ptr=weights.row_ptr, col_idx=weights.stored_col, blocks=weights.blocks,
-                                   shape=(2 * nbr * weights.block, k), block_size=(weights.block, weights.block))
-        d_blocks = sparse_linear_weight_grad(dp, x, stored, TransposedBsr(matrix=wt.matrix, perm=perm_stored),
-                                             out_dtype=dwt, check=check)
+        d_blocks = weights.blocks.new_empty((nnzb, b, b), dtype=dwt)
+        ws = x.new_empty(st.sddmm_bytes, dtype=torch.uint8)
+        _lib.launch(op, lib.kairo_bsr_sddmm, index, ctypes.byref(_with_blocks(st.desc_w, weights.blocks)),
+                    st.kept[0].data_ptr(), st.kept[1].data_ptr(), st.perm_stored.data_ptr(), dp.data_ptr(), dp.shape[1],
+                    x.data_ptr(), max(_ld(x), k), n, d_blocks.data_ptr(), _lib.kairo_dtype(dwt), ws.data_ptr(),
+                    ws.numel())
+        if check:
+            _lib.raise_on_device_error(ws)
     return dX, d_blocks
 
 

@@ -55,11 +55,10 @@ def _problem(op: str, X: Tensor, weight: Tensor, targets: Tensor, reduction: str
             _lib.kairo_dtype(X.dtype), _REDUCTIONS[reduction])
 
 
-def _workspace(op: str, x: Tensor, w: Tensor, tokens: int, v: int, d: int, backward: bool) -> Tensor:
+def _bytes(op: str, fn, *args) -> int:
     nbytes = ctypes.c_size_t(0)
-    _lib.check(_lib.lib().kairo_vocab_loss_workspace_size(x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), tokens, v, d,
-                                                          1 if backward else 0, ctypes.byref(nbytes)), op)
-    return x.new_empty(nbytes.value, dtype=torch.uint8)
+    _lib.check(fn(*args, ctypes.byref(nbytes)), op)
+    return nbytes.value
 
 
 def linear_cross_entropy(X: Tensor, weight: Tensor, targets: Tensor, *, scale: float = 1.0, reduction: str = "mean",
@@ -80,7 +79,8 @@ def linear_cross_entropy(X: Tensor, weight: Tensor, targets: Tensor, *, scale: f
     shape = targets.shape
     lse = x.new_empty(shape, dtype=torch.float32)
     loss = x.new_empty(shape if reduction == "none" else (), dtype=torch.float32)
-    ws = _workspace(op, x, w, tokens, v, d, False)
+    ws = x.new_empty(_bytes(op, _lib.lib().kairo_vocab_loss_workspace_size, x.data_ptr(), _ld(x), w.data_ptr(), _ld(w),
+                            tokens, v, d), dtype=torch.uint8)
     err = _lib.error_word(index)
     if check:
         _lib.take_pending_error(err, op)
@@ -130,14 +130,15 @@ def linear_cross_entropy_backward(grad: Tensor, X: Tensor, weight: Tensor, targe
     elif dw is not None:
         raise ValueError(f"{op}: dw is given and need_dw is False")
     if need_dx or need_dw:
-        ws = _workspace(op, x, w, tokens, v, d, True)
+        results = (_lib.ptr(dX), d, _lib.ptr(dw), d if dw is None else _ld(dw))
+        ws = x.new_empty(_bytes(op, _lib.lib().kairo_vocab_loss_backward_workspace_size, w.data_ptr(), _ld(w), tokens, v,
+                                d, *results), dtype=torch.uint8)
         err = _lib.error_word(index)
         if check:
             _lib.take_pending_error(err, op)
         _lib.launch(op, _lib.lib().kairo_vocab_loss_backward, index, grad.data_ptr(), x.data_ptr(), _ld(x),
                     w.data_ptr(), _ld(w), tokens, v, d, dt, ids.data_ptr(), ids.element_size(), float(scale), red,
-                    lse.data_ptr(), _lib.ptr(dX), d, _lib.ptr(dw), d if dw is None else _ld(dw), ws.data_ptr(),
-                    ws.numel(), err.data_ptr())
+                    lse.data_ptr(), *results, ws.data_ptr(), ws.numel(), err.data_ptr())
         if check:
             _lib.raise_on_device_error(err)
     return dX if dX is None else dX.view(X.shape), dw
