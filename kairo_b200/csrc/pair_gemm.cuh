@@ -61,6 +61,8 @@ struct PairShape {
   int tiles_m, tiles_n, ksteps, group_m;
   int seg;     // stages of one segment
   int splits;  // parts of k, each a tile of its own
+  int copies;  // of A's rows, copy_rows after one another: cluster c reads copy c % copies (one row of tiles only)
+  int copy_rows;
 };
 
 struct PairTile {
@@ -156,12 +158,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const uint32_t mine = lane < NA + NB ? 1u : 0u;
     const bool mn = is_a ? A_MN : B_MN;
     const uint32_t dst_off = (is_a ? 0u : kPairHalf) + static_cast<uint32_t>(mine ? box : 0) * (kPairHalf / kPairBoxes);
+    const int shift = is_a ? first % shape.copies * shape.copy_rows : 0;
     int sidx = 0;
     uint32_t sph = 0;
     bool alive = true;
     for (int t = first; t < ntiles && alive; t += step) {
       const PairTile pt = pair_tile(shape, t);
-      const int r0 = (is_a ? pt.mt : pt.nt) * 256 + static_cast<int>(rank) * 128 + box * kPairBoxRows;
+      const int r0 = (is_a ? pt.mt : pt.nt) * 256 + static_cast<int>(rank) * 128 + box * kPairBoxRows + shift;
       for (int k = pt.k0; k < pt.k1; ++k) {
         int ok = ptx::wait_parity(&empty[sidx], sph ^ 1u, abort_flag, err, kTagEmpty, kWaitCycles);
         ok = __shfl_sync(0xffffffffu, ok, 0);

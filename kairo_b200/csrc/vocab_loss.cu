@@ -428,8 +428,8 @@ __global__ void __launch_bounds__(256) k_join(const float* __restrict__ acc, int
   }
 }
 
-// Rows of 16-bit values with 16-byte alignment: dst (rows x ldd, ldd a multiple of 8) = src, zeros
-// behind column `cols` and, where `ids` is given, in the rows of tokens that do not count.
+// Rows of 16-bit values with 16-byte alignment: dst (rows x ldd, ldd a multiple of 8) = src (its rows over
+// and over where it has fewer), zeros behind column `cols` and, where `ids` is given, in the rows of tokens that do not count.
 // CTA 0 writes the tokens' factors and the one they share (`factor`) first.
 struct PrepArgs {
   const float* grad;  // by the loss: one number, or every token's (kNone)
@@ -480,8 +480,8 @@ __device__ __forceinline__ int lanes_for(int64_t pieces) {
   return l;
 }
 
-__global__ void __launch_bounds__(256) k_rows(const uint16_t* __restrict__ src, int64_t lds, int64_t rows, int64_t cols,
-                                              uint16_t* __restrict__ dst, int64_t ldd, Targets ids, int vocab,
+__global__ void __launch_bounds__(256) k_rows(const uint16_t* __restrict__ src, int64_t lds, int64_t src_rows,
+                                              int64_t cols, int64_t rows, uint16_t* __restrict__ dst, int64_t ldd, Targets ids, int vocab,
                                               PrepArgs prep) {
   int cta = blockIdx.x, ctas = gridDim.x;
   if (prep.f) {
@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(256) k_rows(const uint16_t* __restrict__ src, 
   }
   const int64_t pieces = ldd / 8;
   const int lanes = lanes_for(pieces), per = 256 / lanes;
-  const uint16_t* end = src + (rows - 1) * lds + cols;  // nothing is read outside [src, end)
+  const uint16_t* end = src + (src_rows - 1) * lds + cols;  // nothing is read outside [src, end)
   for (int64_t r = static_cast<int64_t>(cta) * per + threadIdx.x / lanes; r < rows; r += static_cast<int64_t>(ctas) * per) {
     bool live = true;
     if (ids.p) {
@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(256) k_rows(const uint16_t* __restrict__ src, 
     for (int64_t q0 = threadIdx.x % lanes; q0 < pieces; q0 += 4 * lanes) {
       uint4 lo[4], hi[4];
       bool whole[4];
-      const uint16_t* row = src + r * lds;
+      const uint16_t* row = src + (r < src_rows ? r : r % src_rows) * lds;
       // past a 16-byte boundary (the same for all vectors of a row)
       const int e = static_cast<int>((reinterpret_cast<uintptr_t>(row) >> 1) & 7u);
 #pragma unroll
@@ -597,7 +597,16 @@ struct LossWs {
   size_t ticket, target, each, part, x, w, total;
 };
 
-// Everything a call may need, whether or not its rows are aligned: the copies come last.
+// Rows of a few tokens are read by every SM at the same time, all from the same few lines of L2: copies of them
+// for different clusters bring 1 to 15 tokens of 131072 x 4096 from 237..261 us to what 16 take, 200.
+constexpr int64_t kCopyRows = 64;
+int64_t copies_of(int64_t tokens) { return tokens < 16 ? kCopyRows / tokens : 1; }
+
+// Rows of copies begin on 128-byte lines: a box of 64 k of a row then touches one line, not two (4000 tokens, 50021 x
+// 1000: 337 us, 302 with such a pitch; a copy of the table for that alone would cost what it saves).
+int64_t copy_ld(int64_t dim) { return static_cast<int64_t>(align_up(static_cast<size_t>(dim), 64)); }
+
+// Everything a call may need: the copies come last.
 LossWs loss_ws(const Problem& p) {
   LossWs o{};
   size_t at = kWorkspaceHeaderBytes;
@@ -611,8 +620,9 @@ LossWs loss_ws(const Problem& p) {
   o.each = take(4 * static_cast<size_t>(p.tokens));
   const int64_t slots = 2 * tiles(p.vocab);
   o.part = take(8 * static_cast<size_t>(p.tokens) * static_cast<size_t>(slots));
-  const size_t ld = align_up(static_cast<size_t>(p.dim), 8);
-  if (!rows_aligned(p.x, p.ldx, p.tokens)) o.x = take(2 * ld * static_cast<size_t>(p.tokens));
+  const size_t ld = static_cast<size_t>(copy_ld(p.dim));
+  const int64_t copies = copies_of(std::max<int64_t>(1, p.tokens));
+  if (copies > 1 || !rows_aligned(p.x, p.ldx, p.tokens)) o.x = take(2 * ld * static_cast<size_t>(p.tokens * copies));
   if (!rows_aligned(p.w, p.ldw, p.vocab)) o.w = take(2 * ld * static_cast<size_t>(p.vocab));
   o.total = at;
   return o;
@@ -660,7 +670,7 @@ GradWs grad_ws(const Problem& p, const Results& r) {
     at = align_up(at + bytes, 256);
     return here;
   };
-  const size_t ld = align_up(static_cast<size_t>(p.dim), 8);
+  const size_t ld = static_cast<size_t>(copy_ld(p.dim));
   o.cols = piece_cols(p.tokens, p.vocab);
   o.factor = 128;
   o.f = take(4 * static_cast<size_t>(p.tokens));
@@ -691,19 +701,24 @@ kairo_status check_problem(const Problem& p) {
   return KAIRO_STATUS_SUCCESS;
 }
 
+kairo_status copy_rows(const void* src, int64_t ld, int64_t rows, int64_t cols, int64_t copies, uint8_t* dst,
+                       Targets ids, int vocab, const PrepArgs& prep, cudaStream_t s) {
+  const int64_t ldd = copy_ld(cols);
+  const int64_t work = ceil_div64(rows * copies * (ldd / 8), 1024);
+  const int grid = static_cast<int>(std::min<int64_t>(work, device_sm_count(current_device()) * 16)) + (prep.f ? 1 : 0);
+  k_rows<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(src), ld, rows, cols, rows * copies,
+                              reinterpret_cast<uint16_t*>(dst), ldd, ids, vocab, prep);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "launch of the row copy");
+}
+
 // `src` with 16-byte aligned rows: itself, or a copy at `dst`.
 kairo_status aligned_rows(const void** src, int64_t* ld, int64_t rows, int64_t cols, uint8_t* dst, cudaStream_t s) {
   if (rows_aligned(*src, *ld, rows)) return KAIRO_STATUS_SUCCESS;
-  const int64_t ldd = static_cast<int64_t>(align_up(static_cast<size_t>(cols), 8));
-  const int64_t work = ceil_div64(rows * (ldd / 8), 256);
-  const int grid = static_cast<int>(std::min<int64_t>(work, device_sm_count(current_device()) * 16));
-  k_rows<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(*src), *ld, rows, cols, reinterpret_cast<uint16_t*>(dst), ldd,
-                              Targets{nullptr, 8}, 0, PrepArgs{});
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, "launch of the row copy");
+  const kairo_status st = copy_rows(*src, *ld, rows, cols, 1, dst, Targets{nullptr, 8}, 0, PrepArgs{}, s);
   *src = dst;
-  *ld = ldd;
-  return KAIRO_STATUS_SUCCESS;
+  *ld = copy_ld(cols);
+  return st;
 }
 
 // Rows of tiles visited together: their part of the row operand takes about a quarter of the L2.
@@ -719,6 +734,8 @@ PairShape shape_of(int64_t rows, int64_t cols, int64_t k, int seg, int splits = 
   PairShape s;
   s.seg = seg;
   s.splits = splits;
+  s.copies = 1;
+  s.copy_rows = 0;
   s.tiles_m = static_cast<int>(tiles(rows));
   s.tiles_n = static_cast<int>(tiles(cols));
   s.ksteps = static_cast<int>(ceil_div64(k, kPairK));
@@ -744,15 +761,25 @@ kairo_status join(const float* acc, int64_t ldacc, int splits, int64_t rows, int
 template <typename T, int FMT>
 kairo_status run_loss(Problem p, float* loss, float* lse, uint8_t* ws, unsigned* err, cudaStream_t s) {
   const LossWs o = loss_ws(p);
-  kairo_status st = aligned_rows(&p.x, &p.ldx, p.tokens, p.dim, ws + o.x, s);
+  const int64_t copies = copies_of(p.tokens);
+  kairo_status st;
+  if (copies > 1) {
+    st = copy_rows(p.x, p.ldx, p.tokens, p.dim, copies, ws + o.x, Targets{nullptr, 8}, 0, PrepArgs{}, s);
+    p.x = ws + o.x;
+    p.ldx = copy_ld(p.dim);
+  } else {
+    st = aligned_rows(&p.x, &p.ldx, p.tokens, p.dim, ws + o.x, s);
+  }
   if (st == KAIRO_STATUS_SUCCESS) st = aligned_rows(&p.w, &p.ldw, p.vocab, p.dim, ws + o.w, s);
   if (st) return st;
   unsigned* ticket = reinterpret_cast<unsigned*>(ws + o.ticket);
   CUtensorMap ma, mb;
-  st = pair_operand_map(&ma, p.x, p.dt, false, p.tokens, p.dim, p.ldx, "hidden states");
+  st = pair_operand_map(&ma, p.x, p.dt, false, p.tokens * copies, p.dim, p.ldx, "hidden states");
   if (st == KAIRO_STATUS_SUCCESS) st = pair_operand_map(&mb, p.w, p.dt, false, p.vocab, p.dim, p.ldw, "vocabulary table");
   if (st) return st;
-  const PairShape sh = shape_of(p.tokens, p.vocab, p.dim, kSegLogits);
+  PairShape sh = shape_of(p.tokens, p.vocab, p.dim, kSegLogits);
+  sh.copies = static_cast<int>(copies);
+  sh.copy_rows = static_cast<int>(p.tokens);
   StatsEpi::Args a{reinterpret_cast<float2*>(ws + o.part), reinterpret_cast<float*>(ws + o.target), p.ids,
                    static_cast<int>(p.tokens), static_cast<int>(p.vocab), p.scale, sh.tiles_m == 1, ticket};
   st = launch_pair_gemm<FMT, false, false, StatsEpi>(ma, mb, sh, err, a, s);
@@ -770,7 +797,7 @@ kairo_status run_grad(Problem p, const float* grad, const float* lse, const Resu
                       cudaStream_t s) {
   const GradWs o = grad_ws(p, res);
   T *dx = static_cast<T*>(res.dx), *dw = static_cast<T*>(res.dw);
-  const int64_t ld = static_cast<int64_t>(align_up(static_cast<size_t>(p.dim), 8));
+  const int64_t ld = copy_ld(p.dim);
   kairo_status st = aligned_rows(&p.w, &p.ldw, p.vocab, p.dim, ws + o.w, s);
   if (st) return st;
   float* f = reinterpret_cast<float*>(ws + o.f);
@@ -779,12 +806,8 @@ kairo_status run_grad(Problem p, const float* grad, const float* lse, const Resu
   {
     PrepArgs pa{grad, p.ids, static_cast<int>(p.tokens), static_cast<int>(p.vocab), p.reduction, p.scale,
                 FMT == 0 ? kHalfLift : 1.f, f, factor};
-    const int64_t work = ceil_div64(p.tokens * (ld / 8), 256);
-    const int grid = 1 + static_cast<int>(std::min<int64_t>(work, device_sm_count(current_device()) * 8));
-    k_rows<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(p.x), p.ldx, p.tokens, p.dim, static_cast<uint16_t*>(x), ld,
-                                p.ids, static_cast<int>(p.vocab), pa);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return cuda_fail(e, "launch of the tokens' factors");
+    st = copy_rows(p.x, p.ldx, p.tokens, p.dim, 1, ws + o.x, p.ids, static_cast<int>(p.vocab), pa, s);
+    if (st) return st;
   }
   T* g = reinterpret_cast<T*>(ws + o.g);
   CUtensorMap mx, mxt, mg, mgt;

@@ -25,6 +25,7 @@ The reference has no counterpart.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 from torch import Tensor
@@ -55,9 +56,27 @@ def _problem(op: str, X: Tensor, weight: Tensor, targets: Tensor, reduction: str
             _lib.kairo_dtype(X.dtype), _REDUCTIONS[reduction])
 
 
-def _bytes(op: str, fn, *args) -> int:
-    nbytes = ctypes.c_size_t(0)
-    _lib.check(fn(*args, ctypes.byref(nbytes)), op)
+def _aligned(t: Tensor | None) -> tuple[int, int]:
+    """An address and a row pitch that are as 16-byte aligned as ``t``'s rows: all that workspace sizes depend on."""
+    if t is None:
+        return 0, 0
+    return 16 + t.data_ptr() % 16, _ld(t) % 8
+
+
+@functools.lru_cache(maxsize=4096)
+def _forward_bytes(x: tuple[int, int], w: tuple[int, int], tokens: int, v: int, d: int) -> int:
+    nbytes, up = ctypes.c_size_t(0), -(-d // 8) * 8
+    _lib.check(_lib.lib().kairo_vocab_loss_workspace_size(x[0], up + x[1], w[0], up + w[1], tokens, v, d,
+                                                          ctypes.byref(nbytes)), "linear_cross_entropy")
+    return nbytes.value
+
+
+@functools.lru_cache(maxsize=4096)
+def _backward_bytes(w: tuple[int, int], dx: tuple[int, int], dw: tuple[int, int], tokens: int, v: int, d: int) -> int:
+    nbytes, up = ctypes.c_size_t(0), -(-d // 8) * 8
+    _lib.check(_lib.lib().kairo_vocab_loss_backward_workspace_size(
+        w[0], up + w[1], tokens, v, d, dx[0] or None, up + dx[1], dw[0] or None, up + dw[1], ctypes.byref(nbytes)),
+        "linear_cross_entropy_backward")
     return nbytes.value
 
 
@@ -79,8 +98,7 @@ def linear_cross_entropy(X: Tensor, weight: Tensor, targets: Tensor, *, scale: f
     shape = targets.shape
     lse = x.new_empty(shape, dtype=torch.float32)
     loss = x.new_empty(shape if reduction == "none" else (), dtype=torch.float32)
-    ws = x.new_empty(_bytes(op, _lib.lib().kairo_vocab_loss_workspace_size, x.data_ptr(), _ld(x), w.data_ptr(), _ld(w),
-                            tokens, v, d), dtype=torch.uint8)
+    ws = x.new_empty(_forward_bytes(_aligned(x), _aligned(w), tokens, v, d), dtype=torch.uint8)
     err = _lib.error_word(index)
     if check:
         _lib.take_pending_error(err, op)
@@ -131,8 +149,7 @@ def linear_cross_entropy_backward(grad: Tensor, X: Tensor, weight: Tensor, targe
         raise ValueError(f"{op}: dw is given and need_dw is False")
     if need_dx or need_dw:
         results = (_lib.ptr(dX), d, _lib.ptr(dw), d if dw is None else _ld(dw))
-        ws = x.new_empty(_bytes(op, _lib.lib().kairo_vocab_loss_backward_workspace_size, w.data_ptr(), _ld(w), tokens, v,
-                                d, *results), dtype=torch.uint8)
+        ws = x.new_empty(_backward_bytes(_aligned(w), _aligned(dX), _aligned(dw), tokens, v, d), dtype=torch.uint8)
         err = _lib.error_word(index)
         if check:
             _lib.take_pending_error(err, op)
