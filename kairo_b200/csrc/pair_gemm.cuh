@@ -43,15 +43,16 @@ constexpr int kPairEpiWarps = 8;
 constexpr int kPairTileM = 256;      // rows of a cluster's tile (128 a CTA)
 constexpr int kPairTileN = 256;
 constexpr int kPairK = 64;           // k of one stage
-constexpr int kPairStages = 6;
 constexpr int kPairHalf = 128 * kPairK * 2;  // bytes of one operand's part of a stage in one CTA
 constexpr int kPairBoxes = 2;
 constexpr int kPairBoxRows = 128 / kPairBoxes;
-constexpr int kPairStageBytes = 2 * kPairHalf;
+// Bytes of a stage and stages, for A_ROWS rows of A in each CTA (128, or 64: see below); 192 KB in all.
+constexpr int pair_stage_bytes(int a_rows) { return a_rows * kPairK * 2 + kPairHalf; }
+constexpr int pair_stages(int a_rows) { return 192 * 1024 / pair_stage_bytes(a_rows); }
 constexpr int kPairEpiCols = kPairTileN / (kPairEpiWarps / 4);
 constexpr int kPairOutBytes = 4096;  // of each epilogue warp, to turn rows a lane into rows a warp
 constexpr size_t kPairSmem =
-    static_cast<size_t>(kPairStages) * kPairStageBytes + kPairEpiWarps * kPairOutBytes + 2048;
+    192 * 1024 + kPairEpiWarps * kPairOutBytes + 2048;
 constexpr int kPairClusters = 74;    // pairs of a B200's 148 SMs, for plans that must not depend on the current device
 static_assert(kPairSmem <= kMaxSmem, "shared memory");
 
@@ -91,20 +92,27 @@ __device__ __forceinline__ PairTile pair_tile(const PairShape& s, int t) {
 //   __device__ void tile(const PairTile&, float (&v)[kPairEpiCols])   its columns of one tile
 //   __device__ void done()                                            after the CTA's last tile
 // and is made once per thread and launch; `out` is the warp's kPairOutBytes.
-template <int IN_FMT, bool A_MN, bool B_MN, class Epi>
+//
+// A_ROWS = 64: A has at most 64 rows.  Only the leader loads them, 64 of its 128; what the MMAs
+// read in the place of the others (the stage's B, or what an earlier stage left) ends in rows of the
+// accumulator that no epilogue looks at.  B then has 128 KB of copies under way instead of 96.
+template <int IN_FMT, bool A_MN, bool B_MN, class Epi, int A_ROWS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     k_pair_gemm(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                 const PairShape shape, unsigned* err, const typename Epi::Args eargs) {
-  constexpr int ST = kPairStages;
+  constexpr int ST = pair_stages(A_ROWS);
+  constexpr int STAGE = pair_stage_bytes(A_ROWS), A_BYTES = STAGE - kPairHalf;
+  constexpr bool FEW = A_ROWS < 128;
+  static_assert(A_ROWS == 128 || (A_ROWS == 64 && !A_MN), "rows of A");
   constexpr uint32_t IDESC = ptx::make_idesc_f16(IN_FMT, A_MN ? 1u : 0u, B_MN ? 1u : 0u, kPairTileM, kPairTileN);
   constexpr uint32_t TMEM_COLS = 2 * kPairTileN;
   // A CTA's half of an operand comes in kPairBoxes boxes, one lane each: 64 k x 64 rows, or 64
   // columns x 64 k.
-  constexpr int NA = kPairBoxes, NB = kPairBoxes;
+  constexpr int NA = kPairBoxes * A_ROWS / 128, NB = kPairBoxes;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* out = smem + ST * kPairStageBytes;
+  uint8_t* out = smem + ST * STAGE;
   uint64_t* full = reinterpret_cast<uint64_t*>(out + kPairEpiWarps * kPairOutBytes);  // used in the leader
   uint64_t* empty = full + ST;
   uint64_t* tfull = empty + ST;
@@ -155,9 +163,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const bool is_a = lane < NA;
     const int box = is_a ? lane : lane - NA;
     const void* map = is_a ? static_cast<const void*>(&tmap_a) : static_cast<const void*>(&tmap_b);
-    const uint32_t mine = lane < NA + NB ? 1u : 0u;
+    const uint32_t mine = lane < NA + NB && !(FEW && is_a && rank != 0) ? 1u : 0u;
+    constexpr uint32_t BYTES = FEW ? A_BYTES + 2 * kPairHalf : 2 * STAGE;  // of a stage, both CTAs
     const bool mn = is_a ? A_MN : B_MN;
-    const uint32_t dst_off = (is_a ? 0u : kPairHalf) + static_cast<uint32_t>(mine ? box : 0) * (kPairHalf / kPairBoxes);
+    const uint32_t dst_off = (is_a ? 0u : A_BYTES) + static_cast<uint32_t>(mine ? box : 0) * (kPairHalf / kPairBoxes);
     const int shift = is_a ? first % shape.copies * shape.copy_rows : 0;
     int sidx = 0;
     uint32_t sph = 0;
@@ -175,9 +184,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         const uint32_t bar = ptx::peer_smem_u32(&full[sidx], 0);
         if (rank == 0) {
           if (lane == 0) issued[sidx] = static_cast<int>(sph) + 1;
-          ptx::mbar_expect_tx_if(lane == 0 ? 1u : 0u, &full[sidx], 2 * kPairStageBytes);
+          ptx::mbar_expect_tx_if(lane == 0 ? 1u : 0u, &full[sidx], BYTES);
         }
-        ptx::tma_load_2d_pair_if(mine, smem + sidx * kPairStageBytes + dst_off, map, mn ? r0 : k * kPairK,
+        ptx::tma_load_2d_pair_if(mine, smem + sidx * STAGE + dst_off, map, mn ? r0 : k * kPairK,
                                  mn ? k * kPairK : r0, bar, pol);
         __syncwarp();
         if (rank == 0) ptx::mbar_arrive_if(lane == 0 ? 1u : 0u, &full[sidx]);
@@ -193,8 +202,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const uint32_t sbase = ptx::smem_u32(smem);
     const uint64_t adesc = A_MN ? ptx::make_smem_desc(sbase, kPairHalf / 2, 1024, 2u)
                                 : ptx::make_smem_desc(sbase, 16, 1024, 2u);
-    const uint64_t bdesc = B_MN ? ptx::make_smem_desc(sbase + kPairHalf, kPairHalf / 2, 1024, 2u)
-                                : ptx::make_smem_desc(sbase + kPairHalf, 16, 1024, 2u);
+    const uint64_t bdesc = B_MN ? ptx::make_smem_desc(sbase + A_BYTES, kPairHalf / 2, 1024, 2u)
+                                : ptx::make_smem_desc(sbase + A_BYTES, 16, 1024, 2u);
     const uint32_t a_lo = static_cast<uint32_t>(adesc), a_hi = static_cast<uint32_t>(adesc >> 32);
     const uint32_t b_lo = static_cast<uint32_t>(bdesc), b_hi = static_cast<uint32_t>(bdesc >> 32);
     // 16 k further: 32 bytes along a 128-byte row, or 16 rows of 128 bytes
@@ -221,7 +230,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             alive = false;
             break;
           }
-          const uint32_t s16 = static_cast<uint32_t>(sidx * kPairStageBytes) >> 4;
+          const uint32_t s16 = static_cast<uint32_t>(sidx * STAGE) >> 4;
 #pragma unroll
           for (int kk = 0; kk < kPairK / 16; ++kk)
             ptx::mma_f16_ss_pair_if(leader, d, a_lo + s16 + kk * AK, a_hi, b_lo + s16 + kk * BK, b_hi, IDESC,
@@ -327,10 +336,10 @@ inline int pair_clusters(int64_t tiles) {
   return static_cast<int>(std::min<int64_t>(tiles, std::max(1, device_sm_count(current_device()) / 2)));
 }
 
-template <int IN_FMT, bool A_MN, bool B_MN, class Epi>
+template <int IN_FMT, bool A_MN, bool B_MN, class Epi, int A_ROWS = 128>
 kairo_status launch_pair_gemm(const CUtensorMap& a, const CUtensorMap& b, const PairShape& shape, unsigned* err,
                               const typename Epi::Args& args, cudaStream_t s) {
-  auto* fn = &k_pair_gemm<IN_FMT, A_MN, B_MN, Epi>;
+  auto* fn = &k_pair_gemm<IN_FMT, A_MN, B_MN, Epi, A_ROWS>;
   static std::atomic<uint64_t> ready{0};
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(fn), kPairSmem, &ready);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic smem)");

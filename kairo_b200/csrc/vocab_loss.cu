@@ -782,7 +782,9 @@ kairo_status run_loss(Problem p, float* loss, float* lse, uint8_t* ws, unsigned*
   sh.copy_rows = static_cast<int>(p.tokens);
   StatsEpi::Args a{reinterpret_cast<float2*>(ws + o.part), reinterpret_cast<float*>(ws + o.target), p.ids,
                    static_cast<int>(p.tokens), static_cast<int>(p.vocab), p.scale, sh.tiles_m == 1, ticket};
-  st = launch_pair_gemm<FMT, false, false, StatsEpi>(ma, mb, sh, err, a, s);
+  // up to 64 tokens the table alone bounds it: more of it under way
+  st = p.tokens <= 64 ? launch_pair_gemm<FMT, false, false, StatsEpi, 64>(ma, mb, sh, err, a, s)
+                      : launch_pair_gemm<FMT, false, false, StatsEpi>(ma, mb, sh, err, a, s);
   if (st) return st;
   const int slots = 2 * (a.by_cluster ? pair_clusters(sh.tiles_n) : sh.tiles_n);
   k_lse<<<static_cast<int>(ceil_div64(p.tokens, 32)), 1024, 0, s>>>(
