@@ -117,6 +117,9 @@ class GatedWeights:
         """What the backward products need beside the values; made once per pattern."""
         made = self._structure.get("backward")
         if made is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("sparse_gated_linear_backward: the first backward pass of a pattern makes its "
+                                   "transposed structure and synchronises; run one before capturing")
             made = self._structure["backward"] = _Structure(self)
         return made
 
@@ -151,6 +154,7 @@ class _Structure:
         return _BANDS_128 if self.rows_t * -(-tokens // 256) < 148 else _BANDS_256
 
 
+_ZEROED = 256 + 2 * 16384 * 4  # header and arrival counters of an SpMM workspace, zero before its first launch
 _AUTO = KernelConfig().to_c()
 _BANDS_128 = KernelConfig(schedule="bands", band_rows=1, n_tile=128).to_c()
 _BANDS_256 = KernelConfig(schedule="bands", band_rows=1, n_tile=256).to_c()
@@ -325,7 +329,12 @@ def sparse_gated_linear_backward(dH: Tensor, X: Tensor, weights: GatedWeights, *
         with torch.cuda.device(index):
             _lib.check(lib.kairo_bsr_spmm_workspace_size(ctypes.byref(desc_t), _lib.LAYOUT_LINEAR, n, ctypes.byref(cfg),
                                                          ctypes.byref(nbytes)), op)
-            ws = _lib.workspace(nbytes.value, x.device)
+            if torch.cuda.is_current_stream_capturing():
+                # a graph's own: two captured graphs may replay at the same time
+                ws = x.new_empty(nbytes.value, dtype=torch.uint8)
+                ws[:_ZEROED].zero_()
+            else:
+                ws = _lib.workspace(nbytes.value, x.device)
         if check:
             _lib.take_pending_error(ws, op)
         _lib.launch(op, lib.kairo_bsr_spmm, index, ctypes.byref(desc_t), dp.data_ptr(), dp.shape[1],
@@ -379,17 +388,18 @@ class SparseGatedLinear(torch.nn.Module):
         self.blocks = torch.nn.Parameter(w.blocks.detach())
         for name in ("ent_ptr", "entries", "row_ptr", "col_idx", "blk_idx", "stored_col"):
             self.register_buffer(name, getattr(w, name))
-        self._made: tuple | None = None
+        self._made: tuple = ((), (), {})
 
     def weights(self, blocks: Tensor | None = None) -> GatedWeights:
         b = (self.blocks if blocks is None else blocks).detach()
         parts = (self.ent_ptr, self.entries, self.row_ptr, self.col_idx, self.blk_idx, self.stored_col)
-        # the patterns' transposed structure is kept as long as the buffers are the same tensors
-        if self._made is None or any(p is not q for p, q in zip(self._made[0], parts)):
-            self._made = (parts, {})
+        # the patterns' transposed structure is kept until a buffer is replaced or written (load_state_dict)
+        versions = tuple(p._version for p in parts)
+        if self._made[1] != versions or any(p is not q for p, q in zip(self._made[0], parts)):
+            self._made = (parts, versions, {})
         return GatedWeights(blocks=b, gate_blocks=self.gate_blocks, shape=self.shape, block=self.block,
                             ent_ptr=parts[0], entries=parts[1], row_ptr=parts[2], col_idx=parts[3], blk_idx=parts[4],
-                            stored_col=parts[5], _structure=self._made[1])
+                            stored_col=parts[5], _structure=self._made[2])
 
     def forward(self, X: Tensor) -> Tensor:
         if not torch.is_grad_enabled():

@@ -13,7 +13,7 @@ import math
 import pytest
 import torch
 
-from kairo_b200 import ops
+from kairo_b200 import _lib, ops
 from kairo_b200.ops import bsr_from_tiles
 
 pytestmark = pytest.mark.gpu
@@ -119,3 +119,252 @@ def test_tokens(tokens, b, dtype):
                                                       (260, 640, 2048, 64, 0.05, False), (40, 1, 1, 16, 1.0, True)])
 def test_shapes(tokens, m, k, b, keep, shared, act):
     run_case(tokens, m, k, b, torch.bfloat16 if tokens % 20 else torch.float16, act=act, keep=keep, shared=shared)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens", [9, 16, 17, 32, 33, 64, 65])
+def test_many_rows(tokens, dtype):
+    """256 block-rows and more: the blocks are streamed."""
+    run_case(tokens, 64 * 259 - 7, 136, 64, dtype, act="silu")
+
+
+@pytest.mark.parametrize("tokens,b,nbc", [(1, 64, 70), (3, 16, 300), (20, 32, 67), (40, 32, 67), (50, 16, 80),
+                                          (600, 64, 70), (300, 16, 140)])
+def test_long_rows(tokens, b, nbc):
+    """Rows of more entries than a window holds."""
+    run_case(tokens, 2 * b, b * nbc, b, torch.bfloat16, keep=0.95, act="gelu")
+
+
+@pytest.mark.parametrize("tokens", [1, 12, 50, 300])
+@pytest.mark.parametrize("b", [64, 32, 16])
+def test_empty_parts(tokens, b):
+    """Rows that keep nothing, a weight that keeps nothing, two that keep nothing."""
+    m, k = 5 * b - 3, 4 * b
+    g = torch.Generator(device="cuda").manual_seed(3)
+    some = torch.tensor([0, 1, 3, 9, 10, 17], device="cuda")  # rows 0, 2 and 4 of 5
+    none = some[:0]
+    for pg, pu in ((some, some), (some, none), (none, some), (none, none), (some[:2], some[3:])):
+        gate, wg, _ = weight(m, k, b, 0.5, torch.bfloat16, g, pos=pg)
+        up, wu, _ = weight(m, k, b, 0.5, torch.bfloat16, g, pos=pu)
+        w = ops.gated_weights(gate, up)
+        x = torch.randn(tokens, k, generator=g, device="cuda").bfloat16()
+        dh = torch.randn(tokens, m, generator=g, device="cuda").bfloat16()
+        out = torch.full((tokens + 1, m), 7.0, device="cuda").bfloat16()
+        h = ops.sparse_gated_linear(x, w, out=out[:tokens], check=True)
+        assert (out[tokens] == 7).all()  # the row behind the last token is left as it was
+        dx, db = ops.sparse_gated_linear_backward(dh, x, w, check=True)
+        check(x, dh, wg, wu, gate, up, "silu", h, dx, *w.split(db))
+
+
+@pytest.mark.parametrize("tokens", [5, 40, 300])
+def test_layouts(tokens):
+    """Blocks out of order, rows of a wider matrix, rows at odd addresses, a transposed X, a broadcast dH."""
+    x, dh, gate, up, wg, wu = case(tokens, 200, 203, 32, torch.bfloat16, shuffle=True)
+    w = ops.gated_weights(gate, up)
+    assert gate.blk_idx is not None
+    g, u = w.matrices()
+    assert torch.equal(g.col_idx, gate.col_idx) and torch.equal(u.row_ptr, up.row_ptr)
+    want = ops.sparse_gated_linear(x, w)
+    wide = torch.full((tokens, 512), 9.0, device="cuda").bfloat16()
+    for at in (0, 1, 8):
+        wide[:, at:at + 203] = x
+        assert torch.equal(ops.sparse_gated_linear(wide[:, at:at + 203], w, check=True), want)
+    assert torch.equal(ops.sparse_gated_linear(x.t().contiguous().t(), w), want)
+    for at in (0, 3):
+        out = torch.full((tokens, 256), 5.0, device="cuda").bfloat16()
+        ops.sparse_gated_linear(x, w, out=out[:, at:at + 200])
+        assert torch.equal(out[:, at:at + 200], want) and (out[:, at + 200:] == 5).all() and (out[:, :at] == 5).all()
+    row = torch.randn(1, 200, device="cuda").bfloat16().expand(tokens, 200)
+    for d in (row, dh.t().contiguous().t()):
+        a = ops.sparse_gated_linear_backward(d, x, w)
+        b = ops.sparse_gated_linear_backward(d.contiguous(), x, w)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    dx, db = ops.sparse_gated_linear_backward(dh, x, w, need_dw=False)
+    assert db is None
+    dx2, db = ops.sparse_gated_linear_backward(dh, x, w, need_dx=False)
+    assert dx2 is None
+    dx3, db32 = ops.sparse_gated_linear_backward(dh, x, w, dw_dtype=torch.float32)
+    assert torch.equal(dx, dx3) and db32.dtype == torch.float32 and torch.equal(db32.bfloat16(), db)
+
+
+def test_no_tokens():
+    x, dh, gate, up, wg, wu = case(4, 100, 100, 32, torch.float16)
+    w = ops.gated_weights(gate, up)
+    assert ops.sparse_gated_linear(x[:0], w).shape == (0, 100)
+    dx, db = ops.sparse_gated_linear_backward(dh[:0], x[:0], w)
+    assert dx.shape == (0, 100) and db.shape == w.blocks.shape and not db.any()
+
+
+@pytest.mark.parametrize("tokens", [6, 40, 300])
+@pytest.mark.parametrize("b", [64, 16])
+def test_not_finite(tokens, b):
+    """An infinity or a NaN reaches the rows that keep a block in its column, of its token, and no others."""
+    x, dh, gate, up, wg, wu = case(tokens, 6 * b, 5 * b, b, torch.bfloat16, keep=0.3)
+    w = ops.gated_weights(gate, up)
+    want = ops.sparse_gated_linear(x, w)
+    bad = x.clone()
+    bad[2, 0], bad[4, 3 * b + 1] = float("nan"), float("inf")
+    got = ops.sparse_gated_linear(bad, w)
+    keeps = (wg.view(6, b, 5, b).abs().amax((1, 3)) + wu.view(6, b, 5, b).abs().amax((1, 3))) > 0  # row, column
+    for token, col in ((2, 0), (4, 3)):
+        hit = keeps[:, col].repeat_interleave(b)
+        assert not torch.isfinite(got[token, hit]).any()
+        assert torch.equal(got[token, ~hit], want[token, ~hit])
+    others = [t for t in range(tokens) if t not in (2, 4)]
+    assert torch.equal(got[others], want[others])
+
+
+@pytest.mark.parametrize("tokens", [4, 20, 50, 300])
+@pytest.mark.parametrize("b", [64, 32])
+def test_malformed_entries(tokens, b):
+    """An entry out of range is recorded and read nowhere; the next call is clean."""
+    x, dh, gate, up, wg, wu = case(tokens, 260 * b if tokens == 20 else 3 * b, 4 * b, b, torch.bfloat16, keep=0.9)
+    w = ops.gated_weights(gate, up)
+    want = ops.sparse_gated_linear(x, w, check=True)
+    for field, value in ((0, 4), (0, -1), (1, w.blocks.shape[0]), (2, 1 << 30), (1, -2)):
+        kept = w.entries[1].clone()
+        w.entries[1, field] = value
+        with pytest.raises(_lib.KairoDeviceError) as e:
+            ops.sparse_gated_linear(x, w, check=True)
+        assert e.value.code & 0xFF == _lib.DEVERR_BAD_INDEX
+        ops.sparse_gated_linear(x, w)
+        assert ops.pending_device_error() & 0xFF == _lib.DEVERR_BAD_INDEX
+        assert ops.pending_device_error() == 0
+        w.entries[1] = kept
+    kept = w.ent_ptr.clone()
+    w.ent_ptr[-1] = 1 << 30  # clamped to the entries there are
+    assert torch.equal(ops.sparse_gated_linear(x, w, check=True), want)
+    w.ent_ptr.copy_(kept)
+    assert torch.equal(ops.sparse_gated_linear(x, w, check=True), want)
+
+
+@pytest.mark.parametrize("tokens", [7, 50, 700])
+def test_repeats_graphs_and_streams(tokens):
+    x, dh, gate, up, wg, wu = case(tokens, 320, 320, 64, torch.bfloat16)
+    w = ops.gated_weights(gate, up)
+
+    def both(x, dh):
+        return (ops.sparse_gated_linear(x, w), *ops.sparse_gated_linear_backward(dh, x, w))
+
+    want = both(x, dh)
+    assert all(torch.equal(a, b) for a, b in zip(want, both(x, dh)))
+    other = [torch.randn_like(x), torch.randn_like(dh)]
+    want2 = both(*other)
+    # two graphs, captured on one stream, replayed at the same time
+    inputs = [[x.clone(), dh.clone()] for _ in range(2)]
+    graphs, outs, side = [], [], torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both(x, dh)
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            outs.append(both(*inputs[i]))
+        graphs.append(g)
+    for t, v in zip(inputs[1], other):
+        t.copy_(v)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs[0], want))
+    assert all(torch.equal(a, b) for a, b in zip(outs[1], want2))
+    # eager calls on two streams at once
+    got = [None, None]
+    for _ in range(3):
+        for i, (args, s) in enumerate(zip(((x, dh), tuple(other)), streams)):
+            with torch.cuda.stream(s):
+                got[i] = both(*args)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got[0], want))
+        assert all(torch.equal(a, b) for a, b in zip(got[1], want2))
+
+
+def test_first_backward_in_a_capture_is_refused():
+    x, dh, gate, up, wg, wu = case(8, 64, 64, 32, torch.bfloat16)
+    w = ops.gated_weights(gate, up)
+    ops.sparse_gated_linear(x, w)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="before capturing"):
+        with torch.cuda.graph(g, stream=s):
+            ops.sparse_gated_linear_backward(dh, x, w)
+    torch.cuda.synchronize()
+    ops.sparse_gated_linear_backward(dh, x, w, check=True)
+
+
+def test_offsets_beyond_32_bits():
+    """H and dP of more than 2^32 values: the last tokens' rows are those of the same tokens alone."""
+    tokens, m, k = 70_000, 32_768, 64
+    x, dh, gate, up, wg, wu = case(130, m, k, 64, torch.bfloat16, keep=0.9)
+    w = ops.gated_weights(gate, up)
+    big = torch.zeros(tokens, k, device="cuda").bfloat16()
+    big[-130:] = x
+    h = ops.sparse_gated_linear(big, w, check=True)
+    assert h.numel() > 2**31 and torch.equal(h[-130:], ops.sparse_gated_linear(x, w)) and not h[:-130].any()
+    del h
+    d = torch.zeros(tokens, m, device="cuda").bfloat16()
+    d[-130:] = dh
+    dx, db = ops.sparse_gated_linear_backward(d, big, w, check=True)
+    dx1, db1 = ops.sparse_gated_linear_backward(dh, x, w)
+    assert torch.equal(dx[-130:], dx1) and not dx[:-130].any()
+    # the weight gradient adds the same 130 rows, in other steps of 16
+    assert (db.double() - db1.double()).norm() <= torch.finfo(torch.bfloat16).eps * db1.double().norm()
+
+
+def test_module_and_differences():
+    """Gradients of the module against the formula's, and against differences of its own outputs."""
+    x, dh, gate, up, wg, wu = case(60, 130, 100, 32, torch.float16, act="gelu_tanh", keep=0.6)
+    layer = ops.SparseGatedLinear(gate, up, activation="gelu_tanh")
+    xr = x.clone().requires_grad_(True)
+    h = layer(xr)
+    h.backward(dh)
+    check(x, dh, wg, wu, gate, up, "gelu_tanh", h.detach(), xr.grad, *layer.weights().split(layer.blocks.grad))
+    with torch.no_grad():
+        assert torch.equal(layer(x), h)
+    # along a direction: <dX, d> against (<dH, H(x + d)> - <dH, H(x - d)>) / 2.  H is rounded to fp16 and
+    # its sums are off as above; beside that the difference of third order, taken from the formula.
+    d = torch.randn_like(x) * 2.0**-5
+    plus, minus = x + d, x - d
+    delta = (plus.double() - minus.double()) / 2
+    slope = (xr.grad.double() * delta).sum()
+    with torch.no_grad():
+        diff = ((layer(plus).double() - layer(minus).double()) * dh.double()).sum() / 2
+
+    def exact(v):
+        return act64(v.double() @ wg.t(), "gelu_tanh")[0] * (v.double() @ wu.t())
+
+    true = ((exact(plus) - exact(minus)) * dh.double()).sum() / 2
+    eps = torch.finfo(torch.float16).eps / 2
+    noise = 2 * eps * ((exact(plus).abs() + exact(minus).abs()) * dh.double().abs()).sum() / 2
+    assert (diff - true).abs() <= noise
+    rounding = 4 * eps * ((xr.grad.double() * delta).abs()).sum() + noise
+    f, da = act64(x.double() @ wg.t(), "gelu_tanh")
+    grad64 = (dh.double() * (x.double() @ wu.t()) * da) @ wg + (dh.double() * f) @ wu
+    curvature = (true - (grad64 * delta).sum()).abs()
+    assert (slope - diff).abs() <= rounding + curvature
+
+
+def test_module_patterns_may_be_loaded():
+    """A state dict of another pattern with as many blocks: the kept structure follows."""
+    pos = torch.tensor([0, 3, 5], device="cuda"), torch.tensor([1, 2, 6], device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    mats = [weight(96, 96, 32, 0.3, torch.bfloat16, g, pos=p) for p in (*pos, pos[1], pos[0])]
+    one = ops.SparseGatedLinear(mats[0][0], mats[1][0])
+    two = ops.SparseGatedLinear(mats[2][0], mats[3][0])
+    x, dh = torch.randn(9, 96, device="cuda").bfloat16(), torch.randn(9, 96, device="cuda").bfloat16()
+
+    def grads(layer):
+        layer.blocks.grad = None
+        xr = x.clone().requires_grad_(True)
+        layer(xr).backward(dh)
+        return xr.grad, layer.blocks.grad.clone()
+
+    grads(one)
+    want = grads(two)
+    one.load_state_dict(two.state_dict())
+    assert all(torch.equal(a, b) for a, b in zip(grads(one), want))
