@@ -44,15 +44,13 @@ constexpr int kPairTileM = 256;      // rows of a cluster's tile (128 a CTA)
 constexpr int kPairTileN = 256;
 constexpr int kPairK = 64;           // k of one stage
 constexpr int kPairHalf = 128 * kPairK * 2;  // bytes of one operand's part of a stage in one CTA
-constexpr int kPairBoxes = 2;
-constexpr int kPairBoxRows = 128 / kPairBoxes;
-// Bytes of a stage and stages, for A_ROWS rows of A in each CTA (128, or 64: see below); 192 KB in all.
-constexpr int pair_stage_bytes(int a_rows) { return a_rows * kPairK * 2 + kPairHalf; }
-constexpr int pair_stages(int a_rows) { return 192 * 1024 / pair_stage_bytes(a_rows); }
+constexpr int kPairBoxRows = 64;  // of a copy, at most
+// Bytes of a stage and stages, for tiles of `tn` columns; 192 KB in all.
+constexpr int pair_stage_bytes(int tn) { return kPairHalf + tn / 2 * kPairK * 2; }
+constexpr int pair_stages(int tn) { return 192 * 1024 / pair_stage_bytes(tn); }
 constexpr int kPairEpiCols = kPairTileN / (kPairEpiWarps / 4);
 constexpr int kPairOutBytes = 4096;  // of each epilogue warp, to turn rows a lane into rows a warp
-constexpr size_t kPairSmem =
-    192 * 1024 + kPairEpiWarps * kPairOutBytes + 2048;
+constexpr size_t kPairSmem = 192 * 1024 + kPairEpiWarps * kPairOutBytes + 2048;
 constexpr int kPairClusters = 74;    // pairs of a B200's 148 SMs, for plans that must not depend on the current device
 static_assert(kPairSmem <= kMaxSmem, "shared memory");
 
@@ -62,7 +60,7 @@ struct PairShape {
   int tiles_m, tiles_n, ksteps, group_m;
   int seg;     // stages of one segment
   int splits;  // parts of k, each a tile of its own
-  int copies;  // of A's rows, copy_rows after one another: cluster c reads copy c % copies (one row of tiles only)
+  int copies;  // of B's rows, copy_rows after one another: cluster c reads copy c % copies (one column of tiles only)
   int copy_rows;
 };
 
@@ -89,26 +87,25 @@ __device__ __forceinline__ PairTile pair_tile(const PairShape& s, int t) {
 
 // Epi supplies `struct Args` and
 //   __device__ Epi(const Args&, int row_in_tile, int part, uint8_t* out)
-//   __device__ void tile(const PairTile&, float (&v)[kPairEpiCols])   its columns of one tile
-//   __device__ void done()                                            after the CTA's last tile
+//   __device__ void tile(const PairTile&, float (&v)[TN / 2])   its columns of one tile
+//   __device__ void done()                                      after the CTA's last tile
 // and is made once per thread and launch; `out` is the warp's kPairOutBytes.
 //
-// A_ROWS = 64: A has at most 64 rows.  Only the leader loads them, 64 of its 128; what the MMAs
-// read in the place of the others (the stage's B, or what an earlier stage left) ends in rows of the
-// accumulator that no epilogue looks at.  B then has 128 KB of copies under way instead of 96.
-template <int IN_FMT, bool A_MN, bool B_MN, class Epi, int A_ROWS>
+// TN: columns of a tile.  64 where B has few rows (the tokens to be scored) and A is the large operand: a
+// stage is then 16 KB of A and 4 KB of B, and a product costs 70 cycles instead of 128.
+template <int IN_FMT, bool A_MN, bool B_MN, class Epi, int TN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     k_pair_gemm(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                 const PairShape shape, unsigned* err, const typename Epi::Args eargs) {
-  constexpr int ST = pair_stages(A_ROWS);
-  constexpr int STAGE = pair_stage_bytes(A_ROWS), A_BYTES = STAGE - kPairHalf;
-  constexpr bool FEW = A_ROWS < 128;
-  static_assert(A_ROWS == 128 || (A_ROWS == 64 && !A_MN), "rows of A");
-  constexpr uint32_t IDESC = ptx::make_idesc_f16(IN_FMT, A_MN ? 1u : 0u, B_MN ? 1u : 0u, kPairTileM, kPairTileN);
-  constexpr uint32_t TMEM_COLS = 2 * kPairTileN;
-  // A CTA's half of an operand comes in kPairBoxes boxes, one lane each: 64 k x 64 rows, or 64
-  // columns x 64 k.
-  constexpr int NA = kPairBoxes * A_ROWS / 128, NB = kPairBoxes;
+  constexpr int ST = pair_stages(TN);
+  constexpr int STAGE = pair_stage_bytes(TN);
+  static_assert(TN == 256 || (TN == 64 && !B_MN), "columns of a tile");
+  constexpr uint32_t IDESC = ptx::make_idesc_f16(IN_FMT, A_MN ? 1u : 0u, B_MN ? 1u : 0u, kPairTileM, TN);
+  constexpr uint32_t TMEM_COLS = 2 * TN;
+  constexpr int COLS = TN / (kPairEpiWarps / 4);  // of an epilogue warp
+  // A CTA's half of an operand comes in boxes, one lane each: 64 k x up to 64 rows, or 64 columns x 64 k.
+  constexpr int BOX_B = TN / 2 < kPairBoxRows ? TN / 2 : kPairBoxRows;
+  constexpr int NA = 128 / kPairBoxRows, NB = TN / 2 / BOX_B;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -159,21 +156,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 
   if (warp == 0) {
     // ------------------------------------------------------------ loads
-    const uint64_t pol = ptx::policy_evict_last();
     const bool is_a = lane < NA;
+    const uint64_t pol = ptx::policy_evict_last();
     const int box = is_a ? lane : lane - NA;
     const void* map = is_a ? static_cast<const void*>(&tmap_a) : static_cast<const void*>(&tmap_b);
-    const uint32_t mine = lane < NA + NB && !(FEW && is_a && rank != 0) ? 1u : 0u;
-    constexpr uint32_t BYTES = FEW ? A_BYTES + 2 * kPairHalf : 2 * STAGE;  // of a stage, both CTAs
+    const uint32_t mine = lane < NA + NB ? 1u : 0u;
     const bool mn = is_a ? A_MN : B_MN;
-    const uint32_t dst_off = (is_a ? 0u : A_BYTES) + static_cast<uint32_t>(mine ? box : 0) * (kPairHalf / kPairBoxes);
-    const int shift = is_a ? first % shape.copies * shape.copy_rows : 0;
+    const uint32_t dst_off = (is_a ? 0u : kPairHalf) + static_cast<uint32_t>(mine ? box : 0) * (kPairBoxRows * kPairK * 2);
+    const int shift = is_a ? 0 : first % shape.copies * shape.copy_rows;
     int sidx = 0;
     uint32_t sph = 0;
     bool alive = true;
     for (int t = first; t < ntiles && alive; t += step) {
       const PairTile pt = pair_tile(shape, t);
-      const int r0 = (is_a ? pt.mt : pt.nt) * 256 + static_cast<int>(rank) * 128 + box * kPairBoxRows + shift;
+      const int r0 = (is_a ? pt.mt * 256 + static_cast<int>(rank) * 128 : pt.nt * TN + static_cast<int>(rank) * (TN / 2)) +
+                     box * kPairBoxRows + shift;
       for (int k = pt.k0; k < pt.k1; ++k) {
         int ok = ptx::wait_parity(&empty[sidx], sph ^ 1u, abort_flag, err, kTagEmpty, kWaitCycles);
         ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -184,7 +181,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         const uint32_t bar = ptx::peer_smem_u32(&full[sidx], 0);
         if (rank == 0) {
           if (lane == 0) issued[sidx] = static_cast<int>(sph) + 1;
-          ptx::mbar_expect_tx_if(lane == 0 ? 1u : 0u, &full[sidx], BYTES);
+          ptx::mbar_expect_tx_if(lane == 0 ? 1u : 0u, &full[sidx], 2 * STAGE);
         }
         ptx::tma_load_2d_pair_if(mine, smem + sidx * STAGE + dst_off, map, mn ? r0 : k * kPairK,
                                  mn ? k * kPairK : r0, bar, pol);
@@ -200,10 +197,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     // ------------------------------------------------------------ MMA issuer
     const uint32_t leader = lane == 0 ? 1u : 0u;
     const uint32_t sbase = ptx::smem_u32(smem);
-    const uint64_t adesc = A_MN ? ptx::make_smem_desc(sbase, kPairHalf / 2, 1024, 2u)
+    const uint64_t adesc = A_MN ? ptx::make_smem_desc(sbase, kPairBoxRows * kPairK * 2, 1024, 2u)
                                 : ptx::make_smem_desc(sbase, 16, 1024, 2u);
-    const uint64_t bdesc = B_MN ? ptx::make_smem_desc(sbase + A_BYTES, kPairHalf / 2, 1024, 2u)
-                                : ptx::make_smem_desc(sbase + A_BYTES, 16, 1024, 2u);
+    const uint64_t bdesc = B_MN ? ptx::make_smem_desc(sbase + kPairHalf, kPairBoxRows * kPairK * 2, 1024, 2u)
+                                : ptx::make_smem_desc(sbase + kPairHalf, 16, 1024, 2u);
     const uint32_t a_lo = static_cast<uint32_t>(adesc), a_hi = static_cast<uint32_t>(adesc >> 32);
     const uint32_t b_lo = static_cast<uint32_t>(bdesc), b_hi = static_cast<uint32_t>(bdesc >> 32);
     // 16 k further: 32 bytes along a 128-byte row, or 16 rows of 128 bytes
@@ -221,7 +218,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           break;
         }
         ptx::tc_fence_after();
-        const uint32_t d = tmem_base + static_cast<uint32_t>(slot * kPairTileN);
+        const uint32_t d = tmem_base + static_cast<uint32_t>(slot * TN);
         const int k1 = min(pt.k1, k0 + shape.seg);
         for (int k = k0; k < k1; ++k) {
           ok = ptx::wait_parity(&full[sidx], sph, abort_flag, err, kTagFull, kWaitCycles);
@@ -267,7 +264,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     bool alive = true;
     for (int t = first; t < ntiles && alive; t += step) {
       const PairTile pt = pair_tile(shape, t);
-      float v[kPairEpiCols];
+      float v[COLS];
       for (int k0 = pt.k0; k0 < pt.k1; k0 += shape.seg) {
         int ok = ptx::wait_parity(&tfull[slot], aphase, abort_flag, err, kTagTmemFull, kWaitCycles);
         ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -276,14 +273,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           break;
         }
         ptx::tc_fence_after();
-        const uint32_t at = tmem_base + lane_addr + static_cast<uint32_t>(slot * kPairTileN + part * kPairEpiCols);
+        const uint32_t at = tmem_base + lane_addr + static_cast<uint32_t>(slot * TN + part * COLS);
         if (k0 == pt.k0) {
 #pragma unroll
-          for (int c = 0; c < kPairEpiCols; c += 32) ptx::tmem_ld32(at + c, v + c);
+          for (int c = 0; c < COLS; c += 32) ptx::tmem_ld32(at + c, v + c);
           ptx::tmem_wait_ld();
         } else {
 #pragma unroll
-          for (int c = 0; c < kPairEpiCols; c += 32) {
+          for (int c = 0; c < COLS; c += 32) {
             float w[32];
             ptx::tmem_ld32(at + c, w);
             ptx::tmem_wait_ld();
@@ -323,12 +320,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 
 // Tensor map of one operand: K-major `rows` x `k`, or MN-major `k` x `rows` (rows of the tile along x).
 inline kairo_status pair_operand_map(CUtensorMap* map, const void* base, kairo_dtype dt, bool mn, int64_t rows,
-                                     int64_t k, int64_t ld, const char* what) {
+                                     int64_t k, int64_t ld, const char* what, int box_rows = kPairBoxRows) {
   const CUtensorMapDataType t = dt == KAIRO_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   return mn ? make_map_2d(map, base, t, 2, static_cast<uint64_t>(rows), static_cast<uint64_t>(k),
                           static_cast<uint64_t>(ld), 64, kPairK, what)
             : make_map_2d(map, base, t, 2, static_cast<uint64_t>(k), static_cast<uint64_t>(rows),
-                          static_cast<uint64_t>(ld), kPairK, kPairBoxRows, what);
+                          static_cast<uint64_t>(ld), kPairK, static_cast<uint32_t>(box_rows), what);
 }
 
 // Clusters of a launch of `tiles` tiles.
@@ -336,10 +333,10 @@ inline int pair_clusters(int64_t tiles) {
   return static_cast<int>(std::min<int64_t>(tiles, std::max(1, device_sm_count(current_device()) / 2)));
 }
 
-template <int IN_FMT, bool A_MN, bool B_MN, class Epi, int A_ROWS = 128>
+template <int IN_FMT, bool A_MN, bool B_MN, class Epi, int TN = kPairTileN>
 kairo_status launch_pair_gemm(const CUtensorMap& a, const CUtensorMap& b, const PairShape& shape, unsigned* err,
                               const typename Epi::Args& args, cudaStream_t s) {
-  auto* fn = &k_pair_gemm<IN_FMT, A_MN, B_MN, Epi, A_ROWS>;
+  auto* fn = &k_pair_gemm<IN_FMT, A_MN, B_MN, Epi, TN>;
   static std::atomic<uint64_t> ready{0};
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(fn), kPairSmem, &ready);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic smem)");

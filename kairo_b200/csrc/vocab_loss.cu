@@ -11,7 +11,10 @@
 // Forward: one pass of k_pair_gemm over W.  A thread of its epilogue owns one
 // token of the tile; it keeps the running maximum and sum of its columns (base
 // 2) and picks the target's logit as it goes by, so 8 bytes leave the SM per
-// token and 128 columns.  k_lse joins them.
+// token and 128 columns.  k_lse joins them.  Up to 64 tokens the two operands change
+// places: the table, all there is to read, fills whole tiles, and the products
+// cost half (and draw less power, which the clock shows: 64 tokens of 131072 x
+// 4096 take 265 us with tiles of 256 tokens when calls follow one another).
 //
 // Backward: pieces of the vocabulary, as many columns as keep a 16-bit G of
 // all tokens within kPieceBytes.  Per piece the logits are formed again and
@@ -142,6 +145,82 @@ __device__ __forceinline__ uint4 shift8(uint4 a, uint4 b, int e) {
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
+
+// The same for few tokens, with the vocabulary down the rows: a warp has 32 rows of the table and 32 tokens,
+// lane j keeps token j.
+struct FewStatsEpi {
+  static constexpr int TOKENS = 64;  // columns of a tile
+  struct Args {
+    float2* part;  // [clusters * 8][tokens]
+    float* target;
+    Targets ids;
+    int tokens, vocab;
+    float scale;
+    unsigned* ticket;
+  };
+  const Args& a;
+  int row, token;
+  int64_t id;
+  float m = -INFINITY, s = 0.f;
+
+  __device__ FewStatsEpi(const Args& args, int row_in_tile, int part, uint8_t*)
+      : a(args), row(row_in_tile), token(part * 32 + static_cast<int>(threadIdx.x & 31)) {
+    if (blockIdx.x == 0 && row_in_tile == 0 && part == 0) *a.ticket = 0u;
+    id = token < a.tokens ? a.ids[token] : -1;
+    if (id >= a.vocab) id = -1;
+  }
+
+  // 32 values of each lane -> lane j has `op` over all lanes' value j
+  template <class F>
+  static __device__ __forceinline__ float across(float (&v)[32], F op) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const bool up = lane & o;
+#pragma unroll
+      for (int i = 0; i < o; ++i) {
+        const float give = up ? v[i] : v[i + o], keep = up ? v[i + o] : v[i];
+        v[i] = op(keep, __shfl_xor_sync(0xffffffffu, give, o));
+      }
+    }
+    return v[0];
+  }
+
+  __device__ void tile(const PairTile& pt, float (&v)[32]) {
+    const int lane = threadIdx.x & 31;
+    const int r = pt.mt * kPairTileM + row;
+    const int64_t at = id - (r - lane);
+    const unsigned hits = __ballot_sync(0xffffffffu, id >= 0 && at >= 0 && at < 32);
+    if (hits) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (hits >> j & 1u) {
+          const float z = __shfl_sync(0xffffffffu, v[j], static_cast<int>(__shfl_sync(0xffffffffu, at, j)));
+          if (lane == j) a.target[token] = z * a.scale;
+        }
+    }
+    const float k = a.scale * kLog2e;
+    const bool in = r < a.vocab;
+    float w[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      v[j] = in ? v[j] * k : -INFINITY;
+      w[j] = v[j];
+    }
+    const float top = fmaxf(m, across(w, [](float x, float y) { return fmaxf(x, y); }));
+    const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) w[j] = ex2(v[j] - __shfl_sync(0xffffffffu, ref, j));
+    const float sum = across(w, [](float x, float y) { return x + y; });
+    s = s * ex2(m - ref) + sum;
+    m = top;
+  }
+
+  __device__ void done() {
+    const int64_t slot = static_cast<int64_t>(blockIdx.x) * 4 + ((row >> 5) & 3);
+    if (token < a.tokens) a.part[slot * a.tokens + token] = make_float2(m, s);
+  }
+};
 
 // A warp's 32 rows x kPairEpiCols results, a row a lane, rounded to T at p (16-byte aligned rows of
 // pitch ld; `rows` and `cols` of them exist).  They pass through shared memory, 64 columns at a
@@ -618,7 +697,7 @@ LossWs loss_ws(const Problem& p) {
   o.ticket = 128;
   o.target = take(4 * static_cast<size_t>(p.tokens));
   o.each = take(4 * static_cast<size_t>(p.tokens));
-  const int64_t slots = 2 * tiles(p.vocab);
+  const int64_t slots = p.tokens <= FewStatsEpi::TOKENS ? 8 * kPairClusters : 2 * tiles(p.vocab);
   o.part = take(8 * static_cast<size_t>(p.tokens) * static_cast<size_t>(slots));
   const size_t ld = static_cast<size_t>(copy_ld(p.dim));
   const int64_t copies = copies_of(std::max<int64_t>(1, p.tokens));
@@ -773,22 +852,33 @@ kairo_status run_loss(Problem p, float* loss, float* lse, uint8_t* ws, unsigned*
   if (st == KAIRO_STATUS_SUCCESS) st = aligned_rows(&p.w, &p.ldw, p.vocab, p.dim, ws + o.w, s);
   if (st) return st;
   unsigned* ticket = reinterpret_cast<unsigned*>(ws + o.ticket);
-  CUtensorMap ma, mb;
-  st = pair_operand_map(&ma, p.x, p.dt, false, p.tokens * copies, p.dim, p.ldx, "hidden states");
-  if (st == KAIRO_STATUS_SUCCESS) st = pair_operand_map(&mb, p.w, p.dt, false, p.vocab, p.dim, p.ldw, "vocabulary table");
+  float2* part = reinterpret_cast<float2*>(ws + o.part);
+  float* target = reinterpret_cast<float*>(ws + o.target);
+  const int tokens = static_cast<int>(p.tokens), vocab = static_cast<int>(p.vocab);
+  const bool few = p.tokens <= FewStatsEpi::TOKENS;
+  CUtensorMap mx, mw;
+  st = pair_operand_map(&mx, p.x, p.dt, false, p.tokens * copies, p.dim, p.ldx, "hidden states",
+                        few ? FewStatsEpi::TOKENS / 2 : kPairBoxRows);
+  if (st == KAIRO_STATUS_SUCCESS) st = pair_operand_map(&mw, p.w, p.dt, false, p.vocab, p.dim, p.ldw, "vocabulary table");
   if (st) return st;
-  PairShape sh = shape_of(p.tokens, p.vocab, p.dim, kSegLogits);
-  sh.copies = static_cast<int>(copies);
-  sh.copy_rows = static_cast<int>(p.tokens);
-  StatsEpi::Args a{reinterpret_cast<float2*>(ws + o.part), reinterpret_cast<float*>(ws + o.target), p.ids,
-                   static_cast<int>(p.tokens), static_cast<int>(p.vocab), p.scale, sh.tiles_m == 1, ticket};
-  // up to 64 tokens the table alone bounds it: more of it under way
-  st = p.tokens <= 64 ? launch_pair_gemm<FMT, false, false, StatsEpi, 64>(ma, mb, sh, err, a, s)
-                      : launch_pair_gemm<FMT, false, false, StatsEpi>(ma, mb, sh, err, a, s);
+  int slots;
+  if (few) {
+    PairShape sh = shape_of(p.vocab, 1, p.dim, kSegLogits);
+    sh.copies = static_cast<int>(copies);
+    sh.copy_rows = tokens;
+    slots = 8 * pair_clusters(sh.tiles_m);
+    if (slots > 8 * kPairClusters) return fail(KAIRO_STATUS_NOT_SUPPORTED, "more SMs than the workspace is laid out for");
+    const FewStatsEpi::Args a{part, target, p.ids, tokens, vocab, p.scale, ticket};
+    st = launch_pair_gemm<FMT, false, false, FewStatsEpi, FewStatsEpi::TOKENS>(mw, mx, sh, err, a, s);
+  } else {
+    const PairShape sh = shape_of(p.tokens, p.vocab, p.dim, kSegLogits);
+    const StatsEpi::Args a{part, target, p.ids, tokens, vocab, p.scale, sh.tiles_m == 1, ticket};
+    slots = 2 * (a.by_cluster ? pair_clusters(sh.tiles_n) : sh.tiles_n);
+    st = launch_pair_gemm<FMT, false, false, StatsEpi>(mx, mw, sh, err, a, s);
+  }
   if (st) return st;
-  const int slots = 2 * (a.by_cluster ? pair_clusters(sh.tiles_n) : sh.tiles_n);
   k_lse<<<static_cast<int>(ceil_div64(p.tokens, 32)), 1024, 0, s>>>(
-      a.part, slots, a.target, p.ids, a.tokens, a.vocab, p.reduction,
+      part, slots, target, p.ids, tokens, vocab, p.reduction,
       p.reduction == kNone ? loss : reinterpret_cast<float*>(ws + o.each), lse, loss, ticket);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "launch of k_lse");
