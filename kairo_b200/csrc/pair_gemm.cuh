@@ -91,15 +91,15 @@ __device__ __forceinline__ PairTile pair_tile(const PairShape& s, int t) {
 //   __device__ void done()                                      after the CTA's last tile
 // and is made once per thread and launch; `out` is the warp's kPairOutBytes.
 //
-// TN: columns of a tile.  64 where B has few rows (the tokens to be scored) and A is the large operand: a
-// stage is then 16 KB of A and 4 KB of B, and a product costs 70 cycles instead of 128.
+// TN: columns of a tile.  64 or 128 where B has few rows (the tokens to be scored) and A is the large
+// operand: a stage is then 16 KB of A and 4 or 8 of B, and a product costs 70 cycles instead of 128.
 template <int IN_FMT, bool A_MN, bool B_MN, class Epi, int TN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     k_pair_gemm(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                 const PairShape shape, unsigned* err, const typename Epi::Args eargs) {
   constexpr int ST = pair_stages(TN);
   constexpr int STAGE = pair_stage_bytes(TN);
-  static_assert(TN == 256 || (TN == 64 && !B_MN), "columns of a tile");
+  static_assert(TN == 256 || ((TN == 64 || TN == 128) && !B_MN), "columns of a tile");
   constexpr uint32_t IDESC = ptx::make_idesc_f16(IN_FMT, A_MN ? 1u : 0u, B_MN ? 1u : 0u, kPairTileM, TN);
   constexpr uint32_t TMEM_COLS = 2 * TN;
   constexpr int COLS = TN / (kPairEpiWarps / 4);  // of an epilogue warp

@@ -11,7 +11,7 @@
 // Forward: one pass of k_pair_gemm over W.  A thread of its epilogue owns one
 // token of the tile; it keeps the running maximum and sum of its columns (base
 // 2) and picks the target's logit as it goes by, so 8 bytes leave the SM per
-// token and 128 columns.  k_lse joins them.  Up to 64 tokens the two operands change
+// token and 128 columns.  k_lse joins them.  Up to 128 tokens the two operands change
 // places: the table, all there is to read, fills whole tiles, and the products
 // cost half (and draw less power, which the clock shows: 64 tokens of 131072 x
 // 4096 take 265 us with tiles of 256 tokens when calls follow one another).
@@ -146,10 +146,11 @@ __device__ __forceinline__ uint4 shift8(uint4 a, uint4 b, int e) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// The same for few tokens, with the vocabulary down the rows: a warp has 32 rows of the table and 32 tokens,
-// lane j keeps token j.
+// The same for few tokens, with the vocabulary down the rows: a warp has 32 rows of the table and GROUPS times 32
+// tokens, of which lane j keeps the j-th.
+template <int GROUPS>
 struct FewStatsEpi {
-  static constexpr int TOKENS = 64;  // columns of a tile
+  static constexpr int TOKENS = 64 * GROUPS;  // columns of a tile
   struct Args {
     float2* part;  // [clusters * 8][tokens]
     float* target;
@@ -159,15 +160,20 @@ struct FewStatsEpi {
     unsigned* ticket;
   };
   const Args& a;
-  int row, token;
-  int64_t id;
-  float m = -INFINITY, s = 0.f;
+  int row, token;  // of the first group
+  int64_t id[GROUPS];
+  float m[GROUPS], s[GROUPS];
 
   __device__ FewStatsEpi(const Args& args, int row_in_tile, int part, uint8_t*)
-      : a(args), row(row_in_tile), token(part * 32 + static_cast<int>(threadIdx.x & 31)) {
+      : a(args), row(row_in_tile), token(part * 32 * GROUPS + static_cast<int>(threadIdx.x & 31)) {
     if (blockIdx.x == 0 && row_in_tile == 0 && part == 0) *a.ticket = 0u;
-    id = token < a.tokens ? a.ids[token] : -1;
-    if (id >= a.vocab) id = -1;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      id[g] = token + 32 * g < a.tokens ? a.ids[token + 32 * g] : -1;
+      if (id[g] >= a.vocab) id[g] = -1;
+      m[g] = -INFINITY;
+      s[g] = 0.f;
+    }
   }
 
   // 32 values of each lane -> lane j has `op` over all lanes' value j
@@ -186,39 +192,46 @@ struct FewStatsEpi {
     return v[0];
   }
 
-  __device__ void tile(const PairTile& pt, float (&v)[32]) {
+  __device__ void tile(const PairTile& pt, float (&all)[32 * GROUPS]) {
     const int lane = threadIdx.x & 31;
     const int r = pt.mt * kPairTileM + row;
-    const int64_t at = id - (r - lane);
-    const unsigned hits = __ballot_sync(0xffffffffu, id >= 0 && at >= 0 && at < 32);
-    if (hits) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (hits >> j & 1u) {
-          const float z = __shfl_sync(0xffffffffu, v[j], static_cast<int>(__shfl_sync(0xffffffffu, at, j)));
-          if (lane == j) a.target[token] = z * a.scale;
-        }
-    }
     const float k = a.scale * kLog2e;
     const bool in = r < a.vocab;
-    float w[32];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      v[j] = in ? v[j] * k : -INFINITY;
-      w[j] = v[j];
+    for (int g = 0; g < GROUPS; ++g) {
+      if (token - lane + 32 * g >= a.tokens) break;
+      const int64_t at = id[g] - (r - lane);
+      const unsigned hits = __ballot_sync(0xffffffffu, id[g] >= 0 && at >= 0 && at < 32);
+      if (hits) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (hits >> j & 1u) {
+            const int from = static_cast<int>(__shfl_sync(0xffffffffu, at, j));
+            const float z = __shfl_sync(0xffffffffu, all[32 * g + j], from);
+            if (lane == j) a.target[token + 32 * g] = z * a.scale;
+          }
+      }
+      float v[32], w[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        v[j] = in ? all[32 * g + j] * k : -INFINITY;
+        w[j] = v[j];
+      }
+      const float top = fmaxf(m[g], across(w, [](float x, float y) { return fmaxf(x, y); }));
+      const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) w[j] = ex2(v[j] - __shfl_sync(0xffffffffu, ref, j));
+      const float sum = across(w, [](float x, float y) { return x + y; });
+      s[g] = s[g] * ex2(m[g] - ref) + sum;
+      m[g] = top;
     }
-    const float top = fmaxf(m, across(w, [](float x, float y) { return fmaxf(x, y); }));
-    const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) w[j] = ex2(v[j] - __shfl_sync(0xffffffffu, ref, j));
-    const float sum = across(w, [](float x, float y) { return x + y; });
-    s = s * ex2(m - ref) + sum;
-    m = top;
   }
 
   __device__ void done() {
     const int64_t slot = static_cast<int64_t>(blockIdx.x) * 4 + ((row >> 5) & 3);
-    if (token < a.tokens) a.part[slot * a.tokens + token] = make_float2(m, s);
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g)
+      if (token + 32 * g < a.tokens) a.part[slot * a.tokens + token + 32 * g] = make_float2(m[g], s[g]);
   }
 };
 
@@ -672,6 +685,8 @@ int64_t piece_cols(int64_t tokens, int64_t vocab) {
   return tiles(ceil_div64(vocab, pieces)) * kPairTileN;
 }
 
+constexpr int64_t kFewTokens = FewStatsEpi<2>::TOKENS;  // of the forward pass with the table down the rows
+
 struct LossWs {
   size_t ticket, target, each, part, x, w, total;
 };
@@ -697,7 +712,7 @@ LossWs loss_ws(const Problem& p) {
   o.ticket = 128;
   o.target = take(4 * static_cast<size_t>(p.tokens));
   o.each = take(4 * static_cast<size_t>(p.tokens));
-  const int64_t slots = p.tokens <= FewStatsEpi::TOKENS ? 8 * kPairClusters : 2 * tiles(p.vocab);
+  const int64_t slots = p.tokens <= kFewTokens ? 8 * kPairClusters : 2 * tiles(p.vocab);
   o.part = take(8 * static_cast<size_t>(p.tokens) * static_cast<size_t>(slots));
   const size_t ld = static_cast<size_t>(copy_ld(p.dim));
   const int64_t copies = copies_of(std::max<int64_t>(1, p.tokens));
@@ -855,10 +870,13 @@ kairo_status run_loss(Problem p, float* loss, float* lse, uint8_t* ws, unsigned*
   float2* part = reinterpret_cast<float2*>(ws + o.part);
   float* target = reinterpret_cast<float*>(ws + o.target);
   const int tokens = static_cast<int>(p.tokens), vocab = static_cast<int>(p.vocab);
-  const bool few = p.tokens <= FewStatsEpi::TOKENS;
+  const bool few = p.tokens <= kFewTokens;
+  // tiles of 128 columns take as long as of 64, but draw more power: 64 tokens of 131072 x 4096, called one after
+  // the other, 218 us against 185
+  const bool half = p.tokens <= FewStatsEpi<1>::TOKENS;
   CUtensorMap mx, mw;
   st = pair_operand_map(&mx, p.x, p.dt, false, p.tokens * copies, p.dim, p.ldx, "hidden states",
-                        few ? FewStatsEpi::TOKENS / 2 : kPairBoxRows);
+                        few ? (half ? FewStatsEpi<1>::TOKENS : FewStatsEpi<2>::TOKENS) / 2 : kPairBoxRows);
   if (st == KAIRO_STATUS_SUCCESS) st = pair_operand_map(&mw, p.w, p.dt, false, p.vocab, p.dim, p.ldw, "vocabulary table");
   if (st) return st;
   int slots;
@@ -868,8 +886,12 @@ kairo_status run_loss(Problem p, float* loss, float* lse, uint8_t* ws, unsigned*
     sh.copy_rows = tokens;
     slots = 8 * pair_clusters(sh.tiles_m);
     if (slots > 8 * kPairClusters) return fail(KAIRO_STATUS_NOT_SUPPORTED, "more SMs than the workspace is laid out for");
-    const FewStatsEpi::Args a{part, target, p.ids, tokens, vocab, p.scale, ticket};
-    st = launch_pair_gemm<FMT, false, false, FewStatsEpi, FewStatsEpi::TOKENS>(mw, mx, sh, err, a, s);
+    auto go = [&](auto groups) {
+      using Epi = FewStatsEpi<decltype(groups)::value>;
+      const typename Epi::Args a{part, target, p.ids, tokens, vocab, p.scale, ticket};
+      return launch_pair_gemm<FMT, false, false, Epi, Epi::TOKENS>(mw, mx, sh, err, a, s);
+    };
+    st = half ? go(std::integral_constant<int, 1>{}) : go(std::integral_constant<int, 2>{});
   } else {
     const PairShape sh = shape_of(p.tokens, p.vocab, p.dim, kSegLogits);
     const StatsEpi::Args a{part, target, p.ids, tokens, vocab, p.scale, sh.tiles_m == 1, ticket};
