@@ -798,7 +798,7 @@ kairo_status check_problem(const Problem& p) {
 kairo_status copy_rows(const void* src, int64_t ld, int64_t rows, int64_t cols, int64_t copies, uint8_t* dst,
                        Targets ids, int vocab, const PrepArgs& prep, cudaStream_t s) {
   const int64_t ldd = copy_ld(cols);
-  const int64_t work = ceil_div64(rows * copies * (ldd / 8), 1024);
+  const int64_t work = ceil_div64(rows * copies * (ldd / 8), 256);
   const int grid = static_cast<int>(std::min<int64_t>(work, device_sm_count(current_device()) * 16)) + (prep.f ? 1 : 0);
   k_rows<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(src), ld, rows, cols, rows * copies,
                               reinterpret_cast<uint16_t*>(dst), ldd, ids, vocab, prep);

@@ -137,6 +137,7 @@ class _Structure:
         self.desc_t = _bsr_desc(t.matrix)
         self.desc_w = _bsr_desc(BlockSparseMatrix(row_ptr=w.row_ptr, col_idx=w.stored_col, blocks=w.blocks,
                                                   shape=a.shape, block_size=a.block_size))
+        self.spmm_bytes: dict[int, int] = {}  # by tokens
         self.rows_t, self.longest_t = t.matrix.nbr, t.matrix.max_row_blocks
         nbytes = ctypes.c_size_t(0)
         _lib.check(_lib.lib().kairo_bsr_sddmm_workspace_size(ctypes.byref(self.desc_w), ctypes.byref(nbytes)), "sddmm")
@@ -317,7 +318,6 @@ def sparse_gated_linear_backward(dH: Tensor, X: Tensor, weights: GatedWeights, *
         return dX, weights.blocks.new_zeros(weights.blocks.shape, dtype=dwt) if need_dw else None
     lib = _lib.lib()
     st = weights._backward_structure()
-    nbytes = ctypes.c_size_t(0)
     if need_dx:
         # the transposed weight's values are of this call alone: the structure serves calls on several streams
         blocks_t = weights.blocks.new_empty((nnzb, b, b))
@@ -326,15 +326,21 @@ def sparse_gated_linear_backward(dH: Tensor, X: Tensor, weights: GatedWeights, *
                     st.kept[2].data_ptr(), blocks_t.data_ptr(), scratch.data_ptr(), 256)
         desc_t, cfg = _with_blocks(st.desc_t, blocks_t), st.config(nnzb, n)
         dX = x.new_empty((n, k))
-        with torch.cuda.device(index):
-            _lib.check(lib.kairo_bsr_spmm_workspace_size(ctypes.byref(desc_t), _lib.LAYOUT_LINEAR, n, ctypes.byref(cfg),
-                                                         ctypes.byref(nbytes)), op)
-            if torch.cuda.is_current_stream_capturing():
-                # a graph's own: two captured graphs may replay at the same time
-                ws = x.new_empty(nbytes.value, dtype=torch.uint8)
-                ws[:_ZEROED].zero_()
-            else:
-                ws = _lib.workspace(nbytes.value, x.device)
+        size = st.spmm_bytes.get(n)
+        if size is None:
+            nbytes = ctypes.c_size_t(0)
+            with torch.cuda.device(index):
+                _lib.check(lib.kairo_bsr_spmm_workspace_size(ctypes.byref(desc_t), _lib.LAYOUT_LINEAR, n,
+                                                             ctypes.byref(cfg), ctypes.byref(nbytes)), op)
+            size = nbytes.value
+            if len(st.spmm_bytes) < 4096:
+                st.spmm_bytes[n] = size
+        if torch.cuda.is_current_stream_capturing():
+            # a graph's own: two captured graphs may replay at the same time
+            ws = x.new_empty(size, dtype=torch.uint8)
+            ws[:_ZEROED].zero_()
+        else:
+            ws = _lib.workspace(size, x.device)
         if check:
             _lib.take_pending_error(ws, op)
         _lib.launch(op, lib.kairo_bsr_spmm, index, ctypes.byref(desc_t), dp.data_ptr(), dp.shape[1],
