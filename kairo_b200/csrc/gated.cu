@@ -19,8 +19,13 @@
 // block-row: an entry is one tcgen05.mma (cta_group::2) per 16 k and 256 tokens with
 // M = 256 tokens and N = 2 * BM outputs; the even CTA's shared memory holds
 // the gate block, the odd one's the up block, and each holds its own tokens'
-// panels of X.  With blocks of 64 an entry costs a CTA 32 KB of X and 8 KB of weights for
-// 512 tensor cycles, 80 bytes a cycle (two separate products: 160).
+// panels of X.  With blocks of 64 an entry costs a CTA 32 KB of X and 8 KB of weights (two
+// separate products: 80 KB) and 8 products of 72 cycles.  Bound by the copies out of L2:
+// 8192 tokens, 8192 -> 32768 at 20 % of shared blocks, moves 17 GB into the SMs and takes 1.6 ms, 1100
+// TFLOP/s; 1.25 ms is what the copies alone need (13.7 TB/s, this GPU's rate for
+// gathers of panels), 0.95 the products alone.  Measured and not kept: tiles of
+// 256 tokens (1.95 ms), blocks brought into L2 ahead (1.65), one 32 KB copy of a
+// panel instead of four (1.61), other groups of token tiles (1.6 to 1.85).
 //
 // k_gated_stream (9 to 64 tokens of many block-rows).  A warp brings blocks and panels of X into a ring in shared
 // memory with the copy engine, four more multiply them (mma.sync), each CTA whole block-rows.
@@ -29,6 +34,8 @@
 // rows of a block-row, its warps share out the entries; mma.sync fragments come
 // straight from global memory, 16 bytes a lane (the order of k inside a block is
 // free as long as both operands agree), and the warps' sums meet in shared memory.
+// One token, 8192 -> 32768 at 20 %: 41 us, 5.2 TB/s.  A persistent form that asks
+// for the next rows' operands before it joins the sums took 43.
 #include <algorithm>
 
 #include "convert.cuh"

@@ -13,14 +13,18 @@
 // 2) and picks the target's logit as it goes by, so 8 bytes leave the SM per
 // token and 128 columns.  k_lse joins them.  Up to 128 tokens the two operands change
 // places: the table, all there is to read, fills whole tiles, and the products
-// cost half (and draw less power, which the clock shows: 64 tokens of 131072 x
-// 4096 take 265 us with tiles of 256 tokens when calls follow one another).
+// cost half and draw less power, which the clock shows (64 tokens of 131072 x
+// 4096 took 270 us with tiles of 256 tokens when calls followed one another, and 200 from a cool start).
 //
 // Backward: pieces of the vocabulary, as many columns as keep a 16-bit G of
 // all tokens within kPieceBytes.  Per piece the logits are formed again and
 // leave as G; dX += G W_piece and dW_piece = G^T X read it as it lies.  That is
 // 8 tokens * vocab * dim operations for the 6 that logits kept in memory would
 // need; it keeps 2 * tokens bytes a column of the piece instead of 4 * tokens * vocab.
+//
+// Measured.  8192 tokens, 131072 x 2048, bf16: the forward pass 3.3 ms (1340 TFLOP/s), G 4.0, dX 3.1, dW 3.0
+// (1465): 14 ms, 1260 TFLOP/s of what is done, where the power limit leaves cuBLAS 1355.  One to 64 tokens
+// of 131072 x 4096: 185 to 190 us, 5.6 to 5.8 TB/s.
 //
 // Rounding.  z, the maxima, sums and lse are fp32.  G is rounded once to the
 // operands' 16 bits, as an operand of both products must be: relative to each
