@@ -321,6 +321,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 // Tensor map of one operand: K-major `rows` x `k`, or MN-major `k` x `rows` (rows of the tile along x).
 inline kairo_status pair_operand_map(CUtensorMap* map, const void* base, kairo_dtype dt, bool mn, int64_t rows,
                                      int64_t k, int64_t ld, const char* what, int box_rows = kPairBoxRows) {
+  if ((mn ? k : rows) <= 1) ld = static_cast<int64_t>(align_up(static_cast<size_t>(mn ? rows : k), 8));  // one row: any pitch
   const CUtensorMapDataType t = dt == KAIRO_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   return mn ? make_map_2d(map, base, t, 2, static_cast<uint64_t>(rows), static_cast<uint64_t>(k),
                           static_cast<uint64_t>(ld), 64, kPairK, what)

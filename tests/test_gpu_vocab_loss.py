@@ -100,6 +100,12 @@ def test_sizes(tokens, vocab, dim, dtype):
     run_case(tokens, vocab, dim, dtype)
 
 
+@pytest.mark.parametrize("tokens,vocab,dim", [(40, 1, 1001), (200, 1, 33), (1, 1, 5), (1, 300, 1001), (200, 2, 999)])
+def test_single_rows(tokens, vocab, dim):
+    """A table or a batch of one row whose width is no multiple of 8."""
+    run_case(tokens, vocab, dim, torch.bfloat16, pad=0.0)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
 @pytest.mark.parametrize("scale", [1.0, -0.7, 3.0, 0.0])
