@@ -840,7 +840,8 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
         if (lane == 0) ptx::mbar_arrive(&empty[sidx]);
         advance();
       }
-      if (!alive) break;
+      // where the warps meet at barriers below, they leave together
+      if (GROUPS > 1 ? epi_any(!alive) : !alive) break;
       if constexpr (GROUPS > 1) {
         // the groups' sums meet in shared memory; group 0 carries on with the total
         constexpr int PITCH = NT * 8 + 1;
