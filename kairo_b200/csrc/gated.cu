@@ -72,11 +72,12 @@ __device__ __forceinline__ float activate(int act, float g, float& slope) {
     // 0.5 * (1 + tanh(y)) = sigmoid(2 y), which keeps its digits for negative g
     const float c2 = 1.5957691216057308f;  // 2 * sqrt(2 / pi)
     const float s = sigmoid(c2 * (g + 0.044715f * g * g * g));
-    if (GRAD) slope = s + g * s * (1.f - s) * c2 * (1.f + 0.134145f * g * g);
+    const float t = s * (1.f - s);  // 0 from some |g| on, where g * g may be infinite
+    if (GRAD) slope = s + (t == 0.f ? 0.f : g * t * c2 * (1.f + 0.134145f * g * g));
     return g * s;
   }
-  if (GRAD) slope = g > 0.f ? 1.f : 0.f;
-  return fmaxf(g, 0.f);
+  if (GRAD) slope = g <= 0.f ? 0.f : 1.f;
+  return g <= 0.f ? 0.f : g;  // a NaN stays one
 }
 
 struct GatedArgs {
