@@ -21,10 +21,12 @@
 // the next segment runs in the other half of TMEM.  A segment of 256 k takes 2048
 // tensor cycles and its addition some 600 of the epilogue's.
 //
-// Roles (320 threads, one CTA per SM, persistent): warp 0 loads, warp 1
-// allocates TMEM and (in the leader) issues the MMAs, warps 2..9 are the
+// Roles (384 threads, one CTA per SM, persistent): warp 0 loads, warp 1
+// allocates TMEM and (in the leader) issues the MMAs, warps 4..11 are the
 // epilogue: two warps share each quarter of the lanes and take 128 columns
-// each.  Every wait on a barrier is bounded (ptx::wait_parity).
+// each.  The 128 sums leave no room in the 168 registers that every thread
+// starts with, so tiles of 256 columns move registers from the first four warps
+// to the others.  Every wait on a barrier is bounded (ptx::wait_parity).
 #pragma once
 
 #include <cuda.h>
@@ -38,8 +40,12 @@
 namespace kairo {
 namespace {
 
-constexpr int kPairThreads = 320;
+constexpr int kPairThreads = 384;
 constexpr int kPairEpiWarps = 8;
+constexpr int kPairEpiFirst = 4;  // the first of them
+// Registers a thread after the launch: of warps 0..3 and of the epilogue's (tiles of 256 columns)
+constexpr int kPairRegsLow = 72, kPairRegsHigh = 208;
+constexpr int kPairRegsAll = 32 * (kPairEpiFirst * kPairRegsLow + kPairEpiWarps * kPairRegsHigh);
 constexpr int kPairTileM = 256;      // rows of a cluster's tile (128 a CTA)
 constexpr int kPairTileN = 256;
 constexpr int kPairK = 64;           // k of one stage
@@ -70,18 +76,24 @@ struct PairTile {
 };
 
 __device__ __forceinline__ PairTile pair_tile(const PairShape& s, int t) {
+  // divisions, the 64-bit ones above all, cost more than a short tile's products
   PairTile o;
-  const int all = s.tiles_m * s.tiles_n;
-  o.split = t / all;
-  t -= o.split * all;
+  o.split = 0;
+  o.k0 = 0;
+  o.k1 = s.ksteps;
+  if (s.splits > 1) {
+    const int all = s.tiles_m * s.tiles_n;
+    o.split = t / all;
+    t -= o.split * all;
+    o.k0 = static_cast<int>(static_cast<int64_t>(s.ksteps) * o.split / s.splits);
+    o.k1 = static_cast<int>(static_cast<int64_t>(s.ksteps) * (o.split + 1) / s.splits);
+  }
   const int per = s.group_m * s.tiles_n;
   const int g = t / per, r = t - g * per;
   const int m0 = g * s.group_m;
   const int gm = min(s.group_m, s.tiles_m - m0);
   o.nt = r / gm;
   o.mt = m0 + (r - o.nt * gm);
-  o.k0 = static_cast<int>(static_cast<int64_t>(s.ksteps) * o.split / s.splits);
-  o.k1 = static_cast<int>(static_cast<int64_t>(s.ksteps) * (o.split + 1) / s.splits);
   return o;
 }
 
@@ -96,7 +108,7 @@ __device__ __forceinline__ PairTile pair_tile(const PairShape& s, int t) {
 template <int IN_FMT, bool A_MN, bool B_MN, class Epi, int TN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     k_pair_gemm(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
-                const PairShape shape, unsigned* err, const typename Epi::Args eargs) {
+                const PairShape shape, unsigned* err, const __grid_constant__ typename Epi::Args eargs) {
   constexpr int ST = pair_stages(TN);
   constexpr int STAGE = pair_stage_bytes(TN);
   static_assert(TN == 256 || ((TN == 64 || TN == 128) && !B_MN), "columns of a tile");
@@ -154,110 +166,115 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   const int ntiles = shape.tiles_m * shape.tiles_n * shape.splits;
   const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ loads
-    const bool is_a = lane < NA;
-    const uint64_t pol = ptx::policy_evict_last();
-    const int box = is_a ? lane : lane - NA;
-    const void* map = is_a ? static_cast<const void*>(&tmap_a) : static_cast<const void*>(&tmap_b);
-    const uint32_t mine = lane < NA + NB ? 1u : 0u;
-    const bool mn = is_a ? A_MN : B_MN;
-    const uint32_t dst_off = (is_a ? 0u : kPairHalf) + static_cast<uint32_t>(mine ? box : 0) * (kPairBoxRows * kPairK * 2);
-    const int shift = is_a ? 0 : first % shape.copies * shape.copy_rows;
-    int sidx = 0;
-    uint32_t sph = 0;
-    bool alive = true;
-    for (int t = first; t < ntiles && alive; t += step) {
-      const PairTile pt = pair_tile(shape, t);
-      const int r0 = (is_a ? pt.mt * 256 + static_cast<int>(rank) * 128 : pt.nt * TN + static_cast<int>(rank) * (TN / 2)) +
-                     box * kPairBoxRows + shift;
-      for (int k = pt.k0; k < pt.k1; ++k) {
-        int ok = ptx::wait_parity(&empty[sidx], sph ^ 1u, abort_flag, err, kTagEmpty, kWaitCycles);
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        if (!ok) {
-          alive = false;
-          break;
-        }
-        const uint32_t bar = ptx::peer_smem_u32(&full[sidx], 0);
-        if (rank == 0) {
-          if (lane == 0) issued[sidx] = static_cast<int>(sph) + 1;
-          ptx::mbar_expect_tx_if(lane == 0 ? 1u : 0u, &full[sidx], 2 * STAGE);
-        }
-        ptx::tma_load_2d_pair_if(mine, smem + sidx * STAGE + dst_off, map, mn ? r0 : k * kPairK,
-                                 mn ? k * kPairK : r0, bar, pol);
-        __syncwarp();
-        if (rank == 0) ptx::mbar_arrive_if(lane == 0 ? 1u : 0u, &full[sidx]);
-        if (++sidx == ST) {
-          sidx = 0;
-          sph ^= 1u;
-        }
-      }
-    }
-  } else if (warp == 1 && rank == 0) {
-    // ------------------------------------------------------------ MMA issuer
-    const uint32_t leader = lane == 0 ? 1u : 0u;
-    const uint32_t sbase = ptx::smem_u32(smem);
-    const uint64_t adesc = A_MN ? ptx::make_smem_desc(sbase, kPairBoxRows * kPairK * 2, 1024, 2u)
-                                : ptx::make_smem_desc(sbase, 16, 1024, 2u);
-    const uint64_t bdesc = B_MN ? ptx::make_smem_desc(sbase + kPairHalf, kPairBoxRows * kPairK * 2, 1024, 2u)
-                                : ptx::make_smem_desc(sbase + kPairHalf, 16, 1024, 2u);
-    const uint32_t a_lo = static_cast<uint32_t>(adesc), a_hi = static_cast<uint32_t>(adesc >> 32);
-    const uint32_t b_lo = static_cast<uint32_t>(bdesc), b_hi = static_cast<uint32_t>(bdesc >> 32);
-    // 16 k further: 32 bytes along a 128-byte row, or 16 rows of 128 bytes
-    constexpr uint32_t AK = (A_MN ? 2048 : 32) >> 4, BK = (B_MN ? 2048 : 32) >> 4;
-    int sidx = 0, slot = 0;
-    uint32_t sph = 0, aphase = 0;
-    bool alive = true;
-    for (int t = first; t < ntiles && alive; t += step) {
-      const PairTile pt = pair_tile(shape, t);
-      for (int k0 = pt.k0; k0 < pt.k1; k0 += shape.seg) {
-        int ok = ptx::wait_parity(&tempty[slot], aphase ^ 1u, abort_flag, err, kTagTmemEmpty, kWaitCycles);
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        if (!ok) {
-          alive = false;
-          break;
-        }
-        ptx::tc_fence_after();
-        const uint32_t d = tmem_base + static_cast<uint32_t>(slot * TN);
-        const int k1 = min(pt.k1, k0 + shape.seg);
-        for (int k = k0; k < k1; ++k) {
-          ok = ptx::wait_parity(&full[sidx], sph, abort_flag, err, kTagFull, kWaitCycles);
+  if (warp < kPairEpiFirst) {
+    if constexpr (TN == 256) ptx::registers_down<kPairRegsLow>();
+    if (warp == 0) {
+      // ------------------------------------------------------------ loads
+      const bool is_a = lane < NA;
+      const uint64_t pol = ptx::policy_evict_last();
+      const int box = is_a ? lane : lane - NA;
+      const void* map = is_a ? static_cast<const void*>(&tmap_a) : static_cast<const void*>(&tmap_b);
+      const uint32_t mine = lane < NA + NB ? 1u : 0u;
+      const bool mn = is_a ? A_MN : B_MN;
+      const uint32_t dst_off =
+          (is_a ? 0u : kPairHalf) + static_cast<uint32_t>(mine ? box : 0) * (kPairBoxRows * kPairK * 2);
+      const int shift = is_a ? 0 : first % shape.copies * shape.copy_rows;
+      int sidx = 0;
+      uint32_t sph = 0;
+      bool alive = true;
+      for (int t = first; t < ntiles && alive; t += step) {
+        const PairTile pt = pair_tile(shape, t);
+        const int tile0 = is_a ? pt.mt * 256 + static_cast<int>(rank) * 128 : pt.nt * TN + static_cast<int>(rank) * (TN / 2);
+        const int r0 = tile0 + box * kPairBoxRows + shift;
+        for (int k = pt.k0; k < pt.k1; ++k) {
+          int ok = ptx::wait_parity(&empty[sidx], sph ^ 1u, abort_flag, err, kTagEmpty, kWaitCycles);
           ok = __shfl_sync(0xffffffffu, ok, 0);
           if (!ok) {
             alive = false;
             break;
           }
-          const uint32_t s16 = static_cast<uint32_t>(sidx * STAGE) >> 4;
-#pragma unroll
-          for (int kk = 0; kk < kPairK / 16; ++kk)
-            ptx::mma_f16_ss_pair_if(leader, d, a_lo + s16 + kk * AK, a_hi, b_lo + s16 + kk * BK, b_hi, IDESC,
-                                    (k > k0 || kk > 0) ? 1u : 0u);
-          ptx::mma_commit_pair_if(leader, &empty[sidx]);
+          const uint32_t bar = ptx::peer_smem_u32(&full[sidx], 0);
+          if (rank == 0) {
+            if (lane == 0) issued[sidx] = static_cast<int>(sph) + 1;
+            ptx::mbar_expect_tx_if(lane == 0 ? 1u : 0u, &full[sidx], 2 * STAGE);
+          }
+          ptx::tma_load_2d_pair_if(mine, smem + sidx * STAGE + dst_off, map, mn ? r0 : k * kPairK,
+                                   mn ? k * kPairK : r0, bar, pol);
+          __syncwarp();
+          if (rank == 0) ptx::mbar_arrive_if(lane == 0 ? 1u : 0u, &full[sidx]);
           if (++sidx == ST) {
             sidx = 0;
             sph ^= 1u;
           }
         }
-        if (!alive) break;
-        ptx::mma_commit_pair_if(leader, &tfull[slot]);
-        slot ^= 1;
-        if (slot == 0) aphase ^= 1u;
       }
+    } else if (warp == 1 && rank == 0) {
+      // ------------------------------------------------------------ MMA issuer
+      const uint32_t leader = lane == 0 ? 1u : 0u;
+      const uint32_t sbase = ptx::smem_u32(smem);
+      const uint64_t adesc = A_MN ? ptx::make_smem_desc(sbase, kPairBoxRows * kPairK * 2, 1024, 2u)
+                                  : ptx::make_smem_desc(sbase, 16, 1024, 2u);
+      const uint64_t bdesc = B_MN ? ptx::make_smem_desc(sbase + kPairHalf, kPairBoxRows * kPairK * 2, 1024, 2u)
+                                  : ptx::make_smem_desc(sbase + kPairHalf, 16, 1024, 2u);
+      const uint32_t a_lo = static_cast<uint32_t>(adesc), a_hi = static_cast<uint32_t>(adesc >> 32);
+      const uint32_t b_lo = static_cast<uint32_t>(bdesc), b_hi = static_cast<uint32_t>(bdesc >> 32);
+      // 16 k further: 32 bytes along a 128-byte row, or 16 rows of 128 bytes
+      constexpr uint32_t AK = (A_MN ? 2048 : 32) >> 4, BK = (B_MN ? 2048 : 32) >> 4;
+      int sidx = 0, slot = 0;
+      uint32_t sph = 0, aphase = 0;
+      bool alive = true;
+      for (int t = first; t < ntiles && alive; t += step) {
+        const PairTile pt = pair_tile(shape, t);
+        for (int k0 = pt.k0; k0 < pt.k1; k0 += shape.seg) {
+          int ok = ptx::wait_parity(&tempty[slot], aphase ^ 1u, abort_flag, err, kTagTmemEmpty, kWaitCycles);
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+          if (!ok) {
+            alive = false;
+            break;
+          }
+          ptx::tc_fence_after();
+          const uint32_t d = tmem_base + static_cast<uint32_t>(slot * TN);
+          const int k1 = min(pt.k1, k0 + shape.seg);
+          for (int k = k0; k < k1; ++k) {
+            ok = ptx::wait_parity(&full[sidx], sph, abort_flag, err, kTagFull, kWaitCycles);
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            if (!ok) {
+              alive = false;
+              break;
+            }
+            const uint32_t s16 = static_cast<uint32_t>(sidx * STAGE) >> 4;
+#pragma unroll
+            for (int kk = 0; kk < kPairK / 16; ++kk)
+              ptx::mma_f16_ss_pair_if(leader, d, a_lo + s16 + kk * AK, a_hi, b_lo + s16 + kk * BK, b_hi, IDESC,
+                                      (k > k0 || kk > 0) ? 1u : 0u);
+            ptx::mma_commit_pair_if(leader, &empty[sidx]);
+            if (++sidx == ST) {
+              sidx = 0;
+              sph ^= 1u;
+            }
+          }
+          if (!alive) break;
+          ptx::mma_commit_pair_if(leader, &tfull[slot]);
+          slot ^= 1;
+          if (slot == 0) aphase ^= 1u;
+        }
+      }
+      ptx::mma_commit_pair_if(leader, mma_done);
+      int dummy = 0;
+      ptx::wait_parity(mma_done, 0, reinterpret_cast<volatile int*>(&dummy), err, kTagDrain, kWaitCycles);
+      __syncwarp();
+    } else if (warp == 1) {
+      // the leader's last commit arrives here after all its earlier ones
+      int dummy = 0;
+      ptx::wait_parity(mma_done, 0, reinterpret_cast<volatile int*>(&dummy), err, kTagDrain, 4 * kWaitCycles);
+      __syncwarp();
     }
-    ptx::mma_commit_pair_if(leader, mma_done);
-    int dummy = 0;
-    ptx::wait_parity(mma_done, 0, reinterpret_cast<volatile int*>(&dummy), err, kTagDrain, kWaitCycles);
-    __syncwarp();
-  } else if (warp == 1) {
-    // the leader's last commit arrives here after all its earlier ones
-    int dummy = 0;
-    ptx::wait_parity(mma_done, 0, reinterpret_cast<volatile int*>(&dummy), err, kTagDrain, 4 * kWaitCycles);
-    __syncwarp();
-  } else if (warp >= 2) {
+  } else {
+    if constexpr (TN == 256) ptx::registers_up<kPairRegsHigh>();  // the launch checks that there are so many
     // ------------------------------------------------------------ epilogue
     const int q = warp & 3;
-    const int part = (warp - 2) >> 2;  // which kPairEpiCols columns of the tile
-    Epi epi(eargs, static_cast<int>(rank) * 128 + q * 32 + lane, part, out + (warp - 2) * kPairOutBytes);
+    const int part = (warp - kPairEpiFirst) >> 2;  // which kPairEpiCols columns of the tile
+    Epi epi(eargs, static_cast<int>(rank) * 128 + q * 32 + lane, part, out + (warp - kPairEpiFirst) * kPairOutBytes);
     const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
     int slot = 0;
     uint32_t aphase = 0;
@@ -280,12 +297,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           ptx::tmem_wait_ld();
         } else {
 #pragma unroll
-          for (int c = 0; c < COLS; c += 32) {
-            float w[32];
-            ptx::tmem_ld32(at + c, w);
+          for (int c = 0; c < COLS; c += 16) {
+            float w[16];  // 32 more beside v would not stay in registers
+            ptx::tmem_ld16(at + c, w);
             ptx::tmem_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[c + j] += w[j];
+            for (int j = 0; j < 16; ++j) v[c + j] += w[j];
           }
         }
         ptx::tc_fence_before();
@@ -341,6 +358,17 @@ kairo_status launch_pair_gemm(const CUtensorMap& a, const CUtensorMap& b, const 
   static std::atomic<uint64_t> ready{0};
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(fn), kPairSmem, &ready);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic smem)");
+  if constexpr (TN == 256) {
+    static std::atomic<int> regs{0};  // a thread's at the launch
+    if (regs.load(std::memory_order_relaxed) == 0) {
+      cudaFuncAttributes attr;
+      e = cudaFuncGetAttributes(&attr, reinterpret_cast<const void*>(fn));
+      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncGetAttributes");
+      regs.store(attr.numRegs, std::memory_order_relaxed);
+    }
+    if (regs.load(std::memory_order_relaxed) * kPairThreads < kPairRegsAll)
+      return fail(KAIRO_STATUS_NOT_SUPPORTED, "the paired product was compiled for too few registers");
+  }
   const int clusters = pair_clusters(static_cast<int64_t>(shape.tiles_m) * shape.tiles_n * shape.splits);
   fn<<<2 * clusters, kPairThreads, kPairSmem, s>>>(a, b, shape, err, args);
   e = cudaGetLastError();

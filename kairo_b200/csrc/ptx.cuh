@@ -108,6 +108,13 @@ __device__ __forceinline__ bool wait_parity(uint64_t* bar, uint32_t parity,
 // cores and bulk copies (the async proxy).
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// Registers a thread of this warpgroup (4 warps, all of which come here): fewer, or more than at the launch.  All
+// warpgroups' shares together stay within what the block was launched with, or the larger ones wait for ever.
+template <int N>
+__device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ uint64_t policy_evict_first() {
   uint64_t p;

@@ -246,33 +246,47 @@ struct FewStatsEpi {
 template <typename T>
 __device__ __forceinline__ void put_rows(uint8_t* out, const float (&v)[kPairEpiCols], T* p, int64_t ld, int rows,
                                          int cols) {
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, c = lane & 7, r0 = lane >> 3;
+  uint8_t* const mine = out + lane * 128;            // the row this lane puts down,
+  const uint8_t* const even = out + r0 * 128 + ((c ^ r0) * 16);  // and its piece of rows r0 + 8 i
+  const uint8_t* const odd = out + r0 * 128 + ((c ^ (r0 + 4)) * 16) + 512;  // and r0 + 8 i + 4
+  T* at = p + r0 * ld + 8 * c;
 #pragma unroll
   for (int h = 0; h < kPairEpiCols; h += 64) {
     if (h >= cols) return;
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
+    for (int e = 0; e < 8; ++e) {
       float w[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = v[h + 8 * c + j];
-      store_f32<T, 8>(reinterpret_cast<T*>(out + lane * 128 + ((c ^ (lane & 7)) * 16)), w);
+      for (int j = 0; j < 8; ++j) w[j] = v[h + 8 * e + j];
+      store_f32<T, 8>(reinterpret_cast<T*>(mine + ((e ^ c) * 16)), w);
     }
     __syncwarp();
-    const int c = lane & 7;
     const int n = cols - (h + 8 * c);
+    T* dst = at + h;
+    if (rows >= 32 && n >= 8) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = 4 * i + (lane >> 3);
-      if (r >= rows || n <= 0) continue;
-      const uint4 w = *reinterpret_cast<const uint4*>(out + r * 128 + ((c ^ (r & 7)) * 16));
-      T* dst = p + r * ld + h + 8 * c;
-      if (n >= 8) {
-        *reinterpret_cast<uint4*>(dst) = w;
-      } else {
-        const T* e = reinterpret_cast<const T*>(&w);
+      for (int i = 0; i < 4; ++i) {
+        const uint4 a = *reinterpret_cast<const uint4*>(even + i * 1024);
+        const uint4 b = *reinterpret_cast<const uint4*>(odd + i * 1024);
+        *reinterpret_cast<uint4*>(dst) = a;
+        dst += 4 * ld;
+        *reinterpret_cast<uint4*>(dst) = b;
+        dst += 4 * ld;
+      }
+    } else {
+#pragma unroll 1
+      for (int r = r0; r < rows; r += 4, dst += 4 * ld) {
+        if (r >= 32) break;
+        const uint4 w = *reinterpret_cast<const uint4*>(out + r * 128 + ((c ^ (r & 7)) * 16));
+        if (n >= 8) {
+          *reinterpret_cast<uint4*>(dst) = w;
+        } else {
+          const T* e = reinterpret_cast<const T*>(&w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (j < n) dst[j] = e[j];
+          for (int j = 0; j < 8; ++j)
+            if (j < n) dst[j] = e[j];
+        }
       }
     }
     __syncwarp();
@@ -282,28 +296,42 @@ __device__ __forceinline__ void put_rows(uint8_t* out, const float (&v)[kPairEpi
 // The same in fp32 (rows of p 16-byte aligned, room for whole groups of 4 columns), added to what is there unless `first`.
 __device__ __forceinline__ void sum_rows(uint8_t* out, const float (&v)[kPairEpiCols], float* p, int64_t ld, int rows,
                                          int cols, bool first) {
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, c = lane & 7, r0 = lane >> 3;
+  uint8_t* const mine = out + lane * 128;
+  const uint8_t* const even = out + r0 * 128 + ((c ^ r0) * 16);
+  const int other = 512 + ((c ^ (r0 + 4)) - (c ^ r0)) * 16;  // to the same piece four rows on
+  float* at = p + r0 * ld + 4 * c;
+  const int last = min(rows, 32);
 #pragma unroll
   for (int h = 0; h < kPairEpiCols; h += 32) {
     if (h >= cols) return;
 #pragma unroll
-    for (int c = 0; c < 8; ++c)
-      *reinterpret_cast<float4*>(out + lane * 128 + ((c ^ (lane & 7)) * 16)) =
-          make_float4(v[h + 4 * c], v[h + 4 * c + 1], v[h + 4 * c + 2], v[h + 4 * c + 3]);
+    for (int e = 0; e < 8; ++e)
+      *reinterpret_cast<float4*>(mine + ((e ^ c) * 16)) =
+          make_float4(v[h + 4 * e], v[h + 4 * e + 1], v[h + 4 * e + 2], v[h + 4 * e + 3]);
     __syncwarp();
-    const int c = lane & 7;
-    const bool in = h + 4 * c < cols;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = 4 * i + (lane >> 3);
-      if (r >= rows || !in) continue;
-      float4 w = *reinterpret_cast<const float4*>(out + r * 128 + ((c ^ (r & 7)) * 16));
-      float4* dst = reinterpret_cast<float4*>(p + r * ld + h + 4 * c);
-      if (!first) {
-        const float4 o = *dst;
-        w = make_float4(w.x + o.x, w.y + o.y, w.z + o.z, w.w + o.w);
+    if (h + 4 * c < cols) {
+      float* dst = at + h;
+      const uint8_t* src = even;
+#pragma unroll 1  // unrolled, its addresses do not stay in registers beside v
+      for (int r = r0; r < last; r += 8, src += 1024) {
+        float4 w = *reinterpret_cast<const float4*>(src);
+        float4 u = *reinterpret_cast<const float4*>(src + other);
+        float4* const to = reinterpret_cast<float4*>(dst);
+        float4* const next = reinterpret_cast<float4*>(dst + 4 * ld);
+        const bool two = r + 4 < last;
+        if (!first) {
+          const float4 o = *to;
+          w = make_float4(w.x + o.x, w.y + o.y, w.z + o.z, w.w + o.w);
+          if (two) {
+            const float4 n = *next;
+            u = make_float4(u.x + n.x, u.y + n.y, u.z + n.z, u.w + n.w);
+          }
+        }
+        *to = w;
+        if (two) *next = u;
+        dst += 8 * ld;
       }
-      *dst = w;
     }
     __syncwarp();
   }
