@@ -27,8 +27,10 @@
 // 256 tokens (1.95 ms), blocks brought into L2 ahead (1.65), one 32 KB copy of a
 // panel instead of four (1.61), other groups of token tiles (1.6 to 1.85).
 //
-// k_gated_stream (9 to 64 tokens of many block-rows).  A warp brings blocks and panels of X into a ring in shared
-// memory with the copy engine, four more multiply them (mma.sync), each CTA whole block-rows.
+// k_gated_short (33 to 128 tokens; from 17 on where blocks of 64 have many rows).  The same with one CTA a block-row and
+// two CTAs an SM: a pair would multiply and fill panels of 256 tokens, and has half as many places to share the
+// block-rows out to.  128 tokens, 4096 -> 14336 at 20 %: 27 us (k_gated 47), 64 tokens, 8192 -> 32768: 61 us, where the
+// blocks alone are 33 and the L2 hands each block-row the panels of its columns.
 //
 // k_gated_few (up to 32 tokens).  Bound by reading the blocks once.  A CTA takes 16
 // rows of a block-row, its warps share out the entries; mma.sync fragments come
@@ -450,6 +452,253 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGatedThreads, 1)
   }
 }
 
+// ------------------------------------------------------------ up to 128 tokens on the tensor cores
+
+constexpr int kShortThreads = 192;
+constexpr int kShortEpiWarps = 4;
+constexpr int kShortTokens = 128;
+constexpr int short_slot_bytes(int bm) { return kShortTokens * bm * 2 + 2 * bm * bm * 2; }  // X, gate, up
+constexpr int short_stage_bytes(int bm) { return gated_group(bm) * short_slot_bytes(bm); }
+constexpr int short_stages(int bm) { return 100 * 1024 / short_stage_bytes(bm); }
+constexpr size_t short_smem(int bm) { return static_cast<size_t>(short_stages(bm)) * short_stage_bytes(bm) + 2048; }
+static_assert(2 * (short_smem(64) + 1024) <= 228 * 1024 && 2 * (short_smem(32) + 1024) <= 228 * 1024 &&
+                  2 * (short_smem(16) + 1024) <= 228 * 1024,
+              "two CTAs of an SM");
+
+// k_gated with one CTA for all tokens of a block-row: M = 128 tokens (64 of them copied where there are no more), N = 2 * BM
+// outputs, the gate block's rows followed by the up block's.
+template <int BM, int IN_FMT, typename TT, bool GRAD>
+__global__ void __launch_bounds__(kShortThreads, 2)
+    k_gated_short(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
+                  const GatedArgs args) {
+  constexpr int ST = short_stages(BM);
+  constexpr int E = gated_group(BM);
+  constexpr int SLOT = short_slot_bytes(BM);
+  constexpr int STAGE = short_stage_bytes(BM);
+  constexpr int PANEL = kShortTokens * BM * 2;
+  constexpr uint32_t IDESC = ptx::make_idesc_f16(IN_FMT, 0u, 0u, kShortTokens, 2 * BM);
+  constexpr uint32_t SW = ptx::swizzle_code_for_row_bytes(BM * 2);
+  constexpr uint32_t ACC = 2 * BM;
+  constexpr uint32_t TMEM_COLS = 2 * ACC;
+  static_assert(SLOT % 1024 == 0 && PANEL % 1024 == 0 && TMEM_COLS >= 32 && TMEM_COLS <= 256, "layout");
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + ST * STAGE);
+  uint64_t* empty = full + ST;
+  uint64_t* tfull = empty + ST;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* mma_done = tempty + 2;
+  int* misc = reinterpret_cast<int*>(mma_done + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc);
+  volatile int* abort_flag = misc + 1;
+  int* issued = misc + 4;  // [ST]: parity + 1 of the last load into each stage
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      ptx::mbar_init(&full[s], 1);
+      ptx::mbar_init(&empty[s], 1);
+      issued[s] = 0;
+    }
+    for (int k = 0; k < 2; ++k) {
+      ptx::mbar_init(&tfull[k], 1);
+      ptx::mbar_init(&tempty[k], kShortEpiWarps);
+    }
+    ptx::mbar_init(mma_done, 1);
+    misc[1] = 0;
+    ptx::mbar_init_fence();
+  }
+  if (warp == 0 && lane == 0) {
+    ptx::prefetch_tmap(&tmap_x);
+    ptx::prefetch_tmap(&tmap_w);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(tmem_slot, TMEM_COLS);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  // entries of a block-row; offsets outside them are clamped by every role alike
+  auto first_of = [&](int row) { return min(max(__ldg(args.ent_ptr + row), 0), args.nentries); };
+  auto end_of = [&](int row, int e0) { return min(max(__ldg(args.ent_ptr + row + 1), e0), args.nentries); };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ loads
+    const uint64_t pol_w = ptx::policy_evict_first();
+    const uint64_t pol_x = ptx::policy_evict_last();
+    constexpr int BOXES = 4;  // two of 64 tokens, the gate block, the up block
+    const int xboxes = args.n > 64 ? 2 : 1;
+    const int e = lane / BOXES, part = lane - e * BOXES;
+    const bool is_w = part >= 2;
+    const uint32_t bytes = static_cast<uint32_t>(xboxes * 64 * BM * 2 + 2 * BM * BM * 2);  // of an entry
+    const uint32_t dst_off =
+        static_cast<uint32_t>((e < E ? e : 0) * SLOT + (is_w ? PANEL + (part - 2) * BM * BM * 2 : part * 64 * BM * 2));
+    const void* map = is_w ? static_cast<const void*>(&tmap_w) : static_cast<const void*>(&tmap_x);
+    const uint64_t pol = is_w ? pol_w : pol_x;
+    int sidx = 0;
+    uint32_t sph = 0;
+    bool alive = true;
+    for (int row = blockIdx.x; row < args.nbr && alive; row += gridDim.x) {
+      const int e0 = first_of(row), cnt = end_of(row, e0) - e0;
+      for (int at = 0; at < cnt && alive; at += 32) {
+        const int4 w = at + lane < cnt ? __ldg(args.entries + e0 + at + lane) : make_int4(0, -1, -1, 0);
+        int col = w.x, gate = w.y, up = w.z;
+        if (at + lane < cnt && (static_cast<unsigned>(col) >= static_cast<unsigned>(args.nbc) || gate < -1 ||
+                                gate >= args.nblocks || up < -1 || up >= args.nblocks)) {
+          atomicCAS(args.err, 0u, KAIRO_DEVERR_BAD_INDEX);
+          col = 0;
+          gate = up = -1;
+        }
+        if (gate < 0) gate = args.nblocks;  // behind the storage: zeros
+        if (up < 0) up = args.nblocks;
+        for (int b0 = 0; b0 < 32 && at + b0 < cnt; b0 += E) {
+          const int take = min(E, cnt - at - b0);
+          int ok = ptx::wait_parity(&empty[sidx], sph ^ 1u, abort_flag, args.err, kTagEmpty, kWaitCycles);
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+          if (!ok) {
+            alive = false;
+            break;
+          }
+          if (lane == 0) issued[sidx] = static_cast<int>(sph) + 1;
+          ptx::mbar_expect_tx_if(lane == 0 ? 1u : 0u, &full[sidx], bytes * static_cast<uint32_t>(take));
+          __syncwarp();
+          const uint32_t mine = e < take && (is_w || part < xboxes) ? 1u : 0u;
+          const int src = (b0 + e) & 31;
+          const int ecol = __shfl_sync(0xffffffffu, col, src);
+          const int egate = __shfl_sync(0xffffffffu, gate, src);
+          const int eup = __shfl_sync(0xffffffffu, up, src);
+          ptx::tma_load_2d_if(mine, smem + sidx * STAGE + dst_off, map, is_w ? 0 : ecol * BM,
+                              is_w ? (part == 2 ? egate : eup) * BM : part * 64, &full[sidx], pol);
+          __syncwarp();
+          ptx::mbar_arrive_if(lane == 0 ? 1u : 0u, &full[sidx]);
+          if (++sidx == ST) {
+            sidx = 0;
+            sph ^= 1u;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    const uint32_t leader = lane == 0 ? 1u : 0u;
+    const uint32_t sbase = ptx::smem_u32(smem);
+    const uint64_t adesc = ptx::make_smem_desc(sbase, 16, 8 * BM * 2, SW);
+    const uint64_t bdesc = ptx::make_smem_desc(sbase + PANEL, 16, 8 * BM * 2, SW);
+    const uint32_t a_lo = static_cast<uint32_t>(adesc), a_hi = static_cast<uint32_t>(adesc >> 32);
+    const uint32_t b_lo = static_cast<uint32_t>(bdesc), b_hi = static_cast<uint32_t>(bdesc >> 32);
+    int sidx = 0, slot = 0;
+    uint32_t sph = 0, aphase = 0;
+    bool alive = true;
+    for (int row = blockIdx.x; row < args.nbr && alive; row += gridDim.x) {
+      const int e0 = first_of(row), cnt = end_of(row, e0) - e0;
+      if (cnt == 0) continue;
+      int ok = ptx::wait_parity(&tempty[slot], aphase ^ 1u, abort_flag, args.err, kTagTmemEmpty, kWaitCycles);
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok) break;
+      ptx::tc_fence_after();
+      const uint32_t d = tmem_base + static_cast<uint32_t>(slot) * ACC;
+      for (int at = 0; at < cnt; at += E) {
+        ok = ptx::wait_parity(&full[sidx], sph, abort_flag, args.err, kTagFull, kWaitCycles);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) {
+          alive = false;
+          break;
+        }
+        ptx::tc_fence_after();
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          if (at + e >= cnt) break;
+          const uint32_t s16 = static_cast<uint32_t>(sidx * STAGE + e * SLOT) >> 4;
+#pragma unroll
+          for (int kk = 0; kk < BM / 16; ++kk)
+            ptx::mma_f16_ss_if(leader, d, a_lo + s16 + ((kk * 32) >> 4), a_hi, b_lo + s16 + ((kk * 32) >> 4), b_hi, IDESC,
+                               (at > 0 || e > 0 || kk > 0) ? 1u : 0u);
+        }
+        ptx::mma_commit_if(leader, &empty[sidx]);
+        if (++sidx == ST) {
+          sidx = 0;
+          sph ^= 1u;
+        }
+      }
+      if (!alive) break;
+      ptx::mma_commit_if(leader, &tfull[slot]);
+      slot ^= 1;
+      if (slot == 0) aphase ^= 1u;
+    }
+    ptx::mma_commit_if(leader, mma_done);
+    int dummy = 0;
+    ptx::wait_parity(mma_done, 0, reinterpret_cast<volatile int*>(&dummy), args.err, kTagDrain, kWaitCycles);
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ epilogue
+    constexpr int UN = BM < 32 ? BM : 32;  // outputs of one step
+    const int q = warp & 3;
+    const int token = q * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
+    int slot = 0;
+    uint32_t aphase = 0;
+    for (int row = blockIdx.x; row < args.nbr; row += gridDim.x) {
+      const int e0 = first_of(row);
+      const bool some = end_of(row, e0) > e0;
+      if (some) {
+        int ok = ptx::wait_parity(&tfull[slot], aphase, abort_flag, args.err, kTagTmemFull, kWaitCycles);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+        ptx::tc_fence_after();
+      }
+      const uint32_t at = tmem_base + lane_addr + static_cast<uint32_t>(slot) * ACC;
+      if (q * 32 < args.n) {
+#pragma unroll 1
+        for (int c0 = 0; c0 < BM; c0 += UN) {
+          float g[UN], u[UN];
+          if (some) {
+            if constexpr (UN == 32) {
+              ptx::tmem_ld32(at + static_cast<uint32_t>(c0), g);
+              ptx::tmem_ld32(at + static_cast<uint32_t>(BM + c0), u);
+            } else {
+              ptx::tmem_ld16(at + static_cast<uint32_t>(c0), g);
+              ptx::tmem_ld16(at + static_cast<uint32_t>(BM + c0), u);
+            }
+            ptx::tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int j = 0; j < UN; ++j) g[j] = u[j] = 0.f;
+          }
+          if (token < args.n) gated_out<TT, GRAD, UN>(args, token, row, BM, c0, g, u);
+          __syncwarp();
+        }
+      }
+      if (some) {
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&tempty[slot]);
+        slot ^= 1;
+        if (slot == 0) aphase ^= 1u;
+      }
+    }
+  }
+
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag) {
+    // copies that were issued land before shared memory is given up
+    int dummy = 0;
+    for (int s = 0; s < ST; ++s)
+      if (issued[s])
+        ptx::wait_parity(&full[s], static_cast<uint32_t>(issued[s] - 1), reinterpret_cast<volatile int*>(&dummy),
+                         args.err, kTagDrain, kWaitCycles);
+  }
+  __syncthreads();
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
 // ------------------------------------------------------------ few tokens
 
 template <typename T>
@@ -624,282 +873,11 @@ __global__ void __launch_bounds__(32 * kFewWarps, NT == 1 ? 3 : 2) k_gated_few(c
   }
 }
 
-// ------------------------------------------------------------ blocks streamed for a batch of tokens
-
-constexpr int kStreamThreads = 160;  // four warps that multiply, one that loads
-constexpr int kStreamSmem = 110 * 1024;  // two CTAs an SM
-
-// Both blocks and the panel of X: multiples of the swizzle's period (256, 512, 1024 bytes) all three.
-constexpr int stream_entry_bytes(int bm, int nt) { return 2 * bm * bm * 2 + nt * 8 * bm * 2; }
-// Entries of one stage (a power of two): up to 16 KB of blocks and about 20 KB in all, and four lanes
-// each, so that one instruction issues a stage's copies (one lane's copies go out one after the other,
-// some 450 cycles each).
-constexpr int stream_group(int bm, int nt) {
-  int e = 1;
-  while (e < 8 && 2 * e * bm * bm <= 4096 && 2 * e * stream_entry_bytes(bm, nt) <= 20 * 1024) e *= 2;
-  return e;
-}
-constexpr int stream_stage_bytes(int bm, int nt) { return stream_group(bm, nt) * stream_entry_bytes(bm, nt); }
-constexpr int stream_sums_bytes(int bm, int nt) { return bm == 64 ? 0 : 4 * 2 * 16 * (nt * 8 + 1) * 4; }
-constexpr int stream_stages(int bm, int nt) {
-  return (kStreamSmem - 2048 - stream_sums_bytes(bm, nt)) / stream_stage_bytes(bm, nt);
-}
-
-__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
-__device__ __forceinline__ void ldmatrix2(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr));
-}
-
-// Byte offset of 16-byte chunk c of row r in a box of BM columns, as the copy engine's swizzle lays it out.
-template <int BM>
-__device__ __forceinline__ uint32_t box_at(int r, int c) {
-  const int x = BM == 64 ? (r & 7) : BM == 32 ? ((r >> 1) & 3) : ((r >> 2) & 1);
-  return static_cast<uint32_t>(r * BM * 2 + ((c ^ x) * 16));
-}
-
-// NT * 8 tokens; persistent, a CTA takes whole block-rows.
-template <int BM, int NT, typename TT, bool GRAD>
-__global__ void __launch_bounds__(kStreamThreads, 2)
-    k_gated_stream(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
-                   const GatedArgs args) {
-  constexpr int ST = stream_stages(BM, NT);
-  constexpr int E = stream_group(BM, NT);
-  constexpr int ENTRY = stream_entry_bytes(BM, NT), STAGE = stream_stage_bytes(BM, NT);
-  constexpr int BLOCK = BM * BM * 2, PANEL = NT * 8 * BM * 2;
-  constexpr int SLICES = BM / 16, GROUPS = 4 / SLICES;  // warps: slice of 16 rows x group of entries
-  static_assert(ST >= 2, "stages");
-
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* sums = reinterpret_cast<float*>(smem + ST * STAGE);  // [4 warps][gate, up][16][NT * 8 + 1]
-  __shared__ uint64_t full[ST], empty[ST];
-  __shared__ uint8_t has[ST][E];  // bit 0: gate, bit 1: up
-  __shared__ int abort_s, issued[ST];
-  volatile int* abort_flag = &abort_s;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < ST; ++s) {
-      ptx::mbar_init(&full[s], 1);
-      ptx::mbar_init(&empty[s], 4);
-      issued[s] = 0;
-    }
-    abort_s = 0;
-    ptx::mbar_init_fence();
-  }
-  __syncthreads();
-  auto range = [&](int row, int& e0, int& e1) {
-    e0 = min(max(__ldg(args.ent_ptr + row), 0), args.nentries);
-    e1 = min(max(__ldg(args.ent_ptr + row + 1), e0), args.nentries);
-  };
-  int sidx = 0;
-  uint32_t sph = 0;
-  auto advance = [&]() {
-    if (++sidx == ST) {
-      sidx = 0;
-      sph ^= 1u;
-    }
-  };
-
-  if (warp == 4) {
-    // ------------------------------------------------------------ loads
-    const uint64_t pol_w = ptx::policy_evict_first();
-    const uint64_t pol_x = ptx::policy_evict_last();
-    const void* map_x = &tmap_x;
-    const void* map_w = &tmap_w;
-    bool alive = true;
-    auto fetch = [&](int e, int e1) { return e < e1 ? __ldg(args.entries + e) : make_int4(0, -1, -1, 0); };
-    int e0 = 0, e1 = 0, n0 = 0, n1 = 0;
-    int4 w0 = make_int4(0, -1, -1, 0), nw = w0;
-    const int first = blockIdx.x, step = gridDim.x;
-    if (first < args.nbr) {
-      range(first, e0, e1);
-      w0 = fetch(e0 + lane, e1);
-    }
-    for (int row = first; row < args.nbr && alive; row += step) {
-      if (row + step < args.nbr) {
-        range(row + step, n0, n1);
-        nw = fetch(n0 + lane, n1);
-      }
-      for (int at = e0; at < e1 && alive; at += 32) {
-        int4 w = w0;
-        if (at + 32 < e1) w0 = fetch(at + 32 + lane, e1);
-        if (static_cast<unsigned>(w.x) >= static_cast<unsigned>(args.nbc) || w.y < -1 || w.y >= args.nblocks ||
-            w.z < -1 || w.z >= args.nblocks) {
-          atomicCAS(args.err, 0u, KAIRO_DEVERR_BAD_INDEX);
-          w = make_int4(0, -1, -1, 0);
-        }
-        for (int b0 = 0; b0 < 32 && at + b0 < e1; b0 += E) {
-          const int take = min(E, e1 - at - b0);
-          int ok = ptx::wait_parity(&empty[sidx], sph ^ 1u, abort_flag, args.err, kTagEmpty, kWaitCycles);
-          ok = __shfl_sync(0xffffffffu, ok, 0);
-          if (!ok) {
-            alive = false;
-            break;
-          }
-          // lanes 4 l .. 4 l + 2: gate block, up block and panel of entry b0 + l of the window
-          const int slot = lane >> 2, part = lane & 3;
-          const int src = (b0 + slot) & 31;
-          const int col = __shfl_sync(0xffffffffu, w.x, src), gb = __shfl_sync(0xffffffffu, w.y, src),
-                    ub = __shfl_sync(0xffffffffu, w.z, src);
-          const bool mine = slot < take;
-          const bool wanted = part == 0 ? gb >= 0 : part == 1 ? ub >= 0 : part == 2 && (gb >= 0 || ub >= 0);
-          const uint32_t issue = mine && wanted ? 1u : 0u;
-          const unsigned sent = __ballot_sync(0xffffffffu, issue != 0u);
-          const uint32_t bytes = static_cast<uint32_t>(__popc(sent & 0x33333333u) * BLOCK + __popc(sent & 0x44444444u) * PANEL);
-          if (lane == 0) issued[sidx] = static_cast<int>(sph) + 1;
-          if (mine && part == 0) has[sidx][slot] = static_cast<uint8_t>((gb >= 0 ? 1 : 0) | (ub >= 0 ? 2 : 0));
-          ptx::mbar_expect_tx_if(lane == 0 ? 1u : 0u, &full[sidx], bytes);
-          __syncwarp();
-          uint8_t* st = smem + sidx * STAGE + (mine ? slot : 0) * ENTRY + (part < 2 ? part : 2) * BLOCK;
-          const bool is_w = part < 2;
-          ptx::tma_load_2d_if(issue, st, is_w ? map_w : map_x, is_w ? 0 : col * BM, is_w ? (part == 0 ? gb : ub) * BM : 0,
-                              &full[sidx], is_w ? pol_w : pol_x);
-          __syncwarp();
-          ptx::mbar_arrive_if(lane == 0 ? 1u : 0u, &full[sidx]);
-          advance();
-        }
-      }
-      e0 = n0;
-      e1 = n1;
-      w0 = nw;
-    }
-  } else {
-    // ------------------------------------------------------------ products
-    const int slice = warp % SLICES, group = warp / SLICES;
-    const int gid = lane >> 2, t = lane & 3;
-    bool alive = true;
-    for (int row = blockIdx.x; row < args.nbr && alive; row += gridDim.x) {
-      int e0, e1;
-      range(row, e0, e1);
-      float g[NT][4], u[NT][4];
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) g[i][j] = u[i][j] = 0.f;
-      // the same stages as the loads: windows of 32 entries, E at a time
-      for (int at = e0; at < e1; at += E) {
-        const int take = min(E, e1 - at);
-        int ok = ptx::wait_parity(&full[sidx], sph, abort_flag, args.err, kTagFull, kWaitCycles);
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        if (!ok) {
-          alive = false;
-          break;
-        }
-        for (int e = group; e < take; e += GROUPS) {
-          const int have = has[sidx][e];
-          const uint32_t st = ptx::smem_u32(smem + sidx * STAGE + e * ENTRY);
-          const int ar = slice * 16 + (lane & 15), ac = lane >> 4;   // A: 16 rows, two chunks
-          const int br = lane & 7, bc = lane >> 3;                   // B: 8 tokens, four chunks
-          uint32_t ga[BM / 16][4], ua[BM / 16][4];
-          if (have & 1) {
-#pragma unroll
-            for (int q = 0; q < BM / 16; ++q) ldmatrix4(ga[q], st + box_at<BM>(ar, 2 * q + ac));
-          }
-          if (have & 2) {
-#pragma unroll
-            for (int q = 0; q < BM / 16; ++q) ldmatrix4(ua[q], st + BLOCK + box_at<BM>(ar, 2 * q + ac));
-          }
-          // 32 k and up to 8 groups of tokens at a time; successive products go to different sums
-          constexpr int TG = NT < 8 ? NT : 8;
-#pragma unroll
-          for (int i0 = 0; i0 < NT; i0 += TG) {
-#pragma unroll
-            for (int h = 0; h < (BM + 31) / 32; ++h) {
-              uint32_t xb[TG][4];
-#pragma unroll
-              for (int i = 0; i < TG; ++i) {
-                if constexpr (BM == 16) ldmatrix2(xb[i], st + 2 * BLOCK + box_at<BM>((i0 + i) * 8 + br, bc & 1));
-                else ldmatrix4(xb[i], st + 2 * BLOCK + box_at<BM>((i0 + i) * 8 + br, 4 * h + bc));
-              }
-#pragma unroll
-              for (int q = 2 * h; q < 2 * h + 2 && q < BM / 16; ++q) {
-                const int k = 2 * (q & 1);
-                if (have == 3) {
-#pragma unroll
-                  for (int i = 0; i < TG; ++i) {
-                    mma_16816<TT>(g[i0 + i], ga[q][0], ga[q][1], ga[q][2], ga[q][3], xb[i][k], xb[i][k + 1]);
-                    mma_16816<TT>(u[i0 + i], ua[q][0], ua[q][1], ua[q][2], ua[q][3], xb[i][k], xb[i][k + 1]);
-                  }
-                } else if (have == 1) {
-#pragma unroll
-                  for (int i = 0; i < TG; ++i)
-                    mma_16816<TT>(g[i0 + i], ga[q][0], ga[q][1], ga[q][2], ga[q][3], xb[i][k], xb[i][k + 1]);
-                } else if (have == 2) {
-#pragma unroll
-                  for (int i = 0; i < TG; ++i)
-                    mma_16816<TT>(u[i0 + i], ua[q][0], ua[q][1], ua[q][2], ua[q][3], xb[i][k], xb[i][k + 1]);
-                }
-              }
-            }
-          }
-        }
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&empty[sidx]);
-        advance();
-      }
-      // where the warps meet at barriers below, they leave together
-      if (GROUPS > 1 ? epi_any(!alive) : !alive) break;
-      if constexpr (GROUPS > 1) {
-        // the groups' sums meet in shared memory; group 0 carries on with the total
-        constexpr int PITCH = NT * 8 + 1;
-        float* own = sums + warp * 2 * 16 * PITCH;
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int at = (gid + (j >> 1) * 8) * PITCH + i * 8 + 2 * t + (j & 1);
-            own[at] = g[i][j];
-            own[16 * PITCH + at] = u[i][j];
-          }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        if (group == 0) {
-#pragma unroll
-          for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int at = (gid + (j >> 1) * 8) * PITCH + i * 8 + 2 * t + (j & 1);
-#pragma unroll
-              for (int q = 1; q < GROUPS; ++q) {
-                const float* other = sums + (warp + q * SLICES) * 2 * 16 * PITCH;
-                g[i][j] += other[at];
-                u[i][j] += other[16 * PITCH + at];
-              }
-            }
-        }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-      }
-      if (group == 0) {
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int token = i * 8 + 2 * t + (j & 1);
-            if (token < args.n)
-              gated_out<TT, GRAD, 1>(args, token, row, BM, slice * 16 + gid + (j >> 1) * 8, &g[i][j], &u[i][j]);
-          }
-      }
-    }
-  }
-  __syncthreads();
-  if (threadIdx.x == 0 && *abort_flag) {
-    int dummy = 0;
-    for (int s = 0; s < ST; ++s)
-      if (issued[s])
-        ptx::wait_parity(&full[s], static_cast<uint32_t>(issued[s] - 1), reinterpret_cast<volatile int*>(&dummy),
-                         args.err, kTagDrain, kWaitCycles);
-  }
-}
-
 // ------------------------------------------------------------ host side
 
 constexpr int kAnyTokens = 8;   // up to here X may have any alignment
 constexpr int kFewTokens = 32;
-constexpr int kStreamTokens = 64;
-constexpr int kStreamRows = 256;  // block-rows
+constexpr int kShortRows = 192;  // block-rows
 
 template <int BM, int NT, typename T, bool GRAD>
 void launch_few(const GatedArgs& a, cudaStream_t s) {
@@ -907,42 +885,15 @@ void launch_few(const GatedArgs& a, cudaStream_t s) {
   k_gated_few<BM, NT, T, GRAD><<<a.nbr * (BM / 16), 32 * kFewWarps, 0, s>>>(a, vec_x);
 }
 
-template <int BM, int NT, typename TT, int IN_FMT, bool GRAD>
-kairo_status launch_stream(const GatedArgs& a, cudaStream_t s) {
-  const CUtensorMapDataType dt = IN_FMT == 0 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  CUtensorMap mx, mw;
-  kairo_status st = make_map_2d(&mx, a.x, dt, 2, static_cast<uint64_t>(a.k), static_cast<uint64_t>(a.n),
-                                static_cast<uint64_t>(a.ldx), BM, NT * 8, "X");
-  if (st == KAIRO_STATUS_SUCCESS)
-    st = make_map_2d(&mw, a.blocks, dt, 2, BM, static_cast<uint64_t>(std::max(1, a.nblocks)) * BM, BM, BM, BM,
-                     "block storage");
-  if (st) return st;
-  auto* fn = &k_gated_stream<BM, NT, TT, GRAD>;
-  static std::atomic<uint64_t> ready{0};
-  cudaError_t e = allow_smem(reinterpret_cast<const void*>(fn), kStreamSmem, &ready);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic smem)");
-  const int grid = std::min(a.nbr, 2 * device_sm_count(current_device()));
-  fn<<<grid, kStreamThreads, kStreamSmem, s>>>(mx, mw, a);
-  e = cudaGetLastError();
-  return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "launch of k_gated_stream");
-}
-
 template <int BM, typename TT, int IN_FMT, bool GRAD>
 kairo_status run_gated(GatedArgs a, cudaStream_t s) {
-  // Streamed blocks where a CTA per block-row fills the SMs.  Blocks of 64, 32768 x 8192 at 20 % twice (the
-  // blocks alone 33 us): 16 / 32 / 64 tokens 56 / 64 / 86 us, by fragments 64 / 82 / -, by k_gated 121;
-  // 4096 x 4096 (64 block-rows): 32 tokens 25 us, by fragments 15; 64 tokens 31, by k_gated 23.  Smaller blocks:
-  // fragments up to 32 tokens (12288 x 4096, blocks of 32, 24 tokens: 26 us against 40), then streamed (64
-  // tokens: 51 against 82 by k_gated).
-  const bool rows = a.nbr >= kStreamRows;
-  if (BM == 64 ? rows && a.n > 8 && a.n <= kStreamTokens : a.n > kFewTokens && a.n <= kStreamTokens) {
-    if constexpr (BM == 64) {
-      if (a.n <= 16) return launch_stream<BM, 2, TT, IN_FMT, GRAD>(a, s);
-      if (a.n <= 32) return launch_stream<BM, 4, TT, IN_FMT, GRAD>(a, s);
-    }
-    return launch_stream<BM, 8, TT, IN_FMT, GRAD>(a, s);
-  }
-  if (a.n <= kFewTokens) {
+  // Fragments up to 32 tokens, or up to 16 where blocks of 64 have rows enough for the SMs: 32768 x 8192 at 20 %
+  // twice (the blocks alone 33 us), 16 / 32 tokens 64 / 82 us by fragments, 59 / 59 by k_gated_short; 14336 x 4096 (224
+  // block-rows) 23 / 29 and 25 / 25; 4096 x 4096 (64) 10 / 12 and 21 / 21.  Blocks of 32 and 16, 14336 x 4096, 32
+  // tokens: 31 and 39, by k_gated_short 33 and 70.  Between 33 and 128 tokens k_gated takes 45, 84 and 205 us (blocks of 64,
+  // 32, 16) where k_gated_short takes 27, 37 and 84.
+  const bool rows = BM == 64 && a.nbr >= kShortRows;
+  if (a.n <= (rows ? kFewTokens / 2 : kFewTokens)) {
     if (a.n <= 8) launch_few<BM, 1, TT, GRAD>(a, s);
     else if (a.n <= 16) launch_few<BM, 2, TT, GRAD>(a, s);
     else if (a.n <= 24) launch_few<BM, 3, TT, GRAD>(a, s);
@@ -951,6 +902,23 @@ kairo_status run_gated(GatedArgs a, cudaStream_t s) {
     return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "launch of k_gated_few");
   }
   const CUtensorMapDataType dt = IN_FMT == 0 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  if (a.n <= kShortTokens) {
+    CUtensorMap mx, mw;
+    kairo_status st = make_map_2d(&mx, a.x, dt, 2, static_cast<uint64_t>(a.k), static_cast<uint64_t>(a.n),
+                                  static_cast<uint64_t>(a.ldx), BM, 64, "X");
+    if (st == KAIRO_STATUS_SUCCESS)
+      st = make_map_2d(&mw, a.blocks, dt, 2, BM, static_cast<uint64_t>(std::max(1, a.nblocks)) * BM, BM, BM, BM,
+                       "block storage");
+    if (st) return st;
+    auto* fn = &k_gated_short<BM, IN_FMT, TT, GRAD>;
+    static std::atomic<uint64_t> ready{0};
+    cudaError_t e = allow_smem(reinterpret_cast<const void*>(fn), short_smem(BM), &ready);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic smem)");
+    const int grid = std::min(a.nbr, 2 * device_sm_count(current_device()));
+    fn<<<grid, kShortThreads, short_smem(BM), s>>>(mx, mw, a);
+    e = cudaGetLastError();
+    return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "launch of k_gated_short");
+  }
   auto go = [&](auto tc) -> kairo_status {
     constexpr int T = decltype(tc)::value;
     CUtensorMap mx, mw;
