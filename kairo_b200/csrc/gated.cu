@@ -27,10 +27,12 @@
 // 256 tokens (1.95 ms), blocks brought into L2 ahead (1.65), one 32 KB copy of a
 // panel instead of four (1.61), other groups of token tiles (1.6 to 1.85).
 //
-// k_gated_short (33 to 128 tokens; from 17 on where blocks of 64 have many rows).  The same with one CTA a block-row and
-// two CTAs an SM: a pair would multiply and fill panels of 256 tokens, and has half as many places to share the
-// block-rows out to.  128 tokens, 4096 -> 14336 at 20 %: 27 us (k_gated 47), 64 tokens, 8192 -> 32768: 61 us, where the
-// blocks alone are 33 and the L2 hands each block-row the panels of its columns.
+// k_gated_short (33 to 256 tokens; blocks of 64: to 128, or 17 to 256 where they
+// have many rows).  The same with one CTA a block-row and two CTAs an SM: a pair
+// would multiply and fill panels of 256 tokens, and has half as many places to share
+// the block-rows out to.  128 tokens, 4096 -> 14336 at 20 %: 27 us (k_gated 47); 64
+// tokens, 8192 -> 32768: 61 us, where the blocks alone are 33 and the L2 hands each
+// block-row the panels of its columns.
 //
 // k_gated_few (up to 32 tokens).  Bound by reading the blocks once.  A CTA takes 16
 // rows of a block-row, its warps share out the entries; mma.sync fragments come
@@ -452,34 +454,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGatedThreads, 1)
   }
 }
 
-// ------------------------------------------------------------ up to 128 tokens on the tensor cores
+// ------------------------------------------------------------ up to 256 tokens on the tensor cores
 
 constexpr int kShortThreads = 192;
 constexpr int kShortEpiWarps = 4;
-constexpr int kShortTokens = 128;
-constexpr int short_slot_bytes(int bm) { return kShortTokens * bm * 2 + 2 * bm * bm * 2; }  // X, gate, up
-constexpr int short_stage_bytes(int bm) { return gated_group(bm) * short_slot_bytes(bm); }
-constexpr int short_stages(int bm) { return 100 * 1024 / short_stage_bytes(bm); }
-constexpr size_t short_smem(int bm) { return static_cast<size_t>(short_stages(bm)) * short_stage_bytes(bm) + 2048; }
-static_assert(2 * (short_smem(64) + 1024) <= 228 * 1024 && 2 * (short_smem(32) + 1024) <= 228 * 1024 &&
-                  2 * (short_smem(16) + 1024) <= 228 * 1024,
-              "two CTAs of an SM");
+constexpr int kShortTokens = 128;  // of a subtile; a CTA takes T of them
+constexpr int short_slot_bytes(int bm, int t) { return t * kShortTokens * bm * 2 + 2 * bm * bm * 2; }  // X, gate, up
+constexpr int short_stage_bytes(int bm, int t) { return gated_group(bm) * short_slot_bytes(bm, t); }
+constexpr int short_stages(int bm, int t) { return 100 * 1024 / short_stage_bytes(bm, t); }
+constexpr size_t short_smem(int bm, int t) {
+  return static_cast<size_t>(short_stages(bm, t)) * short_stage_bytes(bm, t) + 2048;
+}
+constexpr bool short_fits(int t) {  // twice in an SM
+  return 2 * (short_smem(64, t) + 1024) <= 228 * 1024 && 2 * (short_smem(32, t) + 1024) <= 228 * 1024 &&
+         2 * (short_smem(16, t) + 1024) <= 228 * 1024;
+}
+static_assert(short_fits(1) && short_fits(2), "two CTAs of an SM");
 
-// k_gated with one CTA for all tokens of a block-row: M = 128 tokens (64 of them copied where there are no more), N = 2 * BM
-// outputs, the gate block's rows followed by the up block's.
-template <int BM, int IN_FMT, typename TT, bool GRAD>
+// k_gated with one CTA for all tokens of a block-row: M = 128 tokens (64 of them copied where there are no more), N = 2 *
+// BM outputs, the gate block's rows followed by the up block's.
+template <int BM, int T, int IN_FMT, typename TT, bool GRAD>
 __global__ void __launch_bounds__(kShortThreads, 2)
     k_gated_short(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
                   const GatedArgs args) {
-  constexpr int ST = short_stages(BM);
+  constexpr int ST = short_stages(BM, T);
   constexpr int E = gated_group(BM);
-  constexpr int SLOT = short_slot_bytes(BM);
-  constexpr int STAGE = short_stage_bytes(BM);
-  constexpr int PANEL = kShortTokens * BM * 2;
+  constexpr int SLOT = short_slot_bytes(BM, T);
+  constexpr int STAGE = short_stage_bytes(BM, T);
+  constexpr int PANEL = T * kShortTokens * BM * 2;
   constexpr uint32_t IDESC = ptx::make_idesc_f16(IN_FMT, 0u, 0u, kShortTokens, 2 * BM);
   constexpr uint32_t SW = ptx::swizzle_code_for_row_bytes(BM * 2);
-  constexpr uint32_t ACC = 2 * BM;
-  constexpr uint32_t TMEM_COLS = 2 * ACC;
+  constexpr uint32_t ACC = T * 2 * BM;
+  constexpr int SLOTS = 2 * ACC <= 256 ? 2 : 1;  // accumulators: half the columns of an SM are this CTA's
+  constexpr uint32_t TMEM_COLS = SLOTS * ACC;
   static_assert(SLOT % 1024 == 0 && PANEL % 1024 == 0 && TMEM_COLS >= 32 && TMEM_COLS <= 256, "layout");
 
   extern __shared__ uint8_t smem_raw[];
@@ -502,7 +509,7 @@ __global__ void __launch_bounds__(kShortThreads, 2)
       ptx::mbar_init(&empty[s], 1);
       issued[s] = 0;
     }
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < SLOTS; ++k) {
       ptx::mbar_init(&tfull[k], 1);
       ptx::mbar_init(&tempty[k], kShortEpiWarps);
     }
@@ -531,13 +538,14 @@ __global__ void __launch_bounds__(kShortThreads, 2)
     // ------------------------------------------------------------ loads
     const uint64_t pol_w = ptx::policy_evict_first();
     const uint64_t pol_x = ptx::policy_evict_last();
-    constexpr int BOXES = 4;  // two of 64 tokens, the gate block, the up block
-    const int xboxes = args.n > 64 ? 2 : 1;
+    constexpr int BOXES = 2 * T + 2;  // of 64 tokens, the gate block, the up block
+    static_assert(E * BOXES <= 32, "one lane per copy");
+    const int xboxes = (args.n + 63) / 64;
     const int e = lane / BOXES, part = lane - e * BOXES;
-    const bool is_w = part >= 2;
+    const bool is_w = part >= 2 * T;
     const uint32_t bytes = static_cast<uint32_t>(xboxes * 64 * BM * 2 + 2 * BM * BM * 2);  // of an entry
     const uint32_t dst_off =
-        static_cast<uint32_t>((e < E ? e : 0) * SLOT + (is_w ? PANEL + (part - 2) * BM * BM * 2 : part * 64 * BM * 2));
+        static_cast<uint32_t>((e < E ? e : 0) * SLOT + (is_w ? PANEL + (part - 2 * T) * BM * BM * 2 : part * 64 * BM * 2));
     const void* map = is_w ? static_cast<const void*>(&tmap_w) : static_cast<const void*>(&tmap_x);
     const uint64_t pol = is_w ? pol_w : pol_x;
     int sidx = 0;
@@ -573,7 +581,7 @@ __global__ void __launch_bounds__(kShortThreads, 2)
           const int egate = __shfl_sync(0xffffffffu, gate, src);
           const int eup = __shfl_sync(0xffffffffu, up, src);
           ptx::tma_load_2d_if(mine, smem + sidx * STAGE + dst_off, map, is_w ? 0 : ecol * BM,
-                              is_w ? (part == 2 ? egate : eup) * BM : part * 64, &full[sidx], pol);
+                              is_w ? (part == 2 * T ? egate : eup) * BM : part * 64, &full[sidx], pol);
           __syncwarp();
           ptx::mbar_arrive_if(lane == 0 ? 1u : 0u, &full[sidx]);
           if (++sidx == ST) {
@@ -586,6 +594,7 @@ __global__ void __launch_bounds__(kShortThreads, 2)
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     const uint32_t leader = lane == 0 ? 1u : 0u;
+    const int subs = (args.n + kShortTokens - 1) / kShortTokens;
     const uint32_t sbase = ptx::smem_u32(smem);
     const uint64_t adesc = ptx::make_smem_desc(sbase, 16, 8 * BM * 2, SW);
     const uint64_t bdesc = ptx::make_smem_desc(sbase + PANEL, 16, 8 * BM * 2, SW);
@@ -615,9 +624,13 @@ __global__ void __launch_bounds__(kShortThreads, 2)
           if (at + e >= cnt) break;
           const uint32_t s16 = static_cast<uint32_t>(sidx * STAGE + e * SLOT) >> 4;
 #pragma unroll
-          for (int kk = 0; kk < BM / 16; ++kk)
-            ptx::mma_f16_ss_if(leader, d, a_lo + s16 + ((kk * 32) >> 4), a_hi, b_lo + s16 + ((kk * 32) >> 4), b_hi, IDESC,
-                               (at > 0 || e > 0 || kk > 0) ? 1u : 0u);
+          for (int kk = 0; kk < BM / 16; ++kk) {
+#pragma unroll
+            for (int i = 0; i < T; ++i)
+              ptx::mma_f16_ss_if(i < subs ? leader : 0u, d + static_cast<uint32_t>(i * 2 * BM),
+                                 a_lo + s16 + ((i * kShortTokens * BM * 2 + kk * 32) >> 4), a_hi,
+                                 b_lo + s16 + ((kk * 32) >> 4), b_hi, IDESC, (at > 0 || e > 0 || kk > 0) ? 1u : 0u);
+          }
         }
         ptx::mma_commit_if(leader, &empty[sidx]);
         if (++sidx == ST) {
@@ -627,8 +640,10 @@ __global__ void __launch_bounds__(kShortThreads, 2)
       }
       if (!alive) break;
       ptx::mma_commit_if(leader, &tfull[slot]);
-      slot ^= 1;
-      if (slot == 0) aphase ^= 1u;
+      if (++slot == SLOTS) {
+        slot = 0;
+        aphase ^= 1u;
+      }
     }
     ptx::mma_commit_if(leader, mma_done);
     int dummy = 0;
@@ -638,7 +653,6 @@ __global__ void __launch_bounds__(kShortThreads, 2)
     // ------------------------------------------------------------ epilogue
     constexpr int UN = BM < 32 ? BM : 32;  // outputs of one step
     const int q = warp & 3;
-    const int token = q * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(q * 32) << 16;
     int slot = 0;
     uint32_t aphase = 0;
@@ -652,33 +666,37 @@ __global__ void __launch_bounds__(kShortThreads, 2)
         ptx::tc_fence_after();
       }
       const uint32_t at = tmem_base + lane_addr + static_cast<uint32_t>(slot) * ACC;
-      if (q * 32 < args.n) {
 #pragma unroll 1
-        for (int c0 = 0; c0 < BM; c0 += UN) {
-          float g[UN], u[UN];
-          if (some) {
-            if constexpr (UN == 32) {
-              ptx::tmem_ld32(at + static_cast<uint32_t>(c0), g);
-              ptx::tmem_ld32(at + static_cast<uint32_t>(BM + c0), u);
-            } else {
-              ptx::tmem_ld16(at + static_cast<uint32_t>(c0), g);
-              ptx::tmem_ld16(at + static_cast<uint32_t>(BM + c0), u);
-            }
-            ptx::tmem_wait_ld();
+      for (int s = 0; s < T * (BM / UN); ++s) {
+        const int i = s / (BM / UN), c0 = (s % (BM / UN)) * UN;
+        const int token0 = i * kShortTokens + q * 32, token = token0 + lane;
+        if (token0 >= args.n) break;
+        const uint32_t here = at + static_cast<uint32_t>(i * 2 * BM + c0);
+        float g[UN], u[UN];
+        if (some) {
+          if constexpr (UN == 32) {
+            ptx::tmem_ld32(here, g);
+            ptx::tmem_ld32(here + BM, u);
           } else {
-#pragma unroll
-            for (int j = 0; j < UN; ++j) g[j] = u[j] = 0.f;
+            ptx::tmem_ld16(here, g);
+            ptx::tmem_ld16(here + BM, u);
           }
-          if (token < args.n) gated_out<TT, GRAD, UN>(args, token, row, BM, c0, g, u);
-          __syncwarp();
+          ptx::tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int j = 0; j < UN; ++j) g[j] = u[j] = 0.f;
         }
+        if (token < args.n) gated_out<TT, GRAD, UN>(args, token, row, BM, c0, g, u);
+        __syncwarp();
       }
       if (some) {
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&tempty[slot]);
-        slot ^= 1;
-        if (slot == 0) aphase ^= 1u;
+        if (++slot == SLOTS) {
+          slot = 0;
+          aphase ^= 1u;
+        }
       }
     }
   }
@@ -888,10 +906,11 @@ void launch_few(const GatedArgs& a, cudaStream_t s) {
 template <int BM, typename TT, int IN_FMT, bool GRAD>
 kairo_status run_gated(GatedArgs a, cudaStream_t s) {
   // Fragments up to 32 tokens, or up to 16 where blocks of 64 have rows enough for the SMs: 32768 x 8192 at 20 %
-  // twice (the blocks alone 33 us), 16 / 32 tokens 64 / 82 us by fragments, 59 / 59 by k_gated_short; 14336 x 4096 (224
-  // block-rows) 23 / 29 and 25 / 25; 4096 x 4096 (64) 10 / 12 and 21 / 21.  Blocks of 32 and 16, 14336 x 4096, 32
-  // tokens: 31 and 39, by k_gated_short 33 and 70.  Between 33 and 128 tokens k_gated takes 45, 84 and 205 us (blocks of 64,
-  // 32, 16) where k_gated_short takes 27, 37 and 84.
+  // twice (the blocks alone 33 us), 16 / 32 tokens 64 / 82 us by fragments, 59 / 59 by k_gated_short; 14336 x 4096
+  // (224 block-rows) 23 / 29 and 25 / 25; 4096 x 4096 (64) 10 / 12 and 21 / 21.  Blocks of 32 and 16, 14336 x 4096,
+  // 32 tokens: 31 and 39, by k_gated_short 33 and 70.  Between 33 and 256 tokens k_gated takes 47, 85 and 206 us
+  // (blocks of 64, 32, 16); k_gated_short 27, 37 and 84 up to 128, and 45, 61 and 133 up to 256, where 4096 x 4096 in
+  // blocks of 64 takes 37 us (k_gated 23).
   const bool rows = BM == 64 && a.nbr >= kShortRows;
   if (a.n <= (rows ? kFewTokens / 2 : kFewTokens)) {
     if (a.n <= 8) launch_few<BM, 1, TT, GRAD>(a, s);
@@ -902,7 +921,8 @@ kairo_status run_gated(GatedArgs a, cudaStream_t s) {
     return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "launch of k_gated_few");
   }
   const CUtensorMapDataType dt = IN_FMT == 0 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  if (a.n <= kShortTokens) {
+  auto few = [&](auto tc) -> kairo_status {
+    constexpr int T = decltype(tc)::value;
     CUtensorMap mx, mw;
     kairo_status st = make_map_2d(&mx, a.x, dt, 2, static_cast<uint64_t>(a.k), static_cast<uint64_t>(a.n),
                                   static_cast<uint64_t>(a.ldx), BM, 64, "X");
@@ -910,15 +930,17 @@ kairo_status run_gated(GatedArgs a, cudaStream_t s) {
       st = make_map_2d(&mw, a.blocks, dt, 2, BM, static_cast<uint64_t>(std::max(1, a.nblocks)) * BM, BM, BM, BM,
                        "block storage");
     if (st) return st;
-    auto* fn = &k_gated_short<BM, IN_FMT, TT, GRAD>;
+    auto* fn = &k_gated_short<BM, T, IN_FMT, TT, GRAD>;
     static std::atomic<uint64_t> ready{0};
-    cudaError_t e = allow_smem(reinterpret_cast<const void*>(fn), short_smem(BM), &ready);
+    cudaError_t e = allow_smem(reinterpret_cast<const void*>(fn), short_smem(BM, T), &ready);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(max dynamic smem)");
     const int grid = std::min(a.nbr, 2 * device_sm_count(current_device()));
-    fn<<<grid, kShortThreads, short_smem(BM), s>>>(mx, mw, a);
+    fn<<<grid, kShortThreads, short_smem(BM, T), s>>>(mx, mw, a);
     e = cudaGetLastError();
     return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "launch of k_gated_short");
-  }
+  };
+  if (a.n <= kShortTokens) return few(std::integral_constant<int, 1>{});
+  if (a.n <= 2 * kShortTokens && (BM < 64 || rows)) return few(std::integral_constant<int, 2>{});
   auto go = [&](auto tc) -> kairo_status {
     constexpr int T = decltype(tc)::value;
     CUtensorMap mx, mw;
@@ -941,7 +963,10 @@ kairo_status run_gated(GatedArgs a, cudaStream_t s) {
     e = cudaGetLastError();
     return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "launch of k_gated");
   };
-  return a.n > 256 ? go(std::integral_constant<int, 2>{}) : go(std::integral_constant<int, 1>{});
+  if constexpr (BM == 64) {
+    if (a.n <= 256) return go(std::integral_constant<int, 1>{});
+  }
+  return go(std::integral_constant<int, 2>{});
 }
 
 template <bool GRAD>

@@ -22,9 +22,9 @@
 // 8 tokens * vocab * dim operations for the 6 that logits kept in memory would
 // need; it keeps 2 * tokens bytes a column of the piece instead of 4 * tokens * vocab.
 //
-// Measured.  8192 tokens, 131072 x 2048, bf16: the forward pass 3.3 ms (1340 TFLOP/s), G 4.0, dX 3.1, dW 3.0
-// (1465): 14 ms, 1260 TFLOP/s of what is done, where the power limit leaves cuBLAS 1355.  One to 64 tokens
-// of 131072 x 4096: 185 to 190 us, 5.6 to 5.8 TB/s.
+// Measured.  8192 tokens, 131072 x 2048, bf16: the forward pass 3.1 ms (1400 TFLOP/s), G 3.4, dX 3.0, dW 3.0
+// (1465) one after the other from a cool start; in a row 13.7 ms, 1280 TFLOP/s of what is done, where the power
+// limit leaves cuBLAS 1355.  One to 64 tokens of 131072 x 4096: 185 to 190 us, 5.6 to 5.8 TB/s.
 //
 // Rounding.  z, the maxima, sums and lse are fp32.  G is rounded once to the
 // operands' 16 bits, as an operand of both products must be: relative to each

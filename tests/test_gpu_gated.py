@@ -129,6 +129,13 @@ def test_many_rows(tokens, dtype):
     run_case(tokens, 64 * 259 - 7, 136, 64, dtype, act="silu")
 
 
+@pytest.mark.parametrize("tokens", [20, 64, 65, 128, 129, 256])
+@pytest.mark.parametrize("b", [64, 16])
+def test_more_rows_than_places(tokens, b):
+    """Several block-rows for each resident CTA, some of them empty."""
+    run_case(tokens, b * 700 - 5, 2 * b + 8, b, torch.float16, act="gelu", keep=0.4)
+
+
 @pytest.mark.parametrize("tokens,b,nbc", [(1, 64, 70), (3, 16, 300), (20, 32, 67), (40, 32, 67), (50, 16, 80),
                                           (600, 64, 70), (300, 16, 140)])
 def test_long_rows(tokens, b, nbc):
