@@ -18,7 +18,7 @@
 // 9e-8 of the sum so far: over 256 steps a logit would lose 1.2e-5 of itself, ten
 // times what fp32 sums lose.  So a tile's sum is cut into segments of `seg` stages;
 // the epilogue adds them up in registers (128 fp32 a thread), with rounding, while
-// the next segment runs in the other half of TMEM.  A segment of 256 k takes 2048
+// the next segment runs in the other half of TMEM.  A segment of 512 k takes 4096
 // tensor cycles and its addition some 600 of the epilogue's.
 //
 // Roles (384 threads, one CTA per SM, persistent): warp 0 loads, warp 1

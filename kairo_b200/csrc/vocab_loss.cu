@@ -744,7 +744,8 @@ LossWs loss_ws(const Problem& p) {
   o.ticket = 128;
   o.target = take(4 * static_cast<size_t>(p.tokens));
   o.each = take(4 * static_cast<size_t>(p.tokens));
-  const int64_t slots = p.tokens <= kFewTokens ? 8 * kPairClusters : 2 * tiles(p.vocab);
+  const int64_t slots =
+      p.tokens <= kFewTokens ? 8 * std::min<int64_t>(kPairClusters, tiles(p.vocab)) : 2 * tiles(p.vocab);
   o.part = take(8 * static_cast<size_t>(p.tokens) * static_cast<size_t>(slots));
   const size_t ld = static_cast<size_t>(copy_ld(p.dim));
   const int64_t copies = copies_of(std::max<int64_t>(1, p.tokens));
@@ -852,7 +853,7 @@ int group_rows(int64_t tiles_m, int64_t k) {
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(tiles_m, (32LL << 20) / (kPairTileM * 2 * std::max<int64_t>(k, 64)))));
 }
 
-// Stages of a segment.  Logits: 256 k, so that lse and losses are as exact as fp32 sums (7e-7 of a
+// Stages of a segment.  Logits: 512 k, so that lse and losses are as exact as fp32 sums (7e-7 of a
 // logit at worst).  The gradients are rounded to 16 bits: 4096 k leave 1e-5.
 constexpr int kSegLogits = 8, kSegGrads = 64;
 
