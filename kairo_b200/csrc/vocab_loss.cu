@@ -43,7 +43,6 @@ namespace kairo {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 constexpr int64_t kPieceBytes = 512LL << 20;
 constexpr float kHalfLift = 32768.f;  // 2^15, see above
 
@@ -64,11 +63,15 @@ struct Targets {
 
 // ------------------------------------------------------------ epilogues
 
-// Running maximum and sum of exp2 of one token's columns.
+// Logits in base 2 are v * stats_scale(scale), of -v where scale < 0.  Not 0: masked columns are -inf.
+__host__ __device__ __forceinline__ float stats_scale(float scale) { return fmaxf(fabsf(scale) * kLog2e, 1e-38f); }
+
+// Running maximum and sum of exp2 of one token's columns.  The maximum is a rounded product, but what is subtracted
+// from the exact ones (fma), so that the terms that count are as exact as v.
 struct StatsEpi {
   struct Args {
     float2* part;   // [slots][tokens]
-    float* target;  // [tokens], the target's logit
+    float* target;  // [tokens], the target's v
     Targets ids;
     int tokens, vocab;
     float scale;
@@ -105,23 +108,26 @@ struct StatsEpi {
 #pragma unroll
       for (int j = 0; j < kPairEpiCols; ++j)
         if (at == j) z = v[j];
-      if (here && token < a.tokens) a.target[token] = z * a.scale;
+      if (here && token < a.tokens) a.target[token] = z;
     }
-    const float k = a.scale * kLog2e;
+    const float k = stats_scale(a.scale);
+    if (a.scale < 0.f) {
 #pragma unroll
-    for (int j = 0; j < kPairEpiCols; ++j) v[j] *= k;
+      for (int j = 0; j < kPairEpiCols; ++j) v[j] = -v[j];
+    }
     if (col0 + kPairEpiCols > a.vocab) {
 #pragma unroll
       for (int j = 0; j < kPairEpiCols; ++j)
         if (col0 + j >= a.vocab) v[j] = -INFINITY;
     }
-    float top = m;
+    float top = v[0];
 #pragma unroll
-    for (int j = 0; j < kPairEpiCols; ++j) top = fmaxf(top, v[j]);
+    for (int j = 1; j < kPairEpiCols; ++j) top = fmaxf(top, v[j]);
+    top = fmaxf(m, top * k);
     const float ref = top == -INFINITY ? 0.f : top;
     float sum[4] = {s * ex2(m - ref), 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < kPairEpiCols; ++j) sum[j & 3] += ex2(v[j] - ref);
+    for (int j = 0; j < kPairEpiCols; ++j) sum[j & 3] += ex2(fmaf(v[j], k, -ref));
     m = top;
     s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
     if (!a.by_cluster) flush(token, static_cast<int64_t>(pt.nt) * (kPairTileN / kPairEpiCols) + part);
@@ -199,8 +205,8 @@ struct FewStatsEpi {
   __device__ void tile(const PairTile& pt, float (&all)[32 * GROUPS]) {
     const int lane = threadIdx.x & 31;
     const int r = pt.mt * kPairTileM + row;
-    const float k = a.scale * kLog2e;
-    const bool in = r < a.vocab;
+    const float k = stats_scale(a.scale);
+    const bool in = r < a.vocab, minus = a.scale < 0.f;
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
       if (token - lane + 32 * g >= a.tokens) break;
@@ -212,19 +218,19 @@ struct FewStatsEpi {
           if (hits >> j & 1u) {
             const int from = static_cast<int>(__shfl_sync(0xffffffffu, at, j));
             const float z = __shfl_sync(0xffffffffu, all[32 * g + j], from);
-            if (lane == j) a.target[token + 32 * g] = z * a.scale;
+            if (lane == j) a.target[token + 32 * g] = z;
           }
       }
       float v[32], w[32];
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
-        v[j] = in ? all[32 * g + j] * k : -INFINITY;
+        v[j] = in ? (minus ? -all[32 * g + j] : all[32 * g + j]) : -INFINITY;
         w[j] = v[j];
       }
-      const float top = fmaxf(m[g], across(w, [](float x, float y) { return fmaxf(x, y); }));
+      const float top = fmaxf(m[g], across(w, [](float x, float y) { return fmaxf(x, y); }) * k);
       const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
-      for (int j = 0; j < 32; ++j) w[j] = ex2(v[j] - __shfl_sync(0xffffffffu, ref, j));
+      for (int j = 0; j < 32; ++j) w[j] = ex2(fmaf(v[j], k, -__shfl_sync(0xffffffffu, ref, j)));
       const float sum = across(w, [](float x, float y) { return x + y; });
       s[g] = s[g] * ex2(m[g] - ref) + sum;
       m[g] = top;
@@ -455,8 +461,8 @@ __device__ float cta_sum(float v) {
 // reduces the losses, always in the same order.
 __global__ void __launch_bounds__(1024) k_lse(const float2* __restrict__ part, int slots,
                                               const float* __restrict__ target, Targets ids, int tokens, int vocab,
-                                              int reduction, float* __restrict__ each, float* __restrict__ lse,
-                                              float* __restrict__ loss, unsigned* ticket) {
+                                              float scale, int reduction, float* __restrict__ each,
+                                              float* __restrict__ lse, float* __restrict__ loss, unsigned* ticket) {
   __shared__ float2 sm[32][33];
   __shared__ bool last;
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
@@ -487,11 +493,15 @@ __global__ void __launch_bounds__(1024) k_lse(const float2* __restrict__ part, i
     const float ref = top == -INFINITY ? 0.f : top;
     float sum = 0.f;
     for (int u = 0; u < 32; ++u) sum += sm[u][x].y * ex2(sm[u][x].x - ref);
-    const float l = (ref + log2f(sum)) * kLn2;
+    // back from base 2 by what the logits were scaled with; in 64 bits, so that a small loss, the difference of
+    // two large numbers, has no more of their rounding than v has
+    const double high = scale == 0.f ? 0.0 : static_cast<double>(ref) * (fabs(static_cast<double>(scale)) / stats_scale(scale));
+    const double rest = static_cast<double>(logf(sum));
     const int64_t id = ids[t];
-    const float v = id >= 0 && id < vocab ? l - target[t] : 0.f;
-    lse[t] = l;
-    each[t] = v;
+    lse[t] = static_cast<float>(high + rest);
+    each[t] = id >= 0 && id < vocab
+                  ? static_cast<float>((high - static_cast<double>(target[t]) * static_cast<double>(scale)) + rest)
+                  : 0.f;
   }
   if (reduction == kNone) return;
   __threadfence();
@@ -853,9 +863,11 @@ int group_rows(int64_t tiles_m, int64_t k) {
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(tiles_m, (32LL << 20) / (kPairTileM * 2 * std::max<int64_t>(k, 64)))));
 }
 
-// Stages of a segment.  Logits: 512 k, so that lse and losses are as exact as fp32 sums (7e-7 of a
-// logit at worst).  The gradients are rounded to 16 bits: 4096 k leave 1e-5.
-constexpr int kSegLogits = 8, kSegGrads = 64;
+// Stages of a segment.  A loss is the difference of lse and a logit, a fraction of either: 256 k of a logit, and 128
+// for few tokens, which wait for the table all the same, leave a loss about as exact as fp32 products do (512 k: 3.5e-6 of the
+// loss of a single token, which is rarely averaged out; many tokens 3 % faster).  Logits formed again for G: 512 k.
+// The gradients are rounded to 16 bits: 4096 k leave 1e-5.
+constexpr int kSegLogits = 4, kSegFew = 2, kSegAgain = 8, kSegGrads = 64;
 
 PairShape shape_of(int64_t rows, int64_t cols, int64_t k, int seg, int splits = 1) {
   PairShape s;
@@ -914,7 +926,7 @@ kairo_status run_loss(Problem p, float* loss, float* lse, uint8_t* ws, unsigned*
   if (st) return st;
   int slots;
   if (few) {
-    PairShape sh = shape_of(p.vocab, 1, p.dim, kSegLogits);
+    PairShape sh = shape_of(p.vocab, 1, p.dim, kSegFew);
     sh.copies = static_cast<int>(copies);
     sh.copy_rows = tokens;
     slots = 8 * pair_clusters(sh.tiles_m);
@@ -933,7 +945,7 @@ kairo_status run_loss(Problem p, float* loss, float* lse, uint8_t* ws, unsigned*
   }
   if (st) return st;
   k_lse<<<static_cast<int>(ceil_div64(p.tokens, 32)), 1024, 0, s>>>(
-      part, slots, target, p.ids, tokens, vocab, p.reduction,
+      part, slots, target, p.ids, tokens, vocab, p.scale, p.reduction,
       p.reduction == kNone ? loss : reinterpret_cast<float*>(ws + o.each), lse, loss, ticket);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "launch of k_lse");
@@ -972,7 +984,7 @@ kairo_status run_grad(Problem p, const float* grad, const float* lse, const Resu
     if (st) return st;
     typename GradEpi<T>::Args ga{g, o.cols, lse, f, p.ids, static_cast<int>(p.tokens), static_cast<int>(p.vocab),
                                  static_cast<int>(v0), p.scale};
-    st = launch_pair_gemm<FMT, false, false, GradEpi<T>>(mx, mw, shape_of(p.tokens, n, p.dim, kSegLogits), err, ga, s);
+    st = launch_pair_gemm<FMT, false, false, GradEpi<T>>(mx, mw, shape_of(p.tokens, n, p.dim, kSegAgain), err, ga, s);
     if (st) return st;
     if (dx) {
       // a last piece of few columns has fewer parts than the others: those it leaves out keep their sums
