@@ -24,7 +24,7 @@
 //
 // Measured.  8192 tokens, 131072 x 2048, bf16: the forward pass 3.1 ms (1400 TFLOP/s), G 3.4, dX 3.0, dW 3.0
 // (1465) one after the other from a cool start; in a row 13.7 ms, 1280 TFLOP/s of what is done, where the power
-// limit leaves cuBLAS 1355.  One to 64 tokens of 131072 x 4096: 185 to 190 us, 5.6 to 5.8 TB/s.
+// limit leaves cuBLAS 1355.  One to 64 tokens of 131072 x 4096: 190 to 200 us, 5.4 to 5.6 TB/s.
 //
 // Rounding.  z, the maxima, sums and lse are fp32.  G is rounded once to the
 // operands' 16 bits, as an operand of both products must be: relative to each
@@ -863,11 +863,12 @@ int group_rows(int64_t tiles_m, int64_t k) {
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(tiles_m, (32LL << 20) / (kPairTileM * 2 * std::max<int64_t>(k, 64)))));
 }
 
-// Stages of a segment.  A loss is the difference of lse and a logit, a fraction of either: 256 k of a logit, and 128
-// for few tokens, which wait for the table all the same, leave a loss about as exact as fp32 products do (512 k: 3.5e-6 of the
-// loss of a single token, which is rarely averaged out; many tokens 3 % faster).  Logits formed again for G: 512 k.
-// The gradients are rounded to 16 bits: 4096 k leave 1e-5.
-constexpr int kSegLogits = 4, kSegFew = 2, kSegAgain = 8, kSegGrads = 64;
+// Stages of a segment.  A loss is the difference of lse and a logit, a fraction of either: 384 k of a logit, and 128 or
+// 256 for up to 64 or 128 tokens, which wait for the table all the same, leave a loss about as exact as fp32 products do
+// (512 k: 3.5e-6 of the loss of a single token, which is rarely averaged out; 64 k: 64 tokens of 131072 x 4096 241 us
+// instead of 197; 256 k: 1024 tokens 824 us, 512 k: 750).  Logits formed again for G: 512 k.  The gradients are
+// rounded to 16 bits: 4096 k leave 1e-5.
+constexpr int kSegLogits = 6, kSegFew = 2, kSegAgain = 8, kSegGrads = 64;
 
 PairShape shape_of(int64_t rows, int64_t cols, int64_t k, int seg, int splits = 1) {
   PairShape s;
@@ -926,7 +927,7 @@ kairo_status run_loss(Problem p, float* loss, float* lse, uint8_t* ws, unsigned*
   if (st) return st;
   int slots;
   if (few) {
-    PairShape sh = shape_of(p.vocab, 1, p.dim, kSegFew);
+    PairShape sh = shape_of(p.vocab, 1, p.dim, half ? kSegFew : 2 * kSegFew);
     sh.copies = static_cast<int>(copies);
     sh.copy_rows = tokens;
     slots = 8 * pair_clusters(sh.tiles_m);
