@@ -30,6 +30,15 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
+// A thread that has made no call of the runtime that needs a context (a new one, or autograd's, whose first call
+// this may be) has none, and the driver refuses to encode: it then gets its device's, the one that the launch takes.
+template <class... Args>
+CUresult encode(EncodeTiledFn fn, Args... args) {
+  const CUresult r = fn(args...);
+  if (r != CUDA_ERROR_INVALID_CONTEXT) return r;
+  return cudaSetDevice(current_device()) == cudaSuccess ? fn(args...) : r;
+}
+
 CUtensorMapSwizzle swizzle_for_bytes(int inner_bytes) {
   return inner_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
          : inner_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
@@ -47,7 +56,7 @@ kairo_status make_map_2d(CUtensorMap* map, const void* base, CUtensorMapDataType
   const cuuint64_t strides[1] = {row_stride_elems * static_cast<uint64_t>(elem_bytes)};
   const cuuint32_t box[2] = {box_inner, box_outer};
   const cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  CUresult r = encode(fn, map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   swizzle_for_bytes(static_cast<int>(box_inner) * elem_bytes), CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
@@ -66,7 +75,7 @@ kairo_status make_map_b3d(CUtensorMap* map, const void* base, CUtensorMapDataTyp
   const cuuint64_t strides[2] = {ldb * 2, 128};
   const cuuint32_t box[3] = {64, bk, atoms};
   const cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = fn(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  CUresult r = encode(fn, map, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     std::ostringstream os;
