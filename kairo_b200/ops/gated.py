@@ -125,7 +125,8 @@ class GatedWeights:
 
 
 class _Structure:
-    """The stacked matrix transposed (structure only), descriptors and workspace sizes of the backward products."""
+    """The stacked matrix transposed (structure only), descriptors and workspace sizes of the backward products.
+    It serves values of both types: a descriptor's type and blocks are those of the call (``_with_blocks``)."""
 
     def __init__(self, w: GatedWeights) -> None:
         a = w.stacked()
@@ -137,7 +138,7 @@ class _Structure:
         self.desc_t = _bsr_desc(t.matrix)
         self.desc_w = _bsr_desc(BlockSparseMatrix(row_ptr=w.row_ptr, col_idx=w.stored_col, blocks=w.blocks,
                                                   shape=a.shape, block_size=a.block_size))
-        self.spmm_bytes: dict[int, int] = {}  # by tokens
+        self.spmm_bytes: dict[tuple[int, torch.dtype], int] = {}  # by tokens and type
         self.rows_t, self.longest_t = t.matrix.nbr, t.matrix.max_row_blocks
         nbytes = ctypes.c_size_t(0)
         _lib.check(_lib.lib().kairo_bsr_sddmm_workspace_size(ctypes.byref(self.desc_w), ctypes.byref(nbytes)), "sddmm")
@@ -163,7 +164,7 @@ _BANDS_256 = KernelConfig(schedule="bands", band_rows=1, n_tile=256).to_c()
 
 def _with_blocks(desc: _lib.KairoBsr, blocks: Tensor) -> _lib.KairoBsr:
     d = _lib.KairoBsr.from_buffer_copy(desc)
-    d.blocks = blocks.data_ptr()
+    d.blocks, d.dtype = blocks.data_ptr(), _lib.kairo_dtype(blocks.dtype)
     return d
 
 
@@ -326,7 +327,7 @@ def sparse_gated_linear_backward(dH: Tensor, X: Tensor, weights: GatedWeights, *
                     st.kept[2].data_ptr(), blocks_t.data_ptr(), scratch.data_ptr(), 256)
         desc_t, cfg = _with_blocks(st.desc_t, blocks_t), st.config(nnzb, n)
         dX = x.new_empty((n, k))
-        size = st.spmm_bytes.get(n)
+        size = st.spmm_bytes.get((n, x.dtype))
         if size is None:
             nbytes = ctypes.c_size_t(0)
             with torch.cuda.device(index):
@@ -334,7 +335,7 @@ def sparse_gated_linear_backward(dH: Tensor, X: Tensor, weights: GatedWeights, *
                                                              ctypes.byref(cfg), ctypes.byref(nbytes)), op)
             size = nbytes.value
             if len(st.spmm_bytes) < 4096:
-                st.spmm_bytes[n] = size
+                st.spmm_bytes[n, x.dtype] = size
         if torch.cuda.is_current_stream_capturing():
             # a graph's own: two captured graphs may replay at the same time
             ws = x.new_empty(size, dtype=torch.uint8)

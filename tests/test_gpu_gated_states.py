@@ -1,0 +1,65 @@
+"""Gated projection: weights whose values, streams, modules or patterns change between calls, against the
+same call with weights that were never used before.  Equal inputs give equal bits, so most of it is compared exactly."""
+
+from __future__ import annotations
+
+import copy
+import io
+from dataclasses import fields, replace
+
+import pytest
+import torch
+
+from kairo_b200 import _lib, ops
+from kairo_b200.ops import gated as gated_module
+from tests.test_gpu_gated import case, weight
+
+pytestmark = pytest.mark.gpu
+TYPES = [(torch.bfloat16, torch.float16), (torch.float16, torch.bfloat16)]
+
+
+def fresh(w):
+    """The same weights without anything kept."""
+    return replace(w, _structure={})
+
+
+def step(layer, x, dh):
+    """(output, dX, gradients of the parameters) of one training step."""
+    for p in layer.parameters():
+        p.grad = None
+    xr = x.clone().requires_grad_(True)
+    y = layer(xr)
+    y.backward(dh)
+    return [y.detach(), xr.grad, *(p.grad.clone() for p in layer.parameters())]
+
+
+def same(a, b):
+    assert len(a) == len(b)
+    for p, q in zip(a, b):
+        assert p.dtype == q.dtype and torch.equal(p, q)
+
+
+@pytest.mark.parametrize("b", [64, 32])
+@pytest.mark.parametrize("first,then", TYPES)
+def test_values_of_the_other_type(first, then, b):
+    """A backward pass in one 16-bit type, then the same patterns with values of the other."""
+    x, dh, gate, up, wg, wu = case(300, 200, 136, b, first)
+    w = ops.gated_weights(gate, up)
+    ops.sparse_gated_linear_backward(dh, x, w, check=True)
+    w2, x2, dh2 = w.with_blocks(w.blocks.to(then)), x.to(then), dh.to(then)
+    for how in ({}, {"need_dx": False, "dw_dtype": torch.float32}, {"need_dw": False}):
+        got = ops.sparse_gated_linear_backward(dh2, x2, w2, check=True, **how)
+        want = ops.sparse_gated_linear_backward(dh2, x2, fresh(w2), check=True, **how)
+        same([t for t in got if t is not None], [t for t in want if t is not None])
+    # and back
+    same(ops.sparse_gated_linear_backward(dh, x, w), ops.sparse_gated_linear_backward(dh, x, fresh(w)))
+
+
+@pytest.mark.parametrize("first,then", TYPES)
+def test_module_cast_after_a_step(first, then):
+    x, dh, gate, up, wg, wu = case(70, 96, 96, 32, first)
+    layer = ops.SparseGatedLinear(gate, up)
+    step(layer, x, dh)
+    layer.to(then)
+    other = ops.SparseGatedLinear(gate, up).to(then)
+    same(step(layer, x.to(then), dh.to(then)), step(other, x.to(then), dh.to(then)))
