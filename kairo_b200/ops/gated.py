@@ -134,6 +134,8 @@ class _Structure:
         self.kept = (t.matrix.row_ptr, t.matrix.col_idx, t.perm, w.row_ptr, w.col_idx, w.blk_idx, w.stored_col)
         # positions of the transposed structure name stored blocks, so that the weight gradient lands in the blocks' own order
         self.perm_stored = w.blk_idx[t.perm.long()] if a.nnzb else t.perm
+        # the next call to find the structure may be on another stream
+        torch.cuda.current_stream(w.device).synchronize()
         self.desc = _bsr_desc(a)
         self.desc_t = _bsr_desc(t.matrix)
         self.desc_w = _bsr_desc(BlockSparseMatrix(row_ptr=w.row_ptr, col_idx=w.stored_col, blocks=w.blocks,

@@ -63,3 +63,27 @@ def test_module_cast_after_a_step(first, then):
     layer.to(then)
     other = ops.SparseGatedLinear(gate, up).to(then)
     same(step(layer, x.to(then), dh.to(then)), step(other, x.to(then), dh.to(then)))
+
+
+def test_first_backward_on_two_streams(monkeypatch):
+    """The kept structure is there before another stream finds it, however long its stream is behind."""
+    x, dh, gate, up, wg, wu = case(300, 320, 320, 64, torch.bfloat16)
+    w = ops.gated_weights(gate, up)
+    want = ops.sparse_gated_linear_backward(dh, x, fresh(w), check=True)
+    real = gated_module.bsr_transpose
+
+    def behind(*args, **kw):
+        out = real(*args, **kw)
+        torch.cuda._sleep(200_000_000)  # what follows on this stream waits about 0.1 s
+        return out
+
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    monkeypatch.setattr(gated_module, "bsr_transpose", behind)
+    with torch.cuda.stream(a):
+        got_a = ops.sparse_gated_linear_backward(dh, x, w)
+    with torch.cuda.stream(b):
+        got_b = ops.sparse_gated_linear_backward(dh, x, w)
+    torch.cuda.synchronize()
+    same(got_a, want)
+    same(got_b, want)
