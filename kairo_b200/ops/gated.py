@@ -135,7 +135,9 @@ class _Structure:
         # positions of the transposed structure name stored blocks, so that the weight gradient lands in the blocks' own order
         self.perm_stored = w.blk_idx[t.perm.long()] if a.nnzb else t.perm
         # the next call to find the structure may be on another stream
-        torch.cuda.current_stream(w.device).synchronize()
+        stream = torch.cuda.current_stream(w.device)
+        stream.synchronize()
+        self.streams = {stream.cuda_stream}
         self.desc = _bsr_desc(a)
         self.desc_t = _bsr_desc(t.matrix)
         self.desc_w = _bsr_desc(BlockSparseMatrix(row_ptr=w.row_ptr, col_idx=w.stored_col, blocks=w.blocks,
@@ -145,6 +147,19 @@ class _Structure:
         nbytes = ctypes.c_size_t(0)
         _lib.check(_lib.lib().kairo_bsr_sddmm_workspace_size(ctypes.byref(self.desc_w), ctypes.byref(nbytes)), "sddmm")
         self.sddmm_bytes = max(nbytes.value, 256)
+
+    def used_on_current_stream(self, index: int) -> None:
+        """Before a call's launches: memory that only this object names must outlive them.  Work of another stream
+        than the one it was made on is recorded with the allocator; a captured graph may replay at any time, whatever
+        has become of the weights, so what it reads is kept for good."""
+        raw = torch._C._cuda_getCurrentRawStream(index)
+        if raw not in self.streams:
+            stream = torch.cuda.current_stream(index)
+            for t in (*self.kept, self.perm_stored):
+                t.record_stream(stream)
+            self.streams.add(raw)
+        if torch.cuda.is_current_stream_capturing() and self not in _CAPTURED:
+            _CAPTURED.append(self)
 
     def config(self, nnzb: int, tokens: int) -> _lib.KairoSpmmConfig:
         """Schedule of dP times the stacked weight.  Whole block-rows per CTA (bands of one) beat the row-split
@@ -158,6 +173,7 @@ class _Structure:
         return _BANDS_128 if self.rows_t * -(-tokens // 256) < 148 else _BANDS_256
 
 
+_CAPTURED: list[_Structure] = []
 _ZEROED = 256 + 2 * 16384 * 4  # header and arrival counters of an SpMM workspace, zero before its first launch
 _AUTO = KernelConfig().to_c()
 _BANDS_128 = KernelConfig(schedule="bands", band_rows=1, n_tile=128).to_c()
@@ -321,6 +337,7 @@ def sparse_gated_linear_backward(dH: Tensor, X: Tensor, weights: GatedWeights, *
         return dX, weights.blocks.new_zeros(weights.blocks.shape, dtype=dwt) if need_dw else None
     lib = _lib.lib()
     st = weights._backward_structure()
+    st.used_on_current_stream(index)
     if need_dx:
         # the transposed weight's values are of this call alone: the structure serves calls on several streams
         blocks_t = weights.blocks.new_empty((nnzb, b, b))

@@ -87,3 +87,55 @@ def test_first_backward_on_two_streams(monkeypatch):
     torch.cuda.synchronize()
     same(got_a, want)
     same(got_b, want)
+
+
+def tensors_of(w):
+    return [getattr(w, f.name) for f in fields(w) if isinstance(getattr(w, f.name), torch.Tensor)]
+
+
+def refill(structure_sizes):
+    """Takes memory that was given back on the current stream, and overwrites it with numbers that are no index."""
+    return [torch.full((n,), -1, dtype=torch.int32, device="cuda") for n in structure_sizes for _ in range(8)]
+
+
+def test_structure_freed_while_another_stream_uses_it():
+    x, dh, gate, up, wg, wu = case(300, 320, 320, 64, torch.bfloat16)
+    w = ops.gated_weights(gate, up)
+    want = ops.sparse_gated_linear_backward(dh, x, w, check=True)  # made on this stream
+    sizes = [t.numel() for t in w._backward_structure().kept] + [w._backward_structure().perm_stored.numel()]
+    b = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(b):
+        torch.cuda._sleep(200_000_000)
+        got = ops.sparse_gated_linear_backward(dh, x, w)
+    for t in tensors_of(w):
+        t.record_stream(b)  # the caller's own tensors
+    del w
+    kept = refill(sizes)
+    torch.cuda.synchronize()
+    same(got, want)
+    del kept
+
+
+def test_structure_of_a_captured_pass_is_kept():
+    """A graph of a training step goes on when its layer's patterns have been loaded again."""
+    x, dh, gate, up, wg, wu = case(40, 320, 320, 64, torch.bfloat16)
+    layer = ops.SparseGatedLinear(gate, up)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        want = ops.sparse_gated_linear_backward(dh, x, layer.weights(), check=True)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        got = ops.sparse_gated_linear_backward(dh, x, layer.weights())
+    st = layer.weights()._backward_structure()
+    sizes = [t.numel() for t in st.kept] + [st.perm_stored.numel()]
+    del st
+    layer.load_state_dict(layer.state_dict())
+    with torch.no_grad():
+        layer(x)
+    kept = refill(sizes)
+    g.replay()
+    torch.cuda.synchronize()
+    same(got, want)
+    del kept
