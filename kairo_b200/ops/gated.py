@@ -85,6 +85,14 @@ class GatedWeights:
     def device(self) -> torch.device:
         return self.blocks.device
 
+    # copied and pickled as tensors and numbers; the descriptor names this object's memory, and the structure is made again
+    def __getstate__(self) -> dict:
+        return {k: v for k, v in self.__dict__.items() if k not in ("_desc", "_structure")}
+
+    def __setstate__(self, state: dict) -> None:
+        self.__dict__.update(state, _structure={})
+        self.__post_init__()
+
     def with_blocks(self, blocks: Tensor) -> "GatedWeights":
         """The same patterns with other values."""
         return replace(self, blocks=blocks)
@@ -416,16 +424,24 @@ class SparseGatedLinear(torch.nn.Module):
             self.register_buffer(name, getattr(w, name))
         self._made: tuple = ((), (), {})
 
+    def __getstate__(self) -> dict:
+        # a copy makes its own structure: this one's descriptors name this layer's memory
+        return {**self.__dict__, "_made": ((), (), {})}
+
     def weights(self, blocks: Tensor | None = None) -> GatedWeights:
         b = (self.blocks if blocks is None else blocks).detach()
         parts = (self.ent_ptr, self.entries, self.row_ptr, self.col_idx, self.blk_idx, self.stored_col)
-        # the patterns' transposed structure is kept until a buffer is replaced or written (load_state_dict)
-        versions = tuple(p._version for p in parts)
-        if self._made[1] != versions or any(p is not q for p, q in zip(self._made[0], parts)):
-            self._made = (parts, versions, {})
+        # the patterns' transposed structure is kept until a buffer is replaced or written (load_state_dict);
+        # writes of inference tensors are not counted, so nothing is kept for them
+        structure: dict = {}
+        if not any(p.is_inference() for p in parts):
+            versions = tuple(p._version for p in parts)
+            if self._made[1] != versions or any(p is not q for p, q in zip(self._made[0], parts)):
+                self._made = (parts, versions, structure)
+            structure = self._made[2]
         return GatedWeights(blocks=b, gate_blocks=self.gate_blocks, shape=self.shape, block=self.block,
                             ent_ptr=parts[0], entries=parts[1], row_ptr=parts[2], col_idx=parts[3], blk_idx=parts[4],
-                            stored_col=parts[5], _structure=self._made[2])
+                            stored_col=parts[5], _structure=structure)
 
     def forward(self, X: Tensor) -> Tensor:
         if not torch.is_grad_enabled():

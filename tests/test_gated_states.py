@@ -2,6 +2,9 @@
 
 from __future__ import annotations
 
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -20,3 +23,23 @@ def test_kept_descriptors_take_the_type_of_the_call(first, then):
     d = gated_module._with_blocks(kept, blocks)
     assert d.dtype == _lib.kairo_dtype(then) and d.blocks == blocks.data_ptr() and d.nnzb == 1
     assert kept.dtype == _lib.kairo_dtype(first)
+
+
+def some_weights(dtype=torch.bfloat16):
+    i32 = torch.int32
+    return gated_module.GatedWeights(
+        blocks=torch.arange(512, dtype=torch.float32).view(2, 16, 16).to(dtype), gate_blocks=1, shape=(16, 16), block=16,
+        ent_ptr=torch.tensor([0, 1], dtype=i32), entries=torch.tensor([[0, 0, 1, 0]], dtype=i32),
+        row_ptr=torch.tensor([0, 1, 2], dtype=i32), col_idx=torch.zeros(2, dtype=i32),
+        blk_idx=torch.tensor([0, 1], dtype=i32), stored_col=torch.zeros(2, dtype=i32))
+
+
+def test_weights_are_copied_without_what_names_their_memory():
+    w = some_weights()
+    w._structure["backward"] = w._desc  # a descriptor with pointers, as the kept structure has
+    for other in (copy.deepcopy(w), pickle.loads(pickle.dumps(w))):
+        assert other._structure == {} and other.gate_blocks == 1 and other.shape == (16, 16)
+        assert torch.equal(other.blocks, w.blocks) and other.blocks.data_ptr() != w.blocks.data_ptr()
+        assert other._desc.blocks == other.blocks.data_ptr() and other._desc.entries == other.entries.data_ptr()
+    with pytest.raises(AttributeError):
+        other.block = 32  # frozen, like the original

@@ -139,3 +139,55 @@ def test_structure_of_a_captured_pass_is_kept():
     torch.cuda.synchronize()
     same(got, want)
     del kept
+
+
+def copies(layer):
+    """The layer, copied in memory and through a file."""
+    buf = io.BytesIO()
+    torch.save(layer, buf)
+    buf.seek(0)
+    return copy.deepcopy(layer), torch.load(buf, weights_only=False)
+
+
+def test_copies_of_a_trained_module():
+    x, dh, gate, up, wg, wu = case(70, 96, 96, 32, torch.bfloat16)
+    down, _, _ = weight(96, 96, 32, 0.5, torch.bfloat16, torch.Generator(device="cuda").manual_seed(7))
+    for layer in (ops.SparseGatedLinear(gate, up, activation="gelu"), ops.SparseFeedForward(gate, up, down)):
+        want = step(layer, x, dh)
+        for other in copies(layer):
+            same(step(other, x, dh), want)
+            with torch.no_grad():
+                for p in other.parameters():
+                    p.mul_(2)
+            twice = step(other, x, dh)
+            assert not torch.equal(twice[0], want[0])
+            same(step(layer, x, dh), want)  # the copies have tensors of their own
+
+
+def test_copies_of_weights():
+    x, dh, gate, up, wg, wu = case(70, 96, 96, 32, torch.float16)
+    w = ops.gated_weights(gate, up)
+    want = [ops.sparse_gated_linear(x, w), *ops.sparse_gated_linear_backward(dh, x, w)]
+    for other in copies(w):
+        assert other.blocks.data_ptr() != w.blocks.data_ptr()
+        same([ops.sparse_gated_linear(x, other, check=True), *ops.sparse_gated_linear_backward(dh, x, other, check=True)], want)
+
+
+def test_layer_made_in_inference_mode():
+    x, dh, gate, up, wg, wu = case(40, 96, 96, 32, torch.bfloat16)
+    want = [ops.sparse_gated_linear(x, ops.gated_weights(gate, up)),
+            *ops.sparse_gated_linear_backward(dh, x, ops.gated_weights(gate, up))]
+    with torch.inference_mode():
+        layer = ops.SparseGatedLinear(gate, up)
+        got = [layer(x), *ops.sparse_gated_linear_backward(dh, x, layer.weights())]
+    same(got, want)
+    with torch.no_grad():
+        same([layer(x)], want[:1])
+    # another pattern written over the buffers, whose writes are not counted: nothing is kept from the first
+    gate2, up2 = (weight(96, 96, 32, 0.4, torch.bfloat16, torch.Generator(device="cuda"), pos=p)[0]
+                  for p in (torch.randperm(9, device="cuda")[:m.nnzb] for m in (gate, up)))
+    with torch.inference_mode():
+        other = ops.SparseGatedLinear(gate2, up2)
+        layer.load_state_dict(other.state_dict())
+        same(ops.sparse_gated_linear_backward(dh, x, layer.weights()),
+             ops.sparse_gated_linear_backward(dh, x, other.weights()))
