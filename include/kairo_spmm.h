@@ -671,6 +671,12 @@ KAIRO_API kairo_status kairo_partition_rows(const int64_t* row_ptr, int32_t nbr,
 KAIRO_API kairo_status kairo_workspace_error(void* workspace, int32_t clear, uint32_t* code,
                                    void* stream);
 
+/* `*count` error words of the current device, for operators that take an
+ * error_word and for captured graphs: 256 bytes apart from `*words` on, zero
+ * when the library is loaded, there until it is unloaded.  The caller shares
+ * them out; nothing is launched, so the call may stand in a stream capture. */
+KAIRO_API kairo_status kairo_error_words(void** words, int32_t* count);
+
 KAIRO_API const char* kairo_status_string(kairo_status s);
 KAIRO_API const char* kairo_last_error_message(void);
 KAIRO_API int32_t kairo_abi_version(void);

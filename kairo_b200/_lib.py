@@ -276,6 +276,7 @@ _SIGNATURES = {
                                                         c_int32, POINTER(c_size_t)]),
     "kairo_partition_rows": (c_int32, [POINTER(c_int64), c_int32, c_int32, POINTER(c_int32)]),
     "kairo_workspace_error": (c_int32, [c_void_p, c_int32, POINTER(c_uint32), c_void_p]),
+    "kairo_error_words": (c_int32, [POINTER(c_void_p), POINTER(c_int32)]),
     "kairo_status_string": (c_char_p, [c_int32]),
     "kairo_last_error_message": (c_char_p, []),
     "kairo_abi_version": (c_int32, []),
@@ -412,22 +413,47 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
         return buf
 
 
-_error_words: dict[tuple[int, int], torch.Tensor] = {}
+class ErrorWord:
+    """256 bytes of the library's own memory on ``device``, whose first word takes device errors."""
+
+    __slots__ = ("device", "_at")
+
+    def __init__(self, device: torch.device, at: int) -> None:
+        self.device = device
+        self._at = at
+
+    def data_ptr(self) -> int:
+        return self._at
 
 
-def error_word(index: int) -> torch.Tensor:
-    """The 256 zero-initialised bytes whose first word takes the device errors
-    of operators on the current stream of device ``index`` that bring their own
-    workspace to every call.  Kept for good: captured graphs may write it."""
-    key = (index, torch._C._cuda_getCurrentRawStream(index))
-    word = _error_words.get(key)
-    if word is None:
-        with _ws_lock:
-            word = _error_words.get(key)
-            if word is None:
-                word = torch.zeros(256, dtype=torch.uint8, device=torch.device("cuda", index))
-                _error_words[key] = word
-    return word
+_error_words: dict[tuple[int, int | None], ErrorWord] = {}
+
+
+def error_word(index: int) -> ErrorWord:
+    """The word that takes the device errors of operators that bring their own
+    workspace to every call: the current stream's of device ``index`` or, in a
+    capture, one that all captured graphs of the device share, as they may
+    replay on any stream.  The words are memory of the library: neither their
+    allocation nor their zeros can become part of a graph."""
+    if torch.cuda.is_current_stream_capturing():
+        return _error_words.get((index, None)) or _error_word_of(index, None)
+    raw = torch._C._cuda_getCurrentRawStream(index)
+    return _error_words.get((index, raw)) or _error_word_of(index, raw)
+
+
+def _error_word_of(index: int, raw: int | None) -> ErrorWord:
+    """The word of stream ``raw``, or of captures (None).  More streams than there are words share the last one."""
+    with _ws_lock:
+        word = _error_words.get((index, raw))
+        if word is None:
+            words, count = c_void_p(None), c_int32(0)
+            with torch.cuda.device(index):
+                check(lib().kairo_error_words(ctypes.byref(words), ctypes.byref(count)), "kairo_error_words")
+            # the first is the captures'
+            slot = 0 if raw is None else 1 + sum(1 for i, r in _error_words if i == index and r is not None)
+            word = ErrorWord(torch.device("cuda", index), words.value + 256 * min(slot, count.value - 1))
+            _error_words[index, raw] = word
+        return word
 
 
 def read_workspace_error(ws: torch.Tensor, clear: bool = True) -> int:
@@ -464,10 +490,12 @@ def take_pending_error(ws: torch.Tensor, where: str) -> int:
 
 
 def pending_device_error(device: torch.device | int | None = None, clear: bool = True) -> int:
-    """The device error word of the cached workspace of ``device``'s current
-    stream: what launches made with ``check=False`` there have recorded
-    since it was last read (KAIRO_DEVERR_* in the low 8 bits, the wait site
-    above them; 0 = none).  Synchronises that stream."""
+    """The device error words of ``device``'s current stream: what launches
+    made with ``check=False`` there have recorded since they were last read,
+    and what replays of captured graphs, on any stream, have recorded of the
+    operators that bring their own workspace (KAIRO_DEVERR_* in the low 8 bits,
+    the wait site above them; 0 = none; the first of several).  Synchronises
+    that stream."""
     if device is None:
         dev = torch.device("cuda", torch.cuda.current_device())
     elif isinstance(device, int):
@@ -475,8 +503,10 @@ def pending_device_error(device: torch.device | int | None = None, clear: bool =
     else:
         dev = torch.device(device)
     code = read_workspace_error(workspace(0, dev), clear=clear)
-    word = _error_words.get((dev.index if dev.index is not None else torch.cuda.current_device(),
-                             torch.cuda.current_stream(dev).cuda_stream))
-    if word is not None and (code == 0 or clear):
-        code = code or read_workspace_error(word, clear=clear)
+    index = dev.index if dev.index is not None else torch.cuda.current_device()
+    for raw in (torch.cuda.current_stream(dev).cuda_stream, None):
+        word = _error_words.get((index, raw))
+        if word is not None and (code == 0 or clear):
+            found = read_workspace_error(word, clear=clear)
+            code = code or found
     return code

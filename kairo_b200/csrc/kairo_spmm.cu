@@ -18,6 +18,10 @@ namespace {
 thread_local std::string g_last_error;
 }
 
+// kairo_error_words: memory of the module, so that no allocation or fill is needed that a capture could take in.
+constexpr int kErrorWords = 512;
+__device__ unsigned g_error_words[kErrorWords][64];
+
 void set_error(const std::string& msg) { g_last_error = msg; }
 
 kairo_status fail(kairo_status s, const std::string& msg) {
@@ -465,6 +469,21 @@ kairo_status kairo_workspace_error(void* workspace, int32_t clear, uint32_t* cod
   if (e == cudaSuccess) e = cudaStreamSynchronize(s);
   if (e != cudaSuccess) return cuda_fail(e, "reading the workspace error word");
   *code = v;
+  return KAIRO_STATUS_SUCCESS;
+}
+
+kairo_status kairo_error_words(void** words, int32_t* count) {
+  if (!words || !count) return fail(KAIRO_STATUS_INVALID_VALUE, "null argument");
+  // the first reference to the module's memory may load it: never part of another stream's capture
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e == cudaSuccess) {
+    e = cudaGetSymbolAddress(words, g_error_words);
+    const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e == cudaSuccess) e = back;
+  }
+  if (e != cudaSuccess) return cuda_fail(e, "address of the error words");
+  *count = kErrorWords;
   return KAIRO_STATUS_SUCCESS;
 }
 

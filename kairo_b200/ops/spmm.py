@@ -101,7 +101,8 @@ class KernelConfig:
 
 def pending_device_error(device: torch.device | int | None = None, clear: bool = True) -> int:
     """Device error word left by ``check=False`` launches on ``device``'s
-    current stream (0 = none; KAIRO_DEVERR_* in the low 8 bits, the wait
+    current stream, or by replays of captured graphs with operators that bring
+    their own workspace (0 = none; KAIRO_DEVERR_* in the low 8 bits, the wait
     site above).  Synchronises that stream; ``clear`` resets the word."""
     return _lib.pending_device_error(device, clear)
 

@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import copy
+import ctypes
 import pickle
 
 import pytest
@@ -43,3 +44,9 @@ def test_weights_are_copied_without_what_names_their_memory():
         assert other._desc.blocks == other.blocks.data_ptr() and other._desc.entries == other.entries.data_ptr()
     with pytest.raises(AttributeError):
         other.block = 32  # frozen, like the original
+
+
+def test_error_words_of_the_library():
+    n, at = ctypes.c_int32(0), ctypes.c_void_p(None)
+    assert _lib.lib().kairo_error_words(None, ctypes.byref(n)) == _lib.INVALID_VALUE
+    assert _lib.lib().kairo_error_words(ctypes.byref(at), None) == _lib.INVALID_VALUE
