@@ -184,8 +184,12 @@ def test_layer_made_in_inference_mode():
     with torch.no_grad():
         same([layer(x)], want[:1])
     # another pattern written over the buffers, whose writes are not counted: nothing is kept from the first
-    gate2, up2 = (weight(96, 96, 32, 0.4, torch.bfloat16, torch.Generator(device="cuda"), pos=p)[0]
-                  for p in (torch.randperm(9, device="cuda")[:m.nnzb] for m in (gate, up)))
+    # (both patterns moved alike, so that they have as many entries together)
+    to = torch.tensor([4, 0, 8, 2, 6, 1, 3, 7, 5], device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(4)
+    rows = [torch.repeat_interleave(torch.arange(3, device="cuda"), m.row_ptr.diff().long()) for m in (gate, up)]
+    gate2, up2 = (weight(96, 96, 32, 0.4, torch.bfloat16, g, pos=to[r * 3 + m.col_idx.long()])[0]
+                  for r, m in zip(rows, (gate, up)))
     with torch.inference_mode():
         other = ops.SparseGatedLinear(gate2, up2)
         layer.load_state_dict(other.state_dict())
