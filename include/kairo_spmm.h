@@ -671,6 +671,12 @@ KAIRO_API kairo_status kairo_partition_rows(const int64_t* row_ptr, int32_t nbr,
 KAIRO_API kairo_status kairo_workspace_error(void* workspace, int32_t clear, uint32_t* code,
                                    void* stream);
 
+/* Copies the first error recorded in the headers of `count` (1 to 4) workspaces
+ * to `*error_word` where that holds none: for workspaces that are given back
+ * before anyone has read them.  Asynchronous on `stream`. */
+KAIRO_API kairo_status kairo_collect_errors(const void* const* workspaces, int32_t count, unsigned* error_word,
+                                            void* stream);
+
 /* `*count` error words of the current device, for operators that take an
  * error_word and for captured graphs: 256 bytes apart from `*words` on, zero
  * when the library is loaded, there until it is unloaded.  The caller shares

@@ -276,6 +276,7 @@ _SIGNATURES = {
                                                         c_int32, POINTER(c_size_t)]),
     "kairo_partition_rows": (c_int32, [POINTER(c_int64), c_int32, c_int32, POINTER(c_int32)]),
     "kairo_workspace_error": (c_int32, [c_void_p, c_int32, POINTER(c_uint32), c_void_p]),
+    "kairo_collect_errors": (c_int32, [POINTER(c_void_p), c_int32, c_void_p, c_void_p]),
     "kairo_error_words": (c_int32, [POINTER(c_void_p), POINTER(c_int32)]),
     "kairo_status_string": (c_char_p, [c_int32]),
     "kairo_last_error_message": (c_char_p, []),
@@ -454,6 +455,12 @@ def _error_word_of(index: int, raw: int | None) -> ErrorWord:
             word = ErrorWord(torch.device("cuda", index), words.value + 256 * min(slot, count.value - 1))
             _error_words[index, raw] = word
         return word
+
+
+def collect_errors(op: str, index: int, word: ErrorWord, *workspaces: torch.Tensor) -> None:
+    """What launches on the current stream record in ``workspaces``, which nobody else will read, goes to ``word``."""
+    at = (c_void_p * len(workspaces))(*(w.data_ptr() for w in workspaces))
+    launch(op, lib().kairo_collect_errors, index, at, len(workspaces), word.data_ptr())
 
 
 def read_workspace_error(ws: torch.Tensor, clear: bool = True) -> int:

@@ -22,6 +22,20 @@ thread_local std::string g_last_error;
 constexpr int kErrorWords = 512;
 __device__ unsigned g_error_words[kErrorWords][64];
 
+struct ErrorSources {
+  const unsigned* word[4];
+};
+
+__global__ void k_collect_errors(ErrorSources from, int count, unsigned* err) {
+  for (int i = 0; i < count; ++i) {
+    const unsigned code = *from.word[i];
+    if (code) {
+      atomicCAS(err, 0u, code);
+      return;
+    }
+  }
+}
+
 void set_error(const std::string& msg) { g_last_error = msg; }
 
 kairo_status fail(kairo_status s, const std::string& msg) {
@@ -470,6 +484,18 @@ kairo_status kairo_workspace_error(void* workspace, int32_t clear, uint32_t* cod
   if (e != cudaSuccess) return cuda_fail(e, "reading the workspace error word");
   *code = v;
   return KAIRO_STATUS_SUCCESS;
+}
+
+kairo_status kairo_collect_errors(const void* const* workspaces, int32_t count, unsigned* error_word, void* stream) {
+  if (!workspaces || count < 1 || count > 4 || !error_word) return fail(KAIRO_STATUS_INVALID_VALUE, "invalid argument");
+  ErrorSources from{};
+  for (int i = 0; i < count; ++i) {
+    if (!workspaces[i]) return fail(KAIRO_STATUS_INVALID_VALUE, "null workspace");
+    from.word[i] = static_cast<const unsigned*>(workspaces[i]);
+  }
+  k_collect_errors<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(from, count, error_word);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "launch of k_collect_errors");
 }
 
 kairo_status kairo_error_words(void** words, int32_t* count) {

@@ -314,7 +314,10 @@ def sparse_gated_linear_backward(dH: Tensor, X: Tensor, weights: GatedWeights, *
     ``weights.blocks`` (``weights.split`` gives the two weights' parts).
     Either may be left out (None).
 
-    dG and dU are rounded to the weights' type, as operands of both products."""
+    dG and dU are rounded to the weights' type, as operands of both products.
+    ``check=True`` synchronises and raises KairoDeviceError where one of the
+    kernels met a malformed structure or a wait ran out; without it
+    ``pending_device_error`` tells."""
     op = "sparse_gated_linear_backward"
     index = _lib.device_index(op, dH, X, weights.blocks)
     x, act = _input(op, X, weights, activation)
@@ -346,12 +349,13 @@ def sparse_gated_linear_backward(dH: Tensor, X: Tensor, weights: GatedWeights, *
     lib = _lib.lib()
     st = weights._backward_structure()
     st.used_on_current_stream(index)
+    own: list[Tensor] = []  # workspaces that end with the call
     if need_dx:
         # the transposed weight's values are of this call alone: the structure serves calls on several streams
         blocks_t = weights.blocks.new_empty((nnzb, b, b))
-        scratch = x.new_empty(256, dtype=torch.uint8)
+        # its workspace is an error word and nothing else
         _lib.launch(op, lib.kairo_bsr_transpose_values, index, ctypes.byref(_with_blocks(st.desc, weights.blocks)),
-                    st.kept[2].data_ptr(), blocks_t.data_ptr(), scratch.data_ptr(), 256)
+                    st.kept[2].data_ptr(), blocks_t.data_ptr(), err.data_ptr(), 256)
         desc_t, cfg = _with_blocks(st.desc_t, blocks_t), st.config(nnzb, n)
         dX = x.new_empty((n, k))
         size = st.spmm_bytes.get((n, x.dtype))
@@ -367,6 +371,7 @@ def sparse_gated_linear_backward(dH: Tensor, X: Tensor, weights: GatedWeights, *
             # a graph's own: two captured graphs may replay at the same time
             ws = x.new_empty(size, dtype=torch.uint8)
             ws[:_ZEROED].zero_()
+            own.append(ws)
         else:
             ws = _lib.workspace(size, x.device)
         if check:
@@ -383,8 +388,11 @@ def sparse_gated_linear_backward(dH: Tensor, X: Tensor, weights: GatedWeights, *
                     st.kept[0].data_ptr(), st.kept[1].data_ptr(), st.perm_stored.data_ptr(), dp.data_ptr(), dp.shape[1],
                     x.data_ptr(), max(_ld(x), k), n, d_blocks.data_ptr(), _lib.kairo_dtype(dwt), ws.data_ptr(),
                     ws.numel())
-        if check:
-            _lib.raise_on_device_error(ws)
+        own.append(ws)
+    if own:
+        _lib.collect_errors(op, index, err, *own)
+    if check:
+        _lib.raise_on_device_error(err)
     return dX, d_blocks
 
 

@@ -50,3 +50,13 @@ def test_error_words_of_the_library():
     n, at = ctypes.c_int32(0), ctypes.c_void_p(None)
     assert _lib.lib().kairo_error_words(None, ctypes.byref(n)) == _lib.INVALID_VALUE
     assert _lib.lib().kairo_error_words(ctypes.byref(at), None) == _lib.INVALID_VALUE
+
+
+def test_collect_errors_refusals():
+    some, lib = ctypes.c_void_p(256), _lib.lib()  # never read: each call is refused first
+    two = (ctypes.c_void_p * 2)(256, 256)
+    assert lib.kairo_collect_errors(two, 0, some, None) == _lib.INVALID_VALUE
+    assert lib.kairo_collect_errors(two, 5, some, None) == _lib.INVALID_VALUE
+    assert lib.kairo_collect_errors(two, 2, None, None) == _lib.INVALID_VALUE
+    assert lib.kairo_collect_errors(None, 1, some, None) == _lib.INVALID_VALUE
+    assert lib.kairo_collect_errors((ctypes.c_void_p * 2)(256, None), 2, some, None) == _lib.INVALID_VALUE

@@ -195,3 +195,38 @@ def test_layer_made_in_inference_mode():
         layer.load_state_dict(other.state_dict())
         same(ops.sparse_gated_linear_backward(dh, x, layer.weights()),
              ops.sparse_gated_linear_backward(dh, x, other.weights()))
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("table,how", [(1, {"need_dx": False}), (2, {"need_dw": False}), (1, {"need_dw": False})])
+def test_errors_of_the_backward_products_can_be_read(table, how, captured):
+    """A block-row or position out of range in the kept structure is read nowhere, and recorded where the caller finds it."""
+    x, dh, gate, up, wg, wu = case(200, 320, 320, 64, torch.bfloat16)
+    w = ops.gated_weights(gate, up)
+
+    def call(check=False):
+        return ops.sparse_gated_linear_backward(dh, x, w, check=check, **how)
+
+    call(check=True)
+    ops.pending_device_error()
+    values = w._backward_structure().kept[table]
+    kept = values.clone()
+    if captured:
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            call()
+        values[3] = 1 << 28
+        g.replay()
+    else:
+        values[3] = 1 << 28
+        with pytest.raises(_lib.KairoDeviceError) as e:
+            call(check=True)
+        assert e.value.code & 0xFF == _lib.DEVERR_BAD_INDEX
+        call()
+    assert ops.pending_device_error() & 0xFF == _lib.DEVERR_BAD_INDEX
+    assert ops.pending_device_error() == 0
+    values.copy_(kept)
+    call(check=True)
+    assert ops.pending_device_error() == 0
