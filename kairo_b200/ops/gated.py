@@ -138,7 +138,13 @@ class _Structure:
 
     def __init__(self, w: GatedWeights) -> None:
         a = w.stacked()
-        t = bsr_transpose(a)
+        try:
+            t = bsr_transpose(a, check=True)
+        except _lib.KairoDeviceError as e:
+            if e.code & 0xFF != _lib.DEVERR_ROW_TOO_LONG:
+                raise
+            raise ValueError("sparse_gated_linear_backward: a block-column keeps more than 16384 blocks of gate and up "
+                             "together, more than the transposed structure is sorted for") from e
         self.kept = (t.matrix.row_ptr, t.matrix.col_idx, t.perm, w.row_ptr, w.col_idx, w.blk_idx, w.stored_col)
         # positions of the transposed structure name stored blocks, so that the weight gradient lands in the blocks' own order
         self.perm_stored = w.blk_idx[t.perm.long()] if a.nnzb else t.perm
@@ -315,6 +321,7 @@ def sparse_gated_linear_backward(dH: Tensor, X: Tensor, weights: GatedWeights, *
     Either may be left out (None).
 
     dG and dU are rounded to the weights' type, as operands of both products.
+    A block-column may keep 16384 blocks, gate and up together (ValueError).
     ``check=True`` synchronises and raises KairoDeviceError where one of the
     kernels met a malformed structure or a wait ran out; without it
     ``pending_device_error`` tells."""

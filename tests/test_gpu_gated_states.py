@@ -230,3 +230,21 @@ def test_errors_of_the_backward_products_can_be_read(table, how, captured):
     values.copy_(kept)
     call(check=True)
     assert ops.pending_device_error() == 0
+
+
+
+def test_long_block_column_is_refused():
+    """The transposed structure sorts block-columns of up to 16384 stored blocks, gate and up together."""
+    rows, b = 8200, 16
+    pos = torch.arange(rows, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(5)
+    gate, wg, _ = weight(rows * b, b, b, 1.0, torch.bfloat16, g, pos=pos)
+    up, wu, _ = weight(rows * b, b, b, 1.0, torch.bfloat16, g, pos=pos)
+    w = ops.gated_weights(gate, up)
+    x = torch.randn(4, b, generator=g, device="cuda").bfloat16()
+    h = ops.sparse_gated_linear(x, w, check=True)
+    want = torch.nn.functional.silu(x.double() @ wg.t()) * (x.double() @ wu.t())
+    assert (h.double() - want).norm() < 2.0**-8 * want.norm()
+    for _ in range(2):  # nothing is kept of the refused call
+        with pytest.raises(ValueError, match="16384"):
+            ops.sparse_gated_linear_backward(h, x, w)
