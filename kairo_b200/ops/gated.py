@@ -403,19 +403,26 @@ def sparse_gated_linear_backward(dH: Tensor, X: Tensor, weights: GatedWeights, *
     return dX, d_blocks
 
 
+_PATTERN = ("ent_ptr", "entries", "row_ptr", "col_idx", "blk_idx", "stored_col")
+
+
 class _GatedFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, X: Tensor, blocks: Tensor, module: "SparseGatedLinear") -> Tensor:
-        ctx.save_for_backward(X, blocks)
-        ctx.module = module
-        return sparse_gated_linear(X, module.weights(blocks), activation=module.activation)
+        w = module.weights(blocks)
+        # all that the backward pass needs is this call's: the module may have changed by then
+        ctx.save_for_backward(X, blocks, *(getattr(w, name) for name in _PATTERN))
+        ctx.activation = module.activation
+        ctx.weights = {"gate_blocks": w.gate_blocks, "shape": w.shape, "block": w.block, "_structure": w._structure}
+        return sparse_gated_linear(X, w, activation=ctx.activation)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dH: Tensor):
-        X, blocks = ctx.saved_tensors
-        dX, dW = sparse_gated_linear_backward(dH, X, ctx.module.weights(blocks), activation=ctx.module.activation,
-                                              need_dx=ctx.needs_input_grad[0], need_dw=ctx.needs_input_grad[1])
+        X, blocks, *pattern = ctx.saved_tensors
+        w = GatedWeights(blocks=blocks.detach(), **dict(zip(_PATTERN, pattern)), **ctx.weights)
+        dX, dW = sparse_gated_linear_backward(dH, X, w, activation=ctx.activation, need_dx=ctx.needs_input_grad[0],
+                                              need_dw=ctx.needs_input_grad[1])
         return dX, dW, None
 
 
@@ -435,7 +442,7 @@ class SparseGatedLinear(torch.nn.Module):
         self.gate_blocks = w.gate_blocks
         self.block = w.block
         self.blocks = torch.nn.Parameter(w.blocks.detach())
-        for name in ("ent_ptr", "entries", "row_ptr", "col_idx", "blk_idx", "stored_col"):
+        for name in _PATTERN:
             self.register_buffer(name, getattr(w, name))
         self._made: tuple = ((), (), {})
 
@@ -445,7 +452,7 @@ class SparseGatedLinear(torch.nn.Module):
 
     def weights(self, blocks: Tensor | None = None) -> GatedWeights:
         b = (self.blocks if blocks is None else blocks).detach()
-        parts = (self.ent_ptr, self.entries, self.row_ptr, self.col_idx, self.blk_idx, self.stored_col)
+        parts = tuple(getattr(self, name) for name in _PATTERN)
         # the patterns' transposed structure is kept until a buffer is replaced or written (load_state_dict);
         # writes of inference tensors are not counted, so nothing is kept for them
         structure: dict = {}
@@ -455,8 +462,7 @@ class SparseGatedLinear(torch.nn.Module):
                 self._made = (parts, versions, structure)
             structure = self._made[2]
         return GatedWeights(blocks=b, gate_blocks=self.gate_blocks, shape=self.shape, block=self.block,
-                            ent_ptr=parts[0], entries=parts[1], row_ptr=parts[2], col_idx=parts[3], blk_idx=parts[4],
-                            stored_col=parts[5], _structure=structure)
+                            _structure=structure, **dict(zip(_PATTERN, parts)))
 
     def forward(self, X: Tensor) -> Tensor:
         if not torch.is_grad_enabled():

@@ -248,3 +248,43 @@ def test_long_block_column_is_refused():
     for _ in range(2):  # nothing is kept of the refused call
         with pytest.raises(ValueError, match="16384"):
             ops.sparse_gated_linear_backward(h, x, w)
+
+
+def test_activation_of_the_call():
+    """The gradient is that of the function which the forward pass applied."""
+    x, dh, gate, up, wg, wu = case(40, 96, 96, 32, torch.bfloat16)
+    layer = ops.SparseGatedLinear(gate, up, activation="gelu")
+    want = step(layer, x, dh)
+    layer.blocks.grad = None
+    xr = x.clone().requires_grad_(True)
+    h = layer(xr)
+    layer.activation = "relu"
+    h.backward(dh)
+    same([h.detach(), xr.grad, layer.blocks.grad], want)
+
+
+def test_patterns_of_the_call():
+    """Patterns that are replaced between the passes change nothing; written in between, they are refused like any saved tensor."""
+    x, dh, gate, up, wg, wu = case(40, 96, 96, 32, torch.bfloat16)
+    layer = ops.SparseGatedLinear(gate, up)
+    want = step(layer, x, dh)
+    layer.blocks.grad = None
+    xr = x.clone().requires_grad_(True)
+    h = layer(xr)
+    kept = layer.col_idx
+    layer.col_idx = torch.zeros_like(kept)
+    h.backward(dh)
+    same([h.detach(), xr.grad, layer.blocks.grad], want)
+    layer.col_idx = kept
+    h = layer(xr)
+    layer.col_idx.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        h.backward(dh)
+
+
+def test_saved_tensors_that_are_copied():
+    x, dh, gate, up, wg, wu = case(40, 96, 96, 32, torch.bfloat16)
+    layer = ops.SparseGatedLinear(gate, up)
+    want = step(layer, x, dh)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda()):
+        same(step(layer, x, dh), want)
