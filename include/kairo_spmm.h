@@ -597,7 +597,8 @@ KAIRO_API kairo_status kairo_vocab_loss_backward(const float* grad, const void* 
  * 8 tokens.  Sums are fp32, H, dG and dU rounded once.  A value of X that is
  * not finite makes those results non-finite whose row keeps a block of Wg or Wu in
  * its column.  error_word: see kairo_vocab_loss; an entry out of range is
- * recorded there (KAIRO_DEVERR_BAD_INDEX) and counts as empty.  Asynchronous on `stream`.
+ * recorded there (KAIRO_DEVERR_BAD_INDEX) and counts as empty; ent_ptr is clamped to 0 .. nentries.  Asynchronous on
+ * `stream`.
  * ---------------------------------------------------------------------- */
 typedef enum kairo_activation {
   KAIRO_ACTIVATION_SILU = 0,

@@ -246,7 +246,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGatedThreads, 1)
       it.tile = t0 + (r - it.row * gn);
       it.subs = T;
     }
-    // offsets outside the entries are clamped by every role alike (and reported by the loads)
+    // offsets outside the entries are clamped by every role alike
     it.e0 = min(max(__ldg(args.ent_ptr + it.row), 0), args.nentries);
     it.e1 = min(max(__ldg(args.ent_ptr + it.row + 1), it.e0), args.nentries);
     return it;
@@ -288,8 +288,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGatedThreads, 1)
         const int4 w = w0;
         if (at + 32 < cnt) w0 = fetch(cur, at + 32);
         int col = w.x, blk = rank == 0 ? w.y : w.z;
-        if (at + lane < cnt && (static_cast<unsigned>(col) >= static_cast<unsigned>(args.nbc) || blk < -1 ||
-                                blk >= args.nblocks)) {
+        // one number out of range empties the entry in both CTAs
+        if (at + lane < cnt && (static_cast<unsigned>(col) >= static_cast<unsigned>(args.nbc) || w.y < -1 ||
+                                w.y >= args.nblocks || w.z < -1 || w.z >= args.nblocks)) {
           atomicCAS(args.err, 0u, KAIRO_DEVERR_BAD_INDEX);
           col = 0;
           blk = -1;

@@ -288,3 +288,21 @@ def test_saved_tensors_that_are_copied():
     want = step(layer, x, dh)
     with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda()):
         same(step(layer, x, dh), want)
+
+
+@pytest.mark.parametrize("tokens", [4, 20, 50, 300, 700])
+@pytest.mark.parametrize("b", [64, 32, 16])
+def test_malformed_entries_count_as_empty(tokens, b):
+    """One bad number of an entry empties all of it, for every token."""
+    x, dh, gate, up, wg, wu = case(tokens, 260 * b if tokens == 20 else 3 * b, 4 * b, b, torch.bfloat16, keep=0.9)
+    w = ops.gated_weights(gate, up)
+    kept = w.entries[1].clone()
+    assert (kept[1:3] >= 0).all()  # both weights keep this block
+    w.entries[1, 1:3] = -1
+    want = ops.sparse_gated_linear(x, w, check=True)
+    for field, value in ((0, 4), (0, -1), (1, w.blocks.shape[0]), (2, 1 << 30), (1, -2), (2, -2)):
+        w.entries[1] = kept
+        w.entries[1, field] = value
+        got = ops.sparse_gated_linear(x, w)
+        assert ops.pending_device_error() & 0xFF == _lib.DEVERR_BAD_INDEX
+        assert torch.equal(got, want)
