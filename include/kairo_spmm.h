@@ -587,7 +587,7 @@ KAIRO_API kairo_status kairo_vocab_loss_backward(const float* grad, const void* 
  * Wg and Wu are rows x cols with square blocks of 16, 32 or 64, f16 or bf16, in
  * one block storage (nblocks x block x block, 16-byte aligned).  Block-row i's entries
  * ent_ptr[i] .. ent_ptr[i + 1] - 1 are four int32 each (16-byte aligned):
- * block-column, stored block of Wg or -1, stored block of Wu or -1, 0.
+ * block-column, stored block of Wg or -1, stored block of Wu or -1, 0; with entries there is a stored block.
  *   kairo_gated_linear       H (n x rows)
  *   kairo_gated_linear_grad  dG = dH * U * act'(G) and dU = dH * act(G), G and U
  *                            formed from X anew, as dP (n x 2 ceil(rows / block)

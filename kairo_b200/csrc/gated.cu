@@ -928,7 +928,7 @@ kairo_status run_gated(GatedArgs a, cudaStream_t s) {
     kairo_status st = make_map_2d(&mx, a.x, dt, 2, static_cast<uint64_t>(a.k), static_cast<uint64_t>(a.n),
                                   static_cast<uint64_t>(a.ldx), BM, 64, "X");
     if (st == KAIRO_STATUS_SUCCESS)
-      st = make_map_2d(&mw, a.blocks, dt, 2, BM, static_cast<uint64_t>(std::max(1, a.nblocks)) * BM, BM, BM, BM,
+      st = make_map_2d(&mw, a.blocks, dt, 2, BM, static_cast<uint64_t>(a.nblocks) * BM, BM, BM, BM,
                        "block storage");
     if (st) return st;
     auto* fn = &k_gated_short<BM, T, IN_FMT, TT, GRAD>;
@@ -948,7 +948,7 @@ kairo_status run_gated(GatedArgs a, cudaStream_t s) {
     kairo_status st = make_map_2d(&mx, a.x, dt, 2, static_cast<uint64_t>(a.k), static_cast<uint64_t>(a.n),
                                   static_cast<uint64_t>(a.ldx), BM, 64, "X");
     if (st == KAIRO_STATUS_SUCCESS)
-      st = make_map_2d(&mw, a.blocks, dt, 2, BM, static_cast<uint64_t>(std::max(1, a.nblocks)) * BM, BM, BM, BM,
+      st = make_map_2d(&mw, a.blocks, dt, 2, BM, static_cast<uint64_t>(a.nblocks) * BM, BM, BM, BM,
                        "block storage");
     if (st) return st;
     auto* fn = &k_gated<BM, T, IN_FMT, TT, GRAD>;
@@ -1003,6 +1003,8 @@ kairo_status gated_check(const kairo_gated* w, const void* x, int64_t ldx, int64
   if (n == 0 || w->rows == 0) return KAIRO_STATUS_SUCCESS;
   if (!w->ent_ptr || !err || (w->nentries > 0 && (!w->entries || !w->blocks || !x)))
     return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+  // a missing block is a copy from behind the storage, which needs a block in front
+  if (w->nentries > 0 && w->nblocks == 0) return fail(KAIRO_STATUS_INVALID_VALUE, "entries without a stored block");
   if (reinterpret_cast<uintptr_t>(w->entries) % 16 || reinterpret_cast<uintptr_t>(w->blocks) % 16)
     return fail(KAIRO_STATUS_INVALID_VALUE, "entries and blocks must be 16-byte aligned");
   if (n > kAnyTokens && w->nentries > 0 && !row_vec(x, ldx, n))

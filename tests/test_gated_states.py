@@ -60,3 +60,16 @@ def test_collect_errors_refusals():
     assert lib.kairo_collect_errors(two, 2, None, None) == _lib.INVALID_VALUE
     assert lib.kairo_collect_errors(None, 1, some, None) == _lib.INVALID_VALUE
     assert lib.kairo_collect_errors((ctypes.c_void_p * 2)(256, None), 2, some, None) == _lib.INVALID_VALUE
+
+
+def test_entries_without_blocks_are_refused():
+    """Every number of the entries is then -1 or out of range; the kernels would copy zeros from behind a block that is not there."""
+    lib, some = _lib.lib(), ctypes.c_void_p(256)  # never read: each call is refused first
+    w = _lib.KairoGated(rows=64, cols=64, nentries=1, nblocks=0, ent_ptr=256, entries=256, blocks=256, block=64,
+                        dtype=_lib.DTYPE_BF16)
+    for n in (1, 40, 100, 300):
+        assert lib.kairo_gated_linear(ctypes.byref(w), some, 64, n, 0, some, 64, some, None) == _lib.INVALID_VALUE
+        assert b"without a stored block" in lib.kairo_last_error_message()
+        assert lib.kairo_gated_linear_grad(ctypes.byref(w), some, 64, n, 0, some, 64, some, 128, some,
+                                           None) == _lib.INVALID_VALUE
+        assert b"without a stored block" in lib.kairo_last_error_message()
