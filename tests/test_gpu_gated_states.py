@@ -306,3 +306,17 @@ def test_malformed_entries_count_as_empty(tokens, b):
         got = ops.sparse_gated_linear(x, w)
         assert ops.pending_device_error() & 0xFF == _lib.DEVERR_BAD_INDEX
         assert torch.equal(got, want)
+
+
+def test_loaded_patterns_with_another_split():
+    """As many blocks in all, of which another number is the gate's."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    pos = [torch.tensor(p, device="cuda") for p in ([0, 4, 8], [1, 2, 6], [0, 3, 4, 8], [1, 5])]
+    mats = [weight(96, 96, 32, 0.3, torch.bfloat16, g, pos=p)[0] for p in pos]
+    one, two = ops.SparseGatedLinear(mats[0], mats[1]), ops.SparseGatedLinear(mats[2], mats[3])
+    one.load_state_dict(two.state_dict())
+    for w in (one.weights(), copy.deepcopy(one).weights()):
+        got, want = w.matrices(), two.weights().matrices()
+        for p, q in zip(got, want):
+            same([p.row_ptr, p.col_idx, p.blocks], [q.row_ptr, q.col_idx, q.blocks])
+        assert [p.shape[0] for p in w.split(w.blocks)] == [4, 2]
