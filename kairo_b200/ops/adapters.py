@@ -336,7 +336,7 @@ class _AdaptedLinearFn(torch.autograd.Function):
         dY = dY.contiguous()
         need_dx, need_blocks = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         need_dw = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
-        wt = transpose_values(W, layer.transposed()) if need_dx or need_blocks else None
+        wt = transpose_values(W, layer.transposed(blocks)) if need_dx or need_blocks else None
         base_dx = sparse_linear(dY, wt.matrix, out_dtype=torch.float32) if need_dx else None
         dX = d_down = d_up = None
         if need_dx or need_dw:

@@ -85,6 +85,11 @@ def bsr_transpose(a: BlockSparseMatrix, *, check: bool = False, row_hint: bool =
 
 def transpose_values(a: BlockSparseMatrix, t: TransposedBsr) -> TransposedBsr:
     """Refresh W^T's blocks from W's current values (structure unchanged)."""
+    b = t.matrix.blocks
+    if b.dtype != a.dtype or b.device != a.device:
+        raise TypeError(f"transpose_values: W is {a.dtype} on {a.device}, W^T {b.dtype} on {b.device}")
+    if t.perm.numel() != a.nnzb or tuple(b.shape) != (a.nnzb, a.block_size[1], a.block_size[0]):
+        raise ValueError(f"transpose_values: W has {a.nnzb} blocks of {a.block_size}, W^T {tuple(b.shape)}")
     if a.nnzb == 0:
         return t
     lib = _lib.lib()
@@ -196,7 +201,7 @@ class _SparseLinearFn(torch.autograd.Function):
         X = kept[0] if ctx.kept_dtype is None else QuantizedActivations._from_parts(*kept, module.shape[1],
                                                                                      ctx.kept_dtype)
         W = module.weight_matrix(blocks)
-        wt = transpose_values(W, module.transposed())
+        wt = transpose_values(W, module.transposed(blocks))
         dY = dY.contiguous()
         if X is None:
             dX = sparse_linear(dY, wt.matrix, out_dtype=ctx.x_dtype) if ctx.needs_input_grad[0] else None
@@ -238,10 +243,12 @@ class BlockSparseLinear(torch.nn.Module):
         return BlockSparseMatrix(row_ptr=self.row_ptr, col_idx=self.col_idx, blocks=b.detach(), shape=self.shape,
                                  block_size=self.block_size, max_row_blocks=self.max_row_blocks)
 
-    def transposed(self) -> TransposedBsr:
-        """Cached W^T structure (its blocks are refreshed on every backward)."""
-        if self._wt is None:
-            self._wt = bsr_transpose(self.weight_matrix())
+    def transposed(self, blocks: Tensor | None = None) -> TransposedBsr:
+        """Cached W^T structure (its blocks are refreshed on every backward), made again for ``blocks`` of another
+        type or on another device than it was made for, as after a cast of the module."""
+        W = self.weight_matrix(blocks)
+        if self._wt is None or self._wt.matrix.dtype != W.dtype or self._wt.matrix.device != W.device:
+            self._wt = bsr_transpose(W)
         return self._wt
 
     def forward(self, X: Tensor) -> Tensor:

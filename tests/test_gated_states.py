@@ -10,6 +10,7 @@ import pytest
 import torch
 
 from kairo_b200 import _lib
+from kairo_b200.ops import backward as backward_module
 from kairo_b200.ops import gated as gated_module
 from kairo_b200.types import BlockSparseMatrix
 
@@ -73,3 +74,35 @@ def test_entries_without_blocks_are_refused():
         assert lib.kairo_gated_linear_grad(ctypes.byref(w), some, 64, n, 0, some, 64, some, 128, some,
                                            None) == _lib.INVALID_VALUE
         assert b"without a stored block" in lib.kairo_last_error_message()
+
+
+def bsr(dtype, n=2, b=16):
+    i32 = torch.int32
+    return BlockSparseMatrix(row_ptr=torch.tensor([0, n], dtype=i32), col_idx=torch.arange(n, dtype=i32),
+                             blocks=torch.zeros(n, b, b, dtype=dtype), shape=(b, n * b), block_size=(b, b))
+
+
+def test_transposed_values_of_another_type_are_refused():
+    t = backward_module.TransposedBsr(matrix=bsr(torch.bfloat16), perm=torch.arange(2, dtype=torch.int32))
+    with pytest.raises(TypeError, match="transpose_values"):
+        backward_module.transpose_values(bsr(torch.float32), t)
+    with pytest.raises(ValueError, match="transpose_values"):
+        backward_module.transpose_values(bsr(torch.bfloat16, n=3), t)
+    with pytest.raises(ValueError, match="transpose_values"):
+        backward_module.transpose_values(bsr(torch.bfloat16, b=32), t)
+
+
+def test_layer_makes_its_transposed_structure_again_for_another_type(monkeypatch):
+    made = []
+
+    def fake(a):
+        made.append(a.dtype)
+        return backward_module.TransposedBsr(matrix=a, perm=torch.arange(a.nnzb, dtype=torch.int32))
+
+    monkeypatch.setattr(backward_module, "bsr_transpose", fake)
+    layer = backward_module.BlockSparseLinear(bsr(torch.bfloat16))
+    kept = layer.blocks.detach().clone()
+    assert layer.transposed() is layer.transposed() and made == [torch.bfloat16]
+    layer.float()
+    assert layer.transposed() is layer.transposed() and made[1:] == [torch.float32]
+    assert layer.transposed(kept).matrix.dtype == torch.bfloat16  # a pass that began before the cast

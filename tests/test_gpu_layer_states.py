@@ -1,0 +1,58 @@
+"""Block-sparse layers whose values or patterns change between training steps, against layers that were never used
+before.  Equal inputs give equal bits."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from kairo_b200 import ops
+from tests.test_gpu_gated import case, weight
+from tests.test_gpu_gated_states import same, step
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.bfloat16, torch.float16]  # the types of the layer
+
+
+def layers(first, b=32, seed=7):
+    x, dh, gate, up, wg, wu = case(70, 96, 96, b, first, seed=seed)
+    down, _, _ = weight(96, 96, b, 0.5, first, torch.Generator(device="cuda").manual_seed(seed), shuffle=True)
+    return x, dh, gate, up, down
+
+
+@pytest.mark.parametrize("first,then", [(p, q) for p in TYPES for q in TYPES if p != q])
+def test_layer_cast_after_a_step(first, then):
+    x, dh, gate, up, down = layers(torch.bfloat16)
+    x, dh = x.to(first), dh.to(first)
+    layer = ops.BlockSparseLinear(down).to(first)
+    step(layer, x, dh)
+    layer.to(then)
+    other = ops.BlockSparseLinear(down).to(first).to(then)
+    same(step(layer, x.to(then), dh.to(then)), step(other, x.to(then), dh.to(then)))
+
+
+@pytest.mark.parametrize("first,then", [(TYPES[0], TYPES[1]), (TYPES[1], TYPES[0])])
+def test_feed_forward_cast_after_a_step(first, then):
+    x, dh, gate, up, down = layers(first)
+    layer = ops.SparseFeedForward(gate, up, down)
+    step(layer, x, dh)
+    layer.to(then)
+    other = ops.SparseFeedForward(gate, up, down).to(then)
+    same(step(layer, x.to(then), dh.to(then)), step(other, x.to(then), dh.to(then)))
+
+
+def test_adapted_layer_cast_after_a_step():
+    x, dh, gate, up, down = layers(torch.bfloat16)
+    plan = ops.adapter_plan(torch.zeros(70, dtype=torch.int32, device="cuda"), 1)
+    one, two = (ops.AdaptedSparseLinear(ops.BlockSparseLinear(down), 1, 8) for _ in range(2))
+    two.load_state_dict(one.state_dict())
+
+    def grads(layer, x, dh):
+        for p in layer.parameters():
+            p.grad = None
+        xr = x.clone().requires_grad_(True)
+        layer(xr, plan).backward(dh)
+        return [xr.grad, *(p.grad for p in layer.parameters())]
+
+    grads(one, x, dh)
+    same(grads(one.half(), x.half(), dh.half()), grads(two.half(), x.half(), dh.half()))
