@@ -211,6 +211,9 @@ class _SparseLinearFn(torch.autograd.Function):
         return dX, dW, None
 
 
+_REPLACED: list[TransposedBsr] = []
+
+
 class BlockSparseLinear(torch.nn.Module):
     """``Y = X @ W^T`` with a block-sparse weight of fixed sparsity pattern.
 
@@ -237,6 +240,20 @@ class BlockSparseLinear(torch.nn.Module):
         self.block_size = W.block_size
         self.max_row_blocks = W.max_row_blocks
         self._wt: TransposedBsr | None = None
+
+    def _load_from_state_dict(self, *args, **kw) -> None:
+        before = self.row_ptr.clone(), self.col_idx.clone()
+        super()._load_from_state_dict(*args, **kw)
+        after = self.row_ptr, self.col_idx
+        if any(t.is_meta for t in (*before, *after)) or all(torch.equal(p, q.to(p.device)) for p, q in zip(before, after)):
+            return
+        # another pattern with as many blocks: neither the transposed structure nor the hint is this one's.  A captured
+        # graph may still replay with the old structure, so that is not given back
+        if self._wt is not None:
+            _REPLACED.append(self._wt)
+            self._wt = None
+        if self.max_row_blocks:
+            self.max_row_blocks = int(self.row_ptr.diff().max())
 
     def weight_matrix(self, blocks: Tensor | None = None) -> BlockSparseMatrix:
         b = self.blocks if blocks is None else blocks

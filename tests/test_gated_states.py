@@ -106,3 +106,12 @@ def test_layer_makes_its_transposed_structure_again_for_another_type(monkeypatch
     layer.float()
     assert layer.transposed() is layer.transposed() and made[1:] == [torch.float32]
     assert layer.transposed(kept).matrix.dtype == torch.bfloat16  # a pass that began before the cast
+
+
+def test_layer_loads_without_memory():
+    """A layer on the meta device has no pattern to compare."""
+    layer = backward_module.BlockSparseLinear(bsr(torch.bfloat16))
+    state = layer.state_dict()
+    bare = copy.deepcopy(layer).to("meta")
+    bare.load_state_dict(state, assign=True)
+    assert torch.equal(bare.col_idx, layer.col_idx) and not bare.blocks.is_meta

@@ -56,3 +56,23 @@ def test_adapted_layer_cast_after_a_step():
 
     grads(one, x, dh)
     same(grads(one.half(), x.half(), dh.half()), grads(two.half(), x.half(), dh.half()))
+
+
+@pytest.mark.parametrize("b", [64, 32])
+def test_loaded_patterns_are_followed(b):
+    """A state dict of another pattern with as many blocks, after a step: a layer alone and in a feed-forward block."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    n = 3 * b
+    mats = [weight(n, n, b, 0.3, torch.bfloat16, g, pos=torch.tensor(p, device="cuda"))[0]
+            for p in ([0, 1, 2], [0, 4, 7], [2, 3, 8])]
+    x, dh = torch.randn(70, n, device="cuda").bfloat16(), torch.randn(70, n, device="cuda").bfloat16()
+    for make in (lambda m: ops.BlockSparseLinear(m), lambda m: ops.SparseFeedForward(mats[2], mats[2], m)):
+        one, two = make(mats[0]), make(mats[1])
+        step(one, x, dh)
+        one.load_state_dict(two.state_dict())
+        same(step(one, x, dh), step(two, x, dh))
+        layer = one if isinstance(one, ops.BlockSparseLinear) else one.down
+        assert layer.max_row_blocks == mats[1].max_row_blocks
+        kept = layer.transposed()
+        one.load_state_dict(two.state_dict())
+        assert layer.transposed() is kept  # the same pattern: the structure stays, as captured graphs expect
