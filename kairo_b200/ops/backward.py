@@ -211,7 +211,7 @@ class _SparseLinearFn(torch.autograd.Function):
         return dX, dW, None
 
 
-_REPLACED: list[TransposedBsr] = []
+_CAPTURED: list[TransposedBsr] = []  # what captured graphs may still read, whatever has become of their layers
 
 
 class BlockSparseLinear(torch.nn.Module):
@@ -247,11 +247,8 @@ class BlockSparseLinear(torch.nn.Module):
         after = self.row_ptr, self.col_idx
         if any(t.is_meta for t in (*before, *after)) or all(torch.equal(p, q.to(p.device)) for p, q in zip(before, after)):
             return
-        # another pattern with as many blocks: neither the transposed structure nor the hint is this one's.  A captured
-        # graph may still replay with the old structure, so that is not given back
-        if self._wt is not None:
-            _REPLACED.append(self._wt)
-            self._wt = None
+        # another pattern with as many blocks: neither the transposed structure nor the hint is this one's
+        self._wt = None
         if self.max_row_blocks:
             self.max_row_blocks = int(self.row_ptr.diff().max())
 
@@ -266,6 +263,8 @@ class BlockSparseLinear(torch.nn.Module):
         W = self.weight_matrix(blocks)
         if self._wt is None or self._wt.matrix.dtype != W.dtype or self._wt.matrix.device != W.device:
             self._wt = bsr_transpose(W)
+        if W.blocks.is_cuda and torch.cuda.is_current_stream_capturing() and not any(t is self._wt for t in _CAPTURED):
+            _CAPTURED.append(self._wt)
         return self._wt
 
     def forward(self, X: Tensor) -> Tensor:

@@ -453,7 +453,8 @@ class SparseGatedLinear(torch.nn.Module):
     def _load_from_state_dict(self, *args, **kw) -> None:
         super()._load_from_state_dict(*args, **kw)
         # patterns of as many blocks in all may give the gate another number of them
-        self.gate_blocks = int((self.row_ptr[1::2] - self.row_ptr[0:-1:2]).sum())
+        if not self.row_ptr.is_meta:
+            self.gate_blocks = int((self.row_ptr[1::2] - self.row_ptr[0:-1:2]).sum())
 
     def weights(self, blocks: Tensor | None = None) -> GatedWeights:
         b = (self.blocks if blocks is None else blocks).detach()

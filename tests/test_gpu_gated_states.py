@@ -320,3 +320,13 @@ def test_loaded_patterns_with_another_split():
         for p, q in zip(got, want):
             same([p.row_ptr, p.col_idx, p.blocks], [q.row_ptr, q.col_idx, q.blocks])
         assert [p.shape[0] for p in w.split(w.blocks)] == [4, 2]
+
+
+def test_layer_loads_without_memory():
+    x, dh, gate, up, wg, wu = case(40, 96, 96, 32, torch.bfloat16)
+    layer = ops.SparseGatedLinear(gate, up)
+    want, bare = step(layer, x, dh), copy.deepcopy(layer).to("meta")
+    bare.load_state_dict({k: v.to("meta") for k, v in layer.state_dict().items()})
+    bare.load_state_dict(layer.state_dict(), assign=True)
+    assert bare.gate_blocks == layer.gate_blocks
+    same(step(bare, x, dh), want)

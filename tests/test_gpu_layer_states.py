@@ -76,3 +76,34 @@ def test_loaded_patterns_are_followed(b):
         kept = layer.transposed()
         one.load_state_dict(two.state_dict())
         assert layer.transposed() is kept  # the same pattern: the structure stays, as captured graphs expect
+
+
+def test_structure_of_a_captured_step_is_kept():
+    """A graph of a backward pass replays with the structure that it was captured with, after another pattern was loaded."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    one, two = (ops.BlockSparseLinear(weight(192, 192, 64, 0.3, torch.bfloat16, g, pos=torch.tensor(p, device="cuda"))[0])
+                for p in ([0, 1, 2, 5], [0, 4, 7, 8]))
+    dy, x = torch.randn(70, 192, device="cuda").bfloat16(), torch.randn(70, 192, device="cuda").bfloat16()
+    W, blocks = one.weight_matrix(), one.blocks.detach().clone()
+
+    def grads():
+        return ops.sparse_linear_backward(dy, x, W, ops.transpose_values(W, one.transposed()))
+
+    want = [t.clone() for t in grads()]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        got = grads()
+    sizes = [t.numel() for t in (one.transposed().matrix.row_ptr, one.transposed().matrix.col_idx, one.transposed().perm)]
+    pattern = one.row_ptr.clone(), one.col_idx.clone()
+    one.load_state_dict(two.state_dict())
+    kept = [torch.full((n,), -1, dtype=torch.int32, device="cuda") for n in sizes for _ in range(8)]
+    with torch.no_grad():
+        one.blocks.copy_(blocks)
+        one.row_ptr.copy_(pattern[0])
+        one.col_idx.copy_(pattern[1])
+    graph.replay()
+    torch.cuda.synchronize()
+    same(got, want)
+    del kept
