@@ -580,7 +580,8 @@ __device__ void prep_factors(const PrepArgs& p) {
     const int64_t id = p.ids[i];
     if (id >= 0 && id < p.vocab) {
       count += 1.f;
-      if (p.reduction == kNone) top = fmaxf(top, fabsf(p.grad[i]));
+      // one that is not finite spoils its own token's G; the others keep their power of two
+      if (p.reduction == kNone && isfinite(p.grad[i])) top = fmaxf(top, fabsf(p.grad[i]));
     }
   }
   float shared_factor;
@@ -593,7 +594,7 @@ __device__ void prep_factors(const PrepArgs& p) {
     __syncthreads();
     for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) top = fmaxf(top, tops[i]);
     int e = 0;
-    if (top > 0.f && isfinite(top)) frexpf(top, &e);
+    if (top > 0.f) frexpf(top, &e);
     shared_factor = ldexpf(1.f, max(-100, min(100, e)));
   } else {
     count = cta_sum(count);
