@@ -37,3 +37,22 @@ def test_a_factor_that_is_not_finite(dtype, bad):
     assert not torch.isfinite(got[7]).any() and not torch.isfinite(dw).all()
     others = torch.arange(50, device="cuda") != 7
     assert torch.equal(got[others], dx[others])
+
+
+@pytest.mark.parametrize("dtype,powers", [(torch.float16, (-18, -9, 13)), (torch.bfloat16, (-60, -20, 20, 60))])
+def test_factors_keep_their_digits(dtype, powers):
+    """grad times 2^p gives the same digits: p is taken back by an operand times 2^p and a scale of 2^-p, which leave the logits as they are."""
+    x, w, ids, g = inputs(dtype)
+    grad = torch.rand(50, generator=g, device="cuda") + 0.25
+    dx, dw = backward(x, w, ids, grad)
+    assert dx.any() and dw.any()
+    for p in powers:
+        big = torch.tensor(2.0**p, dtype=torch.float64)
+        up = (x.double() * big).to(dtype)
+        assert torch.equal(up.double(), x.double() * big)  # exact
+        got, _ = backward(up, w, ids, grad * 2.0**p, 2.0**-p)
+        assert torch.equal(got, dx), p
+        up = (w.double() * big).to(dtype)
+        assert torch.equal(up.double(), w.double() * big)
+        _, got = backward(x, up, ids, grad * 2.0**p, 2.0**-p)
+        assert torch.equal(got, dw), p
