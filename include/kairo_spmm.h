@@ -328,6 +328,13 @@ KAIRO_API kairo_status kairo_bsr_sddmm(const kairo_bsr* a, const int32_t* row_pt
                                        int64_t ldx, int64_t n, void* dblocks, kairo_dtype out_dtype,
                                        void* workspace, size_t workspace_bytes, void* stream);
 KAIRO_API kairo_status kairo_bsr_sddmm_workspace_size(const kairo_bsr* a, size_t* bytes);
+/* The same with device errors going to a word of the caller's (not cleared), for a
+ * workspace that nobody reads after the call. */
+KAIRO_API kairo_status kairo_bsr_sddmm_word(const kairo_bsr* a, const int32_t* row_ptr_t, const int32_t* col_idx_t,
+                                            const int32_t* perm_t, const void* dy, int64_t lddy, const void* x,
+                                            int64_t ldx, int64_t n, void* dblocks, kairo_dtype out_dtype,
+                                            void* workspace, size_t workspace_bytes, unsigned* error_word,
+                                            void* stream);
 
 /* ------------------------------------------------------------------------
  * Activations kept in 8 bits for the backward pass (no counterpart in the

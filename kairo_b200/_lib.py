@@ -203,6 +203,8 @@ _SIGNATURES = {
     "kairo_bsr_transpose_values": (c_int32, [POINTER(KairoBsr), c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "kairo_bsr_sddmm": (c_int32, [POINTER(KairoBsr), c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
                                   c_int64, c_int64, c_void_p, c_int32, c_void_p, c_size_t, c_void_p]),
+    "kairo_bsr_sddmm_word": (c_int32, [POINTER(KairoBsr), c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
+                                       c_int64, c_int64, c_void_p, c_int32, c_void_p, c_size_t, c_void_p, c_void_p]),
     "kairo_bsr_sddmm_workspace_size": (c_int32, [POINTER(KairoBsr), POINTER(c_size_t)]),
     "kairo_quantize_q8": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_int32, c_void_p, c_int64, c_void_p,
                                     c_int64, c_void_p]),

@@ -673,7 +673,7 @@ namespace {
 
 kairo_status run_sddmm(const kairo_bsr* a, const int32_t* row_ptr_t, const int32_t* col_idx_t, const int32_t* perm_t,
                        const void* dy, int64_t lddy, const SddX& x, int64_t n, void* dblocks, kairo_dtype out_dtype,
-                       void* workspace, size_t workspace_bytes, void* stream) {
+                       void* workspace, size_t workspace_bytes, unsigned* error_word, void* stream) {
   kairo_status st = sddmm_check(a, row_ptr_t, col_idx_t, perm_t, dy, lddy, x.codes ? x.codes : x.x,
                                 x.codes ? a->cols : x.ldx, n, dblocks, out_dtype, workspace);
   if (st) return st;
@@ -684,8 +684,13 @@ kairo_status run_sddmm(const kairo_bsr* a, const int32_t* row_ptr_t, const int32
   if (workspace_bytes < need) return fail(KAIRO_STATUS_WORKSPACE_TOO_SMALL, "SDDMM workspace too small");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   SddWs w = carve_sdd(workspace);
-  cudaError_t e = cudaMemsetAsync(workspace, 0, kWorkspaceHeaderBytes, s);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync(SDDMM workspace)");
+  cudaError_t e = cudaSuccess;
+  if (error_word) {
+    w.err = error_word;  // the caller's, which is not cleared
+  } else {
+    e = cudaMemsetAsync(workspace, 0, kWorkspaceHeaderBytes, s);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync(SDDMM workspace)");
+  }
   const size_t osz = out_dtype == KAIRO_DTYPE_F32 ? 4 : 2;
   if (n == 0) {
     e = cudaMemsetAsync(dblocks, 0, static_cast<size_t>(a->nnzb) * a->bm * a->bk * osz, s);
@@ -767,7 +772,17 @@ extern "C" kairo_status kairo_bsr_sddmm(const kairo_bsr* a, const int32_t* row_p
                                         int64_t ldx, int64_t n, void* dblocks, kairo_dtype out_dtype,
                                         void* workspace, size_t workspace_bytes, void* stream) {
   return run_sddmm(a, row_ptr_t, col_idx_t, perm_t, dy, lddy, SddX{x, ldx, nullptr, 0, nullptr, 0}, n, dblocks,
-                   out_dtype, workspace, workspace_bytes, stream);
+                   out_dtype, workspace, workspace_bytes, nullptr, stream);
+}
+
+extern "C" kairo_status kairo_bsr_sddmm_word(const kairo_bsr* a, const int32_t* row_ptr_t, const int32_t* col_idx_t,
+                                             const int32_t* perm_t, const void* dy, int64_t lddy, const void* x,
+                                             int64_t ldx, int64_t n, void* dblocks, kairo_dtype out_dtype,
+                                             void* workspace, size_t workspace_bytes, unsigned* error_word,
+                                             void* stream) {
+  if (!error_word) return fail(KAIRO_STATUS_INVALID_VALUE, "null pointer argument");
+  return run_sddmm(a, row_ptr_t, col_idx_t, perm_t, dy, lddy, SddX{x, ldx, nullptr, 0, nullptr, 0}, n, dblocks,
+                   out_dtype, workspace, workspace_bytes, error_word, stream);
 }
 
 extern "C" kairo_status kairo_bsr_sddmm_q8(const kairo_bsr* a, const int32_t* row_ptr_t, const int32_t* col_idx_t,
@@ -780,5 +795,5 @@ extern "C" kairo_status kairo_bsr_sddmm_q8(const kairo_bsr* a, const int32_t* ro
   if (st) return st;
   if (!codes) ldq = 0;  // an empty batch
   return run_sddmm(a, row_ptr_t, col_idx_t, perm_t, dy, lddy, SddX{nullptr, a->cols, codes, ldq, steps, lds}, n,
-                   dblocks, out_dtype, workspace, workspace_bytes, stream);
+                   dblocks, out_dtype, workspace, workspace_bytes, nullptr, stream);
 }

@@ -356,7 +356,6 @@ def sparse_gated_linear_backward(dH: Tensor, X: Tensor, weights: GatedWeights, *
     lib = _lib.lib()
     st = weights._backward_structure()
     st.used_on_current_stream(index)
-    own: list[Tensor] = []  # workspaces that end with the call
     if need_dx:
         # the transposed weight's values are of this call alone: the structure serves calls on several streams
         blocks_t = weights.blocks.new_empty((nnzb, b, b))
@@ -374,11 +373,11 @@ def sparse_gated_linear_backward(dH: Tensor, X: Tensor, weights: GatedWeights, *
             size = nbytes.value
             if len(st.spmm_bytes) < 4096:
                 st.spmm_bytes[n, x.dtype] = size
-        if torch.cuda.is_current_stream_capturing():
+        captured = torch.cuda.is_current_stream_capturing()
+        if captured:
             # a graph's own: two captured graphs may replay at the same time
             ws = x.new_empty(size, dtype=torch.uint8)
             ws[:_ZEROED].zero_()
-            own.append(ws)
         else:
             ws = _lib.workspace(size, x.device)
         if check:
@@ -386,18 +385,17 @@ def sparse_gated_linear_backward(dH: Tensor, X: Tensor, weights: GatedWeights, *
         _lib.launch(op, lib.kairo_bsr_spmm, index, ctypes.byref(desc_t), dp.data_ptr(), dp.shape[1],
                     _lib.LAYOUT_LINEAR, n, dX.data_ptr(), k, _lib.kairo_dtype(x.dtype), ctypes.byref(cfg),
                     ws.data_ptr(), ws.numel())
+        if captured:
+            _lib.collect_errors(op, index, err, ws)
         if check:
             _lib.raise_on_device_error(ws)
     if need_dw:
         d_blocks = weights.blocks.new_empty((nnzb, b, b), dtype=dwt)
         ws = x.new_empty(st.sddmm_bytes, dtype=torch.uint8)
-        _lib.launch(op, lib.kairo_bsr_sddmm, index, ctypes.byref(_with_blocks(st.desc_w, weights.blocks)),
+        _lib.launch(op, lib.kairo_bsr_sddmm_word, index, ctypes.byref(_with_blocks(st.desc_w, weights.blocks)),
                     st.kept[0].data_ptr(), st.kept[1].data_ptr(), st.perm_stored.data_ptr(), dp.data_ptr(), dp.shape[1],
                     x.data_ptr(), max(_ld(x), k), n, d_blocks.data_ptr(), _lib.kairo_dtype(dwt), ws.data_ptr(),
-                    ws.numel())
-        own.append(ws)
-    if own:
-        _lib.collect_errors(op, index, err, *own)
+                    ws.numel(), err.data_ptr())
     if check:
         _lib.raise_on_device_error(err)
     return dX, d_blocks

@@ -63,6 +63,16 @@ def test_collect_errors_refusals():
     assert lib.kairo_collect_errors((ctypes.c_void_p * 2)(256, None), 2, some, None) == _lib.INVALID_VALUE
 
 
+def test_weight_gradient_needs_its_error_word():
+    some, d = ctypes.c_void_p(256), _lib.KairoBsr(rows=64, cols=64, bm=64, bk=64, nbr=1, nnzb=0, dtype=_lib.DTYPE_BF16)
+
+    def call(word):
+        return _lib.lib().kairo_bsr_sddmm_word(ctypes.byref(d), some, some, some, some, 64, some, 64, 8, some,
+                                               _lib.DTYPE_F32, some, 1 << 20, word, None)
+
+    assert call(None) == _lib.INVALID_VALUE and call(some) == _lib.SUCCESS  # no blocks: nothing is launched
+
+
 def test_entries_without_blocks_are_refused():
     """Every number of the entries is then -1 or out of range; the kernels would copy zeros from behind a block that is not there."""
     lib, some = _lib.lib(), ctypes.c_void_p(256)  # never read: each call is refused first
