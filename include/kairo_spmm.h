@@ -685,6 +685,11 @@ KAIRO_API kairo_status kairo_workspace_error(void* workspace, int32_t clear, uin
 KAIRO_API kairo_status kairo_collect_errors(const void* const* workspaces, int32_t count, unsigned* error_word,
                                             void* stream);
 
+/* Id of the capture that `stream` is in, 0 without one: what a captured graph
+ * needs for itself (a workspace: two graphs may replay at the same time) is
+ * allotted by it. */
+KAIRO_API kairo_status kairo_capture_id(void* stream, uint64_t* id);
+
 /* `*count` error words of the current device, for operators that take an
  * error_word and for captured graphs: 256 bytes apart from `*words` on, zero
  * when the library is loaded, there until it is unloaded.  The caller shares

@@ -68,6 +68,7 @@ def acc_spmm_forward(
             A_tiles.data_ptr() if num_tiles else None, tile_row_ids.data_ptr() if num_tiles else None,
             tile_col_ids.data_ptr() if num_tiles else None, B.data_ptr(), C.data_ptr(), M, K, N, num_tiles,
             tile_m, tile_k, dt, ws.data_ptr(), ws.numel(), _lib.stream_handle(device)), "acc_spmm_forward")
+        _lib.report_captured("acc_spmm_forward", torch.cuda.current_device(), ws)
     return C
 
 

@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
-from ctypes import POINTER, Structure, c_char_p, c_float, c_int32, c_int64, c_size_t, c_uint32, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_float, c_int32, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
 
 import torch
 
@@ -279,6 +279,7 @@ _SIGNATURES = {
     "kairo_partition_rows": (c_int32, [POINTER(c_int64), c_int32, c_int32, POINTER(c_int32)]),
     "kairo_workspace_error": (c_int32, [c_void_p, c_int32, POINTER(c_uint32), c_void_p]),
     "kairo_collect_errors": (c_int32, [POINTER(c_void_p), c_int32, c_void_p, c_void_p]),
+    "kairo_capture_id": (c_int32, [c_void_p, POINTER(c_uint64)]),
     "kairo_error_words": (c_int32, [POINTER(c_void_p), POINTER(c_int32)]),
     "kairo_status_string": (c_char_p, [c_int32]),
     "kairo_last_error_message": (c_char_p, []),
@@ -401,12 +402,26 @@ _ws_lock = threading.Lock()
 _ws_cache: dict[tuple[int, int], torch.Tensor] = {}
 
 
+# of an SpMM workspace: header and arrival counters, zero before its first launch
+_ZEROED = 256 + 2 * 16384 * 4
+_capture_ws: dict[tuple[int, int], tuple[int, torch.Tensor]] = {}
+
+
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
-    """A zero-initialised device buffer of at least ``nbytes`` bytes for the
+    """A device buffer of at least ``nbytes`` bytes, its counters zero, for the
     current stream of ``device``.  The library leaves the counters it uses at
-    zero, so the buffer is reused across launches on that stream."""
+    zero, so the buffer is reused across launches on that stream.
+
+    A capture has buffers of its own, zeroed in the graph: two captured graphs
+    may replay at the same time, or beside eager calls on the stream that they
+    were captured on, and an eager buffer may be replaced by a larger one."""
     dev = device.index if device.index is not None else torch.cuda.current_device()
     key = (dev, torch.cuda.current_stream(dev).cuda_stream)
+    if torch.cuda.is_current_stream_capturing():
+        capture = c_uint64(0)
+        check(lib().kairo_capture_id(key[1], ctypes.byref(capture)), "workspace")
+        if capture.value:
+            return _captured_workspace(max(nbytes, _ZEROED), key, capture.value)
     with _ws_lock:
         buf = _ws_cache.get(key)
         if buf is None or buf.numel() < nbytes:
@@ -414,6 +429,25 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
             buf = torch.zeros(size, dtype=torch.uint8, device=torch.device("cuda", dev))
             _ws_cache[key] = buf
         return buf
+
+
+def _captured_workspace(nbytes: int, key: tuple[int, int], capture: int) -> torch.Tensor:
+    """The buffer of one capture on one stream: memory of the graph's pool, which later launches of the same capture
+    share and which nothing else has while the graph lives."""
+    with _ws_lock:
+        of, buf = _capture_ws.get(key, (0, None))
+        if of != capture or buf.numel() < nbytes:
+            buf = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", key[0]))
+            buf[:_ZEROED].zero_()
+            _capture_ws[key] = capture, buf
+        return buf
+
+
+def report_captured(op: str, index: int, ws: torch.Tensor) -> None:
+    """After a launch with ``workspace``: in a capture, what it records goes to the captures' error word."""
+    if torch.cuda.is_current_stream_capturing():
+        at = (c_void_p * 1)(ws.data_ptr())
+        launch(op, lib().kairo_collect_errors, index, at, 1, error_word(index).data_ptr())
 
 
 class ErrorWord:
@@ -457,12 +491,6 @@ def _error_word_of(index: int, raw: int | None) -> ErrorWord:
             word = ErrorWord(torch.device("cuda", index), words.value + 256 * min(slot, count.value - 1))
             _error_words[index, raw] = word
         return word
-
-
-def collect_errors(op: str, index: int, word: ErrorWord, *workspaces: torch.Tensor) -> None:
-    """What launches on the current stream record in ``workspaces``, which nobody else will read, goes to ``word``."""
-    at = (c_void_p * len(workspaces))(*(w.data_ptr() for w in workspaces))
-    launch(op, lib().kairo_collect_errors, index, at, len(workspaces), word.data_ptr())
 
 
 def read_workspace_error(ws: torch.Tensor, clear: bool = True) -> int:

@@ -498,6 +498,16 @@ kairo_status kairo_collect_errors(const void* const* workspaces, int32_t count, 
   return e == cudaSuccess ? KAIRO_STATUS_SUCCESS : cuda_fail(e, "launch of k_collect_errors");
 }
 
+kairo_status kairo_capture_id(void* stream, uint64_t* id) {
+  if (!id) return fail(KAIRO_STATUS_INVALID_VALUE, "null argument");
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long at = 0;
+  const cudaError_t e = cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &at);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaStreamGetCaptureInfo");
+  *id = status == cudaStreamCaptureStatusActive ? at : 0;
+  return KAIRO_STATUS_SUCCESS;
+}
+
 kairo_status kairo_error_words(void** words, int32_t* count) {
   if (!words || !count) return fail(KAIRO_STATUS_INVALID_VALUE, "null argument");
   // the first reference to the module's memory may load it: never part of another stream's capture

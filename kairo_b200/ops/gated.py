@@ -188,7 +188,6 @@ class _Structure:
 
 
 _CAPTURED: list[_Structure] = []
-_ZEROED = 256 + 2 * 16384 * 4  # header and arrival counters of an SpMM workspace, zero before its first launch
 _AUTO = KernelConfig().to_c()
 _BANDS_128 = KernelConfig(schedule="bands", band_rows=1, n_tile=128).to_c()
 _BANDS_256 = KernelConfig(schedule="bands", band_rows=1, n_tile=256).to_c()
@@ -373,20 +372,13 @@ def sparse_gated_linear_backward(dH: Tensor, X: Tensor, weights: GatedWeights, *
             size = nbytes.value
             if len(st.spmm_bytes) < 4096:
                 st.spmm_bytes[n, x.dtype] = size
-        captured = torch.cuda.is_current_stream_capturing()
-        if captured:
-            # a graph's own: two captured graphs may replay at the same time
-            ws = x.new_empty(size, dtype=torch.uint8)
-            ws[:_ZEROED].zero_()
-        else:
-            ws = _lib.workspace(size, x.device)
+        ws = _lib.workspace(size, x.device)
         if check:
             _lib.take_pending_error(ws, op)
         _lib.launch(op, lib.kairo_bsr_spmm, index, ctypes.byref(desc_t), dp.data_ptr(), dp.shape[1],
                     _lib.LAYOUT_LINEAR, n, dX.data_ptr(), k, _lib.kairo_dtype(x.dtype), ctypes.byref(cfg),
                     ws.data_ptr(), ws.numel())
-        if captured:
-            _lib.collect_errors(op, index, err, ws)
+        _lib.report_captured(op, index, ws)
         if check:
             _lib.raise_on_device_error(ws)
     if need_dw:

@@ -401,6 +401,7 @@ def _launch(a: BlockSparseMatrix, b: Tensor, ldb: int, layout: int, n: int, out:
             _lib.check(lib.kairo_bsr_spmm(ctypes.byref(desc), b.data_ptr(), ldb, layout, n, out.data_ptr(), ldc,
                                           _lib.kairo_dtype(out.dtype), ctypes.byref(cfg), ws.data_ptr(), ws.numel(),
                                           _lib.stream_handle(dev)), name)
+        _lib.report_captured(name, torch.cuda.current_device(), ws)
         if check_device:
             _lib.raise_on_device_error(ws)
 

@@ -125,3 +125,7 @@ def test_layer_loads_without_memory():
     bare = copy.deepcopy(layer).to("meta")
     bare.load_state_dict(state, assign=True)
     assert torch.equal(bare.col_idx, layer.col_idx) and not bare.blocks.is_meta
+
+
+def test_capture_id_refusals():
+    assert _lib.lib().kairo_capture_id(None, None) == _lib.INVALID_VALUE
