@@ -20,11 +20,11 @@
 // M = 256 tokens and N = 2 * BM outputs; the even CTA's shared memory holds
 // the gate block, the odd one's the up block, and each holds its own tokens'
 // panels of X.  With blocks of 64 an entry costs a CTA 32 KB of X and 8 KB of weights (two
-// separate products: 80 KB) and 8 products of 72 cycles.  Bound by the copies out of L2:
-// 8192 tokens, 8192 -> 32768 at 20 % of shared blocks, moves 17 GB into the SMs and takes 1.6 ms, 1100
-// TFLOP/s; 1.25 ms is what the copies alone need (13.7 TB/s, this GPU's rate for
-// gathers of panels), 0.95 the products alone.  Measured and not kept: tiles of
-// 256 tokens (1.95 ms), blocks brought into L2 ahead (1.65), one 32 KB copy of a
+// separate products: 80 KB) and 8 products of 72 cycles.  8192 tokens, 8192 -> 32768 at 20 % of shared
+// blocks, moves 17 GB into the SMs: 1.25 ms at the rate that gathers of panels reach by themselves (13.7 TB/s), 1.07
+// the products.  It takes 1.6 to 1.7 ms from a cool start (1030 to 1100 TFLOP/s) and 1.80 to 1.86 in a row, where the
+// power limit holds the SMs at 1.58 GHz; which role waits for the rest was not measured.  Not kept, all from a cool start
+// against 1.6: tiles of 256 tokens (1.95 ms), blocks brought into L2 ahead (1.65), one 32 KB copy of a
 // panel instead of four (1.61), other groups of token tiles (1.6 to 1.85).
 //
 // k_gated_short (33 to 256 tokens; blocks of 64: to 128, or 17 to 256 where they
@@ -38,7 +38,7 @@
 // rows of a block-row, its warps share out the entries; mma.sync fragments come
 // straight from global memory, 16 bytes a lane (the order of k inside a block is
 // free as long as both operands agree), and the warps' sums meet in shared memory.
-// One token, 8192 -> 32768 at 20 %: 41 us, 5.2 TB/s.  A persistent form that asks
+// One token, 8192 -> 32768 at 20 %: 42 us, 5.1 TB/s.  A persistent form that asks
 // for the next rows' operands before it joins the sums took 43.
 #include <algorithm>
 

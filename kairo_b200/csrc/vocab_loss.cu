@@ -23,8 +23,9 @@
 // need; it keeps 2 * tokens bytes a column of the piece instead of 4 * tokens * vocab.
 //
 // Measured.  8192 tokens, 131072 x 2048, bf16: the forward pass 3.1 ms (1400 TFLOP/s), G 3.4, dX 3.0, dW 3.0
-// (1465) one after the other from a cool start; in a row 13.7 ms, 1280 TFLOP/s of what is done, where the power
-// limit leaves cuBLAS 1355.  One to 64 tokens of 131072 x 4096: 190 to 200 us, 5.4 to 5.6 TB/s.
+// (1465) one after the other from a cool start; in a row 13.7 to 14.5 ms, 1215 to 1285 TFLOP/s of what is done, where
+// the power limit leaves cuBLAS 1355 (SM clock 1.27 GHz).  131072 x 4096 in a row: one token 190 to 207 us (5.2 to 5.7
+// TB/s), 64 tokens 197 to 225 (the power limit again, 1.74 GHz).
 //
 // Rounding.  z, the maxima, sums and lse are fp32.  G is rounded once to the
 // operands' 16 bits, as an operand of both products must be: relative to each
