@@ -260,10 +260,10 @@ class BlockSparseLinear(torch.nn.Module):
     def transposed(self, blocks: Tensor | None = None) -> TransposedBsr:
         """Cached W^T structure (its blocks are refreshed on every backward), made again for ``blocks`` of another
         type or on another device than it was made for, as after a cast of the module."""
-        W = self.weight_matrix(blocks)
-        if self._wt is None or self._wt.matrix.dtype != W.dtype or self._wt.matrix.device != W.device:
-            self._wt = bsr_transpose(W)
-        if W.blocks.is_cuda and torch.cuda.is_current_stream_capturing() and not any(t is self._wt for t in _CAPTURED):
+        b = self.blocks if blocks is None else blocks
+        if self._wt is None or self._wt.matrix.dtype != b.dtype or self._wt.matrix.device != b.device:
+            self._wt = bsr_transpose(self.weight_matrix(b))
+        if b.is_cuda and torch.cuda.is_current_stream_capturing() and not any(t is self._wt for t in _CAPTURED):
             _CAPTURED.append(self._wt)
         return self._wt
 

@@ -394,6 +394,8 @@ def sparse_gated_linear_backward(dH: Tensor, X: Tensor, weights: GatedWeights, *
 
 
 _PATTERN = ("ent_ptr", "entries", "row_ptr", "col_idx", "blk_idx", "stored_col")
+# of a layer's buffers: the buffers, their versions, the kept structure, copies for backward passes by stream
+_NOTHING: tuple = ((), (), {}, {})
 
 
 class _GatedFn(torch.autograd.Function):
@@ -401,16 +403,17 @@ class _GatedFn(torch.autograd.Function):
     def forward(ctx, X: Tensor, blocks: Tensor, module: "SparseGatedLinear") -> Tensor:
         w = module.weights(blocks)
         # all that the backward pass needs is this call's: the module may have changed by then
-        ctx.save_for_backward(X, blocks, *(getattr(w, name) for name in _PATTERN))
+        ctx.save_for_backward(X, blocks)
         ctx.activation = module.activation
-        ctx.weights = {"gate_blocks": w.gate_blocks, "shape": w.shape, "block": w.block, "_structure": w._structure}
+        ctx.weights = {"gate_blocks": w.gate_blocks, "shape": w.shape, "block": w.block, "_structure": w._structure,
+                       **dict(zip(_PATTERN, module._pattern_of_call(X.get_device())))}
         return sparse_gated_linear(X, w, activation=ctx.activation)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dH: Tensor):
-        X, blocks, *pattern = ctx.saved_tensors
-        w = GatedWeights(blocks=blocks.detach(), **dict(zip(_PATTERN, pattern)), **ctx.weights)
+        X, blocks = ctx.saved_tensors
+        w = GatedWeights(blocks=blocks.detach(), **ctx.weights)
         dX, dW = sparse_gated_linear_backward(dH, X, w, activation=ctx.activation, need_dx=ctx.needs_input_grad[0],
                                               need_dw=ctx.needs_input_grad[1])
         return dX, dW, None
@@ -434,11 +437,11 @@ class SparseGatedLinear(torch.nn.Module):
         self.blocks = torch.nn.Parameter(w.blocks.detach())
         for name in _PATTERN:
             self.register_buffer(name, getattr(w, name))
-        self._made: tuple = ((), (), {})
+        self._made: tuple = _NOTHING
 
     def __getstate__(self) -> dict:
         # a copy makes its own structure: this one's descriptors name this layer's memory
-        return {**self.__dict__, "_made": ((), (), {})}
+        return {**self.__dict__, "_made": _NOTHING}
 
     def _load_from_state_dict(self, *args, **kw) -> None:
         super()._load_from_state_dict(*args, **kw)
@@ -455,10 +458,25 @@ class SparseGatedLinear(torch.nn.Module):
         if not any(p.is_inference() for p in parts):
             versions = tuple(p._version for p in parts)
             if self._made[1] != versions or any(p is not q for p, q in zip(self._made[0], parts)):
-                self._made = (parts, versions, structure)
+                self._made = (parts, versions, structure, {})
             structure = self._made[2]
         return GatedWeights(blocks=b, gate_blocks=self.gate_blocks, shape=self.shape, block=self.block,
                             _structure=structure, **dict(zip(_PATTERN, parts)))
+
+    def _pattern_of_call(self, index: int) -> list[Tensor]:
+        """The patterns that ``weights`` has just given, for the backward pass.  Copies, as the buffers may be written
+        before it (by a state dict, or a broadcast before the model's next forward pass): one set for each writing of
+        the buffers and stream, on which autograd runs the backward pass as well.  In a capture the buffers
+        themselves, which the graph's forward pass reads."""
+        parts, _, _, copies = self._made
+        if torch.cuda.is_current_stream_capturing():
+            return [getattr(self, name) for name in _PATTERN]
+        if not parts:  # inference tensors: nothing is kept
+            return [getattr(self, name).clone() for name in _PATTERN]
+        raw = torch._C._cuda_getCurrentRawStream(index)
+        if raw not in copies:
+            copies[raw] = [p.clone() for p in parts]
+        return copies[raw]
 
     def forward(self, X: Tensor) -> Tensor:
         if not torch.is_grad_enabled():

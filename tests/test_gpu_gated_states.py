@@ -264,7 +264,8 @@ def test_activation_of_the_call():
 
 
 def test_patterns_of_the_call():
-    """Patterns that are replaced between the passes change nothing; written in between, they are refused like any saved tensor."""
+    """Patterns that are replaced or written between the passes change nothing, nor do two forward passes with a writing
+    of the same numbers in between."""
     x, dh, gate, up, wg, wu = case(40, 96, 96, 32, torch.bfloat16)
     layer = ops.SparseGatedLinear(gate, up)
     want = step(layer, x, dh)
@@ -276,10 +277,41 @@ def test_patterns_of_the_call():
     h.backward(dh)
     same([h.detach(), xr.grad, layer.blocks.grad], want)
     layer.col_idx = kept
-    h = layer(xr)
-    layer.col_idx.zero_()
-    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+    buffers = dict(layer.named_buffers())
+    before = {k: v.clone() for k, v in buffers.items()}
+    for write in (lambda b: b.zero_(), lambda b: b.copy_(b.clone())):
+        layer.blocks.grad, xr.grad = None, None
+        h = layer(xr)
+        for b in buffers.values():
+            write(b)
+        again = layer(xr)  # of the patterns as they are now
+        del again
         h.backward(dh)
+        same([h.detach(), xr.grad, layer.blocks.grad], want)
+        for k, b in buffers.items():
+            b.copy_(before[k])
+    same(step(layer, x, dh), want)
+
+
+def test_passes_of_a_layer_on_two_streams():
+    """Forward and backward passes through autograd on two streams at once, the first of a layer among them."""
+    x, dh, gate, up, wg, wu = case(300, 320, 320, 64, torch.bfloat16)
+    want = step(ops.SparseGatedLinear(gate, up), x, dh)
+    layer = ops.SparseGatedLinear(gate, up)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for s in streams:
+            with torch.cuda.stream(s):
+                torch.cuda._sleep(20_000_000)
+                xr = x.clone().requires_grad_(True)
+                h = layer(xr)
+                got.append((h, *torch.autograd.grad(h, (xr, layer.blocks), dh)))
+        torch.cuda.synchronize()
+        for g in got:
+            same(g, want)
+        layer.load_state_dict(layer.state_dict())  # the buffers are written again
 
 
 def test_saved_tensors_that_are_copied():
