@@ -29,7 +29,8 @@
 //
 // Rounding.  z, the maxima, sums and lse are fp32.  G is rounded once to the
 // operands' 16 bits, as an operand of both products must be: relative to each
-// entry 2^-9 (bf16) or 2^-12, as the results' own rounding.  The factor that all tokens
+// entry up to 2^-8 (bf16) or 2^-11, as the results' own rounding; over many entries the two together are off by 1.4 times
+// what one is.  Up to 128 tokens G is held as the sum of two such numbers (`halves`).  The factor that all tokens
 // share (the gradient by a mean or a sum) stays out of G and is applied to the
 // fp32 sums: -1 + p of a target is then near -1, which rounds exactly, where f *
 // (-1 + p) would round every target's entry alike.  In fp16 G also carries 2^15,
@@ -46,6 +47,9 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int64_t kPieceBytes = 512LL << 20;
 constexpr float kHalfLift = 32768.f;  // 2^15, see above
+// Probabilities up to here need no second row in G.  They add up to 1 at most, so that their squares' root is an eighth
+// (the root of this number), and each is rounded by itself: an eighth of what one rounding does to an entry of 1.
+constexpr float kLargeProbability = 1.f / 64.f;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -249,8 +253,8 @@ struct FewStatsEpi {
 // A warp's 32 rows x kPairEpiCols results, a row a lane, rounded to T at p (16-byte aligned rows of
 // pitch ld; `rows` and `cols` of them exist).  They pass through shared memory, 64 columns at a
 // time, so that a store instruction writes 128 bytes of each of four rows (a row a lane: 16 bytes of
-// each of 32 rows).
-template <typename T>
+// each of 32 rows).  REST: not the results but what rounding them leaves.
+template <typename T, bool REST = false>
 __device__ __forceinline__ void put_rows(uint8_t* out, const float (&v)[kPairEpiCols], T* p, int64_t ld, int rows,
                                          int cols) {
   const int lane = threadIdx.x & 31, c = lane & 7, r0 = lane >> 3;
@@ -265,7 +269,10 @@ __device__ __forceinline__ void put_rows(uint8_t* out, const float (&v)[kPairEpi
     for (int e = 0; e < 8; ++e) {
       float w[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = v[h + 8 * e + j];
+      for (int j = 0; j < 8; ++j) {
+        w[j] = v[h + 8 * e + j];
+        if (REST) w[j] -= to_f32<T>(from_f32<T>(w[j]));
+      }
       store_f32<T, 8>(reinterpret_cast<T*>(mine + ((e ^ c) * 16)), w);
     }
     __syncwarp();
@@ -344,8 +351,8 @@ __device__ __forceinline__ void sum_rows(uint8_t* out, const float (&v)[kPairEpi
   }
 }
 
-// G of one piece of the vocabulary.
-template <typename T>
+// G of one piece of the vocabulary.  TWO: what its rounding leaves goes to the rows from `tokens` on.
+template <typename T, bool TWO>
 struct GradEpi {
   struct Args {
     T* g;              // [tokens][ldg]
@@ -382,10 +389,17 @@ struct GradEpi {
     const int64_t at = id - (a.v0 + col0);
 #pragma unroll
     for (int j = 0; j < kPairEpiCols; ++j) v[j] = ex2(fmaf(v[j], k, -lse2)) * f;
-    if (__any_sync(0xffffffffu, at >= 0 && at < kPairEpiCols)) {
+    bool large = __any_sync(0xffffffffu, at >= 0 && at < kPairEpiCols);
+    if (large) {
 #pragma unroll
       for (int j = 0; j < kPairEpiCols; ++j)
         if (at == j) v[j] -= f;
+    }
+    if constexpr (TWO) {
+      float top = 0.f;
+#pragma unroll
+      for (int j = 0; j < kPairEpiCols; ++j) top = fmaxf(top, fabsf(v[j]));
+      large |= __any_sync(0xffffffffu, top > kLargeProbability * fabsf(f));
     }
     // a token that does not count has no gradient, whatever its logits are
     const int n = f == 0.f ? 0 : a.vocab - (a.v0 + col0);
@@ -394,7 +408,19 @@ struct GradEpi {
       for (int j = 0; j < kPairEpiCols; ++j)
         if (j >= n) v[j] = 0.f;
     }
-    put_rows<T>(out, v, a.g + static_cast<int64_t>(token0) * a.ldg + col0, a.ldg, a.tokens - token0, kPairEpiCols);
+    T* const p = a.g + static_cast<int64_t>(token0) * a.ldg + col0;
+    put_rows<T>(out, v, p, a.ldg, a.tokens - token0, kPairEpiCols);
+    if constexpr (TWO) {
+      T* const rest = p + a.tokens * a.ldg;
+      if (large) {
+        put_rows<T, true>(out, v, rest, a.ldg, a.tokens - token0, kPairEpiCols);
+      } else {
+        constexpr int kPieces = kPairEpiCols * sizeof(T) / 16;  // of a row
+        const int lane = threadIdx.x & 31, rows = min(32, a.tokens - token0);
+        for (int r = lane / kPieces; r < rows; r += 32 / kPieces)
+          reinterpret_cast<uint4*>(rest + r * a.ldg)[lane % kPieces] = make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
   }
 
   __device__ void done() {}
@@ -631,7 +657,7 @@ __global__ void __launch_bounds__(256) k_rows(const uint16_t* __restrict__ src, 
   for (int64_t r = static_cast<int64_t>(cta) * per + threadIdx.x / lanes; r < rows; r += static_cast<int64_t>(ctas) * per) {
     bool live = true;
     if (ids.p) {
-      const int64_t id = ids[r];
+      const int64_t id = ids[r < src_rows ? r : r % src_rows];
       live = id >= 0 && id < vocab;
     }
     // four vectors at a time, so that their loads are under way together
@@ -774,9 +800,15 @@ struct Results {
   int64_t lddw;
 };
 
+// Rows of G, of X beside it and of dX's sums for each token.  A single token's dW is its entries of G times its X, and a
+// dX is mostly its target's row of the table: G's rounding then stands in the result at full size.  Up to 128 tokens, whose
+// tiles have the rows and the k to spare, a second row holds what the first one's rounding left (bf16, 100000 x 1024: 16
+// tokens 221 -> 230 us, 64 229 -> 248, 128 247 -> 287; the gradients' error 1.4 to 2 times that of one rounding -> 1.0).
+int64_t halves(int64_t tokens) { return tokens <= kPairTileM / 2 ? 2 : 1; }
+
 struct GradWs {
   size_t f, factor, acc_x, acc_w, x, w, g, out, total;
-  int64_t cols;
+  int64_t rows, cols;  // of G
   int splits_x, splits_w;  // parts of the vocabulary piece for dX, of the tokens for dW
   bool direct_x;           // dX leaves from its product
 };
@@ -810,19 +842,20 @@ GradWs grad_ws(const Problem& p, const Results& r) {
     return here;
   };
   const size_t ld = static_cast<size_t>(copy_ld(p.dim));
-  o.cols = piece_cols(p.tokens, p.vocab);
+  o.rows = halves(p.tokens) * p.tokens;
+  o.cols = piece_cols(o.rows, p.vocab);
   o.factor = 128;
   o.f = take(4 * static_cast<size_t>(p.tokens));
-  o.x = take(2 * ld * static_cast<size_t>(p.tokens));
-  o.splits_x = splits_for(p.tokens, p.dim, std::min(o.cols, p.vocab));
-  o.splits_w = splits_for(std::min(o.cols, p.vocab), p.dim, p.tokens);
-  o.direct_x = o.cols >= p.vocab && o.splits_x == 1 && rows_aligned(r.dx, r.lddx, p.tokens);
-  if (r.dx && !o.direct_x) o.acc_x = take(4 * ld * static_cast<size_t>(p.tokens) * o.splits_x);
+  o.x = take(2 * ld * static_cast<size_t>(o.rows));
+  o.splits_x = splits_for(o.rows, p.dim, std::min(o.cols, p.vocab));
+  o.splits_w = splits_for(std::min(o.cols, p.vocab), p.dim, o.rows);
+  o.direct_x = o.rows == p.tokens && o.cols >= p.vocab && o.splits_x == 1 && rows_aligned(r.dx, r.lddx, p.tokens);
+  if (r.dx && !o.direct_x) o.acc_x = take(4 * ld * static_cast<size_t>(o.rows) * o.splits_x);
   if (r.dw && o.splits_w > 1) o.acc_w = take(4 * ld * static_cast<size_t>(std::min(o.cols, p.vocab)) * o.splits_w);
   if (!rows_aligned(p.w, p.ldw, p.vocab)) o.w = take(2 * ld * static_cast<size_t>(p.vocab));
   if (r.dw && o.splits_w == 1 && !rows_aligned(r.dw, r.lddw, p.vocab))
     o.out = take(2 * ld * static_cast<size_t>(std::min(o.cols, p.vocab)));
-  o.g = take(2 * static_cast<size_t>(p.tokens) * static_cast<size_t>(o.cols));
+  o.g = take(2 * static_cast<size_t>(o.rows) * static_cast<size_t>(o.cols));
   o.total = at;
   return o;
 }
@@ -968,15 +1001,15 @@ kairo_status run_grad(Problem p, const float* grad, const float* lse, const Resu
   {
     PrepArgs pa{grad, p.ids, static_cast<int>(p.tokens), static_cast<int>(p.vocab), p.reduction, p.scale,
                 FMT == 0 ? kHalfLift : 1.f, f, factor};
-    st = copy_rows(p.x, p.ldx, p.tokens, p.dim, 1, ws + o.x, p.ids, static_cast<int>(p.vocab), pa, s);
+    st = copy_rows(p.x, p.ldx, p.tokens, p.dim, o.rows / p.tokens, ws + o.x, p.ids, static_cast<int>(p.vocab), pa, s);
     if (st) return st;
   }
   T* g = reinterpret_cast<T*>(ws + o.g);
   CUtensorMap mx, mxt, mg, mgt;
   st = pair_operand_map(&mx, x, p.dt, false, p.tokens, p.dim, ld, "hidden states");
-  if (st == KAIRO_STATUS_SUCCESS) st = pair_operand_map(&mxt, x, p.dt, true, p.dim, p.tokens, ld, "hidden states");
-  if (st == KAIRO_STATUS_SUCCESS) st = pair_operand_map(&mg, g, p.dt, false, p.tokens, o.cols, o.cols, "gradient of the logits");
-  if (st == KAIRO_STATUS_SUCCESS) st = pair_operand_map(&mgt, g, p.dt, true, o.cols, p.tokens, o.cols, "gradient of the logits");
+  if (st == KAIRO_STATUS_SUCCESS) st = pair_operand_map(&mxt, x, p.dt, true, p.dim, o.rows, ld, "hidden states");
+  if (st == KAIRO_STATUS_SUCCESS) st = pair_operand_map(&mg, g, p.dt, false, o.rows, o.cols, o.cols, "gradient of the logits");
+  if (st == KAIRO_STATUS_SUCCESS) st = pair_operand_map(&mgt, g, p.dt, true, o.cols, o.rows, o.cols, "gradient of the logits");
   if (st) return st;
   for (int64_t v0 = 0; v0 < p.vocab; v0 += o.cols) {
     const int64_t n = std::min(o.cols, p.vocab - v0);
@@ -985,19 +1018,24 @@ kairo_status run_grad(Problem p, const float* grad, const float* lse, const Resu
     st = pair_operand_map(&mw, w, p.dt, false, n, p.dim, p.ldw, "vocabulary table");
     if (st == KAIRO_STATUS_SUCCESS) st = pair_operand_map(&mwt, w, p.dt, true, p.dim, n, p.ldw, "vocabulary table");
     if (st) return st;
-    typename GradEpi<T>::Args ga{g, o.cols, lse, f, p.ids, static_cast<int>(p.tokens), static_cast<int>(p.vocab),
-                                 static_cast<int>(v0), p.scale};
-    st = launch_pair_gemm<FMT, false, false, GradEpi<T>>(mx, mw, shape_of(p.tokens, n, p.dim, kSegAgain), err, ga, s);
+    auto form = [&](auto two) {
+      using Epi = GradEpi<T, decltype(two)::value>;
+      const typename Epi::Args ga{g, o.cols, lse, f, p.ids, static_cast<int>(p.tokens), static_cast<int>(p.vocab),
+                                  static_cast<int>(v0), p.scale};
+      return launch_pair_gemm<FMT, false, false, Epi>(mx, mw, shape_of(p.tokens, n, p.dim, kSegAgain), err, ga, s);
+    };
+    st = o.rows > p.tokens ? form(std::true_type{}) : form(std::false_type{});
     if (st) return st;
     if (dx) {
       // a last piece of few columns has fewer parts than the others: those it leaves out keep their sums
       const int splits = static_cast<int>(std::min<int64_t>(o.splits_x, ceil_div64(n, kPairK)));
       typename SumEpi<T>::Args sa{dx, res.lddx, o.direct_x ? nullptr : reinterpret_cast<float*>(ws + o.acc_x), ld,
-                                  factor, static_cast<int>(p.tokens), static_cast<int>(p.dim), v0 == 0};
-      st = launch_pair_gemm<FMT, false, true, SumEpi<T>>(mg, mwt, shape_of(p.tokens, p.dim, n, kSegGrads, splits), err,
+                                  factor, static_cast<int>(o.rows), static_cast<int>(p.dim), v0 == 0};
+      st = launch_pair_gemm<FMT, false, true, SumEpi<T>>(mg, mwt, shape_of(o.rows, p.dim, n, kSegGrads, splits), err,
                                                          sa, s);
       if (st == KAIRO_STATUS_SUCCESS && !o.direct_x && v0 + n == p.vocab)
-        st = join<T>(sa.acc, ld, o.splits_x, p.tokens, p.dim, factor, dx, res.lddx, s);
+        // a token's second row lies as another part's row of it would
+        st = join<T>(sa.acc, ld, o.splits_x * static_cast<int>(o.rows / p.tokens), p.tokens, p.dim, factor, dx, res.lddx, s);
       if (st) return st;
     }
     if (dw) {
@@ -1006,7 +1044,7 @@ kairo_status run_grad(Problem p, const float* grad, const float* lse, const Resu
       typename SumEpi<T>::Args sa{copy ? reinterpret_cast<T*>(ws + o.out) : out, copy ? ld : res.lddw,
                                   o.splits_w > 1 ? reinterpret_cast<float*>(ws + o.acc_w) : nullptr, ld,
                                   factor, static_cast<int>(n), static_cast<int>(p.dim), 1};
-      st = launch_pair_gemm<FMT, true, true, SumEpi<T>>(mgt, mxt, shape_of(n, p.dim, p.tokens, kSegGrads, o.splits_w),
+      st = launch_pair_gemm<FMT, true, true, SumEpi<T>>(mgt, mxt, shape_of(n, p.dim, o.rows, kSegGrads, o.splits_w),
                                                         err, sa, s);
       if (st == KAIRO_STATUS_SUCCESS && sa.acc) st = join<T>(sa.acc, ld, o.splits_w, n, p.dim, factor, out, res.lddw, s);
       if (st) return st;

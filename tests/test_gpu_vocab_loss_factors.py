@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from kairo_b200 import ops
+from tests.test_gpu_vocab_loss import make, tiny, within
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +57,32 @@ def test_factors_keep_their_digits(dtype, powers):
         assert torch.equal(up.double(), w.double() * big)
         _, got = backward(x, up, ids, grad * 2.0**p, 2.0**-p)
         assert torch.equal(got, dw), p
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+@pytest.mark.parametrize("tokens,vocab,dim", [(1, 1891, 256), (2, 1891, 250), (17, 700, 1024), (33, 5000, 130),
+                                              (64, 257, 320), (100, 40000, 72), (128, 3001, 200)])
+def test_few_tokens_are_rounded_once(tokens, vocab, dim, reduction, dtype):
+    """Up to 128 tokens an entry of G over a 64th of its token's factor, and every target's, is held in two numbers: what
+    stands in the results is their own rounding (h), h of the small entries, and the products' errors of 2^-13 as in
+    test_gpu_vocab_loss; with G rounded once every target's h would stand there as well."""
+    x, w, ids, g = make(tokens, vocab, dim, dtype, pad=0.0 if tokens < 5 else 0.1)
+    grad = torch.rand(tokens, generator=g, device="cuda") + 0.5 if reduction == "none" else torch.tensor(0.7, device="cuda")
+    loss, lse = ops.linear_cross_entropy(x, w, ids, reduction=reduction, return_lse=True, check=True)
+    dx, dw = ops.linear_cross_entropy_backward(grad, x, w, ids, lse, reduction=reduction, check=True)
+    live = (ids >= 0) & (ids < vocab)
+    f = (grad.double() * live if reduction == "none" else grad.double() * live / live.sum().clamp(min=1))[:, None]
+    xd, wd, at, h = x.double(), w.double(), ids.clamp(0, vocab - 1)[:, None], torch.finfo(dtype).eps / 2
+    z = xd @ wd.t()
+    lse64 = torch.logsumexp(z, 1)
+    p = torch.exp(z - lse64[:, None])
+    one = torch.zeros_like(p).scatter(1, at, 1.0)
+    gd = (p - one) * f
+    dz = (xd.abs() @ wd.abs().t()).amax(1) * 2.0**-17 + (lse64.abs() + 8) * 2.0**-21
+    two = (one > 0) | (gd.abs() > f.abs() / 64 * 1.001)
+    ga = gd.abs() * (torch.where(two, h * h, h) + 2.0**-13) + p * f.abs() * 2 * dz[:, None] + f.abs() * 2.0**-126
+    if dtype == torch.float16:
+        ga = ga + 2 * f.abs().max() * 2.0**-39  # of either number
+    for name, got, want, tol in (("dX", dx, gd @ wd, ga @ wd.abs()), ("dW", dw, gd.t() @ xd, ga.t() @ xd.abs())):
+        within(name, got, want, tol + (h + 2.0**-20) * want.abs() + tiny(dtype))
