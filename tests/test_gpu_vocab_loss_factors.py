@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from kairo_b200 import ops
-from tests.test_gpu_vocab_loss import make, tiny, within
+from tests.test_gpu_vocab_loss import make, run_case, tiny, within
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +86,9 @@ def test_few_tokens_are_rounded_once(tokens, vocab, dim, reduction, dtype):
         ga = ga + 2 * f.abs().max() * 2.0**-39  # of either number
     for name, got, want, tol in (("dX", dx, gd @ wd, ga @ wd.abs()), ("dW", dw, gd.t() @ xd, ga.t() @ xd.abs())):
         within(name, got, want, tol + (h + 2.0**-20) * want.abs() + tiny(dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_few_tokens_in_pieces(dtype):
+    """A vocabulary of more than one piece for 128 tokens' two rows each; the last piece is narrow."""
+    run_case(128, 1_048_576 + 300, 8, dtype, reduction="sum")
