@@ -402,12 +402,13 @@ class _GatedFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, X: Tensor, blocks: Tensor, module: "SparseGatedLinear") -> Tensor:
         w = module.weights(blocks)
+        H = sparse_gated_linear(X, w, activation=module.activation)
         # all that the backward pass needs is this call's: the module may have changed by then
         ctx.save_for_backward(X, blocks)
         ctx.activation = module.activation
         ctx.weights = {"gate_blocks": w.gate_blocks, "shape": w.shape, "block": w.block, "_structure": w._structure,
                        **dict(zip(_PATTERN, module._pattern_of_call(X.get_device())))}
-        return sparse_gated_linear(X, w, activation=ctx.activation)
+        return H
 
     @staticmethod
     @once_differentiable

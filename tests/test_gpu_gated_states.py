@@ -362,3 +362,10 @@ def test_layer_loads_without_memory():
     bare.load_state_dict(layer.state_dict(), assign=True)
     assert bare.gate_blocks == layer.gate_blocks
     same(step(bare, x, dh), want)
+
+
+def test_module_refuses_host_tensors():
+    x, dh, gate, up, wg, wu = case(8, 64, 64, 32, torch.bfloat16)
+    layer = ops.SparseGatedLinear(gate, up)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        layer(x.cpu())

@@ -125,3 +125,35 @@ def test_feed_forward_block_in_two_graphs():
                 gr.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(out, w) for (_, out), w in zip(made, want))
+
+
+def test_model_step_as_graphed_callables():
+    """Forward and backward pass of a feed-forward block and the loss as two graphs that share a pool."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    mats = [weight(m, k, 64, 0.5, torch.bfloat16, g)[0] for m, k in ((512, 256), (512, 256), (256, 512))]
+
+    class Model(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.ffn = ops.SparseFeedForward(*mats)
+            self.head = ops.LinearCrossEntropy(torch.nn.Parameter(
+                (torch.randn(1000, 256, generator=g, device="cuda") / 16).bfloat16()))
+
+        def forward(self, x, ids):
+            return self.head(x + self.ffn(x), ids)
+
+    model = Model()
+    xs = [torch.randn(300, 256, generator=g, device="cuda").bfloat16() for _ in range(2)]
+    ids = torch.randint(0, 1000, (300,), generator=g, device="cuda")
+
+    def step(f, x):
+        xr = x.clone().requires_grad_(True)
+        loss = f(xr, ids)
+        return [loss.detach().clone(), *(t.clone() for t in torch.autograd.grad(loss, (xr, *model.parameters())))]
+
+    want = [step(model, x) for x in xs]
+    graphed = torch.cuda.make_graphed_callables(model, (xs[0].clone().requires_grad_(True), ids.clone()))
+    for _ in range(3):
+        for x, w in zip(xs, want):
+            assert all(torch.equal(a, b) for a, b in zip(step(graphed, x), w))
+    assert ops.pending_device_error() == 0
